@@ -382,6 +382,69 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
                               long long v_bs, long long v_rs, long long o_bs, long long o_rs,
                               long long do_bs, long long do_rs, double scale, int dtype);
 
+/* ---- layers whose weight depends on the row (no counterpart in the reference) ----
+ * Rows in groups: group g holds rows [offsets[g], offsets[g + 1]).  offsets is DEVICE memory (int32, groups + 1 entries, not
+ * decreasing), so that no call waits for the host; values outside [0, rows] are clamped, an end before its beginning is an
+ * empty group, and rows behind the last group are neither read nor written.  Operands: strides in elements, non-negative;
+ * outputs overlap neither an operand nor each other.  All types; sums are in the accumulate type (float32, float64 for
+ * float64) and rounded once, to nearest even.  No entry takes a block of the pool except where its comment says so. */
+
+/* Routing: each of `tokens` rows of logits (row stride logits_rs) is given its k largest entries, equal ones in the order of
+ * their index; an entry of -inf is never taken (a padding token has nothing else), NaN is above every number.  Slot
+ * token * k + j is the token's j-th: experts[slot] its expert, -1 where none was left; weights[slot] = exp(logit - max) / sum, 0 where
+ * none was left, with the sum over the entries taken (normalize != 0) or over all.  (A row whose largest entry is NaN or +inf has NaN
+ * weights.)  The slots are then sorted by expert, in slot order within an expert: offsets[num_experts + 1], order[place] = slot
+ * (-1 behind the last), position[slot] = place (-1 where none was left).
+ * weights [tokens, k]: float32 (float64 for float64) whatever the logits' type; experts, order, position: int32 [tokens * k].
+ * At most 1024 experts, k of 16 and 2^30 slots. */
+int rp_hip_route_forward(void* weights, int* experts, int* offsets, int* order, int* position, const void* logits, long long logits_rs,
+                         int tokens, int num_experts, int k, int normalize, int dtype);
+/* grad_logits [tokens, num_experts], dense, overwritten: the gradient of the weights with respect to the logits times grad_weights (entries of
+ * slots without an expert are not used).  logits may be NULL with normalize != 0. */
+int rp_hip_route_backward(void* grad_logits, const void* grad_weights, const void* weights, const int* experts, const void* logits, long long logits_rs,
+                          int tokens, int num_experts, int k, int normalize, int dtype);
+/* The sort alone: ids int32 [count] in [0, groups), others (-1) belong to no group.  At most 1024 groups, 2^30 entries. */
+int rp_hip_group_rows(int* offsets, int* order, int* position, const int* ids, int count, int groups);
+
+/* Exchange of rows between tokens and groups, by the position [tokens, k] that routing leaves (each place at most once; entries outside
+ * [0, tokens * k) are slots without a row).  d elements a row.
+ * dispatch: out[position[t, j]] = x[t]; rows of `out` that no slot names stay as they are.
+ * combine:  y[t] = sum over j of weights[t, j] z[position[t, j]] in the order of j; weights [tokens, k] as rp_hip_route_forward leaves them, or
+ *           NULL for ones, which is the gradient of dispatch.  A token without rows gets zeros.
+ * combine_backward: grad_z[position[t, j]] = weights[t, j] grad_y[t] (other rows stay as they are), grad_weights[t, j] = grad_y[t] . z[position[t, j]]
+ *           (0 for slots without a row). */
+int rp_hip_dispatch_rows(void* out, const void* x, const int* position, int tokens, int k, int d, long long x_rs, long long out_rs, int dtype);
+int rp_hip_combine_forward(void* y, const void* z, const void* weights, const int* position, int tokens, int k, int d, long long y_rs, long long z_rs, int dtype);
+int rp_hip_combine_backward(void* grad_z, void* grad_weights, const void* grad_y, const void* z, const void* weights, const int* position, int tokens, int k, int d,
+                            long long grad_y_rs, long long z_rs, long long grad_z_rs, int dtype);
+
+/* Grouped linear layer, one weight for each group: y[i] = x[i] . w_g + bias_g for the rows i of group g.  x [rows, k], w [groups, k, n] with strides
+ * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for. */
+int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,
+                                  long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long y_rs, int dtype);
+/* Its gradients: dx[i] = dy[i] . w_g^T, dw_g = sum of x[i]^T dy[i], db_g = sum of dy[i] over the group's rows (zeros for an empty group).  dx [rows, k] with
+ * unit column stride, dw [groups, k, n] and db [groups, n] dense; any of the three may be NULL; accumulate_* adds to what is there. */
+int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w, const int* offsets, int groups, int rows, int k, int n,
+                                   long long dy_rs, long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long dx_rs,
+                                   int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);
+
+/* Low-rank adapters of many requests beside one shared projection.  Segment s holds rows [offsets[s], offsets[s + 1]) and uses adapter ids[s]
+ * (device int32 [segments]; outside [0, adapters): none; several segments may use the same one):
+ *   h[i] = scales[a] x[i] . a_a,   y[i] = x[i] . w + bias + h[i] . b_a       (rows without an adapter: y[i] = x[i] . w + bias)
+ * x [rows, k], w [k, n], bias [n] or NULL, a [adapters, k, rank] and b [adapters, rank, n] dense, scales float32 [adapters] or NULL for ones, y [rows, n] with
+ * unit column stride.  h [rows, rank], dense, in the accumulate type: written for rows with an adapter, kept by the caller for the backward pass.
+ * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection. */
+int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
+                                  int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);
+/* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):
+ *   u[i] = scales[a] dy[i] . b_a^T,   dx[i] = dy[i] . w^T + u[i] . a_a^T,   da_a = sum of x[i]^T u[i],   db_a = sum of h[i]^T dy[i]
+ * over the rows of all segments that use adapter a (zeros for one that none uses).  u [rows, rank]: room for it, in the accumulate type.  Any of dx [rows, k] (unit column
+ * stride), da and db (dense) may be NULL; accumulate_* adds to what is there. */
+int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
+                                   const float* scales, const int* ids, const int* offsets, int segments, int adapters, int rows, int k, int n, int rank,
+                                   long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,
+                                   int accumulate_dx, int accumulate_da, int accumulate_db, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -98,6 +98,16 @@ SIGNATURES = {
     "rp_hip_scatter_strided": (_i, [_vp, _vp, _i, _ip, ctypes.POINTER(ctypes.c_longlong), _sz, _i]),
     "rp_hip_attention_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i] + [_ll] * 8 + [_d, _i]),
     "rp_hip_attention_backward": (_i, [_vp] * 9 + [_i] * 4 + [_ll] * 10 + [_d, _i]),
+    "rp_hip_route_forward": (_i, [_vp] * 6 + [_ll] + [_i] * 5),
+    "rp_hip_route_backward": (_i, [_vp] * 5 + [_ll] + [_i] * 5),
+    "rp_hip_group_rows": (_i, [_vp] * 4 + [_i] * 2),
+    "rp_hip_dispatch_rows": (_i, [_vp] * 3 + [_i] * 3 + [_ll] * 2 + [_i]),
+    "rp_hip_combine_forward": (_i, [_vp] * 4 + [_i] * 3 + [_ll] * 2 + [_i]),
+    "rp_hip_combine_backward": (_i, [_vp] * 6 + [_i] * 3 + [_ll] * 3 + [_i]),
+    "rp_hip_grouped_linear_forward": (_i, [_vp] * 5 + [_i] * 4 + [_ll] * 6 + [_i]),
+    "rp_hip_grouped_linear_backward": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 7 + [_i] * 4),
+    "rp_hip_adapter_linear_forward": (_i, [_vp] * 10 + [_i] * 6 + [_ll] * 5 + [_i]),
+    "rp_hip_adapter_linear_backward": (_i, [_vp] * 13 + [_i] * 6 + [_ll] * 6 + [_i] * 4),
 }
 
 _lib = None

@@ -1,0 +1,31 @@
+// Grouped products: rows in groups, a weight for each group (or one that several groups share).
+#pragma once
+#include "rp_gemm.h"
+#include "rp_rows.h"
+
+namespace rp {
+
+// By rows:     C[i, :] (+)= scale_w * A[i, :] . B_w + bias_w      for every row i of a group whose weight is w
+// By weights:  C_w (+)= sum over the rows i of w's groups of A[i, :]^T . B[i, :]
+// Strides in elements; B (by rows) and C (by weights) have a stride b_ws / c_ws from weight to weight.
+struct GroupedArgs {
+    void* C;
+    const void* A;
+    const void* B;
+    const void* bias;              // [weights, n] dense, or null
+    const float* scales;           // [weights] float32, or null
+    RowGroups gr;
+    int k, n;                      // by rows: A [rows, k], C [rows, n];  by weights: C_w [k, n], A [rows, k], B [rows, n]
+    long long a_rs, a_cs, b_ws, b_rs, b_cs, c_ws, c_rs;        // C has unit column stride
+    int accumulate;
+};
+
+// Any strides and sizes, all types (rp_grouped_generic.hip).  LOW: which operand is in the accumulate type (float32, float64 for float64)
+// whatever the tensors' type is: the low-rank activations of an adapter.
+enum GroupedLow { LOW_NONE = 0, LOW_A = 1, LOW_B = 2, LOW_C = 3 };
+int launch_grouped_rows_generic(const GroupedArgs& g, GroupedLow low, int dtype);
+int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dtype);
+// out[w, :] (+)= sum over the rows of w's groups of x[i, :]
+int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype);
+
+}  // namespace rp

@@ -1,0 +1,85 @@
+// Entry points and dispatch of the grouped products (experts) and of the adapters beside a shared projection.
+//
+// Experts: y[i] = x[i] . W_g + b_g for the rows i of group g;  dx[i] = dy[i] . W_g^T,  dW_g = sum x[i]^T dy[i],  db_g = sum dy[i].
+// Adapters, a the adapter of row i's segment:  h[i] = s_a x[i] . A_a,  y[i] = x[i] . W + b + h[i] . B_a;
+//   u[i] = s_a dy[i] . B_a^T,  dx[i] = dy[i] . W^T + u[i] . A_a^T,  dA_a = sum x[i]^T u[i],  dB_a = sum h[i]^T dy[i].
+// h and u are in the accumulate type (float32, float64 for float64): they are sums that are multiplied on.
+#include "rp_grouped.h"
+
+namespace rp {
+
+static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) { return launch_grouped_rows_generic(g, low, dtype); }
+static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) { return launch_grouped_weights_generic(g, low, dtype); }
+
+static bool grouped_args_ok(const char* who, bool pointers, int groups, int rows, int k, int n, std::initializer_list<long long> strides, int dtype) {
+    if (!pointers || groups <= 0 || rows <= 0 || k <= 0 || n <= 0) { set_error("%s: null operand or non-positive extent (groups=%d rows=%d k=%d n=%d)", who, groups, rows, k, n); return false; }
+    if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
+    for (long long s : strides)
+        if (s < 0) { set_error("%s: negative stride", who); return false; }
+    return true;
+}
+
+static bool output_rows_ok(const char* who, const char* what, int rows, int width, long long rs) {
+    if (rows == 1 || rs >= width) return true;
+    set_error("%s: rows of %s are %lld elements apart and hold %d", who, what, rs, width);
+    return false;
+}
+
+}  // namespace rp
+
+using namespace rp;
+
+extern "C" {
+
+int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,
+                                  long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long y_rs, int dtype) {
+    const char* who = "rp_hip_grouped_linear_forward";
+    if (!grouped_args_ok(who, y && x && w && offsets, groups, rows, k, n, {x_rs, x_cs, w_gs, w_rs, w_cs, y_rs}, dtype) || !output_rows_ok(who, "y", rows, n, y_rs)) return -1;
+    const RowGroups gr{offsets, nullptr, groups, rows, groups};
+    return grouped_rows(GroupedArgs{y, x, w, bias, nullptr, gr, k, n, x_rs, x_cs, w_gs, w_rs, w_cs, 0, y_rs, 0}, LOW_NONE, dtype);
+}
+
+int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w, const int* offsets, int groups, int rows, int k, int n,
+                                   long long dy_rs, long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long dx_rs,
+                                   int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype) {
+    const char* who = "rp_hip_grouped_linear_backward";
+    if (!grouped_args_ok(who, dy && offsets && (!dx || w) && (!dw || x), groups, rows, k, n, {dy_rs, x_rs, x_cs, w_gs, w_rs, w_cs, dx_rs}, dtype)) return -1;
+    if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
+    const RowGroups gr{offsets, nullptr, groups, rows, groups};
+    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx}, LOW_NONE, dtype) != 0) return -1;
+    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw}, LOW_NONE, dtype) != 0) return -1;
+    if (db && launch_grouped_sums(db, dy, gr, n, dy_rs, accumulate_db, dtype) != 0) return -1;
+    return 0;
+}
+
+int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
+                                  int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype) {
+    const char* who = "rp_hip_adapter_linear_forward";
+    if (!grouped_args_ok(who, y && h && x && w && a && b && ids && offsets && adapters > 0 && rank > 0, segments, rows, k, n, {x_rs, x_cs, w_rs, w_cs, y_rs}, dtype) ||
+        !output_rows_ok(who, "y", rows, n, y_rs)) return -1;
+    const RowGroups gr{offsets, ids, segments, rows, adapters};
+    if (grouped_rows(GroupedArgs{h, x, a, nullptr, scales, gr, k, rank, x_rs, x_cs, (long long)k * rank, rank, 1, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
+    if (rp_hip_gemm_strided_batched(y, x, w, bias, 1, rows, k, n, 0, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 1, 0, dtype) != 0) return -1;
+    return grouped_rows(GroupedArgs{y, h, b, nullptr, nullptr, gr, rank, n, rank, 1, (long long)rank * n, n, 1, 0, y_rs, 1}, LOW_A, dtype);
+}
+
+int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
+                                   const float* scales, const int* ids, const int* offsets, int segments, int adapters, int rows, int k, int n, int rank,
+                                   long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,
+                                   int accumulate_dx, int accumulate_da, int accumulate_db, int dtype) {
+    const char* who = "rp_hip_adapter_linear_backward";
+    if (!grouped_args_ok(who, dy && ids && offsets && adapters > 0 && rank > 0 && (!(dx || da) || (u && b)) && (!dx || (w && a)) && (!da || x) && (!db || h), segments, rows, k, n,
+                         {dy_rs, x_rs, x_cs, w_rs, w_cs, dx_rs}, dtype)) return -1;
+    if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
+    const RowGroups gr{offsets, ids, segments, rows, adapters};
+    if ((dx || da) && grouped_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
+    if (dx) {
+        if (rp_hip_gemm_strided_batched(dx, dy, w, nullptr, 1, rows, n, k, 0, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, 1, accumulate_dx, dtype) != 0) return -1;
+        if (grouped_rows(GroupedArgs{dx, u, a, nullptr, nullptr, gr, rank, k, rank, 1, (long long)k * rank, 1, rank, 0, dx_rs, 1}, LOW_A, dtype) != 0) return -1;
+    }
+    if (da && grouped_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da}, LOW_B, dtype) != 0) return -1;
+    if (db && grouped_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db}, LOW_A, dtype) != 0) return -1;
+    return 0;
+}
+
+}  // extern "C"

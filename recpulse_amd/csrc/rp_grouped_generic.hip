@@ -1,0 +1,168 @@
+// Grouped products for any strides, sizes and types: 64 x 64 tiles, 16 of k at a time through LDS, scalar multiply-adds, 4 x 4 outputs a
+// thread.  What no other kernel takes comes here: widths below a vector, operands without a unit stride, float64 and float32
+// next to low-rank activations in the accumulate type.  Sums in the accumulate type, one rounding at the end.
+#include "rp_grouped.h"
+
+#include <type_traits>
+
+namespace rp {
+
+constexpr int GG_T = 64, GG_K = 16;
+
+// One 64 x 64 tile: acc += A[0 .. m, 0 .. k] . B[0 .. k, 0 .. n], both masked past their extents.  Pointers at the tile's origin.
+template <typename TA, typename TB, typename A>
+__device__ __forceinline__ void generic_tile(A acc[4][4], A (*as)[GG_T + 4], A (*bs)[GG_T + 4], const TA* a, const TB* b, int m, int n, int k,
+                                             long long a_rs, long long a_cs, long long b_rs, long long b_cs) {
+    const int t = threadIdx.x, tr = (t >> 4) * 4, tc = (t & 15) * 4;
+    for (int k0 = 0; k0 < k; k0 += GG_K) {
+        A av[4], bv[4];
+        // neighbouring threads along the axis with the smaller stride
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int id = t + 256 * i;
+            const int ar = a_cs <= a_rs ? id / GG_K : id % GG_T, ak = a_cs <= a_rs ? id % GG_K : id / GG_T;
+            const int bc = b_cs <= b_rs ? id % GG_T : id / GG_K, bk = b_cs <= b_rs ? id / GG_T : id % GG_K;
+            av[i] = ar < m && k0 + ak < k ? (A)widen(a[ar * a_rs + (k0 + ak) * a_cs]) : (A)0;
+            bv[i] = bc < n && k0 + bk < k ? (A)widen(b[(k0 + bk) * b_rs + bc * b_cs]) : (A)0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int id = t + 256 * i;
+            const int ar = a_cs <= a_rs ? id / GG_K : id % GG_T, ak = a_cs <= a_rs ? id % GG_K : id / GG_T;
+            const int bc = b_cs <= b_rs ? id % GG_T : id / GG_K, bk = b_cs <= b_rs ? id / GG_T : id % GG_K;
+            as[ak][ar] = av[i];
+            bs[bk][bc] = bv[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < GG_K; kk++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] += as[kk][tr + i] * bs[kk][tc + j];
+    }
+}
+
+template <typename TA, typename TB, typename TC>
+__global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g, int tiles_n) {
+    using A = typename traits<TA>::acc;
+    __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
+    const RowTile rt = find_row_tile(g.gr, GG_T, (int)(blockIdx.x / tiles_n));
+    if (rt.group < 0) return;
+    const int n0 = (int)(blockIdx.x % tiles_n) * GG_T, m = rt.end - rt.begin, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
+    const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
+    A acc[4][4] = {};
+    generic_tile<TA, TB, A>(acc, as, bs, (const TA*)g.A + rt.begin * g.a_rs, (const TB*)g.B + rt.weight * g.b_ws + n0 * g.b_cs, m, n, g.k, g.a_rs, g.a_cs, g.b_rs, g.b_cs);
+    const A scale = g.scales ? (A)g.scales[rt.weight] : (A)1;
+    const TC* bias = (const TC*)g.bias;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (tr + i >= m || tc + j >= n) continue;
+            TC* p = (TC*)g.C + (rt.begin + tr + i) * g.c_rs + n0 + tc + j;
+            A v = scale * acc[i][j];
+            if (bias) v += widen(bias[(long long)rt.weight * g.n + n0 + tc + j]);
+            if (g.accumulate) v += widen(*p);
+            *p = round_to<TC>(v);
+        }
+}
+
+// A tile of C_w walks the rows of all groups whose weight is w, in the order of the groups
+template <typename TA, typename TB, typename TC>
+__global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArgs g, int tiles_k, int tiles_n) {
+    using A = typename traits<TA>::acc;
+    __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
+    const int tn = (int)(blockIdx.x % tiles_n), tk = (int)(blockIdx.x / tiles_n % tiles_k), w = (int)(blockIdx.x / tiles_n / tiles_k);
+    const int m0 = tk * GG_T, n0 = tn * GG_T, m = g.k - m0 < GG_T ? g.k - m0 : GG_T, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
+    const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
+    A acc[4][4] = {};
+    for (int s = g.gr.ids ? 0 : w; s < (g.gr.ids ? g.gr.groups : w + 1); s++) {
+        if (g.gr.weight(s) != w) continue;
+        const int b = g.gr.begin(s), e = g.gr.end(s);
+        generic_tile<TA, TB, A>(acc, as, bs, (const TA*)g.A + b * g.a_rs + m0 * g.a_cs, (const TB*)g.B + b * g.b_rs + n0 * g.b_cs, m, n, e - b, g.a_cs, g.a_rs, g.b_rs, g.b_cs);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (tr + i >= m || tc + j >= n) continue;
+            TC* p = (TC*)g.C + w * g.c_ws + (m0 + tr + i) * g.c_rs + n0 + tc + j;
+            A v = acc[i][j];
+            if (g.accumulate) v += widen(*p);
+            *p = round_to<TC>(v);
+        }
+}
+
+// Column sums: 64 columns a workgroup, four rows at a time, the four partial sums added in order
+template <typename T>
+__global__ void __launch_bounds__(256) grouped_sums_kernel(T* out, const T* x, RowGroups gr, int cols, long long x_rs, int accumulate, int strips) {
+    using A = typename traits<T>::acc;
+    __shared__ A parts[4][64];
+    const int strip = (int)(blockIdx.x % strips), w = (int)(blockIdx.x / strips);
+    const int c = strip * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    A sum = 0;
+    for (int s = gr.ids ? 0 : w; s < (gr.ids ? gr.groups : w + 1); s++) {
+        if (gr.weight(s) != w || c >= cols) continue;
+        const int e = gr.end(s);
+#pragma unroll 8
+        for (int i = gr.begin(s) + q; i < e; i += 4) sum += widen(x[i * x_rs + c]);
+    }
+    parts[q][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (q || c >= cols) return;
+    A v = ((parts[0][threadIdx.x] + parts[1][threadIdx.x]) + parts[2][threadIdx.x]) + parts[3][threadIdx.x];
+    T* p = out + (long long)w * cols + c;
+    if (accumulate) v += widen(*p);
+    *p = round_to<T>(v);
+}
+
+static bool grid_ok(long long blocks, const char* what) {
+    if (blocks <= 0x7fffffffll) return true;
+    set_error("%s: %lld tiles are more than a launch takes", what, blocks);
+    return false;
+}
+
+template <typename T, typename F>
+static int with_low(GroupedLow low, F f) {
+    using A = typename traits<T>::acc;
+    switch (low) {
+        case LOW_NONE: return f(T{}, T{}, T{});
+        case LOW_A: return f(A{}, T{}, T{});
+        case LOW_B: return f(T{}, A{}, T{});
+        default: return f(T{}, T{}, A{});
+    }
+}
+
+int launch_grouped_rows_generic(const GroupedArgs& g, GroupedLow low, int dtype) {
+    const int tiles_n = (g.n + GG_T - 1) / GG_T;
+    const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, GG_T) * tiles_n;
+    if (!grid_ok(blocks, "grouped product")) return -1;
+    RP_DISPATCH_DTYPE(dtype, return with_low<T>(low, [&](auto a, auto b, auto c) {
+        hipLaunchKernelGGL((grouped_rows_generic_kernel<decltype(a), decltype(b), decltype(c)>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
+        return check_launch("grouped_rows_generic_kernel") ? 0 : -1;
+    }));
+    return 0;
+}
+
+int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dtype) {
+    const int tiles_k = (g.k + GG_T - 1) / GG_T, tiles_n = (g.n + GG_T - 1) / GG_T;
+    const long long blocks = (long long)g.gr.weights * tiles_k * tiles_n;
+    if (!grid_ok(blocks, "grouped weight gradient")) return -1;
+    RP_DISPATCH_DTYPE(dtype, return with_low<T>(low, [&](auto a, auto b, auto c) {
+        hipLaunchKernelGGL((grouped_weights_generic_kernel<decltype(a), decltype(b), decltype(c)>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_k, tiles_n);
+        return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
+    }));
+    return 0;
+}
+
+int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype) {
+    const int strips = (cols + 63) / 64;
+    const long long blocks = (long long)gr.weights * strips;
+    if (!grid_ok(blocks, "grouped bias gradient")) return -1;
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, current_stream(), (T*)out, (const T*)x, gr, cols, x_rs, accumulate, strips));
+    return check_launch("grouped_sums_kernel") ? 0 : -1;
+}
+
+}  // namespace rp

@@ -1,0 +1,70 @@
+// Shared by the layers whose weight depends on the row (routing, exchange of rows, grouped products, adapters).
+#pragma once
+#include "rp_common.h"
+
+namespace rp {
+
+// One rounding to the tensor type, nearest even (the hardware's conversions): these layers have no counterpart in the
+// reference whose round-half-up they would have to follow, and nearest even keeps every NaN a NaN.
+template <typename T> __device__ __forceinline__ T round_to(typename traits<T>::acc v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ double round_to<double>(double v) { return v; }
+template <> __device__ __forceinline__ bf16_t round_to<bf16_t>(float v) { bf16_t r; r.bits = __builtin_bit_cast(uint16_t, (__bf16)v); return r; }
+template <> __device__ __forceinline__ f16_t round_to<f16_t>(float v) { f16_t r; r.bits = __builtin_bit_cast(uint16_t, (_Float16)v); return r; }
+
+// Rows in groups: group g holds rows [offsets[g], offsets[g + 1]) of `rows`, and its weight is number ids[g] of `weights` (ids null:
+// g itself).  The offsets are device memory that no host code has seen: whatever they hold, begin and end are clamped to
+// the rows there are, and a weight number out of range stands for a group without a weight.
+struct RowGroups {
+    const int* offsets;
+    const int* ids;
+    int groups, rows, weights;
+    __device__ __forceinline__ int begin(int g) const { const int o = offsets[g]; return o < 0 ? 0 : o > rows ? rows : o; }
+    __device__ __forceinline__ int end(int g) const { const int b = begin(g), e = offsets[g + 1] > rows ? rows : offsets[g + 1]; return e > b ? e : b; }
+    __device__ __forceinline__ int weight(int g) const { const int w = ids ? ids[g] : g; return w >= 0 && w < weights ? w : -1; }
+};
+
+// Tiles of `tile` rows that `rows` rows in `groups` groups can come to, whatever the offsets hold as long as the groups do not overlap
+static inline long long max_row_tiles(long long rows, long long groups, int tile) {
+    const long long parted = rows / tile + (groups < rows ? groups : rows);
+    return parted < rows ? parted : rows;
+}
+
+// Tile number `id` of the groups' row tiles, found by the whole wave together: 64 groups at a time, a lane each, their tile counts added up
+// across the lanes.  All results are wave-uniform.
+struct RowTile { int group, weight, begin, end; };       // rows [begin, end) of `group`; group < 0: there is no such tile
+__device__ __forceinline__ int wave_prefix_sum(int v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int below = __shfl_up(v, d);
+        v += lane >= d ? below : 0;
+    }
+    return v;
+}
+__device__ __forceinline__ RowTile find_row_tile(const RowGroups& gr, int tile, int id) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int g0 = 0; g0 < gr.groups; g0 += 64) {
+        const int g = g0 + lane;
+        int b = 0, e = 0, w = -1;
+        if (g < gr.groups) { b = gr.begin(g); e = gr.end(g); w = gr.weight(g); }
+        const int tiles = w < 0 ? 0 : (e - b + tile - 1) / tile;
+        const int upto = before + wave_prefix_sum(tiles, lane);
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > id);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const int first = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l);
+            RowTile t;
+            t.group = g0 + l;
+            t.weight = __builtin_amdgcn_readlane(w, l);
+            t.begin = __builtin_amdgcn_readlane(b, l) + (id - first) * tile;
+            const int end = __builtin_amdgcn_readlane(e, l);
+            t.end = t.begin + tile < end ? t.begin + tile : end;
+            return t;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return RowTile{-1, -1, 0, 0};
+}
+
+}  // namespace rp
