@@ -387,7 +387,8 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
  * decreasing), so that no call waits for the host; values outside [0, rows] are clamped, an end before its beginning is an
  * empty group, and rows behind the last group are neither read nor written.  Operands: strides in elements, non-negative;
  * outputs overlap neither an operand nor each other.  All types; sums are in the accumulate type (float32, float64 for
- * float64) and rounded once, to nearest even.  No entry takes a block of the pool except where its comment says so. */
+ * float64) and rounded once, to nearest even; with accumulate_* the rounded product is added to what is there and the sum
+ * rounded.  No entry takes a block of the pool except where its comment says so. */
 
 /* Routing: each of `tokens` rows of logits (row stride logits_rs) is given its k largest entries, equal ones in the order of
  * their index; an entry of -inf is never taken (a padding token has nothing else), NaN is above every number.  Slot

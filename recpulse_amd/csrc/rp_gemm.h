@@ -131,7 +131,7 @@ __device__ __forceinline__ TileCoord schedule_tile(int bid, int tiles_m, int til
     return tc;
 }
 
-static inline int scheduled_grid(int tiles_m, int tiles_n) {
+__host__ __device__ static inline int scheduled_grid(int tiles_m, int tiles_n) {
     constexpr int XCDS = 8, GM = 4, GN = 8, PER = GM * GN;
     if (!schedule_by_xcd(tiles_m, tiles_n)) return tiles_m * tiles_n;
     int sup = ((tiles_m + GM - 1) / GM) * ((tiles_n + GN - 1) / GN);

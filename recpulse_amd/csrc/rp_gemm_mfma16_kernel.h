@@ -2,6 +2,7 @@
 // per-tile translation units.
 #pragma once
 #include "rp_gemm.h"
+#include "rp_rows.h"
 
 #include <type_traits>
 
@@ -172,9 +173,14 @@ __device__ __forceinline__ u32x4_t m16_pull_shift(u32x4_t v, int pull) {
 }
 typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));       // a 16-byte vector at any element
 
+// Where a workgroup's tiles come from and what else they may do.  M16Plain: the schedule of one matrix of the batch, the reference's roundings.
+// Another source (the grouped products') has `tile`, which points `args` at the matrix that slot `tile_id` belongs to and answers with the tile's
+// coordinates in it, and ONCE: the sum and the bias of its column are rounded together, to nearest even.
+struct M16Plain { static constexpr bool ONCE = false; };
+
 // What one workgroup does: slots first_slot, first_slot + stride, ... of the schedule of matrix z
-template <typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE, bool SPLITK, int PF>
-__device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m, int tiles_n, float* partials, int k_per_split, int sched_total, int first_slot, int z, int stride) {
+template <typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE, bool SPLITK, int PF, typename SRC = M16Plain>
+__device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, GemmArgs, const GemmArgs>& g, int tiles_m, int tiles_n, float* partials, int k_per_split, int sched_total, int first_slot, int z, int stride, SRC* source = nullptr) {
     constexpr int WGN = 4 / WGM;
     constexpr int WM = BM / WGM, WN = BN / WGN;       // wave patch
     constexpr int MT = SPLITK ? 32 : m16_mfma_tile(BM, BN);      // MFMA tile edge; k-steps of 16 (MT 32) or 32 (MT 16)
@@ -199,7 +205,9 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
     // run; a workgroup per tile would hold the CU idle until its last store was acknowledged.  A stride that is a
     // multiple of 8 keeps a workgroup's tiles on the XCD the schedule assigned them to.
     for (int tile_id = first_slot; tile_id < sched_total; tile_id += stride) {
-    TileCoord tc = schedule_tile(tile_id, tiles_m, tiles_n);
+    TileCoord tc;
+    if constexpr (SRC::ONCE) tc = source->tile(tile_id, g);
+    else tc = schedule_tile(tile_id, tiles_m, tiles_n);
     if (!tc.valid) continue;
     const int m0 = tc.tm * BM, n0 = tc.tn * BN;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -516,6 +524,10 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
         constexpr int LPR = WN / 8, RPS = 64 / LPR;      // lanes per row, rows per step
         uint16_t* region = smem + wave * (WM * EP);
         const bool c_vec = (g.c_cs == 1) && (g.c_rs % 8 == 0) && (((uintptr_t)C & 15) == 0);
+        auto joined = [](T was, T y) {
+            if constexpr (SRC::ONCE) return round_to<T>(widen(was) + widen(y));
+            else return narrow<T>(widen(was) + widen(y));
+        };
         __syncthreads();                                 // every wave is done with the main loop's LDS
         // (compile-time tile indices: a loop that the compiler declines to unroll would index the accumulators at run
         // time and move all of them to scratch memory for the whole kernel)
@@ -525,7 +537,7 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
             const bool by_row = g.bias_by_row != 0;
             const float bcol = (has_bias && !by_row && (!EDGE || gnl < g.n)) ? widen(bias[gnl]) : 0.f;
             auto stage = [&](auto with_bias, auto row_bias) {
-                if constexpr (std::is_same<T, f16_t>::value && !decltype(with_bias)::value) {
+                if constexpr (std::is_same<T, f16_t>::value && !decltype(with_bias)::value && !SRC::ONCE) {
                     // fp16 without a bias: when every value of this column of tiles narrows to a normal number (one
                     // unsigned maximum per value to find out, wave-uniform), the two-instruction narrowing is exact
                     uint32_t worst = 0;
@@ -548,8 +560,11 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
                         constexpr int i = decltype(ivc)::value / NV, v = decltype(ivc)::value % NV;
                         // accumulator register v: 32 x 32 tiles hold rows 8 * (v / 4) + 4 * (lane / 32) + v % 4, 16 x 16 tiles rows 4 * (lane / 16) + v
                         const int row = MT == 32 ? i * 32 + 8 * (v / 4) + 4 * (lane >> 5) + (v % 4) : i * 16 + 4 * (lane >> 4) + v;
-                        T y = narrow<T>(acc[i][j][v]);
-                        if constexpr (decltype(row_bias)::value) {
+                        T y;
+                        if constexpr (SRC::ONCE) y = round_to<T>(decltype(with_bias)::value ? acc[i][j][v] + bcol : acc[i][j][v]);
+                        else y = narrow<T>(acc[i][j][v]);
+                        if constexpr (SRC::ONCE) {
+                        } else if constexpr (decltype(row_bias)::value) {
                             const int gmr = m0 + wm0 + row;
                             y = narrow<T>(widen(y) + ((!EDGE || gmr < g.m) ? widen(bias[gmr]) : 0.f));
                         } else if constexpr (decltype(with_bias)::value) {
@@ -559,7 +574,7 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
                     }
                 });
             };
-            if (has_bias && by_row) stage(std::true_type{}, std::true_type{});
+            if (!SRC::ONCE && has_bias && by_row) stage(std::true_type{}, std::true_type{});
             else if (has_bias) stage(std::true_type{}, std::false_type{});
             else stage(std::false_type{}, std::false_type{});
         });
@@ -590,7 +605,7 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
                     memcpy(y, &staged, 16);
                     memcpy(old, &was, 16);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) out[e] = narrow<T>(widen(old[e]) + widen(y[e]));
+                    for (int e = 0; e < 8; e++) out[e] = joined(old[e], y[e]);
                     memcpy(&o, out, 16);
                 }
                 __builtin_nontemporal_store(o, (u32x4_t*)(crow + gn_out));  // written once, never re-read: keep it out of the way of the operand panels in L2
@@ -604,7 +619,7 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
                     memcpy(y, &staged, 16);
                     memcpy(old, &was, 16);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) out[e] = narrow<T>(widen(old[e]) + widen(y[e]));
+                    for (int e = 0; e < 8; e++) out[e] = joined(old[e], y[e]);
                     memcpy(&o, out, 16);
                 }
                 *(u32x4_any_t*)(crow + gn) = o;
@@ -615,7 +630,7 @@ __device__ __forceinline__ void gemm_mfma16_block(const GemmArgs& g, int tiles_m
                 for (int e = 0; e < 8; e++) {
                     if (EDGE && gn + e >= g.n) break;
                     T* pc = crow + (long long)(gn + e) * g.c_cs;
-                    *pc = accum ? narrow<T>(widen(*pc) + widen(y[e])) : y[e];
+                    *pc = accum ? joined(*pc, y[e]) : y[e];
                 }
             }
         }

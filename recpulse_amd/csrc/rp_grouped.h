@@ -8,6 +8,8 @@ namespace rp {
 // By rows:     C[i, :] (+)= scale_w * A[i, :] . B_w + bias_w      for every row i of a group whose weight is w
 // By weights:  C_w (+)= sum over the rows i of w's groups of A[i, :]^T . B[i, :]
 // Strides in elements; B (by rows) and C (by weights) have a stride b_ws / c_ws from weight to weight.
+// accumulate: added to what C holds, after the product has been rounded (as a product of its own would be) or together with it
+enum { ACCUMULATE = 1, ACCUMULATE_JOINED = 2 };
 struct GroupedArgs {
     void* C;
     const void* A;
@@ -27,5 +29,16 @@ int launch_grouped_rows_generic(const GroupedArgs& g, GroupedLow low, int dtype)
 int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dtype);
 // out[w, :] (+)= sum over the rows of w's groups of x[i, :]
 int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype);
+
+
+// bf16 / fp16 on the tiles of the 16-bit MFMA kernel (rp_grouped_mfma16*.hip).  ragged: rows of any length and start.
+int launch_grouped_rows16_256_bf16(const GroupedArgs& g);
+int launch_grouped_rows16_256_f16(const GroupedArgs& g);
+int launch_grouped_weights16_256_bf16(const GroupedArgs& g);
+int launch_grouped_weights16_256_f16(const GroupedArgs& g);
+int launch_grouped_rows16_128(const GroupedArgs& g, bool ragged, int dtype);
+int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
+int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
+int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
 
 }  // namespace rp

@@ -8,8 +8,46 @@
 
 namespace rp {
 
-static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) { return launch_grouped_rows_generic(g, low, dtype); }
-static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) { return launch_grouped_weights_generic(g, low, dtype); }
+static bool is16(int dtype) { return dtype == RP_DTYPE_BFLOAT16 || dtype == RP_DTYPE_FLOAT16; }
+static int cus() {
+    const int n = device_cu_count() / 8 * 8;
+    return n >= 8 ? n : 256;
+}
+
+// How an operand of the tiled kernels lies: rows of whole 16-byte vectors that start on them, rows of at least a vector that do not overlap, or neither.
+enum Lie { LIE_WHOLE, LIE_RAGGED, LIE_NEITHER };
+static Lie lies(const void* p, long long row_stride, long long weight_stride, int length, int elem) {
+    const int vec = 16 / elem;
+    if (length < vec || row_stride < length || row_stride >= (1ll << 22)) return LIE_NEITHER;
+    return ((uintptr_t)p & 15) || row_stride % vec || weight_stride % vec || length % vec ? LIE_RAGGED : LIE_WHOLE;
+}
+static Lie worse(Lie a, Lie b) { return a > b ? a : b; }
+
+static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
+    if (is16(dtype) && low == LOW_NONE && g.a_cs == 1 && (g.b_cs == 1 || g.b_rs == 1) && !path_disabled("mfma")) {
+        const bool b_mc = g.b_cs == 1;
+        const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
+        const long long tiles256 = (long long)((g.gr.rows + 255) / 256) * ((g.n + 255) / 256), tiles128 = (long long)((g.gr.rows + 127) / 128) * ((g.n + 127) / 128);
+        const int mean = g.gr.rows / g.gr.groups;
+        if (lie == LIE_WHOLE && mean >= 256 && g.n >= 256 && g.k >= 256 && tiles256 >= cus() / 2)
+            return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_rows16_256_bf16(g) : launch_grouped_rows16_256_f16(g);
+        if (lie != LIE_NEITHER)
+            return mean >= 96 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_rows16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_rows16_64(g, lie == LIE_RAGGED, dtype);
+    }
+    return launch_grouped_rows_generic(g, low, dtype);
+}
+
+static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
+    if (is16(dtype) && low == LOW_NONE && !g.gr.ids && g.a_cs == 1 && g.b_cs == 1 && !path_disabled("mfma")) {
+        const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
+        const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
+        if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && tiles256 >= cus() / 2)
+            return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_weights16_256_bf16(g) : launch_grouped_weights16_256_f16(g);
+        if (lie != LIE_NEITHER)
+            return g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_weights16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_weights16_64(g, lie == LIE_RAGGED, dtype);
+    }
+    return launch_grouped_weights_generic(g, low, dtype);
+}
 
 static bool grouped_args_ok(const char* who, bool pointers, int groups, int rows, int k, int n, std::initializer_list<long long> strides, int dtype) {
     if (!pointers || groups <= 0 || rows <= 0 || k <= 0 || n <= 0) { set_error("%s: null operand or non-positive extent (groups=%d rows=%d k=%d n=%d)", who, groups, rows, k, n); return false; }
@@ -46,8 +84,8 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
     if (!grouped_args_ok(who, dy && offsets && (!dx || w) && (!dw || x), groups, rows, k, n, {dy_rs, x_rs, x_cs, w_gs, w_rs, w_cs, dx_rs}, dtype)) return -1;
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, nullptr, groups, rows, groups};
-    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx}, LOW_NONE, dtype) != 0) return -1;
-    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw}, LOW_NONE, dtype) != 0) return -1;
+    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0}, LOW_NONE, dtype) != 0) return -1;
+    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0}, LOW_NONE, dtype) != 0) return -1;
     if (db && launch_grouped_sums(db, dy, gr, n, dy_rs, accumulate_db, dtype) != 0) return -1;
     return 0;
 }
@@ -60,7 +98,7 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
     const RowGroups gr{offsets, ids, segments, rows, adapters};
     if (grouped_rows(GroupedArgs{h, x, a, nullptr, scales, gr, k, rank, x_rs, x_cs, (long long)k * rank, rank, 1, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
     if (rp_hip_gemm_strided_batched(y, x, w, bias, 1, rows, k, n, 0, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 1, 0, dtype) != 0) return -1;
-    return grouped_rows(GroupedArgs{y, h, b, nullptr, nullptr, gr, rank, n, rank, 1, (long long)rank * n, n, 1, 0, y_rs, 1}, LOW_A, dtype);
+    return grouped_rows(GroupedArgs{y, h, b, nullptr, nullptr, gr, rank, n, rank, 1, (long long)rank * n, n, 1, 0, y_rs, ACCUMULATE_JOINED}, LOW_A, dtype);
 }
 
 int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
@@ -75,10 +113,10 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
     if ((dx || da) && grouped_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
     if (dx) {
         if (rp_hip_gemm_strided_batched(dx, dy, w, nullptr, 1, rows, n, k, 0, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, 1, accumulate_dx, dtype) != 0) return -1;
-        if (grouped_rows(GroupedArgs{dx, u, a, nullptr, nullptr, gr, rank, k, rank, 1, (long long)k * rank, 1, rank, 0, dx_rs, 1}, LOW_A, dtype) != 0) return -1;
+        if (grouped_rows(GroupedArgs{dx, u, a, nullptr, nullptr, gr, rank, k, rank, 1, (long long)k * rank, 1, rank, 0, dx_rs, ACCUMULATE_JOINED}, LOW_A, dtype) != 0) return -1;
     }
-    if (da && grouped_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da}, LOW_B, dtype) != 0) return -1;
-    if (db && grouped_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db}, LOW_A, dtype) != 0) return -1;
+    if (da && grouped_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0}, LOW_B, dtype) != 0) return -1;
+    if (db && grouped_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, LOW_A, dtype) != 0) return -1;
     return 0;
 }
 

@@ -1,6 +1,7 @@
 // Grouped products for any strides, sizes and types: 64 x 64 tiles, 16 of k at a time through LDS, scalar multiply-adds, 4 x 4 outputs a
 // thread.  What no other kernel takes comes here: widths below a vector, operands without a unit stride, float64 and float32
-// next to low-rank activations in the accumulate type.  Sums in the accumulate type, one rounding at the end.
+// next to low-rank activations in the accumulate type.  Sums in the accumulate type, rounded at the end, and once more where they are added to what the
+// output holds (as a product of its own would be).
 #include "rp_grouped.h"
 
 #include <type_traits>
@@ -64,8 +65,10 @@ __global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g
             TC* p = (TC*)g.C + (rt.begin + tr + i) * g.c_rs + n0 + tc + j;
             A v = scale * acc[i][j];
             if (bias) v += widen(bias[(long long)rt.weight * g.n + n0 + tc + j]);
-            if (g.accumulate) v += widen(*p);
-            *p = round_to<TC>(v);
+            if (g.accumulate == ACCUMULATE_JOINED) v += widen(*p);
+            TC y = round_to<TC>(v);
+            if (g.accumulate == ACCUMULATE) y = round_to<TC>(widen(*p) + widen(y));
+            *p = y;
         }
 }
 
@@ -90,8 +93,9 @@ __global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArg
             if (tr + i >= m || tc + j >= n) continue;
             TC* p = (TC*)g.C + w * g.c_ws + (m0 + tr + i) * g.c_rs + n0 + tc + j;
             A v = acc[i][j];
-            if (g.accumulate) v += widen(*p);
-            *p = round_to<TC>(v);
+            TC y = round_to<TC>(v);
+            if (g.accumulate) y = round_to<TC>(widen(*p) + widen(y));
+            *p = y;
         }
 }
 
@@ -114,8 +118,9 @@ __global__ void __launch_bounds__(256) grouped_sums_kernel(T* out, const T* x, R
     if (q || c >= cols) return;
     A v = ((parts[0][threadIdx.x] + parts[1][threadIdx.x]) + parts[2][threadIdx.x]) + parts[3][threadIdx.x];
     T* p = out + (long long)w * cols + c;
-    if (accumulate) v += widen(*p);
-    *p = round_to<T>(v);
+    T y = round_to<T>(v);
+    if (accumulate) y = round_to<T>(widen(*p) + widen(y));
+    *p = y;
 }
 
 static bool grid_ok(long long blocks, const char* what) {

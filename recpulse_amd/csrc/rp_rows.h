@@ -67,4 +67,32 @@ __device__ __forceinline__ RowTile find_row_tile(const RowGroups& gr, int tile, 
     return RowTile{-1, -1, 0, 0};
 }
 
+// The same for a workgroup that looks up many tiles: up to 64 groups are read and added up once and kept a lane each.
+struct RowTiles {
+    RowGroups gr;
+    int tile, total;                   // rows of a tile; how many tiles there are
+    int b, e, w, upto, tiles;          // of this lane's group, if there are at most 64
+    __device__ __forceinline__ RowTiles(const RowGroups& groups, int rows_of_tile) : gr(groups), tile(rows_of_tile), b(0), e(0), w(-1) {
+        const int lane = threadIdx.x & 63;
+        total = 0;
+        for (int g0 = 0; g0 < gr.groups; g0 += 64) {
+            b = e = 0;
+            w = -1;
+            if (g0 + lane < gr.groups) { b = gr.begin(g0 + lane); e = gr.end(g0 + lane); w = gr.weight(g0 + lane); }
+            tiles = w < 0 ? 0 : (e - b + tile - 1) / tile;
+            upto = total + wave_prefix_sum(tiles, lane);
+            total = __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    __device__ __forceinline__ RowTile find(int id) const {
+        if (gr.groups > 64) return find_row_tile(gr, tile, id);
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > id);
+        if (!past) return RowTile{-1, -1, 0, 0};
+        const int l = __builtin_ctzll(past);
+        const int first = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l);
+        const int begin = __builtin_amdgcn_readlane(b, l) + (id - first) * tile, end = __builtin_amdgcn_readlane(e, l);
+        return RowTile{l, __builtin_amdgcn_readlane(w, l), begin, begin + tile < end ? begin + tile : end};
+    }
+};
+
 }  // namespace rp

@@ -25,11 +25,13 @@ def ids_of(dt):
     return NAMES[dt]
 
 
-def within(got, want, magnitude, terms, dt, roundings=1):
-    """got and want float64; magnitude: the sum of the products' magnitudes."""
+def within(got, want, magnitude, terms, dt, roundings=1, added=0.0):
+    """got and want float64; magnitude: the sum of the products' magnitudes; added: what the rounded product (want - added) was added to,
+    which is a rounding of the product's value and one of the sum's."""
     fine = np.isfinite(want)
     assert np.array_equal(np.isfinite(got), fine) and np.array_equal(np.isnan(got), np.isnan(want))
-    bound = roundings * (HALF_STEP[dt] * np.abs(want) + TINY[dt]) + (terms + 8) * UNIT[dt] * magnitude * (1 + HALF_STEP[dt])
+    value = np.abs(want) + (np.abs(want - added) if added else 0.0)
+    bound = roundings * (HALF_STEP[dt] * value * (1 + HALF_STEP[dt]) + 2 * TINY[dt]) + (terms + 8) * UNIT[dt] * magnitude * (1 + HALF_STEP[dt])
     worst = np.max(np.where(fine, np.abs(np.where(fine, got - want, 0)) - bound, -1.0), initial=-1.0)
     assert worst <= 0, f"{worst} beyond the bound"
 
@@ -320,21 +322,20 @@ class Grouped:
     def check_backward(self, out, accumulate=0):
         dx, dw, db = out
         last, dt, old = self.offsets[-1], self.dt, 3.0 if accumulate else 0.0
-        roundings = 1
         if dx is not None:
             got = oracle.to_f64(dx.numpy(), dt)
             ref, size = grouped_want(self.g, self.w.transpose(0, 2, 1), None, self.offsets)
-            within(got[:last, :self.k], ref[:last] + old, size[:last] + old, self.n + 1, dt, roundings)
+            within(got[:last, :self.k], ref[:last] + old, size[:last] + old, self.n + 1, dt, added=old)
             assert np.all(got[last:] == 3.0) and np.all(got[:, self.k:] == 3.0)
         spans = list(zip(self.offsets, self.offsets[1:]))
         most = max(f - b for b, f in spans)
         if dw is not None:
             ref = np.stack([self.x[b:f].T @ self.g[b:f] for b, f in spans])
             size = np.stack([np.abs(self.x[b:f]).T @ np.abs(self.g[b:f]) for b, f in spans])
-            within(oracle.to_f64(dw.numpy(), dt), ref + old, size + old, most + 1, dt, roundings)
+            within(oracle.to_f64(dw.numpy(), dt), ref + old, size + old, most + 1, dt, added=old)
         if db is not None:
             ref, size = (np.stack([f(self.g[b:e]).sum(0) for b, e in spans]) for f in (lambda a: a, np.abs))
-            within(oracle.to_f64(db.numpy(), dt), ref + old, size + old, most + 1, dt, roundings)
+            within(oracle.to_f64(db.numpy(), dt), ref + old, size + old, most + 1, dt, added=old)
 
 
 SHAPES = [  # groups, rows, k, n, empty groups, rows behind the last
@@ -524,9 +525,9 @@ class Adapters:
             else:
                 self.thrice_rounded(got, dx, base, old, size + reach, n + rank + 2)
         if out[1] is not None:
-            within(oracle.to_f64(out[1].numpy(), dt), da + old, da_size + old, rows + n + 2, dt)
+            within(oracle.to_f64(out[1].numpy(), dt), da + old, da_size + old, rows + n + 2, dt, added=old)
         if out[2] is not None:
-            within(oracle.to_f64(out[2].numpy(), dt), db + old, db_size + old, rows + k + 2, dt)
+            within(oracle.to_f64(out[2].numpy(), dt), db + old, db_size + old, rows + k + 2, dt, added=old)
 
 
 ADAPTER_SHAPES = [  # segments, adapters, rows, k, n, rank, rows behind the last segment
