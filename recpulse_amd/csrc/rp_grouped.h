@@ -41,4 +41,21 @@ int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
 
+// bf16 / fp16, row tiles of a few rows against a row-major weight that is streamed once (rp_grouped_stream16.hip)
+bool grouped_stream16_takes(const GroupedArgs& g);
+int launch_grouped_stream16(const GroupedArgs& g, const struct AdapterTerm* term, int dtype);
+
+// + h[i] . b_a for the rows i of adapter a: what a layer's adapters add to its shared product (strides of b in elements)
+struct AdapterTerm {
+    const float* h;                // [rows, rank] dense
+    const void* b;                 // [adapters, rank, n]
+    RowGroups gr;                  // the segments
+    int rank;
+    long long b_ws, b_rs, b_cs;
+};
+
+// h[i] = scales[a] x[i] . a_a in float32 for bf16 / fp16 operands (rp_adapter16.hip); C is h
+bool adapter_shrink16_takes(const GroupedArgs& g);
+int launch_adapter_shrink16(const GroupedArgs& g, int dtype);
+
 }  // namespace rp

@@ -14,13 +14,22 @@ template <> __device__ __forceinline__ f16_t round_to<f16_t>(float v) { f16_t r;
 
 // Rows in groups: group g holds rows [offsets[g], offsets[g + 1]) of `rows`, and its weight is number ids[g] of `weights` (ids null:
 // g itself).  The offsets are device memory that no host code has seen: whatever they hold, begin and end are clamped to
-// the rows there are, and a weight number out of range stands for a group without a weight.
+// the rows there are, and a weight number out of range stands for a group without a weight.  Without offsets (null) there is one group of all rows.
 struct RowGroups {
     const int* offsets;
     const int* ids;
     int groups, rows, weights;
-    __device__ __forceinline__ int begin(int g) const { const int o = offsets[g]; return o < 0 ? 0 : o > rows ? rows : o; }
-    __device__ __forceinline__ int end(int g) const { const int b = begin(g), e = offsets[g + 1] > rows ? rows : offsets[g + 1]; return e > b ? e : b; }
+    __device__ __forceinline__ int begin(int g) const { const int o = offsets ? offsets[g] : g ? rows : 0; return o < 0 ? 0 : o > rows ? rows : o; }
+    __device__ __forceinline__ int end(int g) const { const int b = begin(g), o = offsets ? offsets[g + 1] : rows, e = o > rows ? rows : o; return e > b ? e : b; }
+    // the weight of row i's group, -1 if it has none (offsets in order; the last group that begins at or before i and does not end before it)
+    __device__ __forceinline__ int weight_of_row(int i) const {
+        int lo = 0, hi = groups;                              // the number of groups that end at or before i
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (end(mid) <= i) lo = mid + 1; else hi = mid;
+        }
+        return lo < groups && begin(lo) <= i ? weight(lo) : -1;
+    }
     __device__ __forceinline__ int weight(int g) const { const int w = ids ? ids[g] : g; return w >= 0 && w < weights ? w : -1; }
 };
 
