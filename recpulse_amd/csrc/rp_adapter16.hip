@@ -1,182 +1,20 @@
-// bf16 / fp16 rows times an adapter's narrow factor: h[i] = scale x[i] . A_a (k x rank) in float32, and with B_a^T for A_a the gradient's
-// u[i] = scale dy[i] . B_a^T.
-//
-// The product is bound by reading x (rows * k * 2 bytes) and, where every request has an adapter of its own, the adapters; its
-// arithmetic is rank / 16 MFMAs per 16 rows and 32 of k.  A workgroup of sixteen waves owns 16 or 32 rows of one segment and the
-// whole rank; the waves share k, 32 at a time in turn, and add their sums in wave order: few rows still have 64 KB of loads in
-// flight a CU, and there is one launch and no workspace.
-//
-// v_mfma_f32_16x16x32: lane (q, j) = (lane / 16, lane % 16) supplies k = 8q .. 8q + 7 of row j, one 16-byte load of x.  A factor that is
-// contiguous along k (B^T) is read the same way.  One that is contiguous along the rank goes through LDS of the wave's own as it lies and
-// comes back with the transposing read (ds_read_b64_tr_b16): 2-byte loads straight from memory would keep a CU's address unit busy for 8 us
-// at 32 requests of k = 4096 and rank 16.
-#include "rp_grouped.h"
-
-#include <type_traits>
+// bf16 / fp16 rows times an adapter's narrow factor in a launch of its own, and beside the first pass of a few rows' shared projection.
+#include "rp_adapter16.h"
+#include "rp_grouped_stream16.h"
 
 namespace rp {
 
-constexpr int SH_WAVES = 16, SH_STEP = 32, SH_MAX_RANK = 128;
-
-typedef unsigned int u32x4_odd_t __attribute__((ext_vector_type(4), aligned(2)));       // a 16-byte vector at any element
-typedef uint16_t __attribute__((address_space(3))) sh_lds_u16;
-
-template <typename T> struct sh_ops;
-template <> struct sh_ops<bf16_t> {
-    static __device__ __forceinline__ f32x4_t mma(u32x4_t a, u32x4_t b, f32x4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    }
-};
-template <> struct sh_ops<f16_t> {
-    static __device__ __forceinline__ f32x4_t mma(u32x4_t a, u32x4_t b, f32x4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-    }
-};
-
-// eight consecutive 16-bit values at p, of which the first n are there
-__device__ __forceinline__ u32x4_t load8(const uint16_t* p, int n) {
-    if (n >= 8) return *(const u32x4_odd_t*)p;
-    u32x4_t v = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 7; e++)
-        if (e < n) v[e / 2] |= (uint32_t)p[e] << (16 * (e % 2));
-    return v;
-}
-
-// LDS of a wave's piece of the factor: 32 rows of k, 16 * NC columns and 8 more, so that the rows that a transposing read takes together start in different banks
-template <int NC> constexpr int sh_pitch() { return 16 * NC + 8; }
-template <int NC, int RT> constexpr int sh_lds_bytes(bool along_k) {
-    const int stage = along_k ? 0 : SH_WAVES * SH_STEP * sh_pitch<NC>() * 2, sums = SH_WAVES * 4 * 64 * 16;
-    return stage > sums ? stage : sums;
-}
-
-// NC: 16-column tiles of the rank; RT: 16-row tiles; ALONG_K: the factor is contiguous along k; PIECE: values a load of the factor takes (8, or 1 where its
-// rows are no whole vectors)
 template <typename T, int NC, int RT, bool ALONG_K, int PIECE>
-__global__ void __launch_bounds__(SH_WAVES * 64) adapter_shrink16_kernel(GroupedArgs g) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char sh_lds[];
-    const RowTile rt = find_row_tile(g.gr, 16 * RT, (int)blockIdx.x);
-    if (rt.group < 0) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
-    const int rank = g.n;
-    const uint16_t* xp[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {                               // (rows past the segment repeat its last: their sums are not stored)
-        const int r = rt.begin + 16 * i + j;
-        xp[i] = (const uint16_t*)g.A + (r < rt.end ? r : rt.end - 1) * g.a_rs;
-    }
-    const uint16_t* f = (const uint16_t*)g.B + rt.weight * g.b_ws;
-    constexpr int PITCH = sh_pitch<NC>(), PER_ROW = 16 * NC / PIECE, PIECES = ALONG_K ? NC : SH_STEP * PER_ROW / 64;
-    uint16_t* stage = (uint16_t*)sh_lds + wave * SH_STEP * PITCH;
-    if constexpr (!ALONG_K) {
-        if (rank < 16 * NC)
-            for (int i = lane; i < SH_STEP * PITCH / 2; i += 64) ((uint32_t*)stage)[i] = 0;       // columns past the rank
-    }
-    using piece_t = std::conditional_t<ALONG_K || PIECE == 8, u32x4_t, uint16_t>;
-    u32x4_t xv[2][RT];
-    piece_t fv[2][PIECES];
-    auto request = [&](auto slotc, int k0) {
-        constexpr int S = decltype(slotc)::value;
-#pragma unroll
-        for (int i = 0; i < RT; i++) xv[S][i] = load8(xp[i] + k0 + 8 * q, g.k - k0 - 8 * q);
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-            if constexpr (ALONG_K) {
-                const int c = 16 * p + j < rank ? 16 * p + j : rank - 1;
-                fv[S][p] = load8(f + c * g.b_cs + k0 + 8 * q, g.k - k0 - 8 * q);
-            } else {
-                const int id = lane + 64 * p, r = k0 + id / PER_ROW, c = id % PER_ROW * PIECE;
-                fv[S][p] = piece_t{};
-                if (r < g.k && c < rank) {
-                    if constexpr (PIECE == 8) fv[S][p] = *(const u32x4_t*)(f + r * g.b_rs + c);
-                    else fv[S][p] = f[r * g.b_rs + c];
-                }
-            }
-        }
-    };
-    f32x4_t acc[RT][NC];
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int c = 0; c < NC; c++) acc[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](auto slotc) {
-        constexpr int S = decltype(slotc)::value;
-        u32x4_t b[NC];
-        if constexpr (ALONG_K) {
-#pragma unroll
-            for (int c = 0; c < NC; c++) b[c] = fv[S][c];
-        } else {
-#pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-                const int id = lane + 64 * p;
-                uint16_t* at = stage + id / PER_ROW * PITCH + id % PER_ROW * PIECE;
-                if (id % PER_ROW * PIECE < rank) {
-                    if constexpr (PIECE == 8) *(u32x4_t*)at = fv[S][p];
-                    else *at = fv[S][p];
-                }
-            }
-            // (the wave's own LDS, and its instructions are executed in order: no barrier)
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint16_t* at = stage + (8 * q + 4 * h + (j >> 2)) * PITCH + 16 * c + 4 * (j & 3);
-                    const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(sh_lds_u16*)at);
-                    const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
-                    b[c][2 * h] = w[0];
-                    b[c][2 * h + 1] = w[1];
-                }
-            __builtin_amdgcn_wave_barrier();
-        }
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int c = 0; c < NC; c++) acc[i][c] = sh_ops<T>::mma(xv[S][i], b[c], acc[i][c]);
-    };
-    using S0 = std::integral_constant<int, 0>;
-    using S1 = std::integral_constant<int, 1>;
-    constexpr int TURN = SH_WAVES * SH_STEP;
-    const int first = wave * SH_STEP;
-    if (first < g.k) request(S0{}, first);
-    for (int k0 = first; k0 < g.k; k0 += 2 * TURN) {
-        if (k0 + TURN < g.k) request(S1{}, k0 + TURN);
-        multiply(S0{});
-        if (k0 + TURN >= g.k) break;
-        if (k0 + 2 * TURN < g.k) request(S0{}, k0 + 2 * TURN);
-        multiply(S1{});
-    }
-
-    // the waves' sums, four 16 x 16 tiles at a time, a value a thread
-    float* sums = (float*)sh_lds;
-    float* h = (float*)g.C;
-    const float scale = g.scales ? g.scales[rt.weight] : 1.f;
-    constexpr int TILES = RT * NC;
-    static_for<0, (TILES + 3) / 4>([&](auto passc) {
-        constexpr int P0 = decltype(passc)::value * 4, P1 = P0 + 4 < TILES ? P0 + 4 : TILES;
-        __syncthreads();
-        static_for<P0, P1>([&](auto pc) {
-            constexpr int p = decltype(pc)::value;
-            *(f32x4_t*)(sums + ((wave * 4 + p - P0) * 64 + lane) * 4) = acc[p / NC][p % NC];
-        });
-        __syncthreads();
-        const int p = P0 + (int)(threadIdx.x >> 8), l = (threadIdx.x & 255) >> 2, v = threadIdx.x & 3;
-        if (p < P1) {
-            float s = 0;
-#pragma unroll
-            for (int w = 0; w < SH_WAVES; w++) s += sums[((w * 4 + p - P0) * 64 + l) * 4 + v];
-            const int row = rt.begin + 16 * (p / NC) + 4 * (l >> 4) + v, col = 16 * (p % NC) + (l & 15);
-            if (row < rt.end && col < rank) h[(long long)row * g.c_rs + col] = scale * s;
-        }
-    });
+__global__ void __launch_bounds__((sh_waves<NC, PIECE>() * 64)) adapter_shrink16_kernel(GroupedArgs g) {
+    adapter_shrink16_block<T, NC, RT, ALONG_K, PIECE, sh_waves<NC, PIECE>()>(g, (int)blockIdx.x);
 }
 
 template <typename T, int NC, int RT, bool ALONG_K, int PIECE>
 static int launch_shrink(const GroupedArgs& g) {
-    constexpr int lds = sh_lds_bytes<NC, RT>(ALONG_K);
+    constexpr int waves = sh_waves<NC, PIECE>(), lds = sh_lds_bytes<NC, RT, waves>(ALONG_K);
     auto kern = adapter_shrink16_kernel<T, NC, RT, ALONG_K, PIECE>;
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)max_row_tiles(g.gr.rows, g.gr.groups, 16 * RT)), dim3(SH_WAVES * 64), lds, current_stream(), g);
+    hipLaunchKernelGGL(kern, dim3((unsigned)max_row_tiles(g.gr.rows, g.gr.groups, 16 * RT)), dim3(waves * 64), lds, current_stream(), g);
     return check_launch("adapter_shrink16_kernel") ? 0 : -1;
 }
 
@@ -206,5 +44,58 @@ bool adapter_shrink16_takes(const GroupedArgs& g) {
 }
 
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype) { return dtype == RP_DTYPE_BFLOAT16 ? launch_shrink_rank<bf16_t>(g) : launch_shrink_rank<f16_t>(g); }
+
+// ---- a few rows: the shared projection's shares of k and the rows' h side by side, then one launch that adds them up with the adapters' terms ----
+// 32 rows with adapters of their own, 4096 x 4096 and rank 16 in bf16: ADAPTER_DECODE_FIGURES
+template <typename T, int CPL, int RB, int NC>
+__global__ void __launch_bounds__(GS_THREADS) adapter_first16_kernel(GroupedArgs shared, StreamGrid sg, GroupedArgs low, int low_blocks) {
+    if ((int)blockIdx.x < low_blocks) adapter_shrink16_block<T, NC, 1, false, 8, GS_WAVES>(low, (int)blockIdx.x);
+    else stream16_block<T, CPL, RB>(shared, sg, blockIdx.x - low_blocks);
+}
+
+template <typename T, int CPL, int RB, int NC>
+static int launch_first(const GroupedArgs& shared, const StreamGrid& sg, const GroupedArgs& low) {
+    constexpr int a = gs_lds_bytes<CPL>(), b = sh_lds_bytes<NC, 1, GS_WAVES>(false), lds = a > b ? a : b;
+    const long long low_blocks = (max_row_tiles(low.gr.rows, low.gr.groups, 16) + 7) / 8 * 8, blocks = low_blocks + stream16_blocks(shared, 16 * RB, CPL, sg.nsplit);
+    auto kern = adapter_first16_kernel<T, CPL, RB, NC>;
+    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), shared, sg, low, (int)low_blocks);
+    return check_launch("adapter_first16_kernel") ? 0 : -1;
+}
+
+template <typename T, int NC>
+static int launch_first_rows(const GroupedArgs& shared, const StreamGrid& sg, const GroupedArgs& low) {
+    const int rb = stream16_row_blocks(shared.gr);
+    if (rb == 1) return launch_first<T, 8, 1, NC>(shared, sg, low);
+    if (rb == 2) return launch_first<T, 8, 2, NC>(shared, sg, low);
+    return launch_first<T, 4, 4, NC>(shared, sg, low);
+}
+
+template <typename T>
+static int launch_first_rank(const GroupedArgs& shared, const StreamGrid& sg, const GroupedArgs& low) {
+    if (low.n <= 16) return launch_first_rows<T, 1>(shared, sg, low);
+    if (low.n <= 32) return launch_first_rows<T, 2>(shared, sg, low);
+    return launch_first_rows<T, 4>(shared, sg, low);
+}
+
+bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term) {
+    return grouped_stream16_takes(shared) && adapter_shrink16_takes(low) && low.b_cs == 1 && low.n % 8 == 0 && low.n <= 64 && ((uintptr_t)low.B & 15) == 0 &&
+           term.b_cs == 1 && term.b_rs % 8 == 0 && ((uintptr_t)term.b & 15) == 0;
+}
+
+int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype) {
+    // The sums lie in the null stream's own memory, or, as the split products of rp_hip_gemm_strided_batched do, in a block of the pool.
+    constexpr size_t most = 16 << 20;
+    StreamGrid sg{(shared.n + 127) / 128, stream16_splits(shared, most), nullptr};
+    const size_t bytes = (size_t)sg.nsplit * shared.gr.rows * shared.n * sizeof(float);
+    NullStreamScratch lease(bytes);
+    void* block = nullptr;
+    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
+    sg.partials = (float*)(lease.ptr ? lease.ptr : block);
+    int rc = dtype == RP_DTYPE_BFLOAT16 ? launch_first_rank<bf16_t>(shared, sg, low) : launch_first_rank<f16_t>(shared, sg, low);
+    if (rc == 0) rc = launch_stream16_combine(shared, sg, &term, dtype);
+    if (block) rp_hip_free(block);
+    return rc;
+}
 
 }  // namespace rp

@@ -41,10 +41,6 @@ int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
 
-// bf16 / fp16, row tiles of a few rows against a row-major weight that is streamed once (rp_grouped_stream16.hip)
-bool grouped_stream16_takes(const GroupedArgs& g);
-int launch_grouped_stream16(const GroupedArgs& g, const struct AdapterTerm* term, int dtype);
-
 // + h[i] . b_a for the rows i of adapter a: what a layer's adapters add to its shared product (strides of b in elements)
 struct AdapterTerm {
     const float* h;                // [rows, rank] dense
@@ -54,8 +50,17 @@ struct AdapterTerm {
     long long b_ws, b_rs, b_cs;
 };
 
+// bf16 / fp16, row tiles of a few rows against a row-major weight that is streamed once (rp_grouped_stream16.hip)
+bool grouped_stream16_takes(const GroupedArgs& g);
+int launch_grouped_stream16(const GroupedArgs& g, int dtype);
+struct StreamGrid;
+int launch_stream16_combine(const GroupedArgs& g, const StreamGrid& sg, const AdapterTerm* term, int dtype);
+
 // h[i] = scales[a] x[i] . a_a in float32 for bf16 / fp16 operands (rp_adapter16.hip); C is h
 bool adapter_shrink16_takes(const GroupedArgs& g);
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype);
+// The whole layer for a few rows: `shared` one group of all rows, `low` the product above, `term` what it adds
+bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term);
+int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype);
 
 }  // namespace rp

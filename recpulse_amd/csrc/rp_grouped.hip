@@ -25,7 +25,7 @@ static Lie worse(Lie a, Lie b) { return a > b ? a : b; }
 
 static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
     if (is16(dtype) && low == LOW_C && adapter_shrink16_takes(g)) return launch_adapter_shrink16(g, dtype);
-    if (is16(dtype) && low == LOW_NONE && grouped_stream16_takes(g)) return launch_grouped_stream16(g, nullptr, dtype);
+    if (is16(dtype) && low == LOW_NONE && grouped_stream16_takes(g)) return launch_grouped_stream16(g, dtype);
     if (is16(dtype) && low == LOW_NONE && g.a_cs == 1 && (g.b_cs == 1 || g.b_rs == 1) && !path_disabled("mfma")) {
         const bool b_mc = g.b_cs == 1;
         const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
@@ -98,10 +98,11 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
     if (!grouped_args_ok(who, y && h && x && w && a && b && ids && offsets && adapters > 0 && rank > 0, segments, rows, k, n, {x_rs, x_cs, w_rs, w_cs, y_rs}, dtype) ||
         !output_rows_ok(who, "y", rows, n, y_rs)) return -1;
     const RowGroups gr{offsets, ids, segments, rows, adapters};
-    if (grouped_rows(GroupedArgs{h, x, a, nullptr, scales, gr, k, rank, x_rs, x_cs, (long long)k * rank, rank, 1, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
+    const GroupedArgs low{h, x, a, nullptr, scales, gr, k, rank, x_rs, x_cs, (long long)k * rank, rank, 1, 0, rank, 0};
     const GroupedArgs shared{y, x, w, bias, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, k, n, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 0};
     const AdapterTerm term{(const float*)h, b, gr, rank, (long long)rank * n, n, 1};
-    if (is16(dtype) && ((uintptr_t)b & 15) == 0 && grouped_stream16_takes(shared)) return launch_grouped_stream16(shared, &term, dtype);
+    if (is16(dtype) && adapter_few_rows16_takes(shared, low, term)) return launch_adapter_few_rows16(shared, low, term, dtype);
+    if (grouped_rows(low, LOW_C, dtype) != 0) return -1;
     if (rp_hip_gemm_strided_batched(y, x, w, bias, 1, rows, k, n, 0, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 1, 0, dtype) != 0) return -1;
     return grouped_rows(GroupedArgs{y, h, b, nullptr, nullptr, gr, rank, n, rank, 1, (long long)rank * n, n, 1, 0, y_rs, ACCUMULATE_JOINED}, LOW_A, dtype);
 }

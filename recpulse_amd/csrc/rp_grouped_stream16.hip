@@ -1,220 +1,127 @@
-// bf16 / fp16 rows in groups of a few rows each against row-major weights: decoding with experts, or with adapters beside a shared weight.
-//
-// Bound by reading the weights: every weight that has a row is read once.  As in the few-row kernel for one matrix
-// (rp_gemm_mfma16_stream128.hip) they go from memory to registers to the MFMAs: lane (q, j) = (lane / 16, lane % 16) loads CPL adjacent
-// columns of eight rows of k (8q .. 8q + 7), the 8 x CPL block is transposed in registers with byte permutes, and column residue c becomes the
-// operand of one v_mfma_f32_16x16x32 whose column j is column CPL * j + c of the strip.  The rows of x are the other operand, 16 bytes a lane.
-//
-// A workgroup owns 16 * RB rows of one group and a strip of 16 * CPL columns; its eight waves share k, 32 rows of it at a time in turn, two
-// rounds in flight each, and add their tiles through LDS in wave order: one launch, no workspace, repeatable bits.  Strips are as wide
-// as leaves about a workgroup a CU (launch_grouped_stream16).
-#include "rp_grouped.h"
-
-#include <type_traits>
+// Launches of the kernel for a few rows a group (rp_grouped_stream16.h), and the second launch that adds shares of k.
+#include "rp_grouped_stream16.h"
 
 namespace rp {
 
-constexpr int GS_WAVES = 8, GS_ROUND = 32;
+template <typename T, int CPL, int RB>
+__global__ void __launch_bounds__(GS_THREADS) grouped_stream16_kernel(GroupedArgs g, StreamGrid sg) { stream16_block<T, CPL, RB>(g, sg, blockIdx.x); }
 
-template <typename T> struct gs_ops;
-template <> struct gs_ops<bf16_t> {
-    static __device__ __forceinline__ f32x4_t mma(u32x4_t a, u32x4_t b, f32x4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+// y[row] = the shares' sums in order + bias + what the row's adapter adds, rounded once; rows of no group are left alone.  A workgroup does 32
+// vectors of 8 columns of one row: eight threads share a vector's shares of k and its rank, and their sums are added in order.  The loads
+// of a thread are two or three, so the launch takes the time of a few round trips.
+template <typename T>
+__global__ void __launch_bounds__(256) stream16_combine_kernel(GroupedArgs g, StreamGrid sg, AdapterTerm term, int blocks_per_row) {
+    __shared__ __attribute__((aligned(16))) float parts[8][32][8];
+    const int row = (int)(blockIdx.x / blocks_per_row), col = ((int)(blockIdx.x % blocks_per_row) * 32 + (threadIdx.x & 31)) * 8, part = threadIdx.x >> 5;
+    const bool in = col < g.n;
+    float s[8];
+#pragma unroll
+    for (int v = 0; v < 8; v++) s[v] = 0.f;
+    for (int p = part; p < sg.nsplit && in; p += 8) {
+        const float* at = sg.partials + ((long long)p * g.gr.rows + row) * g.n + col;
+        const f32x4_t lo = *(const f32x4_t*)at, hi = *(const f32x4_t*)(at + 4);
+#pragma unroll
+        for (int v = 0; v < 4; v++) { s[v] += lo[v]; s[4 + v] += hi[v]; }
     }
-};
-template <> struct gs_ops<f16_t> {
-    static __device__ __forceinline__ f32x4_t mma(u32x4_t a, u32x4_t b, f32x4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-    }
-};
-
-template <int CPL> struct gs_vec;                    // CPL 16-bit values
-template <> struct gs_vec<8> { using type = u32x4_t; };
-template <> struct gs_vec<4> { using type = u32x2_t; };
-template <> struct gs_vec<2> { using type = uint32_t; };
-template <int CPL> __device__ __forceinline__ uint32_t gs_word(typename gs_vec<CPL>::type v, int i) {
-    if constexpr (CPL == 2) return v;
-    else return v[i];
-}
-template <int CPL> __device__ __forceinline__ typename gs_vec<CPL>::type gs_load(__amdgpu_buffer_rsrc_t r, uint32_t off) {       // (streamed: read once)
-    if constexpr (CPL == 8) return __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 2);
-    else if constexpr (CPL == 4) return __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 2);
-    else return __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 2);
-}
-
-// ADAPT: `term` is added to the rows (one group; the rows' adapters in `term`)
-template <typename T, int CPL, int RB, bool ADAPT>
-__global__ void __launch_bounds__(GS_WAVES * 64, 2) grouped_stream16_kernel(GroupedArgs g, AdapterTerm term, int strips) {
-    constexpr int COLS = 16 * CPL, PITCH = COLS + 4, ROWS = 16 * RB;
-    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [GS_WAVES][16][PITCH]
-    const RowTile rt = find_row_tile(g.gr, ROWS, (int)(blockIdx.x / strips));
-    if (rt.group < 0) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
-    const int n0 = (int)(blockIdx.x % strips) * COLS, m = rt.end - rt.begin;
-    const uint16_t* B = (const uint16_t*)g.B + rt.weight * g.b_ws + n0;
-    const uint16_t* A = (const uint16_t*)g.A + rt.begin * g.a_rs;
-    const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc(B, ((long long)(g.k - 1) * g.b_rs + g.n - n0) * 2), a_rsrc = buffer_rsrc(A, ((long long)(m - 1) * g.a_rs + g.k) * 2);
-    const bool col_in = n0 + CPL * j < g.n;                               // (n is a multiple of 8)
-    const uint32_t b_lane = (uint32_t)((8 * q * g.b_rs + CPL * j) * 2), b_step = (uint32_t)(g.b_rs * 2);
-    uint32_t a_lane[RB];
-#pragma unroll
-    for (int i = 0; i < RB; i++) a_lane[i] = 16 * i + j < m ? (uint32_t)(((16 * i + j) * g.a_rs + 8 * q) * 2) : BUFFER_OOB;
-
-    typename gs_vec<CPL>::type raw[2][8];
-    u32x4_t av[2][RB];
-    auto request = [&](auto slotc, int k0) {                              // (rounds past k read zeros)
-        constexpr int S = decltype(slotc)::value;
-#pragma unroll
-        for (int e = 0; e < 8; e++) raw[S][e] = gs_load<CPL>(b_rsrc, col_in && k0 + 8 * q + e < g.k ? b_lane + (uint32_t)(k0 + e) * b_step : BUFFER_OOB);
-#pragma unroll
-        for (int i = 0; i < RB; i++) av[S][i] = __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, (int)(k0 + 8 * q < g.k ? a_lane[i] + 2 * k0 : BUFFER_OOB), 0, 0);      // (k is a multiple of 8)
+    // the row's group: how many end at or before the row (uniform: the same loads for the whole workgroup)
+    auto weight_of = [&](const RowGroups& gr) {
+        int before = 0;
+        for (int i = 0; i < gr.groups; i++) before += gr.end(i) <= row ? 1 : 0;
+        return before < gr.groups && gr.begin(before) <= row ? gr.weight(before) : -1;
     };
-    f32x4_t acc[RB][CPL];
-#pragma unroll
-    for (int i = 0; i < RB; i++)
-#pragma unroll
-        for (int c = 0; c < CPL; c++) acc[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](auto slotc) {
-        constexpr int S = decltype(slotc)::value;
-#pragma unroll
-        for (int c = 0; c < CPL; c++) {
-            u32x4_t b;
-#pragma unroll
-            for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(gs_word<CPL>(raw[S][2 * d + 1], c / 2), gs_word<CPL>(raw[S][2 * d], c / 2), (c & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int i = 0; i < RB; i++) acc[i][c] = gs_ops<T>::mma(av[S][i], b, acc[i][c]);
-        }
-    };
-    using S0 = std::integral_constant<int, 0>;
-    using S1 = std::integral_constant<int, 1>;
-    constexpr int TURN = GS_WAVES * GS_ROUND;
-    const int first = wave * GS_ROUND;
-    request(S0{}, first);
-    request(S1{}, first + TURN);
-
-    // this thread's outputs: EACH vectors of 8 columns of a row
-    constexpr int VPR = COLS / 8, EACH = (ROWS * VPR + GS_WAVES * 64 - 1) / (GS_WAVES * 64);
-    float extra[EACH][8];
-#pragma unroll
-    for (int o = 0; o < EACH; o++) {
-        const int id = threadIdx.x + o * GS_WAVES * 64, row = id / VPR, col = n0 + id % VPR * 8;
-        const bool in = row < m && col < g.n;
-#pragma unroll
-        for (int v = 0; v < 8; v++) extra[o][v] = 0.f;
-        if (in && g.bias) {
-            T e[8];
-            const u32x4_t w = *(const u32x4_t*)((const uint16_t*)g.bias + (long long)rt.weight * g.n + col);
-            __builtin_memcpy(e, &w, 16);
-#pragma unroll
-            for (int v = 0; v < 8; v++) extra[o][v] = widen(e[v]);
-        }
-        if constexpr (ADAPT) {                                            // (while the first rounds are on their way)
-            const int a = in ? term.gr.weight_of_row(rt.begin + row) : -1;
-            if (a >= 0) {
-                const float* h = term.h + (long long)(rt.begin + row) * term.rank;
-                const uint16_t* b = (const uint16_t*)term.b + a * term.b_ws + col;
+    const int w = weight_of(g.gr);
+    if (w < 0) return;                                       // (the whole workgroup)
+    if (term.h) {
+        const int a = weight_of(term.gr);
+        if (a >= 0 && in) {
+            const float* h = term.h + (long long)row * term.rank;
+            const uint16_t* b = (const uint16_t*)term.b + a * term.b_ws + col;
 #pragma unroll 4
-                for (int r = 0; r < term.rank; r++) {
-                    const float hr = h[r];
-                    T e[8];
-                    const u32x4_t w = *(const u32x4_t*)(b + r * term.b_rs);
-                    __builtin_memcpy(e, &w, 16);
+            for (int r = part; r < term.rank; r += 8) {
+                const float hr = h[r];
+                T e[8];
+                const u32x4_t x = *(const u32x4_t*)(b + r * term.b_rs);
+                __builtin_memcpy(e, &x, 16);
 #pragma unroll
-                    for (int v = 0; v < 8; v++) extra[o][v] += hr * widen(e[v]);
-                }
+                for (int v = 0; v < 8; v++) s[v] += hr * widen(e[v]);
             }
         }
     }
+    *(f32x4_t*)&parts[part][threadIdx.x & 31][0] = f32x4_t{s[0], s[1], s[2], s[3]};
+    *(f32x4_t*)&parts[part][threadIdx.x & 31][4] = f32x4_t{s[4], s[5], s[6], s[7]};
+    __syncthreads();
+    // a column a thread
+    const int c = threadIdx.x, gc = (int)(blockIdx.x % blocks_per_row) * 256 + c;
+    if (gc >= g.n) return;
+    float t = parts[0][c >> 3][c & 7];
+#pragma unroll
+    for (int p = 1; p < 8; p++) t += parts[p][c >> 3][c & 7];
+    if (g.bias) t += widen(((const T*)g.bias)[(long long)w * g.n + gc]);
+    T* out = (T*)g.C + row * g.c_rs + gc;
+    T y = round_to<T>(t);
+    if (g.accumulate) y = round_to<T>(widen(*out) + widen(y));
+    *out = y;
+}
 
-    for (int k0 = first; k0 < g.k; k0 += 2 * TURN) {
-        multiply(S0{});
-        request(S0{}, k0 + 2 * TURN);
-        multiply(S1{});
-        request(S1{}, k0 + 3 * TURN);
-    }
-
-    static_for<0, RB>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        if (i) __syncthreads();
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-#pragma unroll
-            for (int c = 0; c < CPL; c += 2) {
-                float* at = gs_sums + (wave * 16 + 4 * q + v) * PITCH + CPL * j + c;
-                at[0] = acc[i][c][v];
-                at[1] = acc[i][c + 1][v];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int o = 0; o < EACH; o++) {
-            const int id = threadIdx.x + o * GS_WAVES * 64, row = id / VPR, cv = id % VPR * 8;
-            if (row / 16 != i || row >= m || n0 + cv >= g.n) continue;
-            float s[8];
-#pragma unroll
-            for (int v = 0; v < 8; v++) s[v] = 0.f;
-#pragma unroll
-            for (int w = 0; w < GS_WAVES; w++) {
-                const float* at = gs_sums + (w * 16 + row % 16) * PITCH + cv;
-                const f32x4_t lo = *(const f32x4_t*)at, hi = *(const f32x4_t*)(at + 4);
-#pragma unroll
-                for (int v = 0; v < 4; v++) { s[v] += lo[v]; s[4 + v] += hi[v]; }
-            }
-            uint16_t* out = (uint16_t*)g.C + (rt.begin + row) * g.c_rs + n0 + cv;
-            T y[8];
-#pragma unroll
-            for (int v = 0; v < 8; v++) y[v] = round_to<T>(s[v] + extra[o][v]);
-            if (g.accumulate) {
-                T was[8];
-                __builtin_memcpy(was, out, 16);
-#pragma unroll
-                for (int v = 0; v < 8; v++) y[v] = round_to<T>(widen(was[v]) + widen(y[v]));
-            }
-            __builtin_memcpy(out, y, 16);
-        }
-    });
+int launch_stream16_combine(const GroupedArgs& g, const StreamGrid& sg, const AdapterTerm* term, int dtype) {
+    const int per_row = (g.n + 255) / 256;
+    const dim3 grid((unsigned)(g.gr.rows * per_row));
+    if (dtype == RP_DTYPE_BFLOAT16) hipLaunchKernelGGL(stream16_combine_kernel<bf16_t>, grid, dim3(256), 0, current_stream(), g, sg, term ? *term : AdapterTerm{}, per_row);
+    else hipLaunchKernelGGL(stream16_combine_kernel<f16_t>, grid, dim3(256), 0, current_stream(), g, sg, term ? *term : AdapterTerm{}, per_row);
+    return check_launch("stream16_combine_kernel") ? 0 : -1;
 }
 
 template <typename T, int CPL, int RB>
-static int launch_stream(const GroupedArgs& g, const AdapterTerm* term) {
-    constexpr int lds = GS_WAVES * 16 * (16 * CPL + 4) * 4;
-    const int strips = (g.n + 16 * CPL - 1) / (16 * CPL);
-    const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, 16 * RB) * strips;
+static int launch_stream(const GroupedArgs& g, StreamGrid sg) {
+    const long long blocks = stream16_blocks(g, 16 * RB, CPL, sg.nsplit);
     if (blocks > 0x7fffffffll) { set_error("grouped product: %lld tiles are more than a launch takes", blocks); return -1; }
-    auto launch = [&](auto kern) {
-        if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_WAVES * 64), lds, current_stream(), g, term ? *term : AdapterTerm{}, strips);
-        return check_launch("grouped_stream16_kernel") ? 0 : -1;
-    };
-    return term ? launch(grouped_stream16_kernel<T, CPL, RB, true>) : launch(grouped_stream16_kernel<T, CPL, RB, false>);
+    constexpr int lds = gs_lds_bytes<CPL>();
+    auto kern = grouped_stream16_kernel<T, CPL, RB>;
+    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), g, sg);
+    return check_launch("grouped_stream16_kernel") ? 0 : -1;
 }
 
 template <typename T, int CPL>
-static int launch_stream_rows(const GroupedArgs& g, const AdapterTerm* term) {
-    const int mean = (g.gr.rows + g.gr.groups - 1) / g.gr.groups;
-    if (g.gr.groups == 1 ? mean <= 16 : mean <= 10) return launch_stream<T, CPL, 1>(g, term);
-    if (g.gr.groups == 1 ? mean <= 32 : mean <= 20) return launch_stream<T, CPL, 2>(g, term);
-    return launch_stream<T, CPL, 4>(g, term);
+static int launch_stream_rows(const GroupedArgs& g, const StreamGrid& sg) {
+    const int rb = stream16_row_blocks(g.gr);
+    if (rb == 1) return launch_stream<T, CPL, 1>(g, sg);
+    if (rb == 2) return launch_stream<T, CPL, 2>(g, sg);
+    return launch_stream<T, 4, 4>(g, sg);                     // (64 rows of the wider strips do not fit the registers)
 }
 
 template <typename T>
-static int launch_stream_width(const GroupedArgs& g, const AdapterTerm* term) {
-    const long long used = g.gr.groups < g.gr.rows ? g.gr.groups : g.gr.rows;        // groups that have a row, at most
-    const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    if (used * ((g.n + 127) / 128) * 4 >= cus * 3) return launch_stream_rows<T, 8>(g, term);
-    if (used * ((g.n + 63) / 64) * 4 >= cus * 3) return launch_stream_rows<T, 4>(g, term);
-    return launch_stream_rows<T, 2>(g, term);
+static int launch_stream_t(const GroupedArgs& g, int dtype) {
+    StreamGrid sg{(g.n + 127) / 128, 1, nullptr};
+    // a second launch is worth its 4 us from about 2048 of k on (us, one weight of n = 4096 and one row, 64-column strips and shares of k: k = 1024 8.2 / 11.2, 4096 19.2 / 12.1)
+    const int want = g.k < 2048 ? 1 : stream16_splits(g, 16 << 20);
+    if (want == 1) {
+        const long long used = g.gr.groups < g.gr.rows ? g.gr.groups : g.gr.rows;
+        const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+        return used * sg.pieces * 4 >= cus * 3ll ? launch_stream_rows<T, 8>(g, sg) : launch_stream_rows<T, 4>(g, sg);
+    }
+    // Memory for the shares' sums that no other stream's call can touch: the null stream's own, or a block that stays with the graph being recorded.
+    const size_t bytes = (size_t)want * g.gr.rows * g.n * sizeof(float);
+    NullStreamScratch lease(bytes);
+    void* block = nullptr;
+    if (!lease.ptr && stream_is_capturing() && rp_hip_malloc(&block, bytes) != 0) return -1;
+    sg.partials = (float*)(lease.ptr ? lease.ptr : block);
+    if (!sg.partials) return launch_stream_rows<T, 4>(g, sg);
+    sg.nsplit = want;
+    int rc = launch_stream_rows<T, 8>(g, sg);
+    if (rc == 0) rc = launch_stream16_combine(g, sg, nullptr, dtype);
+    if (block) rp_hip_free(block);
+    return rc;
 }
 
 bool grouped_stream16_takes(const GroupedArgs& g) {
     if (path_disabled("stream16") || path_disabled("mfma")) return false;
     if (g.a_cs != 1 || g.b_cs != 1 || g.k % 8 || g.n % 8 || g.a_rs % 8 || g.b_rs % 8 || g.b_ws % 8 || g.c_rs % 8) return false;
     if (((uintptr_t)g.A | (uintptr_t)g.B | (uintptr_t)g.C | (uintptr_t)g.bias) & 15) return false;
-    if (g.b_rs < g.n || (long long)(g.k + 2 * GS_WAVES * GS_ROUND + 64) * g.b_rs * 2 >= (1ll << 31) || (64 * g.a_rs + g.k) * 2 >= (1ll << 31)) return false;      // 32-bit offsets
+    if (g.b_rs < g.n || g.b_rs >= (1ll << 22) || g.a_rs >= (1ll << 22)) return false;      // 32-bit offsets within a round
     return g.gr.rows / g.gr.groups <= 48;
 }
 
-int launch_grouped_stream16(const GroupedArgs& g, const AdapterTerm* term, int dtype) {
-    return dtype == RP_DTYPE_BFLOAT16 ? launch_stream_width<bf16_t>(g, term) : launch_stream_width<f16_t>(g, term);
-}
+int launch_grouped_stream16(const GroupedArgs& g, int dtype) { return dtype == RP_DTYPE_BFLOAT16 ? launch_stream_t<bf16_t>(g, dtype) : launch_stream_t<f16_t>(g, dtype); }
 
 }  // namespace rp
