@@ -34,6 +34,20 @@ template <> struct sh_ops<f16_t> {
     }
 };
 
+// eight float32 values as two of T each: the nearest, and the nearest to what is left (nothing, where the first overflows)
+template <typename T>
+__device__ __forceinline__ void split_low(const float* v, u32x4_t& hi, u32x4_t& lo) {
+    T h[8], l[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        h[e] = round_to<T>(v[e]);
+        const float left = v[e] - widen(h[e]);
+        l[e] = round_to<T>(__builtin_isfinite(left) ? left : 0.f);
+    }
+    __builtin_memcpy(&hi, h, 16);
+    __builtin_memcpy(&lo, l, 16);
+}
+
 // eight consecutive 16-bit values at p, of which the first n are there
 __device__ __forceinline__ u32x4_t load8(const uint16_t* p, int n) {
     if (n >= 8) return *(const u32x4_odd_t*)p;

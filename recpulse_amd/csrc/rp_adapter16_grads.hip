@@ -1,0 +1,156 @@
+// bf16 / fp16 gradients of an adapter's factors: D_a = sum over the rows i of adapter a of low[i]^T . s[i], low [rows, rank] in float32, s [rows, width].
+// With low = h and s = dy this is dB_a [rank, n]; with low = u and s = x it is dA_a^T, stored transposed.
+//
+// Bound by reading s, once per 32 of the rank: a workgroup owns one adapter, a strip of 128 columns of s and up to 32 of the rank, and its eight
+// waves share the rows of the adapter's segments, 32 at a time in turn.  s goes from memory to registers to v_mfma_f32_16x16x32 as a
+// weight does in the kernel for few rows (rp_grouped_stream16.h): a lane transposes 8 rows x 8 columns with byte permutes.  low is
+// rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, and values beyond 65504 overflow), a product each: h and u are
+// sums in float32, and one rounding of theirs would be as large as the result's own.
+#include "rp_adapter16.h"
+#include "rp_grouped_stream16.h"
+
+namespace rp {
+
+constexpr int AG_COLS = 128, AG_PITCH = AG_COLS + 4;
+
+// NC: 16-row tiles of the rank; RAGGED: rows of s that are no whole 16-byte vectors, or start anywhere
+template <typename T, int NC, bool TRANSPOSED, bool RAGGED>
+__global__ void __launch_bounds__(GS_THREADS) adapter_grad16_kernel(T* out, const uint16_t* s, const float* low, RowGroups gr, int width, int rank, long long s_rs, long long out_ws, long long out_rs,
+                                                                    int accumulate, int strips, int rank_blocks) {
+    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [GS_WAVES][16][AG_PITCH]
+    const int strip = (int)(blockIdx.x % strips), rb = (int)(blockIdx.x / strips % rank_blocks), w = (int)(blockIdx.x / strips / rank_blocks);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
+    const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
+    const uint16_t* S = s + n0;
+    uint32_t s_off[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) s_off[e] = n0 + 8 * j < width ? (uint32_t)(((8 * q + e) * s_rs + 8 * j) * 2) : BUFFER_OOB;
+    constexpr int SLOTS = 2;
+    u32x4_t raw[SLOTS][8];
+    float lv[SLOTS][NC][8];
+    int end = 0;                                              // of the segment in hand
+    auto request = [&](auto slotc, int row0) {
+        constexpr int SL = decltype(slotc)::value;
+        if constexpr (RAGGED) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int row = row0 + 8 * q + e;
+                raw[SL][e] = load8(S + (long long)row * s_rs + 8 * j, row < end ? width - n0 - 8 * j : 0);
+            }
+        } else {                                              // (rows past the segment are another's: the descriptor ends with it)
+            const char* at = (const char*)(S + (long long)row0 * s_rs);
+            const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width - n0) * 2 : 0);
+#pragma unroll
+            for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
+        }
+        const float* l = low + (long long)row0 * rank;
+        const __amdgpu_buffer_rsrc_t l_rsrc = buffer_rsrc(l, row0 < end ? (long long)(end - row0) * rank * 4 : 0);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = r0 + 16 * c + j;
+                lv[SL][c][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(l_rsrc, r < rank ? ((8 * q + e) * rank + r) * 4 : (int)BUFFER_OOB, 0, 0));
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x4_t acc[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](auto slotc) {
+        constexpr int SL = decltype(slotc)::value;
+        u32x4_t hi[NC], lo[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) split_low<T>(lv[SL][c], hi[c], lo[c]);
+#pragma unroll
+        for (int f = 0; f < 8; f++) {
+            u32x4_t b;
+#pragma unroll
+            for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[SL][2 * d + 1][f / 2], raw[SL][2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                acc[c][f] = gs_ops<T>::mma(hi[c], b, acc[c][f]);
+                acc[c][f] = gs_ops<T>::mma(lo[c], b, acc[c][f]);
+            }
+        }
+    };
+    int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
+    for (int g = 0; g < gr.groups; g++) {
+        if (gr.weight(g) != w) continue;
+        const int b = gr.begin(g);
+        end = gr.end(g);
+        constexpr int turn = GS_WAVES * GS_ROUND;
+        const int first = b + ((wave - rounds) & (GS_WAVES - 1)) * GS_ROUND;
+        rounds += (end - b + GS_ROUND - 1) / GS_ROUND;
+        if (first >= end) continue;
+        static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
+        for (int row0 = first; row0 < end; row0 += SLOTS * turn)
+            static_for<0, SLOTS>([&](auto sc) {
+                multiply(sc);
+                request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
+            });
+    }
+    static_for<0, NC>([&](auto cc) {
+        constexpr int c = decltype(cc)::value;
+        if (c) __syncthreads();
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = acc[c][f][v];
+        __syncthreads();
+        // four outputs a thread, neighbours along the output's rows
+#pragma unroll
+        for (int o = 0; o < 4; o++) {
+            const int id = threadIdx.x + o * GS_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
+            if (r0 + 16 * c + r >= rank || n0 + col >= width) continue;
+            float t = gs_sums[r * AG_PITCH + col];
+#pragma unroll
+            for (int p = 1; p < GS_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
+            T* at = out + w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
+            T y = round_to<T>(t);
+            if (accumulate) y = round_to<T>(widen(*at) + widen(y));
+            *at = y;
+        }
+    });
+}
+
+template <typename T, int NC, bool TRANSPOSED>
+static int launch_grad(const GroupedArgs& g) {
+    const int width = TRANSPOSED ? g.k : g.n, rank = TRANSPOSED ? g.n : g.k;
+    const void* s = TRANSPOSED ? g.A : g.B;
+    const float* low = (const float*)(TRANSPOSED ? g.B : g.A);
+    const long long s_rs = TRANSPOSED ? g.a_rs : g.b_rs;
+    const int strips = (width + AG_COLS - 1) / AG_COLS, rank_blocks = (rank + 16 * NC - 1) / (16 * NC);
+    const long long blocks = (long long)strips * rank_blocks * g.gr.weights;
+    if (blocks > 0x7fffffffll) { set_error("adapter gradient: %lld tiles are more than a launch takes", blocks); return -1; }
+    constexpr int lds = GS_WAVES * 16 * AG_PITCH * 4;
+    auto launch = [&](auto kern) {
+        if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
+        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), (T*)g.C, (const uint16_t*)s, low, g.gr, width, rank, s_rs, g.c_ws, g.c_rs, g.accumulate, strips, rank_blocks);
+        return check_launch("adapter_grad16_kernel") ? 0 : -1;
+    };
+    const bool ragged = width % 8 || s_rs % 8 || ((uintptr_t)s & 15);
+    return ragged ? launch(adapter_grad16_kernel<T, NC, TRANSPOSED, true>) : launch(adapter_grad16_kernel<T, NC, TRANSPOSED, false>);
+}
+
+template <typename T>
+static int launch_grad_shape(const GroupedArgs& g, bool transposed) {
+    const int rank = transposed ? g.n : g.k;
+    if (rank <= 16) return transposed ? launch_grad<T, 1, true>(g) : launch_grad<T, 1, false>(g);
+    return transposed ? launch_grad<T, 2, true>(g) : launch_grad<T, 2, false>(g);
+}
+
+bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
+    const bool transposed = low == LOW_B;
+    const long long s_rs = transposed ? g.a_rs : g.b_rs, s_cs = transposed ? g.a_cs : g.b_cs, l_rs = transposed ? g.b_rs : g.a_rs, l_cs = transposed ? g.b_cs : g.a_cs;
+    const int width = transposed ? g.k : g.n, rank = transposed ? g.n : g.k;
+    return s_cs == 1 && s_rs >= width && s_rs < (1ll << 22) && l_rs == rank && (l_cs == 1 || rank == 1) && rank < (1 << 20) && !path_disabled("mfma");
+}
+
+int launch_adapter_grad16(const GroupedArgs& g, GroupedLow low, int dtype) {
+    return dtype == RP_DTYPE_BFLOAT16 ? launch_grad_shape<bf16_t>(g, low == LOW_B) : launch_grad_shape<f16_t>(g, low == LOW_B);
+}
+
+}  // namespace rp

@@ -59,6 +59,9 @@ int launch_stream16_combine(const GroupedArgs& g, const StreamGrid& sg, const Ad
 // h[i] = scales[a] x[i] . a_a in float32 for bf16 / fp16 operands (rp_adapter16.hip); C is h
 bool adapter_shrink16_takes(const GroupedArgs& g);
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype);
+// the gradients of an adapter's factors (rp_adapter16_grads.hip): by weights, LOW_A (dB) or LOW_B (dA)
+bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low);
+int launch_adapter_grad16(const GroupedArgs& g, GroupedLow low, int dtype);
 // The whole layer for a few rows: `shared` one group of all rows, `low` the product above, `term` what it adds
 bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term);
 int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype);

@@ -40,6 +40,7 @@ static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
 }
 
 static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
+    if (is16(dtype) && (low == LOW_A || low == LOW_B) && adapter_grad16_takes(g, low)) return launch_adapter_grad16(g, low, dtype);
     if (is16(dtype) && low == LOW_NONE && !g.gr.ids && g.a_cs == 1 && g.b_cs == 1 && !path_disabled("mfma")) {
         const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
         const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
