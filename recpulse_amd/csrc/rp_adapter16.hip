@@ -98,4 +98,91 @@ int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low,
     return rc;
 }
 
+// ---- the term by itself: y[i] += h[i] . b_a, where the shared product is too small for tiles that would fill the CUs ----
+// 16 rows of a segment and 2048 columns a workgroup, 8 columns a thread: b is read once for the 16 rows, h through the scalar cache.
+template <typename T, bool ALONG_RANK>
+__global__ void __launch_bounds__(256) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int parts) {
+    const RowTile rt = find_row_tile(term.gr, 16, (int)(blockIdx.x / parts));
+    if (rt.group < 0) return;
+    const int col = (int)(blockIdx.x % parts) * 2048 + threadIdx.x * 8, m = rt.end - rt.begin, there = n - col;
+    if (there <= 0) return;
+    const float* h = term.h + (long long)rt.begin * term.rank;
+    const uint16_t* b = (const uint16_t*)term.b + rt.weight * term.b_ws + (long long)col * term.b_cs;
+    float acc[16][8];
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+#pragma unroll
+        for (int v = 0; v < 8; v++) acc[i][v] = 0.f;
+    auto multiply = [&](const T (&bv)[8], int r) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if (i < m) {                                                  // (uniform)
+                const float hr = h[(long long)i * term.rank + r];
+#pragma unroll
+                for (int v = 0; v < 8; v++) acc[i][v] += hr * widen(bv[v]);
+            }
+        }
+    };
+    if constexpr (ALONG_RANK) {
+        for (int r0 = 0; r0 < term.rank; r0 += 8) {
+            T cols[8][8], bv[8];
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                const u32x4_t x = load8(b + (v < there ? v : 0) * term.b_cs + r0, term.rank - r0);
+                __builtin_memcpy(cols[v], &x, 16);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                if (r0 + u < term.rank) {
+#pragma unroll
+                    for (int v = 0; v < 8; v++) bv[v] = cols[v][u];
+                    multiply(bv, r0 + u);
+                }
+            }
+        }
+    } else {
+        for (int r = 0; r < term.rank; r++) {
+            T bv[8];
+            const u32x4_t x = load8(b + r * term.b_rs, there);
+            __builtin_memcpy(bv, &x, 16);
+            multiply(bv, r);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        if (i >= m) continue;
+        uint16_t* p = y + (rt.begin + i) * y_rs + col;
+        T o[8];
+        const u32x4_t was = load8(p, there);
+        __builtin_memcpy(o, &was, 16);
+#pragma unroll
+        for (int v = 0; v < 8; v++) o[v] = round_to<T>(widen(o[v]) + acc[i][v]);
+        if (there >= 8) {
+            u32x4_t x;
+            __builtin_memcpy(&x, o, 16);
+            *(u32x4_odd_t*)p = x;
+        } else {
+#pragma unroll
+            for (int v = 0; v < 7; v++)
+                if (v < there) p[v] = o[v].bits;
+        }
+    }
+}
+
+bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) { return (term.b_cs == 1 || term.b_rs == 1) && !path_disabled("mfma"); }
+
+template <typename T>
+static int launch_expand(const GroupedArgs& shared, const AdapterTerm& term) {
+    const int parts = (shared.n + 2047) / 2048;
+    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups, 16) * parts;
+    if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
+    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
+    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
+    return check_launch("adapter_expand16_kernel") ? 0 : -1;
+}
+
+int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, int dtype) {
+    return dtype == RP_DTYPE_BFLOAT16 ? launch_expand<bf16_t>(shared, term) : launch_expand<f16_t>(shared, term);
+}
+
 }  // namespace rp

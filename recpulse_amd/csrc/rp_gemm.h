@@ -47,6 +47,8 @@ struct Plan {
     bool ragged = false;      // rows that are no whole number of 16-byte vectors, or start at any element (MFMA kernels)
 };
 
+void choose_tile16(Plan& p, int batch, int m, int k, int n);       // tile of the 16-bit MFMA kernel (p.a_mc, p.b_mc and p.ragged given)
+
 constexpr int SK_MAX_M = 8;           // rows the skinny kernel takes
 constexpr int SK_MAX_GROUPS = 4096;   // column groups it can track
 constexpr int M16_BK = 64;            // k slab of the 16-bit MFMA kernels

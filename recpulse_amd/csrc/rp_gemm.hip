@@ -67,7 +67,7 @@ static bool small_tiles_win(long long tiles256, long long tiles128, int m, int n
 }
 
 // Tile of the 16-bit MFMA kernel for an output of batch x m x n with reduction length k.
-static void choose_tile16(Plan& p, int batch, int m, int k, int n) {
+void choose_tile16(Plan& p, int batch, int m, int k, int n) {
     p.fam = FAM_MFMA16;
     const long long tiles256 = (long long)((m + 255) / 256) * ((n + 255) / 256) * batch;
     const long long tiles128 = (long long)((m + 127) / 128) * ((n + 127) / 128) * batch;

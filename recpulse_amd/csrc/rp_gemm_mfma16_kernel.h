@@ -175,8 +175,8 @@ typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)))
 
 // Where a workgroup's tiles come from and what else they may do.  M16Plain: the schedule of one matrix of the batch, the reference's roundings.
 // Another source (the grouped products') has `tile`, which points `args` at the matrix that slot `tile_id` belongs to and answers with the tile's
-// coordinates in it, and ONCE: the sum and the bias of its column are rounded together, to nearest even.
-struct M16Plain { static constexpr bool ONCE = false; };
+// coordinates in it, ONCE: the sum and the bias of its column are rounded together, to nearest even, and TERM: `add_term` adds to a wave's sums before that.
+struct M16Plain { static constexpr bool ONCE = false, TERM = false; };
 
 // What one workgroup does: slots first_slot, first_slot + stride, ... of the schedule of matrix z
 template <typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE, bool SPLITK, int PF, typename SRC = M16Plain>
@@ -511,6 +511,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, 
         slab_step(I0{}, nslabs, no{}, no{});
     }
 
+    if constexpr (SRC::TERM) source->template add_term<T, MT, TMI, TNI>(acc, m0 + wm0, n0 + wn0, lane);
     if constexpr (MT == 16) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the in-place MFMAs above are opaque to the compiler: let the last ones drain before their results are read
     // ---- epilogue ----
     T* C = (T*)g.C + (long long)z * g.c_bs;

@@ -52,6 +52,26 @@ static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
     return launch_grouped_weights_generic(g, low, dtype);
 }
 
+// The shared product of a layer with adapters, and the adapters' term
+static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int dtype) {
+    if (is16(dtype) && s.a_cs == 1 && (s.b_cs == 1 || s.b_rs == 1) && !path_disabled("mfma")) {
+        Plan p{FAM_MFMA16, 64, 64, false, s.b_cs == 1, true, ""};
+        const Lie lie = worse(lies(s.A, s.a_rs, 0, s.k, 2), p.b_mc ? lies(s.B, s.b_rs, 0, s.n, 2) : lies(s.B, s.b_cs, 0, s.k, 2));
+        p.ragged = lie == LIE_RAGGED;
+        choose_tile16(p, 1, s.gr.rows, s.k, s.n);
+        if (p.ragged && p.bm == 256) p.bm = p.bn = 128;
+        const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
+        // from about a tile for every other CU on, and while a tile's rows are few segments': each costs it 2 us
+        if (lie != LIE_NEITHER && p.bm == p.bn && tiles * 2 >= cus() && term.gr.rows / term.gr.groups >= 16) {
+            if (p.bm == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_tiles16_256_bf16(s, term, p.edge) : launch_adapter_tiles16_256_f16(s, term, p.edge);
+            return p.bm == 128 ? launch_adapter_tiles16_128(s, term, p.edge, p.ragged, dtype) : launch_adapter_tiles16_64(s, term, p.ragged, dtype);
+        }
+    }
+    if (rp_hip_gemm_strided_batched(s.C, s.A, s.B, s.bias, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate, dtype) != 0) return -1;
+    if (is16(dtype) && adapter_expand16_takes(s, term)) return launch_adapter_expand16(s, term, dtype);
+    return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, LOW_A, dtype);
+}
+
 static bool grouped_args_ok(const char* who, bool pointers, int groups, int rows, int k, int n, std::initializer_list<long long> strides, int dtype) {
     if (!pointers || groups <= 0 || rows <= 0 || k <= 0 || n <= 0) { set_error("%s: null operand or non-positive extent (groups=%d rows=%d k=%d n=%d)", who, groups, rows, k, n); return false; }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
@@ -104,8 +124,7 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
     const AdapterTerm term{(const float*)h, b, gr, rank, (long long)rank * n, n, 1};
     if (is16(dtype) && adapter_few_rows16_takes(shared, low, term)) return launch_adapter_few_rows16(shared, low, term, dtype);
     if (grouped_rows(low, LOW_C, dtype) != 0) return -1;
-    if (rp_hip_gemm_strided_batched(y, x, w, bias, 1, rows, k, n, 0, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 1, 0, dtype) != 0) return -1;
-    return grouped_rows(GroupedArgs{y, h, b, nullptr, nullptr, gr, rank, n, rank, 1, (long long)rank * n, n, 1, 0, y_rs, ACCUMULATE_JOINED}, LOW_A, dtype);
+    return shared_with_term(shared, term, dtype);
 }
 
 int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
@@ -119,8 +138,8 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
     const RowGroups gr{offsets, ids, segments, rows, adapters};
     if ((dx || da) && grouped_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
     if (dx) {
-        if (rp_hip_gemm_strided_batched(dx, dy, w, nullptr, 1, rows, n, k, 0, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, 1, accumulate_dx, dtype) != 0) return -1;
-        if (grouped_rows(GroupedArgs{dx, u, a, nullptr, nullptr, gr, rank, k, rank, 1, (long long)k * rank, 1, rank, 0, dx_rs, ACCUMULATE_JOINED}, LOW_A, dtype) != 0) return -1;
+        const GroupedArgs shared{dx, dy, w, nullptr, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, n, k, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
+        if (shared_with_term(shared, AdapterTerm{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank}, dtype) != 0) return -1;
     }
     if (da && grouped_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0}, LOW_B, dtype) != 0) return -1;
     if (db && grouped_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, LOW_A, dtype) != 0) return -1;
