@@ -1,26 +1,44 @@
 // bf16 / fp16 shared projection with its rows' adapters, y[i] = x[i] . w + bias + h[i] . b_a, on the tiles of the 16-bit MFMA kernel: the adapters'
-// term goes into a tile's accumulators between its last slab and its one rounding, so y is written once and never read.
+// term is what a tile's accumulators start from, so y is rounded once, written once and never read.
 //
-// A wave adds the term of every segment that has rows in its patch: rank / 32 (or / 16) more k-steps with the other segments' rows zero.  h is
-// float32 and is multiplied as two values of the tensors' type (split_low).  b comes straight from memory, 16 bytes a lane where it is
-// contiguous along the rank (a_a^T, for dx) and else eight 2-byte loads: some 2 us a segment on a tile that takes 50 at k = 4096.
+// For every segment that has rows in a wave's patch: rank / 32 (/ 16) k-steps of MFMAs, the other segments' rows zero.  h is float32 and is
+// multiplied as two values of the tensors' type (split_low).  b comes straight from memory, 16 bytes a lane where it is contiguous along
+// the rank (a_a^T, for dx) and else in 2-byte loads.  4096 x 4096 x 4096 with seven segments in bf16: 122 us at rank 16 and 132 at rank 32, beside 103 for the product
+// alone and 18 and more for a pass over y.
+// (Between the last slab and the epilogue the same code takes registers from the main loop of the 256 x 256 tile: a value or two reloaded
+// from memory a slab, behind which all of its loads are waited for; 130.  In the epilogue, into registers of its own 16 rows at a
+// time, it is unrolled eightfold and waits for its instructions: 134.)
 #pragma once
 #include "rp_adapter16.h"
 #include "rp_gemm_mfma16_kernel.h"
 
 namespace rp {
 
-struct AdapterTiles {
-    static constexpr bool ONCE = true, TERM = true;
+struct AdapterTileArgs {
+    GemmArgs g;
+    int tiles_m, tiles_n, total;
     AdapterTerm term;
-    int tiles_m, tiles_n, m, n;
-    __device__ __forceinline__ TileCoord tile(int id, GemmArgs&) const { return schedule_tile(id, tiles_m, tiles_n); }
+};
 
-    template <typename T, int MT, int TMI, int TNI, typename ACC>
-    __device__ __forceinline__ void add_term(ACC (&acc)[TMI][TNI], int row0, int col0, int lane) const {
+struct AdapterTiles {
+    static constexpr bool MOVES = false, ONCE = true, TERM = true;
+
+    // acc: the sums of the calling wave's patch of the tile at (m0, n0), waves WGN to a row of patches
+    template <typename T, int MT, int WGN, int TMI, int TNI, typename ACC>
+    __device__ __forceinline__ void add_term(ACC (&acc)[TMI][TNI], int m0, int n0) const {
         constexpr int KSTEP = MT == 32 ? 16 : 32;
+        // The term's arguments are read here, from where the launch left them, and the lane's numbers are made anew: kept for the next tile they
+        // would take registers that the main loop needs.
+        typedef const __attribute__((address_space(4))) AdapterTileArgs* args_t;       // (constant memory: scalar loads)
+        args_t args = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+        unsigned t = threadIdx.x;
+        asm volatile("" : "+s"(args), "+v"(t));
+        const RowGroups gr{args->term.gr.offsets, args->term.gr.ids, args->term.gr.groups, args->term.gr.rows, args->term.gr.weights};
+        const AdapterTerm term{args->term.h, args->term.b, gr, args->term.rank, args->term.b_ws, args->term.b_rs, args->term.b_cs};
+        const int m = args->g.m, n = args->g.n;
+        const int lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), fr = lane % MT, oct = lane / MT;
+        const int row0 = m0 + wave / WGN * (TMI * MT), col0 = n0 + wave % WGN * (TNI * MT), row_end = row0 + TMI * MT < m ? row0 + TMI * MT : m;
         const bool whole = term.rank % 4 == 0 && ((uintptr_t)term.h & 15) == 0;
-        const int fr = lane % MT, oct = lane / MT, row_end = row0 + TMI * MT < m ? row0 + TMI * MT : m;
         for (int g0 = 0; g0 < term.gr.groups; g0 += 64) {
             int b = 0, e = 0, w = -1;
             if (g0 + lane < term.gr.groups) { b = term.gr.begin(g0 + lane); e = term.gr.end(g0 + lane); w = term.gr.weight(g0 + lane); }
@@ -32,53 +50,69 @@ struct AdapterTiles {
                 const uint16_t* bp = (const uint16_t*)term.b + a * term.b_ws;
                 for (int k0 = 0; k0 < term.rank; k0 += KSTEP) {
                     const int kk = k0 + 8 * oct, left = term.rank - kk;
-                    s16x8_t hi[TMI], lo[TMI];
+                    // All loads first, and none behind a branch (out of range they read zeros): one round trip for them together.
+                    const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc(bp, ((long long)(term.rank - 1) * term.b_rs + (long long)(n - 1) * term.b_cs + 1) * 2);
+                    const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)sb * term.rank, (long long)(se - sb) * term.rank * 4);
+                    s16x8_t bf[TNI];
+                    float hv[TMI][8];
 #pragma unroll
                     for (int i = 0; i < TMI; i++) {
-                        const int row = row0 + i * MT + fr;
-                        float v[8];
-                        const float* h = term.h + (long long)row * term.rank + kk;
-                        const bool in = row >= sb && row < se;
+                        const uint32_t at = (uint32_t)(((row0 + i * MT + fr - sb) * term.rank + kk) * 4);      // (rows before the segment wrap around, out of range)
                         if (whole) {
-                            const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-                            const f32x4_t p = in && left > 0 ? *(const f32x4_t*)h : zero, r = in && left > 4 ? *(const f32x4_t*)(h + 4) : zero;
+                            const u32x4_t p = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 0 ? at : BUFFER_OOB), 0, 0);
+                            const u32x4_t q = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 4 ? at + 16 : BUFFER_OOB), 0, 0);
 #pragma unroll
-                            for (int u = 0; u < 4; u++) { v[u] = p[u]; v[4 + u] = r[u]; }
+                            for (int u = 0; u < 4; u++) { hv[i][u] = __uint_as_float(p[u]); hv[i][4 + u] = __uint_as_float(q[u]); }
                         } else {
 #pragma unroll
-                            for (int u = 0; u < 8; u++) v[u] = in && u < left ? h[u] : 0.f;
+                            for (int u = 0; u < 8; u++) hv[i][u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(u < left ? at + 4 * u : BUFFER_OOB), 0, 0));
                         }
-                        u32x4_t hv, lv;
-                        split_low<T>(v, hv, lv);
-                        hi[i] = __builtin_bit_cast(s16x8_t, hv);
-                        lo[i] = __builtin_bit_cast(s16x8_t, lv);
                     }
-                    static_for<0, TNI>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value;
-                        const int col = col0 + j * MT + fr;
-                        s16x8_t bf = {0, 0, 0, 0, 0, 0, 0, 0};
-                        if (col < n) {
-                            const uint16_t* p = bp + (long long)kk * term.b_rs + (long long)col * term.b_cs;
-                            if (term.b_rs == 1) bf = __builtin_bit_cast(s16x8_t, load8(p, left));
-                            else {
+                    if (term.b_rs == 1) {                     // (values past the rank are another column's: made zeros)
 #pragma unroll
-                                for (int u = 0; u < 8; u++) bf[u] = u < left ? (short)p[u * term.b_rs] : (short)0;
-                            }
-                        }
-                        // (the in-place MFMAs are opaque to the compiler: what vector instructions wrote for them has to be there)
-                        if constexpr (MT == 16) {
-                            __builtin_amdgcn_sched_barrier(0);
-                            asm volatile("s_nop 7" : "+v"(bf) : : "memory");
-                            if constexpr (j == 0) {
+                        for (int j = 0; j < TNI; j++) {
+                            const int col = col0 + j * MT + fr;
+                            u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col < n && left > 0 ? (uint32_t)((col * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0);
 #pragma unroll
-                                for (int i = 0; i < TMI; i++) asm volatile("s_nop 7" : "+v"(hi[i]), "+v"(lo[i]) : : "memory");
-                            }
+                            for (int d = 0; d < 4; d++) x[d] &= left > 2 * d + 1 ? 0xFFFFFFFFu : left > 2 * d ? 0xFFFFu : 0u;
+                            bf[j] = __builtin_bit_cast(s16x8_t, x);
                         }
-                        static_for<0, TMI>([&](auto ic) {
-                            constexpr int i = decltype(ic)::value;
-                            if (row0 + i * MT >= se || row0 + (i + 1) * MT <= sb) return;
-                            acc[i][j] = mfma16_ops<T>::mma(hi[i], bf, acc[i][j]);
-                            acc[i][j] = mfma16_ops<T>::mma(lo[i], bf, acc[i][j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < TNI; j++) {
+                            const int col = col0 + j * MT + fr;
+                            const uint32_t at = (uint32_t)((kk * term.b_rs + col) * 2), step = (uint32_t)(term.b_rs * 2);
+                            uint32_t x[8];
+#pragma unroll
+                            for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col < n && u < left ? at + u * step : BUFFER_OOB), 0, 0);
+                            u32x4_t y;
+#pragma unroll
+                            for (int d = 0; d < 4; d++) y[d] = x[2 * d] | x[2 * d + 1] << 16;
+                            bf[j] = __builtin_bit_cast(s16x8_t, y);
+                        }
+                    }
+                    u32x4_t hi[TMI], lo[TMI];
+#pragma unroll
+                    for (int i = 0; i < TMI; i++) split_low<T>(hv[i], hi[i], lo[i]);
+                    // (the in-place MFMAs are opaque to the compiler: what vector instructions wrote for them has to be there)
+                    if constexpr (MT == 16) {
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int j = 0; j < TNI; j++) asm volatile("" : "+v"(bf[j]) : : "memory");
+#pragma unroll
+                        for (int i = 0; i < TMI; i++) asm volatile("" : "+v"(hi[i]), "+v"(lo[i]) : : "memory");
+                        asm volatile("s_nop 15" ::: "memory");
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    static_for<0, TMI>([&](auto ic) {
+                        constexpr int i = decltype(ic)::value;
+                        static_for<0, TNI>([&](auto jc) {
+                            constexpr int j = decltype(jc)::value;
+                            acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, hi[i]), bf[j], acc[i][j]);
+                        });
+                        static_for<0, TNI>([&](auto jc) {
+                            constexpr int j = decltype(jc)::value;
+                            acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, lo[i]), bf[j], acc[i][j]);
                         });
                     });
                 }
@@ -88,10 +122,11 @@ struct AdapterTiles {
 };
 
 template <typename T, int BM, int BN, int WGM, bool B_MC, int EDGE>
-__global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) adapter_tiles16_kernel(GemmArgs args, AdapterTerm term, int tiles_m, int tiles_n, int total) {
-    AdapterTiles source{term, tiles_m, tiles_n, args.m, args.n};
-    GemmArgs g = args;
-    gemm_mfma16_block<T, BM, BN, WGM, false, B_MC, EDGE, false, 1, AdapterTiles>(g, 0, 0, nullptr, 0, total, (int)blockIdx.x, 0, (int)gridDim.x, &source);
+__global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) adapter_tiles16_kernel(AdapterTileArgs args) {
+    AdapterTiles source;
+    // (one plain matrix: the options that GemmArgs has beside are known to be unused here)
+    const GemmArgs g{args.g.C, args.g.A, args.g.B, args.g.bias, 1, args.g.m, args.g.k, args.g.n, 0, args.g.a_rs, 1, 0, B_MC ? args.g.b_rs : 1, B_MC ? 1 : args.g.b_cs, 0, args.g.c_rs, 1, args.g.accumulate};
+    gemm_mfma16_block<T, BM, BN, WGM, false, B_MC, EDGE, false, 1, AdapterTiles>(g, args.tiles_m, args.tiles_n, nullptr, 0, args.total, (int)blockIdx.x, 0, (int)gridDim.x, &source);
 }
 
 template <typename T, int BM, int BN, int WGM, bool B_MC, int EDGE>
@@ -103,7 +138,7 @@ static int launch_adapter_tiles16(const GroupedArgs& s, const AdapterTerm& term)
     const int blocks = BM == 256 && BN == 256 && cus >= 8 && total > cus ? cus : total;      // one resident workgroup a CU, as for a product of its own
     auto kern = adapter_tiles16_kernel<T, BM, BN, WGM, B_MC, EDGE>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), smem, current_stream(), g, term, tiles_m, tiles_n, total);
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), smem, current_stream(), AdapterTileArgs{g, tiles_m, tiles_n, total, term});
     return check_launch("adapter_tiles16_kernel") ? 0 : -1;
 }
 

@@ -174,13 +174,14 @@ __device__ __forceinline__ u32x4_t m16_pull_shift(u32x4_t v, int pull) {
 typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));       // a 16-byte vector at any element
 
 // Where a workgroup's tiles come from and what else they may do.  M16Plain: the schedule of one matrix of the batch, the reference's roundings.
-// Another source (the grouped products') has `tile`, which points `args` at the matrix that slot `tile_id` belongs to and answers with the tile's
-// coordinates in it, ONCE: the sum and the bias of its column are rounded together, to nearest even, and TERM: `add_term` adds to a wave's sums before that.
-struct M16Plain { static constexpr bool ONCE = false, TERM = false; };
+// Another source may have MOVES: its `tile` points `g` at the matrix that slot `tile_id` belongs to and answers with the tile's
+// coordinates in it; ONCE: the sum and the bias of its column are rounded together, to nearest even; TERM: `add_term` gives a wave's sums
+// what they start from.
+struct M16Plain { static constexpr bool MOVES = false, ONCE = false, TERM = false; };
 
 // What one workgroup does: slots first_slot, first_slot + stride, ... of the schedule of matrix z
 template <typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE, bool SPLITK, int PF, typename SRC = M16Plain>
-__device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, GemmArgs, const GemmArgs>& g, int tiles_m, int tiles_n, float* partials, int k_per_split, int sched_total, int first_slot, int z, int stride, SRC* source = nullptr) {
+__device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES, GemmArgs, const GemmArgs>& g, int tiles_m, int tiles_n, float* partials, int k_per_split, int sched_total, int first_slot, int z, int stride, SRC* source = nullptr) {
     constexpr int WGN = 4 / WGM;
     constexpr int WM = BM / WGM, WN = BN / WGN;       // wave patch
     constexpr int MT = SPLITK ? 32 : m16_mfma_tile(BM, BN);      // MFMA tile edge; k-steps of 16 (MT 32) or 32 (MT 16)
@@ -206,7 +207,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, 
     // multiple of 8 keeps a workgroup's tiles on the XCD the schedule assigned them to.
     for (int tile_id = first_slot; tile_id < sched_total; tile_id += stride) {
     TileCoord tc;
-    if constexpr (SRC::ONCE) tc = source->tile(tile_id, g);
+    if constexpr (SRC::MOVES) tc = source->tile(tile_id, g);
     else tc = schedule_tile(tile_id, tiles_m, tiles_n);
     if (!tc.valid) continue;
     const int m0 = tc.tm * BM, n0 = tc.tn * BN;
@@ -373,6 +374,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, 
         a_slab += a_step;
         advance_b();
     };
+    if constexpr (SRC::TERM) source->template add_term<T, MT, WGN, TMI, TNI>(acc, m0, n0);
     static_for<0, PF>([&](auto setc) { load_slab(setc, decltype(setc)::value); });
     if (tile_id != first_slot) __syncthreads();            // the previous tile's epilogue has read its staged rows out of LDS
     if (EDGE == M16_RAGGED && nslabs == 1) pull_into_place(I0{});
@@ -511,7 +513,6 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::ONCE, 
         slab_step(I0{}, nslabs, no{}, no{});
     }
 
-    if constexpr (SRC::TERM) source->template add_term<T, MT, TMI, TNI>(acc, m0 + wm0, n0 + wn0, lane);
     if constexpr (MT == 16) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the in-place MFMAs above are opaque to the compiler: let the last ones drain before their results are read
     // ---- epilogue ----
     T* C = (T*)g.C + (long long)z * g.c_bs;

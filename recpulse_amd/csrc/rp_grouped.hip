@@ -62,7 +62,7 @@ static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int d
         if (p.ragged && p.bm == 256) p.bm = p.bn = 128;
         const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
         // from about a tile for every other CU on, and while a tile's rows are few segments': each costs it 2 us
-        if (lie != LIE_NEITHER && p.bm == p.bn && tiles * 2 >= cus() && term.gr.rows / term.gr.groups >= 16) {
+        if (lie != LIE_NEITHER && p.bm == p.bn && !path_disabled("adapter_tiles") && tiles * 2 >= cus() && term.gr.rows / term.gr.groups >= 16) {
             if (p.bm == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_tiles16_256_bf16(s, term, p.edge) : launch_adapter_tiles16_256_f16(s, term, p.edge);
             return p.bm == 128 ? launch_adapter_tiles16_128(s, term, p.edge, p.ragged, dtype) : launch_adapter_tiles16_64(s, term, p.ragged, dtype);
         }

@@ -10,7 +10,7 @@ namespace rp {
 // as if they were one matrix's, so that an XCD's workgroups share a few row panels and a few weight panels at a time.
 template <int BM>
 struct GroupedRowTiles {
-    static constexpr bool ONCE = true, TERM = false;
+    static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     RowTiles rows;
     int tiles_n;
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) group
 // By weights: tile for tile the same in every group, so that resident workgroups, each with one tile of every group in turn, all do the
 // same work however uneven the groups are.  The reduction runs over the group's rows; an empty group leaves zeros.
 struct GroupedWeightTiles {
-    static constexpr bool ONCE = true, TERM = false;
+    static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     int tiles_k, tiles_n, slots;
     __device__ __forceinline__ TileCoord tile(int id, GemmArgs& g) const {
