@@ -31,6 +31,12 @@ int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dty
 int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype);
 
 
+// fp32 / fp64 (rp_grouped_wavek.hip), rows of any length and start
+bool grouped_rows_wavek_takes(const GroupedArgs& g, int dtype);
+bool grouped_weights_wavek_takes(const GroupedArgs& g, int dtype);
+int launch_grouped_rows_wavek(const GroupedArgs& g, int dtype);
+int launch_grouped_weights_wavek(const GroupedArgs& g, int dtype);
+
 // bf16 / fp16 on the tiles of the 16-bit MFMA kernel (rp_grouped_mfma16*.hip).  ragged: rows of any length and start.
 int launch_grouped_rows16_256_bf16(const GroupedArgs& g);
 int launch_grouped_rows16_256_f16(const GroupedArgs& g);

@@ -36,6 +36,8 @@ static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
         if (lie != LIE_NEITHER)
             return mean >= 96 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_rows16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_rows16_64(g, lie == LIE_RAGGED, dtype);
     }
+    // (h and u of fp32 and fp64 tensors are of their type: any of the operands may be low; the scale of h is the generic kernel's)
+    if (!is16(dtype) && !g.scales && g.accumulate != ACCUMULATE_JOINED && grouped_rows_wavek_takes(g, dtype)) return launch_grouped_rows_wavek(g, dtype);
     return launch_grouped_rows_generic(g, low, dtype);
 }
 
@@ -49,6 +51,7 @@ static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
         if (lie != LIE_NEITHER)
             return g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_weights16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_weights16_64(g, lie == LIE_RAGGED, dtype);
     }
+    if (!is16(dtype) && grouped_weights_wavek_takes(g, dtype)) return launch_grouped_weights_wavek(g, dtype);
     return launch_grouped_weights_generic(g, low, dtype);
 }
 
