@@ -1,0 +1,105 @@
+// An adapter's narrow products and the gradients of its factors for fp32, fp64 and operands of any strides, on scalar multiply-adds in the accumulate type.
+//
+// h[i] = scale x[i] . A_a has rank outputs a row and k products each: 64 x 64 tiles of it would leave most CUs without one and each with a long chain.
+// Here a workgroup owns eight rows and sixteen of the rank, and its sixteen groups of sixteen lanes share k.
+// dB_a = sum of h[i]^T dy[i] (and dA_a^T = sum of u[i]^T x[i]): a workgroup owns 64 columns and sixteen of the rank, a column a lane, and its four waves share the
+// rows; the row's sixteen low values are uniform, one scalar load.
+// fp32, 2048 rows of 4096, rank 16, us, on 64 x 64 tiles and here: ANY_FIGURES
+#include "rp_grouped.h"
+
+#include <type_traits>
+
+namespace rp {
+
+constexpr int NR_ROWS = 8, NR_COLS = 16, NR_LANES = 16;          // rows and columns of a workgroup, lanes that share k
+
+template <typename T>
+__global__ void __launch_bounds__(NR_COLS * NR_LANES) narrow_rows_kernel(GroupedArgs g, int col_blocks) {
+    using A = typename traits<T>::acc;
+    __shared__ A sums[NR_LANES][NR_ROWS][NR_COLS + 1];
+    const RowTile rt = find_row_tile(g.gr, NR_ROWS, (int)(blockIdx.x / col_blocks));
+    if (rt.group < 0) return;
+    const int c = threadIdx.x % NR_COLS, p = threadIdx.x / NR_COLS, col = (int)(blockIdx.x % col_blocks) * NR_COLS + c, last = rt.end - rt.begin - 1;
+    const T* x = (const T*)g.A + rt.begin * g.a_rs;
+    const T* f = (const T*)g.B + rt.weight * g.b_ws + (col < g.n ? col : g.n - 1) * g.b_cs;
+    A acc[NR_ROWS];
+#pragma unroll
+    for (int r = 0; r < NR_ROWS; r++) acc[r] = 0;
+#pragma unroll 4
+    for (int k = p; k < g.k; k += NR_LANES) {
+        const A fv = widen(f[k * g.b_rs]);
+#pragma unroll
+        for (int r = 0; r < NR_ROWS; r++) acc[r] += widen(x[(r < last ? r : last) * g.a_rs + k * g.a_cs]) * fv;       // (rows past the segment repeat its last and are not stored)
+    }
+#pragma unroll
+    for (int r = 0; r < NR_ROWS; r++) sums[p][r][c] = acc[r];
+    __syncthreads();
+    const int r = threadIdx.x / NR_COLS;
+    if (r >= NR_ROWS || r > last || col >= g.n) return;
+    A s = sums[0][r][c];
+#pragma unroll
+    for (int q = 1; q < NR_LANES; q++) s += sums[q][r][c];
+    ((A*)g.C)[(rt.begin + r) * g.c_rs + col] = g.scales ? (A)g.scales[rt.weight] * s : s;
+}
+
+// TRANSPOSED: dA; else dB
+template <typename T, bool TRANSPOSED>
+__global__ void __launch_bounds__(256) narrow_weights_kernel(GroupedArgs g, int strips, int rank_blocks) {
+    using A = typename traits<T>::acc;
+    __shared__ A sums[4][NR_COLS][65];
+    const int strip = (int)(blockIdx.x % strips), rb = (int)(blockIdx.x / strips % rank_blocks), w = (int)(blockIdx.x / strips / rank_blocks);
+    const int width = TRANSPOSED ? g.k : g.n, rank = TRANSPOSED ? g.n : g.k;
+    const T* s = (const T*)(TRANSPOSED ? g.A : g.B);
+    const A* low = (const A*)(TRANSPOSED ? g.B : g.A);
+    const long long s_rs = TRANSPOSED ? g.a_rs : g.b_rs, s_cs = TRANSPOSED ? g.a_cs : g.b_cs, l_rs = TRANSPOSED ? g.b_rs : g.a_rs;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = strip * 64 + lane, r0 = rb * NR_COLS;
+    A acc[NR_COLS];
+#pragma unroll
+    for (int r = 0; r < NR_COLS; r++) acc[r] = 0;
+    for (int q = 0; q < g.gr.groups; q++) {
+        if (g.gr.weight(q) != w) continue;
+        const int e = g.gr.end(q);
+#pragma unroll 4
+        for (int i = g.gr.begin(q) + wave; i < e; i += 4) {
+            const A v = col < width ? (A)widen(s[i * s_rs + col * s_cs]) : (A)0;
+            const A* l = low + i * l_rs;
+#pragma unroll
+            for (int r = 0; r < NR_COLS; r++) acc[r] += v * l[r0 + r < rank ? r0 + r : rank - 1];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NR_COLS; r++) sums[wave][r][lane] = acc[r];
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < NR_COLS / 4; o++) {
+        const int id = threadIdx.x + 256 * o, r = TRANSPOSED ? id % NR_COLS : id / 64, c = TRANSPOSED ? id / NR_COLS : id % 64;
+        if (r0 + r >= rank || strip * 64 + c >= width) continue;
+        const A t = ((sums[0][r][c] + sums[1][r][c]) + sums[2][r][c]) + sums[3][r][c];
+        T* at = (T*)g.C + w * g.c_ws + (TRANSPOSED ? (strip * 64 + c) * g.c_rs + r0 + r : (r0 + r) * g.c_rs + strip * 64 + c);
+        T y = round_to<T>(t);
+        if (g.accumulate) y = round_to<T>(widen(*at) + widen(y));
+        *at = y;
+    }
+}
+
+int launch_narrow_rows(const GroupedArgs& g, int dtype) {
+    const int col_blocks = (g.n + NR_COLS - 1) / NR_COLS;
+    const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, NR_ROWS) * col_blocks;
+    if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(narrow_rows_kernel<T>, dim3((unsigned)blocks), dim3(NR_COLS * NR_LANES), 0, current_stream(), g, col_blocks));
+    return check_launch("narrow_rows_kernel") ? 0 : -1;
+}
+
+int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
+    const bool transposed = low == LOW_B;
+    const int width = transposed ? g.k : g.n, rank = transposed ? g.n : g.k, strips = (width + 63) / 64, rank_blocks = (rank + NR_COLS - 1) / NR_COLS;
+    const long long blocks = (long long)strips * rank_blocks * g.gr.weights;
+    if (blocks > 0x7fffffffll) { set_error("adapter gradient: %lld tiles are more than a launch takes", blocks); return -1; }
+    RP_DISPATCH_DTYPE(dtype, {
+        if (transposed) hipLaunchKernelGGL((narrow_weights_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, strips, rank_blocks);
+        else hipLaunchKernelGGL((narrow_weights_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, strips, rank_blocks);
+    });
+    return check_launch("narrow_weights_kernel") ? 0 : -1;
+}
+
+}  // namespace rp

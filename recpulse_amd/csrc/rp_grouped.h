@@ -22,11 +22,15 @@ struct GroupedArgs {
     int accumulate;
 };
 
-// Any strides and sizes, all types (rp_grouped_generic.hip).  LOW: which operand is in the accumulate type (float32, float64 for float64)
-// whatever the tensors' type is: the low-rank activations of an adapter.
+// Which operand is in the accumulate type (float32, float64 for float64) whatever the tensors' type is: the low-rank activations of an adapter
 enum GroupedLow { LOW_NONE = 0, LOW_A = 1, LOW_B = 2, LOW_C = 3 };
-int launch_grouped_rows_generic(const GroupedArgs& g, GroupedLow low, int dtype);
-int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dtype);
+
+// Any strides and sizes, all types (rp_grouped_generic.hip); low: A is.  No scales; by weights: no ids.
+int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype);
+int launch_grouped_weights_generic(const GroupedArgs& g, int dtype);
+// The same for an adapter's narrow products (rp_adapter_any.hip): by rows LOW_C, scales taken; by weights LOW_A or LOW_B, ids taken
+int launch_narrow_rows(const GroupedArgs& g, int dtype);
+int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype);
 // out[w, :] (+)= sum over the rows of w's groups of x[i, :]
 int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype);
 

@@ -23,10 +23,9 @@ static Lie lies(const void* p, long long row_stride, long long weight_stride, in
 }
 static Lie worse(Lie a, Lie b) { return a > b ? a : b; }
 
-static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
-    if (is16(dtype) && low == LOW_C && adapter_shrink16_takes(g)) return launch_adapter_shrink16(g, dtype);
-    if (is16(dtype) && low == LOW_NONE && grouped_stream16_takes(g)) return launch_grouped_stream16(g, dtype);
-    if (is16(dtype) && low == LOW_NONE && g.a_cs == 1 && (g.b_cs == 1 || g.b_rs == 1) && !path_disabled("mfma")) {
+static int grouped_rows(const GroupedArgs& g, int dtype) {
+    if (is16(dtype) && grouped_stream16_takes(g)) return launch_grouped_stream16(g, dtype);
+    if (is16(dtype) && g.a_cs == 1 && (g.b_cs == 1 || g.b_rs == 1) && !path_disabled("mfma")) {
         const bool b_mc = g.b_cs == 1;
         const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
         const long long tiles256 = (long long)((g.gr.rows + 255) / 256) * ((g.n + 255) / 256), tiles128 = (long long)((g.gr.rows + 127) / 128) * ((g.n + 127) / 128);
@@ -36,14 +35,12 @@ static int grouped_rows(const GroupedArgs& g, GroupedLow low, int dtype) {
         if (lie != LIE_NEITHER)
             return mean >= 96 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_rows16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_rows16_64(g, lie == LIE_RAGGED, dtype);
     }
-    // (h and u of fp32 and fp64 tensors are of their type: any of the operands may be low; the scale of h is the generic kernel's)
-    if (!is16(dtype) && !g.scales && g.accumulate != ACCUMULATE_JOINED && grouped_rows_wavek_takes(g, dtype)) return launch_grouped_rows_wavek(g, dtype);
-    return launch_grouped_rows_generic(g, low, dtype);
+    if (!is16(dtype) && grouped_rows_wavek_takes(g, dtype)) return launch_grouped_rows_wavek(g, dtype);
+    return launch_grouped_rows_generic(g, false, dtype);
 }
 
-static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
-    if (is16(dtype) && (low == LOW_A || low == LOW_B) && adapter_grad16_takes(g, low)) return launch_adapter_grad16(g, low, dtype);
-    if (is16(dtype) && low == LOW_NONE && !g.gr.ids && g.a_cs == 1 && g.b_cs == 1 && !path_disabled("mfma")) {
+static int grouped_weights(const GroupedArgs& g, int dtype) {
+    if (is16(dtype) && g.a_cs == 1 && g.b_cs == 1 && !path_disabled("mfma")) {
         const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
         const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
         if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && tiles256 >= cus() / 2)
@@ -52,7 +49,13 @@ static int grouped_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
             return g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_weights16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_weights16_64(g, lie == LIE_RAGGED, dtype);
     }
     if (!is16(dtype) && grouped_weights_wavek_takes(g, dtype)) return launch_grouped_weights_wavek(g, dtype);
-    return launch_grouped_weights_generic(g, low, dtype);
+    return launch_grouped_weights_generic(g, dtype);
+}
+
+// An adapter's narrow product (C is h or u) and the gradients of its factors
+static int narrow_rows(const GroupedArgs& g, int dtype) { return is16(dtype) && adapter_shrink16_takes(g) ? launch_adapter_shrink16(g, dtype) : launch_narrow_rows(g, dtype); }
+static int narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
+    return is16(dtype) && adapter_grad16_takes(g, low) ? launch_adapter_grad16(g, low, dtype) : launch_narrow_weights(g, low, dtype);
 }
 
 // The shared product of a layer with adapters, and the adapters' term
@@ -72,7 +75,7 @@ static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int d
     }
     if (rp_hip_gemm_strided_batched(s.C, s.A, s.B, s.bias, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate, dtype) != 0) return -1;
     if (is16(dtype) && adapter_expand16_takes(s, term)) return launch_adapter_expand16(s, term, dtype);
-    return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, LOW_A, dtype);
+    return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, true, dtype);
 }
 
 static bool grouped_args_ok(const char* who, bool pointers, int groups, int rows, int k, int n, std::initializer_list<long long> strides, int dtype) {
@@ -100,7 +103,7 @@ int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const v
     const char* who = "rp_hip_grouped_linear_forward";
     if (!grouped_args_ok(who, y && x && w && offsets, groups, rows, k, n, {x_rs, x_cs, w_gs, w_rs, w_cs, y_rs}, dtype) || !output_rows_ok(who, "y", rows, n, y_rs)) return -1;
     const RowGroups gr{offsets, nullptr, groups, rows, groups};
-    return grouped_rows(GroupedArgs{y, x, w, bias, nullptr, gr, k, n, x_rs, x_cs, w_gs, w_rs, w_cs, 0, y_rs, 0}, LOW_NONE, dtype);
+    return grouped_rows(GroupedArgs{y, x, w, bias, nullptr, gr, k, n, x_rs, x_cs, w_gs, w_rs, w_cs, 0, y_rs, 0}, dtype);
 }
 
 int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w, const int* offsets, int groups, int rows, int k, int n,
@@ -110,8 +113,8 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
     if (!grouped_args_ok(who, dy && offsets && (!dx || w) && (!dw || x), groups, rows, k, n, {dy_rs, x_rs, x_cs, w_gs, w_rs, w_cs, dx_rs}, dtype)) return -1;
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, nullptr, groups, rows, groups};
-    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0}, LOW_NONE, dtype) != 0) return -1;
-    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0}, LOW_NONE, dtype) != 0) return -1;
+    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0}, dtype) != 0) return -1;
+    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0}, dtype) != 0) return -1;
     if (db && launch_grouped_sums(db, dy, gr, n, dy_rs, accumulate_db, dtype) != 0) return -1;
     return 0;
 }
@@ -126,7 +129,7 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
     const GroupedArgs shared{y, x, w, bias, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, k, n, x_rs, x_cs, 0, w_rs, w_cs, 0, y_rs, 0};
     const AdapterTerm term{(const float*)h, b, gr, rank, (long long)rank * n, n, 1};
     if (is16(dtype) && adapter_few_rows16_takes(shared, low, term)) return launch_adapter_few_rows16(shared, low, term, dtype);
-    if (grouped_rows(low, LOW_C, dtype) != 0) return -1;
+    if (narrow_rows(low, dtype) != 0) return -1;
     return shared_with_term(shared, term, dtype);
 }
 
@@ -139,13 +142,13 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
                          {dy_rs, x_rs, x_cs, w_rs, w_cs, dx_rs}, dtype)) return -1;
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, ids, segments, rows, adapters};
-    if ((dx || da) && grouped_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, LOW_C, dtype) != 0) return -1;
+    if ((dx || da) && narrow_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, dtype) != 0) return -1;
     if (dx) {
         const GroupedArgs shared{dx, dy, w, nullptr, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, n, k, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
         if (shared_with_term(shared, AdapterTerm{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank}, dtype) != 0) return -1;
     }
-    if (da && grouped_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0}, LOW_B, dtype) != 0) return -1;
-    if (db && grouped_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, LOW_A, dtype) != 0) return -1;
+    if (da && narrow_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0}, LOW_B, dtype) != 0) return -1;
+    if (db && narrow_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, LOW_A, dtype) != 0) return -1;
     return 0;
 }
 

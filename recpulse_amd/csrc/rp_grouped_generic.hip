@@ -1,6 +1,6 @@
 // Grouped products for any strides, sizes and types: 64 x 64 tiles, 16 of k at a time through LDS, scalar multiply-adds, 4 x 4 outputs a
-// thread.  What no other kernel takes comes here: widths below a vector, operands without a unit stride, float64 and float32
-// next to low-rank activations in the accumulate type.  Sums in the accumulate type, rounded at the end, and once more where they are added to what the
+// thread.  What no other kernel takes comes here: the narrowest widths, operands without a unit stride, and the adapters' term of
+// float32 and float64, whose rank is a few steps of k.  Sums in the accumulate type, rounded at the end, and once more where they are added to what the
 // output holds (as a product of its own would be).
 #include "rp_grouped.h"
 
@@ -45,56 +45,50 @@ __device__ __forceinline__ void generic_tile(A acc[4][4], A (*as)[GG_T + 4], A (
     }
 }
 
-template <typename TA, typename TB, typename TC>
+template <typename TA, typename T>
 __global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g, int tiles_n) {
-    using A = typename traits<TA>::acc;
+    using A = typename traits<T>::acc;
     __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
     const RowTile rt = find_row_tile(g.gr, GG_T, (int)(blockIdx.x / tiles_n));
     if (rt.group < 0) return;
     const int n0 = (int)(blockIdx.x % tiles_n) * GG_T, m = rt.end - rt.begin, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
     const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
     A acc[4][4] = {};
-    generic_tile<TA, TB, A>(acc, as, bs, (const TA*)g.A + rt.begin * g.a_rs, (const TB*)g.B + rt.weight * g.b_ws + n0 * g.b_cs, m, n, g.k, g.a_rs, g.a_cs, g.b_rs, g.b_cs);
-    const A scale = g.scales ? (A)g.scales[rt.weight] : (A)1;
-    const TC* bias = (const TC*)g.bias;
+    generic_tile<TA, T, A>(acc, as, bs, (const TA*)g.A + rt.begin * g.a_rs, (const T*)g.B + rt.weight * g.b_ws + n0 * g.b_cs, m, n, g.k, g.a_rs, g.a_cs, g.b_rs, g.b_cs);
+    const T* bias = (const T*)g.bias;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (tr + i >= m || tc + j >= n) continue;
-            TC* p = (TC*)g.C + (rt.begin + tr + i) * g.c_rs + n0 + tc + j;
-            A v = scale * acc[i][j];
+            T* p = (T*)g.C + (rt.begin + tr + i) * g.c_rs + n0 + tc + j;
+            A v = acc[i][j];
             if (bias) v += widen(bias[(long long)rt.weight * g.n + n0 + tc + j]);
             if (g.accumulate == ACCUMULATE_JOINED) v += widen(*p);
-            TC y = round_to<TC>(v);
-            if (g.accumulate == ACCUMULATE) y = round_to<TC>(widen(*p) + widen(y));
+            T y = round_to<T>(v);
+            if (g.accumulate == ACCUMULATE) y = round_to<T>(widen(*p) + widen(y));
             *p = y;
         }
 }
 
-// A tile of C_w walks the rows of all groups whose weight is w, in the order of the groups
-template <typename TA, typename TB, typename TC>
+// A tile of C_w is a sum over the rows of group w
+template <typename T>
 __global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArgs g, int tiles_k, int tiles_n) {
-    using A = typename traits<TA>::acc;
+    using A = typename traits<T>::acc;
     __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
     const int tn = (int)(blockIdx.x % tiles_n), tk = (int)(blockIdx.x / tiles_n % tiles_k), w = (int)(blockIdx.x / tiles_n / tiles_k);
-    const int m0 = tk * GG_T, n0 = tn * GG_T, m = g.k - m0 < GG_T ? g.k - m0 : GG_T, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
+    const int m0 = tk * GG_T, n0 = tn * GG_T, m = g.k - m0 < GG_T ? g.k - m0 : GG_T, n = g.n - n0 < GG_T ? g.n - n0 : GG_T, b = g.gr.begin(w), e = g.gr.end(w);
     const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
     A acc[4][4] = {};
-    for (int s = g.gr.ids ? 0 : w; s < (g.gr.ids ? g.gr.groups : w + 1); s++) {
-        if (g.gr.weight(s) != w) continue;
-        const int b = g.gr.begin(s), e = g.gr.end(s);
-        generic_tile<TA, TB, A>(acc, as, bs, (const TA*)g.A + b * g.a_rs + m0 * g.a_cs, (const TB*)g.B + b * g.b_rs + n0 * g.b_cs, m, n, e - b, g.a_cs, g.a_rs, g.b_rs, g.b_cs);
-    }
+    generic_tile<T, T, A>(acc, as, bs, (const T*)g.A + b * g.a_rs + m0 * g.a_cs, (const T*)g.B + b * g.b_rs + n0 * g.b_cs, m, n, e - b, g.a_cs, g.a_rs, g.b_rs, g.b_cs);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (tr + i >= m || tc + j >= n) continue;
-            TC* p = (TC*)g.C + w * g.c_ws + (m0 + tr + i) * g.c_rs + n0 + tc + j;
-            A v = acc[i][j];
-            TC y = round_to<TC>(v);
-            if (g.accumulate) y = round_to<TC>(widen(*p) + widen(y));
+            T* p = (T*)g.C + w * g.c_ws + (m0 + tr + i) * g.c_rs + n0 + tc + j;
+            T y = round_to<T>(acc[i][j]);
+            if (g.accumulate) y = round_to<T>(widen(*p) + widen(y));
             *p = y;
         }
 }
@@ -107,11 +101,10 @@ __global__ void __launch_bounds__(256) grouped_sums_kernel(T* out, const T* x, R
     const int strip = (int)(blockIdx.x % strips), w = (int)(blockIdx.x / strips);
     const int c = strip * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
     A sum = 0;
-    for (int s = gr.ids ? 0 : w; s < (gr.ids ? gr.groups : w + 1); s++) {
-        if (gr.weight(s) != w || c >= cols) continue;
-        const int e = gr.end(s);
+    if (c < cols) {
+        const int e = gr.end(w);
 #pragma unroll 8
-        for (int i = gr.begin(s) + q; i < e; i += 4) sum += widen(x[i * x_rs + c]);
+        for (int i = gr.begin(w) + q; i < e; i += 4) sum += widen(x[i * x_rs + c]);
     }
     parts[q][threadIdx.x & 63] = sum;
     __syncthreads();
@@ -129,37 +122,23 @@ static bool grid_ok(long long blocks, const char* what) {
     return false;
 }
 
-template <typename T, typename F>
-static int with_low(GroupedLow low, F f) {
-    using A = typename traits<T>::acc;
-    switch (low) {
-        case LOW_NONE: return f(T{}, T{}, T{});
-        case LOW_A: return f(A{}, T{}, T{});
-        case LOW_B: return f(T{}, A{}, T{});
-        default: return f(T{}, T{}, A{});
-    }
-}
-
-int launch_grouped_rows_generic(const GroupedArgs& g, GroupedLow low, int dtype) {
+int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype) {
     const int tiles_n = (g.n + GG_T - 1) / GG_T;
     const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, GG_T) * tiles_n;
     if (!grid_ok(blocks, "grouped product")) return -1;
-    RP_DISPATCH_DTYPE(dtype, return with_low<T>(low, [&](auto a, auto b, auto c) {
-        hipLaunchKernelGGL((grouped_rows_generic_kernel<decltype(a), decltype(b), decltype(c)>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
-        return check_launch("grouped_rows_generic_kernel") ? 0 : -1;
-    }));
-    return 0;
+    RP_DISPATCH_DTYPE(dtype, {
+        if (low) hipLaunchKernelGGL((grouped_rows_generic_kernel<typename traits<T>::acc, T>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
+        else hipLaunchKernelGGL((grouped_rows_generic_kernel<T, T>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
+    });
+    return check_launch("grouped_rows_generic_kernel") ? 0 : -1;
 }
 
-int launch_grouped_weights_generic(const GroupedArgs& g, GroupedLow low, int dtype) {
+int launch_grouped_weights_generic(const GroupedArgs& g, int dtype) {
     const int tiles_k = (g.k + GG_T - 1) / GG_T, tiles_n = (g.n + GG_T - 1) / GG_T;
     const long long blocks = (long long)g.gr.weights * tiles_k * tiles_n;
     if (!grid_ok(blocks, "grouped weight gradient")) return -1;
-    RP_DISPATCH_DTYPE(dtype, return with_low<T>(low, [&](auto a, auto b, auto c) {
-        hipLaunchKernelGGL((grouped_weights_generic_kernel<decltype(a), decltype(b), decltype(c)>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_k, tiles_n);
-        return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
-    }));
-    return 0;
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_weights_generic_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_k, tiles_n));
+    return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
 }
 
 int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype) {
