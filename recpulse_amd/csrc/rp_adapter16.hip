@@ -99,12 +99,12 @@ int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low,
 }
 
 // ---- the term by itself: y[i] += h[i] . b_a, where the shared product is too small for tiles that would fill the CUs ----
-// 16 rows of a segment and 2048 columns a workgroup, 8 columns a thread: b is read once for the 16 rows, h through the scalar cache.
+// 16 rows of a segment and 512 columns a workgroup (one wave), 8 columns a lane: b is read once for the 16 rows, h through the scalar cache.
 template <typename T, bool ALONG_RANK>
-__global__ void __launch_bounds__(256) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int parts) {
+__global__ void __launch_bounds__(64) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int parts) {
     const RowTile rt = find_row_tile(term.gr, 16, (int)(blockIdx.x / parts));
     if (rt.group < 0) return;
-    const int col = (int)(blockIdx.x % parts) * 2048 + threadIdx.x * 8, m = rt.end - rt.begin, there = n - col;
+    const int col = (int)(blockIdx.x % parts) * 512 + threadIdx.x * 8, m = rt.end - rt.begin, there = n - col;
     if (there <= 0) return;
     const float* h = term.h + (long long)rt.begin * term.rank;
     const uint16_t* b = (const uint16_t*)term.b + rt.weight * term.b_ws + (long long)col * term.b_cs;
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(256) adapter_expand16_kernel(uint16_t* y, Adap
             }
         }
     } else {
+#pragma unroll 4
         for (int r = 0; r < term.rank; r++) {
             T bv[8];
             const u32x4_t x = load8(b + r * term.b_rs, there);
@@ -173,11 +174,11 @@ bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) 
 
 template <typename T>
 static int launch_expand(const GroupedArgs& shared, const AdapterTerm& term) {
-    const int parts = (shared.n + 2047) / 2048;
+    const int parts = (shared.n + 511) / 512;
     const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups, 16) * parts;
     if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
-    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
+    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
+    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
     return check_launch("adapter_expand16_kernel") ? 0 : -1;
 }
 

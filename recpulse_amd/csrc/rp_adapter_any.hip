@@ -2,9 +2,8 @@
 //
 // h[i] = scale x[i] . A_a has rank outputs a row and k products each: 64 x 64 tiles of it would leave most CUs without one and each with a long chain.
 // Here a workgroup owns eight rows and sixteen of the rank, and its sixteen groups of sixteen lanes share k.
-// dB_a = sum of h[i]^T dy[i] (and dA_a^T = sum of u[i]^T x[i]): a workgroup owns 64 columns and sixteen of the rank, a column a lane, and its four waves share the
+// dB_a = sum of h[i]^T dy[i] (and dA_a^T = sum of u[i]^T x[i]): a workgroup owns 64 columns and sixteen of the rank, a column a lane, and its sixteen waves share the
 // rows; the row's sixteen low values are uniform, one scalar load.
-// fp32, 2048 rows of 4096, rank 16, us, on 64 x 64 tiles and here: ANY_FIGURES
 #include "rp_grouped.h"
 
 #include <type_traits>
@@ -12,6 +11,7 @@
 namespace rp {
 
 constexpr int NR_ROWS = 8, NR_COLS = 16, NR_LANES = 16;          // rows and columns of a workgroup, lanes that share k
+constexpr int NW_WAVES = 16;                                     // waves that share the rows
 
 template <typename T>
 __global__ void __launch_bounds__(NR_COLS * NR_LANES) narrow_rows_kernel(GroupedArgs g, int col_blocks) {
@@ -44,9 +44,10 @@ __global__ void __launch_bounds__(NR_COLS * NR_LANES) narrow_rows_kernel(Grouped
 
 // TRANSPOSED: dA; else dB
 template <typename T, bool TRANSPOSED>
-__global__ void __launch_bounds__(256) narrow_weights_kernel(GroupedArgs g, int strips, int rank_blocks) {
+__global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedArgs g, int strips, int rank_blocks) {
     using A = typename traits<T>::acc;
-    __shared__ A sums[4][NR_COLS][65];
+    extern __shared__ __attribute__((aligned(16))) unsigned char nw_lds[];
+    A (*sums)[NR_COLS][65] = (A (*)[NR_COLS][65])nw_lds;         // [NW_WAVES]
     const int strip = (int)(blockIdx.x % strips), rb = (int)(blockIdx.x / strips % rank_blocks), w = (int)(blockIdx.x / strips / rank_blocks);
     const int width = TRANSPOSED ? g.k : g.n, rank = TRANSPOSED ? g.n : g.k;
     const T* s = (const T*)(TRANSPOSED ? g.A : g.B);
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(256) narrow_weights_kernel(GroupedArgs g, int 
         if (g.gr.weight(q) != w) continue;
         const int e = g.gr.end(q);
 #pragma unroll 4
-        for (int i = g.gr.begin(q) + wave; i < e; i += 4) {
+        for (int i = g.gr.begin(q) + wave; i < e; i += NW_WAVES) {
             const A v = col < width ? (A)widen(s[i * s_rs + col * s_cs]) : (A)0;
             const A* l = low + i * l_rs;
 #pragma unroll
@@ -70,11 +71,13 @@ __global__ void __launch_bounds__(256) narrow_weights_kernel(GroupedArgs g, int 
 #pragma unroll
     for (int r = 0; r < NR_COLS; r++) sums[wave][r][lane] = acc[r];
     __syncthreads();
+    {
+        const int id = threadIdx.x, r = TRANSPOSED ? id % NR_COLS : id / 64, c = TRANSPOSED ? id / NR_COLS : id % 64;       // a value a thread
+        static_assert(NR_COLS == NW_WAVES, "as many values as threads");
+        if (r0 + r >= rank || strip * 64 + c >= width) return;
+        A t = sums[0][r][c];
 #pragma unroll
-    for (int o = 0; o < NR_COLS / 4; o++) {
-        const int id = threadIdx.x + 256 * o, r = TRANSPOSED ? id % NR_COLS : id / 64, c = TRANSPOSED ? id / NR_COLS : id % 64;
-        if (r0 + r >= rank || strip * 64 + c >= width) continue;
-        const A t = ((sums[0][r][c] + sums[1][r][c]) + sums[2][r][c]) + sums[3][r][c];
+        for (int p = 1; p < NW_WAVES; p++) t += sums[p][r][c];
         T* at = (T*)g.C + w * g.c_ws + (TRANSPOSED ? (strip * 64 + c) * g.c_rs + r0 + r : (r0 + r) * g.c_rs + strip * 64 + c);
         T y = round_to<T>(t);
         if (g.accumulate) y = round_to<T>(widen(*at) + widen(y));
@@ -96,10 +99,15 @@ int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
     const long long blocks = (long long)strips * rank_blocks * g.gr.weights;
     if (blocks > 0x7fffffffll) { set_error("adapter gradient: %lld tiles are more than a launch takes", blocks); return -1; }
     RP_DISPATCH_DTYPE(dtype, {
-        if (transposed) hipLaunchKernelGGL((narrow_weights_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, strips, rank_blocks);
-        else hipLaunchKernelGGL((narrow_weights_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, strips, rank_blocks);
+        constexpr int lds = NW_WAVES * NR_COLS * 65 * (int)sizeof(typename traits<T>::acc);
+        auto launch = [&](auto kern) {
+            if (!check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(NW_WAVES * 64), lds, current_stream(), g, strips, rank_blocks);
+            return check_launch("narrow_weights_kernel") ? 0 : -1;
+        };
+        return transposed ? launch(narrow_weights_kernel<T, true>) : launch(narrow_weights_kernel<T, false>);
     });
-    return check_launch("narrow_weights_kernel") ? 0 : -1;
+    return 0;
 }
 
 }  // namespace rp
