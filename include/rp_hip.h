@@ -419,6 +419,9 @@ int rp_hip_combine_forward(void* y, const void* z, const void* weights, const in
 int rp_hip_combine_backward(void* grad_z, void* grad_weights, const void* grad_y, const void* z, const void* weights, const int* position, int tokens, int k, int d,
                             long long grad_y_rs, long long z_rs, long long grad_z_rs, int dtype);
 
+/* x[i] = 0 for the rows i of [offsets[groups], rows): what the entries above and below leave as it was. */
+int rp_hip_zero_rows_behind(void* x, const int* offsets, int groups, int rows, int width, long long x_rs, int dtype);
+
 /* Grouped linear layer, one weight for each group: y[i] = x[i] . w_g + bias_g for the rows i of group g.  x [rows, k], w [groups, k, n] with strides
  * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for. */
 int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,

@@ -104,6 +104,7 @@ SIGNATURES = {
     "rp_hip_dispatch_rows": (_i, [_vp] * 3 + [_i] * 3 + [_ll] * 2 + [_i]),
     "rp_hip_combine_forward": (_i, [_vp] * 4 + [_i] * 3 + [_ll] * 2 + [_i]),
     "rp_hip_combine_backward": (_i, [_vp] * 6 + [_i] * 3 + [_ll] * 3 + [_i]),
+    "rp_hip_zero_rows_behind": (_i, [_vp] * 2 + [_i] * 3 + [_ll] + [_i]),
     "rp_hip_grouped_linear_forward": (_i, [_vp] * 5 + [_i] * 4 + [_ll] * 6 + [_i]),
     "rp_hip_grouped_linear_backward": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 7 + [_i] * 4),
     "rp_hip_adapter_linear_forward": (_i, [_vp] * 10 + [_i] * 6 + [_ll] * 5 + [_i]),

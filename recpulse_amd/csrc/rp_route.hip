@@ -473,6 +473,13 @@ __global__ void __launch_bounds__(256) combine_kernel(T* y, const T* z, const we
     }
 }
 
+// Rows behind the last group: a workgroup a row, and nothing to do for nearly all of them
+__global__ void __launch_bounds__(256) zero_rows_behind_kernel(unsigned char* x, const int* offsets, int groups, int rows, long long row_bytes, long long width_bytes) {
+    const int last = offsets[groups];
+    for (long long r = (last < 0 ? 0 : last) + blockIdx.x; r < rows; r += gridDim.x)
+        for (long long i = threadIdx.x; i < width_bytes / 2; i += 256) ((uint16_t*)(x + r * row_bytes))[i] = 0;
+}
+
 // A wave for each token: its gradient stays in registers (HELD pieces a lane; longer rows are read again for each slot), z is read once
 // and dz written once.  The 64 lanes' partial dots are added in a fixed tree.
 template <typename T, int VEC, int HELD>
@@ -606,6 +613,15 @@ int rp_hip_dispatch_rows(void* out, const void* x, const int* position, int toke
         }
     });
     return check_launch("dispatch_kernel") ? 0 : -1;
+}
+
+int rp_hip_zero_rows_behind(void* x, const int* offsets, int groups, int rows, int width, long long x_rs, int dtype) {
+    if (!x || !offsets || groups <= 0 || rows <= 0 || width <= 0) { set_error("rp_hip_zero_rows_behind: null operand or non-positive extent (groups=%d rows=%d width=%d)", groups, rows, width); return -1; }
+    if (x_rs < width) { set_error("rp_hip_zero_rows_behind: rows of %lld elements apart hold %d", x_rs, width); return -1; }
+    const long long es = (long long)dtype_size(dtype);
+    if (!es) { set_error("rp_hip_zero_rows_behind: unsupported dtype %d", dtype); return -1; }
+    hipLaunchKernelGGL(zero_rows_behind_kernel, dim3(rows < 1024 ? rows : 1024), dim3(256), 0, current_stream(), (unsigned char*)x, offsets, groups, rows, x_rs * es, width * es);
+    return check_launch("zero_rows_behind_kernel") ? 0 : -1;
 }
 
 int rp_hip_combine_forward(void* y, const void* z, const void* weights, const int* position, int tokens, int k, int d, long long y_rs, long long z_rs, int dtype) {

@@ -1,5 +1,6 @@
-"""Parameter bookkeeping (`Module`), the affine layer (`Linear`), the convolution layer (`Conv2d`) and the
-recurrent cells (`LSTMCell`, `GRUCell`).
+"""Parameter bookkeeping (`Module`), the affine layer (`Linear`), the convolution layer (`Conv2d`), the
+recurrent cells (`LSTMCell`, `GRUCell`) and, beyond the reference, layers whose weight depends on the row
+(`ExpertLinear`, `MixtureOfExperts`, `AdapterLinear`).
 
 Behaviour kept from the reference's recpulse/module.py:
   * a module records its parameters in `tracked` under their attribute names; assigning a
@@ -188,3 +189,55 @@ class GRUCell(_RecurrentCell):
         h = h if h is not None else self._zero_state(x)
         return self.keep(x.op_gru_cell(h, self.weight_ih, self.weight_hh, self.bias_ih, self.bias_hh))
 
+
+
+class ExpertLinear(Module):
+    """y = x . W[g] + b[g] for the rows of group g of a routing: W [experts, in_features, out_features], b [experts, out_features]."""
+
+    def __init__(self, experts, in_features, out_features, bias=True):
+        super().__init__()
+        self.experts, self.in_features, self.out_features = experts, in_features, out_features
+        init = rp.randn([experts, in_features, out_features]).mul_scalar(1.0 / math.sqrt(in_features))
+        self.weight = self.track("weight", init.requires_grad_(True))
+        self.bias = self.track("bias", rp.zeros([experts, out_features]).requires_grad_(True)) if bias else None
+
+    def forward(self, x, routing):
+        return self.keep(x.op_grouped_linear(self.weight, routing, self.bias))
+
+
+class MixtureOfExperts(Module):
+    """y[t] = sum over the k experts e of token t of w[t, e] relu(x[t] . W1[e] + b1[e]) . W2[e] + b2[e], with the experts of the k largest
+    of x[t] . R and the softmax among them (normalize) or among all as weights.  x [tokens, features]."""
+
+    def __init__(self, features, hidden, experts, k, normalize=True, bias=True):
+        super().__init__()
+        self.features, self.hidden, self.experts, self.k, self.normalize = features, hidden, experts, k, normalize
+        self.router = Linear(features, experts, bias=False)
+        self.up = ExpertLinear(experts, features, hidden, bias)
+        self.down = ExpertLinear(experts, hidden, features, bias)
+
+    def forward(self, x):
+        weights, routing = self.router(x).op_route(self.k, self.normalize)
+        rows = self.keep(x.op_dispatch(routing))
+        out = self.down(self.keep(self.up(rows, routing).op_relu()), routing)
+        return self.keep(out.op_combine(weights, routing))
+
+
+class AdapterLinear(Module):
+    """y = x . W + b + scale (x . A[a]) . B[a] with the adapter a of the row's segment: W [in_features, out_features] as in `Linear`,
+    A [adapters, in_features, rank] initialised N(0, 1/in_features), B [adapters, rank, out_features] zeros (an untrained adapter changes
+    nothing).  The shared weight and bias are frozen unless `train_shared`."""
+
+    def __init__(self, in_features, out_features, adapters, rank, scale=1.0, bias=True, train_shared=False):
+        super().__init__()
+        self.in_features, self.out_features, self.adapters, self.rank = in_features, out_features, adapters, rank
+        self.scales = [float(scale)] * adapters
+        spread = 1.0 / math.sqrt(in_features)
+        self.weight = self.track("weight", rp.randn([in_features, out_features]).mul_scalar(spread).requires_grad_(train_shared))
+        self.bias = self.track("bias", rp.zeros([out_features]).requires_grad_(train_shared)) if bias else None
+        self.a = self.track("a", rp.randn([adapters, in_features, rank]).mul_scalar(spread).requires_grad_(True))
+        self.b = self.track("b", rp.zeros([adapters, rank, out_features]).requires_grad_(True))
+
+    def forward(self, x, ids, lengths):
+        """ids[s]: adapter of segment s (-1: none), lengths[s]: how many rows it has."""
+        return self.keep(x.op_adapter_linear(self.weight, self.a, self.b, ids, lengths, self.bias, self.scales))

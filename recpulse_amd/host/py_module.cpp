@@ -30,6 +30,14 @@ struct PyTensor {
 
 using TensorPtr = std::unique_ptr<PyTensor>;
 
+struct PyRouting {
+    Routing* r;                      // owns one reference
+    explicit PyRouting(Routing* routing) : r(routing) {}
+    PyRouting(const PyRouting&) = delete;
+    PyRouting& operator=(const PyRouting&) = delete;
+    ~PyRouting() { free_routing(r); }
+};
+
 TensorPtr wrap(Tensor* t, const char* op) {
     if (!t) {
         std::string msg = std::string(op) + " operation failed";
@@ -127,9 +135,32 @@ std::vector<int> targets_from(const py::object& o) {  // a sequence of ints or a
 // a temporary cannot be told from a named object on this interpreter: then nothing is ever treated as one.
 static int g_temporary_refs = 0;
 
+// one of a routing's arrays on the host; which: 0 experts [tokens, k], 1 offsets, 2 order, 3 position [tokens, k]
+static py::array routing_array(PyRouting& p, int which) {
+    Routing* r = p.r;
+    std::vector<py::ssize_t> shape;
+    if (which == 1) shape = {(py::ssize_t)r->groups + 1};
+    else if (which == 2) shape = {(py::ssize_t)r->tokens * r->k};
+    else shape = {r->tokens, r->k};
+    py::array_t<int> out(shape);
+    int* to = out.mutable_data();
+    if (routing_read(r, which == 0 ? to : nullptr, which == 1 ? to : nullptr, which == 2 ? to : nullptr, which == 3 ? to : nullptr) != 0) throw std::runtime_error(std::string("routing: ") + rp_last_error());
+    return out;
+}
+
+static Tensor* optional_tensor(const py::object& o) { return o.is_none() ? nullptr : o.cast<PyTensor&>().t; }
+
 PYBIND11_MODULE(recpulse_cuda, m) {
     m.doc() = "RecPulse tensor module for the matmul path, MI355X device layer underneath";
 
+    py::class_<PyRouting>(m, "Routing")
+        .def_property_readonly("tokens", [](PyRouting& p) { return p.r->tokens; })
+        .def_property_readonly("k", [](PyRouting& p) { return p.r->k; })
+        .def_property_readonly("groups", [](PyRouting& p) { return p.r->groups; })
+        .def_property_readonly("experts", [](PyRouting& p) { return routing_array(p, 0); })
+        .def_property_readonly("offsets", [](PyRouting& p) { return routing_array(p, 1); })
+        .def_property_readonly("order", [](PyRouting& p) { return routing_array(p, 2); })
+        .def_property_readonly("position", [](PyRouting& p) { return routing_array(p, 3); });
     py::class_<PyTensor>(m, "Tensor")
         .def_property_readonly("shape", [](PyTensor& s) { py::tuple t(s.t->ndim); for (int i = 0; i < s.t->ndim; i++) t[i] = s.t->shape[i]; return t; })
         .def_property_readonly("strides", [](PyTensor& s) { py::tuple t(s.t->ndim); for (int i = 0; i < s.t->ndim; i++) t[i] = s.t->strides[i]; return t; })
@@ -199,6 +230,23 @@ PYBIND11_MODULE(recpulse_cuda, m) {
         }, py::arg("h"), py::arg("weight_ih"), py::arg("weight_hh"), py::arg("bias_ih") = py::none(), py::arg("bias_hh") = py::none())
         .def("op_attention", [](PyTensor& q, PyTensor& k, PyTensor& v, double scale) { return wrap(op_attention(q.t, k.t, v.t, scale), "op_attention"); },
              py::arg("k"), py::arg("v"), py::arg("scale"))
+        // ---- layers whose weight depends on the row ----
+        .def("op_route", [](PyTensor& a, int k, bool normalize) {
+            Routing* r = nullptr;
+            TensorPtr w = wrap(op_route(a.t, k, normalize, &r), "op_route");
+            return py::make_tuple(py::cast(std::move(w)), py::cast(std::make_unique<PyRouting>(r)));
+        }, py::arg("k"), py::arg("normalize") = true)
+        .def("op_dispatch", [](PyTensor& x, PyRouting& r) { return wrap(op_dispatch(x.t, r.r), "op_dispatch"); }, py::arg("routing"))
+        .def("op_combine", [](PyTensor& z, PyTensor& w, PyRouting& r) { return wrap(op_combine(z.t, w.t, r.r), "op_combine"); }, py::arg("weights"), py::arg("routing"))
+        .def("op_grouped_linear", [](PyTensor& x, PyTensor& w, PyRouting& r, py::object bias) { return wrap(op_grouped_linear(x.t, w.t, optional_tensor(bias), r.r), "op_grouped_linear"); },
+             py::arg("weight"), py::arg("routing"), py::arg("bias") = py::none())
+        .def("op_adapter_linear", [](PyTensor& x, PyTensor& w, PyTensor& a, PyTensor& b, std::vector<int> ids, std::vector<int> lengths, py::object bias, py::object scales) {
+            std::vector<float> sc;
+            if (!scales.is_none()) for (auto item : scales) sc.push_back(item.cast<float>());
+            if (ids.size() != lengths.size()) throw std::runtime_error("op_adapter_linear operation failed: one adapter and one length for each segment");
+            if (!scales.is_none() && (a.t->ndim != 3 || (int)sc.size() != a.t->shape[0])) throw std::runtime_error("op_adapter_linear operation failed: one scale for each adapter");
+            return wrap(op_adapter_linear(x.t, w.t, optional_tensor(bias), a.t, b.t, scales.is_none() ? nullptr : sc.data(), ids.data(), lengths.data(), (int)ids.size()), "op_adapter_linear");
+        }, py::arg("weight"), py::arg("a"), py::arg("b"), py::arg("ids"), py::arg("lengths"), py::arg("bias") = py::none(), py::arg("scales") = py::none())
         .def("op_add", [](PyTensor& a, PyTensor& b) { return wrap(op_add(a.t, b.t), "op_add"); })
         .def("op_relu", [](PyTensor& a) { return wrap(op_relu(a.t), "op_relu"); })
         // `x.op_mul_scalar(s).op_softmax()`: the scaled tensor is a temporary that nothing can read once this call has
@@ -297,6 +345,11 @@ PYBIND11_MODULE(recpulse_cuda, m) {
         int n = (int)v.size();
         return wrap(values_tensor(v.data(), DTYPE_FLOAT64, parse_dtype(dtype), -1, parse_device(device), 1, &n, nullptr), "values");
     }, py::arg("data"), py::arg("dtype") = "float32", py::arg("device") = "cpu");
+    m.def("group_rows", [](std::vector<int> ids, int groups, const std::string& device) {        // rows with a group each, as a routing with k = 1
+        Routing* r = routing_from_ids(ids.data(), (int)ids.size(), groups, parse_device(device));
+        if (!r) throw std::runtime_error(std::string("group_rows operation failed: ") + rp_last_error());
+        return std::make_unique<PyRouting>(r);
+    }, py::arg("ids"), py::arg("groups"), py::arg("device") = "cuda");
     m.def("from_numpy", &from_numpy);
     m.def("randn", [](py::object shape, const std::string& dtype, const std::string& device, const std::string&) {
         auto s = to_shape(shape);

@@ -1046,6 +1046,134 @@ void backward_attention_fn(GradFn* self, Tensor* grad_output) {
     free_tensor(g); free_tensor(od); free_tensor(qd); free_tensor(kd); free_tensor(vd);
 }
 
+// ---- layers whose weight depends on the row ----
+struct RoutingSaved { Routing* routing; int normalize; };
+
+void free_routing_saved(void* p) {
+    free_routing(((RoutingSaved*)p)->routing);
+    free(p);
+}
+
+void save_routing(GradFn* gf, Routing* routing, int normalize = 0) {
+    RoutingSaved* s = (RoutingSaved*)malloc(sizeof(RoutingSaved));
+    s->routing = routing_retain(routing);
+    s->normalize = normalize;
+    gf->saved_data = s;
+    gf->free_saved = free_routing_saved;
+}
+
+DType weights_dtype(DType dtype) { return dtype == DTYPE_FLOAT64 ? DTYPE_FLOAT64 : DTYPE_FLOAT32; }
+
+// the rows of a [rows, d] tensor that belong to no group
+int zero_behind(Tensor* x, Routing* r) { return rp_hip_zero_rows_behind(x->data, r->offsets, r->groups, x->shape[0], x->shape[1], x->shape[1], x->dtype); }
+
+void backward_route_fn(GradFn* self, Tensor* grad_output) {
+    Tensor* logits = self->inputs[0];
+    if (!needs_grad(logits)) return;
+    RoutingSaved* s = (RoutingSaved*)self->saved_data;
+    Routing* r = s->routing;
+    Tensor* gd = dense(grad_output); Tensor* wd = dense(self->owner); Tensor* ld = dense(logits);
+    Tensor* g = empty_tensor(logits->dtype, logits->device_id, 2, logits->shape);
+    const bool ok = gd && wd && ld && g && on_device(r->device_id) &&
+                    rp_hip_route_backward(g->data, gd->data, wd->data, r->experts, ld->data, r->groups, r->tokens, r->groups, r->k, s->normalize, logits->dtype) == 0;
+    if (ok) accumulate_grad(logits, g);
+    else { dev_fail("op_route backward"); free_tensor(g); }
+    free_tensor(gd); free_tensor(wd); free_tensor(ld);
+}
+
+void backward_dispatch_fn(GradFn* self, Tensor* grad_output) {
+    Tensor* x = self->inputs[0];
+    if (!needs_grad(x)) return;
+    Routing* r = ((RoutingSaved*)self->saved_data)->routing;
+    const int d = x->shape[1];
+    Tensor* gd = dense(grad_output);
+    Tensor* g = empty_tensor(x->dtype, x->device_id, 2, x->shape);
+    if (gd && g && on_device(r->device_id) && rp_hip_combine_forward(g->data, gd->data, nullptr, r->position, r->tokens, r->k, d, d, d, x->dtype) == 0) accumulate_grad(x, g);
+    else { dev_fail("op_dispatch backward"); free_tensor(g); }
+    free_tensor(gd);
+}
+
+void backward_combine_fn(GradFn* self, Tensor* grad_output) {
+    Tensor* z = self->inputs[0]; Tensor* w = self->inputs[1];
+    if (!needs_grad(z) && !needs_grad(w)) return;
+    Routing* r = ((RoutingSaved*)self->saved_data)->routing;
+    const int d = z->shape[1];
+    Tensor* gd = dense(grad_output); Tensor* zd = dense(z); Tensor* wd = dense(w);
+    Tensor* gz = empty_tensor(z->dtype, z->device_id, 2, z->shape);
+    Tensor* gw = empty_tensor(w->dtype, w->device_id, 2, w->shape);
+    const bool ok = gd && zd && wd && gz && gw && on_device(r->device_id) &&
+                    rp_hip_combine_backward(gz->data, gw->data, gd->data, zd->data, wd->data, r->position, r->tokens, r->k, d, d, d, d, z->dtype) == 0 && zero_behind(gz, r) == 0;
+    if (!ok) dev_fail("op_combine backward");
+    if (ok && needs_grad(z)) accumulate_grad(z, gz); else free_tensor(gz);
+    if (ok && needs_grad(w)) accumulate_grad(w, gw); else free_tensor(gw);
+    free_tensor(gd); free_tensor(zd); free_tensor(wd);
+}
+
+void backward_grouped_linear_fn(GradFn* self, Tensor* grad_output) {
+    Tensor* x = self->inputs[0]; Tensor* w = self->inputs[1];
+    Tensor* bias = self->num_inputs > 2 ? self->inputs[2] : nullptr;
+    Routing* r = ((RoutingSaved*)self->saved_data)->routing;
+    const int rows = x->shape[0], k = x->shape[1], n = w->shape[2];
+    Tensor* gd = dense(grad_output);
+    GradSlot sx = grad_slot(x), sw = grad_slot(w), sb = grad_slot(bias);
+    bool ok = gd && on_device(x->device_id) &&
+              rp_hip_grouped_linear_backward(sx.into ? sx.into->data : nullptr, sw.into ? sw.into->data : nullptr, sb.into ? sb.into->data : nullptr, gd->data, x->data, w->data,
+                                             r->offsets, r->groups, rows, k, n, n, x->strides[0], x->strides[1], w->strides[0], w->strides[1], w->strides[2], k,
+                                             sx.accumulate, sw.accumulate, sb.accumulate, x->dtype) == 0;
+    if (ok && sx.fresh) ok = zero_behind(sx.fresh, r) == 0;
+    if (!ok) dev_fail("op_grouped_linear backward");
+    Tensor* targets[3] = {x, w, bias};
+    GradSlot* slots[3] = {&sx, &sw, &sb};
+    for (int i = 0; i < 3; i++) {
+        if (!slots[i]->fresh) continue;
+        if (ok) accumulate_grad(targets[i], slots[i]->fresh);
+        else free_tensor(slots[i]->fresh);
+    }
+    free_tensor(gd);
+}
+
+struct AdapterSaved { int segments, device_id; void* plan; void* h; };      // plan: offsets [segments + 1], ids [segments], scales [adapters] or nothing
+const int* plan_offsets(const AdapterSaved* s) { return (const int*)s->plan; }
+const int* plan_ids(const AdapterSaved* s) { return (const int*)s->plan + s->segments + 1; }
+const float* plan_scales(const AdapterSaved* s) { return (const float*)s->plan + 2 * s->segments + 1; }
+
+void free_adapter_saved(void* p) {
+    AdapterSaved* s = (AdapterSaved*)p;
+    if (on_device(s->device_id)) {
+        if (s->plan) rp_hip_free(s->plan);
+        if (s->h) rp_hip_free(s->h);
+    }
+    free(s);
+}
+
+// inputs: x, w, a, b and, if there is one, the bias
+void backward_adapter_linear_fn(GradFn* self, Tensor* grad_output) {
+    Tensor* x = self->inputs[0]; Tensor* w = self->inputs[1]; Tensor* a = self->inputs[2]; Tensor* b = self->inputs[3];
+    Tensor* bias = self->num_inputs > 4 ? self->inputs[4] : nullptr;
+    AdapterSaved* s = (AdapterSaved*)self->saved_data;
+    const int rows = x->shape[0], k = x->shape[1], n = w->shape[1], adapters = a->shape[0], rank = a->shape[2];
+    Tensor* gd = dense(grad_output); Tensor* ad = dense(a); Tensor* bd = dense(b);
+    GradSlot slots[5] = {grad_slot(x), grad_slot(w), grad_slot(a), grad_slot(b), grad_slot(bias)};
+    auto into = [&](int i) { return slots[i].into ? slots[i].into->data : nullptr; };
+    void* u = nullptr;
+    bool ok = gd && ad && bd && on_device(x->device_id) && rp_hip_malloc(&u, dtype_size(weights_dtype(x->dtype)) * (size_t)rows * rank) == 0;
+    if (ok && (into(0) || into(2) || into(3)))
+        ok = rp_hip_adapter_linear_backward(into(0), into(2), into(3), u, gd->data, x->data, w->data, ad->data, bd->data, s->h, plan_scales(s), plan_ids(s), plan_offsets(s), s->segments, adapters, rows, k, n, rank,
+                                            n, x->strides[0], x->strides[1], w->strides[0], w->strides[1], k, slots[0].accumulate, slots[2].accumulate, slots[3].accumulate, x->dtype) == 0;
+    if (ok && (into(1) || into(4)))
+        ok = rp_hip_linear_backward(nullptr, into(1), into(4), gd->data, x->data, w->data, rows, k, n, x->strides[0], x->strides[1], w->strides[0], w->strides[1], k, 1, n, 1,
+                                    0, slots[1].accumulate, slots[4].accumulate, x->dtype) == 0;
+    if (!ok) dev_fail("op_adapter_linear backward");
+    Tensor* targets[5] = {x, w, a, b, bias};
+    for (int i = 0; i < 5; i++) {
+        if (!slots[i].fresh) continue;
+        if (ok) accumulate_grad(targets[i], slots[i].fresh);
+        else free_tensor(slots[i].fresh);
+    }
+    if (u) rp_hip_free(u);
+    free_tensor(gd); free_tensor(ad); free_tensor(bd);
+}
+
 // ---- conv2d ----------------------------------------------------------------------------
 // The reference lowers one sample at a time: im2col, rp_matmul, and for the gradients col2im or a densified transpose
 // per sample (ops/ops.c:4759-4770, 4533-4551, 4575-4617), with the bias and its gradient done on the host.  Here a
@@ -1698,6 +1826,161 @@ Tensor* op_cross_entropy_loss(Tensor* input, const int* targets, int batch_size,
         gf->free_saved = free_ce_saved;
     } else {
         rp_hip_free(tdev);
+    }
+    return out;
+}
+
+// ---- layers whose weight depends on the row (extensions) ----
+static Routing* make_routing(int tokens, int k, int groups, int device_id) {
+    const size_t slots = (size_t)tokens * k;
+    void* block = nullptr;
+    if (!on_device(device_id) || rp_hip_malloc(&block, sizeof(int) * (3 * slots + groups + 1)) != 0) { dev_fail("routing"); return nullptr; }
+    Routing* r = (Routing*)calloc(1, sizeof(Routing));
+    r->tokens = tokens; r->k = k; r->groups = groups; r->device_id = device_id; r->refcount = 1;
+    r->block = block;
+    r->experts = (int*)block; r->order = r->experts + slots; r->position = r->order + slots; r->offsets = r->position + slots;
+    return r;
+}
+
+Routing* routing_retain(Routing* r) { if (r) r->refcount++; return r; }
+
+void free_routing(Routing* r) {
+    if (!r || --r->refcount > 0) return;
+    if (on_device(r->device_id)) rp_hip_free(r->block);
+    free(r);
+}
+
+Routing* routing_from_ids(const int* ids, int count, int groups, int device_id) {
+    if (!ids || count <= 0 || groups <= 0) { fail("group_rows: at least one row and one group"); return nullptr; }
+    if (device_id == -1) { fail("group_rows: routing lives on a GPU"); return nullptr; }
+    Routing* r = make_routing(count, 1, groups, device_id);
+    if (!r) return nullptr;
+    if (rp_hip_memcpy_h2d(r->experts, ids, sizeof(int) * (size_t)count) != 0 || rp_hip_group_rows(r->offsets, r->order, r->position, r->experts, count, groups) != 0) { dev_fail("group_rows"); free_routing(r); return nullptr; }
+    return r;
+}
+
+int routing_read(Routing* r, int* experts, int* offsets, int* order, int* position) {
+    if (!r || !on_device(r->device_id)) return dev_fail("routing");
+    const size_t slots = sizeof(int) * (size_t)r->tokens * r->k;
+    const struct { int* to; const int* from; size_t bytes; } copies[] = {{experts, r->experts, slots}, {offsets, r->offsets, sizeof(int) * (size_t)(r->groups + 1)}, {order, r->order, slots}, {position, r->position, slots}};
+    for (const auto& c : copies)
+        if (c.to && rp_hip_memcpy_d2h(c.to, c.from, c.bytes) != 0) return dev_fail("routing");
+    return 0;
+}
+
+Tensor* op_route(Tensor* logits, int k, bool normalize, Routing** routing) {
+    if (!logits || !routing) return nullptr;
+    *routing = nullptr;
+    if (logits->ndim != 2) { fail("op_route: logits [tokens, experts]"); return nullptr; }
+    if (logits->device_id == -1) { fail("op_route on host tensors is not provided by this build; move the operands to a GPU"); return nullptr; }
+    const int tokens = logits->shape[0], groups = logits->shape[1];
+    if (k < 1 || k > groups) { fail("op_route: k must be between 1 and the %d experts", groups); return nullptr; }
+    const int shape[2] = {tokens, k};
+    Tensor* ld = dense(logits);
+    Tensor* out = ld ? empty_tensor(weights_dtype(logits->dtype), logits->device_id, 2, shape) : nullptr;
+    Routing* r = out ? make_routing(tokens, k, groups, logits->device_id) : nullptr;
+    if (r && rp_hip_route_forward(out->data, r->experts, r->offsets, r->order, r->position, ld->data, groups, tokens, groups, k, normalize, logits->dtype) != 0) {
+        dev_fail("op_route");
+        free_routing(r);
+        r = nullptr;
+    }
+    free_tensor(ld);
+    if (!r) { free_tensor(out); return nullptr; }
+    if (needs_grad(logits)) save_routing(attach(out, backward_route_fn, {logits}), r, normalize);
+    *routing = r;
+    return out;
+}
+
+static bool routed(const Tensor* t, const Routing* r, int rows, const char* op) {
+    if (t->device_id == -1) { fail("%s on host tensors is not provided by this build; move the operands to a GPU", op); return false; }
+    if (t->ndim != 2 || t->shape[0] != rows || t->device_id != r->device_id) { fail("%s: %d rows on the routing's device", op, rows); return false; }
+    return true;
+}
+
+Tensor* op_dispatch(Tensor* x, Routing* r) {
+    if (!x || !r || !routed(x, r, r->tokens, "op_dispatch")) return nullptr;
+    const int shape[2] = {r->tokens * r->k, x->shape[1]}, d = x->shape[1];
+    Tensor* xd = dense(x);
+    Tensor* out = xd ? empty_tensor(x->dtype, x->device_id, 2, shape) : nullptr;
+    const bool ok = out && on_device(x->device_id) && rp_hip_dispatch_rows(out->data, xd->data, r->position, r->tokens, r->k, d, d, d, x->dtype) == 0 && zero_behind(out, r) == 0;
+    free_tensor(xd);
+    if (!ok) { dev_fail("op_dispatch"); free_tensor(out); return nullptr; }
+    if (needs_grad(x)) save_routing(attach(out, backward_dispatch_fn, {x}), r);
+    return out;
+}
+
+Tensor* op_combine(Tensor* z, Tensor* w, Routing* r) {
+    if (!z || !w || !r || !routed(z, r, r->tokens * r->k, "op_combine") || !routed(w, r, r->tokens, "op_combine")) return nullptr;
+    if (w->shape[1] != r->k || w->dtype != weights_dtype(z->dtype)) { fail("op_combine: weights [tokens, k] as op_route leaves them"); return nullptr; }
+    const int shape[2] = {r->tokens, z->shape[1]}, d = z->shape[1];
+    Tensor* zd = dense(z); Tensor* wd = dense(w);
+    Tensor* out = zd && wd ? empty_tensor(z->dtype, z->device_id, 2, shape) : nullptr;
+    const bool ok = out && on_device(z->device_id) && rp_hip_combine_forward(out->data, zd->data, wd->data, r->position, r->tokens, r->k, d, d, d, z->dtype) == 0;
+    free_tensor(zd); free_tensor(wd);
+    if (!ok) { dev_fail("op_combine"); free_tensor(out); return nullptr; }
+    if (needs_grad(z) || needs_grad(w)) save_routing(attach(out, backward_combine_fn, {z, w}), r);
+    return out;
+}
+
+Tensor* op_grouped_linear(Tensor* x, Tensor* w, Tensor* bias, Routing* r) {
+    if (!x || !w || !r || !routed(x, r, r->tokens * r->k, "op_grouped_linear")) return nullptr;
+    if (w->ndim != 3 || !same_place(x, w) || w->shape[0] != r->groups || w->shape[1] != x->shape[1]) { fail("op_grouped_linear: weight [groups, in_features, out_features] of x's dtype and device"); return nullptr; }
+    if (bias && (bias->ndim != 2 || bias->shape[0] != r->groups || bias->shape[1] != w->shape[2] || !same_place(x, bias) || !rp_is_contiguous(bias))) { fail("op_grouped_linear: bias must be dense [groups, out_features]"); return nullptr; }
+    const int shape[2] = {x->shape[0], w->shape[2]};
+    Tensor* out = empty_tensor(x->dtype, x->device_id, 2, shape);
+    const bool ok = out && on_device(x->device_id) &&
+                    rp_hip_grouped_linear_forward(out->data, x->data, w->data, bias ? bias->data : nullptr, r->offsets, r->groups, x->shape[0], x->shape[1], w->shape[2], x->strides[0], x->strides[1],
+                                                  w->strides[0], w->strides[1], w->strides[2], w->shape[2], x->dtype) == 0 && zero_behind(out, r) == 0;
+    if (!ok) { dev_fail("op_grouped_linear"); free_tensor(out); return nullptr; }
+    if (needs_grad(x) || needs_grad(w) || needs_grad(bias)) {
+        if (bias) save_routing(attach(out, backward_grouped_linear_fn, {x, w, bias}), r);
+        else save_routing(attach(out, backward_grouped_linear_fn, {x, w}), r);
+    }
+    return out;
+}
+
+Tensor* op_adapter_linear(Tensor* x, Tensor* w, Tensor* bias, Tensor* a, Tensor* b, const float* scales, const int* ids, const int* lengths, int segments) {
+    if (!x || !w || !a || !b) return nullptr;
+    if (segments <= 0 || !ids || !lengths) { fail("op_adapter_linear: at least one segment"); return nullptr; }
+    if (x->device_id == -1) { fail("op_adapter_linear on host tensors is not provided by this build; move the operands to a GPU"); return nullptr; }
+    if (x->ndim != 2 || w->ndim != 2 || !same_place(x, w) || x->shape[1] != w->shape[0]) { fail("op_adapter_linear: x [rows, in_features] and weight [in_features, out_features] of one dtype and device"); return nullptr; }
+    if (a->ndim != 3 || b->ndim != 3 || !same_place(x, a) || !same_place(x, b) || a->shape[1] != w->shape[0] || b->shape[2] != w->shape[1] || a->shape[0] != b->shape[0] || a->shape[2] != b->shape[1]) {
+        fail("op_adapter_linear: a [adapters, in_features, rank] and b [adapters, rank, out_features] of x's dtype and device");
+        return nullptr;
+    }
+    if (bias && (bias->ndim != 1 || bias->shape[0] != w->shape[1] || !same_place(x, bias) || !rp_is_contiguous(bias))) { fail("op_adapter_linear: bias must be a dense vector of out_features"); return nullptr; }
+    const int rows = x->shape[0], k = x->shape[1], n = w->shape[1], adapters = a->shape[0], rank = a->shape[2];
+    std::vector<int> plan(2 * (size_t)segments + 1 + adapters);
+    long long end = 0;
+    for (int s = 0; s < segments; s++) {
+        if (lengths[s] < 0 || ids[s] < -1 || ids[s] >= adapters) { fail("op_adapter_linear: lengths are not negative, adapters -1 (none) or below %d", adapters); return nullptr; }
+        plan[s] = (int)end;
+        end += lengths[s];
+        plan[segments + 1 + s] = ids[s];
+        if (end > rows) { fail("op_adapter_linear: the segments are longer than the %d rows", rows); return nullptr; }
+    }
+    plan[segments] = (int)end;
+    for (int i = 0; i < adapters; i++) {
+        const float one = scales ? scales[i] : 1.f;
+        memcpy(&plan[2 * (size_t)segments + 1 + i], &one, sizeof(float));
+    }
+    const int shape[2] = {rows, n};
+    Tensor* ad = dense(a); Tensor* bd = dense(b);
+    Tensor* out = ad && bd ? empty_tensor(x->dtype, x->device_id, 2, shape) : nullptr;
+    AdapterSaved* s = (AdapterSaved*)calloc(1, sizeof(AdapterSaved));
+    s->segments = segments; s->device_id = x->device_id;
+    const bool ok = out && on_device(x->device_id) && rp_hip_malloc(&s->plan, sizeof(int) * plan.size()) == 0 && rp_hip_memcpy_h2d(s->plan, plan.data(), sizeof(int) * plan.size()) == 0 &&
+                    rp_hip_malloc(&s->h, dtype_size(weights_dtype(x->dtype)) * (size_t)rows * rank) == 0 &&
+                    rp_hip_adapter_linear_forward(out->data, s->h, x->data, w->data, bias ? bias->data : nullptr, ad->data, bd->data, plan_scales(s), plan_ids(s), plan_offsets(s), segments, adapters, rows, k, n, rank,
+                                                  x->strides[0], x->strides[1], w->strides[0], w->strides[1], n, x->dtype) == 0;
+    free_tensor(ad); free_tensor(bd);
+    if (!ok) { dev_fail("op_adapter_linear"); free_tensor(out); free_adapter_saved(s); return nullptr; }
+    if (needs_grad(x) || needs_grad(w) || needs_grad(a) || needs_grad(b) || needs_grad(bias)) {
+        GradFn* gf = bias ? attach(out, backward_adapter_linear_fn, {x, w, a, b, bias}) : attach(out, backward_adapter_linear_fn, {x, w, a, b});
+        gf->saved_data = s;
+        gf->free_saved = free_adapter_saved;
+    } else {
+        free_adapter_saved(s);
     }
     return out;
 }

@@ -107,6 +107,28 @@ Tensor* op_slice(Tensor* x, int* start, int* stop, int* step);          /* refer
 Tensor* op_lstm_cell(Tensor* x, Tensor* h, Tensor* c, Tensor* w_ih, Tensor* w_hh, Tensor* b_ih, Tensor* b_hh);   /* one step as one node: [B, 2H] = h_next | c_next (extension) */
 Tensor* op_gru_cell(Tensor* x, Tensor* h, Tensor* w_ih, Tensor* w_hh, Tensor* b_ih, Tensor* b_hh);                /* one step as one node: h_next (extension) */
 Tensor* op_attention(Tensor* q, Tensor* k, Tensor* v, double scale);   /* softmax(scale·q·kᵀ)·v in one launch (extension; 16-bit dtypes and float32) */
+/* ---- layers whose weight depends on the row (extensions; device tensors) ---- */
+/* How rows are sent to groups: device arrays that op_route or routing_from_ids fills once and the ops below share.  Reference counted like Tensor. */
+typedef struct {
+    int tokens, k, groups, device_id, refcount;
+    int* experts;                                       /* [tokens * k] group of a slot, -1: none */
+    int* offsets;                                       /* [groups + 1] */
+    int* order;                                         /* [tokens * k] slot of a place, -1 behind the last */
+    int* position;                                      /* [tokens * k] place of a slot, -1: none */
+    void* block;                                        /* what the four lie in */
+} Routing;
+Routing* routing_from_ids(const int* ids, int count, int groups, int device_id);                 /* k = 1; ids outside [0, groups): no group */
+Routing* routing_retain(Routing* routing);
+void free_routing(Routing* routing);
+int routing_read(Routing* routing, int* experts, int* offsets, int* order, int* position);       /* to host arrays, any of which may be NULL */
+Tensor* op_route(Tensor* logits, int k, bool normalize, Routing** routing);                       /* [tokens, groups] -> weights [tokens, k] in float32 (float64) */
+Tensor* op_dispatch(Tensor* x, Routing* routing);                                                 /* [tokens, d] -> [tokens * k, d] in group order */
+Tensor* op_combine(Tensor* z, Tensor* weights, Routing* routing);                                 /* [tokens * k, d], weights [tokens, k] -> [tokens, d] */
+Tensor* op_grouped_linear(Tensor* x, Tensor* w, Tensor* bias, Routing* routing);                  /* [rows, in], [groups, in, out], [groups, out] or NULL */
+/* x·w + bias + scale (x·a)·b, a [adapters, in, rank], b [adapters, rank, out]; the rows are lengths[0] of segment 0, then lengths[1] of segment 1, ...; segment s uses
+ * adapter ids[s], -1: none; scales: host array [adapters] or NULL.  Rows behind the last segment have no adapter. */
+Tensor* op_adapter_linear(Tensor* x, Tensor* w, Tensor* bias, Tensor* a, Tensor* b, const float* scales, const int* ids, const int* lengths, int segments);
+
 Tensor* op_add(Tensor* x1, Tensor* x2);
 Tensor* op_relu(Tensor* x);
 Tensor* op_softmax(Tensor* x, int dim);

@@ -80,3 +80,13 @@ def test_strides():
     refused("rp_hip_grouped_linear_backward", changed(GROUPED_BACK, 17, 63), "rows of dx are 63 elements apart and hold 64")
     refused("rp_hip_adapter_linear_forward", changed(ADAPTER, 20, 71), "rows of y are 71 elements apart and hold 72")
     refused("rp_hip_adapter_linear_backward", changed(ADAPTER_BACK, 24, 63), "rows of dx are 63 elements apart and hold 64")
+
+
+def test_zero_rows_behind():
+    args = (P, P, 4, 10, 64, 64, capi.BF16)
+    for at in (0, 1):
+        refused("rp_hip_zero_rows_behind", changed(args, at, None), "null operand")
+    for at in (2, 3, 4):
+        refused("rp_hip_zero_rows_behind", changed(args, at, 0), "non-positive extent")
+    refused("rp_hip_zero_rows_behind", changed(args, 5, 63), "rows of 63 elements apart hold 64")
+    refused("rp_hip_zero_rows_behind", changed(args, 6, 9), "unsupported dtype")

@@ -262,6 +262,17 @@ def test_exchange(t, k, d, dt):
 
 # ---- the grouped linear layer ----------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("dt", ALL, ids=ids_of)
+@pytest.mark.parametrize("rows, last, width, pad", [(1, 0, 1, 0), (9, 4, 7, 3), (3000, 1, 65, 0), (40, 40, 8, 0), (5, 90, 8, 0), (5, -2, 8, 1)])
+def test_zero_rows_behind(rows, last, width, pad, dt):
+    x = rand_storage(np.random.default_rng(rows), (rows, width + pad), dt)
+    buf = capi.DeviceBuffer.from_numpy(x)
+    call("rp_hip_zero_rows_behind", buf.ptr, ints([0, last]).ptr, 1, rows, width, width + pad, dt)
+    capi.synchronize()
+    x[max(last, 0):, :width] = 0
+    assert np.array_equal(buf.to_numpy(x.dtype, x.shape), x)
+
+
 def grouped_want(x, w, bias, offsets):
     rows, n = x.shape[0], w.shape[2]
     y, size = np.zeros((rows, n)), np.zeros((rows, n))
