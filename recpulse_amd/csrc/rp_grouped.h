@@ -22,6 +22,19 @@ struct GroupedArgs {
     int accumulate;
 };
 
+// Slot `id` of `total` tiles that the eight XCDs take in a run each (workgroup i is XCD i % 8's); past the run's end: `total`
+__device__ __forceinline__ int run_tile(int id, int total) {
+    const int per = (total + 7) / 8, at = id % 8 * per + id / 8;
+    return id / 8 < per && at < total ? at : total;
+}
+// Tile `at` of a matrix of rows x cols tiles: column by column through eight rows of tiles at a time, so that the tiles of a run that are
+// at work together need a few panels of both operands
+__device__ __forceinline__ TileCoord chunk_tile(int at, int rows, int cols) {
+    constexpr int CHUNK = 8;
+    const int r0 = at / (CHUNK * cols) * CHUNK, h = rows - r0 < CHUNK ? rows - r0 : CHUNK, in = at - r0 * cols;
+    return TileCoord{r0 + in % h, in / h, true};
+}
+
 // Which operand is in the accumulate type (float32, float64 for float64) whatever the tensors' type is: the low-rank activations of an adapter
 enum GroupedLow { LOW_NONE = 0, LOW_A = 1, LOW_B = 2, LOW_C = 3 };
 
@@ -31,15 +44,16 @@ int launch_grouped_weights_generic(const GroupedArgs& g, int dtype);
 // The same for an adapter's narrow products (rp_adapter_any.hip): by rows LOW_C, scales taken; by weights LOW_A or LOW_B, ids taken
 int launch_narrow_rows(const GroupedArgs& g, int dtype);
 int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype);
-// out[w, :] (+)= sum over the rows of w's groups of x[i, :]
-int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype);
-
+// out[w, :] (+)= sum over the rows of group w of x[i, :]
+struct GroupedSums;
+int launch_grouped_sums(const GroupedSums& s, int dtype);
 
 // fp32 / fp64 (rp_grouped_wavek.hip), rows of any length and start
 bool grouped_rows_wavek_takes(const GroupedArgs& g, int dtype);
-bool grouped_weights_wavek_takes(const GroupedArgs& g, int dtype);
 int launch_grouped_rows_wavek(const GroupedArgs& g, int dtype);
-int launch_grouped_weights_wavek(const GroupedArgs& g, int dtype);
+// the gradients in one launch: those of x, w and sums whose output is not null
+bool grouped_backward_wavek_takes(const GroupedArgs& x, const GroupedArgs& w, int dtype);
+int launch_grouped_backward_wavek(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int dtype);
 
 // bf16 / fp16 on the tiles of the 16-bit MFMA kernel (rp_grouped_mfma16*.hip).  ragged: rows of any length and start.
 int launch_grouped_rows16_256_bf16(const GroupedArgs& g);
@@ -50,6 +64,9 @@ int launch_grouped_rows16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
+// The gradients in one launch on tiles of 64 or 128: those of x, w and sums whose output is not null; w row-major (rp_grouped_backward16*.hip)
+int launch_grouped_backward16_bf16(const GroupedArgs& x, const GroupedArgs& w, int edge, const GroupedSums& sums, bool ragged);
+int launch_grouped_backward16_f16(const GroupedArgs& x, const GroupedArgs& w, int edge, const GroupedSums& sums, bool ragged);
 
 // + h[i] . b_a for the rows i of adapter a: what a layer's adapters add to its shared product (strides of b in elements)
 struct AdapterTerm {

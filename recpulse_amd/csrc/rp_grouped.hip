@@ -4,7 +4,7 @@
 // Adapters, a the adapter of row i's segment:  h[i] = s_a x[i] . A_a,  y[i] = x[i] . W + b + h[i] . B_a;
 //   u[i] = s_a dy[i] . B_a^T,  dx[i] = dy[i] . W^T + u[i] . A_a^T,  dA_a = sum x[i]^T u[i],  dB_a = sum h[i]^T dy[i].
 // h and u are in the accumulate type (float32, float64 for float64): they are sums that are multiplied on.
-#include "rp_grouped.h"
+#include "rp_grouped_sums.h"
 
 namespace rp {
 
@@ -23,33 +23,64 @@ static Lie lies(const void* p, long long row_stride, long long weight_stride, in
 }
 static Lie worse(Lie a, Lie b) { return a > b ? a : b; }
 
+// Tiles of the 16-bit products: their edge, 0 for none, and how the operands lie
+struct Tile16 { int edge; bool ragged; };
+
+static Tile16 rows_tile16(const GroupedArgs& g, int dtype) {
+    if (!is16(dtype) || g.a_cs != 1 || (g.b_cs != 1 && g.b_rs != 1) || path_disabled("mfma")) return {0, false};
+    const bool b_mc = g.b_cs == 1;
+    const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
+    if (lie == LIE_NEITHER) return {0, false};
+    const long long tiles256 = (long long)((g.gr.rows + 255) / 256) * ((g.n + 255) / 256), tiles128 = (long long)((g.gr.rows + 127) / 128) * ((g.n + 127) / 128);
+    const int mean = g.gr.rows / g.gr.groups;
+    // 128 x 128 tiles from three quarters of a round of the CUs on (bf16, 519 -> 1031, us on 64 and 128: 1999 rows of 6 groups, 144 tiles, 14.5 / 15.2; 4096 of 8, 288 tiles, 23.1 / 19.7)
+    if (lie == LIE_WHOLE && mean >= 256 && g.n >= 256 && g.k >= 256 && tiles256 >= cus() / 2) return {256, false};
+    return {mean >= 96 && g.n > 64 && tiles128 * 4 >= cus() * 3 ? 128 : 64, lie == LIE_RAGGED};
+}
+
+static Tile16 weights_tile16(const GroupedArgs& g, int dtype) {
+    if (!is16(dtype) || g.a_cs != 1 || g.b_cs != 1 || path_disabled("mfma")) return {0, false};
+    const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
+    if (lie == LIE_NEITHER) return {0, false};
+    const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
+    if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && tiles256 >= cus() / 2) return {256, false};
+    return {g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? 128 : 64, lie == LIE_RAGGED};
+}
+
 static int grouped_rows(const GroupedArgs& g, int dtype) {
     if (is16(dtype) && grouped_stream16_takes(g)) return launch_grouped_stream16(g, dtype);
-    if (is16(dtype) && g.a_cs == 1 && (g.b_cs == 1 || g.b_rs == 1) && !path_disabled("mfma")) {
-        const bool b_mc = g.b_cs == 1;
-        const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
-        const long long tiles256 = (long long)((g.gr.rows + 255) / 256) * ((g.n + 255) / 256), tiles128 = (long long)((g.gr.rows + 127) / 128) * ((g.n + 127) / 128);
-        const int mean = g.gr.rows / g.gr.groups;
-        if (lie == LIE_WHOLE && mean >= 256 && g.n >= 256 && g.k >= 256 && tiles256 >= cus() / 2)
-            return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_rows16_256_bf16(g) : launch_grouped_rows16_256_f16(g);
-        if (lie != LIE_NEITHER)
-            return mean >= 96 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_rows16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_rows16_64(g, lie == LIE_RAGGED, dtype);
-    }
+    const Tile16 t = rows_tile16(g, dtype);
+    if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_rows16_256_bf16(g) : launch_grouped_rows16_256_f16(g);
+    if (t.edge) return t.edge == 128 ? launch_grouped_rows16_128(g, t.ragged, dtype) : launch_grouped_rows16_64(g, t.ragged, dtype);
     if (!is16(dtype) && grouped_rows_wavek_takes(g, dtype)) return launch_grouped_rows_wavek(g, dtype);
     return launch_grouped_rows_generic(g, false, dtype);
 }
 
 static int grouped_weights(const GroupedArgs& g, int dtype) {
-    if (is16(dtype) && g.a_cs == 1 && g.b_cs == 1 && !path_disabled("mfma")) {
-        const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
-        const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
-        if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && tiles256 >= cus() / 2)
-            return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_weights16_256_bf16(g) : launch_grouped_weights16_256_f16(g);
-        if (lie != LIE_NEITHER)
-            return g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? launch_grouped_weights16_128(g, lie == LIE_RAGGED, dtype) : launch_grouped_weights16_64(g, lie == LIE_RAGGED, dtype);
-    }
-    if (!is16(dtype) && grouped_weights_wavek_takes(g, dtype)) return launch_grouped_weights_wavek(g, dtype);
+    const Tile16 t = weights_tile16(g, dtype);
+    if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_weights16_256_bf16(g) : launch_grouped_weights16_256_f16(g);
+    if (t.edge) return t.edge == 128 ? launch_grouped_weights16_128(g, t.ragged, dtype) : launch_grouped_weights16_64(g, t.ragged, dtype);
     return launch_grouped_weights_generic(g, dtype);
+}
+
+// The gradients of one layer in one launch unless 256 x 256 tiles, whose workgroups stay on their CU, take one of them.  bf16, us, in launches of their own and in
+// one: 1999 rows of 6 groups, 519 -> 1031, 41 / 23; 4096 of 8 56 / 32; 8192 of 8, 1031 -> 2047, 187 / 150.  One tile edge for both, 128 from a round of the CUs on
+// (64 and 128: 3000 rows of 4 groups, 700 -> 1031, 360 tiles of 128, 32 / 25; 1999 of 6, 350 tiles, 23 / 23).
+static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int dtype, int* result) {
+    if (!x.C && !w.C) return false;
+    if (!is16(dtype)) {
+        const bool takes = grouped_backward_wavek_takes(x, w, dtype);
+        if (takes) *result = launch_grouped_backward_wavek(x, w, sums, dtype);
+        return takes;
+    }
+    if (!x.C + !w.C + !sums.out > 1 || (x.C && (grouped_stream16_takes(x) || x.b_rs != 1)) || path_disabled("grouped_backward")) return false;
+    const Tile16 tx = x.C ? rows_tile16(x, dtype) : Tile16{64, false}, tw = w.C ? weights_tile16(w, dtype) : Tile16{64, false};
+    if (!tx.edge || !tw.edge || tx.edge == 256 || tw.edge == 256) return false;
+    const bool ragged = tx.ragged || tw.ragged;
+    const long long tiles128 = (x.C ? (long long)((x.gr.rows + 127) / 128) * ((x.n + 127) / 128) : 0) + (w.C ? (long long)((w.k + 127) / 128) * ((w.n + 127) / 128) * w.gr.weights : 0);
+    const int edge = tiles128 >= cus() ? 128 : 64;
+    *result = dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_backward16_bf16(x, w, edge, sums, ragged) : launch_grouped_backward16_f16(x, w, edge, sums, ragged);
+    return true;
 }
 
 // An adapter's narrow product (C is h or u) and the gradients of its factors
@@ -113,10 +144,18 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
     if (!grouped_args_ok(who, dy && offsets && (!dx || w) && (!dw || x), groups, rows, k, n, {dy_rs, x_rs, x_cs, w_gs, w_rs, w_cs, dx_rs}, dtype)) return -1;
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, nullptr, groups, rows, groups};
-    if (dx && grouped_rows(GroupedArgs{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0}, dtype) != 0) return -1;
-    if (dw && grouped_weights(GroupedArgs{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0}, dtype) != 0) return -1;
-    if (db && launch_grouped_sums(db, dy, gr, n, dy_rs, accumulate_db, dtype) != 0) return -1;
-    return 0;
+    GroupedArgs xg{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
+    const GroupedArgs wg{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0};
+    const GroupedSums sums{db, dy, gr, n, accumulate_db, dy_rs};
+    int result;
+    if (backward_together(xg, wg, sums, dtype, &result)) return result;
+    if (dx) {
+        if (grouped_rows(xg, dtype) != 0) return -1;
+        xg.C = nullptr;
+        if (backward_together(xg, wg, sums, dtype, &result)) return result;
+    }
+    if (dw && grouped_weights(wg, dtype) != 0) return -1;
+    return db ? launch_grouped_sums(sums, dtype) : 0;
 }
 
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,

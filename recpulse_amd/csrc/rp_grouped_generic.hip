@@ -2,7 +2,7 @@
 // thread.  What no other kernel takes comes here: the narrowest widths, operands without a unit stride, and the adapters' term of
 // float32 and float64, whose rank is a few steps of k.  Sums in the accumulate type, rounded at the end, and once more where they are added to what the
 // output holds (as a product of its own would be).
-#include "rp_grouped.h"
+#include "rp_grouped_sums.h"
 
 #include <type_traits>
 
@@ -93,27 +93,10 @@ __global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArg
         }
 }
 
-// Column sums: 64 columns a workgroup, four rows at a time, the four partial sums added in order
 template <typename T>
-__global__ void __launch_bounds__(256) grouped_sums_kernel(T* out, const T* x, RowGroups gr, int cols, long long x_rs, int accumulate, int strips) {
-    using A = typename traits<T>::acc;
-    __shared__ A parts[4][64];
-    const int strip = (int)(blockIdx.x % strips), w = (int)(blockIdx.x / strips);
-    const int c = strip * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    A sum = 0;
-    if (c < cols) {
-        const int e = gr.end(w);
-#pragma unroll 8
-        for (int i = gr.begin(w) + q; i < e; i += 4) sum += widen(x[i * x_rs + c]);
-    }
-    parts[q][threadIdx.x & 63] = sum;
-    __syncthreads();
-    if (q || c >= cols) return;
-    A v = ((parts[0][threadIdx.x] + parts[1][threadIdx.x]) + parts[2][threadIdx.x]) + parts[3][threadIdx.x];
-    T* p = out + (long long)w * cols + c;
-    T y = round_to<T>(v);
-    if (accumulate) y = round_to<T>(widen(*p) + widen(y));
-    *p = y;
+__global__ void __launch_bounds__(1024) grouped_sums_kernel(GroupedSums s) {
+    __shared__ typename traits<T>::acc parts[16 * 64];
+    grouped_sums_block<T, 16>(s, (int)blockIdx.x, parts);
 }
 
 static bool grid_ok(long long blocks, const char* what) {
@@ -141,11 +124,10 @@ int launch_grouped_weights_generic(const GroupedArgs& g, int dtype) {
     return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
 }
 
-int launch_grouped_sums(void* out, const void* x, const RowGroups& gr, int cols, long long x_rs, int accumulate, int dtype) {
-    const int strips = (cols + 63) / 64;
-    const long long blocks = (long long)gr.weights * strips;
+int launch_grouped_sums(const GroupedSums& s, int dtype) {
+    const long long blocks = sum_blocks(s);
     if (!grid_ok(blocks, "grouped bias gradient")) return -1;
-    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, current_stream(), (T*)out, (const T*)x, gr, cols, x_rs, accumulate, strips));
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)blocks), dim3(1024), 0, current_stream(), s));
     return check_launch("grouped_sums_kernel") ? 0 : -1;
 }
 

@@ -6,26 +6,28 @@
 
 namespace rp {
 
-// By rows: row tiles never span two groups.  How many there are is known on the device only; the row tiles of all groups are scheduled
-// as if they were one matrix's, so that an XCD's workgroups share a few row panels and a few weight panels at a time.
+// By rows: row tiles never span two groups, and how many there are is known on the device only.  All groups' tiles are one list, group by group.
 template <int BM>
 struct GroupedRowTiles {
     static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     RowTiles rows;
-    int tiles_n;
-    __device__ __forceinline__ GroupedRowTiles(const GroupedArgs& g, int tn) : ga(g), rows(g.gr, BM), tiles_n(tn) {}
+    int tiles_n, total;
+    __device__ __forceinline__ GroupedRowTiles(const GroupedArgs& g, int tn) : ga(g), rows(g.gr, BM), tiles_n(tn), total(rows.total * tn) {}
+    __device__ __forceinline__ int slots() const { return (total + 7) / 8 * 8; }
     __device__ __forceinline__ TileCoord tile(int id, GemmArgs& g) const {
-        TileCoord tc = schedule_tile(id, rows.total, tiles_n);
-        if (!tc.valid) return tc;
-        const RowTile rt = rows.find(tc.tm);
-        g.A = (const uint16_t*)ga.A + rt.begin * ga.a_rs;
+        const int at = run_tile(id, total);
+        if (at == total) return TileCoord{0, 0, false};
+        const int row = at / tiles_n;
+        const RowTile rt = rows.find(row);
+        const TileCoord in = chunk_tile(at - rt.first * tiles_n, rt.tiles, tiles_n);
+        const int begin = rt.begin + (in.tm - (row - rt.first)) * BM;
+        g.A = (const uint16_t*)ga.A + begin * ga.a_rs;
         g.B = (const uint16_t*)ga.B + rt.weight * ga.b_ws;
-        g.C = (uint16_t*)ga.C + rt.begin * ga.c_rs;
+        g.C = (uint16_t*)ga.C + begin * ga.c_rs;
         g.bias = ga.bias ? (const uint16_t*)ga.bias + (long long)rt.weight * ga.n : nullptr;
-        g.m = rt.end - rt.begin;
-        tc.tm = 0;
-        return tc;
+        g.m = begin + BM < rt.stop ? BM : rt.stop - begin;
+        return TileCoord{0, in.tn, true};
     }
 };
 
@@ -33,26 +35,26 @@ template <typename T, int BM, int BN, int WGM, bool B_MC, int EDGE>
 __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) grouped_rows16_kernel(GroupedArgs ga, int tiles_n) {
     GroupedRowTiles<BM> source(ga, tiles_n);
     GemmArgs g{nullptr, nullptr, nullptr, nullptr, 1, 0, ga.k, ga.n, 0, ga.a_rs, ga.a_cs, 0, ga.b_rs, ga.b_cs, 0, ga.c_rs, 1, ga.accumulate};
-    gemm_mfma16_block<T, BM, BN, WGM, false, B_MC, EDGE, false, 1, GroupedRowTiles<BM>>(g, 0, 0, nullptr, 0, scheduled_grid(source.rows.total, tiles_n), (int)blockIdx.x, 0,
+    gemm_mfma16_block<T, BM, BN, WGM, false, B_MC, EDGE, false, 1, GroupedRowTiles<BM>>(g, 0, 0, nullptr, 0, source.slots(), (int)blockIdx.x, 0,
                                                                                        (int)gridDim.x, &source);
 }
 
-// By weights: tile for tile the same in every group, so that resident workgroups, each with one tile of every group in turn, all do the
-// same work however uneven the groups are.  The reduction runs over the group's rows; an empty group leaves zeros.
+// By weights: tile for tile the same in every group, each group's tiles a run for each XCD, so that resident workgroups, each with one tile
+// of every group in turn, all do the same work however uneven the groups are.  The reduction runs over the group's rows; an empty group leaves zeros.
 struct GroupedWeightTiles {
     static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     int tiles_k, tiles_n, slots;
     __device__ __forceinline__ TileCoord tile(int id, GemmArgs& g) const {
         const int w = id / slots;
-        const TileCoord tc = schedule_tile(id - w * slots, tiles_k, tiles_n);
-        if (!tc.valid) return tc;
+        const int at = run_tile(id - w * slots, tiles_k * tiles_n);
+        if (at == tiles_k * tiles_n) return TileCoord{0, 0, false};
         const int b = __builtin_amdgcn_readfirstlane(ga.gr.begin(w)), e = __builtin_amdgcn_readfirstlane(ga.gr.end(w));
         g.A = (const uint16_t*)ga.A + b * ga.a_rs;
         g.B = (const uint16_t*)ga.B + b * ga.b_rs;
         g.C = (uint16_t*)ga.C + w * ga.c_ws;
         g.k = e - b;
-        return tc;
+        return chunk_tile(at, tiles_k, tiles_n);
     }
 };
 
@@ -85,7 +87,7 @@ static int launch_grouped_rows16(const GroupedArgs& g) {
 
 template <typename T, int BM, int BN, int WGM, int EDGE>
 static int launch_grouped_weights16(const GroupedArgs& g) {
-    const int tiles_k = (g.k + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN, slots = scheduled_grid(tiles_k, tiles_n);
+    const int tiles_k = (g.k + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN, slots = (int)(((long long)tiles_k * tiles_n + 7) / 8 * 8);
     const long long total = (long long)slots * g.gr.weights;
     if (total > 0x3fffffff) { set_error("grouped weight gradient: %lld tiles are more than a launch takes", total); return -1; }
     constexpr size_t smem = m16_smem_bytes(BM, BN, WGM, true, true, 2, m16_mfma_tile(BM, BN));

@@ -1,39 +1,63 @@
 // Grouped products of fp32 / fp64: the workgroups of one product whose waves share k (rp_gemm_wavekw.h), which take their tiles from the groups.
 //
-// By rows a tile lies in one group; how many row tiles there are is known on the device only, and all of them times the column tiles are dealt
+// By rows a tile lies in one group; how many row tiles there are is known on the device only, and the list of all groups' tiles is dealt
 // to the XCDs in eight runs, so that the tiles of a group share its weight in one L2.  By weights the reduction runs over the group's
 // rows.  Rows may start at any element.  The tile is the largest whose tiles occupy three quarters of the CUs, as for one product:
 // small layers are bound by launch and latency (k goes to eight waves), 64 x 64 tiles of fp32 by the MFMAs.
-// fp32, us, on scalar multiply-adds and here: WAVEK_FIGURES
+// fp32, us, on scalar multiply-adds and here: 1024 rows of 4 groups, 784 -> 256, forward 43 / 12; its three gradients together 100 / 22
+// (in launches of their own 28).  4096 rows of 8 groups, 1024 -> 1024: forward 122, 71 TFLOP/s, gradients 223.
 #include "rp_gemm_wavekw.h"
-#include "rp_grouped.h"
+#include "rp_grouped_sums.h"
 
 namespace rp {
 
 constexpr int GW_WAVES = 8;
 constexpr int gw_waves_per_simd(int tiles) { return tiles <= 4 ? 4 : 2; }
 
+// One tile in the block's own order of a matrix of one tile
 template <typename E, bool B_KC, int TM, int TN>
-__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(TM * TN)) grouped_rows_wavek_kernel(GroupedArgs ga, int tiles_n) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char wkw_lds[];
+__device__ __forceinline__ void rows_block(const GroupedArgs& ga, int tiles_n, int id, unsigned char* lds) {
     const RowTiles rows(ga.gr, 16 * TM);
-    const int total = rows.total * tiles_n, per = (total + 7) / 8, at = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= per || at >= total) return;
-    const RowTile rt = rows.find(at / tiles_n);
-    const GemmArgs g{(E*)ga.C + rt.begin * ga.c_rs, (const E*)ga.A + rt.begin * ga.a_rs, (const E*)ga.B + rt.weight * ga.b_ws, ga.bias ? (const E*)ga.bias + (long long)rt.weight * ga.n : nullptr,
-                     1, rt.end - rt.begin, ga.k, ga.n, 0, ga.a_rs, 1, 0, B_KC ? 1 : ga.b_rs, B_KC ? ga.b_cs : 1, 0, ga.c_rs, 1, ga.accumulate};
+    const int total = rows.total * tiles_n, at = run_tile(id, total);
+    if (at == total) return;
+    const int row = at / tiles_n;
+    const RowTile rt = rows.find(row);
+    const TileCoord in = chunk_tile(at - rt.first * tiles_n, rt.tiles, tiles_n);
+    const int begin = rt.begin + (in.tm - (row - rt.first)) * 16 * TM;
+    const GemmArgs g{(E*)ga.C + begin * ga.c_rs, (const E*)ga.A + begin * ga.a_rs, (const E*)ga.B + rt.weight * ga.b_ws, ga.bias ? (const E*)ga.bias + (long long)rt.weight * ga.n : nullptr,
+                     1, begin + 16 * TM < rt.stop ? 16 * TM : rt.stop - begin, ga.k, ga.n, 0, ga.a_rs, 1, 0, B_KC ? 1 : ga.b_rs, B_KC ? ga.b_cs : 1, 0, ga.c_rs, 1, ga.accumulate};
     // (the block that its schedule gives this column tile)
-    const int tn = at % tiles_n, share = (tiles_n + 7) / 8;
-    gemm_wavekw_block<E, true, B_KC, TM, TN, GW_WAVES>(g, 1, tiles_n, tn % share * 8 + tn / share, 1, wkw_lds);
+    const int share = (tiles_n + 7) / 8;
+    gemm_wavekw_block<E, true, B_KC, TM, TN, GW_WAVES>(g, 1, tiles_n, in.tn % share * 8 + in.tn / share, 1, lds);
 }
 
 template <typename E, int TM, int TN>
-__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(TM * TN)) grouped_weights_wavek_kernel(GroupedArgs ga, int tiles_k, int tiles_n, int slots) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char wkw_lds[];
-    const int w = (int)blockIdx.x / slots, b = __builtin_amdgcn_readfirstlane(ga.gr.begin(w)), e = __builtin_amdgcn_readfirstlane(ga.gr.end(w));
+__device__ __forceinline__ void weights_block(const GroupedArgs& ga, int tiles_k, int tiles_n, int slots, int id, unsigned char* lds) {
+    const int w = id / slots, b = __builtin_amdgcn_readfirstlane(ga.gr.begin(w)), e = __builtin_amdgcn_readfirstlane(ga.gr.end(w));
     const GemmArgs g{(E*)ga.C + w * ga.c_ws, (const E*)ga.A + b * ga.a_rs, (const E*)ga.B + b * ga.b_rs, nullptr,
                      1, ga.k, e - b, ga.n, 0, 1, ga.a_rs, 0, ga.b_rs, 1, 0, ga.c_rs, 1, ga.accumulate};
-    gemm_wavekw_block<E, false, false, TM, TN, GW_WAVES>(g, tiles_k, tiles_n, (int)blockIdx.x - w * slots, 1, wkw_lds);
+    gemm_wavekw_block<E, false, false, TM, TN, GW_WAVES>(g, tiles_k, tiles_n, id - w * slots, 1, lds);
+}
+
+template <typename E, bool B_KC, int TM, int TN>
+__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(TM * TN)) grouped_rows_wavek_kernel(GroupedArgs ga, int tiles_n) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char wkw_lds[];
+    rows_block<E, B_KC, TM, TN>(ga, tiles_n, (int)blockIdx.x, wkw_lds);
+}
+
+// The input's gradient, the weights' and the bias's, as many of them as there are blocks for
+template <typename E, int T>
+__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(T * T)) grouped_backward_wavek_kernel(GroupedArgs x, GroupedArgs w, GroupedSums sums, int s_blocks, int x_blocks, int x_tiles_n,
+                                                                                                      int w_tiles_k, int w_tiles_n, int w_slots) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char wkw_lds[];
+    const int id = (int)blockIdx.x;
+    if (id < s_blocks) {
+        if (id < sums.gr.weights * ((sums.cols + 63) / 64)) grouped_sums_block<E, GW_WAVES>(sums, id, (E*)wkw_lds);
+    } else if (id - s_blocks < x_blocks) {
+        rows_block<E, true, T, T>(x, x_tiles_n, id - s_blocks, wkw_lds);
+    } else {
+        weights_block<E, T, T>(w, w_tiles_k, w_tiles_n, w_slots, id - s_blocks - x_blocks, wkw_lds);
+    }
 }
 
 template <typename E, bool B_KC, int TM, int TN>
@@ -47,14 +71,18 @@ static int launch_rows(const GroupedArgs& g) {
     return check_launch("grouped_rows_wavek_kernel") ? 0 : -1;
 }
 
-template <typename E, int TM, int TN>
-static int launch_weights(const GroupedArgs& g) {
-    constexpr size_t smem = wkw_smem<E, false, false, TM, TN, GW_WAVES>();
-    const int tiles_k = (g.k + 16 * TM - 1) / (16 * TM), tiles_n = (g.n + 16 * TN - 1) / (16 * TN), slots = (tiles_k * tiles_n + 7) / 8 * 8;
-    auto kern = grouped_weights_wavek_kernel<E, TM, TN>;
+template <typename E, int T>
+static int launch_backward(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums) {
+    constexpr size_t smem_x = wkw_smem<E, true, true, T, T, GW_WAVES>(), smem_w = wkw_smem<E, false, false, T, T, GW_WAVES>(), most = smem_x > smem_w ? smem_x : smem_w;
+    constexpr size_t smem = most > 64 * 16 * sizeof(E) ? most : 64 * 16 * sizeof(E);
+    const int x_tiles_n = (x.n + 16 * T - 1) / (16 * T), w_tiles_k = (w.k + 16 * T - 1) / (16 * T), w_tiles_n = (w.n + 16 * T - 1) / (16 * T), w_slots = (w_tiles_k * w_tiles_n + 7) / 8 * 8;
+    const long long x_blocks = x.C ? (max_row_tiles(x.gr.rows, x.gr.groups, 16 * T) * x_tiles_n + 7) / 8 * 8 : 0, w_blocks = w.C ? (long long)w_slots * w.gr.weights : 0;
+    const long long s_blocks = sums.out ? (sum_blocks(sums) + 7) / 8 * 8 : 0;
+    auto kern = grouped_backward_wavek_kernel<E, T>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long long)slots * g.gr.weights)), dim3(64 * GW_WAVES), smem, current_stream(), g, tiles_k, tiles_n, slots);
-    return check_launch("grouped_weights_wavek_kernel") ? 0 : -1;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(s_blocks + x_blocks + w_blocks)), dim3(64 * GW_WAVES), smem, current_stream(), x, w, sums, (int)s_blocks, (int)x_blocks, x_tiles_n,
+                       w_tiles_k, w_tiles_n, w_slots);
+    return check_launch("grouped_backward_wavek_kernel") ? 0 : -1;
 }
 
 constexpr long long GW_MAX_BLOCKS = (1ll << 32) / (64 * GW_WAVES) - 8;       // fewer than 2^32 threads a launch
@@ -68,24 +96,38 @@ static int wavek_tile(int dtype, Tiles tiles, Fits fits) {
     return fits(1) && tiles(1) <= GW_MAX_BLOCKS ? 1 : 0;
 }
 
-static int rows_tile(const GroupedArgs& g, int dtype) {
+// The operands of a product can be addressed: unit strides, 32-bit byte offsets from a tile's first row
+static bool rows_ok(const GroupedArgs& g, int dtype) {
     const long long esz = (long long)dtype_size(dtype), limit = 1ll << 31;
     const bool b_kc = g.b_cs != 1;
-    if (g.a_cs != 1 || (b_kc && g.b_rs != 1) || path_disabled("mfma")) return 0;
-    if ((63 * g.a_rs + g.k) * esz >= limit || (b_kc ? 63 * g.b_cs + g.k : (g.k - 1) * g.b_rs + 64) * esz >= limit) return 0;      // 32-bit byte offsets from a tile's first row
-    return wavek_tile(dtype, [&](int t) { return (max_row_tiles(g.gr.rows, g.gr.groups, 16 * t)) * ((g.n + 16 * t - 1) / (16 * t)); }, [&](int t) { return b_kc || g.n >= 16 * t; });
+    if (g.a_cs != 1 || (b_kc && g.b_rs != 1) || path_disabled("mfma")) return false;
+    return (63 * g.a_rs + g.k) * esz < limit && (b_kc ? 63 * g.b_cs + g.k : (g.k - 1) * g.b_rs + 64) * esz < limit;
 }
-
-static int weights_tile(const GroupedArgs& g, int dtype) {
+static bool weights_ok(const GroupedArgs& g, int dtype) {
     const long long esz = (long long)dtype_size(dtype), limit = 1ll << 31;
-    if (g.a_cs != 1 || g.b_cs != 1 || g.gr.ids || path_disabled("mfma")) return 0;
-    if (((long long)(g.gr.rows - 1) * g.a_rs + 64) * esz >= limit || ((long long)(g.gr.rows - 1) * g.b_rs + 64) * esz >= limit) return 0;
-    return wavek_tile(dtype, [&](int t) { return (long long)g.gr.weights * (((long long)((g.k + 16 * t - 1) / (16 * t)) * ((g.n + 16 * t - 1) / (16 * t)) + 7) / 8 * 8); },
-                      [&](int t) { return g.k >= 16 * t && g.n >= 16 * t; });
+    if (g.a_cs != 1 || g.b_cs != 1 || g.gr.ids || path_disabled("mfma")) return false;
+    return ((long long)(g.gr.rows - 1) * g.a_rs + 64) * esz < limit && ((long long)(g.gr.rows - 1) * g.b_rs + 64) * esz < limit;
+}
+static long long rows_tiles(const GroupedArgs& g, int t) { return max_row_tiles(g.gr.rows, g.gr.groups, 16 * t) * ((g.n + 16 * t - 1) / (16 * t)); }
+static long long weights_tiles(const GroupedArgs& g, int t) { return (long long)g.gr.weights * (((long long)((g.k + 16 * t - 1) / (16 * t)) * ((g.n + 16 * t - 1) / (16 * t)) + 7) / 8 * 8); }
+
+static int rows_tile(const GroupedArgs& g, int dtype) {
+    return rows_ok(g, dtype) ? wavek_tile(dtype, [&](int t) { return rows_tiles(g, t); }, [&](int t) { return g.b_cs != 1 || g.n >= 16 * t; }) : 0;
+}
+// One tile edge for both gradients, whichever of them (C not null) are asked for: they have the same bits alone and together
+static int backward_tile(const GroupedArgs& x, const GroupedArgs& w, int dtype) {
+    if ((x.C && (x.b_cs == 1 || !rows_ok(x, dtype))) || (w.C && !weights_ok(w, dtype))) return 0;
+    return wavek_tile(dtype, [&](int t) { return rows_tiles(x, t) + weights_tiles(w, t) + 16 + (long long)w.gr.weights * ((w.n + 63) / 64); }, [&](int t) { return w.k >= 16 * t && w.n >= 16 * t; });
 }
 
 bool grouped_rows_wavek_takes(const GroupedArgs& g, int dtype) { return rows_tile(g, dtype) != 0; }
-bool grouped_weights_wavek_takes(const GroupedArgs& g, int dtype) { return weights_tile(g, dtype) != 0; }
+bool grouped_backward_wavek_takes(const GroupedArgs& x, const GroupedArgs& w, int dtype) { return backward_tile(x, w, dtype) != 0; }
+
+int launch_grouped_backward_wavek(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int dtype) {
+    const int t = backward_tile(x, w, dtype);
+    if (dtype == RP_DTYPE_FLOAT64) return t == 2 ? launch_backward<double, 2>(x, w, sums) : launch_backward<double, 1>(x, w, sums);
+    return t == 4 ? launch_backward<float, 4>(x, w, sums) : t == 2 ? launch_backward<float, 2>(x, w, sums) : launch_backward<float, 1>(x, w, sums);
+}
 
 template <typename E, int T>
 static int launch_rows_layout(const GroupedArgs& g) { return g.b_cs == 1 ? launch_rows<E, false, T, T>(g) : launch_rows<E, true, T, T>(g); }
@@ -94,12 +136,6 @@ int launch_grouped_rows_wavek(const GroupedArgs& g, int dtype) {
     const int t = rows_tile(g, dtype);
     if (dtype == RP_DTYPE_FLOAT64) return t == 2 ? launch_rows_layout<double, 2>(g) : launch_rows_layout<double, 1>(g);
     return t == 4 ? launch_rows_layout<float, 4>(g) : t == 2 ? launch_rows_layout<float, 2>(g) : launch_rows_layout<float, 1>(g);
-}
-
-int launch_grouped_weights_wavek(const GroupedArgs& g, int dtype) {
-    const int t = weights_tile(g, dtype);
-    if (dtype == RP_DTYPE_FLOAT64) return t == 2 ? launch_weights<double, 2, 2>(g) : launch_weights<double, 1, 1>(g);
-    return t == 4 ? launch_weights<float, 4, 4>(g) : t == 2 ? launch_weights<float, 2, 2>(g) : launch_weights<float, 1, 1>(g);
 }
 
 }  // namespace rp

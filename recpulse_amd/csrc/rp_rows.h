@@ -41,7 +41,8 @@ static inline long long max_row_tiles(long long rows, long long groups, int tile
 
 // Tile number `id` of the groups' row tiles, found by the whole wave together: 64 groups at a time, a lane each, their tile counts added up
 // across the lanes.  All results are wave-uniform.
-struct RowTile { int group, weight, begin, end; };       // rows [begin, end) of `group`; group < 0: there is no such tile
+// rows [begin, end) of `group`, which ends at row `stop` and whose `tiles` tiles begin with number `first`; group < 0: there is no such tile
+struct RowTile { int group, weight, begin, end, stop, first, tiles; };
 __device__ __forceinline__ int wave_prefix_sum(int v, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -62,18 +63,19 @@ __device__ __forceinline__ RowTile find_row_tile(const RowGroups& gr, int tile, 
         const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > id);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const int first = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l);
             RowTile t;
+            t.tiles = __builtin_amdgcn_readlane(tiles, l);
+            t.first = __builtin_amdgcn_readlane(upto, l) - t.tiles;
             t.group = g0 + l;
             t.weight = __builtin_amdgcn_readlane(w, l);
-            t.begin = __builtin_amdgcn_readlane(b, l) + (id - first) * tile;
-            const int end = __builtin_amdgcn_readlane(e, l);
-            t.end = t.begin + tile < end ? t.begin + tile : end;
+            t.begin = __builtin_amdgcn_readlane(b, l) + (id - t.first) * tile;
+            t.stop = __builtin_amdgcn_readlane(e, l);
+            t.end = t.begin + tile < t.stop ? t.begin + tile : t.stop;
             return t;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
     }
-    return RowTile{-1, -1, 0, 0};
+    return RowTile{-1, -1, 0, 0, 0, 0, 0};
 }
 
 // The same for a workgroup that looks up many tiles: up to 64 groups are read and added up once and kept a lane each.
@@ -96,11 +98,11 @@ struct RowTiles {
     __device__ __forceinline__ RowTile find(int id) const {
         if (gr.groups > 64) return find_row_tile(gr, tile, id);
         const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > id);
-        if (!past) return RowTile{-1, -1, 0, 0};
+        if (!past) return RowTile{-1, -1, 0, 0, 0, 0, 0};
         const int l = __builtin_ctzll(past);
-        const int first = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l);
-        const int begin = __builtin_amdgcn_readlane(b, l) + (id - first) * tile, end = __builtin_amdgcn_readlane(e, l);
-        return RowTile{l, __builtin_amdgcn_readlane(w, l), begin, begin + tile < end ? begin + tile : end};
+        const int count = __builtin_amdgcn_readlane(tiles, l), first = __builtin_amdgcn_readlane(upto, l) - count;
+        const int begin = __builtin_amdgcn_readlane(b, l) + (id - first) * tile, stop = __builtin_amdgcn_readlane(e, l);
+        return RowTile{l, __builtin_amdgcn_readlane(w, l), begin, begin + tile < stop ? begin + tile : stop, stop, first, count};
     }
 };
 
