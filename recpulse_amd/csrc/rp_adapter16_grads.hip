@@ -1,8 +1,8 @@
 // bf16 / fp16 gradients of an adapter's factors: D_a = sum over the rows i of adapter a of low[i]^T . s[i], low [rows, rank] in float32, s [rows, width].
 // With low = h and s = dy this is dB_a [rank, n]; with low = u and s = x it is dA_a^T, stored transposed.
 //
-// Bound by reading s, once per 32 of the rank: a workgroup owns one adapter, a strip of 128 columns of s and up to 32 of the rank, and its eight
-// waves share the rows of the adapter's segments, 32 at a time in turn.  s goes from memory to registers to v_mfma_f32_16x16x32 as a
+// Bound by reading s, once per 32 of the rank: a workgroup owns one adapter, a strip of 128 columns of s and up to 32 of the rank, and its waves
+// share the rows of the adapter's segments, 32 at a time in turn.  s goes from memory to registers to v_mfma_f32_16x16x32 as a
 // weight does in the kernel for few rows (rp_grouped_stream16.h): a lane transposes 8 rows x 8 columns with byte permutes.  low is
 // rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, and values beyond 65504 overflow), a product each: h and u are
 // sums in float32, and one rounding of theirs would be as large as the result's own.
@@ -13,12 +13,25 @@ namespace rp {
 
 constexpr int AG_COLS = 128, AG_PITCH = AG_COLS + 4;
 
+struct AdapterGrad {
+    void* out;                     // null: not asked for
+    const void* s;
+    const float* low;
+    int width, accumulate, strips, blocks;
+    long long s_rs, out_ws, out_rs;
+};
+
 // NC: 16-row tiles of the rank; RAGGED: rows of s that are no whole 16-byte vectors, or start anywhere
-template <typename T, int NC, bool TRANSPOSED, bool RAGGED>
-__global__ void __launch_bounds__(GS_THREADS) adapter_grad16_kernel(T* out, const uint16_t* s, const float* low, RowGroups gr, int width, int rank, long long s_rs, long long out_ws, long long out_rs,
-                                                                    int accumulate, int strips, int rank_blocks) {
-    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [GS_WAVES][16][AG_PITCH]
-    const int strip = (int)(blockIdx.x % strips), rb = (int)(blockIdx.x / strips % rank_blocks), w = (int)(blockIdx.x / strips / rank_blocks);
+template <typename T, int NC, bool TRANSPOSED, bool RAGGED, int AG_WAVES>
+__device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int id) {
+    constexpr int AG_THREADS = AG_WAVES * 64;
+    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH]
+    T* out = (T*)ag.out;
+    const uint16_t* s = (const uint16_t*)ag.s;
+    const float* low = ag.low;
+    const int width = ag.width, accumulate = ag.accumulate;
+    const long long s_rs = ag.s_rs, out_ws = ag.out_ws, out_rs = ag.out_rs;
+    const int strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
     const uint16_t* S = s + n0;
@@ -77,21 +90,19 @@ __global__ void __launch_bounds__(GS_THREADS) adapter_grad16_kernel(T* out, cons
         }
     };
     int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
-    for (int g = 0; g < gr.groups; g++) {
-        if (gr.weight(g) != w) continue;
-        const int b = gr.begin(g);
-        end = gr.end(g);
-        constexpr int turn = GS_WAVES * GS_ROUND;
-        const int first = b + ((wave - rounds) & (GS_WAVES - 1)) * GS_ROUND;
-        rounds += (end - b + GS_ROUND - 1) / GS_ROUND;
-        if (first >= end) continue;
+    for_groups_of(gr, w, [&](int begin, int stop) {
+        end = stop;
+        constexpr int turn = AG_WAVES * GS_ROUND;
+        const int first = begin + ((wave - rounds) & (AG_WAVES - 1)) * GS_ROUND;
+        rounds += (end - begin + GS_ROUND - 1) / GS_ROUND;
+        if (first >= end) return;
         static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
         for (int row0 = first; row0 < end; row0 += SLOTS * turn)
             static_for<0, SLOTS>([&](auto sc) {
                 multiply(sc);
                 request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
             });
-    }
+    });
     static_for<0, NC>([&](auto cc) {
         constexpr int c = decltype(cc)::value;
         if (c) __syncthreads();
@@ -102,12 +113,12 @@ __global__ void __launch_bounds__(GS_THREADS) adapter_grad16_kernel(T* out, cons
         __syncthreads();
         // four outputs a thread, neighbours along the output's rows
 #pragma unroll
-        for (int o = 0; o < 4; o++) {
-            const int id = threadIdx.x + o * GS_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
+        for (int o = 0; o < 16 * AG_COLS / AG_THREADS; o++) {
+            const int id = threadIdx.x + o * AG_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
             if (r0 + 16 * c + r >= rank || n0 + col >= width) continue;
             float t = gs_sums[r * AG_PITCH + col];
 #pragma unroll
-            for (int p = 1; p < GS_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
+            for (int p = 1; p < AG_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
             T* at = out + w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
             T y = round_to<T>(t);
             if (accumulate) y = round_to<T>(widen(*at) + widen(y));
@@ -116,30 +127,41 @@ __global__ void __launch_bounds__(GS_THREADS) adapter_grad16_kernel(T* out, cons
     });
 }
 
-template <typename T, int NC, bool TRANSPOSED>
-static int launch_grad(const GroupedArgs& g) {
-    const int width = TRANSPOSED ? g.k : g.n, rank = TRANSPOSED ? g.n : g.k;
-    const void* s = TRANSPOSED ? g.A : g.B;
-    const float* low = (const float*)(TRANSPOSED ? g.B : g.A);
-    const long long s_rs = TRANSPOSED ? g.a_rs : g.b_rs;
-    const int strips = (width + AG_COLS - 1) / AG_COLS, rank_blocks = (rank + 16 * NC - 1) / (16 * NC);
-    const long long blocks = (long long)strips * rank_blocks * g.gr.weights;
-    if (blocks > 0x7fffffffll) { set_error("adapter gradient: %lld tiles are more than a launch takes", blocks); return -1; }
-    constexpr int lds = GS_WAVES * 16 * AG_PITCH * 4;
-    auto launch = [&](auto kern) {
-        if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), (T*)g.C, (const uint16_t*)s, low, g.gr, width, rank, s_rs, g.c_ws, g.c_rs, g.accumulate, strips, rank_blocks);
-        return check_launch("adapter_grad16_kernel") ? 0 : -1;
-    };
-    const bool ragged = width % 8 || s_rs % 8 || ((uintptr_t)s & 15);
-    return ragged ? launch(adapter_grad16_kernel<T, NC, TRANSPOSED, true>) : launch(adapter_grad16_kernel<T, NC, TRANSPOSED, false>);
+// dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads
+template <typename T, int NC, bool RAGGED, int AG_WAVES>
+__global__ void __launch_bounds__(AG_WAVES * 64) adapter_grads16_kernel(AdapterGrad a, AdapterGrad b, RowGroups gr, int rank, int rank_blocks) {
+    const int id = (int)blockIdx.x;
+    if (id < a.blocks) adapter_grad16_block<T, NC, true, RAGGED, AG_WAVES>(a, gr, rank, rank_blocks, id);
+    else adapter_grad16_block<T, NC, false, RAGGED, AG_WAVES>(b, gr, rank, rank_blocks, id - a.blocks);
 }
 
-template <typename T>
-static int launch_grad_shape(const GroupedArgs& g, bool transposed) {
-    const int rank = transposed ? g.n : g.k;
-    if (rank <= 16) return transposed ? launch_grad<T, 1, true>(g) : launch_grad<T, 1, false>(g);
-    return transposed ? launch_grad<T, 2, true>(g) : launch_grad<T, 2, false>(g);
+template <typename T, int NC, bool RAGGED, int AG_WAVES>
+static int launch_grads_as(const AdapterGrad& a, const AdapterGrad& b, const RowGroups& gr, int rank, int rank_blocks) {
+    constexpr int lds = AG_WAVES * 16 * AG_PITCH * 4;
+    auto kern = adapter_grads16_kernel<T, NC, RAGGED, AG_WAVES>;
+    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.blocks + b.blocks)), dim3(AG_WAVES * 64), lds, current_stream(), a, b, gr, rank, rank_blocks);
+    return check_launch("adapter_grads16_kernel") ? 0 : -1;
+}
+
+template <typename T, int NC>
+static int launch_grads(AdapterGrad a, AdapterGrad b, const RowGroups& gr, int rank) {
+    const int rank_blocks = (rank + 16 * NC - 1) / (16 * NC);
+    bool ragged = false;
+    long long both = 0;
+    for (AdapterGrad* g : {&a, &b}) {
+        g->strips = (g->width + AG_COLS - 1) / AG_COLS;
+        const long long own = (long long)g->strips * rank_blocks * gr.weights;
+        both += own;
+        if (both > 0x3fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", both); return -1; }
+        g->blocks = g->out ? (int)own : 0;
+        ragged = ragged || (g->out && (g->width % 8 || g->s_rs % 8 || ((uintptr_t)g->s & 15)));
+    }
+    // Eight waves share a workgroup's rows, four where there are workgroups enough to take a CU in twos (fp16, us, eight and four: 24 + 48 workgroups,
+    // 2048 rows of 3 adapters, 1024 x 2048, rank 8, 9.7 / 11.4; 2 x 2048, 8192 rows of 32 adapters, 4096 x 4096, rank 64, 144 / 93).  The same for one gradient as for both: they have the same bits alone.
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    if (both >= 2 * cus) return ragged ? launch_grads_as<T, NC, true, 4>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, false, 4>(a, b, gr, rank, rank_blocks);
+    return ragged ? launch_grads_as<T, NC, true, 8>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, false, 8>(a, b, gr, rank, rank_blocks);
 }
 
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
@@ -149,8 +171,12 @@ bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
     return s_cs == 1 && s_rs >= width && s_rs < (1ll << 22) && l_rs == rank && (l_cs == 1 || rank == 1) && rank < (1 << 20) && !path_disabled("mfma");
 }
 
-int launch_adapter_grad16(const GroupedArgs& g, GroupedLow low, int dtype) {
-    return dtype == RP_DTYPE_BFLOAT16 ? launch_grad_shape<bf16_t>(g, low == LOW_B) : launch_grad_shape<f16_t>(g, low == LOW_B);
+int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
+    const AdapterGrad a{da.C, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
+    const AdapterGrad b{db.C, db.B, (const float*)db.A, db.n, db.accumulate, 0, 0, db.b_rs, db.c_ws, db.c_rs};
+    const int rank = da.n;
+    if (dtype == RP_DTYPE_BFLOAT16) return rank <= 16 ? launch_grads<bf16_t, 1>(a, b, da.gr, rank) : launch_grads<bf16_t, 2>(a, b, da.gr, rank);
+    return rank <= 16 ? launch_grads<f16_t, 1>(a, b, da.gr, rank) : launch_grads<f16_t, 2>(a, b, da.gr, rank);
 }
 
 }  // namespace rp

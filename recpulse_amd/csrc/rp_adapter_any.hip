@@ -57,17 +57,15 @@ __global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedAr
     A acc[NR_COLS];
 #pragma unroll
     for (int r = 0; r < NR_COLS; r++) acc[r] = 0;
-    for (int q = 0; q < g.gr.groups; q++) {
-        if (g.gr.weight(q) != w) continue;
-        const int e = g.gr.end(q);
+    for_groups_of(g.gr, w, [&](int begin, int end) {
 #pragma unroll 4
-        for (int i = g.gr.begin(q) + wave; i < e; i += NW_WAVES) {
+        for (int i = begin + wave; i < end; i += NW_WAVES) {
             const A v = col < width ? (A)widen(s[i * s_rs + col * s_cs]) : (A)0;
             const A* l = low + i * l_rs;
 #pragma unroll
             for (int r = 0; r < NR_COLS; r++) acc[r] += v * l[r0 + r < rank ? r0 + r : rank - 1];
         }
-    }
+    });
 #pragma unroll
     for (int r = 0; r < NR_COLS; r++) sums[wave][r][lane] = acc[r];
     __syncthreads();

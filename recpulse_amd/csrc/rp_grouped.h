@@ -95,7 +95,7 @@ int launch_adapter_tiles16_128(const GroupedArgs& shared, const AdapterTerm& ter
 int launch_adapter_tiles16_64(const GroupedArgs& shared, const AdapterTerm& term, bool ragged, int dtype);
 // the gradients of an adapter's factors (rp_adapter16_grads.hip): by weights, LOW_A (dB) or LOW_B (dA)
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low);
-int launch_adapter_grad16(const GroupedArgs& g, GroupedLow low, int dtype);
+int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype);       // those whose C is not null
 // The whole layer for a few rows: `shared` one group of all rows, `low` the product above, `term` what it adds
 bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term);
 int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype);

@@ -85,8 +85,10 @@ static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const 
 
 // An adapter's narrow product (C is h or u) and the gradients of its factors
 static int narrow_rows(const GroupedArgs& g, int dtype) { return is16(dtype) && adapter_shrink16_takes(g) ? launch_adapter_shrink16(g, dtype) : launch_narrow_rows(g, dtype); }
-static int narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
-    return is16(dtype) && adapter_grad16_takes(g, low) ? launch_adapter_grad16(g, low, dtype) : launch_narrow_weights(g, low, dtype);
+static int narrow_weights(GroupedArgs da, GroupedArgs db, int dtype) {
+    if (is16(dtype) && (da.C || db.C) && (!da.C || adapter_grad16_takes(da, LOW_B)) && (!db.C || adapter_grad16_takes(db, LOW_A))) return launch_adapter_grads16(da, db, dtype);
+    if (da.C && launch_narrow_weights(da, LOW_B, dtype) != 0) return -1;
+    return db.C ? launch_narrow_weights(db, LOW_A, dtype) : 0;
 }
 
 // The shared product of a layer with adapters, and the adapters' term
@@ -97,6 +99,8 @@ static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int d
         p.ragged = lie == LIE_RAGGED;
         choose_tile16(p, 1, s.gr.rows, s.k, s.n);
         if (p.ragged && p.bm == 256) p.bm = p.bn = 128;
+        // (fp16, 2048 rows of 2048 -> 1024, rank 8, 128 tiles of 128: 26 us, on 64 x 64 tiles 22)
+        if (p.bm == 128 && (long long)((s.gr.rows + 127) / 128) * ((s.n + 127) / 128) * 4 < cus() * 3) p.bm = p.bn = 64;
         const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
         // from about a tile for every other CU on, and while a tile's rows are few segments': each costs it 2 us
         if (lie != LIE_NEITHER && p.bm == p.bn && !path_disabled("adapter_tiles") && tiles * 2 >= cus() && term.gr.rows / term.gr.groups >= 16) {
@@ -186,9 +190,8 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
         const GroupedArgs shared{dx, dy, w, nullptr, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, n, k, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
         if (shared_with_term(shared, AdapterTerm{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank}, dtype) != 0) return -1;
     }
-    if (da && narrow_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0}, LOW_B, dtype) != 0) return -1;
-    if (db && narrow_weights(GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, LOW_A, dtype) != 0) return -1;
-    return 0;
+    return narrow_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0},
+                          GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, dtype);
 }
 
 }  // extern "C"

@@ -21,17 +21,25 @@ struct RowGroups {
     int groups, rows, weights;
     __device__ __forceinline__ int begin(int g) const { const int o = offsets ? offsets[g] : g ? rows : 0; return o < 0 ? 0 : o > rows ? rows : o; }
     __device__ __forceinline__ int end(int g) const { const int b = begin(g), o = offsets ? offsets[g + 1] : rows, e = o > rows ? rows : o; return e > b ? e : b; }
-    // the weight of row i's group, -1 if it has none (offsets in order; the last group that begins at or before i and does not end before it)
-    __device__ __forceinline__ int weight_of_row(int i) const {
-        int lo = 0, hi = groups;                              // the number of groups that end at or before i
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (end(mid) <= i) lo = mid + 1; else hi = mid;
-        }
-        return lo < groups && begin(lo) <= i ? weight(lo) : -1;
-    }
     __device__ __forceinline__ int weight(int g) const { const int w = ids ? ids[g] : g; return w >= 0 && w < weights ? w : -1; }
 };
+
+// f(begin, end) for every group of weight w that has rows, in order; the wave looks at 64 groups at a time (one after the other, their ids and
+// offsets cost a trip to memory each: 32 adapters of 8192 rows in 48 segments, gradients of rank 64 at 4096 x 4096, 188 us, 144 here)
+template <typename F>
+__device__ __forceinline__ void for_groups_of(const RowGroups& gr, int w, F f) {
+    const int lane = threadIdx.x & 63;
+    for (int g0 = 0; g0 < gr.groups; g0 += 64) {
+        int b = 0, e = 0;
+        if (g0 + lane < gr.groups && gr.weight(g0 + lane) == w) { b = gr.begin(g0 + lane); e = gr.end(g0 + lane); }
+        unsigned long long here = __builtin_amdgcn_ballot_w64(e > b);
+        while (here) {
+            const int l = __builtin_ctzll(here);
+            here &= here - 1;
+            f(__builtin_amdgcn_readlane(b, l), __builtin_amdgcn_readlane(e, l));
+        }
+    }
+}
 
 // Tiles of `tile` rows that `rows` rows in `groups` groups can come to, whatever the offsets hold as long as the groups do not overlap
 static inline long long max_row_tiles(long long rows, long long groups, int tile) {
