@@ -23,7 +23,14 @@ static Lie lies(const void* p, long long row_stride, long long weight_stride, in
 }
 static Lie worse(Lie a, Lie b) { return a > b ? a : b; }
 
-// Tiles of the 16-bit products: their edge, 0 for none, and how the operands lie
+// 256 x 256 tiles go in whole rounds of the CUs, each of k / 1024 * 23.3 us + 10; tiles of 128, two to a CU at a time, in any number, 0.043 us each at k = 1024.  fp16,
+// us on 256 and 128: 1024 -> 4096 in 8 groups, 3000 rows (1 round) 38 / 43, 4096 rows (2) 67 / 55, 8192 (3) 102 / 95, 16384 (5) 171 / 189; 4096 -> 4096, 4096 rows (2) 209 / 203.
+static bool prefers256(long long tiles256, long long tiles128, long long k) {
+    const long long rounds = (tiles256 + cus() - 1) / cus();
+    return rounds * cus() * 4 * (k + 440) * 100 < tiles128 * (k + 60) * 187;
+}
+
+// Tiles of the 16-bit products: their edge, 0 for none, and how the operands lie.  How many row tiles there are is known on the device only: each group is taken to end inside a tile.
 struct Tile16 { int edge; bool ragged; };
 
 static Tile16 rows_tile16(const GroupedArgs& g, int dtype) {
@@ -31,20 +38,20 @@ static Tile16 rows_tile16(const GroupedArgs& g, int dtype) {
     const bool b_mc = g.b_cs == 1;
     const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
     if (lie == LIE_NEITHER) return {0, false};
-    const long long tiles256 = (long long)((g.gr.rows + 255) / 256) * ((g.n + 255) / 256), tiles128 = (long long)((g.gr.rows + 127) / 128) * ((g.n + 127) / 128);
     const int mean = g.gr.rows / g.gr.groups;
-    // 128 x 128 tiles from three quarters of a round of the CUs on (bf16, 519 -> 1031, us on 64 and 128: 1999 rows of 6 groups, 144 tiles, 14.5 / 15.2; 4096 of 8, 288 tiles, 23.1 / 19.7)
-    if (lie == LIE_WHOLE && mean >= 256 && g.n >= 256 && g.k >= 256 && tiles256 >= cus() / 2) return {256, false};
-    return {mean >= 96 && g.n > 64 && tiles128 * 4 >= cus() * 3 ? 128 : 64, lie == LIE_RAGGED};
+    auto tiles = [&](int edge) { return ((long long)(g.gr.rows + edge - 1) / edge + g.gr.groups / 2) * ((g.n + edge - 1) / edge); };
+    if (lie == LIE_WHOLE && mean >= 256 && g.n >= 256 && g.k >= 256 && prefers256(tiles(256), tiles(128), g.k)) return {256, false};
+    // 128 x 128 tiles from a round of the CUs on (bf16, 519 -> 1031, us on 64 and 128: 1999 rows of 6 groups, 171 tiles, 14.5 / 15.2; 4096 of 8, 324 tiles, 23.1 / 19.7)
+    return {mean >= 96 && g.n > 64 && tiles(128) >= cus() ? 128 : 64, lie == LIE_RAGGED};
 }
 
 static Tile16 weights_tile16(const GroupedArgs& g, int dtype) {
     if (!is16(dtype) || g.a_cs != 1 || g.b_cs != 1 || path_disabled("mfma")) return {0, false};
     const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), lies(g.B, g.b_rs, 0, g.n, 2));
     if (lie == LIE_NEITHER) return {0, false};
-    const long long tiles256 = (long long)((g.k + 255) / 256) * ((g.n + 255) / 256) * g.gr.weights, tiles128 = (long long)((g.k + 127) / 128) * ((g.n + 127) / 128) * g.gr.weights;
-    if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && tiles256 >= cus() / 2) return {256, false};
-    return {g.k > 64 && g.n > 64 && tiles128 >= cus() / 2 ? 128 : 64, lie == LIE_RAGGED};
+    auto tiles = [&](int edge) { return (long long)((g.k + edge - 1) / edge) * ((g.n + edge - 1) / edge) * g.gr.weights; };
+    if (lie == LIE_WHOLE && g.k >= 256 && g.n >= 256 && prefers256(tiles(256), tiles(128), g.gr.rows / g.gr.groups)) return {256, false};
+    return {g.k > 64 && g.n > 64 && tiles(128) >= cus() / 2 ? 128 : 64, lie == LIE_RAGGED};
 }
 
 static int grouped_rows(const GroupedArgs& g, int dtype) {
