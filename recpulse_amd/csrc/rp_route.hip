@@ -15,7 +15,7 @@
 namespace rp {
 
 constexpr int ROUTE_MAX_K = 16, ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_SLOTS = 1 << 30;
-constexpr int SORT_CHUNK = 1024;             // slots a workgroup of the sort takes; no fewer than there may be groups (see sort_chunks)
+constexpr int SORT_CHUNKS = 256;             // workgroups that a longer list is dealt to, at most
 
 // ---- order-preserving integer keys: larger logit, larger key; equal logits (+0 and -0 too), equal keys ----
 // 0 is "not there": an expert that is taken already, one past the last, or a logit of -inf.  NaN is above every number.
@@ -65,40 +65,102 @@ template <int LANES, typename V, typename F> __device__ __forceinline__ V reduce
     return v;
 }
 
+// ---- a logit and its expert in one number: the largest is the largest logit's, the lowest index among equal ones ----
+// Below 1: not there.  float32: key and 1023 - expert are the upper 32 and lower 10 bits of a whole number that float64 holds exactly, and a
+// maximum is one instruction (the value is never NaN or negative; written as an instruction, the compiler would quiet both operands first).
+// 16 bits: the same in a uint32.  float64 has no wider type: key and expert are found one after the other.
+template <typename T> struct Candidate {
+    using type = double;
+    static __device__ __forceinline__ type of(float x, int e) {
+        const uint32_t k = logit_key<float>::of(x);
+        return k ? __builtin_fma((double)k, 1024.0, (double)(1023 - e)) : 0.0;
+    }
+    static __device__ __forceinline__ type largest(type a, type b) {
+        double r;
+        asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+        return r;
+    }
+    static __device__ __forceinline__ bool there(type c) { return c >= 1.0; }
+    static __device__ __forceinline__ type without(type c, type taken) {                   // (the upper word alone: what is left is below 1)
+        const uint64_t b = __builtin_bit_cast(uint64_t, c);
+        return __builtin_bit_cast(double, (uint64_t)(c == taken ? 0u : (uint32_t)(b >> 32)) << 32 | (uint32_t)b);
+    }
+    static __device__ __forceinline__ uint32_t key(type c) { return (uint32_t)(c * (1.0 / 1024.0)); }
+    static __device__ __forceinline__ int expert(type c) { return 1023 - (int)(c - (double)key(c) * 1024.0); }
+    static __device__ __forceinline__ float value(type c) { return logit_key<float>::value(key(c)); }
+};
+// DROP: bits of a 16-bit value's float32 key that say nothing (all zeros, of a negative value all ones)
+template <int DROP> struct Candidate16 {
+    using type = uint32_t;
+    static __device__ __forceinline__ type of(float x, int e) {
+        const uint32_t k = logit_key<float>::of(x) >> DROP;
+        return k ? k << 10 | (uint32_t)(1023 - e) : 0u;
+    }
+    static __device__ __forceinline__ type largest(type a, type b) { return a > b ? a : b; }
+    static __device__ __forceinline__ bool there(type c) { return c != 0; }
+    static __device__ __forceinline__ type without(type c, type taken) { return c == taken ? 0u : c; }
+    static __device__ __forceinline__ int expert(type c) { return 1023 - (int)(c & 1023u); }
+    static __device__ __forceinline__ float value(type c) {
+        const uint32_t k = c >> 10 << DROP;
+        return logit_key<float>::value(k & 0x80000000u ? k : k | ((1u << DROP) - 1));
+    }
+};
+template <> struct Candidate<bf16_t> : Candidate16<16> {};
+template <> struct Candidate<f16_t> : Candidate16<13> {};
+
 // The k largest of a token's logits by LANES lanes, V experts a lane (expert e sits in lane e % LANES).  Lane j < k returns slot j's
 // expert (-1: none was left) and weight.
-// What bounds it is the chain of k selections, each a maximum over the experts and the lowest index that has it; rows of 16 lanes
-// keep four tokens in a wave and every reduction inside a DPP row.
+// What bounds it is the chain of k selections, each a maximum over the experts; rows of 16 lanes keep four tokens in a wave and every
+// reduction inside a DPP row.  (With the largest key found first and then the lowest index that has it, 200000 tokens of 128 took 100 us, now 72.)
 template <typename T, int LANES, int V>
 __device__ __forceinline__ void route_token(const T* row, bool live, int experts, int k, bool normalize, int l, int& expert, typename traits<T>::acc& weight) {
     using A = typename traits<T>::acc;
-    using K = typename logit_key<A>::type;
-    K key[V];
     A x[V];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int e = v * LANES + l;
-        const bool in = live && e < experts;
-        x[v] = in ? widen(row[e]) : (A)-INFINITY;
-        key[v] = in ? logit_key<A>::of(x[v]) : (K)0;
+        x[v] = live && e < experts ? widen(row[e]) : (A)-INFINITY;
     }
     expert = -1;
     A value = 0, top = 0;
-    for (int j = 0; j < k; j++) {
-        K best = key[0];
+    if constexpr (sizeof(A) == 4) {
+        using C = Candidate<T>;
+        using P = typename C::type;
+        P cand[V], mine = 0;
 #pragma unroll
-        for (int v = 1; v < V; v++) best = key[v] > best ? key[v] : best;
-        best = reduce_lanes<LANES>(best, [](K a, K b) { return a > b ? a : b; });
-        int at = 0x7fffffff;
+        for (int v = 0; v < V; v++) cand[v] = C::of(x[v], v * LANES + l);
+        for (int j = 0; j < k; j++) {
+            P best = cand[0];
 #pragma unroll
-        for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v * LANES + l : at;
-        at = reduce_lanes<LANES>(at, [](int a, int b) { return a < b ? a : b; });
-        if (best == 0) continue;                              // (the same for all lanes of the token)
+            for (int v = 1; v < V; v++) best = C::largest(best, cand[v]);
+            best = reduce_lanes<LANES>(best, [](P a, P b) { return C::largest(a, b); });
 #pragma unroll
-        for (int v = 0; v < V; v++) key[v] = at == v * LANES + l ? (K)0 : key[v];
-        const A got = logit_key<A>::value(best);
-        if (j == 0) top = got;
-        if (l == j) { expert = at; value = got; }
+            for (int v = 0; v < V; v++) cand[v] = C::without(cand[v], best);
+            if (j == 0) top = C::there(best) ? C::value(best) : (A)0;
+            if (l == j) mine = best;
+        }
+        if (C::there(mine)) { expert = C::expert(mine); value = C::value(mine); }
+    } else {
+        using K = typename logit_key<A>::type;
+        K key[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = logit_key<A>::of(x[v]);
+        for (int j = 0; j < k; j++) {
+            K best = key[0];
+#pragma unroll
+            for (int v = 1; v < V; v++) best = key[v] > best ? key[v] : best;
+            best = reduce_lanes<LANES>(best, [](K a, K b) { return a > b ? a : b; });
+            int at = 0x7fffffff;
+#pragma unroll
+            for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v * LANES + l : at;
+            at = reduce_lanes<LANES>(at, [](int a, int b) { return a < b ? a : b; });
+            if (best == 0) continue;                          // (the same for all lanes of the token)
+#pragma unroll
+            for (int v = 0; v < V; v++) key[v] = at == v * LANES + l ? (K)0 : key[v];
+            const A got = logit_key<A>::value(best);
+            if (j == 0) top = got;
+            if (l == j) { expert = at; value = got; }
+        }
     }
     const A e = expert >= 0 ? exp(value - top) : (A)0;        // (an infinite or NaN top leaves NaN weights)
     A sum = 0;
@@ -194,84 +256,94 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_one_kernel(const int
     sort_all(ids, count, groups, bits, sort_lds, offsets, order, position);
 }
 
-// Longer lists in three launches: count each chunk's slots by expert, add the counts up over the chunks, place each chunk's slots.  The
-// counts and the places need groups ints a chunk: they are kept in the chunk's own part of `position`, which is written
-// last and by the workgroup that has read them, so the sort takes no workspace and calls on several streams share nothing.
-// A last chunk of less than SORT_CHUNK slots is joined to the one before.
-static inline int sort_chunks(int count) { return count / SORT_CHUNK > 1 ? count / SORT_CHUNK : 1; }
-
-__global__ void __launch_bounds__(256) sort_count_kernel(const int* ids, int count, int groups, int chunks, int* position) {
-    __shared__ int counts[ROUTE_MAX_EXPERTS];
-    for (int g = threadIdx.x; g < groups; g += 256) counts[g] = 0;
-    __syncthreads();
-    const int s0 = blockIdx.x * SORT_CHUNK, s1 = (int)blockIdx.x == chunks - 1 ? count : s0 + SORT_CHUNK;
-    for (int s = s0 + threadIdx.x; s < s1; s += 256) {
+// Longer lists in two launches: count each chunk's slots by expert, into counts [chunks][groups], then place each chunk's slots.  A workgroup of
+// the second adds up the counts of all chunks by itself: 256 chunks of 128 experts are 128 KB out of the L2, which takes less than a launch
+// between the two that adds them up once (16384 tokens, 8 of 128 experts: 13.8 us in three launches, 6.6 here, the counts coming from the selection).
+__device__ __forceinline__ void count_ids(const int* ids, int s0, int s1, int groups, int* counts) {
+    for (int s = s0 + threadIdx.x; s < s1; s += SORT_ONE_WAVES * 64) {
         const int id = ids[s];
         if ((unsigned)id < (unsigned)groups) atomicAdd(&counts[id], 1);
     }
-    __syncthreads();
-    for (int g = threadIdx.x; g < groups; g += 256) position[s0 + g] = counts[g];
 }
 
-// One workgroup: `parts` threads to an expert, each a run of chunks
-__global__ void __launch_bounds__(1024) sort_scan_kernel(int* position, int* offsets, int* order, int count, int groups, int chunks, int parts) {
-    __shared__ int totals[ROUTE_MAX_EXPERTS + 1];
-    __shared__ int sums[1024];
-    const int width = 1024 / parts, g = threadIdx.x % width, part = threadIdx.x / width;
-    const int per = (chunks + parts - 1) / parts, c0 = part * per < chunks ? part * per : chunks, c1 = c0 + per < chunks ? c0 + per : chunks;
-    int sum = 0;
-    if (g < groups) {
-#pragma unroll 8
-        for (int c = c0; c < c1; c++) sum += position[(size_t)c * SORT_CHUNK + g];
-    }
-    sums[threadIdx.x] = sum;
+__global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_count_kernel(const int* ids, int count, int groups, int chunk, int* counts) {
+    __shared__ int own[ROUTE_MAX_EXPERTS];
+    for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) own[g] = 0;
     __syncthreads();
-    int before = 0;
-    if (g < groups) {
-        for (int p = 0; p < part; p++) before += sums[p * width + g];
-        if (part == parts - 1) totals[g] = before + sum;
+    const int s0 = blockIdx.x * chunk, s1 = count - s0 < chunk ? count : s0 + chunk;
+    count_ids(ids, s0, s1, groups, own);
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) counts[(size_t)blockIdx.x * groups + g] = own[g];
+}
+
+// `parts` threads to an expert (their number a power of two, `width` experts), each a run of chunks
+__global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_place_kernel(const int* ids, int count, int groups, int bits, int chunk, int parts, const int* counts, int* offsets, int* order, int* position) {
+    extern __shared__ int sort_lds[];                          // [SORT_ONE_WAVES][groups] counts, where [groups], totals [groups + 1], sums [2][1024]
+    int* where = sort_lds + SORT_ONE_WAVES * groups;
+    int* totals = where + groups;
+    int* sums = totals + groups + 1;
+    const int chunks = (int)gridDim.x, own = (int)blockIdx.x, width = SORT_ONE_WAVES * 64 / parts;
+    for (int i = threadIdx.x; i < SORT_ONE_WAVES * groups; i += SORT_ONE_WAVES * 64) sort_lds[i] = 0;
+    {
+        const int g = threadIdx.x % width, part = threadIdx.x / width, per = (chunks + parts - 1) / parts;
+        const int c0 = part * per < chunks ? part * per : chunks, c1 = c0 + per < chunks ? c0 + per : chunks;
+        int before = 0, all = 0;
+        if (g < groups) {
+#pragma unroll 16
+            for (int c = c0; c < c1; c++) {
+                const int n = counts[(size_t)c * groups + g];
+                all += n;
+                before += c < own ? n : 0;
+            }
+        }
+        sums[threadIdx.x] = before;
+        sums[SORT_ONE_WAVES * 64 + threadIdx.x] = all;
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) {
+        int before = 0, all = 0;
+        for (int p = 0; p < parts; p++) {
+            before += sums[p * width + g];
+            all += sums[SORT_ONE_WAVES * 64 + p * width + g];
+        }
+        where[g] = before;
+        totals[g] = all;
     }
     __syncthreads();
     sum_totals(totals, groups);
-    for (int i = threadIdx.x; i <= groups; i += 1024) offsets[i] = totals[i];
-    if (g < groups) {
-        int at = totals[g] + before;
-        for (int c = c0; c < c1; c += 8) {
-            int n[8];
-#pragma unroll
-            for (int u = 0; u < 8; u++) n[u] = c + u < c1 ? position[(size_t)(c + u) * SORT_CHUNK + g] : 0;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                if (c + u < c1) position[(size_t)(c + u) * SORT_CHUNK + g] = at;
-                at += n[u];
-            }
-        }
-    }
-    for (int s = totals[groups] + threadIdx.x; s < count; s += 1024) order[s] = -1;
-}
-
-constexpr int SORT_PLACE_WAVES = 8;
-__global__ void __launch_bounds__(SORT_PLACE_WAVES * 64) sort_place_kernel(const int* ids, int count, int groups, int bits, int chunks, int* order, int* position) {
-    extern __shared__ int sort_lds[];                          // [SORT_PLACE_WAVES][groups] counts, then the chunk's places
-    int* where = sort_lds + SORT_PLACE_WAVES * groups;
-    const int s0 = blockIdx.x * SORT_CHUNK, s1 = (int)blockIdx.x == chunks - 1 ? count : s0 + SORT_CHUNK;
-    for (int i = threadIdx.x; i < SORT_PLACE_WAVES * groups; i += SORT_PLACE_WAVES * 64) sort_lds[i] = 0;
-    for (int g = threadIdx.x; g < groups; g += SORT_PLACE_WAVES * 64) where[g] = position[s0 + g];
+    for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) where[g] += totals[g];
+    if (own == 0)
+        for (int g = threadIdx.x; g <= groups; g += SORT_ONE_WAVES * 64) offsets[g] = totals[g];
     __syncthreads();
-    sort_slots<SORT_PLACE_WAVES>(ids, s0, s1, groups, bits, sort_lds, where, order, position);
+    const int s0 = own * chunk, s1 = count - s0 < chunk ? count : s0 + chunk;
+    sort_slots<SORT_ONE_WAVES>(ids, s0, s1, groups, bits, sort_lds, where, order, position);
+    for (long long s = (long long)totals[groups] + own * (SORT_ONE_WAVES * 64) + threadIdx.x; s < count; s += chunks * (SORT_ONE_WAVES * 64)) order[s] = -1;
 }
 
 // ---- routing: kernels ----
 template <typename T> using weight_t = typename traits<T>::acc;        // routing weights: float32 (float64 for float64), not rounded to 16 bits
 
+// A chunk of `per_block` tokens a workgroup, whose slots it counts by expert for the sort
 template <typename T, int LANES, int V>
-__global__ void __launch_bounds__(256) route_topk_kernel(weight_t<T>* weights, int* experts_out, const T* logits, long long rs, int tokens, int experts, int k, int normalize) {
-    const int l = threadIdx.x % LANES, t = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const bool live = t < tokens;
-    int expert;
-    weight_t<T> w;
-    route_token<T, LANES, V>(logits + (long long)(live ? t : 0) * rs, live, experts, k, normalize != 0, l, expert, w);
-    if (live && l < k) { weights[(size_t)t * k + l] = w; experts_out[(size_t)t * k + l] = expert; }
+__global__ void __launch_bounds__(SORT_ONE_WAVES * 64) route_topk_kernel(weight_t<T>* weights, int* experts_out, int* counts, const T* logits, long long rs, int tokens, int experts, int k, int normalize,
+                                                                        int per_block) {
+    __shared__ int own[ROUTE_MAX_EXPERTS];
+    for (int g = threadIdx.x; g < experts; g += SORT_ONE_WAVES * 64) own[g] = 0;
+    __syncthreads();
+    const int l = threadIdx.x % LANES, t0 = (int)blockIdx.x * per_block, t1 = tokens - t0 < per_block ? tokens : t0 + per_block;
+    for (int t = t0 + threadIdx.x / LANES; t - (int)threadIdx.x / LANES < t1; t += SORT_ONE_WAVES * 64 / LANES) {      // (whole waves together)
+        const bool live = t < t1;
+        int expert;
+        weight_t<T> w;
+        route_token<T, LANES, V>(logits + (long long)(live ? t : 0) * rs, live, experts, k, normalize != 0, l, expert, w);
+        if (live && l < k) {
+            weights[(size_t)t * k + l] = w;
+            experts_out[(size_t)t * k + l] = expert;
+            if (expert >= 0) atomicAdd(&own[expert], 1);
+        }
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < experts; g += SORT_ONE_WAVES * 64) counts[(size_t)blockIdx.x * experts + g] = own[g];
 }
 
 // A few tokens: selection and sort in one workgroup and one launch
@@ -355,33 +427,50 @@ static int bits_of(int groups) {
 }
 
 // Lists up to this length are sorted by one workgroup in one launch
-constexpr int SORT_ONE_MAX = 4 * SORT_CHUNK;
+constexpr int SORT_ONE_MAX = 4096;
+
+// The counts of a longer list: the null stream's own memory, or a block of the pool
+struct SortCounts {
+    NullStreamScratch lease;
+    void* block = nullptr;
+    explicit SortCounts(size_t ints) : lease(ints * sizeof(int)) {
+        if (!lease.ptr && rp_hip_malloc(&block, ints * sizeof(int)) != 0) block = nullptr;
+    }
+    ~SortCounts() { if (block) rp_hip_free(block); }
+    int* ptr() const { return (int*)(lease.ptr ? lease.ptr : block); }
+};
+
+static int launch_place(int* offsets, int* order, int* position, const int* ids, int count, int groups, int chunk, int chunks, const int* counts) {
+    int width = 32;
+    while (width < groups) width *= 2;
+    const size_t lds = ((size_t)(SORT_ONE_WAVES + 2) * groups + 1 + 2 * SORT_ONE_WAVES * 64) * sizeof(int);
+    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)sort_place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute")) return -1;
+    hipLaunchKernelGGL(sort_place_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), lds, current_stream(), ids, count, groups, bits_of(groups), chunk, SORT_ONE_WAVES * 64 / width, counts, offsets, order, position);
+    return check_launch("sort_place_kernel") ? 0 : -1;
+}
+
+static int launch_sort_one(int* offsets, int* order, int* position, const int* ids, int count, int groups) {
+    const size_t lds = ((size_t)(SORT_ONE_WAVES + 1) * groups + 1) * sizeof(int);
+    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)sort_one_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute")) return -1;
+    hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(SORT_ONE_WAVES * 64), lds, current_stream(), ids, count, groups, bits_of(groups), offsets, order, position);
+    return check_launch("sort_one_kernel") ? 0 : -1;
+}
 
 static int launch_sort(int* offsets, int* order, int* position, const int* ids, int count, int groups) {
-    const int bits = bits_of(groups);
-    if (count <= SORT_ONE_MAX) {
-        const size_t lds = ((size_t)(SORT_ONE_WAVES + 1) * groups + 1) * sizeof(int);
-        if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)sort_one_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute")) return -1;
-        hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(SORT_ONE_WAVES * 64), lds, current_stream(), ids, count, groups, bits, offsets, order, position);
-        return check_launch("sort_one_kernel") ? 0 : -1;
-    }
-    const int chunks = sort_chunks(count);
-    hipLaunchKernelGGL(sort_count_kernel, dim3(chunks), dim3(256), 0, current_stream(), ids, count, groups, chunks, position);
+    if (count <= SORT_ONE_MAX) return launch_sort_one(offsets, order, position, ids, count, groups);
+    const int chunk = ((count + SORT_CHUNKS - 1) / SORT_CHUNKS + 511) / 512 * 512, chunks = (count + chunk - 1) / chunk;
+    const SortCounts counts((size_t)chunks * groups);
+    if (!counts.ptr()) return -1;
+    hipLaunchKernelGGL(sort_count_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), ids, count, groups, chunk, counts.ptr());
     if (!check_launch("sort_count_kernel")) return -1;
-    int width = 1;
-    while (width < groups) width *= 2;
-    hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, current_stream(), position, offsets, order, count, groups, chunks, 1024 / width);
-    if (!check_launch("sort_scan_kernel")) return -1;
-    const size_t lds = (size_t)(SORT_PLACE_WAVES + 1) * groups * sizeof(int);
-    hipLaunchKernelGGL(sort_place_kernel, dim3(chunks), dim3(SORT_PLACE_WAVES * 64), lds, current_stream(), ids, count, groups, bits, chunks, order, position);
-    return check_launch("sort_place_kernel") ? 0 : -1;
+    return launch_place(offsets, order, position, ids, count, groups, chunk, chunks, counts.ptr());
 }
 
 template <typename T>
 static int launch_route(void* weights, int* experts_out, int* offsets, int* order, int* position, const void* logits, long long rs, int tokens, int experts, int k, int normalize) {
     return pick_route_shape(experts, [&](auto lanes_c, auto v_c) -> int {
-        constexpr int LANES = decltype(lanes_c)::value, V = decltype(v_c)::value;
-        if (tokens <= ROUTE_ONE_THREADS / LANES) {
+        constexpr int LANES = decltype(lanes_c)::value, V = decltype(v_c)::value, PER = ROUTE_ONE_THREADS / LANES;
+        if (tokens <= PER) {
             const size_t lds = ((size_t)(SORT_ONE_WAVES + 1) * experts + 1 + (size_t)tokens * k) * sizeof(int);
             auto kern = route_one_kernel<T, LANES, V>;
             if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute")) return -1;
@@ -389,11 +478,13 @@ static int launch_route(void* weights, int* experts_out, int* offsets, int* orde
                                tokens, experts, k, normalize, bits_of(experts));
             return check_launch("route_one_kernel") ? 0 : -1;
         }
-        constexpr int PER = 256 / LANES;
-        hipLaunchKernelGGL((route_topk_kernel<T, LANES, V>), dim3((tokens + PER - 1) / PER), dim3(256), 0, current_stream(), (weight_t<T>*)weights, experts_out, (const T*)logits, rs,
-                           tokens, experts, k, normalize);
+        const int per_block = ((tokens + PER - 1) / PER + SORT_CHUNKS - 1) / SORT_CHUNKS * PER, chunks = (tokens + per_block - 1) / per_block;
+        const SortCounts counts((size_t)chunks * experts);
+        if (!counts.ptr()) return -1;
+        hipLaunchKernelGGL((route_topk_kernel<T, LANES, V>), dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), (weight_t<T>*)weights, experts_out, counts.ptr(), (const T*)logits, rs,
+                           tokens, experts, k, normalize, per_block);
         if (!check_launch("route_topk_kernel")) return -1;
-        return launch_sort(offsets, order, position, experts_out, tokens * k, experts);
+        return launch_place(offsets, order, position, experts_out, tokens * k, experts, per_block * k, chunks, counts.ptr());
     });
 }
 
