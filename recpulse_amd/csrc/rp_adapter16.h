@@ -48,15 +48,10 @@ __device__ __forceinline__ void split_low(const float* v, u32x4_t& hi, u32x4_t& 
     __builtin_memcpy(&lo, l, 16);
 }
 
-// eight consecutive 16-bit values at p, of which the first n are there
-__device__ __forceinline__ u32x4_t load8(const uint16_t* p, int n) {
-    if (n >= 8) return *(const u32x4_odd_t*)p;
-    u32x4_t v = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 7; e++)
-        if (e < n) v[e / 2] |= (uint32_t)p[e] << (16 * (e % 2));
-    return v;
-}
+// A vector of eight 16-bit values may straddle the end of its row, of which `left` are there: it is loaded `pulled(left)` values early, where it ends with the row (which
+// holds eight at least), and shifted into place with zeros behind.  So every load is within its operand, none is behind a branch, and rows may start at any element.
+__device__ __forceinline__ int pulled(int left) { return left > 0 && left < 8 ? 8 - left : 0; }
+__device__ __forceinline__ u32x4_t pull_into_place(u32x4_t v, int by) { return __builtin_bit_cast(u32x4_t, __builtin_bit_cast(unsigned __int128, v) >> (16 * by)); }
 
 // LDS of a wave's piece of the factor: 32 rows of k, 16 * NC columns and 8 more, so that the rows that a transposing read takes together start in different banks
 template <int NC> constexpr int sh_pitch() { return 16 * NC + 8; }
@@ -79,14 +74,16 @@ __device__ __forceinline__ void adapter_shrink16_block(const GroupedArgs& g, int
     if (rt.group < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int rank = g.n;
-    const uint16_t* xp[RT];
+    const __amdgpu_buffer_rsrc_t x_rsrc = buffer_rsrc((const uint16_t*)g.A + rt.begin * g.a_rs, ((rt.end - 1 - rt.begin) * g.a_rs + g.k) * 2);
+    uint32_t x_off[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {                               // (rows past the segment repeat its last: their sums are not stored)
         const int r = rt.begin + 16 * i + j;
-        xp[i] = (const uint16_t*)g.A + (r < rt.end ? r : rt.end - 1) * g.a_rs;
+        x_off[i] = (uint32_t)(((r < rt.end ? r : rt.end - 1) - rt.begin) * g.a_rs * 2);
     }
     const uint16_t* f = (const uint16_t*)g.B + rt.weight * g.b_ws;
     constexpr int PITCH = sh_pitch<NC>(), PER_ROW = 16 * NC / PIECE, PIECES = ALONG_K ? NC : SH_STEP * PER_ROW / 64;
+    const __amdgpu_buffer_rsrc_t f_rsrc = buffer_rsrc(f, ALONG_K ? ((rank - 1) * g.b_cs + g.k) * 2 : (long long)g.k * g.b_rs * 2);
     uint16_t* stage = (uint16_t*)sh_lds + wave * SH_STEP * PITCH;
     if constexpr (!ALONG_K) {
         if (rank < 16 * NC)
@@ -98,34 +95,40 @@ __device__ __forceinline__ void adapter_shrink16_block(const GroupedArgs& g, int
     piece_t fv[SLOTS][PIECES];
     auto request = [&](auto slotc, int k0) {
         constexpr int S = decltype(slotc)::value;
+        const int left = g.k - k0 - 8 * q, at = (k0 + 8 * q - pulled(left)) * 2;
 #pragma unroll
-        for (int i = 0; i < RT; i++) xv[S][i] = load8(xp[i] + k0 + 8 * q, g.k - k0 - 8 * q);
+        for (int i = 0; i < RT; i++) xv[S][i] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, (int)(left > 0 ? x_off[i] + at : BUFFER_OOB), 0, 0);
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
             if constexpr (ALONG_K) {
                 const int c = 16 * p + j < rank ? 16 * p + j : rank - 1;
-                fv[S][p] = load8(f + c * g.b_cs + k0 + 8 * q, g.k - k0 - 8 * q);
+                fv[S][p] = __builtin_amdgcn_raw_buffer_load_b128(f_rsrc, (int)(left > 0 ? (uint32_t)(c * g.b_cs * 2) + at : BUFFER_OOB), 0, 0);
             } else {
                 const int id = lane + 64 * p, r = k0 + id / PER_ROW, c = id % PER_ROW * PIECE;
-                fv[S][p] = piece_t{};
-                if (r < g.k && c < rank) {
-                    if constexpr (PIECE == 8) fv[S][p] = *(const u32x4_t*)(f + r * g.b_rs + c);
-                    else fv[S][p] = f[r * g.b_rs + c];
-                }
+                const int off = (int)(r < g.k && c < rank ? (uint32_t)((r * g.b_rs + c) * 2) : BUFFER_OOB);
+                if constexpr (PIECE == 8) fv[S][p] = __builtin_amdgcn_raw_buffer_load_b128(f_rsrc, off, 0, 0);
+                else fv[S][p] = __builtin_amdgcn_raw_buffer_load_b16(f_rsrc, off, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
     f32x4_t acc[RT][NC];
 #pragma unroll
     for (int i = 0; i < RT; i++)
 #pragma unroll
         for (int c = 0; c < NC; c++) acc[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](auto slotc) {
+    auto multiply = [&](auto slotc, int k0) {
         constexpr int S = decltype(slotc)::value;
+        const int by = pulled(g.k - k0 - 8 * q);
+        const bool last = k0 + SH_STEP > g.k && g.k % 8;
+        if (last) {
+#pragma unroll
+            for (int i = 0; i < RT; i++) xv[S][i] = pull_into_place(xv[S][i], by);
+        }
         u32x4_t b[NC];
         if constexpr (ALONG_K) {
 #pragma unroll
-            for (int c = 0; c < NC; c++) b[c] = fv[S][c];
+            for (int c = 0; c < NC; c++) b[c] = last ? pull_into_place(fv[S][c], by) : fv[S][c];
         } else {
 #pragma unroll
             for (int p = 0; p < PIECES; p++) {
@@ -160,7 +163,7 @@ __device__ __forceinline__ void adapter_shrink16_block(const GroupedArgs& g, int
     static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * TURN); });       // (rounds past k load nothing and are zeros)
     for (int k0 = first; k0 < g.k; k0 += SLOTS * TURN)
         static_for<0, SLOTS>([&](auto sc) {
-            multiply(sc);
+            multiply(sc, k0 + decltype(sc)::value * TURN);
             request(sc, k0 + (SLOTS + decltype(sc)::value) * TURN);
         });
 

@@ -40,7 +40,7 @@ static int launch_shrink_rank(const GroupedArgs& g) {
 }
 
 bool adapter_shrink16_takes(const GroupedArgs& g) {
-    return g.n <= SH_MAX_RANK && g.a_cs == 1 && ((g.b_cs == 1 && g.b_rs == g.n) || g.b_rs == 1) && !path_disabled("mfma");
+    return g.n <= SH_MAX_RANK && g.k >= 8 && g.a_rs >= 0 && g.a_rs < (1ll << 22) && (long long)g.k * g.n < (1 << 28) && g.a_cs == 1 && ((g.b_cs == 1 && g.b_rs == g.n) || g.b_rs == 1) && !path_disabled("mfma");
 }
 
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype) { return dtype == RP_DTYPE_BFLOAT16 ? launch_shrink_rank<bf16_t>(g) : launch_shrink_rank<f16_t>(g); }
@@ -98,87 +98,97 @@ int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low,
     return rc;
 }
 
-// ---- the term by itself: y[i] += h[i] . b_a, where the shared product is too small for tiles that would fill the CUs ----
-// 16 rows of a segment and 512 columns a workgroup (one wave), 8 columns a lane: b is read once for the 16 rows, h through the scalar cache.
+// ---- the term by itself: y[i] += h[i] . b_a, where the shared product is too small, or a tile's rows too many segments, for its tiles to take the term in ----
+// (There y has been rounded as the shared product's and is rounded once more as the sum: an operand of a whole product of any size and layout is not to be had unrounded.)
+// A wave for 16 rows of a segment and 128 columns, the rank 32 at a time; h in two values of T as in the gradients.  b is read as it lies, eight rows of the rank times eight
+// columns a lane, and turned with byte permutes, or, where it is contiguous along the rank, as fragments.  Bound by a few loads in a row; with multiply-adds in
+// float32 and h out of the scalar cache 7 rows of rank 64 took 67 us, 5.4 now.
 template <typename T, bool ALONG_RANK>
-__global__ void __launch_bounds__(64) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int parts) {
-    const RowTile rt = find_row_tile(term.gr, 16, (int)(blockIdx.x / parts));
+__global__ void __launch_bounds__(64) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int strips) {
+    const RowTile rt = find_row_tile(term.gr, 16, (int)(blockIdx.x / strips));
     if (rt.group < 0) return;
-    const int col = (int)(blockIdx.x % parts) * 512 + threadIdx.x * 8, m = rt.end - rt.begin, there = n - col;
-    if (there <= 0) return;
-    const float* h = term.h + (long long)rt.begin * term.rank;
-    const uint16_t* b = (const uint16_t*)term.b + rt.weight * term.b_ws + (long long)col * term.b_cs;
-    float acc[16][8];
+    const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15, rank = term.rank;
+    const int col = (int)(blockIdx.x % strips) * 128 + 8 * j, m = rt.end - rt.begin, left = n - col, by = pulled(left);
+    const bool cut = col - 8 * j + 128 > n && n % 8;                      // (the strip's last vector ends with the row)
+    const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)rt.begin * rank, (long long)m * rank * 4);
+    const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc((const uint16_t*)term.b + rt.weight * term.b_ws, ((rank - 1) * term.b_rs + (n - 1) * term.b_cs + 1) * 2);
+    const __amdgpu_buffer_rsrc_t y_rsrc = buffer_rsrc(y + rt.begin * y_rs, ((m - 1) * y_rs + n) * 2);
+    u32x4_t was[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++)
+    for (int v = 0; v < 4; v++) was[v] = __builtin_amdgcn_raw_buffer_load_b128(y_rsrc, (int)(4 * q + v < m && left > 0 ? (uint32_t)(((4 * q + v) * y_rs + col - by) * 2) : BUFFER_OOB), 0, 0);
+    f32x4_t acc[8];
 #pragma unroll
-        for (int v = 0; v < 8; v++) acc[i][v] = 0.f;
-    auto multiply = [&](const T (&bv)[8], int r) {
+    for (int f = 0; f < 8; f++) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < rank; k0 += 32) {
+        const int kk = k0 + 8 * q;
+        float hv[8];
+        u32x4_t raw[8], hi, lo;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            if (i < m) {                                                  // (uniform)
-                const float hr = h[(long long)i * term.rank + r];
+        for (int u = 0; u < 8; u++) hv[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(j < m && kk + u < rank ? (uint32_t)((j * rank + kk + u) * 4) : BUFFER_OOB), 0, 0));
+        if (ALONG_RANK && rank % 8 == 0) {
 #pragma unroll
-                for (int v = 0; v < 8; v++) acc[i][v] += hr * widen(bv[v]);
+            for (int f = 0; f < 8; f++) raw[f] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col + f < n && kk < rank ? (uint32_t)(((col + f) * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0);
+        } else if (ALONG_RANK) {
+#pragma unroll
+            for (int f = 0; f < 8; f++) {
+                uint32_t x[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col + f < n && kk + u < rank ? (uint32_t)(((col + f) * term.b_cs + kk + u) * 2) : BUFFER_OOB), 0, 0);
+#pragma unroll
+                for (int d = 0; d < 4; d++) raw[f][d] = x[2 * d] | x[2 * d + 1] << 16;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) raw[e] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(left > 0 && kk + e < rank ? (uint32_t)(((kk + e) * term.b_rs + col - by) * 2) : BUFFER_OOB), 0, 0);
+            if (cut) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) raw[e] = pull_into_place(raw[e], by);
             }
         }
-    };
-    if constexpr (ALONG_RANK) {
-        for (int r0 = 0; r0 < term.rank; r0 += 8) {
-            T cols[8][8], bv[8];
+        split_low<T>(hv, hi, lo);
 #pragma unroll
-            for (int v = 0; v < 8; v++) {
-                const u32x4_t x = load8(b + (v < there ? v : 0) * term.b_cs + r0, term.rank - r0);
-                __builtin_memcpy(cols[v], &x, 16);
+        for (int f = 0; f < 8; f++) {
+            u32x4_t b = raw[f];
+            if constexpr (!ALONG_RANK) {
+#pragma unroll
+                for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
             }
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                if (r0 + u < term.rank) {
-#pragma unroll
-                    for (int v = 0; v < 8; v++) bv[v] = cols[v][u];
-                    multiply(bv, r0 + u);
-                }
-            }
-        }
-    } else {
-#pragma unroll 4
-        for (int r = 0; r < term.rank; r++) {
-            T bv[8];
-            const u32x4_t x = load8(b + r * term.b_rs, there);
-            __builtin_memcpy(bv, &x, 16);
-            multiply(bv, r);
+            acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
+            acc[f] = sh_ops<T>::mma(lo, b, acc[f]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if (i >= m) continue;
-        uint16_t* p = y + (rt.begin + i) * y_rs + col;
+    for (int v = 0; v < 4; v++) {
+        if (4 * q + v >= m || left <= 0) continue;
+        const u32x4_t x = cut ? pull_into_place(was[v], by) : was[v];
         T o[8];
-        const u32x4_t was = load8(p, there);
-        __builtin_memcpy(o, &was, 16);
+        __builtin_memcpy(o, &x, 16);
 #pragma unroll
-        for (int v = 0; v < 8; v++) o[v] = round_to<T>(widen(o[v]) + acc[i][v]);
-        if (there >= 8) {
-            u32x4_t x;
-            __builtin_memcpy(&x, o, 16);
-            *(u32x4_odd_t*)p = x;
+        for (int f = 0; f < 8; f++) o[f] = round_to<T>(widen(o[f]) + acc[f][v]);
+        uint16_t* p = y + (rt.begin + 4 * q + v) * y_rs + col;
+        if (left >= 8) {
+            u32x4_t z;
+            __builtin_memcpy(&z, o, 16);
+            *(u32x4_odd_t*)p = z;
         } else {
 #pragma unroll
-            for (int v = 0; v < 7; v++)
-                if (v < there) p[v] = o[v].bits;
+            for (int f = 0; f < 7; f++)
+                if (f < left) p[f] = o[f].bits;
         }
     }
 }
 
-bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) { return (term.b_cs == 1 || term.b_rs == 1) && !path_disabled("mfma"); }
+bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) {
+    return shared.n >= 8 && shared.c_rs < (1ll << 22) && (term.b_cs == 1 || term.b_rs == 1) && (long long)term.rank * shared.n < (1 << 28) && term.rank < (1 << 22) && !path_disabled("mfma");
+}
 
 template <typename T>
 static int launch_expand(const GroupedArgs& shared, const AdapterTerm& term) {
-    const int parts = (shared.n + 511) / 512;
-    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups, 16) * parts;
+    const int strips = (shared.n + 127) / 128;
+    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups, 16) * strips;
     if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
-    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, parts);
+    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, strips);
+    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, strips);
     return check_launch("adapter_expand16_kernel") ? 0 : -1;
 }
 

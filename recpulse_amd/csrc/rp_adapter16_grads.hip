@@ -21,8 +21,8 @@ struct AdapterGrad {
     long long s_rs, out_ws, out_rs;
 };
 
-// NC: 16-row tiles of the rank; RAGGED: rows of s that are no whole 16-byte vectors, or start anywhere
-template <typename T, int NC, bool TRANSPOSED, bool RAGGED, int AG_WAVES>
+// NC: 16-row tiles of the rank
+template <typename T, int NC, bool TRANSPOSED, int AG_WAVES>
 __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int id) {
     constexpr int AG_THREADS = AG_WAVES * 64;
     extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH]
@@ -34,28 +34,21 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     const int strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
-    const uint16_t* S = s + n0;
+    const int left = width - n0 - 8 * j, by = pulled(left);
+    const bool cut = n0 + AG_COLS > width && width % 8;
     uint32_t s_off[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) s_off[e] = n0 + 8 * j < width ? (uint32_t)(((8 * q + e) * s_rs + 8 * j) * 2) : BUFFER_OOB;
+    for (int e = 0; e < 8; e++) s_off[e] = left > 0 ? (uint32_t)(((8 * q + e) * s_rs + n0 + 8 * j - by) * 2) : BUFFER_OOB;
     constexpr int SLOTS = 2;
     u32x4_t raw[SLOTS][8];
     float lv[SLOTS][NC][8];
     int end = 0;                                              // of the segment in hand
     auto request = [&](auto slotc, int row0) {
         constexpr int SL = decltype(slotc)::value;
-        if constexpr (RAGGED) {
+        const char* at = (const char*)(s + (long long)row0 * s_rs);       // (rows past the segment are another's: the descriptor ends with it)
+        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width) * 2 : 0);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int row = row0 + 8 * q + e;
-                raw[SL][e] = load8(S + (long long)row * s_rs + 8 * j, row < end ? width - n0 - 8 * j : 0);
-            }
-        } else {                                              // (rows past the segment are another's: the descriptor ends with it)
-            const char* at = (const char*)(S + (long long)row0 * s_rs);
-            const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width - n0) * 2 : 0);
-#pragma unroll
-            for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
-        }
+        for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
         const float* l = low + (long long)row0 * rank;
         const __amdgpu_buffer_rsrc_t l_rsrc = buffer_rsrc(l, row0 < end ? (long long)(end - row0) * rank * 4 : 0);
 #pragma unroll
@@ -77,6 +70,10 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
         u32x4_t hi[NC], lo[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) split_low<T>(lv[SL][c], hi[c], lo[c]);
+        if (cut) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) raw[SL][e] = pull_into_place(raw[SL][e], by);
+        }
 #pragma unroll
         for (int f = 0; f < 8; f++) {
             u32x4_t b;
@@ -128,17 +125,17 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
 }
 
 // dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads
-template <typename T, int NC, bool RAGGED, int AG_WAVES>
+template <typename T, int NC, int AG_WAVES>
 __global__ void __launch_bounds__(AG_WAVES * 64) adapter_grads16_kernel(AdapterGrad a, AdapterGrad b, RowGroups gr, int rank, int rank_blocks) {
     const int id = (int)blockIdx.x;
-    if (id < a.blocks) adapter_grad16_block<T, NC, true, RAGGED, AG_WAVES>(a, gr, rank, rank_blocks, id);
-    else adapter_grad16_block<T, NC, false, RAGGED, AG_WAVES>(b, gr, rank, rank_blocks, id - a.blocks);
+    if (id < a.blocks) adapter_grad16_block<T, NC, true, AG_WAVES>(a, gr, rank, rank_blocks, id);
+    else adapter_grad16_block<T, NC, false, AG_WAVES>(b, gr, rank, rank_blocks, id - a.blocks);
 }
 
-template <typename T, int NC, bool RAGGED, int AG_WAVES>
+template <typename T, int NC, int AG_WAVES>
 static int launch_grads_as(const AdapterGrad& a, const AdapterGrad& b, const RowGroups& gr, int rank, int rank_blocks) {
     constexpr int lds = AG_WAVES * 16 * AG_PITCH * 4;
-    auto kern = adapter_grads16_kernel<T, NC, RAGGED, AG_WAVES>;
+    auto kern = adapter_grads16_kernel<T, NC, AG_WAVES>;
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.blocks + b.blocks)), dim3(AG_WAVES * 64), lds, current_stream(), a, b, gr, rank, rank_blocks);
     return check_launch("adapter_grads16_kernel") ? 0 : -1;
@@ -147,7 +144,6 @@ static int launch_grads_as(const AdapterGrad& a, const AdapterGrad& b, const Row
 template <typename T, int NC>
 static int launch_grads(AdapterGrad a, AdapterGrad b, const RowGroups& gr, int rank) {
     const int rank_blocks = (rank + 16 * NC - 1) / (16 * NC);
-    bool ragged = false;
     long long both = 0;
     for (AdapterGrad* g : {&a, &b}) {
         g->strips = (g->width + AG_COLS - 1) / AG_COLS;
@@ -155,20 +151,18 @@ static int launch_grads(AdapterGrad a, AdapterGrad b, const RowGroups& gr, int r
         both += own;
         if (both > 0x3fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", both); return -1; }
         g->blocks = g->out ? (int)own : 0;
-        ragged = ragged || (g->out && (g->width % 8 || g->s_rs % 8 || ((uintptr_t)g->s & 15)));
     }
     // Eight waves share a workgroup's rows, four where there are workgroups enough to take a CU in twos (fp16, us, eight and four: 24 + 48 workgroups,
     // 2048 rows of 3 adapters, 1024 x 2048, rank 8, 9.7 / 11.4; 2 x 2048, 8192 rows of 32 adapters, 4096 x 4096, rank 64, 144 / 93).  The same for one gradient as for both: they have the same bits alone.
     const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    if (both >= 2 * cus) return ragged ? launch_grads_as<T, NC, true, 4>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, false, 4>(a, b, gr, rank, rank_blocks);
-    return ragged ? launch_grads_as<T, NC, true, 8>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, false, 8>(a, b, gr, rank, rank_blocks);
+    return both >= 2 * cus ? launch_grads_as<T, NC, 4>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, 8>(a, b, gr, rank, rank_blocks);
 }
 
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
     const bool transposed = low == LOW_B;
     const long long s_rs = transposed ? g.a_rs : g.b_rs, s_cs = transposed ? g.a_cs : g.b_cs, l_rs = transposed ? g.b_rs : g.a_rs, l_cs = transposed ? g.b_cs : g.a_cs;
     const int width = transposed ? g.k : g.n, rank = transposed ? g.n : g.k;
-    return s_cs == 1 && s_rs >= width && s_rs < (1ll << 22) && l_rs == rank && (l_cs == 1 || rank == 1) && rank < (1 << 20) && !path_disabled("mfma");
+    return width >= 8 && s_cs == 1 && s_rs >= width && s_rs < (1ll << 22) && l_rs == rank && (l_cs == 1 || rank == 1) && rank < (1 << 20) && !path_disabled("mfma");
 }
 
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype) {

@@ -68,20 +68,17 @@ struct AdapterTiles {
                             for (int u = 0; u < 8; u++) hv[i][u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(u < left ? at + 4 * u : BUFFER_OOB), 0, 0));
                         }
                     }
-                    if (term.b_rs == 1) {                     // (values past the rank are another column's: made zeros)
+                    if (term.b_rs == 1 && term.rank % 8 == 0) {
 #pragma unroll
                         for (int j = 0; j < TNI; j++) {
                             const int col = col0 + j * MT + fr;
-                            u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col < n && left > 0 ? (uint32_t)((col * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0);
-#pragma unroll
-                            for (int d = 0; d < 4; d++) x[d] &= left > 2 * d + 1 ? 0xFFFFFFFFu : left > 2 * d ? 0xFFFFu : 0u;
-                            bf[j] = __builtin_bit_cast(s16x8_t, x);
+                            bf[j] = __builtin_bit_cast(s16x8_t, __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col < n && left > 0 ? (uint32_t)((col * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0));
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < TNI; j++) {
                             const int col = col0 + j * MT + fr;
-                            const uint32_t at = (uint32_t)((kk * term.b_rs + col) * 2), step = (uint32_t)(term.b_rs * 2);
+                            const uint32_t at = (uint32_t)((kk * term.b_rs + col * term.b_cs) * 2), step = (uint32_t)(term.b_rs * 2);
                             uint32_t x[8];
 #pragma unroll
                             for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col < n && u < left ? at + u * step : BUFFER_OOB), 0, 0);

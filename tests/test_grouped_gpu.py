@@ -558,6 +558,17 @@ def test_adapter_linear(shape, dt):
         p.check_backward(p.backward(accumulate=1), accumulate=1)
 
 
+# ranks that are no whole vectors, rows that end and start inside one, widths below a vector, tiles of every edge
+ODD_ADAPTER_SHAPES = [(3, 2, 700, 264, 520, 5, 0), (2, 2, 300, 129, 515, 3, 1), (1, 1, 2000, 136, 264, 1, 0), (2, 2, 20, 5, 300, 4, 0), (2, 2, 20, 300, 5, 4, 0), (4, 2, 90, 9, 15, 12, 0),
+                      (20, 3, 1500, 264, 1032, 12, 7), (3, 2, 2100, 264, 2056, 7, 0), (48, 2, 400, 1031, 130, 64, 0), (5, 3, 70, 2040, 94, 33, 0), (1, 9, 1, 168, 93, 64, 0)]
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32], ids=ids_of)
+@pytest.mark.parametrize("shape", ODD_ADAPTER_SHAPES, ids=lambda s: "x".join(map(str, s[:6])))
+def test_adapter_linear_odd_sizes(shape, dt):
+    test_adapter_linear(shape, dt)
+
+
 @pytest.mark.parametrize("dt", [BF16, F32], ids=ids_of)
 def test_adapter_linear_without_any(dt):
     """No segment has an adapter: the layer is the shared projection, and the adapters' gradients are zeros."""
