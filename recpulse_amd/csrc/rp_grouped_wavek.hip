@@ -34,6 +34,16 @@ __device__ __forceinline__ void rows_block(const GroupedArgs& ga, int tiles_n, i
 template <typename E, int TM, int TN>
 __device__ __forceinline__ void weights_block(const GroupedArgs& ga, int tiles_k, int tiles_n, int slots, int id, unsigned char* lds) {
     const int w = id / slots, b = __builtin_amdgcn_readfirstlane(ga.gr.begin(w)), e = __builtin_amdgcn_readfirstlane(ga.gr.end(w));
+    if (b == e) {                                              // nothing to add up: zeros, or what is there
+        const int at = run_tile(id - w * slots, tiles_k * tiles_n), k0 = at / tiles_n * 16 * TM, n0 = at % tiles_n * 16 * TN;
+        if (at == tiles_k * tiles_n || ga.accumulate) return;
+        E* out = (E*)ga.C + w * ga.c_ws;
+        for (int i = threadIdx.x; i < 256 * TM * TN; i += 64 * GW_WAVES) {
+            const int r = k0 + i / (16 * TN), c = n0 + i % (16 * TN);
+            if (r < ga.k && c < ga.n) out[r * ga.c_rs + c] = (E)0;
+        }
+        return;
+    }
     const GemmArgs g{(E*)ga.C + w * ga.c_ws, (const E*)ga.A + b * ga.a_rs, (const E*)ga.B + b * ga.b_rs, nullptr,
                      1, ga.k, e - b, ga.n, 0, 1, ga.a_rs, 0, ga.b_rs, 1, 0, ga.c_rs, 1, ga.accumulate};
     gemm_wavekw_block<E, false, false, TM, TN, GW_WAVES>(g, tiles_k, tiles_n, id - w * slots, 1, lds);
@@ -46,17 +56,17 @@ __global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(TM * TN)) gro
 }
 
 // The input's gradient, the weights' and the bias's, as many of them as there are blocks for
-template <typename E, int T>
-__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(T * T)) grouped_backward_wavek_kernel(GroupedArgs x, GroupedArgs w, GroupedSums sums, int s_blocks, int x_blocks, int x_tiles_n,
+template <typename E, int TX, int TW>
+__global__ void __launch_bounds__(64 * GW_WAVES, gw_waves_per_simd(TX > TW ? TX * TX : TW * TW)) grouped_backward_wavek_kernel(GroupedArgs x, GroupedArgs w, GroupedSums sums, int s_blocks, int x_blocks, int x_tiles_n,
                                                                                                       int w_tiles_k, int w_tiles_n, int w_slots) {
     extern __shared__ __attribute__((aligned(16))) unsigned char wkw_lds[];
     const int id = (int)blockIdx.x;
     if (id < s_blocks) {
         if (id < sums.gr.weights * ((sums.cols + 63) / 64)) grouped_sums_block<E, GW_WAVES>(sums, id, (E*)wkw_lds);
     } else if (id - s_blocks < x_blocks) {
-        rows_block<E, true, T, T>(x, x_tiles_n, id - s_blocks, wkw_lds);
+        rows_block<E, true, TX, TX>(x, x_tiles_n, id - s_blocks, wkw_lds);
     } else {
-        weights_block<E, T, T>(w, w_tiles_k, w_tiles_n, w_slots, id - s_blocks - x_blocks, wkw_lds);
+        weights_block<E, TW, TW>(w, w_tiles_k, w_tiles_n, w_slots, id - s_blocks - x_blocks, wkw_lds);
     }
 }
 
@@ -71,18 +81,26 @@ static int launch_rows(const GroupedArgs& g) {
     return check_launch("grouped_rows_wavek_kernel") ? 0 : -1;
 }
 
-template <typename E, int T>
+template <typename E, int TX, int TW>
 static int launch_backward(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums) {
-    constexpr size_t smem_x = wkw_smem<E, true, true, T, T, GW_WAVES>(), smem_w = wkw_smem<E, false, false, T, T, GW_WAVES>(), most = smem_x > smem_w ? smem_x : smem_w;
+    constexpr size_t smem_x = wkw_smem<E, true, true, TX, TX, GW_WAVES>(), smem_w = wkw_smem<E, false, false, TW, TW, GW_WAVES>(), most = smem_x > smem_w ? smem_x : smem_w;
     constexpr size_t smem = most > 64 * 16 * sizeof(E) ? most : 64 * 16 * sizeof(E);
-    const int x_tiles_n = (x.n + 16 * T - 1) / (16 * T), w_tiles_k = (w.k + 16 * T - 1) / (16 * T), w_tiles_n = (w.n + 16 * T - 1) / (16 * T), w_slots = (w_tiles_k * w_tiles_n + 7) / 8 * 8;
-    const long long x_blocks = x.C ? (max_row_tiles(x.gr.rows, x.gr.groups, 16 * T) * x_tiles_n + 7) / 8 * 8 : 0, w_blocks = w.C ? (long long)w_slots * w.gr.weights : 0;
+    const int x_tiles_n = (x.n + 16 * TX - 1) / (16 * TX), w_tiles_k = (w.k + 16 * TW - 1) / (16 * TW), w_tiles_n = (w.n + 16 * TW - 1) / (16 * TW), w_slots = (w_tiles_k * w_tiles_n + 7) / 8 * 8;
+    const long long x_blocks = x.C ? (max_row_tiles(x.gr.rows, x.gr.groups, 16 * TX) * x_tiles_n + 7) / 8 * 8 : 0, w_blocks = w.C ? (long long)w_slots * w.gr.weights : 0;
     const long long s_blocks = sums.out ? (sum_blocks(sums) + 7) / 8 * 8 : 0;
-    auto kern = grouped_backward_wavek_kernel<E, T>;
+    auto kern = grouped_backward_wavek_kernel<E, TX, TW>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
     hipLaunchKernelGGL(kern, dim3((unsigned)(s_blocks + x_blocks + w_blocks)), dim3(64 * GW_WAVES), smem, current_stream(), x, w, sums, (int)s_blocks, (int)x_blocks, x_tiles_n,
                        w_tiles_k, w_tiles_n, w_slots);
     return check_launch("grouped_backward_wavek_kernel") ? 0 : -1;
+}
+
+template <typename E, int TX>
+static int launch_backward_weights(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int tw) {
+    if constexpr (sizeof(E) == 4) {
+        if (tw == 4) return launch_backward<E, TX, 4>(x, w, sums);
+    }
+    return tw == 2 ? launch_backward<E, TX, 2>(x, w, sums) : launch_backward<E, TX, 1>(x, w, sums);
 }
 
 constexpr long long GW_MAX_BLOCKS = (1ll << 32) / (64 * GW_WAVES) - 8;       // fewer than 2^32 threads a launch
@@ -114,19 +132,22 @@ static long long weights_tiles(const GroupedArgs& g, int t) { return (long long)
 static int rows_tile(const GroupedArgs& g, int dtype) {
     return rows_ok(g, dtype) ? wavek_tile(dtype, [&](int t) { return rows_tiles(g, t); }, [&](int t) { return g.b_cs != 1 || g.n >= 16 * t; }) : 0;
 }
-// One tile edge for both gradients, whichever of them (C not null) are asked for: they have the same bits alone and together
-static int backward_tile(const GroupedArgs& x, const GroupedArgs& w, int dtype) {
-    if ((x.C && (x.b_cs == 1 || !rows_ok(x, dtype))) || (w.C && !weights_ok(w, dtype))) return 0;
-    return wavek_tile(dtype, [&](int t) { return rows_tiles(x, t) + weights_tiles(w, t) + 16 + (long long)w.gr.weights * ((w.n + 63) / 64); }, [&](int t) { return w.k >= 16 * t && w.n >= 16 * t; });
+static int weights_tile(const GroupedArgs& g, int dtype) {
+    return weights_ok(g, dtype) ? wavek_tile(dtype, [&](int t) { return weights_tiles(g, t); }, [&](int t) { return g.k >= 16 * t && g.n >= 16 * t; }) : 0;
 }
 
 bool grouped_rows_wavek_takes(const GroupedArgs& g, int dtype) { return rows_tile(g, dtype) != 0; }
-bool grouped_backward_wavek_takes(const GroupedArgs& x, const GroupedArgs& w, int dtype) { return backward_tile(x, w, dtype) != 0; }
+bool grouped_backward_wavek_takes(const GroupedArgs& x, const GroupedArgs& w, int dtype) {
+    const long long tx = x.C ? rows_tile(x, dtype) : 1, tw = w.C ? weights_tile(w, dtype) : 1;
+    if (!tx || !tw || (x.C && x.b_cs == 1)) return false;
+    return (x.C ? rows_tiles(x, (int)tx) : 0) + (w.C ? weights_tiles(w, (int)tw) : 0) + (long long)w.gr.weights * ((w.n + 63) / 64) + 16 <= GW_MAX_BLOCKS;
+}
 
 int launch_grouped_backward_wavek(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int dtype) {
-    const int t = backward_tile(x, w, dtype);
-    if (dtype == RP_DTYPE_FLOAT64) return t == 2 ? launch_backward<double, 2>(x, w, sums) : launch_backward<double, 1>(x, w, sums);
-    return t == 4 ? launch_backward<float, 4>(x, w, sums) : t == 2 ? launch_backward<float, 2>(x, w, sums) : launch_backward<float, 1>(x, w, sums);
+    const int tx = x.C ? rows_tile(x, dtype) : 1, tw = w.C ? weights_tile(w, dtype) : 1;
+    if (dtype == RP_DTYPE_FLOAT64) return tx == 2 ? launch_backward_weights<double, 2>(x, w, sums, tw) : launch_backward_weights<double, 1>(x, w, sums, tw);
+    if (tx == 4) return launch_backward_weights<float, 4>(x, w, sums, tw);
+    return tx == 2 ? launch_backward_weights<float, 2>(x, w, sums, tw) : launch_backward_weights<float, 1>(x, w, sums, tw);
 }
 
 template <typename E, int T>
