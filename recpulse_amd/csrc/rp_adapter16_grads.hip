@@ -100,6 +100,13 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
                 request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
             });
     });
+    if (rounds == 0) {                                        // an adapter without rows: zeros, or what is there
+        for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate; i += AG_THREADS) {
+            const int r = r0 + (TRANSPOSED ? i % (16 * NC) : i / AG_COLS), col = n0 + (TRANSPOSED ? i / (16 * NC) : i % AG_COLS);
+            if (r < rank && col < width) out[w * out_ws + (TRANSPOSED ? col * out_rs + r : r * out_rs + col)] = round_to<T>(0.f);
+        }
+        return;
+    }
     static_for<0, NC>([&](auto cc) {
         constexpr int c = decltype(cc)::value;
         if (c) __syncthreads();

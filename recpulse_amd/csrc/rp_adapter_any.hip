@@ -1,7 +1,8 @@
 // An adapter's narrow products and the gradients of its factors for fp32, fp64 and operands of any strides, on scalar multiply-adds in the accumulate type.
 //
 // h[i] = scale x[i] . A_a has rank outputs a row and k products each: 64 x 64 tiles of it would leave most CUs without one and each with a long chain.
-// Here a workgroup owns eight rows and sixteen of the rank, and its sixteen groups of sixteen lanes share k.
+// Here a workgroup owns eight rows and sixteen of the rank, and its 64 (float64: 32) groups of sixteen lanes share k: the chain of loads is what bounds it
+// (fp32, 2 rows of 2293 and rank 64 14 us; 240 of 3672 and rank 16 in 44 segments 21).
 // dB_a = sum of h[i]^T dy[i] (and dA_a^T = sum of u[i]^T x[i]): a workgroup owns 64 columns and sixteen of the rank, a column a lane, and its sixteen waves share the
 // rows; the row's sixteen low values are uniform, one scalar load.
 #include "rp_grouped.h"
@@ -10,12 +11,14 @@
 
 namespace rp {
 
-constexpr int NR_ROWS = 8, NR_COLS = 16, NR_LANES = 16;          // rows and columns of a workgroup, lanes that share k
+constexpr int NR_ROWS = 8, NR_COLS = 16;                         // rows and columns of a workgroup
+template <typename A> constexpr int nr_lanes() { return sizeof(A) == 8 ? 32 : 64; }         // lanes that share k
 constexpr int NW_WAVES = 16;                                     // waves that share the rows
 
 template <typename T>
-__global__ void __launch_bounds__(NR_COLS * NR_LANES) narrow_rows_kernel(GroupedArgs g, int col_blocks) {
+__global__ void __launch_bounds__(NR_COLS * nr_lanes<typename traits<T>::acc>()) narrow_rows_kernel(GroupedArgs g, int col_blocks) {
     using A = typename traits<T>::acc;
+    constexpr int NR_LANES = nr_lanes<A>();
     __shared__ A sums[NR_LANES][NR_ROWS][NR_COLS + 1];
     const RowTile rt = find_row_tile(g.gr, NR_ROWS, (int)(blockIdx.x / col_blocks));
     if (rt.group < 0) return;
@@ -57,7 +60,9 @@ __global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedAr
     A acc[NR_COLS];
 #pragma unroll
     for (int r = 0; r < NR_COLS; r++) acc[r] = 0;
+    bool any = false;
     for_groups_of(g.gr, w, [&](int begin, int end) {
+        any = true;
 #pragma unroll 4
         for (int i = begin + wave; i < end; i += NW_WAVES) {
             const A v = col < width ? (A)widen(s[i * s_rs + col * s_cs]) : (A)0;
@@ -66,6 +71,11 @@ __global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedAr
             for (int r = 0; r < NR_COLS; r++) acc[r] += v * l[r0 + r < rank ? r0 + r : rank - 1];
         }
     });
+    if (!any) {                                                  // an adapter without rows: zeros, or what is there
+        const int r = TRANSPOSED ? threadIdx.x % NR_COLS : threadIdx.x / 64, c = TRANSPOSED ? threadIdx.x / NR_COLS : threadIdx.x % 64;
+        if (!g.accumulate && r0 + r < rank && strip * 64 + c < width) ((T*)g.C)[w * g.c_ws + (TRANSPOSED ? (strip * 64 + c) * g.c_rs + r0 + r : (r0 + r) * g.c_rs + strip * 64 + c)] = round_to<T>((A)0);
+        return;
+    }
 #pragma unroll
     for (int r = 0; r < NR_COLS; r++) sums[wave][r][lane] = acc[r];
     __syncthreads();
@@ -87,7 +97,7 @@ int launch_narrow_rows(const GroupedArgs& g, int dtype) {
     const int col_blocks = (g.n + NR_COLS - 1) / NR_COLS;
     const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, NR_ROWS) * col_blocks;
     if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(narrow_rows_kernel<T>, dim3((unsigned)blocks), dim3(NR_COLS * NR_LANES), 0, current_stream(), g, col_blocks));
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(narrow_rows_kernel<T>, dim3((unsigned)blocks), dim3(NR_COLS * nr_lanes<typename traits<T>::acc>()), 0, current_stream(), g, col_blocks));
     return check_launch("narrow_rows_kernel") ? 0 : -1;
 }
 

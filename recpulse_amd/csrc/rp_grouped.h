@@ -64,9 +64,9 @@ int launch_grouped_rows16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
-// The gradients in one launch on tiles of 64 or 128: those of x, w and sums whose output is not null; w row-major (rp_grouped_backward16*.hip)
-int launch_grouped_backward16_bf16(const GroupedArgs& x, const GroupedArgs& w, int edge, const GroupedSums& sums, bool ragged);
-int launch_grouped_backward16_f16(const GroupedArgs& x, const GroupedArgs& w, int edge, const GroupedSums& sums, bool ragged);
+// The gradients in one launch, the input's on tiles of 64 or 128, the weights' on no larger ones: those of x, w and sums whose output is not null; w row-major (rp_grouped_backward16*.hip)
+int launch_grouped_backward16_bf16(const GroupedArgs& x, int x_tile, const GroupedArgs& w, int w_tile, const GroupedSums& sums, bool ragged);
+int launch_grouped_backward16_f16(const GroupedArgs& x, int x_tile, const GroupedArgs& w, int w_tile, const GroupedSums& sums, bool ragged);
 
 // + h[i] . b_a for the rows i of adapter a: what a layer's adapters add to its shared product (strides of b in elements)
 struct AdapterTerm {

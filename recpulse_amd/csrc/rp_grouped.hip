@@ -72,7 +72,8 @@ static int grouped_weights(const GroupedArgs& g, int dtype) {
 
 // The gradients of one layer in one launch unless 256 x 256 tiles, whose workgroups stay on their CU, take one of them.  bf16, us, in launches of their own and in
 // one: 1999 rows of 6 groups, 519 -> 1031, 41 / 23; 4096 of 8 56 / 32; 8192 of 8, 1031 -> 2047, 187 / 150.  One tile edge for both, 128 from a round of the CUs on
-// (64 and 128: 3000 rows of 4 groups, 700 -> 1031, 360 tiles of 128, 32 / 25; 1999 of 6, 350 tiles, 23 / 23).
+// (64 and 128: 3000 rows of 4 groups, 700 -> 1031, 360 tiles of 128, 32 / 25; 1999 of 6, 350 tiles, 23 / 23), unless the weights' tiles alone leave CUs idle:
+// each adds up a whole group's rows (14949 rows of 3 groups, 504 -> 427, 48 tiles of 128, 92 / 77).
 static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const GroupedSums& sums, int dtype, int* result) {
     if (!x.C && !w.C) return false;
     if (!is16(dtype)) {
@@ -85,8 +86,8 @@ static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const 
     if (!tx.edge || !tw.edge || tx.edge == 256 || tw.edge == 256) return false;
     const bool ragged = tx.ragged || tw.ragged;
     const long long tiles128 = (x.C ? (long long)((x.gr.rows + 127) / 128) * ((x.n + 127) / 128) : 0) + (w.C ? (long long)((w.k + 127) / 128) * ((w.n + 127) / 128) * w.gr.weights : 0);
-    const int edge = tiles128 >= cus() ? 128 : 64;
-    *result = dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_backward16_bf16(x, w, edge, sums, ragged) : launch_grouped_backward16_f16(x, w, edge, sums, ragged);
+    const int x_tile = tiles128 >= cus() ? 128 : 64, w_tile = tw.edge < x_tile ? tw.edge : x_tile;
+    *result = dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_backward16_bf16(x, x_tile, w, w_tile, sums, ragged) : launch_grouped_backward16_f16(x, x_tile, w, w_tile, sums, ragged);
     return true;
 }
 

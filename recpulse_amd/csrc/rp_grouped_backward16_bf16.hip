@@ -3,9 +3,8 @@
 
 namespace rp {
 
-int launch_grouped_backward16_bf16(const GroupedArgs& x, const GroupedArgs& w, int edge, const GroupedSums& sums, bool ragged) {
-    if (edge == 128) return ragged ? launch_grouped_backward16<bf16_t, 128, M16_RAGGED>(x, w, sums) : launch_grouped_backward16<bf16_t, 128, M16_EDGE>(x, w, sums);
-    return ragged ? launch_grouped_backward16<bf16_t, 64, M16_RAGGED>(x, w, sums) : launch_grouped_backward16<bf16_t, 64, M16_EDGE>(x, w, sums);
+int launch_grouped_backward16_bf16(const GroupedArgs& x, int x_tile, const GroupedArgs& w, int w_tile, const GroupedSums& sums, bool ragged) {
+    return ragged ? launch_grouped_backward16_tiles<bf16_t, M16_RAGGED>(x, x_tile, w, w_tile, sums) : launch_grouped_backward16_tiles<bf16_t, M16_EDGE>(x, x_tile, w, w_tile, sums);
 }
 
 }  // namespace rp
