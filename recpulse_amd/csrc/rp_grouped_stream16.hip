@@ -104,7 +104,11 @@ static int launch_stream_t(const GroupedArgs& g, int dtype) {
     const size_t bytes = (size_t)want * g.gr.rows * g.n * sizeof(float);
     NullStreamScratch lease(bytes);
     void* block = nullptr;
-    if (!lease.ptr && stream_is_capturing() && rp_hip_malloc(&block, bytes) != 0) return -1;
+    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
+    if (block && !stream_is_capturing()) {                    // (taken and given back, so that the pool has it when the same call is recorded)
+        rp_hip_free(block);
+        block = nullptr;
+    }
     sg.partials = (float*)(lease.ptr ? lease.ptr : block);
     if (!sg.partials) return launch_stream_rows<T, 4>(g, sg);
     sg.nsplit = want;

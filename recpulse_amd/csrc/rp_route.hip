@@ -15,7 +15,7 @@
 namespace rp {
 
 constexpr int ROUTE_MAX_K = 16, ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_SLOTS = 1 << 30;
-constexpr int SORT_CHUNKS = 256;             // workgroups that a longer list is dealt to, at most
+constexpr int SORT_CHUNKS = 512;             // workgroups that a longer list is dealt to, at most
 
 // ---- order-preserving integer keys: larger logit, larger key; equal logits (+0 and -0 too), equal keys ----
 // 0 is "not there": an expert that is taken already, one past the last, or a logit of -inf.  NaN is above every number.
@@ -174,7 +174,7 @@ __device__ __forceinline__ void route_token(const T* row, bool live, int experts
 }
 
 // ---- the sort ----
-// Slots [s0, s1) by a workgroup of WAVES waves, each a run of whole 64s; where[e] is the place of the first one of expert e.
+// Slots [s0, s1) by a workgroup of WAVES waves, each a run of whole 64s; where[e] is the place of the first one of expert e.  position may be null.
 // counts: [WAVES][groups] in LDS, zeroed.  Lanes with the same expert find each other bit by bit (a ballot for each bit of the number).
 template <int WAVES>
 __device__ __forceinline__ void sort_slots(const int* ids, int s0, int s1, int groups, int bits, int* counts, const int* where, int* order, int* position) {
@@ -208,9 +208,9 @@ __device__ __forceinline__ void sort_slots(const int* ids, int s0, int s1, int g
         if (in) {
             const int place = first + before;
             order[place] = slot;
-            position[slot] = place;
+            if (position) position[slot] = place;
             if (before == 0) mine[id] = first + __builtin_popcountll(same);   // (one lane of each expert; the wave reads it in its next round)
-        } else if (slot < e) {
+        } else if (slot < e && position) {
             position[slot] = -1;
         }
         __builtin_amdgcn_wave_barrier();
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_count_kernel(const i
     __shared__ int own[ROUTE_MAX_EXPERTS];
     for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) own[g] = 0;
     __syncthreads();
-    const int s0 = blockIdx.x * chunk, s1 = count - s0 < chunk ? count : s0 + chunk;
+    const int s0 = blockIdx.x * chunk, s1 = blockIdx.x + 1 == gridDim.x ? count : s0 + chunk;
     count_ids(ids, s0, s1, groups, own);
     __syncthreads();
     for (int g = threadIdx.x; g < groups; g += SORT_ONE_WAVES * 64) counts[(size_t)blockIdx.x * groups + g] = own[g];
@@ -315,9 +315,18 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_place_kernel(const i
     if (own == 0)
         for (int g = threadIdx.x; g <= groups; g += SORT_ONE_WAVES * 64) offsets[g] = totals[g];
     __syncthreads();
-    const int s0 = own * chunk, s1 = count - s0 < chunk ? count : s0 + chunk;
+    const int s0 = own * chunk, s1 = own + 1 == chunks ? count : s0 + chunk;
     sort_slots<SORT_ONE_WAVES>(ids, s0, s1, groups, bits, sort_lds, where, order, position);
     for (long long s = (long long)totals[groups] + own * (SORT_ONE_WAVES * 64) + threadIdx.x; s < count; s += chunks * (SORT_ONE_WAVES * 64)) order[s] = -1;
+}
+
+// position from order, where the counts lay in position itself
+__global__ void __launch_bounds__(256) sort_invert_kernel(const int* ids, const int* order, int* position, int count, int groups) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
+        const int slot = order[i];
+        if (slot >= 0) position[slot] = (int)i;
+        if ((unsigned)ids[i] >= (unsigned)groups) position[i] = -1;
+    }
 }
 
 // ---- routing: kernels ----
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) route_topk_kernel(weight_
     __shared__ int own[ROUTE_MAX_EXPERTS];
     for (int g = threadIdx.x; g < experts; g += SORT_ONE_WAVES * 64) own[g] = 0;
     __syncthreads();
-    const int l = threadIdx.x % LANES, t0 = (int)blockIdx.x * per_block, t1 = tokens - t0 < per_block ? tokens : t0 + per_block;
+    const int l = threadIdx.x % LANES, t0 = (int)blockIdx.x * per_block, t1 = blockIdx.x + 1 == gridDim.x ? tokens : t0 + per_block;
     for (int t = t0 + threadIdx.x / LANES; t - (int)threadIdx.x / LANES < t1; t += SORT_ONE_WAVES * 64 / LANES) {      // (whole waves together)
         const bool live = t < t1;
         int expert;
@@ -342,6 +351,7 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) route_topk_kernel(weight_
             if (expert >= 0) atomicAdd(&own[expert], 1);
         }
     }
+    if (!counts) return;
     __syncthreads();
     for (int g = threadIdx.x; g < experts; g += SORT_ONE_WAVES * 64) counts[(size_t)blockIdx.x * experts + g] = own[g];
 }
@@ -429,24 +439,27 @@ static int bits_of(int groups) {
 // Lists up to this length are sorted by one workgroup in one launch
 constexpr int SORT_ONE_MAX = 4096;
 
-// The counts of a longer list: the null stream's own memory, or a block of the pool
+// The counts of a longer list lie in the null stream's own memory.  On other streams, whose calls would share a block of the pool, and in graphs they lie in `position`, which
+// a third launch then fills; there are no more of them than slots.
 struct SortCounts {
     NullStreamScratch lease;
-    void* block = nullptr;
-    explicit SortCounts(size_t ints) : lease(ints * sizeof(int)) {
-        if (!lease.ptr && rp_hip_malloc(&block, ints * sizeof(int)) != 0) block = nullptr;
-    }
-    ~SortCounts() { if (block) rp_hip_free(block); }
-    int* ptr() const { return (int*)(lease.ptr ? lease.ptr : block); }
+    int* position;
+    SortCounts(size_t ints, int* p) : lease(ints * sizeof(int)), position(p) {}
+    bool in_place() const { return !lease.ptr; }
+    int* ptr() const { return lease.ptr ? (int*)lease.ptr : position; }
 };
 
-static int launch_place(int* offsets, int* order, int* position, const int* ids, int count, int groups, int chunk, int chunks, const int* counts) {
+static int launch_place(int* offsets, int* order, int* position, const int* ids, int count, int groups, int chunk, int chunks, const SortCounts& counts) {
     int width = 32;
     while (width < groups) width *= 2;
     const size_t lds = ((size_t)(SORT_ONE_WAVES + 2) * groups + 1 + 2 * SORT_ONE_WAVES * 64) * sizeof(int);
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)sort_place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(sort_place_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), lds, current_stream(), ids, count, groups, bits_of(groups), chunk, SORT_ONE_WAVES * 64 / width, counts, offsets, order, position);
-    return check_launch("sort_place_kernel") ? 0 : -1;
+    hipLaunchKernelGGL(sort_place_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), lds, current_stream(), ids, count, groups, bits_of(groups), chunk, SORT_ONE_WAVES * 64 / width, counts.ptr(), offsets, order,
+                       counts.in_place() ? nullptr : position);
+    if (!check_launch("sort_place_kernel")) return -1;
+    if (!counts.in_place()) return 0;
+    hipLaunchKernelGGL(sort_invert_kernel, dim3(count / 256 < 1024 ? count / 256 + 1 : 1024), dim3(256), 0, current_stream(), ids, order, position, count, groups);
+    return check_launch("sort_invert_kernel") ? 0 : -1;
 }
 
 static int launch_sort_one(int* offsets, int* order, int* position, const int* ids, int count, int groups) {
@@ -458,12 +471,11 @@ static int launch_sort_one(int* offsets, int* order, int* position, const int* i
 
 static int launch_sort(int* offsets, int* order, int* position, const int* ids, int count, int groups) {
     if (count <= SORT_ONE_MAX) return launch_sort_one(offsets, order, position, ids, count, groups);
-    const int chunk = ((count + SORT_CHUNKS - 1) / SORT_CHUNKS + 511) / 512 * 512, chunks = (count + chunk - 1) / chunk;
-    const SortCounts counts((size_t)chunks * groups);
-    if (!counts.ptr()) return -1;
+    const int least = (count + SORT_CHUNKS - 1) / SORT_CHUNKS, chunk = ((least > groups ? least : groups) + 511) / 512 * 512, chunks = count / chunk;      // (a rest goes with the last)
+    const SortCounts counts((size_t)chunks * groups, position);
     hipLaunchKernelGGL(sort_count_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), ids, count, groups, chunk, counts.ptr());
     if (!check_launch("sort_count_kernel")) return -1;
-    return launch_place(offsets, order, position, ids, count, groups, chunk, chunks, counts.ptr());
+    return launch_place(offsets, order, position, ids, count, groups, chunk, chunks, counts);
 }
 
 template <typename T>
@@ -478,13 +490,18 @@ static int launch_route(void* weights, int* experts_out, int* offsets, int* orde
                                tokens, experts, k, normalize, bits_of(experts));
             return check_launch("route_one_kernel") ? 0 : -1;
         }
-        const int per_block = ((tokens + PER - 1) / PER + SORT_CHUNKS - 1) / SORT_CHUNKS * PER, chunks = (tokens + per_block - 1) / per_block;
-        const SortCounts counts((size_t)chunks * experts);
-        if (!counts.ptr()) return -1;
+        const int least = (tokens + SORT_CHUNKS - 1) / SORT_CHUNKS, whole = (experts + k - 1) / k, per_block = ((least > whole ? least : whole) + PER - 1) / PER * PER;
+        if (tokens < 2 * per_block) {                          // too few for chunks that hold their counts
+            hipLaunchKernelGGL((route_topk_kernel<T, LANES, V>), dim3((tokens + PER - 1) / PER), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), (weight_t<T>*)weights, experts_out, nullptr,
+                               (const T*)logits, rs, tokens, experts, k, normalize, PER);
+            return check_launch("route_topk_kernel") ? launch_sort(offsets, order, position, experts_out, tokens * k, experts) : -1;
+        }
+        const int chunks = tokens / per_block;                 // (a rest goes with the last)
+        const SortCounts counts((size_t)chunks * experts, position);
         hipLaunchKernelGGL((route_topk_kernel<T, LANES, V>), dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), (weight_t<T>*)weights, experts_out, counts.ptr(), (const T*)logits, rs,
                            tokens, experts, k, normalize, per_block);
         if (!check_launch("route_topk_kernel")) return -1;
-        return launch_place(offsets, order, position, experts_out, tokens * k, experts, per_block * k, chunks, counts.ptr());
+        return launch_place(offsets, order, position, experts_out, tokens * k, experts, per_block * k, chunks, counts);
     });
 }
 

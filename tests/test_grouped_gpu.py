@@ -714,3 +714,49 @@ def test_two_streams_at_once():
         capi.synchronize()
         for name in RESULTS:
             assert np.array_equal(here[name].numpy(), want[name]), name
+
+
+@pytest.mark.parametrize("t, e, k", [(3000, 130, 2), (20001, 8, 2), (40000, 64, 6), (700, 1000, 7), (9000, 1024, 1)])
+def test_routing_on_other_streams_and_in_graphs(t, e, k):
+    """Long lists are sorted with other memory there; the results are the null stream's."""
+    rng = np.random.default_rng(t)
+    logits = oracle.to_storage(rng.normal(0, 1, (t, e)), F32)
+    special_rows(logits, rng)
+    dlogits = Dev(logits, F32)
+    shapes = [(t * k,), (e + 1,), (t * k,), (t * k,)]
+    ids = rng.integers(-1, e + 1, t * k).astype(np.int32)
+    dids, sort = ints(ids), sort_want(ids.astype(np.int64), e)
+
+    def results(r):
+        return [r[0].numpy()] + [read_ints(b, s) for b, s in zip(r[1], shapes)]
+
+    def buffers():
+        return [capi.DeviceBuffer.from_numpy(np.full(n, 7, np.int32)) for n in (e + 1, t * k, t * k)]
+
+    def sort_into(outs):
+        call("rp_hip_group_rows", *(o.ptr for o in outs), dids.ptr, t * k, e)
+
+    def check_sort(outs):
+        for got, ref in zip(outs, sort):
+            assert np.array_equal(read_ints(got, np.shape(ref)), ref)
+
+    want = results(route(dlogits, e, t, e, k, 1, F32))
+    streams, outs, routed = [capi.Stream(), capi.Stream()], [buffers(), buffers()], []
+    for s, o in zip(streams, outs):                            # both at work at once
+        with s:
+            routed.append(route(dlogits, e, t, e, k, 1, F32))
+            sort_into(o)
+    capi.synchronize()
+    for r, o in zip(routed, outs):
+        check_sort(o)
+        for got, ref in zip(results(r), want):
+            assert np.array_equal(got, ref, equal_nan=True)
+    with streams[0]:
+        with capi.Graph.capture() as g:
+            sort_into(outs[0])
+        for _ in range(3):
+            for o in outs[0]:
+                call("rp_hip_memset", o.ptr, 0, o.nbytes)
+            g.launch()
+            capi.check(capi.lib().rp_hip_stream_synchronize(), "rp_hip_stream_synchronize")
+            check_sort(outs[0])
