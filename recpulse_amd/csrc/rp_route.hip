@@ -15,7 +15,7 @@
 namespace rp {
 
 constexpr int ROUTE_MAX_K = 16, ROUTE_MAX_EXPERTS = 1024, ROUTE_MAX_SLOTS = 1 << 30;
-constexpr int SORT_CHUNKS = 512;             // workgroups that a longer list is dealt to, at most
+constexpr int SORT_CHUNKS = 256;             // workgroups that a longer list is dealt to, at most
 
 // ---- order-preserving integer keys: larger logit, larger key; equal logits (+0 and -0 too), equal keys ----
 // 0 is "not there": an expert that is taken already, one past the last, or a logit of -inf.  NaN is above every number.
@@ -439,6 +439,12 @@ static int bits_of(int groups) {
 // Lists up to this length are sorted by one workgroup in one launch
 constexpr int SORT_ONE_MAX = 4096;
 
+// Chunks of a list; a short last one is joined to the one before where the counts would otherwise be more than the slots
+static int sort_chunks(int count, int chunk, int groups) {
+    const int chunks = (count - 1) / chunk + 1;
+    return (long long)chunks * groups > count ? chunks - 1 : chunks;
+}
+
 // The counts of a longer list lie in the null stream's own memory.  On other streams, whose calls would share a block of the pool, and in graphs they lie in `position`, which
 // a third launch then fills; there are no more of them than slots.
 struct SortCounts {
@@ -471,7 +477,7 @@ static int launch_sort_one(int* offsets, int* order, int* position, const int* i
 
 static int launch_sort(int* offsets, int* order, int* position, const int* ids, int count, int groups) {
     if (count <= SORT_ONE_MAX) return launch_sort_one(offsets, order, position, ids, count, groups);
-    const int least = (count + SORT_CHUNKS - 1) / SORT_CHUNKS, chunk = ((least > groups ? least : groups) + 511) / 512 * 512, chunks = count / chunk;      // (a rest goes with the last)
+    const int least = (count + SORT_CHUNKS - 1) / SORT_CHUNKS, chunk = ((least > groups ? least : groups) + 511) / 512 * 512, chunks = sort_chunks(count, chunk, groups);
     const SortCounts counts((size_t)chunks * groups, position);
     hipLaunchKernelGGL(sort_count_kernel, dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), ids, count, groups, chunk, counts.ptr());
     if (!check_launch("sort_count_kernel")) return -1;
@@ -496,7 +502,7 @@ static int launch_route(void* weights, int* experts_out, int* offsets, int* orde
                                (const T*)logits, rs, tokens, experts, k, normalize, PER);
             return check_launch("route_topk_kernel") ? launch_sort(offsets, order, position, experts_out, tokens * k, experts) : -1;
         }
-        const int chunks = tokens / per_block;                 // (a rest goes with the last)
+        const int chunks = sort_chunks(tokens * k, per_block * k, experts);
         const SortCounts counts((size_t)chunks * experts, position);
         hipLaunchKernelGGL((route_topk_kernel<T, LANES, V>), dim3(chunks), dim3(SORT_ONE_WAVES * 64), 0, current_stream(), (weight_t<T>*)weights, experts_out, counts.ptr(), (const T*)logits, rs,
                            tokens, experts, k, normalize, per_block);
