@@ -388,7 +388,8 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
  * empty group, and rows behind the last group are neither read nor written.  Operands: strides in elements, non-negative;
  * outputs overlap neither an operand nor each other.  All types; sums are in the accumulate type (float32, float64 for
  * float64) and rounded once, to nearest even; with accumulate_* the rounded product is added to what is there and the sum
- * rounded.  No entry takes a block of the pool except where its comment says so. */
+ * rounded.  No entry takes a block of the pool except where its comment says so, so that calls on several streams share nothing.
+ * An output's bits do not depend on which of an entry's outputs are asked for, nor on the stream, except where its comment says so. */
 
 /* Routing: each of `tokens` rows of logits (row stride logits_rs) is given its k largest entries, equal ones in the order of
  * their index; an entry of -inf is never taken (a padding token has nothing else), NaN is above every number.  Slot
@@ -397,7 +398,7 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
  * weights.)  The slots are then sorted by expert, in slot order within an expert: offsets[num_experts + 1], order[place] = slot
  * (-1 behind the last), position[slot] = place (-1 where none was left).
  * weights [tokens, k]: float32 (float64 for float64) whatever the logits' type; experts, order, position: int32 [tokens * k].
- * At most 1024 experts, k of 16 and 2^30 slots. */
+ * At most 1024 experts, k of 16 and 2^30 slots.  (On the null stream the sort of a longer list works in memory of that stream's own, elsewhere in `position`.) */
 int rp_hip_route_forward(void* weights, int* experts, int* offsets, int* order, int* position, const void* logits, long long logits_rs,
                          int tokens, int num_experts, int k, int normalize, int dtype);
 /* grad_logits [tokens, num_experts], dense, overwritten: the gradient of the weights with respect to the logits times grad_weights (entries of
@@ -423,7 +424,10 @@ int rp_hip_combine_backward(void* grad_z, void* grad_weights, const void* grad_y
 int rp_hip_zero_rows_behind(void* x, const int* offsets, int groups, int rows, int width, long long x_rs, int dtype);
 
 /* Grouped linear layer, one weight for each group: y[i] = x[i] . w_g + bias_g for the rows i of group g.  x [rows, k], w [groups, k, n] with strides
- * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for. */
+ * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for.
+ * 16-bit products of a few rows a group and k of 2048 or more may share k among workgroups where there would otherwise be too few of them: on the null stream, whose own memory
+ * then holds the partial sums, and in a graph being recorded, with a block of the pool that stays with the graph (a call on the same stream before the recording sees to it that
+ * the pool has one).  Other streams' calls do not: there the order of a sum, and so its last bit, may differ. */
 int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,
                                   long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients: dx[i] = dy[i] . w_g^T, dw_g = sum of x[i]^T dy[i], db_g = sum of dy[i] over the group's rows (zeros for an empty group).  dx [rows, k] with
@@ -437,7 +441,9 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  *   h[i] = scales[a] x[i] . a_a,   y[i] = x[i] . w + bias + h[i] . b_a       (rows without an adapter: y[i] = x[i] . w + bias)
  * x [rows, k], w [k, n], bias [n] or NULL, a [adapters, k, rank] and b [adapters, rank, n] dense, scales float32 [adapters] or NULL for ones, y [rows, n] with
  * unit column stride.  h [rows, rank], dense, in the accumulate type: written for rows with an adapter, kept by the caller for the backward pass.
- * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection. */
+ * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection.  16-bit types multiply h (and u below) by b (a) as two values of the type
+ * that add up to it to 2^-17 (float16: 2^-22), so float16 wants them within 65504; the term is rounded together with the shared product where that is on the same
+ * tiles or strips, otherwise (small outputs, or fewer than 16 rows a segment) added to the rounded product and rounded again. */
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
                                   int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):
