@@ -1,5 +1,6 @@
 // Grouped products of bf16 / fp16 on the tiles of the 16-bit MFMA kernel: the same workgroups as one product's (gemm_mfma16_block),
-// which take their tiles from the groups instead of from one matrix.
+// which take their tiles from the groups instead of from one matrix.  Bound as those are: large tiles by power (16384 rows of 16 groups, 4096 x 4096 in bf16: forward
+// 557 us, dx 548, 1.0 PFLOP/s; dw 584, 16 slabs a tile and 537 MB of output), small ones by the chain of their slabs.
 #pragma once
 #include "rp_gemm_mfma16_kernel.h"
 #include "rp_grouped.h"

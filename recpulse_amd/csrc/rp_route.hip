@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(ROUTE_ONE_THREADS) route_one_kernel(weight_t<T
     sort_all(ids, tokens * k, experts, bits, sort_lds, offsets, order, position);
 }
 
-// Gradient of the logits.  With p the softmax over the experts that the weights were divided by, and g_j the weights' gradients,
+// Gradient of the logits, bound by memory from about 10^5 tokens on (200000 of 128 in fp32 51 us, 4 TB/s; 16384 8 us).  With p the softmax over the experts that the weights were divided by, and g_j the weights' gradients,
 //   dl_e = p_e (g_e - sum over j of w_j g_j),   g_e = 0 where e was not taken; with "normalize" p_e = w_j where taken and 0 elsewhere.
 template <typename T, int LANES, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(T* grad, const weight_t<T>* grad_weights, const weight_t<T>* weights, const int* taken, const T* logits, long long rs,
@@ -523,7 +523,7 @@ static int launch_route_backward(void* grad, const void* grad_weights, const voi
 
 // ---- exchange: kernels ----
 // All of them are bound by memory: a row is read and written once, in pieces of 16 bytes where rows allow it (VEC elements;
-// otherwise element by element).
+// otherwise element by element).  8192 tokens of 4096 in bf16, two rows each: dispatch 31 us (5.9 TB/s), combine 42 (4.4), its gradient 68 (4.5).
 typedef __attribute__((ext_vector_type(4))) unsigned int row_vec_t;
 template <typename T, int VEC>
 struct Piece {
