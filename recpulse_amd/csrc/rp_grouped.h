@@ -28,7 +28,8 @@ __device__ __forceinline__ int run_tile(int id, int total) {
     return id / 8 < per && at < total ? at : total;
 }
 // Tile `at` of a matrix of rows x cols tiles: column by column through eight rows of tiles at a time, so that the tiles of a run that are
-// at work together need a few panels of both operands
+// at work together need a few panels of both operands.  (Row by row over all XCDs, every L2 fetched every weight: dx of 1999 rows of 6 groups, 1032 -> 520 in bf16 on
+// 64 x 64 tiles 18 us, 13.7 so.)
 __device__ __forceinline__ TileCoord chunk_tile(int at, int rows, int cols) {
     constexpr int CHUNK = 8;
     const int r0 = at / (CHUNK * cols) * CHUNK, h = rows - r0 < CHUNK ? rows - r0 : CHUNK, in = at - r0 * cols;

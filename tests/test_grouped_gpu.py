@@ -558,6 +558,57 @@ def test_adapter_linear(shape, dt):
         p.check_backward(p.backward(accumulate=1), accumulate=1)
 
 
+@pytest.mark.parametrize("dt", ALL, ids=ids_of)
+@pytest.mark.parametrize("pad", [8, 3])
+@pytest.mark.parametrize("shape", [(5, 3, 100, 72, 136, 8, 3), (3, 2, 700, 264, 520, 16, 0), (32, 5, 32, 256, 512, 16, 0), (4, 2, 90, 129, 95, 12, 2), (3, 3, 200, 40, 48, 200, 0)], ids=lambda s: "x".join(map(str, s[:6])))
+def test_adapter_linear_strides(shape, pad, dt):
+    """Rows of x, dy, y and dx further apart than they are long, NaN between them: never read, and never written."""
+    *sizes, behind = shape
+    segments, adapters, rows, k, n, rank = sizes
+    p = Adapters(dt, *sizes, behind=behind)
+
+    def wide(name, width, value):
+        a = oracle.to_storage(np.full((rows, width + pad), value), dt)
+        if name:
+            a[:, :width] = p.s[name]
+        return Dev(a, dt)
+
+    def dense(d, width):
+        a = d.numpy()
+        assert np.all(oracle.to_f64(a, dt)[:, width:] == 3.0)
+        return Dev(np.ascontiguousarray(a[:, :width]), dt)
+
+    x, g, y, dx = wide("x", k, np.nan), wide("g", n, np.nan), wide(None, n, 3.0), wide(None, k, 3.0)
+    p.h = Dev(np.full((rows, rank), 3.0, dtype=capi.NP_STORAGE[p.acc]), p.acc)
+    d = p.d
+    call("rp_hip_adapter_linear_forward", y.ptr, p.h.ptr, x.ptr, d["w"].ptr, ptr(d["bias"]), d["a"].ptr, d["b"].ptr, *p.plan(), k + pad, 1, *p.w_st, n + pad, dt)
+    p.y = dense(y, n)
+    p.check_forward()
+    u, da, db = Dev.empty((rows, rank), p.acc), Dev.empty((adapters, k, rank), dt), Dev.empty((adapters, rank, n), dt)
+    call("rp_hip_adapter_linear_backward", dx.ptr, da.ptr, db.ptr, u.ptr, g.ptr, x.ptr, d["w"].ptr, d["a"].ptr, d["b"].ptr, p.h.ptr, *p.plan(),
+         n + pad, k + pad, 1, *p.w_st, k + pad, 0, 0, 0, dt)
+    p.check_backward([dense(dx, k), da, db])
+
+
+@pytest.mark.parametrize("dt", ALL, ids=ids_of)
+@pytest.mark.parametrize("groups, rows, k, n", [(3, 90, 72, 136), (4, 700, 264, 520), (2, 20, 256, 128)])
+def test_grouped_linear_broadcast_operands(groups, rows, k, n, dt):
+    """One row for all rows of x or of dy, one weight for all groups, rows of x that overlap."""
+    p = Grouped(dt, groups, rows, k, n, nan=False)
+    dw, db = Dev.empty((groups, k, n), dt), Dev.empty((groups, n), dt)
+    y, dx = p.mark(rows, n), p.mark(rows, k)
+    flat = p.sx.reshape(-1)
+    x0, w0 = p.x, p.w
+    for x_rs, g_rs, w_gs in ((0, n, k * n), (k, 0, k * n), (k, n, 0), (0, 0, 0), (k // 2, n, k * n)):
+        p.x = oracle.to_f64(np.stack([flat[i * x_rs:i * x_rs + k] for i in range(rows)]), dt)
+        p.g = np.broadcast_to(oracle.to_f64(p.sg, dt)[:1], (rows, n)) if g_rs == 0 else oracle.to_f64(p.sg, dt)
+        p.w = np.broadcast_to(w0[:1], w0.shape) if w_gs == 0 else w0
+        call("rp_hip_grouped_linear_forward", y.ptr, p.dx.ptr, p.dw.ptr, ptr(p.db), p.do.ptr, groups, rows, k, n, x_rs, 1, w_gs, n, 1, n, dt)
+        p.check_forward(y)
+        call("rp_hip_grouped_linear_backward", dx.ptr, dw.ptr, db.ptr, p.dg.ptr, p.dx.ptr, p.dw.ptr, p.do.ptr, groups, rows, k, n, g_rs, x_rs, 1, w_gs, n, 1, k, 0, 0, 0, dt)
+        p.check_backward([dx, dw, db])
+
+
 # ranks that are no whole vectors, rows that end and start inside one, widths below a vector, tiles of every edge
 ODD_ADAPTER_SHAPES = [(3, 2, 700, 264, 520, 5, 0), (2, 2, 300, 129, 515, 3, 1), (1, 1, 2000, 136, 264, 1, 0), (2, 2, 20, 5, 300, 4, 0), (2, 2, 20, 300, 5, 4, 0), (4, 2, 90, 9, 15, 12, 0),
                       (20, 3, 1500, 264, 1032, 12, 7), (3, 2, 2100, 264, 2056, 7, 0), (48, 2, 400, 1031, 130, 64, 0), (5, 3, 70, 2040, 94, 33, 0), (1, 9, 1, 168, 93, 64, 0)]
