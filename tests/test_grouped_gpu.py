@@ -364,6 +364,16 @@ def test_grouped_linear(shape, dt):
     p.check_backward(p.backward(accumulate=1), accumulate=1)
 
 
+# sizes at which a product goes on tiles of 256 (forward; dx; dw) or of 128, aligned and ragged
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("shape", [(3, 4000, 512, 3584), (3, 4000, 3584, 512), (16, 16000, 1024, 1024), (8, 4100, 519, 1031), (7, 2500, 264, 2056)], ids=lambda s: "x".join(map(str, s)))
+def test_grouped_linear_large_tiles(shape, dt):
+    groups, rows, k, n = shape
+    p = Grouped(dt, groups, rows, k, n, empty=(1,), behind=5)
+    p.check_forward(p.forward())
+    p.check_backward(p.backward(accumulate=1), accumulate=1)
+
+
 @pytest.mark.parametrize("dt", ALL, ids=ids_of)
 @pytest.mark.parametrize("pad, transposed", [(8, False), (3, False), (0, True), (8, True), (5, True)])
 def test_grouped_linear_strides(pad, transposed, dt):
@@ -618,6 +628,17 @@ ODD_ADAPTER_SHAPES = [(3, 2, 700, 264, 520, 5, 0), (2, 2, 300, 129, 515, 3, 1), 
 @pytest.mark.parametrize("shape", ODD_ADAPTER_SHAPES, ids=lambda s: "x".join(map(str, s[:6])))
 def test_adapter_linear_odd_sizes(shape, dt):
     test_adapter_linear(shape, dt)
+
+
+# the shared product on tiles of 256 and of 128, aligned and ragged, the rank in one and in several steps
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("shape", [(5, 3, 4100, 512, 4096, 32, 0), (5, 3, 4096, 4096, 512, 100, 6), (3, 2, 2049, 1031, 4099, 12, 0), (7, 4, 2048, 520, 2048, 8, 0)], ids=lambda s: "x".join(map(str, s[:6])))
+def test_adapter_linear_large_tiles(shape, dt):
+    *sizes, behind = shape
+    p = Adapters(dt, *sizes, behind=behind)
+    p.forward()
+    p.check_forward()
+    p.check_backward(p.backward(accumulate=1), accumulate=1)
 
 
 @pytest.mark.parametrize("dt", [BF16, F32], ids=ids_of)
