@@ -23,16 +23,20 @@ __global__ void __launch_bounds__(256) stream16_combine_kernel(GroupedArgs g, St
 #pragma unroll
         for (int v = 0; v < 4; v++) { s[v] += lo[v]; s[4 + v] += hi[v]; }
     }
-    // the row's group: how many end at or before the row (uniform: the same loads for the whole workgroup)
+    // the weight of the row's group: a wave looks at 64 groups at a time
     auto weight_of = [&](const RowGroups& gr) {
-        int before = 0;
-        for (int i = 0; i < gr.groups; i++) before += gr.end(i) <= row ? 1 : 0;
-        return before < gr.groups && gr.begin(before) <= row ? gr.weight(before) : -1;
+        const int lane = threadIdx.x & 63;
+        for (int g0 = 0; g0 < gr.groups; g0 += 64) {
+            const bool in = g0 + lane < gr.groups;
+            const int b = in ? gr.begin(g0 + lane) : 0, e = in ? gr.end(g0 + lane) : 0, w = in ? gr.weight(g0 + lane) : -1;
+            const unsigned long long here = __builtin_amdgcn_ballot_w64(b <= row && row < e);
+            if (here) return __builtin_amdgcn_readlane(w, __builtin_ctzll(here));
+        }
+        return -1;
     };
-    const int w = weight_of(g.gr);
+    const int a = term.h ? weight_of(term.gr) : -1, w = weight_of(g.gr);
     if (w < 0) return;                                       // (the whole workgroup)
-    if (term.h) {
-        const int a = weight_of(term.gr);
+    {
         if (a >= 0 && in) {
             const float* h = term.h + (long long)row * term.rank;
             const uint16_t* b = (const uint16_t*)term.b + a * term.b_ws + col;
