@@ -46,7 +46,7 @@ bool adapter_shrink16_takes(const GroupedArgs& g) {
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype) { return dtype == RP_DTYPE_BFLOAT16 ? launch_shrink_rank<bf16_t>(g) : launch_shrink_rank<f16_t>(g); }
 
 // ---- a few rows: the shared projection's shares of k and the rows' h side by side, then one launch that adds them up with the adapters' terms ----
-// 32 rows with adapters of their own, 4096 x 4096 and rank 16 in bf16: 17.9 us and 6.9 (6.1 for the narrow products by themselves and 12.1 for the shared one).
+// 32 rows with adapters of their own, 4096 x 4096 and rank 16 in bf16: 16.5 us and 4.1 (6.1 for the narrow products by themselves and 12.1 for the shared one).
 template <typename T, int CPL, int RB, int NC>
 __global__ void __launch_bounds__(GS_THREADS) adapter_first16_kernel(GroupedArgs shared, StreamGrid sg, GroupedArgs low, int low_blocks) {
     if ((int)blockIdx.x < low_blocks) adapter_shrink16_block<T, NC, 1, false, 8, GS_WAVES>(low, (int)blockIdx.x);

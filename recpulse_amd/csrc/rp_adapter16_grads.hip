@@ -1,168 +1,15 @@
-// bf16 / fp16 gradients of an adapter's factors: D_a = sum over the rows i of adapter a of low[i]^T . s[i], low [rows, rank] in float32, s [rows, width].
-// With low = h and s = dy this is dB_a [rank, n]; with low = u and s = x it is dA_a^T, stored transposed.
-//
-// Bound by reading s, once per 32 of the rank: a workgroup owns one adapter, a strip of 128 columns of s and up to 32 of the rank, and its waves
-// share the rows of the adapter's segments, 32 at a time in turn.  s goes from memory to registers to v_mfma_f32_16x16x32 as a
-// weight does in the kernel for few rows (rp_grouped_stream16.h): a lane transposes 8 rows x 8 columns with byte permutes.  low is
-// rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, and values beyond 65504 overflow), a product each: h and u are
-// sums in float32, and one rounding of theirs would be as large as the result's own.
-#include "rp_adapter16.h"
-#include "rp_grouped_stream16.h"
+// The gradients of adapters' factors in a launch of their own, where dx is not asked for or goes on tiles of 256.
+#include "rp_adapter16_grads.h"
 
 namespace rp {
 
-constexpr int AG_COLS = 128, AG_PITCH = AG_COLS + 4;
-
-struct AdapterGrad {
-    void* out;                     // null: not asked for
-    const void* s;
-    const float* low;
-    int width, accumulate, strips, blocks;
-    long long s_rs, out_ws, out_rs;
-};
-
-// NC: 16-row tiles of the rank
-template <typename T, int NC, bool TRANSPOSED, int AG_WAVES>
-__device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int id) {
-    constexpr int AG_THREADS = AG_WAVES * 64;
-    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH]
-    T* out = (T*)ag.out;
-    const uint16_t* s = (const uint16_t*)ag.s;
-    const float* low = ag.low;
-    const int width = ag.width, accumulate = ag.accumulate;
-    const long long s_rs = ag.s_rs, out_ws = ag.out_ws, out_rs = ag.out_rs;
-    const int strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
-    const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
-    const int left = width - n0 - 8 * j, by = pulled(left);
-    const bool cut = n0 + AG_COLS > width && width % 8;
-    uint32_t s_off[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) s_off[e] = left > 0 ? (uint32_t)(((8 * q + e) * s_rs + n0 + 8 * j - by) * 2) : BUFFER_OOB;
-    constexpr int SLOTS = 2;
-    u32x4_t raw[SLOTS][8];
-    float lv[SLOTS][NC][8];
-    int end = 0;                                              // of the segment in hand
-    auto request = [&](auto slotc, int row0) {
-        constexpr int SL = decltype(slotc)::value;
-        const char* at = (const char*)(s + (long long)row0 * s_rs);       // (rows past the segment are another's: the descriptor ends with it)
-        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width) * 2 : 0);
-#pragma unroll
-        for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
-        const float* l = low + (long long)row0 * rank;
-        const __amdgpu_buffer_rsrc_t l_rsrc = buffer_rsrc(l, row0 < end ? (long long)(end - row0) * rank * 4 : 0);
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int r = r0 + 16 * c + j;
-                lv[SL][c][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(l_rsrc, r < rank ? ((8 * q + e) * rank + r) * 4 : (int)BUFFER_OOB, 0, 0));
-            }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    f32x4_t acc[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-        for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](auto slotc) {
-        constexpr int SL = decltype(slotc)::value;
-        u32x4_t hi[NC], lo[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c++) split_low<T>(lv[SL][c], hi[c], lo[c]);
-        if (cut) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) raw[SL][e] = pull_into_place(raw[SL][e], by);
-        }
-#pragma unroll
-        for (int f = 0; f < 8; f++) {
-            u32x4_t b;
-#pragma unroll
-            for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[SL][2 * d + 1][f / 2], raw[SL][2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-                acc[c][f] = gs_ops<T>::mma(hi[c], b, acc[c][f]);
-                acc[c][f] = gs_ops<T>::mma(lo[c], b, acc[c][f]);
-            }
-        }
-    };
-    int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
-    for_groups_of(gr, w, [&](int begin, int stop) {
-        end = stop;
-        constexpr int turn = AG_WAVES * GS_ROUND;
-        const int first = begin + ((wave - rounds) & (AG_WAVES - 1)) * GS_ROUND;
-        rounds += (end - begin + GS_ROUND - 1) / GS_ROUND;
-        if (first >= end) return;
-        static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
-        for (int row0 = first; row0 < end; row0 += SLOTS * turn)
-            static_for<0, SLOTS>([&](auto sc) {
-                multiply(sc);
-                request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
-            });
-    });
-    if (rounds == 0) {                                        // an adapter without rows: zeros, or what is there
-        for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate; i += AG_THREADS) {
-            const int r = r0 + (TRANSPOSED ? i % (16 * NC) : i / AG_COLS), col = n0 + (TRANSPOSED ? i / (16 * NC) : i % AG_COLS);
-            if (r < rank && col < width) out[w * out_ws + (TRANSPOSED ? col * out_rs + r : r * out_rs + col)] = round_to<T>(0.f);
-        }
-        return;
-    }
-    static_for<0, NC>([&](auto cc) {
-        constexpr int c = decltype(cc)::value;
-        if (c) __syncthreads();
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-#pragma unroll
-            for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = acc[c][f][v];
-        __syncthreads();
-        // four outputs a thread, neighbours along the output's rows
-#pragma unroll
-        for (int o = 0; o < 16 * AG_COLS / AG_THREADS; o++) {
-            const int id = threadIdx.x + o * AG_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
-            if (r0 + 16 * c + r >= rank || n0 + col >= width) continue;
-            float t = gs_sums[r * AG_PITCH + col];
-#pragma unroll
-            for (int p = 1; p < AG_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
-            T* at = out + w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
-            T y = round_to<T>(t);
-            if (accumulate) y = round_to<T>(widen(*at) + widen(y));
-            *at = y;
-        }
-    });
-}
-
-// dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads
-template <typename T, int NC, int AG_WAVES>
-__global__ void __launch_bounds__(AG_WAVES * 64) adapter_grads16_kernel(AdapterGrad a, AdapterGrad b, RowGroups gr, int rank, int rank_blocks) {
-    const int id = (int)blockIdx.x;
-    if (id < a.blocks) adapter_grad16_block<T, NC, true, AG_WAVES>(a, gr, rank, rank_blocks, id);
-    else adapter_grad16_block<T, NC, false, AG_WAVES>(b, gr, rank, rank_blocks, id - a.blocks);
-}
-
-template <typename T, int NC, int AG_WAVES>
-static int launch_grads_as(const AdapterGrad& a, const AdapterGrad& b, const RowGroups& gr, int rank, int rank_blocks) {
-    constexpr int lds = AG_WAVES * 16 * AG_PITCH * 4;
-    auto kern = adapter_grads16_kernel<T, NC, AG_WAVES>;
-    if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.blocks + b.blocks)), dim3(AG_WAVES * 64), lds, current_stream(), a, b, gr, rank, rank_blocks);
-    return check_launch("adapter_grads16_kernel") ? 0 : -1;
-}
+template <typename T, int NC>
+__global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr) { adapter_grads16_block<T, NC>(ag, gr, (int)blockIdx.x); }
 
 template <typename T, int NC>
-static int launch_grads(AdapterGrad a, AdapterGrad b, const RowGroups& gr, int rank) {
-    const int rank_blocks = (rank + 16 * NC - 1) / (16 * NC);
-    long long both = 0;
-    for (AdapterGrad* g : {&a, &b}) {
-        g->strips = (g->width + AG_COLS - 1) / AG_COLS;
-        const long long own = (long long)g->strips * rank_blocks * gr.weights;
-        both += own;
-        if (both > 0x3fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", both); return -1; }
-        g->blocks = g->out ? (int)own : 0;
-    }
-    // Eight waves share a workgroup's rows, four where there are workgroups enough to take a CU in twos (fp16, us, eight and four: 24 + 48 workgroups,
-    // 2048 rows of 3 adapters, 1024 x 2048, rank 8, 9.7 / 11.4; 2 x 2048, 8192 rows of 32 adapters, 4096 x 4096, rank 64, 144 / 93).  The same for one gradient as for both: they have the same bits alone.
-    const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-    return both >= 2 * cus ? launch_grads_as<T, NC, 4>(a, b, gr, rank, rank_blocks) : launch_grads_as<T, NC, 8>(a, b, gr, rank, rank_blocks);
+static int launch_grads(const AdapterGrads& ag, const RowGroups& gr) {
+    hipLaunchKernelGGL((adapter_grads16_kernel<T, NC>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), AG_LDS, current_stream(), ag, gr);
+    return check_launch("adapter_grads16_kernel") ? 0 : -1;
 }
 
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
@@ -173,11 +20,11 @@ bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
 }
 
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
-    const AdapterGrad a{da.C, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
-    const AdapterGrad b{db.C, db.B, (const float*)db.A, db.n, db.accumulate, 0, 0, db.b_rs, db.c_ws, db.c_rs};
-    const int rank = da.n;
-    if (dtype == RP_DTYPE_BFLOAT16) return rank <= 16 ? launch_grads<bf16_t, 1>(a, b, da.gr, rank) : launch_grads<bf16_t, 2>(a, b, da.gr, rank);
-    return rank <= 16 ? launch_grads<f16_t, 1>(a, b, da.gr, rank) : launch_grads<f16_t, 2>(a, b, da.gr, rank);
+    AdapterGrads ag;
+    if (!plan_grads(da, db, ag)) return -1;
+    const bool one = grads_rank_tiles(ag.rank) == 1;
+    if (dtype == RP_DTYPE_BFLOAT16) return one ? launch_grads<bf16_t, 1>(ag, da.gr) : launch_grads<bf16_t, 2>(ag, da.gr);
+    return one ? launch_grads<f16_t, 1>(ag, da.gr) : launch_grads<f16_t, 2>(ag, da.gr);
 }
 
 }  // namespace rp

@@ -97,6 +97,9 @@ int launch_adapter_tiles16_64(const GroupedArgs& shared, const AdapterTerm& term
 // the gradients of an adapter's factors (rp_adapter16_grads.hip): by weights, LOW_A (dB) or LOW_B (dA)
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low);
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype);       // those whose C is not null
+// both, and dx with its term on tiles of 64 or 128 (w row-major), in one launch (rp_adapter16_backward*.hip)
+int launch_adapter_backward16_bf16(const GroupedArgs& shared, const AdapterTerm& term, const GroupedArgs& da, const GroupedArgs& db, int tile, bool ragged);
+int launch_adapter_backward16_f16(const GroupedArgs& shared, const AdapterTerm& term, const GroupedArgs& da, const GroupedArgs& db, int tile, bool ragged);
 // The whole layer for a few rows: `shared` one group of all rows, `low` the product above, `term` what it adds
 bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term);
 int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype);

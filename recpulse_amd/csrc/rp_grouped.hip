@@ -93,29 +93,39 @@ static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const 
 
 // An adapter's narrow product (C is h or u) and the gradients of its factors
 static int narrow_rows(const GroupedArgs& g, int dtype) { return is16(dtype) && adapter_shrink16_takes(g) ? launch_adapter_shrink16(g, dtype) : launch_narrow_rows(g, dtype); }
-static int narrow_weights(GroupedArgs da, GroupedArgs db, int dtype) {
-    if (is16(dtype) && (da.C || db.C) && (!da.C || adapter_grad16_takes(da, LOW_B)) && (!db.C || adapter_grad16_takes(db, LOW_A))) return launch_adapter_grads16(da, db, dtype);
+static bool grads16_takes(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
+    return is16(dtype) && (da.C || db.C) && (!da.C || adapter_grad16_takes(da, LOW_B)) && (!db.C || adapter_grad16_takes(db, LOW_A));
+}
+static int narrow_weights(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
+    if (grads16_takes(da, db, dtype)) return launch_adapter_grads16(da, db, dtype);
     if (da.C && launch_narrow_weights(da, LOW_B, dtype) != 0) return -1;
     return db.C ? launch_narrow_weights(db, LOW_A, dtype) : 0;
 }
 
-// The shared product of a layer with adapters, and the adapters' term
+// Tiles on which the shared product of a layer with adapters takes their term in (edge 0: none); whole: nothing hangs over
+struct TermTile { int edge; bool whole, ragged; };
+static TermTile term_tile(const GroupedArgs& s, const AdapterTerm& term, int dtype) {
+    if (!is16(dtype) || s.a_cs != 1 || (s.b_cs != 1 && s.b_rs != 1) || path_disabled("mfma") || path_disabled("adapter_tiles")) return {0, false, false};
+    Plan p{FAM_MFMA16, 64, 64, false, s.b_cs == 1, true, ""};
+    const Lie lie = worse(lies(s.A, s.a_rs, 0, s.k, 2), p.b_mc ? lies(s.B, s.b_rs, 0, s.n, 2) : lies(s.B, s.b_cs, 0, s.k, 2));
+    p.ragged = lie == LIE_RAGGED;
+    choose_tile16(p, 1, s.gr.rows, s.k, s.n);
+    if (p.ragged && p.bm == 256) p.bm = p.bn = 128;
+    // (fp16, 2048 rows of 2048 -> 1024, rank 8, 128 tiles of 128: 26 us, on 64 x 64 tiles 22)
+    if (p.bm == 128 && (long long)((s.gr.rows + 127) / 128) * ((s.n + 127) / 128) * 4 < cus() * 3) p.bm = p.bn = 64;
+    const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
+    // byte offsets into h and into an adapter's factor in 32 bits
+    const bool reach = (long long)s.gr.rows * term.rank < (1 << 29) && ((term.rank - 1) * term.b_rs + (s.n - 1) * term.b_cs) < (1 << 30);
+    // from about a tile for every other CU on, and while a tile's rows are few segments: each costs it 2 us
+    if (!reach || lie == LIE_NEITHER || p.bm != p.bn || tiles * 2 < cus() || term.gr.rows / term.gr.groups < 16) return {0, false, false};
+    return {p.bm, !p.edge, p.ragged};
+}
+
+// The shared product and the adapters' term
 static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int dtype) {
-    if (is16(dtype) && s.a_cs == 1 && (s.b_cs == 1 || s.b_rs == 1) && !path_disabled("mfma")) {
-        Plan p{FAM_MFMA16, 64, 64, false, s.b_cs == 1, true, ""};
-        const Lie lie = worse(lies(s.A, s.a_rs, 0, s.k, 2), p.b_mc ? lies(s.B, s.b_rs, 0, s.n, 2) : lies(s.B, s.b_cs, 0, s.k, 2));
-        p.ragged = lie == LIE_RAGGED;
-        choose_tile16(p, 1, s.gr.rows, s.k, s.n);
-        if (p.ragged && p.bm == 256) p.bm = p.bn = 128;
-        // (fp16, 2048 rows of 2048 -> 1024, rank 8, 128 tiles of 128: 26 us, on 64 x 64 tiles 22)
-        if (p.bm == 128 && (long long)((s.gr.rows + 127) / 128) * ((s.n + 127) / 128) * 4 < cus() * 3) p.bm = p.bn = 64;
-        const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
-        // from about a tile for every other CU on, and while a tile's rows are few segments': each costs it 2 us
-        if (lie != LIE_NEITHER && p.bm == p.bn && !path_disabled("adapter_tiles") && tiles * 2 >= cus() && term.gr.rows / term.gr.groups >= 16) {
-            if (p.bm == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_tiles16_256_bf16(s, term, p.edge) : launch_adapter_tiles16_256_f16(s, term, p.edge);
-            return p.bm == 128 ? launch_adapter_tiles16_128(s, term, p.edge, p.ragged, dtype) : launch_adapter_tiles16_64(s, term, p.ragged, dtype);
-        }
-    }
+    const TermTile t = term_tile(s, term, dtype);
+    if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_tiles16_256_bf16(s, term, !t.whole) : launch_adapter_tiles16_256_f16(s, term, !t.whole);
+    if (t.edge) return t.edge == 128 ? launch_adapter_tiles16_128(s, term, !t.whole, t.ragged, dtype) : launch_adapter_tiles16_64(s, term, t.ragged, dtype);
     if (rp_hip_gemm_strided_batched(s.C, s.A, s.B, s.bias, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate, dtype) != 0) return -1;
     if (is16(dtype) && adapter_expand16_takes(s, term)) return launch_adapter_expand16(s, term, dtype);
     return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, true, dtype);
@@ -194,12 +204,18 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, ids, segments, rows, adapters};
     if ((dx || da) && narrow_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, dtype) != 0) return -1;
+    const GroupedArgs ga{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0};
+    const GroupedArgs gb{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0};
     if (dx) {
         const GroupedArgs shared{dx, dy, w, nullptr, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, n, k, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
-        if (shared_with_term(shared, AdapterTerm{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank}, dtype) != 0) return -1;
+        const AdapterTerm term{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank};
+        const TermTile t = term_tile(shared, term, dtype);
+        // dx and the factors' gradients in one launch, unless workgroups that stay on their CU take dx
+        if (t.edge && t.edge < 256 && shared.b_rs == 1 && grads16_takes(ga, gb, dtype))
+            return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_backward16_bf16(shared, term, ga, gb, t.edge, t.ragged) : launch_adapter_backward16_f16(shared, term, ga, gb, t.edge, t.ragged);
+        if (shared_with_term(shared, term, dtype) != 0) return -1;
     }
-    return narrow_weights(GroupedArgs{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0},
-                          GroupedArgs{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0}, dtype);
+    return narrow_weights(ga, gb, dtype);
 }
 
 }  // extern "C"
