@@ -524,6 +524,8 @@ static int launch_route_backward(void* grad, const void* grad_weights, const voi
 // ---- exchange: kernels ----
 // All of them are bound by memory: a row is read and written once, in pieces of 16 bytes where rows allow it (VEC elements;
 // otherwise element by element).  8192 tokens of 4096 in bf16, two rows each: dispatch 31 us (5.9 TB/s), combine 42 (4.4), its gradient 68 (4.5).
+// (Stores that stream past the caches make combine 34 and its gradient 61, and whoever reads the rows next slower by more: dispatch and a kernel that reads its 134 MB
+// take 66 us, 91 with them.)
 typedef __attribute__((ext_vector_type(4))) unsigned int row_vec_t;
 template <typename T, int VEC>
 struct Piece {
