@@ -154,7 +154,7 @@ static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, Adap
     for (AdapterGrad* g : {&ag.a, &ag.b}) {
         g->strips = (g->width + AG_COLS - 1) / AG_COLS;
         const long long blocks = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights : 0;
-        if (blocks > 0x1fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", blocks); return false; }
+        if (blocks > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", blocks); return false; }
         g->blocks = (int)blocks;
     }
     return true;

@@ -37,12 +37,12 @@ __device__ __forceinline__ TileCoord chunk_tile(int at, int rows, int cols) {
 }
 
 // Which operand is in the accumulate type (float32, float64 for float64) whatever the tensors' type is: the low-rank activations of an adapter
-enum GroupedLow { LOW_NONE = 0, LOW_A = 1, LOW_B = 2, LOW_C = 3 };
+enum GroupedLow { LOW_A, LOW_B };
 
 // Any strides and sizes, all types (rp_grouped_generic.hip); low: A is.  No scales; by weights: no ids.
 int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype);
 int launch_grouped_weights_generic(const GroupedArgs& g, int dtype);
-// The same for an adapter's narrow products (rp_adapter_any.hip): by rows LOW_C, scales taken; by weights LOW_A or LOW_B, ids taken
+// The same for an adapter's narrow products (rp_adapter_any.hip): by rows C is, scales taken; by weights A or B, ids taken
 int launch_narrow_rows(const GroupedArgs& g, int dtype);
 int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype);
 // out[w, :] (+)= sum over the rows of group w of x[i, :]
@@ -65,6 +65,7 @@ int launch_grouped_rows16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_128(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_rows16_64(const GroupedArgs& g, bool ragged, int dtype);
 int launch_grouped_weights16_64(const GroupedArgs& g, bool ragged, int dtype);
+constexpr long long GROUPED_BACKWARD16_MOST = 12 << 20;        // workgroups
 // The gradients in one launch, the input's on tiles of 64 or 128, the weights' on no larger ones: those of x, w and sums whose output is not null; w row-major (rp_grouped_backward16*.hip)
 int launch_grouped_backward16_bf16(const GroupedArgs& x, int x_tile, const GroupedArgs& w, int w_tile, const GroupedSums& sums, bool ragged);
 int launch_grouped_backward16_f16(const GroupedArgs& x, int x_tile, const GroupedArgs& w, int w_tile, const GroupedSums& sums, bool ragged);
@@ -94,7 +95,7 @@ int launch_adapter_tiles16_256_bf16(const GroupedArgs& shared, const AdapterTerm
 int launch_adapter_tiles16_256_f16(const GroupedArgs& shared, const AdapterTerm& term, bool edge);
 int launch_adapter_tiles16_128(const GroupedArgs& shared, const AdapterTerm& term, bool edge, bool ragged, int dtype);
 int launch_adapter_tiles16_64(const GroupedArgs& shared, const AdapterTerm& term, bool ragged, int dtype);
-// the gradients of an adapter's factors (rp_adapter16_grads.hip): by weights, LOW_A (dB) or LOW_B (dA)
+// the gradients of an adapter's factors (rp_adapter16_grads.hip): LOW_A for dB, LOW_B for dA
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low);
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype);       // those whose C is not null
 // both, and dx with its term on tiles of 64 or 128 (w row-major), in one launch (rp_adapter16_backward*.hip)

@@ -84,6 +84,8 @@ static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const 
     if (!x.C + !w.C + !sums.out > 1 || (x.C && (grouped_stream16_takes(x) || x.b_rs != 1)) || path_disabled("grouped_backward")) return false;
     const Tile16 tx = x.C ? rows_tile16(x, dtype) : Tile16{64, false}, tw = w.C ? weights_tile16(w, dtype) : Tile16{64, false};
     if (!tx.edge || !tw.edge || tx.edge == 256 || tw.edge == 256) return false;
+    const long long most = max_row_tiles(x.gr.rows, x.gr.groups, 64) * ((x.n + 63) / 64) + ((long long)((w.k + 63) / 64) * ((w.n + 63) / 64) + 8) * w.gr.weights + sum_blocks(sums);
+    if (most > GROUPED_BACKWARD16_MOST) return false;
     const bool ragged = tx.ragged || tw.ragged;
     const long long tiles128 = (x.C ? (long long)((x.gr.rows + 127) / 128) * ((x.n + 127) / 128) : 0) + (w.C ? (long long)((w.k + 127) / 128) * ((w.n + 127) / 128) * w.gr.weights : 0);
     const int x_tile = tiles128 >= cus() ? 128 : 64, w_tile = tw.edge < x_tile ? tw.edge : x_tile;

@@ -38,7 +38,7 @@ static int launch_grouped_backward16(const GroupedArgs& x, const GroupedArgs& w,
     bg.w_tiles_n = (w.n + BW - 1) / BW;
     const long long slots = ((long long)bg.w_tiles_k * bg.w_tiles_n + 7) / 8 * 8, total = w.C ? slots * w.gr.weights : 0;
     const long long x_tiles = x.C ? max_row_tiles(x.gr.rows, x.gr.groups, BX) * bg.x_tiles_n : 0, s_blocks = sums.out ? sum_blocks(sums) : 0;
-    if (total > 1 << 22 || x_tiles > 1 << 22 || s_blocks > 1 << 22) { set_error("grouped backward: more tiles than a launch takes"); return -1; }
+    if (total + x_tiles + s_blocks > GROUPED_BACKWARD16_MOST) { set_error("grouped backward: more tiles than a launch takes"); return -1; }
     bg.w_slots = (int)slots;
     bg.w_total = bg.w_blocks = (int)total;
     bg.x_blocks = (int)((x_tiles + 7) / 8 * 8);

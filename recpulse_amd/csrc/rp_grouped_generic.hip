@@ -94,9 +94,12 @@ __global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArg
 }
 
 template <typename T>
-__global__ void __launch_bounds__(1024) grouped_sums_kernel(GroupedSums s) {
+__global__ void __launch_bounds__(1024) grouped_sums_kernel(GroupedSums s, long long blocks) {
     __shared__ typename traits<T>::acc parts[16 * 64];
-    grouped_sums_block<T, 16>(s, (int)blockIdx.x, parts);
+    for (long long id = blockIdx.x; id < blocks; id += gridDim.x) {
+        grouped_sums_block<T, 16>(s, (int)id, parts);
+        __syncthreads();
+    }
 }
 
 static bool grid_ok(long long blocks, const char* what) {
@@ -127,7 +130,7 @@ int launch_grouped_weights_generic(const GroupedArgs& g, int dtype) {
 int launch_grouped_sums(const GroupedSums& s, int dtype) {
     const long long blocks = sum_blocks(s);
     if (!grid_ok(blocks, "grouped bias gradient")) return -1;
-    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)blocks), dim3(1024), 0, current_stream(), s));
+    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(1024), 0, current_stream(), s, blocks));
     return check_launch("grouped_sums_kernel") ? 0 : -1;
 }
 
