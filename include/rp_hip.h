@@ -449,7 +449,7 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
 /* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):
  *   u[i] = scales[a] dy[i] . b_a^T,   dx[i] = dy[i] . w^T + u[i] . a_a^T,   da_a = sum of x[i]^T u[i],   db_a = sum of h[i]^T dy[i]
  * over the rows of all segments that use adapter a (zeros for one that none uses).  u [rows, rank]: room for it, in the accumulate type.  Any of dx [rows, k] (unit column
- * stride), da and db (dense) may be NULL; accumulate_* adds to what is there. */
+ * stride), da and db (dense) may be NULL; accumulate_* adds to what is there.  May take a block of the pool (16-bit types, thousands of rows of one adapter). */
 int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
                                    const float* scales, const int* ids, const int* offsets, int segments, int adapters, int rows, int k, int n, int rank,
                                    long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,

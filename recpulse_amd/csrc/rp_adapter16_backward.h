@@ -19,19 +19,21 @@ __global__ void __launch_bounds__(256, 2) adapter_backward16_kernel(AdapterTileA
 }
 
 template <typename T, int B, int EDGE, int NC>
-static int launch_adapter_backward16(const GroupedArgs& s, const AdapterTerm& term, const AdapterGrads& ag) {
+static int launch_adapter_backward16(const GroupedArgs& s, const AdapterTerm& term, AdapterGrads& ag) {
     const int tiles_m = (s.gr.rows + B - 1) / B, tiles_n = (s.n + B - 1) / B, total = scheduled_grid(tiles_m, tiles_n);
     constexpr size_t tile = m16_smem_bytes(B, B, 2, false, false, 2, 32), smem = tile > AG_LDS ? tile : AG_LDS;
     const GemmArgs g{s.C, s.A, s.B, nullptr, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate};
     const int grad_blocks = (ag.a.blocks + ag.b.blocks + 7) / 8 * 8;        // (the tiles' schedule goes by workgroup modulo 8)
     auto kern = adapter_backward16_kernel<T, B, EDGE, NC>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(grad_blocks + total)), dim3(256), smem, current_stream(), AdapterTileArgs{g, tiles_m, tiles_n, total, term}, ag, grad_blocks);
-    return check_launch("adapter_backward16_kernel") ? 0 : -1;
+    return with_joined_grads<T>(ag, term.gr, [&]() -> int {
+        hipLaunchKernelGGL(kern, dim3((unsigned)(grad_blocks + total)), dim3(256), smem, current_stream(), AdapterTileArgs{g, tiles_m, tiles_n, total, term}, ag, grad_blocks);
+        return check_launch("adapter_backward16_kernel") ? 0 : -1;
+    });
 }
 
 template <typename T, int B, int EDGE>
-static int launch_adapter_backward16_rank(const GroupedArgs& s, const AdapterTerm& term, const AdapterGrads& ag) {
+static int launch_adapter_backward16_rank(const GroupedArgs& s, const AdapterTerm& term, AdapterGrads& ag) {
     return grads_rank_tiles(ag.rank) == 1 ? launch_adapter_backward16<T, B, EDGE, 1>(s, term, ag) : launch_adapter_backward16<T, B, EDGE, 2>(s, term, ag);
 }
 

@@ -7,7 +7,7 @@
 // rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, and values beyond 65504 overflow), a product each: h and u are
 // sums in float32, and one rounding of theirs would be as large as the result's own.
 // fp16, 2048 rows of 3 adapters, 1024 x 2048, rank 8: both 10 us, 3 beside dx's tiles (25 us together).  (Eight waves a workgroup: 8192 rows of one adapter, 4096 x 4096, 48 us instead of
-// 55, but 32 adapters and rank 64 144 instead of 93: a CU holds one such workgroup.)
+// 55 before its rows were shared out, 34 since, but 32 adapters and rank 64 144 instead of 93: a CU holds one such workgroup.)
 #pragma once
 #include "rp_adapter16.h"
 #include "rp_grouped_stream16.h"
@@ -18,6 +18,7 @@ constexpr int AG_WAVES = 4, AG_THREADS = AG_WAVES * 64, AG_COLS = 128, AG_PITCH 
 
 struct AdapterGrad {
     void* out;                     // null: not asked for
+    float* partials;               // null, or room for the shares' sums, each laid out as `out` (dense)
     const void* s;
     const float* low;
     int width, accumulate, strips, blocks;
@@ -26,14 +27,14 @@ struct AdapterGrad {
 
 // NC: 16-row tiles of the rank
 template <typename T, int NC, bool TRANSPOSED>
-__device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int id) {
+__device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int shares, int block) {
     extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH]
     T* out = (T*)ag.out;
     const uint16_t* s = (const uint16_t*)ag.s;
     const float* low = ag.low;
     const int width = ag.width, accumulate = ag.accumulate;
     const long long s_rs = ag.s_rs, out_ws = ag.out_ws, out_rs = ag.out_rs;
-    const int strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
+    const int share = block % shares, id = block / shares, strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
     const int left = width - n0 - 8 * j, by = pulled(left);
@@ -91,8 +92,8 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
     for_groups_of(gr, w, [&](int begin, int stop) {
         end = stop;
-        constexpr int turn = AG_WAVES * GS_ROUND;
-        const int first = begin + ((wave - rounds) & (AG_WAVES - 1)) * GS_ROUND;
+        const int turn = AG_WAVES * shares * GS_ROUND, lag = (share * AG_WAVES + wave - rounds) % (AG_WAVES * shares);
+        const int first = begin + (lag < 0 ? lag + AG_WAVES * shares : lag) * GS_ROUND;
         rounds += (end - begin + GS_ROUND - 1) / GS_ROUND;
         if (first >= end) return;
         static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
@@ -103,7 +104,7 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
             });
     });
     if (rounds == 0) {                                        // an adapter without rows: zeros, or what is there
-        for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate; i += AG_THREADS) {
+        for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate && share == 0; i += AG_THREADS) {
             const int r = r0 + (TRANSPOSED ? i % (16 * NC) : i / AG_COLS), col = n0 + (TRANSPOSED ? i / (16 * NC) : i % AG_COLS);
             if (r < rank && col < width) out[w * out_ws + (TRANSPOSED ? col * out_rs + r : r * out_rs + col)] = round_to<T>(0.f);
         }
@@ -125,7 +126,12 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
             float t = gs_sums[r * AG_PITCH + col];
 #pragma unroll
             for (int p = 1; p < AG_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
-            T* at = out + w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
+            const long long to = w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
+            if (ag.partials) {
+                ag.partials[share * (out_ws * gr.weights) + to] = t;
+                continue;
+            }
+            T* at = out + to;
             T y = round_to<T>(t);
             if (accumulate) y = round_to<T>(widen(*at) + widen(y));
             *at = y;
@@ -135,29 +141,79 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
 
 constexpr int AG_LDS = AG_WAVES * 16 * AG_PITCH * 4;
 
-// dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads
-struct AdapterGrads { AdapterGrad a, b; int rank, rank_blocks; };
+// dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads.  Where few adapters have many rows each, several workgroups share the rows
+// and a second launch adds their sums in order (adapter_grads16_join_kernel).
+struct AdapterGrads { AdapterGrad a, b; int rank, rank_blocks, shares; };
 template <typename T, int NC>
 __device__ __forceinline__ void adapter_grads16_block(const AdapterGrads& ag, const RowGroups& gr, int id) {
-    if (id < ag.a.blocks) adapter_grad16_block<T, NC, true>(ag.a, gr, ag.rank, ag.rank_blocks, id);
-    else if (id < ag.a.blocks + ag.b.blocks) adapter_grad16_block<T, NC, false>(ag.b, gr, ag.rank, ag.rank_blocks, id - ag.a.blocks);
+    if (id < ag.a.blocks) adapter_grad16_block<T, NC, true>(ag.a, gr, ag.rank, ag.rank_blocks, ag.shares, id);
+    else if (id < ag.a.blocks + ag.b.blocks) adapter_grad16_block<T, NC, false>(ag.b, gr, ag.rank, ag.rank_blocks, ag.shares, id - ag.a.blocks);
 }
 
 static inline int grads_rank_tiles(int rank) { return rank <= 16 ? 1 : 2; }
-// Those gradients whose C is not null; false: more workgroups than a launch takes
+constexpr long long AG_MOST_SUMS = 16 << 20;                  // bytes
+// Those gradients whose C is not null; false: more workgroups than a launch takes.  How many share an adapter's rows goes by the sizes alone, not by what is asked for.
 static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, AdapterGrads& ag) {
-    ag.a = AdapterGrad{da.C, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
-    ag.b = AdapterGrad{db.C, db.B, (const float*)db.A, db.n, db.accumulate, 0, 0, db.b_rs, db.c_ws, db.c_rs};
+    ag.a = AdapterGrad{da.C, nullptr, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
+    ag.b = AdapterGrad{db.C, nullptr, db.B, (const float*)db.A, db.n, db.accumulate, 0, 0, db.b_rs, db.c_ws, db.c_rs};
     ag.rank = da.n;
     const int per = 16 * grads_rank_tiles(ag.rank);
     ag.rank_blocks = (ag.rank + per - 1) / per;
+    ag.a.strips = (ag.a.width + AG_COLS - 1) / AG_COLS;
+    ag.b.strips = (ag.b.width + AG_COLS - 1) / AG_COLS;
+    // Shares of eight turns of 128 rows or more, as many as keep two workgroups on a CU (bf16, 7949 rows of one adapter, 384 x 1512, rank 32, forward and backward: 144 us, 118 with seven shares)
+    const long long used = da.gr.groups < da.gr.weights ? da.gr.groups : da.gr.weights, blocks = used * (ag.a.strips + ag.b.strips) * ag.rank_blocks;
+    const long long cus = device_cu_count() > 0 ? device_cu_count() : 256, turns = da.gr.rows / used / (AG_WAVES * GS_ROUND);
+    const long long room = AG_MOST_SUMS / (((long long)ag.a.width + ag.b.width) * ag.rank * da.gr.weights * (long long)sizeof(float));
+    long long shares = turns / 8 < 2 * cus / blocks ? turns / 8 : 2 * cus / blocks;
+    shares = shares < room ? shares : room;
+    ag.shares = shares > 1 ? (int)shares : 1;
     for (AdapterGrad* g : {&ag.a, &ag.b}) {
-        g->strips = (g->width + AG_COLS - 1) / AG_COLS;
-        const long long blocks = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights : 0;
-        if (blocks > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", blocks); return false; }
-        g->blocks = (int)blocks;
+        const long long own = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights * ag.shares : 0;
+        if (own > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", own); return false; }
+        g->blocks = (int)own;
     }
     return true;
+}
+
+// out = the shares' sums in order, rounded once; adapters without rows have been seen to
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_grads16_join_kernel(AdapterGrads ag, RowGroups gr, int a_blocks, int a_per, int b_per) {
+    const bool first = (int)blockIdx.x < a_blocks;
+    const AdapterGrad& g = first ? ag.a : ag.b;
+    const int id = (int)blockIdx.x - (first ? 0 : a_blocks), per = first ? a_per : b_per, w = id / per, size = g.width * ag.rank, i = (id - w * per) * 256 + threadIdx.x;
+    bool any = false;
+    for_groups_of(gr, w, [&](int, int) { any = true; });
+    if (!any || i >= size) return;
+    const long long all = (long long)size * gr.weights, at = (long long)w * size + i;
+    float t = g.partials[at];
+#pragma unroll 4
+    for (int s = 1; s < ag.shares; s++) t += g.partials[s * all + at];
+    T* out = (T*)g.out + at;
+    T y = round_to<T>(t);
+    if (g.accumulate) y = round_to<T>(widen(*out) + widen(y));
+    *out = y;
+}
+
+// Runs `launch`, with memory for the shares' sums (the null stream's own, or a block of the pool) and the launch that adds them up where there are any
+template <typename T, typename F>
+static int with_joined_grads(AdapterGrads& ag, const RowGroups& gr, F launch) {
+    if (ag.shares == 1) return launch();
+    const size_t a_sums = ag.a.out ? (size_t)ag.shares * ag.a.width * ag.rank * gr.weights : 0, b_sums = ag.b.out ? (size_t)ag.shares * ag.b.width * ag.rank * gr.weights : 0;
+    NullStreamScratch lease((a_sums + b_sums) * sizeof(float));
+    void* block = nullptr;
+    if (!lease.ptr && rp_hip_malloc(&block, (a_sums + b_sums) * sizeof(float)) != 0) return -1;
+    float* sums = (float*)(lease.ptr ? lease.ptr : block);
+    if (ag.a.out) ag.a.partials = sums;
+    if (ag.b.out) ag.b.partials = sums + a_sums;
+    int rc = launch();
+    if (rc == 0) {
+        const int a_per = (ag.a.width * ag.rank + 255) / 256, b_per = (ag.b.width * ag.rank + 255) / 256, a_blocks = ag.a.out ? a_per * gr.weights : 0, b_blocks = ag.b.out ? b_per * gr.weights : 0;
+        hipLaunchKernelGGL(adapter_grads16_join_kernel<T>, dim3((unsigned)(a_blocks + b_blocks)), dim3(256), 0, current_stream(), ag, gr, a_blocks, a_per, b_per);
+        rc = check_launch("adapter_grads16_join_kernel") ? 0 : -1;
+    }
+    if (block) rp_hip_free(block);
+    return rc;
 }
 
 }  // namespace rp

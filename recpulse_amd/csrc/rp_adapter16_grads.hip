@@ -7,9 +7,11 @@ template <typename T, int NC>
 __global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr) { adapter_grads16_block<T, NC>(ag, gr, (int)blockIdx.x); }
 
 template <typename T, int NC>
-static int launch_grads(const AdapterGrads& ag, const RowGroups& gr) {
-    hipLaunchKernelGGL((adapter_grads16_kernel<T, NC>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), AG_LDS, current_stream(), ag, gr);
-    return check_launch("adapter_grads16_kernel") ? 0 : -1;
+static int launch_grads(AdapterGrads& ag, const RowGroups& gr) {
+    return with_joined_grads<T>(ag, gr, [&]() -> int {
+        hipLaunchKernelGGL((adapter_grads16_kernel<T, NC>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), AG_LDS, current_stream(), ag, gr);
+        return check_launch("adapter_grads16_kernel") ? 0 : -1;
+    });
 }
 
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {

@@ -508,9 +508,11 @@ class Adapters:
 
     def thrice_rounded(self, got, want, base, added, magnitude, terms):
         """The shared product p is rounded to the tensor type, p + added (a bias, or what dx held) = base again, and base plus the adapter's
-        part a third time: each by half a step of its own value, |p| + |base| + |want| half steps in all."""
+        part a third time: each by half a step of its own value, |p| + |base| + |want| half steps in all.  Or p and the adapter's part are rounded
+        together, want - added, and their sum with what dx held again: |want - added| + |want| half steps.  Neither bounds the other: with p = -3,
+        added = 3 and an adapter's part of t < 0 they are 3 + |t| and 3 + 2 |t|."""
         dt = self.dt
-        rounded = np.abs(base - added) + np.abs(base) + np.abs(want)
+        rounded = np.maximum(np.abs(base - added) + np.abs(base), np.abs(want - added)) + np.abs(want)
         bound = HALF_STEP[dt] * (1 + 2 * HALF_STEP[dt]) * rounded + 3 * TINY[dt] + (terms + 8) * UNIT[dt] * magnitude * (1 + HALF_STEP[dt])
         worst = np.max(np.abs(got - want) - bound)
         assert worst <= 0, f"{worst} beyond the bound"
@@ -832,3 +834,47 @@ def test_routing_on_other_streams_and_in_graphs(t, e, k):
             g.launch()
             capi.check(capi.lib().rp_hip_stream_synchronize(), "rp_hip_stream_synchronize")
             check_sort(outs[0])
+
+
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("shape", [(1, 1, 4100, 136, 264, 8, 0), (3, 2, 9000, 96, 200, 33, 5), (2, 25, 6000, 264, 520, 16, 0), (1, 1, 8192, 1032, 24, 64, 0)], ids=lambda s: "x".join(map(str, s[:6])))
+def test_adapter_gradients_of_many_rows(shape, dt):
+    """Several workgroups share an adapter's rows; one gradient alone has the same bits, on another stream and in a graph too."""
+    *sizes, behind = shape
+    p = Adapters(dt, *sizes, behind=behind)
+    p.forward()
+    whole = p.backward()
+    p.check_backward(whole)
+    p.check_backward(p.backward(accumulate=1), accumulate=1)
+    for i in range(3):
+        one = p.backward(which=[j == i for j in range(3)])[i]
+        assert np.array_equal(one.numpy(), whole[i].numpy())
+    segments, adapters, rows, k, n, rank = p.sizes
+    out, u, d = [Dev.empty(w.shape, dt) for w in whole], Dev.empty((rows, rank), p.acc), p.d
+
+    def into():
+        call("rp_hip_adapter_linear_backward", *[o.ptr for o in out], u.ptr, d["g"].ptr, d["x"].ptr, d["w"].ptr, d["a"].ptr, d["b"].ptr, p.h.ptr, *p.plan(), n, k, 1, *p.w_st, k, 0, 0, 0, dt)
+
+    def check():
+        capi.check(capi.lib().rp_hip_stream_synchronize(), "rp_hip_stream_synchronize")
+        for a, b in zip(out, whole):
+            assert np.array_equal(a.numpy(), b.numpy())
+            call("rp_hip_memset", a.ptr, 0, a.buf.nbytes)
+
+    with capi.Stream():
+        into()
+        check()
+        with capi.Graph.capture() as g:
+            into()
+        for _ in range(3):
+            g.launch()
+            check()
+
+
+@pytest.mark.parametrize("dt", [F32, F64], ids=ids_of)
+def test_grouped_linear_groups_of_few_rows(dt):
+    for groups, rows, k, n in ((40, 60, 264, 520), (7, 50, 130, 70), (30, 2, 300, 300)):
+        p = Grouped(dt, groups, rows, k, n, empty=(2, 5))
+        p.check_forward(p.forward())
+        p.check_backward(p.backward())
+        p.check_backward(p.backward(accumulate=1), accumulate=1)
