@@ -98,74 +98,133 @@ int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low,
     return rc;
 }
 
-// ---- the term by itself: y[i] += h[i] . b_a, where the shared product is too small, or a tile's rows too many segments, for its tiles to take the term in ----
-// (There y has been rounded as the shared product's and is rounded once more as the sum: an operand of a whole product of any size and layout is not to be had unrounded.)
-// A wave for 16 rows of a segment and 128 columns, the rank 32 at a time; h in two values of T as in the gradients.  b is read as it lies, eight rows of the rank times eight
+// ---- the term by itself, where the shared product is too small, or a tile's rows too many segments, for its tiles to take the term in ----
+// The shared product leaves float32 sums of its shares of k; y = sums + bias + h . b_a is rounded once.  A wave for 16 rows of a segment (or of none: those are only rounded)
+// and 128 columns, the rank 32 at a time; h in two values of T as in the gradients.  b is read as it lies, eight rows of the rank times eight
 // columns a lane, and turned with byte permutes, or, where it is contiguous along the rank, as fragments.  Bound by a few loads in a row; with multiply-adds in
-// float32 and h out of the scalar cache 7 rows of rank 64 took 67 us, 5.4 now.
+// float32 and h out of the scalar cache 7 rows of rank 64 took 67 us, 5.9 now; the product's sums 3.8 (128 x 94).
+struct ExpandArgs {
+    uint16_t* y;
+    const uint16_t* bias;
+    const float* sums;             // [shares][rows][n]
+    int n, rows, shares, accumulate, strips;
+    long long y_rs;
+};
+
+// Tile `id` of all rows: those before the first segment, each segment's whether it has an adapter or not, those behind the last
+__device__ __forceinline__ RowTile find_any_tile(const RowGroups& gr, int tile, int id) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int g0 = 0; g0 < gr.groups + 2; g0 += 64) {
+        const int g = g0 + lane - 1;
+        int b = 0, e = 0, w = -1;
+        if (g < 0) e = gr.begin(0);
+        else if (g < gr.groups) { b = gr.begin(g); e = gr.end(g); w = gr.weight(g); }
+        else if (g == gr.groups) { b = gr.end(g - 1); e = gr.rows; }
+        const int tiles = (e - b + tile - 1) / tile, upto = before + wave_prefix_sum(tiles, lane);
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > id);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            RowTile t;
+            t.group = g0 + l - 1;
+            t.weight = __builtin_amdgcn_readlane(w, l);
+            t.tiles = __builtin_amdgcn_readlane(tiles, l);
+            t.first = __builtin_amdgcn_readlane(upto, l) - t.tiles;
+            t.begin = __builtin_amdgcn_readlane(b, l) + (id - t.first) * tile;
+            t.stop = __builtin_amdgcn_readlane(e, l);
+            t.end = t.begin + tile < t.stop ? t.begin + tile : t.stop;
+            return t;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return RowTile{-1, -1, 0, 0, 0, 0, 0};
+}
+
 template <typename T, bool ALONG_RANK>
-__global__ void __launch_bounds__(64) adapter_expand16_kernel(uint16_t* y, AdapterTerm term, int n, long long y_rs, int strips) {
-    const RowTile rt = find_row_tile(term.gr, 16, (int)(blockIdx.x / strips));
-    if (rt.group < 0) return;
-    const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15, rank = term.rank;
-    const int col = (int)(blockIdx.x % strips) * 128 + 8 * j, m = rt.end - rt.begin, left = n - col, by = pulled(left);
+__global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, AdapterTerm term) {
+    const RowTile rt = find_any_tile(term.gr, 16, (int)(blockIdx.x / ea.strips));
+    const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15, n = ea.n, m = rt.end - rt.begin;
+    if (m <= 0) return;
+    const int col = (int)(blockIdx.x % ea.strips) * 128 + 8 * j, left = n - col, by = pulled(left);
     const bool cut = col - 8 * j + 128 > n && n % 8;                      // (the strip's last vector ends with the row)
-    const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)rt.begin * rank, (long long)m * rank * 4);
-    const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc((const uint16_t*)term.b + rt.weight * term.b_ws, ((rank - 1) * term.b_rs + (n - 1) * term.b_cs + 1) * 2);
-    const __amdgpu_buffer_rsrc_t y_rsrc = buffer_rsrc(y + rt.begin * y_rs, ((m - 1) * y_rs + n) * 2);
-    u32x4_t was[4];
-#pragma unroll
-    for (int v = 0; v < 4; v++) was[v] = __builtin_amdgcn_raw_buffer_load_b128(y_rsrc, (int)(4 * q + v < m && left > 0 ? (uint32_t)(((4 * q + v) * y_rs + col - by) * 2) : BUFFER_OOB), 0, 0);
-    f32x4_t acc[8];
+    f32x4_t acc[8];                                                       // rows 4q + v, column col + f
 #pragma unroll
     for (int f = 0; f < 8; f++) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < rank; k0 += 32) {
-        const int kk = k0 + 8 * q;
-        float hv[8];
-        u32x4_t raw[8], hi, lo;
+    for (int s = 0; s < ea.shares; s++) {
+        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(ea.sums + ((long long)s * ea.rows + rt.begin) * n, (long long)m * n * 4);
+        u32x4_t p[4][2];
 #pragma unroll
-        for (int u = 0; u < 8; u++) hv[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(j < m && kk + u < rank ? (uint32_t)((j * rank + kk + u) * 4) : BUFFER_OOB), 0, 0));
-        if (ALONG_RANK && rank % 8 == 0) {
+        for (int v = 0; v < 4; v++)
 #pragma unroll
-            for (int f = 0; f < 8; f++) raw[f] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col + f < n && kk < rank ? (uint32_t)(((col + f) * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0);
-        } else if (ALONG_RANK) {
+            for (int h = 0; h < 2; h++) p[v][h] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(4 * q + v < m && left > 0 ? (uint32_t)(((long long)(4 * q + v) * n + col + 4 * h) * 4) : BUFFER_OOB), 0, 0);
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int f = 0; f < 8; f++) acc[f][v] += __uint_as_float(p[v][f / 4][f % 4]);
+    }
+    if (rt.weight >= 0) {
+        const int rank = term.rank;
+        const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)rt.begin * rank, (long long)m * rank * 4);
+        const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc((const uint16_t*)term.b + rt.weight * term.b_ws, ((rank - 1) * term.b_rs + (n - 1) * term.b_cs + 1) * 2);
+        for (int k0 = 0; k0 < rank; k0 += 32) {
+            const int kk = k0 + 8 * q;
+            float hv[8];
+            u32x4_t raw[8], hi, lo;
+#pragma unroll
+            for (int u = 0; u < 8; u++) hv[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(j < m && kk + u < rank ? (uint32_t)((j * rank + kk + u) * 4) : BUFFER_OOB), 0, 0));
+            if (ALONG_RANK && rank % 8 == 0) {
+#pragma unroll
+                for (int f = 0; f < 8; f++) raw[f] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col + f < n && kk < rank ? (uint32_t)(((col + f) * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0);
+            } else if (ALONG_RANK) {
+#pragma unroll
+                for (int f = 0; f < 8; f++) {
+                    uint32_t x[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col + f < n && kk + u < rank ? (uint32_t)(((col + f) * term.b_cs + kk + u) * 2) : BUFFER_OOB), 0, 0);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) raw[f][d] = x[2 * d] | x[2 * d + 1] << 16;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) raw[e] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(left > 0 && kk + e < rank ? (uint32_t)(((kk + e) * term.b_rs + col - by) * 2) : BUFFER_OOB), 0, 0);
+                if (cut) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) raw[e] = pull_into_place(raw[e], by);
+                }
+            }
+            split_low<T>(hv, hi, lo);
 #pragma unroll
             for (int f = 0; f < 8; f++) {
-                uint32_t x[8];
+                u32x4_t b = raw[f];
+                if constexpr (!ALONG_RANK) {
 #pragma unroll
-                for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col + f < n && kk + u < rank ? (uint32_t)(((col + f) * term.b_cs + kk + u) * 2) : BUFFER_OOB), 0, 0);
-#pragma unroll
-                for (int d = 0; d < 4; d++) raw[f][d] = x[2 * d] | x[2 * d + 1] << 16;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) raw[e] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(left > 0 && kk + e < rank ? (uint32_t)(((kk + e) * term.b_rs + col - by) * 2) : BUFFER_OOB), 0, 0);
-            if (cut) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) raw[e] = pull_into_place(raw[e], by);
+                    for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
+                }
+                acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
+                acc[f] = sh_ops<T>::mma(lo, b, acc[f]);
             }
         }
-        split_low<T>(hv, hi, lo);
+    }
+    if (left <= 0) return;
+    float bias[8] = {};
+    if (ea.bias) {
 #pragma unroll
-        for (int f = 0; f < 8; f++) {
-            u32x4_t b = raw[f];
-            if constexpr (!ALONG_RANK) {
-#pragma unroll
-                for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
-            }
-            acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
-            acc[f] = sh_ops<T>::mma(lo, b, acc[f]);
-        }
+        for (int f = 0; f < 8; f++) { T b; b.bits = ea.bias[f < left ? col + f : col]; bias[f] = widen(b); }
     }
 #pragma unroll
     for (int v = 0; v < 4; v++) {
-        if (4 * q + v >= m || left <= 0) continue;
-        const u32x4_t x = cut ? pull_into_place(was[v], by) : was[v];
+        if (4 * q + v >= m) continue;
+        uint16_t* p = ea.y + (rt.begin + 4 * q + v) * ea.y_rs + col;
         T o[8];
-        __builtin_memcpy(o, &x, 16);
 #pragma unroll
-        for (int f = 0; f < 8; f++) o[f] = round_to<T>(widen(o[f]) + acc[f][v]);
-        uint16_t* p = y + (rt.begin + 4 * q + v) * y_rs + col;
+        for (int f = 0; f < 8; f++) o[f] = round_to<T>(acc[f][v] + bias[f]);
+        if (ea.accumulate) {                                              // (the product's rounding, and the sum's)
+            const u32x4_t x = pull_into_place(*(const u32x4_odd_t*)(p - by), by);
+            T was[8];
+            __builtin_memcpy(was, &x, 16);
+#pragma unroll
+            for (int f = 0; f < 8; f++) o[f] = round_to<T>(widen(was[f]) + widen(o[f]));
+        }
         if (left >= 8) {
             u32x4_t z;
             __builtin_memcpy(&z, o, 16);
@@ -179,21 +238,36 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(uint16_t* y, Adapt
 }
 
 bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) {
-    return shared.n >= 8 && shared.c_rs < (1ll << 22) && (term.b_cs == 1 || term.b_rs == 1) && (long long)term.rank * shared.n < (1 << 28) && term.rank < (1 << 22) && !path_disabled("mfma");
+    return shared.n >= 8 && shared.c_rs < (1ll << 22) && shared.n < (1 << 24) && (term.b_cs == 1 || term.b_rs == 1) && (long long)term.rank * shared.n < (1 << 28) && term.rank < (1 << 22) && !path_disabled("mfma");
 }
 
 template <typename T>
-static int launch_expand(const GroupedArgs& shared, const AdapterTerm& term) {
-    const int strips = (shared.n + 127) / 128;
-    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups, 16) * strips;
-    if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, strips);
-    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), (uint16_t*)shared.C, term, shared.n, shared.c_rs, strips);
+static int launch_expand(const ExpandArgs& ea, const AdapterTerm& term) {
+    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups + 2, 16) * ea.strips;
+    if (blocks > 0x3fffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
+    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), ea, term);
+    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), ea, term);
     return check_launch("adapter_expand16_kernel") ? 0 : -1;
 }
 
-int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, int dtype) {
-    return dtype == RP_DTYPE_BFLOAT16 ? launch_expand<bf16_t>(shared, term) : launch_expand<f16_t>(shared, term);
+int launch_adapter_expand16(const GroupedArgs& s, const AdapterTerm& term, bool ragged, int dtype) {
+    ragged = ragged || s.n % 8;                               // (the sums are stored in whole vectors otherwise)
+    const int rows = s.gr.rows, cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const bool large = (long long)((rows + 127) / 128) * ((s.n + 127) / 128) * 2 >= cus;
+    const int shares = large ? 1 : skinny16_sums_shares(rows, s.k, s.n);
+    const size_t bytes = (size_t)shares * rows * s.n * sizeof(float);
+    NullStreamScratch lease(bytes);
+    void* block = nullptr;
+    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
+    float* sums = (float*)(lease.ptr ? lease.ptr : block);
+    const GemmArgs g{nullptr, s.A, s.B, nullptr, 1, rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.n, 1, 0};
+    Plan p{FAM_MFMA16_SKINNY, 32, 128, false, s.b_cs == 1, true, ""};
+    p.ragged = ragged;
+    int rc = large ? launch_sums16_128(g, p.b_mc, ragged, sums, dtype) : launch_skinny16_sums(g, p, sums, dtype);
+    const ExpandArgs ea{(uint16_t*)s.C, (const uint16_t*)s.bias, sums, s.n, rows, shares, s.accumulate, (s.n + 127) / 128, s.c_rs};
+    if (rc == 0) rc = dtype == RP_DTYPE_BFLOAT16 ? launch_expand<bf16_t>(ea, term) : launch_expand<f16_t>(ea, term);
+    if (block) rp_hip_free(block);
+    return rc;
 }
 
 }  // namespace rp

@@ -181,6 +181,9 @@ int* noalloc_arrival_counters();
 // per-family launchers (dtype is one of the RP_DTYPE_* codes the family supports)
 int launch_generic(const GemmArgs& g, int dtype);
 int launch_skinny(const GemmArgs& g, int dtype);
+// One 16-bit product on 32 x 128 tiles as float32 sums of its shares of k, [shares][m][n]
+int skinny16_sums_shares(int m, int k, int n);
+int launch_skinny16_sums(const GemmArgs& g, const Plan& p, float* partials, int dtype);
 int launch_mfma16(const GemmArgs& g, const Plan& p, int dtype);
 bool stream128_shape(int batch, int m, int k, int n);      // shapes the streaming kernel on 128-column strips is chosen for (row-major A and B)
 bool stream128_takes(const GemmArgs& g);

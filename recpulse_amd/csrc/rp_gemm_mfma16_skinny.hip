@@ -35,6 +35,19 @@ size_t skinny16_workspace(int batch, int m, int k, int n) {
     return (size_t)batch * skinny16_splits(batch, m, k, n, k_per_split) * m * n * sizeof(float);
 }
 
+int skinny16_sums_shares(int m, int k, int n) {
+    int k_per_split;
+    return skinny16_splits(1, m, k, n, k_per_split);
+}
+
+int launch_skinny16_sums(const GemmArgs& g, const Plan& p, float* partials, int dtype) {
+    int k_per_split;
+    const int nsplit = skinny16_splits(1, g.m, g.k, g.n, k_per_split);
+    const bool bf = dtype == RP_DTYPE_BFLOAT16;
+    if (p.ragged) return bf ? launch_skinny16_t<bf16_t, M16_RAGGED>(g, p, partials, nsplit, k_per_split) : launch_skinny16_t<f16_t, M16_RAGGED>(g, p, partials, nsplit, k_per_split);
+    return bf ? launch_skinny16_t<bf16_t, M16_EDGE>(g, p, partials, nsplit, k_per_split) : launch_skinny16_t<f16_t, M16_EDGE>(g, p, partials, nsplit, k_per_split);
+}
+
 int launch_mfma16_skinny(const GemmArgs& g, const Plan& p, int dtype) {
     if (dtype != RP_DTYPE_BFLOAT16 && dtype != RP_DTYPE_FLOAT16) { set_error("mfma16 skinny GEMM: unsupported dtype %d", dtype); return -1; }
     if (!p.ragged && !p.a_mc && p.b_mc && stream128_takes(g)) return launch_stream128(g, dtype);

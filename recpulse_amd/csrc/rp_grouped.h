@@ -88,9 +88,11 @@ int launch_stream16_combine(const GroupedArgs& g, const StreamGrid& sg, const Ad
 // h[i] = scales[a] x[i] . a_a in float32 for bf16 / fp16 operands (rp_adapter16.hip); C is h
 bool adapter_shrink16_takes(const GroupedArgs& g);
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype);
-// y[i] += h[i] . b_a (rp_adapter16.hip), and the shared product with that term in it, on MFMA tiles (rp_adapter16_tiles*.hip); ragged: rows of any length and start
+// The shared product as float32 sums, then y = sums + bias + h[i] . b_a (rp_adapter16.hip); ragged: rows of any length and start
 bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term);
-int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, int dtype);
+int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, bool ragged, int dtype);
+int launch_sums16_128(const GemmArgs& g, bool b_mc, bool ragged, float* sums, int dtype);      // [m][n], rp_adapter16_sums.hip
+// The shared product with that term in it, on MFMA tiles (rp_adapter16_tiles*.hip)
 int launch_adapter_tiles16_256_bf16(const GroupedArgs& shared, const AdapterTerm& term, bool edge);
 int launch_adapter_tiles16_256_f16(const GroupedArgs& shared, const AdapterTerm& term, bool edge);
 int launch_adapter_tiles16_128(const GroupedArgs& shared, const AdapterTerm& term, bool edge, bool ragged, int dtype);

@@ -632,6 +632,28 @@ def test_adapter_linear_odd_sizes(shape, dt):
     test_adapter_linear(shape, dt)
 
 
+# the term as a launch of its own: each segment a row or a few, large and small shared products
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("shape", [(300, 40, 700, 1024, 2048, 16, 9), (500, 7, 2100, 264, 1032, 33, 0), (90, 90, 90, 520, 2047, 8, 0), (64, 9, 200, 2064, 24, 100, 3), (33, 5, 70, 40, 9, 4, 1)], ids=lambda s: "x".join(map(str, s[:6])))
+def test_adapter_linear_many_segments(shape, dt):
+    """y and dx are rounded once (and once more where dx is added to what is there)."""
+    *sizes, behind = shape
+    segments, adapters, rows, k, n, rank = sizes
+    for transposed in (False, True):
+        p = Adapters(dt, *sizes, behind=behind, transposed=transposed)
+        p.forward()
+        p.check_forward()
+        for accumulate in (0, 1):
+            out = p.backward(accumulate=accumulate)
+            p.check_backward(out, accumulate=accumulate)
+        f, size, y = p.f, np.abs(p.f["x"]) @ np.abs(p.f["w"]) + np.abs(p.f["bias"]), p.f["x"] @ p.f["w"] + p.f["bias"]
+        for at, a, scale in p.spans():
+            y[at] += scale * (f["x"][at] @ f["a"][a]) @ f["b"][a]
+            size[at] += scale * (np.abs(f["x"][at]) @ np.abs(f["a"][a])) @ np.abs(f["b"][a])
+        # h is multiplied as two values that add up to it to 2^-17 (bfloat16): 128 units of 2^-24 of the term's magnitude
+        within(oracle.to_f64(p.y.numpy(), dt), y, size, k + rank + 2 + 128, dt)
+
+
 # the shared product on tiles of 256 and of 128, aligned and ragged, the rank in one and in several steps
 @pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
 @pytest.mark.parametrize("shape", [(5, 3, 4100, 512, 4096, 32, 0), (5, 3, 4096, 4096, 512, 100, 6), (3, 2, 2049, 1031, 4099, 12, 0), (7, 4, 2048, 520, 2048, 8, 0)], ids=lambda s: "x".join(map(str, s[:6])))
