@@ -30,9 +30,9 @@ template <typename F>
 __device__ __forceinline__ void for_groups_of(const RowGroups& gr, int w, F f) {
     const int lane = threadIdx.x & 63;
     for (int g0 = 0; g0 < gr.groups; g0 += 64) {
-        int b = 0, e = 0;
-        if (g0 + lane < gr.groups && gr.weight(g0 + lane) == w) { b = gr.begin(g0 + lane); e = gr.end(g0 + lane); }
-        unsigned long long here = __builtin_amdgcn_ballot_w64(e > b);
+        int b = 0, e = 0, own = -1;
+        if (g0 + lane < gr.groups) { own = gr.weight(g0 + lane); b = gr.begin(g0 + lane); e = gr.end(g0 + lane); }      // (one trip to memory for all three)
+        unsigned long long here = __builtin_amdgcn_ballot_w64(own == w && e > b);
         while (here) {
             const int l = __builtin_ctzll(here);
             here &= here - 1;
