@@ -442,7 +442,7 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  * x [rows, k], w [k, n], bias [n] or NULL, a [adapters, k, rank] and b [adapters, rank, n] dense, scales float32 [adapters] or NULL for ones, y [rows, n] with
  * unit column stride.  h [rows, rank], dense, in the accumulate type: written for rows with an adapter, kept by the caller for the backward pass.
  * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection.  16-bit types multiply h (and u below) by b (a) as two values of the type
- * that add up to it to 2^-17 (float16: 2^-22), so float16 wants them within 65504; y and dx are rounded once, the shared product and the term together
+ * that add up to it to 2^-17 (float16: 2^-22), so float16 wants them within 65504; no row sees what another segment's adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
  * (float32, float64, widths below 8 and operands without a unit stride: the shared product as a layer of its own, and the sum again). */
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
                                   int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);

@@ -147,9 +147,9 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
     if (m <= 0) return;
     const int col = (int)(blockIdx.x % ea.strips) * 128 + 8 * j, left = n - col, by = pulled(left);
     const bool cut = col - 8 * j + 128 > n && n % 8;                      // (the strip's last vector ends with the row)
-    f32x4_t acc[8];                                                       // rows 4q + v, column col + f
+    f32x4_t acc[8], low[8];                                               // rows 4q + v, column col + f; the products with h's lower values
 #pragma unroll
-    for (int f = 0; f < 8; f++) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < 8; f++) acc[f] = low[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < ea.shares; s++) {
         const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(ea.sums + ((long long)s * ea.rows + rt.begin) * n, (long long)m * n * 4);
         u32x4_t p[4][2];
@@ -201,9 +201,13 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
                     for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
                 }
                 acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
-                acc[f] = sh_ops<T>::mma(lo, b, acc[f]);
+                low[f] = sh_ops<T>::mma(lo, b, low[f]);
             }
         }
+#pragma unroll
+        for (int f = 0; f < 8; f++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) acc[f][v] += __builtin_isfinite(low[f][v]) ? low[f][v] : 0.f;      // (an infinity of b: the higher value's product is what there is to add)
     }
     if (left <= 0) return;
     float bias[8] = {};

@@ -20,101 +20,161 @@ struct AdapterTileArgs {
     AdapterTerm term;
 };
 
+// Which of a pair of 16-bit values are an infinity or NaN: their sign bits
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+    constexpr bool f16 = std::is_same<T, f16_t>::value;
+    return ((v & (f16 ? 0x7C007C00u : 0x7F807F80u)) + (f16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;       // (an exponent of ones carries)
+}
+
 struct AdapterTiles {
     static constexpr bool MOVES = false, ONCE = true, TERM = true;
+    bool odd = false;              // the wave met an infinity or NaN in b
 
-    // acc: the sums of the calling wave's patch of the tile at (m0, n0), waves WGN to a row of patches
-    template <typename T, int MT, int WGN, int TMI, int TNI, typename ACC>
-    __device__ __forceinline__ void add_term(ACC (&acc)[TMI][TNI], int m0, int n0) const {
-        constexpr int KSTEP = MT == 32 ? 16 : 32;
-        // The term's arguments are read here, from where the launch left them, and the lane's numbers are made anew: kept for the next tile they
-        // would take registers that the main loop needs.
-        typedef const __attribute__((address_space(4))) AdapterTileArgs* args_t;       // (constant memory: scalar loads)
-        args_t args = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
-        unsigned t = threadIdx.x;
-        asm volatile("" : "+s"(args), "+v"(t));
+    // The term's arguments are read from where the launch left them whenever they are needed: kept for the next tile they would take registers that the main loop needs.
+    typedef const __attribute__((address_space(4))) AdapterTileArgs* args_t;       // (constant memory: scalar loads)
+    static __device__ __forceinline__ args_t arguments() { return (args_t)__builtin_amdgcn_kernarg_segment_ptr(); }
+    static __device__ __forceinline__ AdapterTerm term_of(args_t args) {
         const RowGroups gr{args->term.gr.offsets, args->term.gr.ids, args->term.gr.groups, args->term.gr.rows, args->term.gr.weights};
-        const AdapterTerm term{args->term.h, args->term.b, gr, args->term.rank, args->term.b_ws, args->term.b_rs, args->term.b_cs};
-        const int m = args->g.m, n = args->g.n;
-        const int lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), fr = lane % MT, oct = lane / MT;
-        const int row0 = m0 + wave / WGN * (TMI * MT), col0 = n0 + wave % WGN * (TNI * MT), row_end = row0 + TMI * MT < m ? row0 + TMI * MT : m;
-        const bool whole = term.rank % 4 == 0 && ((uintptr_t)term.h & 15) == 0;
-        for (int g0 = 0; g0 < term.gr.groups; g0 += 64) {
+        return AdapterTerm{args->term.h, args->term.b, gr, args->term.rank, args->term.b_ws, args->term.b_rs, args->term.b_cs};
+    }
+    // f(begin, end, adapter) for every segment with an adapter that has some of the rows [row0, row_end); the wave looks at 64 segments at a time
+    template <typename F> static __device__ __forceinline__ void for_segments(const RowGroups& gr, int row0, int row_end, int lane, F f) {
+        for (int g0 = 0; g0 < gr.groups; g0 += 64) {
             int b = 0, e = 0, w = -1;
-            if (g0 + lane < term.gr.groups) { b = term.gr.begin(g0 + lane); e = term.gr.end(g0 + lane); w = term.gr.weight(g0 + lane); }
+            if (g0 + lane < gr.groups) { b = gr.begin(g0 + lane); e = gr.end(g0 + lane); w = gr.weight(g0 + lane); }
             unsigned long long here = __builtin_amdgcn_ballot_w64(w >= 0 && b < row_end && e > row0);
             while (here) {
                 const int l = __builtin_ctzll(here);
                 here &= here - 1;
-                const int sb = __builtin_amdgcn_readlane(b, l), se = __builtin_amdgcn_readlane(e, l), a = __builtin_amdgcn_readlane(w, l);
-                const uint16_t* bp = (const uint16_t*)term.b + a * term.b_ws;
-                for (int k0 = 0; k0 < term.rank; k0 += KSTEP) {
-                    const int kk = k0 + 8 * oct, left = term.rank - kk;
-                    // All loads first, and none behind a branch (out of range they read zeros): one round trip for them together.
-                    const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc(bp, ((long long)(term.rank - 1) * term.b_rs + (long long)(n - 1) * term.b_cs + 1) * 2);
-                    const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)sb * term.rank, (long long)(se - sb) * term.rank * 4);
-                    s16x8_t bf[TNI];
-                    float hv[TMI][8];
-#pragma unroll
-                    for (int i = 0; i < TMI; i++) {
-                        const uint32_t at = (uint32_t)(((row0 + i * MT + fr - sb) * term.rank + kk) * 4);      // (rows before the segment wrap around, out of range)
-                        if (whole) {
-                            const u32x4_t p = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 0 ? at : BUFFER_OOB), 0, 0);
-                            const u32x4_t q = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 4 ? at + 16 : BUFFER_OOB), 0, 0);
-#pragma unroll
-                            for (int u = 0; u < 4; u++) { hv[i][u] = __uint_as_float(p[u]); hv[i][4 + u] = __uint_as_float(q[u]); }
-                        } else {
-#pragma unroll
-                            for (int u = 0; u < 8; u++) hv[i][u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(u < left ? at + 4 * u : BUFFER_OOB), 0, 0));
-                        }
-                    }
-                    if (term.b_rs == 1 && term.rank % 8 == 0) {
-#pragma unroll
-                        for (int j = 0; j < TNI; j++) {
-                            const int col = col0 + j * MT + fr;
-                            bf[j] = __builtin_bit_cast(s16x8_t, __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col < n && left > 0 ? (uint32_t)((col * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0));
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < TNI; j++) {
-                            const int col = col0 + j * MT + fr;
-                            const uint32_t at = (uint32_t)((kk * term.b_rs + col * term.b_cs) * 2), step = (uint32_t)(term.b_rs * 2);
-                            uint32_t x[8];
-#pragma unroll
-                            for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col < n && u < left ? at + u * step : BUFFER_OOB), 0, 0);
-                            u32x4_t y;
-#pragma unroll
-                            for (int d = 0; d < 4; d++) y[d] = x[2 * d] | x[2 * d + 1] << 16;
-                            bf[j] = __builtin_bit_cast(s16x8_t, y);
-                        }
-                    }
-                    u32x4_t hi[TMI], lo[TMI];
-#pragma unroll
-                    for (int i = 0; i < TMI; i++) split_low<T>(hv[i], hi[i], lo[i]);
-                    // (the in-place MFMAs are opaque to the compiler: what vector instructions wrote for them has to be there)
-                    if constexpr (MT == 16) {
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int j = 0; j < TNI; j++) asm volatile("" : "+v"(bf[j]) : : "memory");
-#pragma unroll
-                        for (int i = 0; i < TMI; i++) asm volatile("" : "+v"(hi[i]), "+v"(lo[i]) : : "memory");
-                        asm volatile("s_nop 15" ::: "memory");
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    static_for<0, TMI>([&](auto ic) {
-                        constexpr int i = decltype(ic)::value;
-                        static_for<0, TNI>([&](auto jc) {
-                            constexpr int j = decltype(jc)::value;
-                            acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, hi[i]), bf[j], acc[i][j]);
-                        });
-                        static_for<0, TNI>([&](auto jc) {
-                            constexpr int j = decltype(jc)::value;
-                            acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, lo[i]), bf[j], acc[i][j]);
-                        });
-                    });
-                }
+                f(__builtin_amdgcn_readlane(b, l), __builtin_amdgcn_readlane(e, l), __builtin_amdgcn_readlane(w, l));
             }
         }
+    }
+
+    // acc: the sums of the calling wave's patch of the tile at (m0, n0), waves WGN to a row of patches
+    template <typename T, int MT, int WGN, int TMI, int TNI, typename ACC>
+    __device__ __forceinline__ void add_term(ACC (&acc)[TMI][TNI], int m0, int n0) {
+        constexpr int KSTEP = MT == 32 ? 16 : 32;
+        args_t args = arguments();
+        unsigned t = threadIdx.x;                             // (the lane's numbers are made anew, too)
+        asm volatile("" : "+s"(args), "+v"(t));
+        const AdapterTerm term = term_of(args);
+        const int m = args->g.m, n = args->g.n;
+        const int lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), fr = lane % MT, oct = lane / MT;
+        const int row0 = m0 + wave / WGN * (TMI * MT), col0 = n0 + wave % WGN * (TNI * MT), row_end = row0 + TMI * MT < m ? row0 + TMI * MT : m;
+        const bool whole = term.rank % 4 == 0 && ((uintptr_t)term.h & 15) == 0;
+        for_segments(term.gr, row0, row_end, lane, [&](int sb, int se, int a) {
+            const uint16_t* bp = (const uint16_t*)term.b + a * term.b_ws;
+            for (int k0 = 0; k0 < term.rank; k0 += KSTEP) {
+                const int kk = k0 + 8 * oct, left = term.rank - kk;
+                // All loads first, and none behind a branch (out of range they read zeros): one round trip for them together.
+                const __amdgpu_buffer_rsrc_t b_rsrc = buffer_rsrc(bp, ((long long)(term.rank - 1) * term.b_rs + (long long)(n - 1) * term.b_cs + 1) * 2);
+                const __amdgpu_buffer_rsrc_t h_rsrc = buffer_rsrc(term.h + (long long)sb * term.rank, (long long)(se - sb) * term.rank * 4);
+                s16x8_t bf[TNI];
+                float hv[TMI][8];
+#pragma unroll
+                for (int i = 0; i < TMI; i++) {
+                    const uint32_t at = (uint32_t)(((row0 + i * MT + fr - sb) * term.rank + kk) * 4);      // (rows before the segment wrap around, out of range)
+                    if (whole) {
+                        const u32x4_t p = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 0 ? at : BUFFER_OOB), 0, 0);
+                        const u32x4_t q = __builtin_amdgcn_raw_buffer_load_b128(h_rsrc, (int)(left > 4 ? at + 16 : BUFFER_OOB), 0, 0);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) { hv[i][u] = __uint_as_float(p[u]); hv[i][4 + u] = __uint_as_float(q[u]); }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 8; u++) hv[i][u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(h_rsrc, (int)(u < left ? at + 4 * u : BUFFER_OOB), 0, 0));
+                    }
+                }
+                if (term.b_rs == 1 && term.rank % 8 == 0) {
+#pragma unroll
+                    for (int j = 0; j < TNI; j++) {
+                        const int col = col0 + j * MT + fr;
+                        bf[j] = __builtin_bit_cast(s16x8_t, __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)(col < n && left > 0 ? (uint32_t)((col * term.b_cs + kk) * 2) : BUFFER_OOB), 0, 0));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < TNI; j++) {
+                        const int col = col0 + j * MT + fr;
+                        const uint32_t at = (uint32_t)((kk * term.b_rs + col * term.b_cs) * 2), step = (uint32_t)(term.b_rs * 2);
+                        uint32_t x[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) x[u] = __builtin_amdgcn_raw_buffer_load_b16(b_rsrc, (int)(col < n && u < left ? at + u * step : BUFFER_OOB), 0, 0);
+                        u32x4_t y;
+#pragma unroll
+                        for (int d = 0; d < 4; d++) y[d] = x[2 * d] | x[2 * d + 1] << 16;
+                        bf[j] = __builtin_bit_cast(s16x8_t, y);
+                    }
+                }
+                // The patch's rows of other segments are zeros here: zero times an infinity or NaN of b would reach them, so that those are left to `finish`.
+                uint32_t any = 0;
+#pragma unroll
+                for (int j = 0; j < TNI; j++) {
+                    const u32x4_t v = __builtin_bit_cast(u32x4_t, bf[j]);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) any |= not_finite<T>(v[d]);
+                }
+                if (__builtin_amdgcn_ballot_w64(any != 0)) {
+                    odd = true;
+#pragma unroll
+                    for (int j = 0; j < TNI; j++) {
+                        u32x4_t v = __builtin_bit_cast(u32x4_t, bf[j]);
+#pragma unroll
+                        for (int d = 0; d < 4; d++) v[d] &= ~((not_finite<T>(v[d]) >> 15) * 0xFFFFu);
+                        bf[j] = __builtin_bit_cast(s16x8_t, v);
+                    }
+                }
+                u32x4_t hi[TMI], lo[TMI];
+#pragma unroll
+                for (int i = 0; i < TMI; i++) split_low<T>(hv[i], hi[i], lo[i]);
+                // (the in-place MFMAs are opaque to the compiler: what vector instructions wrote for them has to be there)
+                if constexpr (MT == 16) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < TNI; j++) asm volatile("" : "+v"(bf[j]) : : "memory");
+#pragma unroll
+                    for (int i = 0; i < TMI; i++) asm volatile("" : "+v"(hi[i]), "+v"(lo[i]) : : "memory");
+                    asm volatile("s_nop 15" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                static_for<0, TMI>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    static_for<0, TNI>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, hi[i]), bf[j], acc[i][j]);
+                    });
+                    static_for<0, TNI>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, lo[i]), bf[j], acc[i][j]);
+                    });
+                });
+            }
+        });
+    }
+
+    // After the tile is stored: what h multiplies an infinity or NaN of b by is added to the rows of that segment alone
+    template <typename T, int MT, int WGN, int TMI, int TNI>
+    __device__ __forceinline__ void finish(int m0, int n0) {
+        if (!odd) return;
+        odd = false;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");           // (a wave adds to what its own lanes stored)
+        const args_t args = arguments();
+        const AdapterTerm term = term_of(args);
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = args->g.m, n = args->g.n;
+        const int row0 = m0 + wave / WGN * (TMI * MT), col0 = n0 + wave % WGN * (TNI * MT), row_end = row0 + TMI * MT < m ? row0 + TMI * MT : m, col_end = col0 + TNI * MT < n ? col0 + TNI * MT : n;
+        T* y = (T*)args->g.C;
+        const long long y_rs = args->g.c_rs;
+        for_segments(term.gr, row0, row_end, lane, [&](int sb, int se, int a) {
+            const int first = sb > row0 ? sb : row0, last = se < row_end ? se : row_end;
+            for (int col = col0 + lane; col < col_end; col += 64)
+            for (int r = 0; r < term.rank; r++) {
+                const T b = ((const T*)term.b)[a * term.b_ws + r * term.b_rs + col * term.b_cs];
+                if (!(not_finite<T>(b.bits) & 0x8000u)) continue;
+                for (int row = first; row < last; row++) {
+                    T* at = y + row * y_rs + col;
+                    *at = round_to<T>(widen(*at) + term.h[(long long)row * term.rank + r] * widen(b));
+                }
+            }
+        });
     }
 };
 

@@ -176,7 +176,7 @@ typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)))
 // Where a workgroup's tiles come from and what else they may do.  M16Plain: the schedule of one matrix of the batch, the reference's roundings.
 // Another source may have MOVES: its `tile` points `g` at the matrix that slot `tile_id` belongs to and answers with the tile's
 // coordinates in it; ONCE: the sum and the bias of its column are rounded together, to nearest even; TERM: `add_term` gives a wave's sums
-// what they start from.
+// what they start from, and `finish` comes after its rows are stored.
 struct M16Plain { static constexpr bool MOVES = false, ONCE = false, TERM = false; };
 
 // What one workgroup does: slots first_slot, first_slot + stride, ... of the schedule of matrix z
@@ -636,6 +636,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
                 }
             }
         }
+        if constexpr (SRC::TERM) source->template finish<T, MT, WGN, TMI, TNI>(m0, n0);
     } else {
         // Split-k: fp32 partial tiles [split][m][n].  Pass p covers CN columns of every wave's patch: accumulators go
         // to the wave's private fp32 LDS region [WM][CN + 4]; then each lane stores 8 adjacent columns of one row.
