@@ -441,15 +441,16 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  *   h[i] = scales[a] x[i] . a_a,   y[i] = x[i] . w + bias + h[i] . b_a       (rows without an adapter: y[i] = x[i] . w + bias)
  * x [rows, k], w [k, n], bias [n] or NULL, a [adapters, k, rank] and b [adapters, rank, n] dense, scales float32 [adapters] or NULL for ones, y [rows, n] with
  * unit column stride.  h [rows, rank], dense, in the accumulate type: written for rows with an adapter, kept by the caller for the backward pass.
- * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection.  16-bit types multiply h (and u below) by b (a) as two values of the type
- * that add up to it to 2^-17 (float16: 2^-22), so float16 wants them within 65504; no row sees what another segment's adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
+ * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection.  16-bit types multiply h (and u below) by b (a) as several values of 16 bits
+ * that add up to it to 2^-17 of its value (float16: 2^-22 of it, and 2^-39 of the largest that it is summed with), whatever its magnitude; no row sees what another segment's
+ * adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
  * (float32, float64, widths below 8 and operands without a unit stride: the shared product as a layer of its own, and the sum again). */
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
                                   int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):
  *   u[i] = scales[a] dy[i] . b_a^T,   dx[i] = dy[i] . w^T + u[i] . a_a^T,   da_a = sum of x[i]^T u[i],   db_a = sum of h[i]^T dy[i]
  * over the rows of all segments that use adapter a (zeros for one that none uses).  u [rows, rank]: room for it, in the accumulate type.  Any of dx [rows, k] (unit column
- * stride), da and db (dense) may be NULL; accumulate_* adds to what is there.  May take a block of the pool (16-bit types, thousands of rows of one adapter). */
+ * stride), da and db (dense) may be NULL; accumulate_* adds to what is there.  (16-bit types: an infinity of x, or of dy, leaves an infinity or NaN in da, or db.)  May take a block of the pool (16-bit types, thousands of rows of one adapter). */
 int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
                                    const float* scales, const int* ids, const int* offsets, int segments, int adapters, int rows, int k, int n, int rank,
                                    long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,

@@ -34,7 +34,7 @@ template <> struct sh_ops<f16_t> {
     }
 };
 
-// eight float32 values as two of T each: the nearest, and the nearest to what is left (nothing, where the first overflows)
+// eight float32 values as two of T each: the nearest, and the nearest to what is left (nothing, where the first is not finite)
 template <typename T>
 __device__ __forceinline__ void split_low(const float* v, u32x4_t& hi, u32x4_t& lo) {
     T h[8], l[8];
@@ -46,6 +46,28 @@ __device__ __forceinline__ void split_low(const float* v, u32x4_t& hi, u32x4_t& 
     }
     __builtin_memcpy(&hi, h, 16);
     __builtin_memcpy(&lo, l, 16);
+}
+
+// float16 reaches from 2^-24 to 65504, and sums of small gradients lie below: before they are split, values that are multiplied together are brought to a largest one of
+// 2^14 .. 2^15 by a power of two, and their product back.  Two values then add up to one to 2^-22 of it and 2^-39 of the largest.  (bfloat16 reaches as far as float32.)
+__device__ __forceinline__ uint32_t finite_bits(float v) { const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu; return b < 0x7F800000u ? b : 0u; }
+// The biased exponent of the largest finite value of the four lanes that share j = lane % 16, at least 15 (so that both powers are normal numbers)
+__device__ __forceinline__ uint32_t low_exponent(const float* v) {
+    uint32_t m = 15u << 23;
+#pragma unroll
+    for (int e = 0; e < 8; e++) { const uint32_t b = finite_bits(v[e]); m = b > m ? b : m; }
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) { const uint32_t b = __shfl_xor(m, d); m = b > m ? b : m; }
+    return m >> 23;
+}
+__device__ __forceinline__ float low_up(uint32_t exponent) { return __uint_as_float((268u - exponent) << 23); }
+__device__ __forceinline__ float low_down(uint32_t exponent) { return __uint_as_float((exponent - 14u) << 23); }
+template <typename T>
+__device__ __forceinline__ void split_scaled(const float* v, float up, u32x4_t& hi, u32x4_t& lo) {
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = v[e] * up;
+    split_low<T>(w, hi, lo);
 }
 
 // A vector of eight 16-bit values may straddle the end of its row, of which `left` are there: it is loaded `pulled(left)` values early, where it ends with the row (which

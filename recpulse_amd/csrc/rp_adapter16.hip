@@ -192,7 +192,15 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
                     for (int e = 0; e < 8; e++) raw[e] = pull_into_place(raw[e], by);
                 }
             }
-            split_low<T>(hv, hi, lo);
+            float down[4];                                                // of rows 4q + v
+            if constexpr (std::is_same<T, f16_t>::value) {
+                const uint32_t top = low_exponent(hv);
+                split_scaled<T>(hv, low_up(top), hi, lo);
+#pragma unroll
+                for (int v = 0; v < 4; v++) down[v] = __shfl(low_down(top), 4 * q + v);
+            } else {
+                split_low<T>(hv, hi, lo);
+            }
 #pragma unroll
             for (int f = 0; f < 8; f++) {
                 u32x4_t b = raw[f];
@@ -200,8 +208,14 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
 #pragma unroll
                     for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
                 }
-                acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
-                low[f] = sh_ops<T>::mma(lo, b, low[f]);
+                if constexpr (std::is_same<T, f16_t>::value) {
+                    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f}, x = sh_ops<T>::mma(hi, b, zero), y = sh_ops<T>::mma(lo, b, zero);
+#pragma unroll
+                    for (int v = 0; v < 4; v++) { acc[f][v] += x[v] * down[v]; low[f][v] += y[v] * down[v]; }
+                } else {
+                    acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
+                    low[f] = sh_ops<T>::mma(lo, b, low[f]);
+                }
             }
         }
 #pragma unroll

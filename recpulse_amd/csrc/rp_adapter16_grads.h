@@ -4,7 +4,7 @@
 // Bound by reading s, once per 32 of the rank: a workgroup owns one adapter, a strip of 128 columns of s and up to 32 of the rank, and its four
 // waves share the rows of the adapter's segments, 32 at a time in turn.  s goes from memory to registers to v_mfma_f32_16x16x32 as a
 // weight does in the kernel for few rows (rp_grouped_stream16.h): a lane transposes 8 rows x 8 columns with byte permutes.  low is
-// rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, and values beyond 65504 overflow), a product each: h and u are
+// rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, scaled by the largest value of the wave's rows, which it looks for first), a product each: h and u are
 // sums in float32, and one rounding of theirs would be as large as the result's own.
 // fp16, 2048 rows of 3 adapters, 1024 x 2048, rank 8: both 10 us, 3 beside dx's tiles (25 us together).  (Eight waves a workgroup: 8192 rows of one adapter, 4096 x 4096, 48 us instead of
 // 55 before its rows were shared out, 34 since, but 32 adapters and rank 64 144 instead of 93: a CU holds one such workgroup.)
@@ -46,12 +46,7 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     u32x4_t raw[SLOTS][8];
     float lv[SLOTS][NC][8];
     int end = 0;                                              // of the segment in hand
-    auto request = [&](auto slotc, int row0) {
-        constexpr int SL = decltype(slotc)::value;
-        const char* at = (const char*)(s + (long long)row0 * s_rs);       // (rows past the segment are another's: the descriptor ends with it)
-        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width) * 2 : 0);
-#pragma unroll
-        for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
+    auto request_low = [&](float (&to)[NC][8], int row0) {
         const float* l = low + (long long)row0 * rank;
         const __amdgpu_buffer_rsrc_t l_rsrc = buffer_rsrc(l, row0 < end ? (long long)(end - row0) * rank * 4 : 0);
 #pragma unroll
@@ -59,8 +54,16 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int r = r0 + 16 * c + j;
-                lv[SL][c][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(l_rsrc, r < rank ? ((8 * q + e) * rank + r) * 4 : (int)BUFFER_OOB, 0, 0));
+                to[c][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(l_rsrc, r < rank ? ((8 * q + e) * rank + r) * 4 : (int)BUFFER_OOB, 0, 0));
             }
+    };
+    auto request = [&](auto slotc, int row0) {
+        constexpr int SL = decltype(slotc)::value;
+        const char* at = (const char*)(s + (long long)row0 * s_rs);       // (rows past the segment are another's: the descriptor ends with it)
+        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(at, row0 < end ? ((long long)(end - 1 - row0) * s_rs + width) * 2 : 0);
+#pragma unroll
+        for (int e = 0; e < 8; e++) raw[SL][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)s_off[e], 0, 0);
+        request_low(lv[SL], row0);
         __builtin_amdgcn_sched_barrier(0);
     };
     f32x4_t acc[NC][8];
@@ -68,11 +71,18 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     for (int c = 0; c < NC; c++)
 #pragma unroll
         for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    constexpr bool SCALED = std::is_same<T, f16_t>::value;
+    uint32_t top[NC];                                         // of column 16 c + j of the rank
+#pragma unroll
+    for (int c = 0; c < NC; c++) top[c] = 15u;
     auto multiply = [&](auto slotc) {
         constexpr int SL = decltype(slotc)::value;
         u32x4_t hi[NC], lo[NC];
 #pragma unroll
-        for (int c = 0; c < NC; c++) split_low<T>(lv[SL][c], hi[c], lo[c]);
+        for (int c = 0; c < NC; c++) {
+            if constexpr (SCALED) split_scaled<T>(lv[SL][c], low_up(top[c]), hi[c], lo[c]);
+            else split_low<T>(lv[SL][c], hi[c], lo[c]);
+        }
         if (cut) {
 #pragma unroll
             for (int e = 0; e < 8; e++) raw[SL][e] = pull_into_place(raw[SL][e], by);
@@ -89,13 +99,29 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
             }
         }
     };
+    // f(first row, rows from one round of the wave's to the next) for every segment that it has rounds of
     int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
-    for_groups_of(gr, w, [&](int begin, int stop) {
-        end = stop;
-        const int turn = AG_WAVES * shares * GS_ROUND, lag = (share * AG_WAVES + wave - rounds) % (AG_WAVES * shares);
-        const int first = begin + (lag < 0 ? lag + AG_WAVES * shares : lag) * GS_ROUND;
-        rounds += (end - begin + GS_ROUND - 1) / GS_ROUND;
-        if (first >= end) return;
+    auto for_rounds = [&](auto f) {
+        rounds = 0;
+        for_groups_of(gr, w, [&](int begin, int stop) {
+            end = stop;
+            const int lag = (share * AG_WAVES + wave - rounds) % (AG_WAVES * shares);
+            const int first = begin + (lag < 0 ? lag + AG_WAVES * shares : lag) * GS_ROUND;
+            rounds += (end - begin + GS_ROUND - 1) / GS_ROUND;
+            if (first < end) f(first, AG_WAVES * shares * GS_ROUND);
+        });
+    };
+    if constexpr (SCALED)
+        for_rounds([&](int first, int turn) {
+            for (int row0 = first; row0 < end; row0 += SLOTS * turn) {
+                static_for<0, SLOTS>([&](auto sc) { request_low(lv[decltype(sc)::value], row0 + decltype(sc)::value * turn); });
+                static_for<0, SLOTS>([&](auto sc) {
+#pragma unroll
+                    for (int c = 0; c < NC; c++) { const uint32_t t = low_exponent(lv[decltype(sc)::value][c]); top[c] = t > top[c] ? t : top[c]; }
+                });
+            }
+        });
+    for_rounds([&](int first, int turn) {
         static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
         for (int row0 = first; row0 < end; row0 += SLOTS * turn)
             static_for<0, SLOTS>([&](auto sc) {
@@ -114,9 +140,11 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
         constexpr int c = decltype(cc)::value;
         if (c) __syncthreads();
 #pragma unroll
-        for (int v = 0; v < 4; v++)
+        for (int v = 0; v < 4; v++) {
+            const float down = SCALED ? __shfl(low_down(top[c]), 4 * q + v) : 1.f;
 #pragma unroll
-            for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = acc[c][f][v];
+            for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = SCALED ? acc[c][f][v] * down : acc[c][f][v];
+        }
         __syncthreads();
         // eight outputs a thread, neighbours along the output's rows
 #pragma unroll

@@ -2,7 +2,7 @@
 // term is what a tile's accumulators start from, so y is rounded once, written once and never read.
 //
 // For every segment that has rows in a wave's patch: rank / 32 (/ 16) k-steps of MFMAs, the other segments' rows zero.  h is float32 and is
-// multiplied as two values of the tensors' type (split_low).  b comes straight from memory, 16 bytes a lane where it is contiguous along
+// multiplied as two values of bfloat16; where the tensors are float16, which does not reach far enough for it, as three, and b, exactly, as two (five products).  b comes straight from memory, 16 bytes a lane where it is contiguous along
 // the rank (a_a^T, for dx) and else in 2-byte loads.  4096 x 4096 x 4096 with seven segments in bf16: 122 us at rank 16 and 132 at rank 32, beside 103 for the product
 // alone and 18 and more for a pass over y.
 // (Between the last slab and the epilogue the same code takes registers from the main loop of the 256 x 256 tile: a value or two reloaded
@@ -51,10 +51,29 @@ struct AdapterTiles {
         }
     }
 
+    // eight values as P of bfloat16 that add up to them: f(number, vector)
+    template <int P, typename F> static __device__ __forceinline__ void parts(const float* v, F f) {
+        float left[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) left[u] = v[u];
+        static_for<0, P>([&](auto pc) {
+            bf16_t part[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                part[u] = round_to<bf16_t>(left[u]);
+                left[u] -= widen(part[u]);
+                left[u] = __builtin_isfinite(left[u]) ? left[u] : 0.f;
+            }
+            u32x4_t vec;
+            __builtin_memcpy(&vec, part, 16);
+            f(pc, vec);
+        });
+    }
+
     // acc: the sums of the calling wave's patch of the tile at (m0, n0), waves WGN to a row of patches
     template <typename T, int MT, int WGN, int TMI, int TNI, typename ACC>
     __device__ __forceinline__ void add_term(ACC (&acc)[TMI][TNI], int m0, int n0) {
-        constexpr int KSTEP = MT == 32 ? 16 : 32;
+        constexpr int KSTEP = MT == 32 ? 16 : 32, HP = std::is_same<T, f16_t>::value ? 3 : 2, BP = HP - 1;       // values that h and b are multiplied as
         args_t args = arguments();
         unsigned t = threadIdx.x;                             // (the lane's numbers are made anew, too)
         asm volatile("" : "+s"(args), "+v"(t));
@@ -123,28 +142,46 @@ struct AdapterTiles {
                         bf[j] = __builtin_bit_cast(s16x8_t, v);
                     }
                 }
-                u32x4_t hi[TMI], lo[TMI];
+                u32x4_t hp[HP][TMI], bp16[BP][TNI];
 #pragma unroll
-                for (int i = 0; i < TMI; i++) split_low<T>(hv[i], hi[i], lo[i]);
+                for (int i = 0; i < TMI; i++) parts<HP>(hv[i], [&](auto pc, u32x4_t v) { hp[decltype(pc)::value][i] = v; });
+#pragma unroll
+                for (int j = 0; j < TNI; j++) {
+                    if constexpr (BP == 1) {
+                        bp16[0][j] = __builtin_bit_cast(u32x4_t, bf[j]);
+                    } else {
+                        T b[8];
+                        float wide[8];
+                        __builtin_memcpy(b, &bf[j], 16);
+#pragma unroll
+                        for (int u = 0; u < 8; u++) wide[u] = widen(b[u]);
+                        parts<BP>(wide, [&](auto pc, u32x4_t v) { bp16[decltype(pc)::value][j] = v; });
+                    }
+                }
                 // (the in-place MFMAs are opaque to the compiler: what vector instructions wrote for them has to be there)
                 if constexpr (MT == 16) {
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < TNI; j++) asm volatile("" : "+v"(bf[j]) : : "memory");
+                    for (int j = 0; j < TNI; j++)
 #pragma unroll
-                    for (int i = 0; i < TMI; i++) asm volatile("" : "+v"(hi[i]), "+v"(lo[i]) : : "memory");
+                        for (int p = 0; p < BP; p++) asm volatile("" : "+v"(bp16[p][j]) : : "memory");
+#pragma unroll
+                    for (int i = 0; i < TMI; i++)
+#pragma unroll
+                        for (int p = 0; p < HP; p++) asm volatile("" : "+v"(hp[p][i]) : : "memory");
                     asm volatile("s_nop 15" ::: "memory");
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 static_for<0, TMI>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
-                    static_for<0, TNI>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value;
-                        acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, hi[i]), bf[j], acc[i][j]);
-                    });
-                    static_for<0, TNI>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value;
-                        acc[i][j] = mfma16_ops<T>::mma(__builtin_bit_cast(s16x8_t, lo[i]), bf[j], acc[i][j]);
+                    static_for<0, HP * BP>([&](auto pc) {
+                        constexpr int p = decltype(pc)::value % HP, q = decltype(pc)::value / HP;
+                        if constexpr (p + q < HP) {           // (the rest is below 2^-24)
+                            static_for<0, TNI>([&](auto jc) {
+                                constexpr int j = decltype(jc)::value;
+                                acc[i][j] = mfma16_ops<bf16_t>::mma(__builtin_bit_cast(s16x8_t, hp[p][i]), __builtin_bit_cast(s16x8_t, bp16[q][j]), acc[i][j]);
+                            });
+                        }
                     });
                 });
             }

@@ -50,11 +50,11 @@ def once(got, want, size, terms, dt):
 
 
 # few rows; the term as a launch of its own; tiles of 64, of 128 and of 256, whole and not; segments that end inside a tile, one row long and without an adapter
-BESIDE = [(9, 4, 32, 256, 512, 16), (90, 5, 300, 264, 136, 8), (7, 3, 700, 264, 520, 12), (6, 3, 2100, 520, 1031, 16), (9, 4, 4100, 512, 4096, 32), (9, 4, 4096, 512, 4096, 40)]
+SMALL = [(9, 4, 32, 256, 512, 16), (90, 5, 300, 264, 136, 8), (7, 3, 700, 264, 520, 12), (6, 3, 2100, 264, 1031, 16)]
+LARGE = [(9, 4, 4100, 136, 4096, 32), (9, 4, 4096, 128, 4096, 40)]
 
 
-@pytest.mark.parametrize("dt", [BF16, F16, F32], ids=ids_of)
-@pytest.mark.parametrize("shape", BESIDE, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape, dt", [(s, d) for s in SMALL for d in (BF16, F16, F32)] + [(s, d) for s in LARGE for d in (BF16, F16)], ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else ids_of(v))
 def test_rows_beside_an_adapter_that_is_not_finite(shape, dt):
     """An infinity and a NaN in one adapter's factors reach the rows of that adapter and no others, and there the columns they belong to."""
     segments, adapters, rows, k, n, rank = shape
@@ -71,3 +71,75 @@ def test_rows_beside_an_adapter_that_is_not_finite(shape, dt):
     put(p, "a", (0, slice(3, 6), rank // 2), [np.inf, np.nan, -np.inf])
     put(p, "a", (1, 7, 0), np.inf)
     once(oracle.to_f64(p.backward()[0].numpy(), dt), *input_gradient(p), n + rank + 2, dt)
+
+
+# the shapes above, many rows of one adapter
+RANGES = SMALL + [(1, 1, 4100, 136, 264, 8)]
+MAGNITUDES = [(2.0 ** 8, 2.0 ** -10, 2.0 ** -14, 2.0 ** -14), (2.0 ** -10, 2.0 ** -10, 2.0 ** 10, 2.0 ** 4), (2.0 ** 7, 2.0 ** 12, 2.0 ** -12, 2.0 ** -12), (2.0 ** -8, 2.0 ** -4, 2.0 ** 10, 1)]
+
+
+def ranged(dt, shape, **scales):
+    """Operands times a power of two each; without a shared weight, whose product would hide the term, and without a bias."""
+    p = Adapters(dt, *shape, ids=[s % (shape[1] + 1) - 1 for s in range(shape[0])] if shape[0] > 1 else [0], scaled=False)
+    put(p, "w", slice(None), 0.0)
+    put(p, "bias", slice(None), 0.0)
+    for name, scale in scales.items():
+        put(p, name, slice(None), p.f[name] * scale)
+    return p
+
+
+def gradients(p):
+    """da and db, their magnitudes, and what a value 2^-22 of the largest of its column would change."""
+    _, adapters, rows, k, n, rank = p.sizes
+    f = p.f
+    da, db = np.zeros((3, adapters, k, rank)), np.zeros((3, adapters, rank, n))
+    for at, a, _ in p.spans():
+        if at.start == at.stop:
+            continue
+        u, h = f["g"][at] @ f["b"][a].T, f["x"][at] @ f["a"][a]
+        usize, hsize = np.abs(f["g"][at]) @ np.abs(f["b"][a]).T, np.abs(f["x"][at]) @ np.abs(f["a"][a])
+        x, g = np.abs(f["x"][at]), np.abs(f["g"][at])
+        for out, parts in ((da, ((f["x"][at].T, u), (x.T, usize), (x.T, np.broadcast_to(np.abs(u).max(0), u.shape)))), (db, ((h.T, f["g"][at]), (hsize.T, g), (np.broadcast_to(np.abs(h).max(0), h.shape).T, g)))):
+            for i, (left, right) in enumerate(parts):
+                out[i, a] += left @ right
+    return da, db
+
+
+@pytest.mark.parametrize("shape, magnitude, dt", [(s, m, F16) for s in RANGES for m in range(4)] + [(s, 1, BF16) for s in RANGES] + [(LARGE[0], 2, F16)],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_term_of_any_magnitude(shape, magnitude, dt):
+    """h and u far below and above what the tensors' type holds, results within it: they are float32 sums, and their products keep their digits.  (u is about
+    2^-25 in the first, h 2^-20 and u 2^17 in the second, h 2^19 and u 2^-20 in the third.)  An h or u that is off by 2^-22 of the largest of its row, or of its column in a gradient, is allowed for."""
+    p = ranged(dt, shape, **dict(zip("xabg", MAGNITUDES[magnitude])))
+    _, adapters, rows, k, n, rank = shape
+    f, unit = p.f, SPLIT[dt] * 2.0 ** -24
+    p.forward()
+    y, size = layer(p)
+    row = np.zeros((rows, n))
+    for at, i, _ in p.spans():
+        row[at] = np.abs(f["x"][at] @ f["a"][i]).max(1, keepdims=True, initial=0) @ np.abs(f["b"][i]).sum(0, keepdims=True)
+    within(oracle.to_f64(p.y.numpy(), dt), y, size + unit / UNIT[dt] / (k + rank + 10) * row, k + rank + 2 + SPLIT[dt], dt)
+    dx, da, db = p.backward()
+    want, size = input_gradient(p)
+    row = np.zeros((rows, k))
+    for at, i, _ in p.spans():
+        row[at] = np.abs(f["g"][at] @ f["b"][i].T).max(1, keepdims=True, initial=0) @ np.abs(f["a"][i]).sum(1, keepdims=True).T
+    within(oracle.to_f64(dx.numpy(), dt), want, size + unit / UNIT[dt] / (n + rank + 10) * row, n + rank + 2 + SPLIT[dt], dt)
+    for got, (want, size, column), width in zip((da, db), gradients(p), (n, k)):
+        within(oracle.to_f64(got.numpy(), dt), want, size + unit / UNIT[dt] / (rows + width + 10) * column, rows + width + 2 + SPLIT[dt], dt)
+
+
+@pytest.mark.parametrize("shape", RANGES, ids=lambda s: "x".join(map(str, s)))
+def test_term_of_rows_of_every_magnitude(shape):
+    """float16: neighbouring rows 2^16 apart, in h and in u."""
+    p = ranged(F16, shape, b=2.0 ** -6)
+    _, adapters, rows, k, n, rank = shape
+    steps = 2.0 ** np.random.default_rng(rows).integers(-12, 5, (rows, 1))
+    put(p, "x", slice(None), p.f["x"] * steps)
+    put(p, "g", slice(None), p.f["g"] * steps)
+    p.forward()
+    once(oracle.to_f64(p.y.numpy(), F16), *layer(p), k + rank + 2, F16)
+    dx, da, db = p.backward()
+    once(oracle.to_f64(dx.numpy(), F16), *input_gradient(p), n + rank + 2, F16)
+    for got, (want, size, _), width in zip((da, db), gradients(p), (n, k)):
+        once(oracle.to_f64(got.numpy(), F16), want, size, rows + width + 2, F16)
