@@ -426,8 +426,8 @@ int rp_hip_zero_rows_behind(void* x, const int* offsets, int groups, int rows, i
 /* Grouped linear layer, one weight for each group: y[i] = x[i] . w_g + bias_g for the rows i of group g.  x [rows, k], w [groups, k, n] with strides
  * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for.
  * 16-bit products of a few rows a group and k of 2048 or more may share k among workgroups where there would otherwise be too few of them: on the null stream, whose own memory
- * then holds the partial sums, and in a graph being recorded, with a block of the pool that stays with the graph (a call on the same stream before the recording sees to it that
- * the pool has one).  Other streams' calls do not: there the order of a sum, and so its last bit, may differ. */
+ * then holds the partial sums, and in a graph being recorded, with a block of the pool that stays with the graph (where the pool has one free: a call on the same stream before the
+ * recording sees to that).  Other calls do not: there the order of a sum, and so its last bit, may differ.  The same goes for dx below, of a w with unit stride along k. */
 int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,
                                   long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients: dx[i] = dy[i] . w_g^T, dw_g = sum of x[i]^T dy[i], db_g = sum of dy[i] over the group's rows (zeros for an empty group).  dx [rows, k] with

@@ -27,6 +27,21 @@ public:
     NullStreamScratch& operator=(const NullStreamScratch&) = delete;
     void* ptr = nullptr;
 };
+// Device memory for one call's sums that no other stream's call can touch: the null stream's own, or, while a graph is recorded, a free block of the
+// pool, which then stays with the graph.  Null on other streams, for more bytes and where there is none: the call goes another way.  (Outside a recording
+// a created stream's call sees to it that the pool has such a block, so that the same call can be recorded with it.)
+class CallScratch {
+public:
+    explicit CallScratch(size_t bytes);
+    ~CallScratch();
+    CallScratch(const CallScratch&) = delete;
+    CallScratch& operator=(const CallScratch&) = delete;
+    static constexpr size_t MOST = (size_t)16 << 20;
+    void* ptr = nullptr;
+private:
+    NullStreamScratch lease;
+    void* block = nullptr;
+};
 int device_cu_count();                                   // compute units of the current device (0 when it cannot be read)
 // Kernel families can be switched off for cross-checks and same-machine comparisons: RP_HIP_DISABLE holds a comma-separated
 // list of names (read once per process).  The dispatcher then takes what it would take if that kernel did not exist.

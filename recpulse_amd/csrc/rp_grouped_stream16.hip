@@ -98,28 +98,18 @@ template <typename T>
 static int launch_stream_t(const GroupedArgs& g, int dtype) {
     StreamGrid sg{(g.n + 127) / 128, 1, nullptr};
     // a second launch is worth its 4 us from about 2048 of k on (us, one weight of n = 4096 and one row, 64-column strips and shares of k: k = 1024 8.2 / 11.2, 4096 19.2 / 12.1)
-    const int want = g.k < 2048 ? 1 : stream16_splits(g, 16 << 20);
+    const int want = g.k < 2048 ? 1 : stream16_splits(g, CallScratch::MOST);
     if (want == 1) {
         const long long used = g.gr.groups < g.gr.rows ? g.gr.groups : g.gr.rows;
         const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
         return used * sg.pieces * 4 >= cus * 3ll ? launch_stream_rows<T, 8>(g, sg) : launch_stream_rows<T, 4>(g, sg);
     }
-    // Memory for the shares' sums that no other stream's call can touch: the null stream's own, or a block that stays with the graph being recorded.
-    const size_t bytes = (size_t)want * g.gr.rows * g.n * sizeof(float);
-    NullStreamScratch lease(bytes);
-    void* block = nullptr;
-    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
-    if (block && !stream_is_capturing()) {                    // (taken and given back, so that the pool has it when the same call is recorded)
-        rp_hip_free(block);
-        block = nullptr;
-    }
-    sg.partials = (float*)(lease.ptr ? lease.ptr : block);
+    const CallScratch sums((size_t)want * g.gr.rows * g.n * sizeof(float));
+    sg.partials = (float*)sums.ptr;
     if (!sg.partials) return launch_stream_rows<T, 4>(g, sg);
     sg.nsplit = want;
-    int rc = launch_stream_rows<T, 8>(g, sg);
-    if (rc == 0) rc = launch_stream16_combine(g, sg, nullptr, dtype);
-    if (block) rp_hip_free(block);
-    return rc;
+    const int rc = launch_stream_rows<T, 8>(g, sg);
+    return rc == 0 ? launch_stream16_combine(g, sg, nullptr, dtype) : rc;
 }
 
 bool grouped_stream16_takes(const GroupedArgs& g) {

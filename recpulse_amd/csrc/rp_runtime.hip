@@ -155,8 +155,31 @@ static size_t round_size(size_t bytes) {
     return (bytes + ((1u << 21) - 1)) & ~(size_t)((1u << 21) - 1);         // 2 MiB steps above
 }
 
+// A block of `size` rounded bytes that the recording in hand has let go of or the pool has free, now live; or null
+static void* free_block(int dev, size_t size) {
+    Pool& p = pool();
+    if (g_capture.active) {
+        for (size_t i = g_capture.freed.size(); i-- > 0;) {
+            const HeldBlock b = g_capture.freed[i];
+            if (b.dev != dev || b.size != size) continue;
+            g_capture.freed.erase(g_capture.freed.begin() + (long)i);
+            std::lock_guard<std::mutex> lk(p.mu);
+            p.live[b.ptr] = {dev, size};
+            return b.ptr;
+        }
+    }
+    if (!p.enabled) return nullptr;
+    std::lock_guard<std::mutex> lk(p.mu);
+    auto it = p.free_lists.find({dev, size});
+    if (it == p.free_lists.end() || it->second.empty()) return nullptr;
+    void* d = it->second.back();
+    it->second.pop_back();
+    p.live[d] = {dev, size};
+    return d;
+}
+
 // One block per device, kept until rp_hip_empty_cache.
-constexpr size_t NULL_STREAM_SCRATCH = (size_t)16 << 20;
+constexpr size_t NULL_STREAM_SCRATCH = CallScratch::MOST;
 constexpr int NULL_STREAM_DEVICES = 64;
 static std::mutex g_null_stream_mu;
 static void* g_null_stream_scratch[NULL_STREAM_DEVICES] = {};
@@ -172,6 +195,20 @@ NullStreamScratch::NullStreamScratch(size_t bytes) {
     if (!ptr) g_null_stream_mu.unlock();
 }
 NullStreamScratch::~NullStreamScratch() { if (ptr) g_null_stream_mu.unlock(); }
+
+CallScratch::CallScratch(size_t bytes) : lease(bytes) {
+    ptr = lease.ptr;
+    if (ptr || !current_stream() || bytes > MOST) return;
+    if (stream_is_capturing()) {
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return; }
+        ptr = block = free_block(dev, round_size(bytes));     // (nothing is allocated: that would end the recording)
+    } else if (pool().enabled) {
+        void* d = nullptr;
+        if (rp_hip_malloc(&d, bytes) == 0) rp_hip_free(d);
+    }
+}
+CallScratch::~CallScratch() { if (block) rp_hip_free(block); }
 
 // Pinned host memory that a copy to the host goes through: a kernel writes it across the bus and the calling thread copies it on once the stream is
 // done.  us behind a chain of six kernels, hipMemcpyAsync to pageable memory and this: 10 KB 12.8 / 3.9, 64 KB 10.7 / 5.6, 128 KB 13.5 / 8.3, 255 KB 18.9 / 13.2; the limit is one of pinned
@@ -289,27 +326,7 @@ int rp_hip_malloc(void** ptr, size_t bytes) {
     if (!check_hip(hipGetDevice(&dev), "hipGetDevice")) return -1;
     Pool& p = pool();
     size_t sz = round_size(bytes);
-    if (g_capture.active) {                          // a block this recording has already let go of
-        for (size_t i = g_capture.freed.size(); i-- > 0;) {
-            const HeldBlock b = g_capture.freed[i];
-            if (b.dev != dev || b.size != sz) continue;
-            g_capture.freed.erase(g_capture.freed.begin() + (long)i);
-            std::lock_guard<std::mutex> lk(p.mu);
-            p.live[b.ptr] = {dev, sz};
-            *ptr = b.ptr;
-            return 0;
-        }
-    }
-    if (p.enabled) {
-        std::lock_guard<std::mutex> lk(p.mu);
-        auto it = p.free_lists.find({dev, sz});
-        if (it != p.free_lists.end() && !it->second.empty()) {
-            *ptr = it->second.back();
-            it->second.pop_back();
-            p.live[*ptr] = {dev, sz};
-            return 0;
-        }
-    }
+    if ((*ptr = free_block(dev, sz))) return 0;
     void* d = nullptr;
     g_device_mallocs.fetch_add(1, std::memory_order_relaxed);
     hipError_t e = hipMalloc(&d, sz);
