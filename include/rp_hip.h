@@ -388,8 +388,10 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
  * empty group, and rows behind the last group are neither read nor written.  Operands: strides in elements, non-negative;
  * outputs overlap neither an operand nor each other.  All types; sums are in the accumulate type (float32, float64 for
  * float64) and rounded once, to nearest even; with accumulate_* the rounded product is added to what is there and the sum
- * rounded.  No entry takes a block of the pool except where its comment says so, so that calls on several streams share nothing.
- * An output's bits do not depend on which of an entry's outputs are asked for, nor on the stream, except where its comment says so. */
+ * rounded.  Calls on several streams share nothing: partial sums lie in memory of the stream's own (the null stream's and that of streams from rp_hip_stream_create; kept until
+ * rp_hip_empty_cache or the stream's end), or, in a graph being recorded, in a block of the pool that stays with the graph, where the pool has one free (a call on the same stream before
+ * the recording sees to that).  With neither a call goes a way that needs none.  An output's bits do not depend on which of an entry's outputs are asked for, nor on the stream, except
+ * where its comment says that the way without memory adds in another order. */
 
 /* Routing: each of `tokens` rows of logits (row stride logits_rs) is given its k largest entries, equal ones in the order of
  * their index; an entry of -inf is never taken (a padding token has nothing else), NaN is above every number.  Slot
@@ -425,9 +427,8 @@ int rp_hip_zero_rows_behind(void* x, const int* offsets, int groups, int rows, i
 
 /* Grouped linear layer, one weight for each group: y[i] = x[i] . w_g + bias_g for the rows i of group g.  x [rows, k], w [groups, k, n] with strides
  * (w_gs, w_rs, w_cs), bias dense [groups, n] or NULL, y [rows, n] with unit column stride.  rows: how many there are room for.
- * 16-bit products of a few rows a group and k of 2048 or more may share k among workgroups where there would otherwise be too few of them: on the null stream, whose own memory
- * then holds the partial sums, and in a graph being recorded, with a block of the pool that stays with the graph (where the pool has one free: a call on the same stream before the
- * recording sees to that).  Other calls do not: there the order of a sum, and so its last bit, may differ.  The same goes for dx below, of a w with unit stride along k. */
+ * 16-bit products of a few rows a group and k of 2048 or more share k among workgroups where there would otherwise be too few of them; without memory for the sums they do not, and
+ * add in another order.  The same goes for dx below, of a w with unit stride along k. */
 int rp_hip_grouped_linear_forward(void* y, const void* x, const void* w, const void* bias, const int* offsets, int groups, int rows, int k, int n,
                                   long long x_rs, long long x_cs, long long w_gs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients: dx[i] = dy[i] . w_g^T, dw_g = sum of x[i]^T dy[i], db_g = sum of dy[i] over the group's rows (zeros for an empty group).  dx [rows, k] with
@@ -441,7 +442,7 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  *   h[i] = scales[a] x[i] . a_a,   y[i] = x[i] . w + bias + h[i] . b_a       (rows without an adapter: y[i] = x[i] . w + bias)
  * x [rows, k], w [k, n], bias [n] or NULL, a [adapters, k, rank] and b [adapters, rank, n] dense, scales float32 [adapters] or NULL for ones, y [rows, n] with
  * unit column stride.  h [rows, rank], dense, in the accumulate type: written for rows with an adapter, kept by the caller for the backward pass.
- * May take a block of the pool, as rp_hip_gemm_strided_batched does for the shared projection.  16-bit types multiply h (and u below) by b (a) as several values of 16 bits
+ * Without memory for partial sums y (and dx below) are added up in another order where the layer is of few rows, of few tiles or of many short segments.  16-bit types multiply h (and u below) by b (a) as several values of 16 bits
  * that add up to it to 2^-17 of its value (float16: 2^-22 of it, and 2^-39 of the largest that it is summed with), whatever its magnitude; no row sees what another segment's
  * adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
  * (float32, float64, widths below 8 and operands without a unit stride: the shared product as a layer of its own, and the sum again). */
@@ -450,7 +451,7 @@ int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w
 /* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):
  *   u[i] = scales[a] dy[i] . b_a^T,   dx[i] = dy[i] . w^T + u[i] . a_a^T,   da_a = sum of x[i]^T u[i],   db_a = sum of h[i]^T dy[i]
  * over the rows of all segments that use adapter a (zeros for one that none uses).  u [rows, rank]: room for it, in the accumulate type.  Any of dx [rows, k] (unit column
- * stride), da and db (dense) may be NULL; accumulate_* adds to what is there.  (16-bit types: an infinity of x, or of dy, leaves an infinity or NaN in da, or db.)  May take a block of the pool (16-bit types, thousands of rows of one adapter). */
+ * stride), da and db (dense) may be NULL; accumulate_* adds to what is there.  (16-bit types: an infinity of x, or of dy, leaves an infinity or NaN in da, or db.) */
 int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const void* dy, const void* x, const void* w, const void* a, const void* b, const void* h,
                                    const float* scales, const int* ids, const int* offsets, int segments, int adapters, int rows, int k, int n, int rank,
                                    long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,

@@ -70,6 +70,17 @@ __device__ __forceinline__ void split_scaled(const float* v, float up, u32x4_t& 
     split_low<T>(w, hi, lo);
 }
 
+// Which of a pair of 16-bit values are an infinity or NaN: their sign bits
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+    constexpr bool f16 = std::is_same<T, f16_t>::value;
+    return ((v & (f16 ? 0x7C007C00u : 0x7F807F80u)) + (f16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;       // (an exponent of ones carries)
+}
+template <typename T> __device__ __forceinline__ u32x4_t finite_only(u32x4_t v) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) v[d] &= ~((not_finite<T>(v[d]) >> 15) * 0xFFFFu);
+    return v;
+}
+
 // A vector of eight 16-bit values may straddle the end of its row, of which `left` are there: it is loaded `pulled(left)` values early, where it ends with the row (which
 // holds eight at least), and shifted into place with zeros behind.  So every load is within its operand, none is behind a branch, and rows may start at any element.
 __device__ __forceinline__ int pulled(int left) { return left > 0 && left < 8 ? 8 - left : 0; }

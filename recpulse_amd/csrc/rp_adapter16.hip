@@ -83,19 +83,34 @@ bool adapter_few_rows16_takes(const GroupedArgs& shared, const GroupedArgs& low,
            term.b_cs == 1 && term.b_rs % 8 == 0 && ((uintptr_t)term.b & 15) == 0;
 }
 
+// Without memory for the sums: h first, then strips of 64 columns whose epilogue adds the term (the 32 rows above 42 us)
+template <typename T, int RB>
+__global__ void __launch_bounds__(GS_THREADS) adapter_strips16_kernel(GroupedArgs shared, StreamGrid sg, AdapterTerm term) { stream16_block<T, 4, RB, true>(shared, sg, blockIdx.x, &term); }
+
+template <typename T, int RB>
+static int launch_strips(const GroupedArgs& shared, const StreamGrid& sg, const AdapterTerm& term) {
+    static_assert(gs_lds_bytes<4>() <= 64 * 1024, "no more than every launch may have");
+    hipLaunchKernelGGL((adapter_strips16_kernel<T, RB>), dim3((unsigned)stream16_blocks(shared, 16 * RB, 4, 1)), dim3(GS_THREADS), gs_lds_bytes<4>(), current_stream(), shared, sg, term);
+    return check_launch("adapter_strips16_kernel") ? 0 : -1;
+}
+
+template <typename T>
+static int launch_strips_rows(const GroupedArgs& shared, const StreamGrid& sg, const AdapterTerm& term) {
+    const int rb = stream16_row_blocks(shared.gr);
+    return rb == 1 ? launch_strips<T, 1>(shared, sg, term) : rb == 2 ? launch_strips<T, 2>(shared, sg, term) : launch_strips<T, 4>(shared, sg, term);
+}
+
 int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low, const AdapterTerm& term, int dtype) {
-    // The sums lie in the null stream's own memory, or, as the split products of rp_hip_gemm_strided_batched do, in a block of the pool.
-    constexpr size_t most = 16 << 20;
-    StreamGrid sg{(shared.n + 127) / 128, stream16_splits(shared, most), nullptr};
-    const size_t bytes = (size_t)sg.nsplit * shared.gr.rows * shared.n * sizeof(float);
-    NullStreamScratch lease(bytes);
-    void* block = nullptr;
-    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
-    sg.partials = (float*)(lease.ptr ? lease.ptr : block);
-    int rc = dtype == RP_DTYPE_BFLOAT16 ? launch_first_rank<bf16_t>(shared, sg, low) : launch_first_rank<f16_t>(shared, sg, low);
-    if (rc == 0) rc = launch_stream16_combine(shared, sg, &term, dtype);
-    if (block) rp_hip_free(block);
-    return rc;
+    StreamGrid sg{(shared.n + 127) / 128, stream16_splits(shared, CallScratch::MOST), nullptr};
+    const CallScratch sums((size_t)sg.nsplit * shared.gr.rows * shared.n * sizeof(float));
+    sg.partials = (float*)sums.ptr;
+    if (!sg.partials) {
+        sg.nsplit = 1;
+        if (launch_adapter_shrink16(low, dtype) != 0) return -1;
+        return dtype == RP_DTYPE_BFLOAT16 ? launch_strips_rows<bf16_t>(shared, sg, term) : launch_strips_rows<f16_t>(shared, sg, term);
+    }
+    const int rc = dtype == RP_DTYPE_BFLOAT16 ? launch_first_rank<bf16_t>(shared, sg, low) : launch_first_rank<f16_t>(shared, sg, low);
+    return rc == 0 ? launch_stream16_combine(shared, sg, &term, dtype) : rc;
 }
 
 // ---- the term by itself, where the shared product is too small, or a tile's rows too many segments, for its tiles to take the term in ----
@@ -147,9 +162,9 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
     if (m <= 0) return;
     const int col = (int)(blockIdx.x % ea.strips) * 128 + 8 * j, left = n - col, by = pulled(left);
     const bool cut = col - 8 * j + 128 > n && n % 8;                      // (the strip's last vector ends with the row)
-    f32x4_t acc[8], low[8];                                               // rows 4q + v, column col + f; the products with h's lower values
+    f32x4_t acc[8];                                                       // rows 4q + v, column col + f
 #pragma unroll
-    for (int f = 0; f < 8; f++) acc[f] = low[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < 8; f++) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < ea.shares; s++) {
         const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(ea.sums + ((long long)s * ea.rows + rt.begin) * n, (long long)m * n * 4);
         u32x4_t p[4][2];
@@ -192,6 +207,12 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
                     for (int e = 0; e < 8; e++) raw[e] = pull_into_place(raw[e], by);
                 }
             }
+            uint32_t any = 0;
+#pragma unroll
+            for (int f = 0; f < 8; f++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) any |= not_finite<T>(raw[f][d]);
+            const bool odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
             float down[4];                                                // of rows 4q + v
             if constexpr (std::is_same<T, f16_t>::value) {
                 const uint32_t top = low_exponent(hv);
@@ -208,20 +229,18 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
 #pragma unroll
                     for (int d = 0; d < 4; d++) b[d] = __builtin_amdgcn_perm(raw[2 * d + 1][f / 2], raw[2 * d][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
                 }
+                // (an infinity of b times a lower value that is 0 or of the other sign is not what there is to add: the higher one's product is)
+                const u32x4_t b_low = odd ? finite_only<T>(b) : b;
                 if constexpr (std::is_same<T, f16_t>::value) {
-                    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f}, x = sh_ops<T>::mma(hi, b, zero), y = sh_ops<T>::mma(lo, b, zero);
+                    const f32x4_t x = sh_ops<T>::mma(lo, b_low, sh_ops<T>::mma(hi, b, f32x4_t{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-                    for (int v = 0; v < 4; v++) { acc[f][v] += x[v] * down[v]; low[f][v] += y[v] * down[v]; }
+                    for (int v = 0; v < 4; v++) acc[f][v] += x[v] * down[v];
                 } else {
                     acc[f] = sh_ops<T>::mma(hi, b, acc[f]);
-                    low[f] = sh_ops<T>::mma(lo, b, low[f]);
+                    acc[f] = sh_ops<T>::mma(lo, b_low, acc[f]);
                 }
             }
         }
-#pragma unroll
-        for (int f = 0; f < 8; f++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) acc[f][v] += __builtin_isfinite(low[f][v]) ? low[f][v] : 0.f;      // (an infinity of b: the higher value's product is what there is to add)
     }
     if (left <= 0) return;
     float bias[8] = {};
@@ -268,24 +287,23 @@ static int launch_expand(const ExpandArgs& ea, const AdapterTerm& term) {
     return check_launch("adapter_expand16_kernel") ? 0 : -1;
 }
 
-int launch_adapter_expand16(const GroupedArgs& s, const AdapterTerm& term, bool ragged, int dtype) {
+int launch_adapter_expand16(const GroupedArgs& s, const AdapterTerm& term, bool ragged, int dtype, bool* taken) {
     ragged = ragged || s.n % 8;                               // (the sums are stored in whole vectors otherwise)
+    constexpr size_t most = (size_t)1 << 30;
     const int rows = s.gr.rows, cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const bool large = (long long)((rows + 127) / 128) * ((s.n + 127) / 128) * 2 >= cus;
     const int shares = large ? 1 : skinny16_sums_shares(rows, s.k, s.n);
-    const size_t bytes = (size_t)shares * rows * s.n * sizeof(float);
-    NullStreamScratch lease(bytes);
-    void* block = nullptr;
-    if (!lease.ptr && rp_hip_malloc(&block, bytes) != 0) return -1;
-    float* sums = (float*)(lease.ptr ? lease.ptr : block);
+    const CallScratch memory((size_t)shares * rows * s.n * sizeof(float), most);
+    float* sums = (float*)memory.ptr;
+    *taken = sums != nullptr;
+    if (!sums) return 0;
     const GemmArgs g{nullptr, s.A, s.B, nullptr, 1, rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.n, 1, 0};
     Plan p{FAM_MFMA16_SKINNY, 32, 128, false, s.b_cs == 1, true, ""};
     p.ragged = ragged;
-    int rc = large ? launch_sums16_128(g, p.b_mc, ragged, sums, dtype) : launch_skinny16_sums(g, p, sums, dtype);
+    const int rc = large ? launch_sums16_128(g, p.b_mc, ragged, sums, dtype) : launch_skinny16_sums(g, p, sums, dtype);
     const ExpandArgs ea{(uint16_t*)s.C, (const uint16_t*)s.bias, sums, s.n, rows, shares, s.accumulate, (s.n + 127) / 128, s.c_rs};
-    if (rc == 0) rc = dtype == RP_DTYPE_BFLOAT16 ? launch_expand<bf16_t>(ea, term) : launch_expand<f16_t>(ea, term);
-    if (block) rp_hip_free(block);
-    return rc;
+    if (rc != 0) return rc;
+    return dtype == RP_DTYPE_BFLOAT16 ? launch_expand<bf16_t>(ea, term) : launch_expand<f16_t>(ea, term);
 }
 
 }  // namespace rp

@@ -23,12 +23,16 @@ static int launch_adapter_backward16(const GroupedArgs& s, const AdapterTerm& te
     const int tiles_m = (s.gr.rows + B - 1) / B, tiles_n = (s.n + B - 1) / B, total = scheduled_grid(tiles_m, tiles_n);
     constexpr size_t tile = m16_smem_bytes(B, B, 2, false, false, 2, 32), smem = tile > AG_LDS ? tile : AG_LDS;
     const GemmArgs g{s.C, s.A, s.B, nullptr, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate};
-    const int grad_blocks = (ag.a.blocks + ag.b.blocks + 7) / 8 * 8;        // (the tiles' schedule goes by workgroup modulo 8)
     auto kern = adapter_backward16_kernel<T, B, EDGE, NC>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
     return with_joined_grads<T>(ag, term.gr, [&]() -> int {
+        const int grad_blocks = (ag.a.blocks + ag.b.blocks + 7) / 8 * 8;        // (the tiles' schedule goes by workgroup modulo 8)
         hipLaunchKernelGGL(kern, dim3((unsigned)(grad_blocks + total)), dim3(256), smem, current_stream(), AdapterTileArgs{g, tiles_m, tiles_n, total, term}, ag, grad_blocks);
         return check_launch("adapter_backward16_kernel") ? 0 : -1;
+    }, [&]() -> int {
+        const int dtype = traits<T>::code;
+        if ((B == 128 ? launch_adapter_tiles16_128(s, term, true, EDGE == M16_RAGGED, dtype) : launch_adapter_tiles16_64(s, term, EDGE == M16_RAGGED, dtype)) != 0) return -1;
+        return launch_adapter_grads16_in_turn(ag, term.gr, dtype);
     });
 }
 

@@ -25,16 +25,16 @@ struct AdapterGrad {
     long long s_rs, out_ws, out_rs;
 };
 
-// NC: 16-row tiles of the rank
-template <typename T, int NC, bool TRANSPOSED>
+// NC: 16-row tiles of the rank; IN_TURN: a workgroup does one share of the rows after the other
+template <typename T, int NC, bool TRANSPOSED, bool IN_TURN>
 __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, const RowGroups& gr, int rank, int rank_blocks, int shares, int block) {
-    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH]
+    extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [AG_WAVES][16][AG_PITCH], and [16 NC][AG_COLS] of the shares before (IN_TURN)
     T* out = (T*)ag.out;
     const uint16_t* s = (const uint16_t*)ag.s;
     const float* low = ag.low;
     const int width = ag.width, accumulate = ag.accumulate;
     const long long s_rs = ag.s_rs, out_ws = ag.out_ws, out_rs = ag.out_rs;
-    const int share = block % shares, id = block / shares, strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
+    const int first_share = IN_TURN ? 0 : block % shares, id = IN_TURN ? block : block / shares, strip = id % ag.strips, rb = id / ag.strips % rank_blocks, w = id / ag.strips / rank_blocks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int n0 = strip * AG_COLS, r0 = rb * 16 * NC;
     const int left = width - n0 - 8 * j, by = pulled(left);
@@ -67,14 +67,8 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
         __builtin_amdgcn_sched_barrier(0);
     };
     f32x4_t acc[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-        for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     constexpr bool SCALED = std::is_same<T, f16_t>::value;
     uint32_t top[NC];                                         // of column 16 c + j of the rank
-#pragma unroll
-    for (int c = 0; c < NC; c++) top[c] = 15u;
     auto multiply = [&](auto slotc) {
         constexpr int SL = decltype(slotc)::value;
         u32x4_t hi[NC], lo[NC];
@@ -100,7 +94,7 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
         }
     };
     // f(first row, rows from one round of the wave's to the next) for every segment that it has rounds of
-    int rounds = 0;                                           // of the segments before, so that short segments go to the waves in turn
+    int share = first_share, rounds = 0;                      // of the segments before, so that short segments go to the waves in turn
     auto for_rounds = [&](auto f) {
         rounds = 0;
         for_groups_of(gr, w, [&](int begin, int stop) {
@@ -111,75 +105,89 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
             if (first < end) f(first, AG_WAVES * shares * GS_ROUND);
         });
     };
-    if constexpr (SCALED)
-        for_rounds([&](int first, int turn) {
-            for (int row0 = first; row0 < end; row0 += SLOTS * turn) {
-                static_for<0, SLOTS>([&](auto sc) { request_low(lv[decltype(sc)::value], row0 + decltype(sc)::value * turn); });
-                static_for<0, SLOTS>([&](auto sc) {
+    while (true) {
 #pragma unroll
-                    for (int c = 0; c < NC; c++) { const uint32_t t = low_exponent(lv[decltype(sc)::value][c]); top[c] = t > top[c] ? t : top[c]; }
+        for (int c = 0; c < NC; c++) {
+            top[c] = 15u;
+#pragma unroll
+            for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        if constexpr (SCALED)
+            for_rounds([&](int first, int turn) {
+                for (int row0 = first; row0 < end; row0 += SLOTS * turn) {
+                    static_for<0, SLOTS>([&](auto sc) { request_low(lv[decltype(sc)::value], row0 + decltype(sc)::value * turn); });
+                    static_for<0, SLOTS>([&](auto sc) {
+#pragma unroll
+                        for (int c = 0; c < NC; c++) { const uint32_t t = low_exponent(lv[decltype(sc)::value][c]); top[c] = t > top[c] ? t : top[c]; }
+                    });
+                }
+            });
+        for_rounds([&](int first, int turn) {
+            static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
+            for (int row0 = first; row0 < end; row0 += SLOTS * turn)
+                static_for<0, SLOTS>([&](auto sc) {
+                    multiply(sc);
+                    request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
                 });
+        });
+        if (rounds == 0) {                                        // an adapter without rows: zeros, or what is there
+            for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate && first_share == 0; i += AG_THREADS) {
+                const int r = r0 + (TRANSPOSED ? i % (16 * NC) : i / AG_COLS), col = n0 + (TRANSPOSED ? i / (16 * NC) : i % AG_COLS);
+                if (r < rank && col < width) out[w * out_ws + (TRANSPOSED ? col * out_rs + r : r * out_rs + col)] = round_to<T>(0.f);
+            }
+            return;
+        }
+        static_for<0, NC>([&](auto cc) {
+            constexpr int c = decltype(cc)::value;
+            if (c || (IN_TURN && share)) __syncthreads();
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const float down = SCALED ? __shfl(low_down(top[c]), 4 * q + v) : 1.f;
+#pragma unroll
+                for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = SCALED ? acc[c][f][v] * down : acc[c][f][v];
+            }
+            __syncthreads();
+            // eight outputs a thread, neighbours along the output's rows
+#pragma unroll
+            for (int o = 0; o < 16 * AG_COLS / AG_THREADS; o++) {
+                const int id = threadIdx.x + o * AG_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
+                if (r0 + 16 * c + r >= rank || n0 + col >= width) continue;
+                float t = gs_sums[r * AG_PITCH + col];
+#pragma unroll
+                for (int p = 1; p < AG_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
+                const long long to = w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
+                if (!IN_TURN && ag.partials) {
+                    ag.partials[share * (out_ws * gr.weights) + to] = t;
+                    continue;
+                }
+                if constexpr (IN_TURN) {                               // (in the order of the launch that adds them up; a thread's own values)
+                    float* before = gs_sums + AG_WAVES * 16 * AG_PITCH + c * 16 * AG_COLS + id;
+                    if (share) t = *before + t;
+                    if (share + 1 < shares) { *before = t; continue; }
+                }
+                T* at = out + to;
+                T y = round_to<T>(t);
+                if (accumulate) y = round_to<T>(widen(*at) + widen(y));
+                *at = y;
             }
         });
-    for_rounds([&](int first, int turn) {
-        static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
-        for (int row0 = first; row0 < end; row0 += SLOTS * turn)
-            static_for<0, SLOTS>([&](auto sc) {
-                multiply(sc);
-                request(sc, row0 + (SLOTS + decltype(sc)::value) * turn);
-            });
-    });
-    if (rounds == 0) {                                        // an adapter without rows: zeros, or what is there
-        for (int i = threadIdx.x; i < 16 * NC * AG_COLS && !accumulate && share == 0; i += AG_THREADS) {
-            const int r = r0 + (TRANSPOSED ? i % (16 * NC) : i / AG_COLS), col = n0 + (TRANSPOSED ? i / (16 * NC) : i % AG_COLS);
-            if (r < rank && col < width) out[w * out_ws + (TRANSPOSED ? col * out_rs + r : r * out_rs + col)] = round_to<T>(0.f);
-        }
-        return;
+        if (!IN_TURN || ++share == shares) break;
     }
-    static_for<0, NC>([&](auto cc) {
-        constexpr int c = decltype(cc)::value;
-        if (c) __syncthreads();
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            const float down = SCALED ? __shfl(low_down(top[c]), 4 * q + v) : 1.f;
-#pragma unroll
-            for (int f = 0; f < 8; f++) gs_sums[(wave * 16 + 4 * q + v) * AG_PITCH + 8 * j + f] = SCALED ? acc[c][f][v] * down : acc[c][f][v];
-        }
-        __syncthreads();
-        // eight outputs a thread, neighbours along the output's rows
-#pragma unroll
-        for (int o = 0; o < 16 * AG_COLS / AG_THREADS; o++) {
-            const int id = threadIdx.x + o * AG_THREADS, r = TRANSPOSED ? id & 15 : id / AG_COLS, col = TRANSPOSED ? id >> 4 : id % AG_COLS;
-            if (r0 + 16 * c + r >= rank || n0 + col >= width) continue;
-            float t = gs_sums[r * AG_PITCH + col];
-#pragma unroll
-            for (int p = 1; p < AG_WAVES; p++) t += gs_sums[(p * 16 + r) * AG_PITCH + col];
-            const long long to = w * out_ws + (TRANSPOSED ? (n0 + col) * out_rs + r0 + 16 * c + r : (r0 + 16 * c + r) * out_rs + n0 + col);
-            if (ag.partials) {
-                ag.partials[share * (out_ws * gr.weights) + to] = t;
-                continue;
-            }
-            T* at = out + to;
-            T y = round_to<T>(t);
-            if (accumulate) y = round_to<T>(widen(*at) + widen(y));
-            *at = y;
-        }
-    });
 }
 
 constexpr int AG_LDS = AG_WAVES * 16 * AG_PITCH * 4;
 
 // dA's workgroups, then dB's: each alone leaves most of the chip waiting for loads.  Where few adapters have many rows each, several workgroups share the rows
-// and a second launch adds their sums in order (adapter_grads16_join_kernel).
+// and a second launch adds their sums in order (adapter_grads16_join_kernel), or one workgroup does one share after the other where there is no memory for the sums.
 struct AdapterGrads { AdapterGrad a, b; int rank, rank_blocks, shares; };
-template <typename T, int NC>
+int launch_adapter_grads16_in_turn(const AdapterGrads& ag, const RowGroups& gr, int dtype);      // (rp_adapter16_grads.hip)
+template <typename T, int NC, bool IN_TURN = false>
 __device__ __forceinline__ void adapter_grads16_block(const AdapterGrads& ag, const RowGroups& gr, int id) {
-    if (id < ag.a.blocks) adapter_grad16_block<T, NC, true>(ag.a, gr, ag.rank, ag.rank_blocks, ag.shares, id);
-    else if (id < ag.a.blocks + ag.b.blocks) adapter_grad16_block<T, NC, false>(ag.b, gr, ag.rank, ag.rank_blocks, ag.shares, id - ag.a.blocks);
+    if (id < ag.a.blocks) adapter_grad16_block<T, NC, true, IN_TURN>(ag.a, gr, ag.rank, ag.rank_blocks, ag.shares, id);
+    else if (id < ag.a.blocks + ag.b.blocks) adapter_grad16_block<T, NC, false, IN_TURN>(ag.b, gr, ag.rank, ag.rank_blocks, ag.shares, id - ag.a.blocks);
 }
 
 static inline int grads_rank_tiles(int rank) { return rank <= 16 ? 1 : 2; }
-constexpr long long AG_MOST_SUMS = 16 << 20;                  // bytes
 // Those gradients whose C is not null; false: more workgroups than a launch takes.  How many share an adapter's rows goes by the sizes alone, not by what is asked for.
 static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, AdapterGrads& ag) {
     ag.a = AdapterGrad{da.C, nullptr, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
@@ -192,13 +200,13 @@ static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, Adap
     // Shares of eight turns of 128 rows or more, as many as keep two workgroups on a CU (bf16, 7949 rows of one adapter, 384 x 1512, rank 32, forward and backward: 144 us, 118 with seven shares)
     const long long used = da.gr.groups < da.gr.weights ? da.gr.groups : da.gr.weights, blocks = used * (ag.a.strips + ag.b.strips) * ag.rank_blocks;
     const long long cus = device_cu_count() > 0 ? device_cu_count() : 256, turns = da.gr.rows / used / (AG_WAVES * GS_ROUND);
-    const long long room = AG_MOST_SUMS / (((long long)ag.a.width + ag.b.width) * ag.rank * da.gr.weights * (long long)sizeof(float));
+    const long long room = (long long)CallScratch::MOST / (((long long)ag.a.width + ag.b.width) * ag.rank * da.gr.weights * (long long)sizeof(float));
     long long shares = turns / 8 < 2 * cus / blocks ? turns / 8 : 2 * cus / blocks;
     shares = shares < room ? shares : room;
     ag.shares = shares > 1 ? (int)shares : 1;
     for (AdapterGrad* g : {&ag.a, &ag.b}) {
-        const long long own = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights * ag.shares : 0;
-        if (own > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", own); return false; }
+        const long long own = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights : 0;
+        if (own * ag.shares > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", own); return false; }
         g->blocks = (int)own;
     }
     return true;
@@ -223,25 +231,22 @@ __global__ void __launch_bounds__(256) adapter_grads16_join_kernel(AdapterGrads 
     *out = y;
 }
 
-// Runs `launch`, with memory for the shares' sums (the null stream's own, or a block of the pool) and the launch that adds them up where there are any
-template <typename T, typename F>
-static int with_joined_grads(AdapterGrads& ag, const RowGroups& gr, F launch) {
+// Where shares of an adapter's rows are added up, `launch` leaves them in the call's memory for a launch of their own, or, without memory, `in_turn` has workgroups do one share after
+// the other: the same bits (bf16, 7949 rows of one adapter, 384 x 1512, rank 32, forward and backward 118 us and 144).
+template <typename T, typename F, typename G>
+static int with_joined_grads(AdapterGrads& ag, const RowGroups& gr, F launch, G in_turn) {
     if (ag.shares == 1) return launch();
     const size_t a_sums = ag.a.out ? (size_t)ag.shares * ag.a.width * ag.rank * gr.weights : 0, b_sums = ag.b.out ? (size_t)ag.shares * ag.b.width * ag.rank * gr.weights : 0;
-    NullStreamScratch lease((a_sums + b_sums) * sizeof(float));
-    void* block = nullptr;
-    if (!lease.ptr && rp_hip_malloc(&block, (a_sums + b_sums) * sizeof(float)) != 0) return -1;
-    float* sums = (float*)(lease.ptr ? lease.ptr : block);
-    if (ag.a.out) ag.a.partials = sums;
-    if (ag.b.out) ag.b.partials = sums + a_sums;
-    int rc = launch();
-    if (rc == 0) {
-        const int a_per = (ag.a.width * ag.rank + 255) / 256, b_per = (ag.b.width * ag.rank + 255) / 256, a_blocks = ag.a.out ? a_per * gr.weights : 0, b_blocks = ag.b.out ? b_per * gr.weights : 0;
-        hipLaunchKernelGGL(adapter_grads16_join_kernel<T>, dim3((unsigned)(a_blocks + b_blocks)), dim3(256), 0, current_stream(), ag, gr, a_blocks, a_per, b_per);
-        rc = check_launch("adapter_grads16_join_kernel") ? 0 : -1;
-    }
-    if (block) rp_hip_free(block);
-    return rc;
+    const CallScratch sums((a_sums + b_sums) * sizeof(float));
+    if (!sums.ptr) return in_turn();
+    ag.a.blocks *= ag.shares;
+    ag.b.blocks *= ag.shares;
+    ag.a.partials = (float*)sums.ptr;
+    ag.b.partials = (float*)sums.ptr + a_sums;
+    if (launch() != 0) return -1;
+    const int a_per = (ag.a.width * ag.rank + 255) / 256, b_per = (ag.b.width * ag.rank + 255) / 256, a_blocks = ag.a.out ? a_per * gr.weights : 0, b_blocks = ag.b.out ? b_per * gr.weights : 0;
+    hipLaunchKernelGGL(adapter_grads16_join_kernel<T>, dim3((unsigned)(a_blocks + b_blocks)), dim3(256), 0, current_stream(), ag, gr, a_blocks, a_per, b_per);
+    return check_launch("adapter_grads16_join_kernel") ? 0 : -1;
 }
 
 }  // namespace rp

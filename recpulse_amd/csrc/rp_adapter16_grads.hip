@@ -3,15 +3,27 @@
 
 namespace rp {
 
-template <typename T, int NC>
-__global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr) { adapter_grads16_block<T, NC>(ag, gr, (int)blockIdx.x); }
+template <typename T, int NC, bool IN_TURN>
+__global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr) { adapter_grads16_block<T, NC, IN_TURN>(ag, gr, (int)blockIdx.x); }
 
-template <typename T, int NC>
-static int launch_grads(AdapterGrads& ag, const RowGroups& gr) {
-    return with_joined_grads<T>(ag, gr, [&]() -> int {
-        hipLaunchKernelGGL((adapter_grads16_kernel<T, NC>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), AG_LDS, current_stream(), ag, gr);
-        return check_launch("adapter_grads16_kernel") ? 0 : -1;
-    });
+template <typename T, int NC, bool IN_TURN>
+static int launch_grads(const AdapterGrads& ag, const RowGroups& gr) {
+    constexpr int lds = AG_LDS + (IN_TURN ? NC * 16 * AG_COLS * 4 : 0);
+    static_assert(lds <= 64 * 1024, "no more than every launch may have");
+    hipLaunchKernelGGL((adapter_grads16_kernel<T, NC, IN_TURN>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), lds, current_stream(), ag, gr);
+    return check_launch("adapter_grads16_kernel") ? 0 : -1;
+}
+
+template <typename T, bool IN_TURN>
+static int launch_grads_rank(const AdapterGrads& ag, const RowGroups& gr) { return grads_rank_tiles(ag.rank) == 1 ? launch_grads<T, 1, IN_TURN>(ag, gr) : launch_grads<T, 2, IN_TURN>(ag, gr); }
+
+int launch_adapter_grads16_in_turn(const AdapterGrads& ag, const RowGroups& gr, int dtype) {
+    return dtype == RP_DTYPE_BFLOAT16 ? launch_grads_rank<bf16_t, true>(ag, gr) : launch_grads_rank<f16_t, true>(ag, gr);
+}
+
+template <typename T>
+static int launch_joined(AdapterGrads& ag, const RowGroups& gr, int dtype) {
+    return with_joined_grads<T>(ag, gr, [&] { return launch_grads_rank<T, false>(ag, gr); }, [&] { return launch_adapter_grads16_in_turn(ag, gr, dtype); });
 }
 
 bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
@@ -24,9 +36,7 @@ bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
     AdapterGrads ag;
     if (!plan_grads(da, db, ag)) return -1;
-    const bool one = grads_rank_tiles(ag.rank) == 1;
-    if (dtype == RP_DTYPE_BFLOAT16) return one ? launch_grads<bf16_t, 1>(ag, da.gr) : launch_grads<bf16_t, 2>(ag, da.gr);
-    return one ? launch_grads<f16_t, 1>(ag, da.gr) : launch_grads<f16_t, 2>(ag, da.gr);
+    return dtype == RP_DTYPE_BFLOAT16 ? launch_joined<bf16_t>(ag, da.gr, dtype) : launch_joined<f16_t>(ag, da.gr, dtype);
 }
 
 }  // namespace rp

@@ -20,12 +20,6 @@ struct AdapterTileArgs {
     AdapterTerm term;
 };
 
-// Which of a pair of 16-bit values are an infinity or NaN: their sign bits
-template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
-    constexpr bool f16 = std::is_same<T, f16_t>::value;
-    return ((v & (f16 ? 0x7C007C00u : 0x7F807F80u)) + (f16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;       // (an exponent of ones carries)
-}
-
 struct AdapterTiles {
     static constexpr bool MOVES = false, ONCE = true, TERM = true;
     bool odd = false;              // the wave met an infinity or NaN in b
@@ -136,10 +130,7 @@ struct AdapterTiles {
                     odd = true;
 #pragma unroll
                     for (int j = 0; j < TNI; j++) {
-                        u32x4_t v = __builtin_bit_cast(u32x4_t, bf[j]);
-#pragma unroll
-                        for (int d = 0; d < 4; d++) v[d] &= ~((not_finite<T>(v[d]) >> 15) * 0xFFFFu);
-                        bf[j] = __builtin_bit_cast(s16x8_t, v);
+                        bf[j] = __builtin_bit_cast(s16x8_t, finite_only<T>(__builtin_bit_cast(u32x4_t, bf[j])));
                     }
                 }
                 u32x4_t hp[HP][TMI], bp16[BP][TNI];

@@ -27,19 +27,21 @@ public:
     NullStreamScratch& operator=(const NullStreamScratch&) = delete;
     void* ptr = nullptr;
 };
-// Device memory for one call's sums that no other stream's call can touch: the null stream's own, or, while a graph is recorded, a free block of the
-// pool, which then stays with the graph.  Null on other streams, for more bytes and where there is none: the call goes another way.  (Outside a recording
-// a created stream's call sees to it that the pool has such a block, so that the same call can be recorded with it.)
+// Device memory for one call's sums that no other stream's call can touch: a block of the stream's own (the null stream's, or that of a stream that rp_hip_stream_create made; work on one
+// stream runs in order, and the lease is held until the call's last launch), or, while a graph is recorded, a free block of the pool, which then stays with the graph.  Null on streams
+// that this library does not know the end of, for more bytes than `most` and where there is none: the call goes another way.  (Outside a recording a created stream's call sees to it
+// that the pool has such a block, so that the same call can be recorded with it.)
+struct StreamMemory;
 class CallScratch {
 public:
-    explicit CallScratch(size_t bytes);
+    static constexpr size_t MOST = (size_t)16 << 20;
+    explicit CallScratch(size_t bytes, size_t most = MOST);
     ~CallScratch();
     CallScratch(const CallScratch&) = delete;
     CallScratch& operator=(const CallScratch&) = delete;
-    static constexpr size_t MOST = (size_t)16 << 20;
     void* ptr = nullptr;
 private:
-    NullStreamScratch lease;
+    StreamMemory* memory = nullptr;                // locked while leased
     void* block = nullptr;
 };
 int device_cu_count();                                   // compute units of the current device (0 when it cannot be read)

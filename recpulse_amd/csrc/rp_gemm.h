@@ -173,6 +173,18 @@ int* splitk_arrival_counters(long long tiles, size_t partial_bytes, bool* failed
 // nothing, a piece of that entry point's fixed device array (then -1 with an error when it is too small).
 int gemm_workspace(void** ws, size_t bytes);
 void gemm_workspace_release(void* ws);
+// While one lives, the calling thread's GEMMs take their workspace from `ptr` (null: there is none) and not from the pool; a product that would need more
+// launches nothing, returns -1 and leaves `refused`.
+class GemmWorkspaceLoan {
+public:
+    GemmWorkspaceLoan(void* ptr, size_t bytes);
+    ~GemmWorkspaceLoan();
+    GemmWorkspaceLoan(const GemmWorkspaceLoan&) = delete;
+    GemmWorkspaceLoan& operator=(const GemmWorkspaceLoan&) = delete;
+    void* const ptr;
+    const size_t bytes;
+    bool refused = false;
+};
 // Inside the entry point that allocates nothing: its arrival counters, cleared by a kernel on the current stream the
 // first time a call asks for them (nullptr with an error when that launch fails).
 bool noalloc_active();

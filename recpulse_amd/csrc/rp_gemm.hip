@@ -495,7 +495,16 @@ static unsigned char* noalloc_scratch_of_current_device() {
     return g_scratch_ptr[dev];
 }
 
+static thread_local GemmWorkspaceLoan* g_loan = nullptr;
+GemmWorkspaceLoan::GemmWorkspaceLoan(void* p, size_t b) : ptr(p), bytes(b) { g_loan = this; }
+GemmWorkspaceLoan::~GemmWorkspaceLoan() { g_loan = nullptr; }
+
 int gemm_workspace(void** ws, size_t bytes) {
+    if (g_loan) {
+        g_loan->refused = !g_loan->ptr || bytes > g_loan->bytes;
+        *ws = g_loan->ptr;
+        return g_loan->refused ? -1 : 0;
+    }
     if (!g_noalloc_base) return rp_hip_malloc(ws, bytes);
     *ws = nullptr;
     if (bytes > NOALLOC_WORKSPACE_BYTES) {
@@ -509,6 +518,7 @@ int gemm_workspace(void** ws, size_t bytes) {
 }
 
 void gemm_workspace_release(void* ws) {
+    if (g_loan) return;
     if (!ws) return;
     if (g_noalloc_base && ws == g_noalloc_base + NOALLOC_COUNTER_BYTES) { g_noalloc_busy = false; return; }
     rp_hip_free(ws);

@@ -90,7 +90,7 @@ bool adapter_shrink16_takes(const GroupedArgs& g);
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype);
 // The shared product as float32 sums, then y = sums + bias + h[i] . b_a (rp_adapter16.hip); ragged: rows of any length and start
 bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term);
-int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, bool ragged, int dtype);
+int launch_adapter_expand16(const GroupedArgs& shared, const AdapterTerm& term, bool ragged, int dtype, bool* taken);      // not taken: no memory for the sums
 int launch_sums16_128(const GemmArgs& g, bool b_mc, bool ragged, float* sums, int dtype);      // [m][n], rp_adapter16_sums.hip
 // The shared product with that term in it, on MFMA tiles (rp_adapter16_tiles*.hip)
 int launch_adapter_tiles16_256_bf16(const GroupedArgs& shared, const AdapterTerm& term, bool edge);

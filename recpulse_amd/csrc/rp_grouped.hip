@@ -105,9 +105,9 @@ static int narrow_weights(const GroupedArgs& da, const GroupedArgs& db, int dtyp
 }
 
 // Tiles on which the shared product of a layer with adapters takes their term in (edge 0: none); whole: nothing hangs over
-struct TermTile { int edge; bool whole, ragged, sums; };       // sums: the product can be had as float32 sums instead
+struct TermTile { int edge; bool whole, ragged, sums; int last; };       // sums: the product can be had as float32 sums instead; last: the edge to take where there is no memory for those
 static TermTile term_tile(const GroupedArgs& s, const AdapterTerm& term, int dtype) {
-    if (!is16(dtype) || s.a_cs != 1 || (s.b_cs != 1 && s.b_rs != 1) || path_disabled("mfma")) return {0, false, false, false};
+    if (!is16(dtype) || s.a_cs != 1 || (s.b_cs != 1 && s.b_rs != 1) || path_disabled("mfma")) return {0, false, false, false, 0};
     Plan p{FAM_MFMA16, 64, 64, false, s.b_cs == 1, true, ""};
     const Lie lie = worse(lies(s.A, s.a_rs, 0, s.k, 2), p.b_mc ? lies(s.B, s.b_rs, 0, s.n, 2) : lies(s.B, s.b_cs, 0, s.k, 2));
     p.ragged = lie == LIE_RAGGED;
@@ -120,8 +120,9 @@ static TermTile term_tile(const GroupedArgs& s, const AdapterTerm& term, int dty
     const bool reach = (long long)s.gr.rows * term.rank < (1 << 29) && ((term.rank - 1) * term.b_rs + (s.n - 1) * term.b_cs) < (1 << 30);
     // from about a tile for every other CU on, and while a tile's rows are few segments: each costs it 2 us (bf16, 4096 rows, us in the tiles and apart: 400 segments, 1024 -> 4096,
     // rank 8 111 / 89, 4096 -> 4096, rank 32 189 / 196; 7 segments 127 / 178)
-    if (!reach || lie == LIE_NEITHER || p.bm != p.bn || tiles * 2 < cus() || term.gr.rows / term.gr.groups < 16 || path_disabled("adapter_tiles")) return {0, false, p.ragged, lie != LIE_NEITHER};
-    return {p.bm, !p.edge, p.ragged, true};
+    const int last = !reach || lie == LIE_NEITHER ? 0 : p.bm == 128 && p.bn == 128 ? 128 : 64;
+    if (!last || p.bm != p.bn || tiles * 2 < cus() || term.gr.rows / term.gr.groups < 16 || path_disabled("adapter_tiles")) return {0, false, p.ragged, lie != LIE_NEITHER, last};
+    return {p.bm, !p.edge, p.ragged, true, last};
 }
 
 // The shared product and the adapters' term
@@ -129,9 +130,23 @@ static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int d
     const TermTile t = term_tile(s, term, dtype);
     if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_tiles16_256_bf16(s, term, !t.whole) : launch_adapter_tiles16_256_f16(s, term, !t.whole);
     if (t.edge) return t.edge == 128 ? launch_adapter_tiles16_128(s, term, !t.whole, t.ragged, dtype) : launch_adapter_tiles16_64(s, term, t.ragged, dtype);
-    if (t.sums && adapter_expand16_takes(s, term)) return launch_adapter_expand16(s, term, t.ragged, dtype);
+    if (t.sums && adapter_expand16_takes(s, term)) {
+        bool taken;
+        const int rc = launch_adapter_expand16(s, term, t.ragged, dtype, &taken);
+        if (rc != 0 || taken) return rc;
+    }
+    if (t.last) return t.last == 128 ? launch_adapter_tiles16_128(s, term, true, t.ragged, dtype) : launch_adapter_tiles16_64(s, term, t.ragged, dtype);
     // what no kernel of the adapters' own takes (float32 and float64, the narrowest widths, operands without a unit stride): the product is rounded, and the sum again
-    if (rp_hip_gemm_strided_batched(s.C, s.A, s.B, s.bias, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate, dtype) != 0) return -1;
+    int rc;
+    bool refused;
+    {
+        const CallScratch memory(CallScratch::MOST);
+        const GemmWorkspaceLoan loan(memory.ptr, CallScratch::MOST);
+        rc = rp_hip_gemm_strided_batched(s.C, s.A, s.B, s.bias, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate, dtype);
+        refused = loan.refused;
+    }
+    if (refused) rc = grouped_rows(s, dtype);                 // (k would be split, and there is no memory for that: one group of all rows needs none)
+    if (rc != 0) return rc;
     return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, true, dtype);
 }
 

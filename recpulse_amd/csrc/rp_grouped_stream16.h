@@ -14,7 +14,7 @@
 // 4096 x 4096 by 32 strips of 128 columns 25.7 us, by 64 strips of 64 columns 19.2, by 128 strips of 32 columns, whose row pieces are
 // half a cache line, 18.1), so all CUs have to fetch.  Where the strips of 128 columns are too few for that, k is cut up among workgroups
 // too and a second launch adds their float32 sums in order (stream16_combine_kernel); where there is no memory for the sums that
-// another stream's call cannot touch (launch_grouped_stream16), strips are 64 columns instead.
+// another stream's call cannot touch (CallScratch), strips are 64 columns instead.
 #pragma once
 #include "rp_grouped.h"
 
@@ -53,8 +53,9 @@ struct StreamGrid {
     float* partials;               // [nsplit][rows][n], or null: the outputs themselves
 };
 
-template <typename T, int CPL, int RB>
-__device__ __forceinline__ void stream16_block(const GroupedArgs& g, const StreamGrid& sg, unsigned block) {
+// TERM: `term` is added to the sums before they are rounded
+template <typename T, int CPL, int RB, bool TERM = false>
+__device__ __forceinline__ void stream16_block(const GroupedArgs& g, const StreamGrid& sg, unsigned block, const AdapterTerm* term = nullptr) {
     constexpr int SLOTS = gs_slots<CPL, RB>(), COLS = 16 * CPL, PITCH = COLS + 4, ROWS = 16 * RB, S = 8 / CPL;
     constexpr bool STAGED = CPL < 8;
     constexpr int LOADS = CPL, PPR = COLS / 8, STAGE_PITCH = gs_stage_pitch<CPL>();      // loads of a round; 16-byte pieces of a strip's row
@@ -160,7 +161,21 @@ __device__ __forceinline__ void stream16_block(const GroupedArgs& g, const Strea
 #pragma unroll
             for (int v = 0; v < 4; v++) { s[v] += lo[v]; s[4 + v] += hi[v]; }
         }
-        if (sg.partials) {
+        if constexpr (TERM) {
+            int a = -1;
+            for (int t = 0; t < term->gr.groups; t++) a = row >= term->gr.begin(t) && row < term->gr.end(t) ? term->gr.weight(t) : a;
+            const float* h = term->h + (long long)row * term->rank;
+            const uint16_t* b = (const uint16_t*)term->b + a * term->b_ws + n0 + cv;
+#pragma unroll 4
+            for (int r = 0; r < (a < 0 ? 0 : term->rank); r++) {
+                const float hr = h[r];
+                T e[8];
+                __builtin_memcpy(e, b + r * term->b_rs, 16);
+#pragma unroll
+                for (int v = 0; v < 8; v++) s[v] += hr * widen(e[v]);
+            }
+        }
+        if (!TERM && sg.partials) {
             float* at = sg.partials + ((long long)split * g.gr.rows + row) * g.n + n0 + cv;
             *(f32x4_t*)at = f32x4_t{s[0], s[1], s[2], s[3]};
             *(f32x4_t*)(at + 4) = f32x4_t{s[4], s[5], s[6], s[7]};

@@ -179,7 +179,7 @@ static void* free_block(int dev, size_t size) {
 }
 
 // One block per device, kept until rp_hip_empty_cache.
-constexpr size_t NULL_STREAM_SCRATCH = CallScratch::MOST;
+constexpr size_t NULL_STREAM_SCRATCH = (size_t)16 << 20;
 constexpr int NULL_STREAM_DEVICES = 64;
 static std::mutex g_null_stream_mu;
 static void* g_null_stream_scratch[NULL_STREAM_DEVICES] = {};
@@ -196,19 +196,63 @@ NullStreamScratch::NullStreamScratch(size_t bytes) {
 }
 NullStreamScratch::~NullStreamScratch() { if (ptr) g_null_stream_mu.unlock(); }
 
-CallScratch::CallScratch(size_t bytes) : lease(bytes) {
-    ptr = lease.ptr;
-    if (ptr || !current_stream() || bytes > MOST) return;
+// A stream's block: of the largest size asked for so far, kept until rp_hip_empty_cache or the end of the stream.  (hipFree waits for the work that uses it.)
+struct StreamMemory {
+    std::mutex mu;
+    void* block = nullptr;
+    size_t size = 0;
+    int device = -1;
+    bool reserve(size_t bytes) {
+        if (bytes <= size) return true;
+        size_t want = CallScratch::MOST;
+        while (want < bytes) want *= 2;
+        // (another thread's recording in the runtime's default mode would be spoilt by an allocation, unless this thread is in the relaxed mode)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) { (void)hipGetLastError(); return false; }
+        release();
+        if (hipMalloc(&block, want) == hipSuccess) size = want;
+        else { (void)hipGetLastError(); block = nullptr; }
+        (void)hipThreadExchangeStreamCaptureMode(&mode);
+        return size != 0;
+    }
+    bool release() {
+        const bool ok = !block || hipFree(block) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
+        block = nullptr;
+        size = 0;
+        return ok;
+    }
+};
+static StreamMemory* null_stream_memory() { static auto* m = new StreamMemory[NULL_STREAM_DEVICES]; return m; }
+static std::mutex g_created_mu;
+static std::unordered_map<void*, StreamMemory*>& created_streams() { static auto* m = new std::unordered_map<void*, StreamMemory*>(); return *m; }
+
+CallScratch::CallScratch(size_t bytes, size_t most) {
+    int dev = 0;
+    if (bytes > most || hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= NULL_STREAM_DEVICES) { (void)hipGetLastError(); return; }
+    const hipStream_t stream = current_stream();
     if (stream_is_capturing()) {
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return; }
         ptr = block = free_block(dev, round_size(bytes));     // (nothing is allocated: that would end the recording)
-    } else if (pool().enabled) {
-        void* d = nullptr;
-        if (rp_hip_malloc(&d, bytes) == 0) rp_hip_free(d);
+        return;
+    }
+    void* warm = nullptr;                                     // (before the lease: an allocation that fails empties every cache)
+    if (stream && pool().enabled && rp_hip_malloc(&warm, bytes) == 0) rp_hip_free(warm);
+    if (!stream) memory = null_stream_memory() + dev;
+    else {
+        std::lock_guard<std::mutex> lk(g_created_mu);
+        auto it = created_streams().find((void*)stream);
+        if (it != created_streams().end() && it->second->device == dev) memory = it->second;
+    }
+    if (memory) {
+        memory->mu.lock();
+        if (memory->reserve(bytes)) ptr = memory->block;
+        else { memory->mu.unlock(); memory = nullptr; }
     }
 }
-CallScratch::~CallScratch() { if (block) rp_hip_free(block); }
+CallScratch::~CallScratch() {
+    if (memory) memory->mu.unlock();
+    if (block) rp_hip_free(block);
+}
 
 // Pinned host memory that a copy to the host goes through: a kernel writes it across the bus and the calling thread copies it on once the stream is
 // done.  us behind a chain of six kernels, hipMemcpyAsync to pageable memory and this: 10 KB 12.8 / 3.9, 64 KB 10.7 / 5.6, 128 KB 13.5 / 8.3, 255 KB 18.9 / 13.2; the limit is one of pinned
@@ -389,6 +433,17 @@ int rp_hip_empty_cache(void) {
     std::lock_guard<std::mutex> lk(g_null_stream_mu);
     for (void*& b : g_null_stream_scratch)              // (hipFree waits for the work that uses a block)
         if (b) { ok = check_hip(hipFree(b), "hipFree") && ok; b = nullptr; }
+    for (int d = 0; d < NULL_STREAM_DEVICES; d++) {
+        std::lock_guard<std::mutex> slk(null_stream_memory()[d].mu);
+        ok = null_stream_memory()[d].release() && ok;
+    }
+    {
+        std::lock_guard<std::mutex> clk(g_created_mu);
+        for (auto& it : created_streams()) {
+            std::lock_guard<std::mutex> slk(it.second->mu);
+            ok = it.second->release() && ok;
+        }
+    }
     std::lock_guard<std::mutex> rlk(rp::g_readback_mu);
     for (void* b : rp::readback_blocks()) ok = check_hip(hipHostFree(b), "hipHostFree") && ok;
     rp::readback_blocks().clear();
@@ -466,12 +521,26 @@ int rp_hip_stream_create(void** stream) {
     if (!stream) { set_error("rp_hip_stream_create: null argument"); return -1; }
     hipStream_t st;
     if (!check_hip(hipStreamCreateWithFlags(&st, hipStreamNonBlocking), "hipStreamCreate")) return -1;   // default priority
+    StreamMemory* memory = new StreamMemory;
+    if (hipGetDevice(&memory->device) != hipSuccess) { (void)hipGetLastError(); memory->device = -1; }
+    std::lock_guard<std::mutex> lk(g_created_mu);
+    created_streams()[(void*)st] = memory;
     *stream = (void*)st;
     return 0;
 }
 
 int rp_hip_stream_destroy(void* stream) {
     if (g_stream == (hipStream_t)stream) g_stream = nullptr;
+    StreamMemory* memory = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(g_created_mu);
+        auto it = created_streams().find(stream);
+        if (it != created_streams().end()) { memory = it->second; created_streams().erase(it); }
+    }
+    if (memory) {
+        memory->release();
+        delete memory;
+    }
     return check_hip(hipStreamDestroy((hipStream_t)stream), "hipStreamDestroy") ? 0 : -1;
 }
 
