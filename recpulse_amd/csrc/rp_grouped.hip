@@ -95,13 +95,16 @@ static bool backward_together(const GroupedArgs& x, const GroupedArgs& w, const 
 
 // An adapter's narrow product (C is h or u) and the gradients of its factors
 static int narrow_rows(const GroupedArgs& g, int dtype) { return is16(dtype) && adapter_shrink16_takes(g) ? launch_adapter_shrink16(g, dtype) : launch_narrow_rows(g, dtype); }
-static bool grads16_takes(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
-    return is16(dtype) && (da.C || db.C) && (!da.C || adapter_grad16_takes(da, LOW_B)) && (!db.C || adapter_grad16_takes(db, LOW_A));
+// Each gradient goes by its own operands, so that its bits do not depend on whether the other is asked for: those on MFMAs, the others with a null C in their place
+struct Grads16 { GroupedArgs da, db; };
+static Grads16 grads16_of(GroupedArgs da, GroupedArgs db, int dtype) {
+    if (!is16(dtype) || !adapter_grad16_takes(da, LOW_B)) da.C = nullptr;
+    if (!is16(dtype) || !adapter_grad16_takes(db, LOW_A)) db.C = nullptr;
+    return {da, db};
 }
-static int narrow_weights(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
-    if (grads16_takes(da, db, dtype)) return launch_adapter_grads16(da, db, dtype);
-    if (da.C && launch_narrow_weights(da, LOW_B, dtype) != 0) return -1;
-    return db.C ? launch_narrow_weights(db, LOW_A, dtype) : 0;
+static int other_grads(const GroupedArgs& da, const GroupedArgs& db, const Grads16& taken, int dtype) {
+    if (da.C && !taken.da.C && launch_narrow_weights(da, LOW_B, dtype) != 0) return -1;
+    return db.C && !taken.db.C ? launch_narrow_weights(db, LOW_A, dtype) : 0;
 }
 
 // Tiles on which the shared product of a layer with adapters takes their term in (edge 0: none); whole: nothing hangs over
@@ -225,16 +228,20 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
     if ((dx || da) && narrow_rows(GroupedArgs{u, dy, b, nullptr, scales, gr, n, rank, dy_rs, 1, (long long)rank * n, 1, n, 0, rank, 0}, dtype) != 0) return -1;
     const GroupedArgs ga{da, x, u, nullptr, nullptr, gr, k, rank, x_rs, x_cs, 0, rank, 1, (long long)k * rank, rank, accumulate_da ? ACCUMULATE : 0};
     const GroupedArgs gb{db, h, dy, nullptr, nullptr, gr, rank, n, rank, 1, 0, dy_rs, 1, (long long)rank * n, n, accumulate_db ? ACCUMULATE : 0};
+    const Grads16 g16 = grads16_of(ga, gb, dtype);
     if (dx) {
         const GroupedArgs shared{dx, dy, w, nullptr, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, n, k, dy_rs, 1, 0, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
         const AdapterTerm term{(const float*)u, a, gr, rank, (long long)k * rank, 1, rank};
         const TermTile t = term_tile(shared, term, dtype);
         // dx and the factors' gradients in one launch, unless workgroups that stay on their CU take dx
-        if (t.edge && t.edge < 256 && shared.b_rs == 1 && grads16_takes(ga, gb, dtype))
-            return dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_backward16_bf16(shared, term, ga, gb, t.edge, t.ragged) : launch_adapter_backward16_f16(shared, term, ga, gb, t.edge, t.ragged);
+        if (t.edge && t.edge < 256 && shared.b_rs == 1 && (g16.da.C || g16.db.C)) {
+            if ((dtype == RP_DTYPE_BFLOAT16 ? launch_adapter_backward16_bf16(shared, term, g16.da, g16.db, t.edge, t.ragged) : launch_adapter_backward16_f16(shared, term, g16.da, g16.db, t.edge, t.ragged)) != 0) return -1;
+            return other_grads(ga, gb, g16, dtype);
+        }
         if (shared_with_term(shared, term, dtype) != 0) return -1;
     }
-    return narrow_weights(ga, gb, dtype);
+    if ((g16.da.C || g16.db.C) && launch_adapter_grads16(g16.da, g16.db, dtype) != 0) return -1;
+    return other_grads(ga, gb, g16, dtype);
 }
 
 }  // extern "C"

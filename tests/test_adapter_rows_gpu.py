@@ -5,7 +5,7 @@ import pytest
 import oracle
 from recpulse_amd import capi
 from devhelp import BF16, F16, F32, Dev
-from test_grouped_gpu import HALF_STEP, TINY, UNIT, Adapters, call, ids_of, ptr, within
+from test_grouped_gpu import UNIT, Adapters, Grouped, call, ids_of, ptr, within
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,38 @@ def test_term_of_rows_of_every_magnitude(shape):
     once(oracle.to_f64(dx.numpy(), F16), *input_gradient(p), n + rank + 2, F16)
     for got, (want, size, _), width in zip((da, db), gradients(p), (n, k)):
         once(oracle.to_f64(got.numpy(), F16), want, size, rows + width + 2, F16)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("k, n, x_cs", [(136, 5, 1), (5, 136, 1), (72, 136, 2), (200, 72, 1)])
+def test_gradients_asked_for_alone(k, n, x_cs, dt):
+    """A factor's gradient has the same bits whichever others are asked for, also where the kernels take one of the two only (widths below a vector, x with a column stride)."""
+    rows, rank, adapters = 700, 12, 3
+    p = Adapters(dt, 7, adapters, rows, k, n, rank, behind=2)
+    p.forward()
+    wide = oracle.to_storage(np.zeros((rows, k * x_cs)), dt)
+    wide[:, ::x_cs] = p.s["x"]
+    x, d = Dev(wide, dt), p.d
+
+    def backward(which):
+        out = [Dev(oracle.to_storage(np.full(shape, 3.0), dt), dt) if use else None for use, shape in zip(which, ((rows, k), (adapters, k, rank), (adapters, rank, n)))]
+        u = Dev.empty((rows, rank), p.acc)
+        call("rp_hip_adapter_linear_backward", *[ptr(o) for o in out], u.ptr, d["g"].ptr, x.ptr, d["w"].ptr, d["a"].ptr, d["b"].ptr, p.h.ptr, *p.plan(),
+             n, k * x_cs, x_cs, *p.w_st, k, 0, 0, 0, dt)
+        return out
+
+    whole = backward((1, 1, 1))
+    p.check_backward(whole)
+    for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 1, 0), (1, 0, 1)):
+        for one, ref in zip(backward(which), whole):
+            assert one is None or np.array_equal(one.numpy(), ref.numpy()), which
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32], ids=ids_of)
+@pytest.mark.parametrize("groups, rows, k, n, transposed", [(6, 1999, 519, 1031, False), (3, 14949, 104, 427, False), (4, 130, 520, 384, True), (3, 700, 256, 5, False), (5, 900, 7, 264, False), (9, 40, 2048, 264, True)])
+def test_gradients_of_groups_asked_for_alone(groups, rows, k, n, transposed, dt):
+    p = Grouped(dt, groups, rows, k, n, transposed=transposed)
+    whole = [o.numpy() for o in p.backward()]
+    for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 1, 0), (1, 0, 1)):
+        for one, ref in zip(p.backward(which=which), whole):
+            assert one is None or np.array_equal(one.numpy(), ref), which
