@@ -391,7 +391,7 @@ int rp_hip_attention_backward(void* dQ, void* dK, void* dV, const void* Q, const
  * rounded.  Calls on several streams share nothing: partial sums lie in memory of the stream's own (the null stream's and that of streams from rp_hip_stream_create; kept until
  * rp_hip_empty_cache or the stream's end), or, in a graph being recorded, in a block of the pool that stays with the graph, where the pool has one free (a call on the same stream before
  * the recording sees to that).  With neither a call goes a way that needs none.  An output's bits do not depend on which of an entry's outputs are asked for, nor on the stream, except
- * where its comment says that the way without memory adds in another order. */
+ * where its comment says that the way without memory adds in another order.  Calls of more tiles than a launch takes are several launches. */
 
 /* Routing: each of `tokens` rows of logits (row stride logits_rs) is given its k largest entries, equal ones in the order of
  * their index; an entry of -inf is never taken (a padding token has nothing else), NaN is above every number.  Slot
@@ -445,7 +445,8 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  * Without memory for partial sums y (and dx below) are added up in another order where the layer is of few rows, of few tiles or of many short segments.  16-bit types multiply h (and u below) by b (a) as several values of 16 bits
  * that add up to it to 2^-17 of its value (float16: 2^-22 of it, and 2^-39 of the largest that it is summed with), whatever its magnitude; no row sees what another segment's
  * adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
- * (float32, float64, widths below 8 and operands without a unit stride: the shared product as a layer of its own, and the sum again). */
+ * (float32, float64, widths below 8, operands without a unit stride and, without memory for partial sums, more than 32768 segments: the shared product as a layer of its own, and
+ * the sum again). */
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
                                   int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);
 /* Its gradients, the shared projection being frozen (dw and the bias gradient are rp_hip_linear_backward's):

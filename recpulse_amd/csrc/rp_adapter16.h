@@ -103,7 +103,7 @@ template <typename T, int NC, int RT, bool ALONG_K, int PIECE, int SH_WAVES>
 __device__ __forceinline__ void adapter_shrink16_block(const GroupedArgs& g, int tile) {
     constexpr int PER_PASS = SH_WAVES / 4;      // waves; 16 x 16 tiles whose sums the threads add at a time, a value each
     extern __shared__ __attribute__((aligned(16))) unsigned char sh_lds[];
-    const RowTile rt = find_row_tile(g.gr, 16 * RT, tile);
+    const RowTile rt = find_row_tile_number(g.gr, 16 * RT, tile);
     if (rt.group < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int rank = g.n;

@@ -5,8 +5,8 @@
 namespace rp {
 
 template <typename T, int NC, int RT, bool ALONG_K, int PIECE>
-__global__ void __launch_bounds__((sh_waves<NC, PIECE>() * 64)) adapter_shrink16_kernel(GroupedArgs g) {
-    adapter_shrink16_block<T, NC, RT, ALONG_K, PIECE, sh_waves<NC, PIECE>()>(g, (int)blockIdx.x);
+__global__ void __launch_bounds__((sh_waves<NC, PIECE>() * 64)) adapter_shrink16_kernel(GroupedArgs g, int first) {
+    adapter_shrink16_block<T, NC, RT, ALONG_K, PIECE, sh_waves<NC, PIECE>()>(g, first + (int)blockIdx.x);
 }
 
 template <typename T, int NC, int RT, bool ALONG_K, int PIECE>
@@ -14,8 +14,10 @@ static int launch_shrink(const GroupedArgs& g) {
     constexpr int waves = sh_waves<NC, PIECE>(), lds = sh_lds_bytes<NC, RT, waves>(ALONG_K);
     auto kern = adapter_shrink16_kernel<T, NC, RT, ALONG_K, PIECE>;
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)max_row_tiles(g.gr.rows, g.gr.groups, 16 * RT)), dim3(waves * 64), lds, current_stream(), g);
-    return check_launch("adapter_shrink16_kernel") ? 0 : -1;
+    return in_launches(row_tile_numbers(g.gr.rows, g.gr.groups, 16 * RT), waves * 64, [&](unsigned blocks, long long first) -> int {
+        hipLaunchKernelGGL(kern, dim3(blocks), dim3(waves * 64), lds, current_stream(), g, (int)first);
+        return check_launch("adapter_shrink16_kernel") ? 0 : -1;
+    });
 }
 
 template <typename T, int NC, bool ALONG_K, int PIECE>
@@ -56,7 +58,7 @@ __global__ void __launch_bounds__(GS_THREADS) adapter_first16_kernel(GroupedArgs
 template <typename T, int CPL, int RB, int NC>
 static int launch_first(const GroupedArgs& shared, const StreamGrid& sg, const GroupedArgs& low) {
     constexpr int a = gs_lds_bytes<CPL>(), b = sh_lds_bytes<NC, 1, GS_WAVES>(false), lds = a > b ? a : b;
-    const long long low_blocks = (max_row_tiles(low.gr.rows, low.gr.groups, 16) + 7) / 8 * 8, blocks = low_blocks + stream16_blocks(shared, 16 * RB, CPL, sg.nsplit);
+    const long long low_blocks = (row_tile_numbers(low.gr.rows, low.gr.groups, 16) + 7) / 8 * 8, blocks = low_blocks + stream16_blocks(shared, 16 * RB, CPL, sg.nsplit);
     auto kern = adapter_first16_kernel<T, CPL, RB, NC>;
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), shared, sg, low, (int)low_blocks);
@@ -129,6 +131,20 @@ struct ExpandArgs {
 // Tile `id` of all rows: those before the first segment, each segment's whether it has an adapter or not, those behind the last
 __device__ __forceinline__ RowTile find_any_tile(const RowGroups& gr, int tile, int id) {
     const int lane = threadIdx.x & 63;
+    if (gr.groups > GROUPS_ADDED_UP) {                        // (numbered as find_row_tile_number's, the rows before the first segment as segment -1)
+        auto begin = [&](int i) { return i == 0 ? 0 : i <= gr.groups ? gr.begin(i - 1) : gr.end(gr.groups - 1); };
+        const int i = last_of(gr.groups + 2, [&](int i) { return begin(i) / tile + i <= id; });
+        auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        RowTile t;
+        t.group = uniform(i - 1);
+        t.weight = uniform(i > 0 && i <= gr.groups ? gr.weight(i - 1) : -1);
+        t.stop = uniform(i == 0 ? gr.begin(0) : i <= gr.groups ? gr.end(i - 1) : gr.rows);
+        t.first = uniform(begin(i) / tile + i);
+        t.begin = uniform(begin(i)) + (id - t.first) * tile;
+        t.tiles = 0;
+        t.end = t.begin + tile < t.stop ? t.begin + tile : t.stop;
+        return t;
+    }
     int before = 0;
     for (int g0 = 0; g0 < gr.groups + 2; g0 += 64) {
         const int g = g0 + lane - 1;
@@ -156,11 +172,12 @@ __device__ __forceinline__ RowTile find_any_tile(const RowGroups& gr, int tile, 
 }
 
 template <typename T, bool ALONG_RANK>
-__global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, AdapterTerm term) {
-    const RowTile rt = find_any_tile(term.gr, 16, (int)(blockIdx.x / ea.strips));
+__global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, AdapterTerm term, int first) {
+    const int id = first + (int)blockIdx.x;
+    const RowTile rt = find_any_tile(term.gr, 16, id / ea.strips);
     const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15, n = ea.n, m = rt.end - rt.begin;
     if (m <= 0) return;
-    const int col = (int)(blockIdx.x % ea.strips) * 128 + 8 * j, left = n - col, by = pulled(left);
+    const int col = id % ea.strips * 128 + 8 * j, left = n - col, by = pulled(left);
     const bool cut = col - 8 * j + 128 > n && n % 8;                      // (the strip's last vector ends with the row)
     f32x4_t acc[8];                                                       // rows 4q + v, column col + f
 #pragma unroll
@@ -280,20 +297,20 @@ bool adapter_expand16_takes(const GroupedArgs& shared, const AdapterTerm& term) 
 
 template <typename T>
 static int launch_expand(const ExpandArgs& ea, const AdapterTerm& term) {
-    const long long blocks = max_row_tiles(term.gr.rows, term.gr.groups + 2, 16) * ea.strips;
-    if (blocks > 0x3fffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), ea, term);
-    else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3((unsigned)blocks), dim3(64), 0, current_stream(), ea, term);
-    return check_launch("adapter_expand16_kernel") ? 0 : -1;
+    const long long segments = term.gr.groups + 2ll, tiles = term.gr.groups > GROUPS_ADDED_UP ? term.gr.rows / 16 + segments : max_row_tiles(term.gr.rows, segments, 16);
+    return in_launches(tiles * ea.strips, 64, [&](unsigned blocks, long long first) -> int {
+        if (term.b_cs == 1) hipLaunchKernelGGL((adapter_expand16_kernel<T, false>), dim3(blocks), dim3(64), 0, current_stream(), ea, term, (int)first);
+        else hipLaunchKernelGGL((adapter_expand16_kernel<T, true>), dim3(blocks), dim3(64), 0, current_stream(), ea, term, (int)first);
+        return check_launch("adapter_expand16_kernel") ? 0 : -1;
+    });
 }
 
 int launch_adapter_expand16(const GroupedArgs& s, const AdapterTerm& term, bool ragged, int dtype, bool* taken) {
     ragged = ragged || s.n % 8;                               // (the sums are stored in whole vectors otherwise)
-    constexpr size_t most = (size_t)1 << 30;
     const int rows = s.gr.rows, cus = device_cu_count() > 0 ? device_cu_count() : 256;
     const bool large = (long long)((rows + 127) / 128) * ((s.n + 127) / 128) * 2 >= cus;
     const int shares = large ? 1 : skinny16_sums_shares(rows, s.k, s.n);
-    const CallScratch memory((size_t)shares * rows * s.n * sizeof(float), most);
+    const CallScratch memory((size_t)shares * rows * s.n * sizeof(float), ~(size_t)0);
     float* sums = (float*)memory.ptr;
     *taken = sums != nullptr;
     if (!sums) return 0;

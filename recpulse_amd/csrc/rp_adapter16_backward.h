@@ -25,15 +25,17 @@ static int launch_adapter_backward16(const GroupedArgs& s, const AdapterTerm& te
     const GemmArgs g{s.C, s.A, s.B, nullptr, 1, s.gr.rows, s.k, s.n, 0, s.a_rs, s.a_cs, 0, s.b_rs, s.b_cs, 0, s.c_rs, 1, s.accumulate};
     auto kern = adapter_backward16_kernel<T, B, EDGE, NC>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
+    auto apart = [&]() -> int {
+        const int dtype = traits<T>::code;
+        if ((B == 128 ? launch_adapter_tiles16_128(s, term, true, EDGE == M16_RAGGED, dtype) : launch_adapter_tiles16_64(s, term, EDGE == M16_RAGGED, dtype)) != 0) return -1;
+        return launch_adapter_grads16_in_turn(ag, term.gr, dtype);
+    };
+    if ((long long)ag.a.blocks + ag.b.blocks + total > (1 << 23)) return apart();              // (more than a launch takes, or near it: the shares are few then)
     return with_joined_grads<T>(ag, term.gr, [&]() -> int {
         const int grad_blocks = (ag.a.blocks + ag.b.blocks + 7) / 8 * 8;        // (the tiles' schedule goes by workgroup modulo 8)
         hipLaunchKernelGGL(kern, dim3((unsigned)(grad_blocks + total)), dim3(256), smem, current_stream(), AdapterTileArgs{g, tiles_m, tiles_n, total, term}, ag, grad_blocks);
         return check_launch("adapter_backward16_kernel") ? 0 : -1;
-    }, [&]() -> int {
-        const int dtype = traits<T>::code;
-        if ((B == 128 ? launch_adapter_tiles16_128(s, term, true, EDGE == M16_RAGGED, dtype) : launch_adapter_tiles16_64(s, term, EDGE == M16_RAGGED, dtype)) != 0) return -1;
-        return launch_adapter_grads16_in_turn(ag, term.gr, dtype);
-    });
+    }, apart);
 }
 
 template <typename T, int B, int EDGE>
@@ -43,8 +45,7 @@ static int launch_adapter_backward16_rank(const GroupedArgs& s, const AdapterTer
 
 template <typename T>
 static int launch_adapter_backward16_tile(const GroupedArgs& s, const AdapterTerm& term, const GroupedArgs& da, const GroupedArgs& db, int tile, bool ragged) {
-    AdapterGrads ag;
-    if (!plan_grads(da, db, ag)) return -1;
+    AdapterGrads ag = plan_grads(da, db);
     if (tile == 128) return ragged ? launch_adapter_backward16_rank<T, 128, M16_RAGGED>(s, term, ag) : launch_adapter_backward16_rank<T, 128, M16_EDGE>(s, term, ag);
     return ragged ? launch_adapter_backward16_rank<T, 64, M16_RAGGED>(s, term, ag) : launch_adapter_backward16_rank<T, 64, M16_EDGE>(s, term, ag);
 }

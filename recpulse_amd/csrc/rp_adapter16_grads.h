@@ -188,8 +188,9 @@ __device__ __forceinline__ void adapter_grads16_block(const AdapterGrads& ag, co
 }
 
 static inline int grads_rank_tiles(int rank) { return rank <= 16 ? 1 : 2; }
-// Those gradients whose C is not null; false: more workgroups than a launch takes.  How many share an adapter's rows goes by the sizes alone, not by what is asked for.
-static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, AdapterGrads& ag) {
+// Those gradients whose C is not null.  How many share an adapter's rows goes by the sizes alone, not by what is asked for.
+static inline AdapterGrads plan_grads(const GroupedArgs& da, const GroupedArgs& db) {
+    AdapterGrads ag;
     ag.a = AdapterGrad{da.C, nullptr, da.A, (const float*)da.B, da.k, da.accumulate, 0, 0, da.a_rs, da.c_ws, da.c_rs};
     ag.b = AdapterGrad{db.C, nullptr, db.B, (const float*)db.A, db.n, db.accumulate, 0, 0, db.b_rs, db.c_ws, db.c_rs};
     ag.rank = da.n;
@@ -204,12 +205,8 @@ static inline bool plan_grads(const GroupedArgs& da, const GroupedArgs& db, Adap
     long long shares = turns / 8 < 2 * cus / blocks ? turns / 8 : 2 * cus / blocks;
     shares = shares < room ? shares : room;
     ag.shares = shares > 1 ? (int)shares : 1;
-    for (AdapterGrad* g : {&ag.a, &ag.b}) {
-        const long long own = g->out ? (long long)g->strips * ag.rank_blocks * da.gr.weights : 0;
-        if (own * ag.shares > 0x5fffff) { set_error("adapter gradients: %lld tiles are more than a launch takes", own); return false; }
-        g->blocks = (int)own;
-    }
-    return true;
+    for (AdapterGrad* g : {&ag.a, &ag.b}) g->blocks = g->out ? g->strips * ag.rank_blocks * da.gr.weights : 0;
+    return ag;
 }
 
 // out = the shares' sums in order, rounded once; adapters without rows have been seen to

@@ -4,14 +4,16 @@
 namespace rp {
 
 template <typename T, int NC, bool IN_TURN>
-__global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr) { adapter_grads16_block<T, NC, IN_TURN>(ag, gr, (int)blockIdx.x); }
+__global__ void __launch_bounds__(AG_THREADS) adapter_grads16_kernel(AdapterGrads ag, RowGroups gr, int first) { adapter_grads16_block<T, NC, IN_TURN>(ag, gr, first + (int)blockIdx.x); }
 
 template <typename T, int NC, bool IN_TURN>
 static int launch_grads(const AdapterGrads& ag, const RowGroups& gr) {
     constexpr int lds = AG_LDS + (IN_TURN ? NC * 16 * AG_COLS * 4 : 0);
     static_assert(lds <= 64 * 1024, "no more than every launch may have");
-    hipLaunchKernelGGL((adapter_grads16_kernel<T, NC, IN_TURN>), dim3((unsigned)(ag.a.blocks + ag.b.blocks)), dim3(AG_THREADS), lds, current_stream(), ag, gr);
-    return check_launch("adapter_grads16_kernel") ? 0 : -1;
+    return in_launches((long long)ag.a.blocks + ag.b.blocks, AG_THREADS, [&](unsigned blocks, long long first) -> int {
+        hipLaunchKernelGGL((adapter_grads16_kernel<T, NC, IN_TURN>), dim3(blocks), dim3(AG_THREADS), lds, current_stream(), ag, gr, (int)first);
+        return check_launch("adapter_grads16_kernel") ? 0 : -1;
+    });
 }
 
 template <typename T, bool IN_TURN>
@@ -34,8 +36,7 @@ bool adapter_grad16_takes(const GroupedArgs& g, GroupedLow low) {
 }
 
 int launch_adapter_grads16(const GroupedArgs& da, const GroupedArgs& db, int dtype) {
-    AdapterGrads ag;
-    if (!plan_grads(da, db, ag)) return -1;
+    AdapterGrads ag = plan_grads(da, db);
     return dtype == RP_DTYPE_BFLOAT16 ? launch_joined<bf16_t>(ag, da.gr, dtype) : launch_joined<f16_t>(ag, da.gr, dtype);
 }
 

@@ -16,13 +16,14 @@ template <typename A> constexpr int nr_lanes() { return sizeof(A) == 8 ? 32 : 64
 constexpr int NW_WAVES = 16;                                     // waves that share the rows
 
 template <typename T>
-__global__ void __launch_bounds__(NR_COLS * nr_lanes<typename traits<T>::acc>()) narrow_rows_kernel(GroupedArgs g, int col_blocks) {
+__global__ void __launch_bounds__(NR_COLS * nr_lanes<typename traits<T>::acc>()) narrow_rows_kernel(GroupedArgs g, int col_blocks, long long first) {
     using A = typename traits<T>::acc;
     constexpr int NR_LANES = nr_lanes<A>();
     __shared__ A sums[NR_LANES][NR_ROWS][NR_COLS + 1];
-    const RowTile rt = find_row_tile(g.gr, NR_ROWS, (int)(blockIdx.x / col_blocks));
+    const long long id = first + blockIdx.x;
+    const RowTile rt = find_row_tile_number(g.gr, NR_ROWS, (int)(id / col_blocks));
     if (rt.group < 0) return;
-    const int c = threadIdx.x % NR_COLS, p = threadIdx.x / NR_COLS, col = (int)(blockIdx.x % col_blocks) * NR_COLS + c, last = rt.end - rt.begin - 1;
+    const int c = threadIdx.x % NR_COLS, p = threadIdx.x / NR_COLS, col = (int)(id % col_blocks) * NR_COLS + c, last = rt.end - rt.begin - 1;
     const T* x = (const T*)g.A + rt.begin * g.a_rs;
     const T* f = (const T*)g.B + rt.weight * g.b_ws + (col < g.n ? col : g.n - 1) * g.b_cs;
     A acc[NR_ROWS];
@@ -47,11 +48,12 @@ __global__ void __launch_bounds__(NR_COLS * nr_lanes<typename traits<T>::acc>())
 
 // TRANSPOSED: dA; else dB
 template <typename T, bool TRANSPOSED>
-__global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedArgs g, int strips, int rank_blocks) {
+__global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedArgs g, int strips, int rank_blocks, long long first) {
     using A = typename traits<T>::acc;
     extern __shared__ __attribute__((aligned(16))) unsigned char nw_lds[];
     A (*sums)[NR_COLS][65] = (A (*)[NR_COLS][65])nw_lds;         // [NW_WAVES]
-    const int strip = (int)(blockIdx.x % strips), rb = (int)(blockIdx.x / strips % rank_blocks), w = (int)(blockIdx.x / strips / rank_blocks);
+    const long long block = first + blockIdx.x;
+    const int strip = (int)(block % strips), rb = (int)(block / strips % rank_blocks), w = (int)(block / strips / rank_blocks);
     const int width = TRANSPOSED ? g.k : g.n, rank = TRANSPOSED ? g.n : g.k;
     const T* s = (const T*)(TRANSPOSED ? g.A : g.B);
     const A* low = (const A*)(TRANSPOSED ? g.B : g.A);
@@ -95,23 +97,28 @@ __global__ void __launch_bounds__(NW_WAVES * 64) narrow_weights_kernel(GroupedAr
 
 int launch_narrow_rows(const GroupedArgs& g, int dtype) {
     const int col_blocks = (g.n + NR_COLS - 1) / NR_COLS;
-    const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, NR_ROWS) * col_blocks;
-    if (blocks > 0x7fffffffll) { set_error("adapters: %lld tiles are more than a launch takes", blocks); return -1; }
-    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(narrow_rows_kernel<T>, dim3((unsigned)blocks), dim3(NR_COLS * nr_lanes<typename traits<T>::acc>()), 0, current_stream(), g, col_blocks));
-    return check_launch("narrow_rows_kernel") ? 0 : -1;
+    const long long all = row_tile_numbers(g.gr.rows, g.gr.groups, NR_ROWS) * col_blocks;
+    RP_DISPATCH_DTYPE(dtype, {
+        constexpr int threads = NR_COLS * nr_lanes<typename traits<T>::acc>();
+        return in_launches(all, threads, [&](unsigned blocks, long long first) -> int {
+            hipLaunchKernelGGL(narrow_rows_kernel<T>, dim3(blocks), dim3(threads), 0, current_stream(), g, col_blocks, first);
+            return check_launch("narrow_rows_kernel") ? 0 : -1;
+        });
+    });
+    return 0;
 }
 
 int launch_narrow_weights(const GroupedArgs& g, GroupedLow low, int dtype) {
     const bool transposed = low == LOW_B;
     const int width = transposed ? g.k : g.n, rank = transposed ? g.n : g.k, strips = (width + 63) / 64, rank_blocks = (rank + NR_COLS - 1) / NR_COLS;
-    const long long blocks = (long long)strips * rank_blocks * g.gr.weights;
-    if (blocks > 0x7fffffffll) { set_error("adapter gradient: %lld tiles are more than a launch takes", blocks); return -1; }
     RP_DISPATCH_DTYPE(dtype, {
         constexpr int lds = NW_WAVES * NR_COLS * 65 * (int)sizeof(typename traits<T>::acc);
         auto launch = [&](auto kern) {
             if (!check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(NW_WAVES * 64), lds, current_stream(), g, strips, rank_blocks);
-            return check_launch("narrow_weights_kernel") ? 0 : -1;
+            return in_launches((long long)strips * rank_blocks * g.gr.weights, NW_WAVES * 64, [&](unsigned blocks, long long first) -> int {
+                hipLaunchKernelGGL(kern, dim3(blocks), dim3(NW_WAVES * 64), lds, current_stream(), g, strips, rank_blocks, first);
+                return check_launch("narrow_weights_kernel") ? 0 : -1;
+            });
         };
         return transposed ? launch(narrow_weights_kernel<T, true>) : launch(narrow_weights_kernel<T, false>);
     });

@@ -34,7 +34,7 @@ static bool prefers256(long long tiles256, long long tiles128, long long k) {
 struct Tile16 { int edge; bool ragged; };
 
 static Tile16 rows_tile16(const GroupedArgs& g, int dtype) {
-    if (!is16(dtype) || g.a_cs != 1 || (g.b_cs != 1 && g.b_rs != 1) || path_disabled("mfma")) return {0, false};
+    if (!is16(dtype) || g.a_cs != 1 || (g.b_cs != 1 && g.b_rs != 1) || g.gr.groups > ROW_TILES_GROUPS || path_disabled("mfma")) return {0, false};
     const bool b_mc = g.b_cs == 1;
     const Lie lie = worse(lies(g.A, g.a_rs, 0, g.k, 2), b_mc ? lies(g.B, g.b_rs, g.b_ws, g.n, 2) : lies(g.B, g.b_cs, g.b_ws, g.k, 2));
     if (lie == LIE_NEITHER) return {0, false};
@@ -123,7 +123,7 @@ static TermTile term_tile(const GroupedArgs& s, const AdapterTerm& term, int dty
     const bool reach = (long long)s.gr.rows * term.rank < (1 << 29) && ((term.rank - 1) * term.b_rs + (s.n - 1) * term.b_cs) < (1 << 30);
     // from about a tile for every other CU on, and while a tile's rows are few segments: each costs it 2 us (bf16, 4096 rows, us in the tiles and apart: 400 segments, 1024 -> 4096,
     // rank 8 111 / 89, 4096 -> 4096, rank 32 189 / 196; 7 segments 127 / 178)
-    const int last = !reach || lie == LIE_NEITHER ? 0 : p.bm == 128 && p.bn == 128 ? 128 : 64;
+    const int last = !reach || lie == LIE_NEITHER || term.gr.groups > ROW_TILES_GROUPS ? 0 : p.bm == 128 && p.bn == 128 ? 128 : 64;
     if (!last || p.bm != p.bn || tiles * 2 < cus() || term.gr.rows / term.gr.groups < 16 || path_disabled("adapter_tiles")) return {0, false, p.ragged, lie != LIE_NEITHER, last};
     return {p.bm, !p.edge, p.ragged, true, last};
 }

@@ -46,12 +46,13 @@ __device__ __forceinline__ void generic_tile(A acc[4][4], A (*as)[GG_T + 4], A (
 }
 
 template <typename TA, typename T>
-__global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g, int tiles_n) {
+__global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g, int tiles_n, long long first) {
     using A = typename traits<T>::acc;
     __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
-    const RowTile rt = find_row_tile(g.gr, GG_T, (int)(blockIdx.x / tiles_n));
+    const long long id = first + blockIdx.x;
+    const RowTile rt = find_row_tile_number(g.gr, GG_T, (int)(id / tiles_n));
     if (rt.group < 0) return;
-    const int n0 = (int)(blockIdx.x % tiles_n) * GG_T, m = rt.end - rt.begin, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
+    const int n0 = (int)(id % tiles_n) * GG_T, m = rt.end - rt.begin, n = g.n - n0 < GG_T ? g.n - n0 : GG_T;
     const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
     A acc[4][4] = {};
     generic_tile<TA, T, A>(acc, as, bs, (const TA*)g.A + rt.begin * g.a_rs, (const T*)g.B + rt.weight * g.b_ws + n0 * g.b_cs, m, n, g.k, g.a_rs, g.a_cs, g.b_rs, g.b_cs);
@@ -73,10 +74,11 @@ __global__ void __launch_bounds__(256) grouped_rows_generic_kernel(GroupedArgs g
 
 // A tile of C_w is a sum over the rows of group w
 template <typename T>
-__global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArgs g, int tiles_k, int tiles_n) {
+__global__ void __launch_bounds__(256) grouped_weights_generic_kernel(GroupedArgs g, int tiles_k, int tiles_n, long long first) {
     using A = typename traits<T>::acc;
     __shared__ A as[GG_K][GG_T + 4], bs[GG_K][GG_T + 4];
-    const int tn = (int)(blockIdx.x % tiles_n), tk = (int)(blockIdx.x / tiles_n % tiles_k), w = (int)(blockIdx.x / tiles_n / tiles_k);
+    const long long id = first + blockIdx.x;
+    const int tn = (int)(id % tiles_n), tk = (int)(id / tiles_n % tiles_k), w = (int)(id / tiles_n / tiles_k);
     const int m0 = tk * GG_T, n0 = tn * GG_T, m = g.k - m0 < GG_T ? g.k - m0 : GG_T, n = g.n - n0 < GG_T ? g.n - n0 : GG_T, b = g.gr.begin(w), e = g.gr.end(w);
     const int tr = (threadIdx.x >> 4) * 4, tc = (threadIdx.x & 15) * 4;
     A acc[4][4] = {};
@@ -97,39 +99,32 @@ template <typename T>
 __global__ void __launch_bounds__(1024) grouped_sums_kernel(GroupedSums s, long long blocks) {
     __shared__ typename traits<T>::acc parts[16 * 64];
     for (long long id = blockIdx.x; id < blocks; id += gridDim.x) {
-        grouped_sums_block<T, 16>(s, (int)id, parts);
+        grouped_sums_block<T, 16>(s, id, parts);
         __syncthreads();
     }
 }
 
-static bool grid_ok(long long blocks, const char* what) {
-    if (blocks <= 0x7fffffffll) return true;
-    set_error("%s: %lld tiles are more than a launch takes", what, blocks);
-    return false;
-}
-
 int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype) {
     const int tiles_n = (g.n + GG_T - 1) / GG_T;
-    const long long blocks = max_row_tiles(g.gr.rows, g.gr.groups, GG_T) * tiles_n;
-    if (!grid_ok(blocks, "grouped product")) return -1;
-    RP_DISPATCH_DTYPE(dtype, {
-        if (low) hipLaunchKernelGGL((grouped_rows_generic_kernel<typename traits<T>::acc, T>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
-        else hipLaunchKernelGGL((grouped_rows_generic_kernel<T, T>), dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_n);
+    return in_launches(row_tile_numbers(g.gr.rows, g.gr.groups, GG_T) * tiles_n, 256, [&](unsigned blocks, long long first) -> int {
+        RP_DISPATCH_DTYPE(dtype, {
+            if (low) hipLaunchKernelGGL((grouped_rows_generic_kernel<typename traits<T>::acc, T>), dim3(blocks), dim3(256), 0, current_stream(), g, tiles_n, first);
+            else hipLaunchKernelGGL((grouped_rows_generic_kernel<T, T>), dim3(blocks), dim3(256), 0, current_stream(), g, tiles_n, first);
+        });
+        return check_launch("grouped_rows_generic_kernel") ? 0 : -1;
     });
-    return check_launch("grouped_rows_generic_kernel") ? 0 : -1;
 }
 
 int launch_grouped_weights_generic(const GroupedArgs& g, int dtype) {
     const int tiles_k = (g.k + GG_T - 1) / GG_T, tiles_n = (g.n + GG_T - 1) / GG_T;
-    const long long blocks = (long long)g.gr.weights * tiles_k * tiles_n;
-    if (!grid_ok(blocks, "grouped weight gradient")) return -1;
-    RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_weights_generic_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, current_stream(), g, tiles_k, tiles_n));
-    return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
+    return in_launches((long long)g.gr.weights * tiles_k * tiles_n, 256, [&](unsigned blocks, long long first) -> int {
+        RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_weights_generic_kernel<T>, dim3(blocks), dim3(256), 0, current_stream(), g, tiles_k, tiles_n, first));
+        return check_launch("grouped_weights_generic_kernel") ? 0 : -1;
+    });
 }
 
 int launch_grouped_sums(const GroupedSums& s, int dtype) {
     const long long blocks = sum_blocks(s);
-    if (!grid_ok(blocks, "grouped bias gradient")) return -1;
     RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(grouped_sums_kernel<T>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(1024), 0, current_stream(), s, blocks));
     return check_launch("grouped_sums_kernel") ? 0 : -1;
 }

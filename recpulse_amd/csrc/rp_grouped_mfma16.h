@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) group
 // A workgroup a tile, except for the 256 x 256 tile: one resident workgroup a CU, as for one product.
 template <int BM, int BN>
 static unsigned grouped16_blocks(long long tiles) {
-    const long long most = BM == 256 && BN == 256 && device_cu_count() >= 8 ? device_cu_count() / 8 * 8 : 1 << 24;
+    const long long most = BM == 256 && BN == 256 && device_cu_count() >= 8 ? device_cu_count() / 8 * 8 : (1 << 24) - 8;      // (fewer than 2^32 threads)
     tiles = (tiles + 7) / 8 * 8;
     return (unsigned)(tiles < most ? tiles : most);
 }

@@ -55,15 +55,15 @@ struct StreamGrid {
 
 // TERM: `term` is added to the sums before they are rounded
 template <typename T, int CPL, int RB, bool TERM = false>
-__device__ __forceinline__ void stream16_block(const GroupedArgs& g, const StreamGrid& sg, unsigned block, const AdapterTerm* term = nullptr) {
+__device__ __forceinline__ void stream16_block(const GroupedArgs& g, const StreamGrid& sg, long long block, const AdapterTerm* term = nullptr) {
     constexpr int SLOTS = gs_slots<CPL, RB>(), COLS = 16 * CPL, PITCH = COLS + 4, ROWS = 16 * RB, S = 8 / CPL;
     constexpr bool STAGED = CPL < 8;
     constexpr int LOADS = CPL, PPR = COLS / 8, STAGE_PITCH = gs_stage_pitch<CPL>();      // loads of a round; 16-byte pieces of a strip's row
     extern __shared__ __attribute__((aligned(16))) float gs_sums[];       // [GS_WAVES][16][PITCH]
-    const unsigned slot = block >> 3, within = slot % (S * sg.nsplit), piece = slot / (S * sg.nsplit) * 8 + (block & 7);
+    const unsigned slot = (unsigned)(block >> 3), within = slot % (S * sg.nsplit), piece = slot / (S * sg.nsplit) * 8 + (unsigned)(block & 7);
     const int split = (int)(within / S), n0 = ((int)(piece % sg.pieces) * S + (int)(within % S)) * COLS;
     if (n0 >= g.n) return;
-    const RowTile rt = find_row_tile(g.gr, ROWS, (int)(piece / sg.pieces));
+    const RowTile rt = find_row_tile_number(g.gr, ROWS, (int)(piece / sg.pieces));
     if (rt.group < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, j = lane & 15;
     const int m = rt.end - rt.begin;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void stream16_block(const GroupedArgs& g, const Strea
 
 // Grid of the blocks above
 static inline long long stream16_blocks(const GroupedArgs& g, int rows_of_tile, int cpl, int nsplit) {
-    return (max_row_tiles(g.gr.rows, g.gr.groups, rows_of_tile) * ((g.n + 127) / 128) + 7) / 8 * 8 * (8 / cpl) * nsplit;
+    return (row_tile_numbers(g.gr.rows, g.gr.groups, rows_of_tile) * ((g.n + 127) / 128) + 7) / 8 * 8 * (8 / cpl) * nsplit;
 }
 
 // 16-row blocks of a row tile: enough for most groups of a draw around the mean

@@ -4,7 +4,7 @@
 namespace rp {
 
 template <typename T, int CPL, int RB>
-__global__ void __launch_bounds__(GS_THREADS) grouped_stream16_kernel(GroupedArgs g, StreamGrid sg) { stream16_block<T, CPL, RB>(g, sg, blockIdx.x); }
+__global__ void __launch_bounds__(GS_THREADS) grouped_stream16_kernel(GroupedArgs g, StreamGrid sg, long long first) { stream16_block<T, CPL, RB>(g, sg, first + blockIdx.x); }
 
 // y[row] = the shares' sums in order + bias + what the row's adapter adds, rounded once; rows of no group are left alone.  A workgroup does 32
 // vectors of 8 columns of one row: eight threads share a vector's shares of k and its rank, and their sums are added in order.  The loads
@@ -77,13 +77,13 @@ int launch_stream16_combine(const GroupedArgs& g, const StreamGrid& sg, const Ad
 
 template <typename T, int CPL, int RB>
 static int launch_stream(const GroupedArgs& g, StreamGrid sg) {
-    const long long blocks = stream16_blocks(g, 16 * RB, CPL, sg.nsplit);
-    if (blocks > 0x7fffffffll) { set_error("grouped product: %lld tiles are more than a launch takes", blocks); return -1; }
     constexpr int lds = gs_lds_bytes<CPL>();
     auto kern = grouped_stream16_kernel<T, CPL, RB>;
     if (lds > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return -1;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GS_THREADS), lds, current_stream(), g, sg);
-    return check_launch("grouped_stream16_kernel") ? 0 : -1;
+    return in_launches(stream16_blocks(g, 16 * RB, CPL, sg.nsplit), GS_THREADS, [&](unsigned blocks, long long first) -> int {
+        hipLaunchKernelGGL(kern, dim3(blocks), dim3(GS_THREADS), lds, current_stream(), g, sg, first);
+        return check_launch("grouped_stream16_kernel") ? 0 : -1;
+    });
 }
 
 template <typename T, int CPL>

@@ -18,11 +18,11 @@ static inline long long sum_blocks(const GroupedSums& s) { return (long long)s.g
 // way at a time (bf16, 14949 rows of 3 groups, 427 columns, in the launch of all gradients, a column a lane and a vector: 163 us and 77).  A vector that straddles the end of its row is loaded
 // early, where it ends with the row, and shifted into place.  parts: room for 16 x 64 sums.
 template <typename T, int WAVES>
-__device__ __forceinline__ void grouped_sums_block(const GroupedSums& s, int id, typename traits<T>::acc* parts) {
+__device__ __forceinline__ void grouped_sums_block(const GroupedSums& s, long long id, typename traits<T>::acc* parts) {
     using A = typename traits<T>::acc;
     typedef unsigned int vector_t __attribute__((ext_vector_type(4), aligned(2)));        // (at any element)
     constexpr int PER = 16 / WAVES, V = 16 / (int)sizeof(T), LANES = 64 / V;
-    const int strips = (s.cols + 63) / 64, w = id / strips, c0 = (id - w * strips) * 64, lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int strips = (s.cols + 63) / 64, w = (int)(id / strips), c0 = (int)(id % strips) * 64, lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = c0 + lane % LANES * V, left = s.cols - c, by = left > 0 && left < V && s.cols >= V ? V - left : 0;
     const bool cut = c0 + 64 > s.cols && s.cols % V;
     A sum[PER][V] = {};

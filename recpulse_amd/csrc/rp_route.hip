@@ -377,9 +377,10 @@ __global__ void __launch_bounds__(ROUTE_ONE_THREADS) route_one_kernel(weight_t<T
 //   dl_e = p_e (g_e - sum over j of w_j g_j),   g_e = 0 where e was not taken; with "normalize" p_e = w_j where taken and 0 elsewhere.
 template <typename T, int LANES, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(T* grad, const weight_t<T>* grad_weights, const weight_t<T>* weights, const int* taken, const T* logits, long long rs,
-                                                             int tokens, int experts, int k, int normalize) {
+                                                             int tokens, int experts, int k, int normalize, long long first) {
     using A = typename traits<T>::acc;
-    const int l = threadIdx.x % LANES, t = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int l = threadIdx.x % LANES;
+    const long long t = (first + blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     if (t >= tokens) return;                                   // (all lanes of a token)
     const int id_l = l < k ? taken[(size_t)t * k + l] : -1;
     const A w_l = id_l >= 0 ? weights[(size_t)t * k + l] : (A)0, g_l = id_l >= 0 ? grad_weights[(size_t)t * k + l] : (A)0;
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(T* grad, const weig
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int e = v * LANES + l;
-            x[v] = e < experts ? widen(logits[(long long)t * rs + e]) : (A)-INFINITY;
+            x[v] = e < experts ? widen(logits[t * rs + e]) : (A)-INFINITY;
             top = x[v] > top ? x[v] : top;
         }
         top = reduce_lanes<LANES>(top, [](A a, A b) { return a > b ? a : b; });
@@ -515,9 +516,11 @@ template <typename T>
 static int launch_route_backward(void* grad, const void* grad_weights, const void* weights, const int* taken, const void* logits, long long rs, int tokens, int experts, int k, int normalize) {
     return pick_route_shape(experts, [&](auto lanes_c, auto v_c) -> int {
         constexpr int LANES = decltype(lanes_c)::value, V = decltype(v_c)::value, PER = 256 / LANES;
-        hipLaunchKernelGGL((route_backward_kernel<T, LANES, V>), dim3((tokens + PER - 1) / PER), dim3(256), 0, current_stream(), (T*)grad, (const weight_t<T>*)grad_weights,
-                           (const weight_t<T>*)weights, taken, (const T*)logits, rs, tokens, experts, k, normalize);
-        return check_launch("route_backward_kernel") ? 0 : -1;
+        return in_launches(((long long)tokens + PER - 1) / PER, 256, [&](unsigned blocks, long long first) -> int {
+            hipLaunchKernelGGL((route_backward_kernel<T, LANES, V>), dim3(blocks), dim3(256), 0, current_stream(), (T*)grad, (const weight_t<T>*)grad_weights,
+                               (const weight_t<T>*)weights, taken, (const T*)logits, rs, tokens, experts, k, normalize, first);
+            return check_launch("route_backward_kernel") ? 0 : -1;
+        });
     });
 }
 

@@ -86,6 +86,49 @@ __device__ __forceinline__ RowTile find_row_tile(const RowGroups& gr, int tile, 
     return RowTile{-1, -1, 0, 0, 0, 0, 0};
 }
 
+// Of more groups than this a tile is looked for by bisection, 64 ways at a time, instead of adding up all groups' tiles before it: a trip to memory for each power of 64 and not for
+// each 64 groups.  The tiles are not numbered one after the other then: tile t of group g is number begin(g) / tile + g + t, which leaves out at most one number a group.
+constexpr int GROUPS_ADDED_UP = 1024;
+// Kernels whose workgroups look through all groups (RowTiles, the adapters' tiles) take no more than this: each 64 cost a workgroup a trip to memory
+constexpr int ROW_TILES_GROUPS = 32768;
+// The last of `count` numbers g for which below(g), which does not grow again, is true; -1: none
+template <typename F> __device__ __forceinline__ int last_of(int count, F below) {
+    const int lane = threadIdx.x & 63;
+    int from = 0;
+    while (count > 0) {
+        const int step = (count + 63) / 64, at = lane * step;
+        const unsigned long long yes = __builtin_amdgcn_ballot_w64(at < count && below(from + at));
+        if (!yes) return from ? from : -1;                    // (from itself is one of them then)
+        const int l = 63 - __builtin_clzll(yes);
+        if (step == 1) return from + l;
+        from += l * step;
+        count = count - l * step < step ? count - l * step : step;
+    }
+    return -1;
+}
+// find_row_tile for a kernel of a workgroup a tile, with row_tile_numbers() of them
+static inline long long row_tile_numbers(long long rows, long long groups, int tile) { return groups > GROUPS_ADDED_UP ? rows / tile + groups : max_row_tiles(rows, groups, tile); }
+__device__ __forceinline__ RowTile find_row_tile_number(const RowGroups& gr, int tile, int id) {
+    if (gr.groups <= GROUPS_ADDED_UP) return find_row_tile(gr, tile, id);
+    const int g = last_of(gr.groups, [&](int i) { return gr.begin(i) / tile + i <= id; });
+    if (g < 0) return RowTile{-1, -1, 0, 0, 0, 0, 0};
+    const int b = gr.begin(g), e = gr.end(g), w = gr.weight(g), t = id - (b / tile + g);
+    if (w < 0 || t >= (e - b + tile - 1) / tile) return RowTile{-1, -1, 0, 0, 0, 0, 0};
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int begin = uniform(b + t * tile), stop = uniform(e);
+    return RowTile{uniform(g), uniform(w), begin, begin + tile < stop ? begin + tile : stop, stop, uniform(id - t), uniform((e - b + tile - 1) / tile)};
+}
+
+// A launch has fewer than 2^32 threads: launch(workgroups, number of the first) as often as it takes; not 0: what one of them returned
+template <typename F> static inline int in_launches(long long blocks, int threads, F launch) {
+    const long long most = ((1ll << 32) / threads - 1) / 8 * 8;
+    for (long long first = 0; first < blocks; first += most) {
+        const int rc = launch((unsigned)(blocks - first < most ? blocks - first : most), first);
+        if (rc != 0) return rc;
+    }
+    return 0;
+}
+
 // The same for a workgroup that looks up many tiles: up to 64 groups are read and added up once and kept a lane each.
 struct RowTiles {
     RowGroups gr;

@@ -205,7 +205,8 @@ struct StreamMemory {
     bool reserve(size_t bytes) {
         if (bytes <= size) return true;
         size_t want = CallScratch::MOST;
-        while (want < bytes) want *= 2;
+        while (want < bytes && want < ((size_t)1 << 30)) want *= 2;
+        if (want < bytes) want = round_size(bytes);
         // (another thread's recording in the runtime's default mode would be spoilt by an allocation, unless this thread is in the relaxed mode)
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
         if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) { (void)hipGetLastError(); return false; }
