@@ -178,3 +178,46 @@ def test_gradients_of_groups_asked_for_alone(groups, rows, k, n, transposed, dt)
     for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 1, 0), (1, 0, 1)):
         for one, ref in zip(p.backward(which=which), whole):
             assert one is None or np.array_equal(one.numpy(), ref), which
+
+
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ids_of)
+@pytest.mark.parametrize("shape", SMALL + [(5, 3, 2048, 264, 2056, 24)] + LARGE[:1], ids=lambda s: "x".join(map(str, s)))
+def test_rounded_once(shape, dt):
+    """y and dx: the shared product, the bias and the term together.  (dx added to what is there: that sum is a rounding of its own.)"""
+    p = Adapters(dt, *shape, behind=2)
+    _, _, rows, k, n, rank = shape
+    p.forward()
+    once(oracle.to_f64(p.y.numpy(), dt), *layer(p), k + rank + 2, dt)
+    want, size = input_gradient(p)
+    once(oracle.to_f64(p.backward(which=(1, 0, 0))[0].numpy(), dt), want, size, n + rank + 2, dt)
+    got = oracle.to_f64(p.backward(accumulate=1, which=(1, 0, 0))[0].numpy(), dt)
+    within(got, want + 3, size + 3, n + rank + 2 + SPLIT[dt], dt, added=3.0)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32], ids=ids_of)
+@pytest.mark.parametrize("rows, k, n", [(60, 64, 96), (500, 317, 256), (12, 1024, 512), (500, 136, 523), (900, 1032, 1048), (9, 2048, 264)])
+def test_infinities_of_one_group(rows, k, n, dt):
+    """An infinity and a NaN in one group's weight, and one in a row of x, reach that group's rows, or that row, in the columns they belong to."""
+    p = Grouped(dt, 3, rows, k, n, bias=False)
+    p.sw[1, k // 2, 5:8] = oracle.to_storage(np.array([np.inf, np.nan, -np.inf]), dt)
+    p.dw, p.w = Dev(p.sw, dt), oracle.to_f64(p.sw, dt)
+    y, dx = (oracle.to_f64(o.numpy(), dt) for o in (p.forward(), p.backward(which=(1, 0, 0))[0]))
+    with np.errstate(invalid="ignore"):
+        for got, left, right, terms in ((y, p.x, p.w, k), (dx, p.g, p.w.transpose(0, 2, 1), n)):
+            for i, (f, t) in enumerate(zip(p.offsets, p.offsets[1:])):
+                want = left[f:t] @ right[i]
+                assert np.array_equal(np.isnan(got[f:t]), np.isnan(want)) and np.array_equal(got[f:t][np.isinf(want)], want[np.isinf(want)])
+                fine = np.isfinite(want)
+                within(np.where(fine, got[f:t], 0), np.where(fine, want, 0), np.where(fine, np.abs(left[f:t]) @ np.where(np.isfinite(right[i]), np.abs(right[i]), 0), 0), terms, dt)
+    p = Grouped(dt, 3, rows, k, n, bias=False)
+    b = rows // 2
+    group = int(np.searchsorted(p.offsets, b, "right")) - 1
+    p.sx[b, 3] = oracle.to_storage(np.array([np.inf]), dt)[0]
+    p.dx, p.x = Dev(p.sx, dt), oracle.to_f64(p.sx, dt)[:, :k]
+    y, dw = oracle.to_f64(p.forward().numpy(), dt), oracle.to_f64(p.backward(which=(0, 1, 0))[1].numpy(), dt)
+    with np.errstate(invalid="ignore"):                     # (zero times infinity is NaN)
+        assert np.array_equal(y[b], p.w[group, 3] * np.inf, equal_nan=True)
+        assert np.array_equal(dw[group, 3], p.g[b] * np.inf, equal_nan=True)
+    assert np.isfinite(np.delete(y, b, axis=0)).all()
+    dw[group, 3] = 0
+    assert np.isfinite(dw).all()
