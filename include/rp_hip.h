@@ -445,7 +445,7 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
  * Without memory for partial sums y (and dx below) are added up in another order where the layer is of few rows, of few tiles or of many short segments.  16-bit types multiply h (and u below) by b (a) as several values of 16 bits
  * that add up to it to 2^-17 of its value (float16: 2^-22 of it, and 2^-39 of the largest that it is summed with), whatever its magnitude; no row sees what another segment's
  * adapter holds, an infinity or NaN either.  y and dx are rounded once, the shared product and the term together
- * (float32, float64, widths below 8, operands without a unit stride and, without memory for partial sums, more than 32768 segments: the shared product as a layer of its own, and
+ * (float32, float64, widths below 8, operands without a unit stride and, without memory for partial sums, more than 4096 segments: the shared product as a layer of its own, and
  * the sum again). */
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
                                   int segments, int adapters, int rows, int k, int n, int rank, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long y_rs, int dtype);

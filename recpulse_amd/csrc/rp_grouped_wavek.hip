@@ -131,7 +131,7 @@ static int wavek_tile(int dtype, Tiles tiles, Fits fits) {
 static bool rows_ok(const GroupedArgs& g, int dtype) {
     const long long esz = (long long)dtype_size(dtype), limit = 1ll << 31;
     const bool b_kc = g.b_cs != 1;
-    if (g.a_cs != 1 || (b_kc && g.b_rs != 1) || g.gr.groups > ROW_TILES_GROUPS || path_disabled("mfma")) return false;
+    if (g.a_cs != 1 || (b_kc && g.b_rs != 1) || g.gr.groups > ROW_TILES_GROUPS / 2 || path_disabled("mfma")) return false;
     return (63 * g.a_rs + g.k) * esz < limit && (b_kc ? 63 * g.b_cs + g.k : (g.k - 1) * g.b_rs + 64) * esz < limit;
 }
 static bool weights_ok(const GroupedArgs& g, int dtype) {

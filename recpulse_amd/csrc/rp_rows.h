@@ -88,9 +88,12 @@ __device__ __forceinline__ RowTile find_row_tile(const RowGroups& gr, int tile, 
 
 // Of more groups than this a tile is looked for by bisection, 64 ways at a time, instead of adding up all groups' tiles before it: a trip to memory for each power of 64 and not for
 // each 64 groups.  The tiles are not numbered one after the other then: tile t of group g is number begin(g) / tile + g + t, which leaves out at most one number a group.
-constexpr int GROUPS_ADDED_UP = 1024;
-// Kernels whose workgroups look through all groups (RowTiles, the adapters' tiles) take no more than this: each 64 cost a workgroup a trip to memory
-constexpr int ROW_TILES_GROUPS = 32768;
+// (bf16, us, added up and bisected: adapters of a segment a row, 256 -> 1024, rank 16, 200 segments 18 / 15, 1000 59 / 33, 4000 437 / 96; groups of a row, 256 -> 520, 200 20 / 21, 1000 152 / 78)
+constexpr int GROUPS_ADDED_UP = 256;
+// Kernels whose workgroups look through all groups (RowTiles, the adapters' tiles) take no more than this, those of fp32 and fp64 half as many; more go to the generic kernel, which bisects.
+// (us, RowTiles and generic, groups of a row, 1025 -> 521: bf16 2000 959 / 2076, 4000 3226 / 4086, of 257 -> 521 2939 / 1074; fp32 1000 1195 / 1052, 2000 3424 / 2055; 30000 groups,
+// 257 -> 521: bf16 157521 / 7944)
+constexpr int ROW_TILES_GROUPS = 4096;
 // The last of `count` numbers g for which below(g), which does not grow again, is true; -1: none
 template <typename F> __device__ __forceinline__ int last_of(int count, F below) {
     const int lane = threadIdx.x & 63;

@@ -6,7 +6,7 @@ import pytest
 import oracle
 from recpulse_amd import capi
 from devhelp import BF16, F16, F32, Dev
-from test_grouped_gpu import UNIT, call, ids_of, ints, within
+from test_grouped_gpu import Adapters, call, ids_of, ints, within
 
 pytestmark = pytest.mark.gpu
 
@@ -47,14 +47,51 @@ def test_adapters_of_a_segment_a_row(dt, rows, k, n, rank):
 
 
 def test_grouped_rows_of_a_group_a_row():
-    """One weight for all groups (a stride of 0): 16-bit rows that stream it, and rows of no whole vectors."""
-    for rows, k, n in ((280000, 8, 4096), (70000, 9, 520)):
+    """One weight for all groups (a stride of 0): 16-bit rows that stream it, and rows of no whole vectors; on either side of where the groups are bisected and left to the generic kernel."""
+    for rows, k, n, dt in ((280000, 8, 4096, BF16), (70000, 9, 520, BF16), (256, 16, 264, F16), (257, 16, 264, F16), (4096, 17, 261, BF16), (4097, 17, 261, BF16), (2048, 20, 70, F32), (2049, 20, 70, F32)):
         rng = np.random.default_rng(n)
-        (x, fx), (w, fw) = (small(rng, s, BF16) for s in ((rows, k), (k, n)))
-        y, off = Dev.empty((rows, n), BF16), ints(np.arange(rows + 1))
-        call("rp_hip_grouped_linear_forward", y.ptr, x.ptr, w.ptr, None, off.ptr, rows, rows, k, n, k, 1, 0, n, 1, n, BF16)
+        (x, fx), (w, fw) = (small(rng, s, dt) for s in ((rows, k), (k, n)))
+        y, off = Dev.empty((rows, n), dt), ints(np.arange(rows + 1))
+        call("rp_hip_grouped_linear_forward", y.ptr, x.ptr, w.ptr, None, off.ptr, rows, rows, k, n, k, 1, 0, n, 1, n, dt)
         for i in some(rng, rows):
-            within(rows_of(y, i, n, BF16), fx[i] @ fw, np.abs(fx[i]) @ np.abs(fw), k, BF16)
+            within(rows_of(y, i, n, dt), fx[i] @ fw, np.abs(fx[i]) @ np.abs(fw), k, dt)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32], ids=ids_of)
+@pytest.mark.parametrize("groups", [300, 5000, 300000])
+def test_very_many_uneven_groups(groups, dt):
+    """Most groups empty, rows before the first and behind the last left as they are, forward and backward."""
+    rng = np.random.default_rng(groups)
+    rows, k, n, first, behind = 3000, 24, 72, 7, 11
+    sizes = rng.multinomial(rows - first - behind, rng.dirichlet(np.full(groups, 0.05)))
+    offsets = first + np.concatenate([[0], np.cumsum(sizes)])
+    (x, fx), (g, fg), (w, fw) = small(rng, (rows, k), dt), small(rng, (rows, n), dt), small(rng, (k, n), dt)
+    mark = [Dev(oracle.to_storage(np.full(s, 3.0), dt), dt) for s in ((rows, n), (rows, k), (groups, k, n))]
+    y, dx, dw = mark
+    off = ints(offsets)
+    call("rp_hip_grouped_linear_forward", y.ptr, x.ptr, w.ptr, None, off.ptr, groups, rows, k, n, k, 1, 0, n, 1, n, dt)
+    call("rp_hip_grouped_linear_backward", dx.ptr, dw.ptr, None, g.ptr, x.ptr, w.ptr, off.ptr, groups, rows, k, n, n, k, 1, 0, n, 1, k, 0, 0, 0, dt)
+    inside = slice(first, rows - behind)
+    for out, left, right, terms in ((y, fx, fw, k), (dx, fg, fw.T, n)):
+        got = oracle.to_f64(out.numpy(), dt)
+        within(got[inside], left[inside] @ right, np.abs(left[inside]) @ np.abs(right), terms, dt)
+        assert np.all(got[:first] == 3.0) and np.all(got[rows - behind:] == 3.0)
+    for e in np.concatenate([np.argsort(sizes)[-20:], some(rng, groups)]):
+        s = slice(offsets[e], offsets[e + 1])
+        within(rows_of(dw, e, k * n, dt), (fx[s].T @ fg[s]).reshape(-1), (np.abs(fx[s]).T @ np.abs(fg[s])).reshape(-1), rows, dt)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32], ids=ids_of)
+@pytest.mark.parametrize("segments", [300, 5000])
+def test_very_many_uneven_segments(segments, dt):
+    rows, k, n, rank, adapters = 2500, 40, 136, 8, 5
+    p = Adapters(dt, segments, adapters, rows, k, n, rank, behind=9)
+    rng = np.random.default_rng(segments)
+    p.offsets = np.concatenate([[0], np.cumsum(rng.multinomial(rows - 16, rng.dirichlet(np.full(segments, 0.05))))]).astype(np.int32) + 7
+    p.doff = ints(p.offsets)
+    p.forward()
+    p.check_forward()
+    p.check_backward(p.backward())
 
 
 @pytest.mark.parametrize("dt, groups, width", [(BF16, 2200000, 8), (BF16, 17000000, 4), (F32, 2200000, 8)])
