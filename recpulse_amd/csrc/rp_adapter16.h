@@ -17,6 +17,8 @@
 
 namespace rp {
 
+// Ranks that have registers for their sums; wider factors go to the scalar kernel, where they would need their columns dealt to workgroups that each read x again (bf16, 2048 rows of 4096: rank
+// 128 19 us here, rank 136 158 there)
 constexpr int SH_STEP = 32, SH_MAX_RANK = 128;
 
 typedef unsigned int u32x4_odd_t __attribute__((ext_vector_type(4), aligned(2)));       // a 16-byte vector at any element
@@ -51,14 +53,15 @@ __device__ __forceinline__ void split_low(const float* v, u32x4_t& hi, u32x4_t& 
 // float16 reaches from 2^-24 to 65504, and sums of small gradients lie below: before they are split, values that are multiplied together are brought to a largest one of
 // 2^14 .. 2^15 by a power of two, and their product back.  Two values then add up to one to 2^-22 of it and 2^-39 of the largest.  (bfloat16 reaches as far as float32.)
 __device__ __forceinline__ uint32_t finite_bits(float v) { const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu; return b < 0x7F800000u ? b : 0u; }
-// The biased exponent of the largest finite value of the four lanes that share j = lane % 16, at least 15 (so that both powers are normal numbers)
-__device__ __forceinline__ uint32_t low_exponent(const float* v) {
-    uint32_t m = 15u << 23;
+__device__ __forceinline__ void largest_bits(uint32_t& bits, const float* v) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) { const uint32_t b = finite_bits(v[e]); m = b > m ? b : m; }
+    for (int e = 0; e < 8; e++) { const uint32_t b = finite_bits(v[e]); bits = b > bits ? b : bits; }
+}
+// The biased exponent of the largest of the four lanes that share j = lane % 16, at least 15 (so that both powers are normal numbers)
+__device__ __forceinline__ uint32_t low_exponent(uint32_t bits) {
 #pragma unroll
-    for (int d = 16; d < 64; d *= 2) { const uint32_t b = __shfl_xor(m, d); m = b > m ? b : m; }
-    return m >> 23;
+    for (int d = 16; d < 64; d *= 2) { const uint32_t b = __shfl_xor(bits, d); bits = b > bits ? b : bits; }
+    return bits >> 23 > 15u ? bits >> 23 : 15u;
 }
 __device__ __forceinline__ float low_up(uint32_t exponent) { return __uint_as_float((268u - exponent) << 23); }
 __device__ __forceinline__ float low_down(uint32_t exponent) { return __uint_as_float((exponent - 14u) << 23); }

@@ -48,7 +48,7 @@ bool adapter_shrink16_takes(const GroupedArgs& g) {
 int launch_adapter_shrink16(const GroupedArgs& g, int dtype) { return dtype == RP_DTYPE_BFLOAT16 ? launch_shrink_rank<bf16_t>(g) : launch_shrink_rank<f16_t>(g); }
 
 // ---- a few rows: the shared projection's shares of k and the rows' h side by side, then one launch that adds them up with the adapters' terms ----
-// 32 rows with adapters of their own, 4096 x 4096 and rank 16 in bf16: 16.5 us and 4.1 (6.1 for the narrow products by themselves and 12.1 for the shared one).
+// 32 rows with adapters of their own, 4096 x 4096 and rank 16 in bf16: 16.8 us and 4.0 (6.1 for the narrow products by themselves and 12.1 for the shared one).
 template <typename T, int CPL, int RB, int NC>
 __global__ void __launch_bounds__(GS_THREADS) adapter_first16_kernel(GroupedArgs shared, StreamGrid sg, GroupedArgs low, int low_blocks) {
     if ((int)blockIdx.x < low_blocks) adapter_shrink16_block<T, NC, 1, false, 8, GS_WAVES>(low, (int)blockIdx.x);
@@ -119,7 +119,7 @@ int launch_adapter_few_rows16(const GroupedArgs& shared, const GroupedArgs& low,
 // The shared product leaves float32 sums of its shares of k; y = sums + bias + h . b_a is rounded once.  A wave for 16 rows of a segment (or of none: those are only rounded)
 // and 128 columns, the rank 32 at a time; h in two values of T as in the gradients.  b is read as it lies, eight rows of the rank times eight
 // columns a lane, and turned with byte permutes, or, where it is contiguous along the rank, as fragments.  Bound by a few loads in a row; with multiply-adds in
-// float32 and h out of the scalar cache 7 rows of rank 64 took 67 us, 5.9 now; the product's sums 3.8 (128 x 94).
+// float32 and h out of the scalar cache 7 rows of rank 64 took 67 us, 6.0 now; the product's sums 3.7 (128 x 94).
 struct ExpandArgs {
     uint16_t* y;
     const uint16_t* bias;
@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(64) adapter_expand16_kernel(ExpandArgs ea, Ada
             const bool odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
             float down[4];                                                // of rows 4q + v
             if constexpr (std::is_same<T, f16_t>::value) {
-                const uint32_t top = low_exponent(hv);
+                uint32_t bits = 0;
+                largest_bits(bits, hv);
+                const uint32_t top = low_exponent(bits);
                 split_scaled<T>(hv, low_up(top), hi, lo);
 #pragma unroll
                 for (int v = 0; v < 4; v++) down[v] = __shfl(low_down(top), 4 * q + v);

@@ -6,7 +6,7 @@
 // weight does in the kernel for few rows (rp_grouped_stream16.h): a lane transposes 8 rows x 8 columns with byte permutes.  low is
 // rounded to two values of the tensors' type that add up to it to 2^-17 (float16: 2^-22, scaled by the largest value of the wave's rows, which it looks for first), a product each: h and u are
 // sums in float32, and one rounding of theirs would be as large as the result's own.
-// fp16, 2048 rows of 3 adapters, 1024 x 2048, rank 8: both 10 us, 3 beside dx's tiles (25 us together).  (Eight waves a workgroup: 8192 rows of one adapter, 4096 x 4096, 48 us instead of
+// fp16, 2048 rows of 3 adapters, 1024 x 2048, rank 8: both 17 us, of which looking for the largest values takes 3, and beside dx's tiles 26 together.  (Eight waves a workgroup: 8192 rows of one adapter, 4096 x 4096, 48 us instead of
 // 55 before its rows were shared out, 34 since, but 32 adapters and rank 64 144 instead of 93: a CU holds one such workgroup.)
 #pragma once
 #include "rp_adapter16.h"
@@ -68,7 +68,7 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     };
     f32x4_t acc[NC][8];
     constexpr bool SCALED = std::is_same<T, f16_t>::value;
-    uint32_t top[NC];                                         // of column 16 c + j of the rank
+    uint32_t top[NC];                                         // of column 16 c + j of the rank: the largest value's bits, then its exponent
     auto multiply = [&](auto slotc) {
         constexpr int SL = decltype(slotc)::value;
         u32x4_t hi[NC], lo[NC];
@@ -108,20 +108,27 @@ __device__ __forceinline__ void adapter_grad16_block(const AdapterGrad& ag, cons
     while (true) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            top[c] = 15u;
+            top[c] = 0;
 #pragma unroll
             for (int f = 0; f < 8; f++) acc[c][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
         if constexpr (SCALED)
             for_rounds([&](int first, int turn) {
-                for (int row0 = first; row0 < end; row0 += SLOTS * turn) {
-                    static_for<0, SLOTS>([&](auto sc) { request_low(lv[decltype(sc)::value], row0 + decltype(sc)::value * turn); });
-                    static_for<0, SLOTS>([&](auto sc) {
+                constexpr int AHEAD = 4;                      // rounds (the registers that the main loop's loads take are free here)
+                for (int row0 = first; row0 < end; row0 += AHEAD * turn) {
+                    float v[AHEAD][NC][8];
 #pragma unroll
-                        for (int c = 0; c < NC; c++) { const uint32_t t = low_exponent(lv[decltype(sc)::value][c]); top[c] = t > top[c] ? t : top[c]; }
-                    });
+                    for (int i = 0; i < AHEAD; i++) request_low(v[i], row0 + i * turn);
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) largest_bits(top[c], v[i][c]);
                 }
             });
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) top[c] = low_exponent(top[c]);
+        }
         for_rounds([&](int first, int turn) {
             static_for<0, SLOTS>([&](auto sc) { request(sc, first + decltype(sc)::value * turn); });
             for (int row0 = first; row0 < end; row0 += SLOTS * turn)
@@ -229,7 +236,7 @@ __global__ void __launch_bounds__(256) adapter_grads16_join_kernel(AdapterGrads 
 }
 
 // Where shares of an adapter's rows are added up, `launch` leaves them in the call's memory for a launch of their own, or, without memory, `in_turn` has workgroups do one share after
-// the other: the same bits (bf16, 7949 rows of one adapter, 384 x 1512, rank 32, forward and backward 118 us and 144).
+// the other: the same bits (bf16, one adapter, backward, us: 7949 rows, 384 x 1512, rank 32 43 and 37; 8192 rows, 4096 x 4096, rank 16 261 and 320).
 template <typename T, typename F, typename G>
 static int with_joined_grads(AdapterGrads& ag, const RowGroups& gr, F launch, G in_turn) {
     if (ag.shares == 1) return launch();
