@@ -3,8 +3,8 @@
 //
 // For every segment that has rows in a wave's patch: rank / 32 (/ 16) k-steps of MFMAs, the other segments' rows zero.  h is float32 and is
 // multiplied as two values of bfloat16; where the tensors are float16, which does not reach far enough for it, as three, and b, exactly, as two (five products).  b comes straight from memory, 16 bytes a lane where it is contiguous along
-// the rank (a_a^T, for dx) and else in 2-byte loads.  4096 x 4096 x 4096 with seven segments in bf16: 122 us at rank 16 and 132 at rank 32, beside 103 for the product
-// alone and 18 and more for a pass over y.
+// the rank (a_a^T, for dx) and else in 2-byte loads.  4096 x 4096 x 4096 with seven segments in bf16: 119 us at rank 16 and 118 at rank 32 (float16 129), 107 without an adapter, beside 18
+// and more for a pass over y.
 // (Between the last slab and the epilogue the same code takes registers from the main loop of the 256 x 256 tile: a value or two reloaded
 // from memory a slab, behind which all of its loads are waited for; 130.  In the epilogue, into registers of its own 16 rows at a
 // time, it is unrolled eightfold and waits for its instructions: 134.)

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(SORT_ONE_WAVES * 64) sort_one_kernel(const int
 
 // Longer lists in two launches: count each chunk's slots by expert, into counts [chunks][groups], then place each chunk's slots.  A workgroup of
 // the second adds up the counts of all chunks by itself: 256 chunks of 128 experts are 128 KB out of the L2, which takes less than a launch
-// between the two that adds them up once (16384 tokens, 8 of 128 experts: 13.8 us in three launches, 6.6 here, the counts coming from the selection).
+// between the two that adds them up once (16384 tokens, 8 of 128 experts: 13.8 us in three launches, 7.3 here, the counts coming from the selection).
 __device__ __forceinline__ void count_ids(const int* ids, int s0, int s1, int groups, int* counts) {
     for (int s = s0 + threadIdx.x; s < s1; s += SORT_ONE_WAVES * 64) {
         const int id = ids[s];
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(ROUTE_ONE_THREADS) route_one_kernel(weight_t<T
     sort_all(ids, tokens * k, experts, bits, sort_lds, offsets, order, position);
 }
 
-// Gradient of the logits, bound by memory from about 10^5 tokens on (200000 of 128 in fp32 51 us, 4 TB/s; 16384 8 us).  With p the softmax over the experts that the weights were divided by, and g_j the weights' gradients,
+// Gradient of the logits, bound by memory from about 10^5 tokens on (200000 of 128 in fp32 51 us, 4 TB/s; 16384 8.6 us).  With p the softmax over the experts that the weights were divided by, and g_j the weights' gradients,
 //   dl_e = p_e (g_e - sum over j of w_j g_j),   g_e = 0 where e was not taken; with "normalize" p_e = w_j where taken and 0 elsewhere.
 template <typename T, int LANES, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(T* grad, const weight_t<T>* grad_weights, const weight_t<T>* weights, const int* taken, const T* logits, long long rs,
@@ -526,7 +526,7 @@ static int launch_route_backward(void* grad, const void* grad_weights, const voi
 
 // ---- exchange: kernels ----
 // All of them are bound by memory: a row is read and written once, in pieces of 16 bytes where rows allow it (VEC elements;
-// otherwise element by element).  8192 tokens of 4096 in bf16, two rows each: dispatch 31 us (5.9 TB/s), combine 42 (4.4), its gradient 68 (4.5).
+// otherwise element by element).  8192 tokens of 4096 in bf16, two rows each: dispatch 31 us (6.0 TB/s), combine 41 (4.6), its gradient 67 (4.5).
 // (Stores that stream past the caches make combine 34 and its gradient 61, and whoever reads the rows next slower by more: dispatch and a kernel that reads its 134 MB
 // take 66 us, 91 with them.)
 typedef __attribute__((ext_vector_type(4))) unsigned int row_vec_t;
