@@ -59,14 +59,12 @@ class ForeignStream(capi.Stream):
     """A stream that the library did not make: it does not know when one ends, and keeps no memory for it."""
 
     def __init__(self):
-        with open("/proc/self/maps") as maps:
-            self.hip = ctypes.CDLL(next(line.split()[-1] for line in maps if "libamdhip64" in line))
         p = ctypes.c_void_p()
-        assert self.hip.hipStreamCreateWithFlags(ctypes.byref(p), 1) == 0
+        assert capi.lib().hipStreamCreateWithFlags(ctypes.byref(p), 1) == 0          # (of the runtime that the library is linked to)
         self.ptr, self._prev = p.value, None
 
     def __del__(self):
-        self.hip.hipStreamDestroy(ctypes.c_void_p(self.ptr))
+        capi.lib().hipStreamDestroy(ctypes.c_void_p(self.ptr))
 
 
 class Step:
