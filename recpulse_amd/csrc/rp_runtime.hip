@@ -196,6 +196,16 @@ NullStreamScratch::NullStreamScratch(size_t bytes) {
 }
 NullStreamScratch::~NullStreamScratch() { if (ptr) g_null_stream_mu.unlock(); }
 
+// Another thread's recording in the runtime's default mode would be spoilt by an allocation, unless the allocating thread is in the relaxed mode.
+class RelaxedCapture {
+public:
+    RelaxedCapture() : ok(hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess) { if (!ok) (void)hipGetLastError(); }
+    ~RelaxedCapture() { if (ok) (void)hipThreadExchangeStreamCaptureMode(&mode); }
+private:
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool ok;
+};
+
 // A stream's block: of the largest size asked for so far, kept until rp_hip_empty_cache or the end of the stream.  (hipFree waits for the work that uses it.)
 struct StreamMemory {
     std::mutex mu;
@@ -207,16 +217,14 @@ struct StreamMemory {
         size_t want = CallScratch::MOST;
         while (want < bytes && want < ((size_t)1 << 30)) want *= 2;
         if (want < bytes) want = round_size(bytes);
-        // (another thread's recording in the runtime's default mode would be spoilt by an allocation, unless this thread is in the relaxed mode)
-        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) { (void)hipGetLastError(); return false; }
+        const RelaxedCapture relaxed;
         release();
         if (hipMalloc(&block, want) == hipSuccess) size = want;
         else { (void)hipGetLastError(); block = nullptr; }
-        (void)hipThreadExchangeStreamCaptureMode(&mode);
         return size != 0;
     }
     bool release() {
+        const RelaxedCapture relaxed;
         const bool ok = !block || hipFree(block) == hipSuccess;
         if (!ok) (void)hipGetLastError();
         block = nullptr;
@@ -226,6 +234,20 @@ struct StreamMemory {
 };
 static StreamMemory* null_stream_memory() { static auto* m = new StreamMemory[NULL_STREAM_DEVICES]; return m; }
 static std::mutex g_created_mu;
+// Blocks of streams that ended while their thread was recording, when nothing may be freed: until the next call that reserves memory, or rp_hip_empty_cache
+static std::vector<void*>& retired_blocks() { static auto* v = new std::vector<void*>(); return *v; }
+static bool free_retired() {
+    std::vector<void*> blocks;
+    {
+        std::lock_guard<std::mutex> lk(g_created_mu);
+        blocks.swap(retired_blocks());
+    }
+    bool ok = true;
+    const RelaxedCapture relaxed;
+    for (void* b : blocks)
+        if (hipFree(b) != hipSuccess) { (void)hipGetLastError(); ok = false; }
+    return ok;
+}
 static std::unordered_map<void*, StreamMemory*>& created_streams() { static auto* m = new std::unordered_map<void*, StreamMemory*>(); return *m; }
 
 CallScratch::CallScratch(size_t bytes, size_t most) {
@@ -245,6 +267,7 @@ CallScratch::CallScratch(size_t bytes, size_t most) {
         if (it != created_streams().end() && it->second->device == dev) memory = it->second;
     }
     if (memory) {
+        free_retired();
         memory->mu.lock();
         if (memory->reserve(bytes)) ptr = memory->block;
         else { memory->mu.unlock(); memory = nullptr; }
@@ -438,6 +461,7 @@ int rp_hip_empty_cache(void) {
         std::lock_guard<std::mutex> slk(null_stream_memory()[d].mu);
         ok = null_stream_memory()[d].release() && ok;
     }
+    ok = free_retired() && ok;
     {
         std::lock_guard<std::mutex> clk(g_created_mu);
         for (auto& it : created_streams()) {
@@ -537,6 +561,10 @@ int rp_hip_stream_destroy(void* stream) {
         std::lock_guard<std::mutex> lk(g_created_mu);
         auto it = created_streams().find(stream);
         if (it != created_streams().end()) { memory = it->second; created_streams().erase(it); }
+        if (memory && memory->block && stream_is_capturing()) {
+            retired_blocks().push_back(memory->block);
+            memory->block = nullptr;
+        }
     }
     if (memory) {
         memory->release();

@@ -155,3 +155,47 @@ def test_adapters_on_two_streams_at_once_and_recorded(shape, kind):
         for _, _, v, want in graphs:
             for a, b in zip(v.bits(), want):
                 assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+def test_a_stream_with_memory_ends_while_another_is_recorded():
+    """The memory is given back later: a recording allows no freeing."""
+    steps = [Step((9, 4, 32, 4096, 512, 16, BF16), seed) for seed in range(2)]
+    here, other = capi.Stream(), capi.Stream()
+    for s, v in zip((here, other), steps):
+        v.clear()
+        with s:
+            v.run()
+        capi.synchronize()
+        v.check()
+    with here:
+        with capi.Graph.capture() as g:
+            steps[0].run()
+            ended, other.ptr = other.ptr, None
+            call("rp_hip_stream_destroy", ended)
+            steps[0].run()
+        for _ in range(3):
+            steps[0].clear()
+            g.launch()
+            capi.synchronize()
+            steps[0].check()
+    with capi.Stream():                                        # (the next one frees it)
+        steps[1].clear()
+        steps[1].run()
+        capi.synchronize()
+        steps[1].check()
+
+
+def test_memory_goes_with_the_streams():
+    """Streams made and ended one after the other do not keep their memory."""
+    v = Step((900, 5, 2500, 264, 2056, 8, BF16), 3)
+    free, total = ctypes.c_size_t(), ctypes.c_size_t()
+    left = []
+    for _ in range(12):
+        v.clear()
+        with capi.Stream():
+            v.run()
+        capi.synchronize()
+        v.check()
+        assert capi.lib().hipMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+        left.append(free.value)
+    assert left[-1] >= left[2] - (8 << 20)
