@@ -121,9 +121,9 @@ static TermTile term_tile(const GroupedArgs& s, const AdapterTerm& term, int dty
     const long long tiles = (long long)((s.gr.rows + p.bm - 1) / p.bm) * ((s.n + p.bn - 1) / p.bn);
     // byte offsets into h and into an adapter's factor in 32 bits
     const bool reach = (long long)s.gr.rows * term.rank < (1 << 29) && ((term.rank - 1) * term.b_rs + (s.n - 1) * term.b_cs) < (1 << 30);
-    // from about a tile for every other CU on, and while a tile's rows are few segments: each costs it 2 us (bf16, 4096 rows, the layer's us in the tiles and apart: 400 segments,
-    // 1024 -> 4096, rank 8 119 / 109, 4096 -> 4096, rank 32 303 / 233; 7 segments 50 / 86 and 128 / 207)
-    const int last = !reach || lie == LIE_NEITHER || term.gr.groups > ROW_TILES_GROUPS ? 0 : p.bm == 128 && p.bn == 128 ? 128 : 64;
+    // from about a tile for every other CU on, and while a tile's rows are few segments, each of which costs it 1 to 2 us a step of the rank (bf16, 4096 rows, the layer's us in tiles of 128 and
+    // apart: 7 segments, 1024 -> 4096, rank 8 50 / 86; 400 segments 77 / 100, 4096 -> 4096, rank 32 205 / 228, 1024 -> 1024, rank 64 62 / 47; 1500 segments 133 / 140, 300 / 281, 142 / 66)
+    const int last = !reach || lie == LIE_NEITHER || term.gr.groups > ROW_TILES_GROUPS ? 0 : p.bm >= 128 && p.bn >= 128 ? 128 : 64;
     if (!last || p.bm != p.bn || tiles * 2 < cus() || term.gr.rows / term.gr.groups < 16 || path_disabled("adapter_tiles")) return {0, false, p.ragged, lie != LIE_NEITHER, last};
     return {p.bm, !p.edge, p.ragged, true, last};
 }

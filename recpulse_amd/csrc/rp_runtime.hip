@@ -242,6 +242,7 @@ static bool free_retired() {
         std::lock_guard<std::mutex> lk(g_created_mu);
         blocks.swap(retired_blocks());
     }
+    if (blocks.empty()) return true;
     bool ok = true;
     const RelaxedCapture relaxed;
     for (void* b : blocks)
