@@ -185,6 +185,7 @@ struct AdapterTiles {
         if (!odd) return;
         odd = false;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");           // (a wave adds to what its own lanes stored)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const args_t args = arguments();
         const AdapterTerm term = term_of(args);
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = args->g.m, n = args->g.n;

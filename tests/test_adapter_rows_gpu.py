@@ -70,7 +70,12 @@ def test_rows_beside_an_adapter_that_is_not_finite(shape, dt):
     p.forward()
     put(p, "a", (0, slice(3, 6), rank // 2), [np.inf, np.nan, -np.inf])
     put(p, "a", (1, 7, 0), np.inf)
-    once(oracle.to_f64(p.backward()[0].numpy(), dt), *input_gradient(p), n + rank + 2, dt)
+    want, size = input_gradient(p)
+    once(oracle.to_f64(p.backward()[0].numpy(), dt), want, size, n + rank + 2, dt)
+    got = oracle.to_f64(p.backward(accumulate=1)[0].numpy(), dt)         # (added to 3: the same places)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    fine = np.isfinite(want)
+    within(np.where(fine, got, 3), np.where(fine, want + 3, 3), np.where(np.isfinite(size), size, 0) + 3, n + rank + 2 + SPLIT[dt], dt, roundings=2 if dt == F32 else 1, added=3.0)
 
 
 # the shapes above, many rows of one adapter
