@@ -458,6 +458,56 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
                                    long long dy_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs,
                                    int accumulate_dx, int accumulate_da, int accumulate_db, int dtype);
 
+/* ---- what stands around a language model's products (no counterpart in the reference) ----
+ * Layer norm, the gated linear layer, the cross entropy of a large vocabulary from the hidden rows, and distillation from a teacher's top logits.  All types; sums and the values between are
+ * in the accumulate type (float32, float64 for float64).  Strides in elements, non-negative; outputs overlap neither an operand nor each other.  `workspace` is device memory of the caller's, as
+ * many bytes as the entry's own _workspace function says (-1: arguments that the entry would refuse), aligned to 16; a call leaves nothing there that another call reads, so that calls in turn on one
+ * stream may share it and calls on several streams may not.  Results do not depend on the stream, and the same call leaves the same bits. */
+
+/* Layer norm of rows [rows, d]: y = (x - mean) / sqrt(variance + eps) * w + b, with the mean of the squared differences as variance.  w, b: dense [d] or NULL.  stats: [rows, 2]
+ * in the accumulate type, mean and 1 / sqrt(variance + eps), for the backward pass; may be NULL. */
+int rp_hip_layer_norm_forward(void* y, void* stats, const void* x, const void* w, const void* b, int rows, int d, long long y_rs, long long x_rs, double eps, int dtype);
+/* Its gradients: dx [rows, d] with a row stride, dw and db dense [d]; any may be NULL.  accumulate_* = 1 adds to what is there (before the one rounding).  workspace is read for dw and db only. */
+long long rp_hip_layer_norm_workspace(int rows, int d, int dtype);
+int rp_hip_layer_norm_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w, const void* stats, void* workspace, int rows, int d,
+                               long long dy_rs, long long x_rs, long long dx_rs, int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);
+
+/* Gated linear layer: h = act(x . Wg + bg) * (x . Wu + bu).  w [k, 2 n]: columns [0, n) are Wg, the others Wu (as a cell's gates lie in one matrix); bias dense [2 n] or NULL; x [rows, k];
+ * h [rows, n] with unit column stride, rounded once.  z: [rows, 2 n] dense, in the accumulate type: g | u before the activation, kept by the caller for the backward pass; NULL where there is none. */
+enum { RP_GATE_SILU = 0, RP_GATE_GELU = 1, RP_GATE_GELU_TANH = 2, RP_GATE_RELU = 3, RP_GATE_SIGMOID = 4 };
+int rp_hip_gated_linear_forward(void* h, void* z, const void* x, const void* w, const void* bias, int rows, int k, int n, int gate,
+                                long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long h_rs, int dtype);
+/* Its gradients.  dz: [rows, 2 n] dense, room for the gradient of g | u in the tensors' type.  dx [rows, k] with unit column stride, dw [k, 2 n] with unit stride along either axis (the
+ * gradient of a transposed weight lies as the weight does), db dense [2 n]; any of the three may be NULL; accumulate_* = 1 adds the rounded product to what is there. */
+int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const void* dh, const void* z, const void* x, const void* w, int rows, int k, int n, int gate,
+                                 long long dh_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs, long long dw_rs, long long dw_cs,
+                                 int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);
+
+/* Cross entropy of a large vocabulary from the rows before it: with z = x . w + bias (x [rows, k], w [k, classes], bias dense [classes] or NULL),
+ *   loss_i = log sum over v of exp(z[i, v]) - z[i, targets[i]].
+ * The logits are made in pieces of the vocabulary and not kept.  targets: device int32 [rows]; a row whose target lies outside [0, classes) is left out: its loss and gradient are zeros.
+ * reduction 0: loss_out [rows]; 1: the mean over the rows with a target (0 where there are none); 2: their sum; loss_out in the accumulate type.  stats: 2 rows + 1 values of the accumulate type, for the
+ * backward pass: log sum exp of each row, its loss, and how many rows have a target. */
+long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, int backward, int dtype);
+int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,
+                                        long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype);
+/* Its gradients times upstream_dev, accumulate type on the device ([rows] for reduction 0, one element otherwise; NULL: 1): dx [rows, k] with unit column stride, dw [k, classes] with unit stride along
+ * either axis, db dense [classes]; any may be NULL.  The logits are made again, piece by piece, and each piece's gradient (rounded to the tensors' type, whatever its magnitude) multiplied at once. */
+int rp_hip_linear_cross_entropy_backward(void* dx, void* dw, void* db, const void* x, const void* w, const void* bias, const int* targets, const void* stats, const void* upstream_dev, void* workspace,
+                                         int rows, int k, int classes, int reduction, long long x_rs, long long x_cs, long long w_rs, long long w_cs,
+                                         long long dx_rs, long long dw_rs, long long dw_cs, int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);
+
+/* Distillation from a teacher's top logits at temperature T: with q = softmax(logits[i] / T) over all classes and p = softmax(teacher[i] / T) over the row's k entries,
+ *   loss_i = T^2 * sum over j of p_j (log p_j - log q[ids[i, j]]).
+ * logits [rows, classes] with a row stride; ids, teacher dense [rows, k] (at most 1024 entries); an entry whose class lies outside [0, classes) or whose logit is -inf is left out, a row without any has
+ * zeros for loss and gradient; a class may be named twice.  reduction 0: loss_out [rows]; 1: the sum over the rows divided by all rows; 2: the sum; in the accumulate type.  stats: 3 rows values of the accumulate
+ * type, for the backward pass.  grad_logits [rows, classes], dense: the gradient times upstream_dev (accumulate type on the device: [rows] for reduction 0, one element otherwise; NULL: 1) from the same read of the logits; may be NULL. */
+int rp_hip_distillation_forward(void* loss_out, void* grad_logits, void* stats, const void* logits, const int* ids, const void* teacher, const void* upstream_dev,
+                                int rows, int classes, int k, long long logits_rs, double temperature, int reduction, int dtype);
+/* The gradient alone, from the stats of a forward call on the same operands */
+int rp_hip_distillation_backward(void* grad_logits, const void* stats, const void* logits, const int* ids, const void* teacher, const void* upstream_dev,
+                                 int rows, int classes, int k, long long logits_rs, double temperature, int reduction, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -109,6 +109,16 @@ SIGNATURES = {
     "rp_hip_grouped_linear_backward": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 7 + [_i] * 4),
     "rp_hip_adapter_linear_forward": (_i, [_vp] * 10 + [_i] * 6 + [_ll] * 5 + [_i]),
     "rp_hip_adapter_linear_backward": (_i, [_vp] * 13 + [_i] * 6 + [_ll] * 6 + [_i] * 4),
+    "rp_hip_layer_norm_forward": (_i, [_vp] * 5 + [_i] * 2 + [_ll] * 2 + [_d, _i]),
+    "rp_hip_layer_norm_workspace": (_ll, [_i] * 3),
+    "rp_hip_layer_norm_backward": (_i, [_vp] * 8 + [_i] * 2 + [_ll] * 3 + [_i] * 4),
+    "rp_hip_gated_linear_forward": (_i, [_vp] * 5 + [_i] * 4 + [_ll] * 5 + [_i]),
+    "rp_hip_gated_linear_backward": (_i, [_vp] * 8 + [_i] * 4 + [_ll] * 8 + [_i] * 4),
+    "rp_hip_linear_cross_entropy_workspace": (_ll, [_i] * 5),
+    "rp_hip_linear_cross_entropy_forward": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 4 + [_i]),
+    "rp_hip_linear_cross_entropy_backward": (_i, [_vp] * 10 + [_i] * 4 + [_ll] * 7 + [_i] * 4),
+    "rp_hip_distillation_forward": (_i, [_vp] * 7 + [_i] * 3 + [_ll, _d, _i, _i]),
+    "rp_hip_distillation_backward": (_i, [_vp] * 6 + [_i] * 3 + [_ll, _d, _i, _i]),
 }
 
 _lib = None

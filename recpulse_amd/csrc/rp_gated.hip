@@ -1,0 +1,237 @@
+// Entry points of the gated linear layer, its kernels for any strides, sizes and types, and its backward pass.
+//
+//   z = x . W + b (columns [0, n): gate g, [n, 2 n): up u),  h = act(g) u
+//   dz = [dh u act'(g) | dh act(g)],  dx = dz . W^T,  dW = x^T . dz,  db = sum of dz over the rows
+//
+// z is kept in the accumulate type (float32 for the 16-bit types), as the sums that they are: rounded to 16 bits, z's own error would reach dz beside dz's, and the gradients'
+// error would be 1.3 times as large.  dz is rounded to the tensors' type, which is what the matrix cores multiply.
+#include "rp_gated.h"
+#include "rp_grouped.h"
+
+namespace rp {
+
+// Any strides and sizes: 64 rows x 32 columns of h a workgroup, 16 of k at a time through LDS, scalar multiply-adds
+template <typename T, int GATE>
+__global__ void __launch_bounds__(256) gated_any_kernel(GatedArgs g, int tiles_n, long long first) {
+    using A = typename traits<T>::acc;
+    constexpr int ROWS = 64, COLS = 32, K = 16;
+    __shared__ A as[K][ROWS + 4], bs[K][2 * COLS + 4];
+    const long long id = first + blockIdx.x;
+    const int m0 = (int)(id / tiles_n) * ROWS, n0 = (int)(id % tiles_n) * COLS;
+    const int t = threadIdx.x, tr = (t >> 4) * 4, tc = (t & 15) * 2;
+    A acc[4][2][2] = {};
+    for (int k0 = 0; k0 < g.k; k0 += K) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = t + 256 * i;
+            const int ar = g.x_cs <= g.x_rs ? e / K : e % ROWS, ak = g.x_cs <= g.x_rs ? e % K : e / ROWS;
+            const int bc = g.w_cs <= g.w_rs ? e % (2 * COLS) : e / K, bk = g.w_cs <= g.w_rs ? e / (2 * COLS) : e % K;
+            const int col = n0 + bc % COLS;
+            as[ak][ar] = m0 + ar < g.rows && k0 + ak < g.k ? (A)widen(((const T*)g.x)[(m0 + ar) * g.x_rs + (k0 + ak) * g.x_cs]) : (A)0;
+            bs[bk][bc] = col < g.n && k0 + bk < g.k ? (A)widen(((const T*)g.w)[(k0 + bk) * g.w_rs + (col + (long long)(bc / COLS) * g.n) * g.w_cs]) : (A)0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < K; kk++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    acc[i][j][0] += as[kk][tr + i] * bs[kk][tc + j];
+                    acc[i][j][1] += as[kk][tr + i] * bs[kk][COLS + tc + j];
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int row = m0 + tr + i, col = n0 + tc + j;
+            if (row >= g.rows || col >= g.n) continue;
+            A gate = acc[i][j][0], up = acc[i][j][1];
+            if (g.bias) {
+                gate += widen(((const T*)g.bias)[col]);
+                up += widen(((const T*)g.bias)[g.n + col]);
+            }
+            if (g.z) {
+                ((A*)g.z)[(long long)row * 2 * g.n + col] = gate;
+                ((A*)g.z)[(long long)row * 2 * g.n + g.n + col] = up;
+            }
+            ((T*)g.h)[row * g.h_rs + col] = round_to<T>(gate_value<GATE>(gate) * up);
+        }
+}
+
+template <typename T>
+static int launch_gated_any(const GatedArgs& g) {
+    const int tiles_n = (g.n + 31) / 32;
+    const long long blocks = (long long)((g.rows + 63) / 64) * tiles_n;
+    return in_launches(blocks, 256, [&](unsigned count, long long first) {
+        RP_DISPATCH_GATE(g.gate, hipLaunchKernelGGL((gated_any_kernel<T, GATE>), dim3(count), dim3(256), 0, current_stream(), g, tiles_n, first));
+        return check_launch("gated_any_kernel") ? 0 : -1;
+    });
+}
+
+// Element-wise passes: a workgroup takes 256 vectors of a row's columns at a time
+constexpr int GATED_GRID = 1 << 20;
+
+// h from z (float32 and float64, whose z comes from a product of its own)
+template <typename T, int GATE>
+__global__ void __launch_bounds__(256) gated_value_kernel(T* h, const typename traits<T>::acc* z, int rows, int n, long long h_rs, int across) {
+    const long long total = (long long)rows * across;
+    for (long long id = blockIdx.x; id < total; id += gridDim.x) {
+        const int row = (int)(id / across), c = (int)(id % across) * 256 + threadIdx.x;
+        if (c >= n) continue;
+        const auto* zr = z + (long long)row * 2 * n;
+        h[row * h_rs + c] = round_to<T>(gate_value<GATE>(zr[c]) * zr[n + c]);
+    }
+}
+
+// dz from dh and z: N columns a thread where there are as many
+template <typename T, int GATE>
+__global__ void __launch_bounds__(256) gated_dz_kernel(T* dz, const T* dh, const typename traits<T>::acc* z, int rows, int n, long long dh_rs, int across) {
+    using A = typename traits<T>::acc;
+    constexpr int N = vec16<T>::N;
+    const long long total = (long long)rows * across;
+    for (long long id = blockIdx.x; id < total; id += gridDim.x) {
+        const int row = (int)(id / across), c = ((int)(id % across) * 256 + (int)threadIdx.x) * N;
+        const T* d = dh + row * dh_rs;
+        const A* zr = z + (long long)row * 2 * n;
+        T* out = dz + (long long)row * 2 * n;
+        if (c >= n) continue;
+        if (n >= N) {
+            const RowVector<T> at(c, n);
+            T dv[N], og[N], ou[N];
+            at.load(dv, d);
+            A gate[N], up[N];
+            __builtin_memcpy(gate, zr + at.at, sizeof(gate));
+            __builtin_memcpy(up, zr + n + at.at, sizeof(up));
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const A v = widen(dv[u]);
+                og[u] = round_to<T>(v * up[u] * gate_slope<GATE>(gate[u]));
+                ou[u] = round_to<T>(v * gate_value<GATE>(gate[u]));
+            }
+            at.store(out, og);
+            at.store(out + n, ou);
+        } else {
+            for (int u = 0; u < n; u++) {
+                const A v = widen(d[u]), gate = zr[u], up = zr[n + u];
+                out[u] = round_to<T>(v * up * gate_slope<GATE>(gate));
+                out[n + u] = round_to<T>(v * gate_value<GATE>(gate));
+            }
+        }
+    }
+}
+
+// C (+)= A . B by the kernels of the plain products, their partial sums in memory of this stream's own; where k would be split and there is no memory for that, as one group of all rows
+static int product(void* C, const void* A, const void* B, const void* bias, int m, int k, int n, long long a_rs, long long a_cs, long long b_rs, long long b_cs, long long c_rs, int accumulate, int dtype) {
+    int rc;
+    bool refused;
+    {
+        const CallScratch memory(CallScratch::MOST);
+        const GemmWorkspaceLoan loan(memory.ptr, CallScratch::MOST);
+        rc = rp_hip_gemm_strided_batched(C, A, B, bias, 1, m, k, n, 0, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, 1, accumulate, dtype);
+        refused = loan.refused;
+    }
+    if (refused) rc = launch_grouped_rows(GroupedArgs{C, A, B, bias, nullptr, RowGroups{nullptr, nullptr, 1, m, 1}, k, n, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, accumulate ? ACCUMULATE : 0}, dtype);
+    return rc;
+}
+
+// float32 and float64: z by a plain product, then h.  Without room for z, as many rows at a time as the stream's own memory holds.
+template <typename T>
+static int launch_gated_by_product(const GatedArgs& g, int dtype, bool* taken) {
+    using A = typename traits<T>::acc;
+    auto values = [&](void* h, const void* z, int rows) {
+        const int across = (g.n + 255) / 256;
+        const long long blocks = (long long)rows * across;
+        RP_DISPATCH_GATE(g.gate, hipLaunchKernelGGL((gated_value_kernel<T, GATE>), dim3((unsigned)(blocks < GATED_GRID ? blocks : GATED_GRID)), dim3(256), 0, current_stream(), (T*)h, (const A*)z, rows, g.n, g.h_rs, across));
+        return check_launch("gated_value_kernel") ? 0 : -1;
+    };
+    *taken = true;
+    if (g.z) {
+        if (product(g.z, g.x, g.w, g.bias, g.rows, g.k, 2 * g.n, g.x_rs, g.x_cs, g.w_rs, g.w_cs, 2ll * g.n, 0, dtype) != 0) return -1;
+        return values(g.h, g.z, g.rows);
+    }
+    // (the memory's other half is for the product's own partial sums)
+    constexpr size_t HALF = CallScratch::MOST / 2;
+    const long long most = (long long)(HALF / (2 * (size_t)g.n * sizeof(A)));
+    if (most < 1) { *taken = false; return 0; }
+    const int chunk = most < g.rows ? (int)most : g.rows;
+    const CallScratch memory(CallScratch::MOST);
+    if (!memory.ptr) { *taken = false; return 0; }
+    for (int row = 0; row < g.rows; row += chunk) {
+        const int rows = g.rows - row < chunk ? g.rows - row : chunk;
+        const T* x = (const T*)g.x + row * g.x_rs;
+        bool refused;
+        int rc;
+        {
+            const GemmWorkspaceLoan loan((char*)memory.ptr + HALF, HALF);
+            rc = rp_hip_gemm_strided_batched(memory.ptr, x, g.w, g.bias, 1, rows, g.k, 2 * g.n, 0, g.x_rs, g.x_cs, 0, g.w_rs, g.w_cs, 0, 2ll * g.n, 1, 0, dtype);
+            refused = loan.refused;
+        }
+        if (refused) rc = launch_grouped_rows(GroupedArgs{memory.ptr, x, g.w, g.bias, nullptr, RowGroups{nullptr, nullptr, 1, rows, 1}, g.k, 2 * g.n, g.x_rs, g.x_cs, 0, g.w_rs, g.w_cs, 0, 2ll * g.n, 0}, dtype);
+        if (rc != 0 || values((T*)g.h + row * g.h_rs, memory.ptr, rows) != 0) return -1;
+    }
+    return 0;
+}
+
+static bool gated_args_ok(const char* who, bool pointers, int rows, int k, int n, int gate, std::initializer_list<long long> strides, int dtype) {
+    if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 30) || n > (1 << 29)) {
+        set_error("%s: null operand, non-positive extent, more than 2^30 rows or 2^29 columns (rows=%d k=%d n=%d)", who, rows, k, n);
+        return false;
+    }
+    if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
+    if (gate < RP_GATE_SILU || gate > RP_GATE_SIGMOID) { set_error("%s: unknown gate %d", who, gate); return false; }
+    for (long long s : strides)
+        if (s < 0) { set_error("%s: negative stride", who); return false; }
+    return true;
+}
+static bool gated_rows_apart(const char* who, const char* what, int rows, int width, long long rs) {
+    if (rows == 1 || rs >= width) return true;
+    set_error("%s: rows of %s are %lld elements apart and hold %d", who, what, rs, width);
+    return false;
+}
+
+}  // namespace rp
+
+using namespace rp;
+
+extern "C" {
+
+int rp_hip_gated_linear_forward(void* h, void* z, const void* x, const void* w, const void* bias, int rows, int k, int n, int gate,
+                                long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long h_rs, int dtype) {
+    const char* who = "rp_hip_gated_linear_forward";
+    if (!gated_args_ok(who, h && x && w, rows, k, n, gate, {x_rs, x_cs, w_rs, w_cs, h_rs}, dtype) || !gated_rows_apart(who, "h", rows, n, h_rs)) return -1;
+    const GatedArgs g{h, z, x, w, bias, rows, k, n, gate, x_rs, x_cs, w_rs, w_cs, h_rs};
+    if (dtype == RP_DTYPE_FLOAT32 || dtype == RP_DTYPE_FLOAT64) {
+        bool taken;
+        const int rc = dtype == RP_DTYPE_FLOAT32 ? launch_gated_by_product<float>(g, dtype, &taken) : launch_gated_by_product<double>(g, dtype, &taken);
+        if (rc != 0 || taken) return rc;
+    }
+    RP_DISPATCH_DTYPE(dtype, return launch_gated_any<T>(g));
+    return -1;
+}
+
+int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const void* dh, const void* z, const void* x, const void* w, int rows, int k, int n, int gate,
+                                 long long dh_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs, long long dw_rs, long long dw_cs,
+                                 int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype) {
+    const char* who = "rp_hip_gated_linear_backward";
+    if (!gated_args_ok(who, dz && dh && z && (!dx || w) && (!dw || x), rows, k, n, gate, {dh_rs, x_rs, x_cs, w_rs, w_cs, dx_rs, dw_rs, dw_cs}, dtype)) return -1;
+    if (dx && !gated_rows_apart(who, "dx", rows, k, dx_rs)) return -1;
+    if (dw && !(dw_cs == 1 && (k == 1 || dw_rs >= 2ll * n)) && !(dw_rs == 1 && dw_cs >= k)) { set_error("%s: dw has unit stride along one axis and rows that do not overlap along the other", who); return -1; }
+    RP_DISPATCH_DTYPE(dtype, using A = typename traits<T>::acc;
+        const int across = (n + 256 * vec16<T>::N - 1) / (256 * vec16<T>::N);
+        const long long blocks = (long long)rows * across;
+        RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_dz_kernel<T, GATE>), dim3((unsigned)(blocks < GATED_GRID ? blocks : GATED_GRID)), dim3(256), 0, current_stream(), (T*)dz, (const T*)dh, (const A*)z, rows, n, dh_rs, across));
+        if (!check_launch("gated_dz_kernel")) return -1);
+    if (dx && product(dx, dz, w, nullptr, rows, 2 * n, k, 2ll * n, 1, w_cs, w_rs, dx_rs, accumulate_dx, dtype) != 0) return -1;
+    if (dw) {
+        // (a transposed dW is the transposed product)
+        const int rc = dw_cs == 1 ? product(dw, x, dz, nullptr, k, rows, 2 * n, x_cs, x_rs, 2ll * n, 1, dw_rs, accumulate_dw, dtype)
+                                  : product(dw, dz, x, nullptr, 2 * n, rows, k, 1, 2ll * n, x_rs, x_cs, dw_cs, accumulate_dw, dtype);
+        if (rc != 0) return -1;
+    }
+    return db ? rp_hip_reduce_rows(db, dz, rows, 2 * n, accumulate_db, dtype) : 0;
+}
+
+}  // extern "C"

@@ -39,6 +39,8 @@ __device__ __forceinline__ TileCoord chunk_tile(int at, int rows, int cols) {
 // Which operand is in the accumulate type (float32, float64 for float64) whatever the tensors' type is: the low-rank activations of an adapter
 enum GroupedLow { LOW_A, LOW_B };
 
+// By rows, on the kernel that suits the sizes (rp_grouped.hip)
+int launch_grouped_rows(const GroupedArgs& g, int dtype);
 // Any strides and sizes, all types (rp_grouped_generic.hip); low: A is.  No scales; by weights: no ids.
 int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype);
 int launch_grouped_weights_generic(const GroupedArgs& g, int dtype);

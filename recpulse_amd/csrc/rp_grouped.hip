@@ -63,6 +63,8 @@ static int grouped_rows(const GroupedArgs& g, int dtype) {
     return launch_grouped_rows_generic(g, false, dtype);
 }
 
+int launch_grouped_rows(const GroupedArgs& g, int dtype) { return grouped_rows(g, dtype); }
+
 static int grouped_weights(const GroupedArgs& g, int dtype) {
     const Tile16 t = weights_tile16(g, dtype);
     if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_grouped_weights16_256_bf16(g) : launch_grouped_weights16_256_f16(g);

@@ -1,0 +1,97 @@
+// Rows that a team of threads holds in registers (layer norm, distillation, the losses of a large vocabulary): a thread's 16-byte vectors of a row, and sums over
+// a wave or a workgroup in a fixed order.
+#pragma once
+#include "rp_rows.h"
+
+#include <type_traits>
+
+namespace rp {
+
+template <typename T> struct vec16 { static constexpr int N = 16 / sizeof(T); };
+// (rows may start at any element)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) any16 { unsigned int v[4]; };
+
+// A thread's vector number `e0` .. of a row of d >= N elements.  The last one of a row whose length is no whole number of vectors is loaded so that it ends with
+// the row, and a thread behind the row's end loads the last one too (no load is out of range, none behind a branch): elements from `skip` on are the thread's own.
+template <typename T> struct RowVector {
+    static constexpr int N = vec16<T>::N;
+    int at, skip;
+    __device__ __forceinline__ RowVector() : at(0), skip(N) {}
+    __device__ __forceinline__ RowVector(int e0, int d) {
+        at = e0 < d - N ? e0 : d - N;
+        skip = e0 - at < N ? e0 - at : N;
+    }
+    __device__ __forceinline__ void load(T (&x)[N], const T* row) const {
+        const any16<T> v = *(const any16<T>*)(row + at);
+        __builtin_memcpy(x, &v, 16);
+    }
+    __device__ __forceinline__ bool has(int u) const { return u >= skip; }
+    // the thread's own elements, once each
+    __device__ __forceinline__ void store(T* row, const T (&y)[N]) const {
+        if (skip == 0) {
+            any16<T> v;
+            __builtin_memcpy(&v, y, 16);
+            *(any16<T>*)(row + at) = v;
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; u++)
+                if (has(u)) row[at + u] = y[u];
+        }
+    }
+};
+
+// The sum (largest) of a value over the wave, in every lane
+template <typename A> __device__ __forceinline__ A wave_sum(A v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+    return v;
+}
+template <typename A> __device__ __forceinline__ A larger(A a, A b) { return a != a ? a : b != b ? b : a > b ? a : b; }      // NaN is above every number
+template <typename A> __device__ __forceinline__ A wave_max(A v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v = larger(v, __shfl_xor(v, d));
+    return v;
+}
+// ... and over the LANES threads of a team: a wave, or the whole workgroup, which meets twice.  `room`: LANES / 64 values of LDS for each of the N.
+template <int LANES, int N, typename A> __device__ __forceinline__ void team_sums(A (&v)[N], A* room) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        __syncthreads();                           // (the room's last readers are done)
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) room[i * WAVES + threadIdx.x / 64] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = room[i * WAVES];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v[i] += room[i * WAVES + w];
+        }
+    }
+}
+template <int LANES, typename A> __device__ __forceinline__ A team_max(A v, A* room) {
+    v = wave_max(v);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) room[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = room[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) v = larger(v, room[w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float natural_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double natural_exp(double x) { return exp(x); }
+__device__ __forceinline__ float natural_log(float x) { return logf(x); }
+__device__ __forceinline__ double natural_log(double x) { return log(x); }
+
+// x * scale - base with one rounding, so that what a value comes to does not depend on what a compiler joins in one kernel or another
+__device__ __forceinline__ float scaled_less(float x, float scale, float base) { return __builtin_fmaf(x, scale, -base); }
+__device__ __forceinline__ double scaled_less(double x, double scale, double base) { return __builtin_fma(x, scale, -base); }
+
+}  // namespace rp

@@ -1,0 +1,35 @@
+// Cross entropy of a large vocabulary straight from the rows before it: z = x . W + b, loss_i = log sum_v exp(z_iv) - z_it.
+#pragma once
+#include "rp_gemm.h"
+#include "rp_teams.h"
+
+namespace rp {
+
+struct VocabArgs {
+    const void *x, *w, *bias;
+    const int* targets;
+    int rows, k, classes, reduction;
+    long long x_rs, x_cs, w_rs, w_cs;
+};
+struct VocabGrads {
+    void *dx, *dw, *db;
+    long long dx_rs, dw_rs, dw_cs;
+    int accumulate_dx, accumulate_dw, accumulate_db;
+};
+
+// A workspace in pieces of whole 256 bytes: counted with a null base, handed out with the caller's
+class VocabRoom {
+public:
+    explicit VocabRoom(void* base) : base_((char*)base) {}
+    template <typename P> P* take(long long count) {
+        P* at = (P*)(base_ + used_);
+        used_ += (count * (long long)sizeof(P) + 255) / 256 * 256;
+        return at;
+    }
+    long long used() const { return used_; }
+private:
+    char* base_;
+    long long used_ = 0;
+};
+
+}  // namespace rp

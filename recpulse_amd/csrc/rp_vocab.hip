@@ -1,0 +1,285 @@
+// Entry points of the cross entropy of a large vocabulary, and its pieces for any strides, sizes and types.
+//
+//   z = x . W + b;  m, s: the row's running largest and sum of exp(z - m);  loss_i = m + log s - z[i, t_i]
+//   d[i, v] = (exp(z[i, v] - lse_i) - [v = t_i]) f_i,  dx = d . W^T,  dW = x^T . d,  db = sum of d over the rows
+//
+// f_i: the upstream gradient, for the mean over the rows with a target divided by their number, 0 for a row without one.  The kernels here take a piece of the vocabulary at a
+// time through the plain products in the accumulate type: 16-bit operands are widened first.
+#include "rp_vocab.h"
+
+namespace rp {
+
+constexpr long long VOCAB_PIECE_BYTES = 64ll << 20;      // of a piece's logits
+constexpr size_t VOCAB_GEMM_BYTES = 16 << 20;            // for the partial sums of its products
+constexpr int VOCAB_GRID = 1 << 20;
+
+static int vocab_piece(int rows, int classes, int elem, long long bytes) {
+    const long long fits = bytes / ((long long)rows * elem) / 256 * 256, all = (classes + 255ll) / 256 * 256;
+    return (int)(fits < 256 ? 256 : fits < all ? fits : all);
+}
+
+// ---- kernels of the pieces ----
+
+// out[i, j] dense = in[i, j] widened
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_widen_kernel(typename traits<T>::acc* out, const T* in, int rows, int cols, long long rs, long long cs) {
+    const long long total = (long long)rows * cols;
+    for (long long id = blockIdx.x * 256ll + threadIdx.x; id < total; id += gridDim.x * 256ll) {
+        // neighbouring threads along the axis with the smaller stride
+        const int i = (int)(cs <= rs ? id / cols : id % rows), j = (int)(cs <= rs ? id % cols : id / rows);
+        out[(long long)i * cols + j] = widen(in[i * rs + j * cs]);
+    }
+}
+// out[i, j] (+)= in[i, j] dense, rounded
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_round_kernel(T* out, const typename traits<T>::acc* in, int rows, int cols, long long rs, long long cs, int accumulate) {
+    const long long total = (long long)rows * cols;
+    for (long long id = blockIdx.x * 256ll + threadIdx.x; id < total; id += gridDim.x * 256ll) {
+        const int i = (int)(cs <= rs ? id / cols : id % rows), j = (int)(cs <= rs ? id % cols : id / rows);
+        T* at = out + i * rs + j * cs;
+        const auto v = in[(long long)i * cols + j];
+        *at = round_to<T>(accumulate ? widen(*at) + v : v);
+    }
+}
+static unsigned flat_grid(long long total) {
+    const long long blocks = (total + 255) / 256;
+    return (unsigned)(blocks < VOCAB_GRID ? blocks : VOCAB_GRID);
+}
+
+// The piece's share of each row's running largest logit, sum and target's logit: state [rows][3]
+template <typename A>
+__global__ void __launch_bounds__(256) vocab_state_kernel(A* state, const A* z, const int* targets, int rows, int width, int v0, int first) {
+    __shared__ A room[8];
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const A* zr = z + (long long)row * width;
+        A* st = state + 3ll * row;
+        A top = first ? -(A)INFINITY : st[0];
+        const A was = top;
+        for (int c = threadIdx.x; c < width; c += 256) top = larger(top, zr[c]);
+        top = team_max<256>(top, room);
+        const A base = top == -(A)INFINITY ? (A)0 : top;
+        A sum[1] = {};
+        for (int c = threadIdx.x; c < width; c += 256) sum[0] += natural_exp(zr[c] - base);
+        team_sums<256>(sum, room + 4);
+        if (threadIdx.x == 0) {
+            st[1] = (first || was == -(A)INFINITY ? (A)0 : st[1] * natural_exp(was - base)) + sum[0];
+            st[0] = top;
+            const int t = targets[row] - v0;
+            if (targets[row] >= 0 && t >= 0 && t < width) st[2] = zr[t];
+        }
+        __syncthreads();
+    }
+}
+// lse and loss of each row from its state
+template <typename A>
+__global__ void __launch_bounds__(256) vocab_rows_kernel(A* stats, const A* state, const int* targets, int rows, int classes) {
+    for (int row = (int)(blockIdx.x * 256 + threadIdx.x); row < rows; row += (int)gridDim.x * 256) {
+        const A* st = state + 3ll * row;
+        const A lse = st[0] == -(A)INFINITY ? st[0] : st[0] + natural_log(st[1]);
+        stats[row] = lse;
+        stats[rows + row] = targets[row] >= 0 && targets[row] < classes ? lse - st[2] : (A)0;
+    }
+}
+// The result, and how many rows have a target: one workgroup, in double, whose threads' sums are added in order
+template <typename A>
+__global__ void __launch_bounds__(1024) vocab_loss_kernel(A* out, A* stats, const int* targets, int rows, int classes, int reduction) {
+    __shared__ double room[32];
+    double sums[2] = {};
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        sums[0] += (double)stats[rows + i];
+        sums[1] += targets[i] >= 0 && targets[i] < classes ? 1.0 : 0.0;
+        if (reduction == 0) out[i] = stats[rows + i];
+    }
+    team_sums<1024>(sums, room);
+    if (threadIdx.x) return;
+    stats[2ll * rows] = (A)sums[1];
+    if (reduction) out[0] = (A)(reduction == 1 ? sums[0] / (sums[1] > 0 ? sums[1] : 1.0) : sums[0]);
+}
+
+template <typename A> __device__ __forceinline__ A vocab_factor(const A* stats, const A* upstream, const int* targets, int row, int rows, int classes, int reduction) {
+    if (targets[row] < 0 || targets[row] >= classes) return (A)0;
+    A f = upstream ? upstream[reduction == 0 ? row : 0] : (A)1;
+    if (reduction == 1) f /= stats[2ll * rows];
+    return f;
+}
+// z of a piece becomes d
+template <typename A>
+__global__ void __launch_bounds__(256) vocab_d_kernel(A* z, const A* stats, const A* upstream, const int* targets, int rows, int width, int v0, int classes, int reduction) {
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const A f = vocab_factor(stats, upstream, targets, row, rows, classes, reduction), lse = stats[row];
+        const bool held = targets[row] >= 0 && targets[row] < classes;
+        const int t = held ? targets[row] - v0 : -1;
+        A* zr = z + (long long)row * width;
+        for (int c = threadIdx.x; c < width; c += 256) zr[c] = held ? (natural_exp(zr[c] - lse) - (c == t ? (A)1 : (A)0)) * f : (A)0;
+    }
+}
+
+// ---- any strides, sizes and types ----
+
+template <typename T> struct VocabAnyRoom {
+    using A = typename traits<T>::acc;
+    static constexpr bool WIDE = sizeof(T) != sizeof(A);          // operands that are widened first
+    int piece;
+    A *state, *z, *x, *w, *bias, *dx, *dw, *db;
+    char* gemm;
+    VocabAnyRoom(VocabRoom& room, int rows, int k, int classes, bool backward) {
+        piece = vocab_piece(rows, classes, sizeof(A), VOCAB_PIECE_BYTES);
+        state = room.take<A>(3ll * rows);
+        z = room.take<A>((long long)rows * piece);
+        gemm = room.take<char>(VOCAB_GEMM_BYTES);
+        x = w = bias = dx = dw = db = nullptr;
+        if (!WIDE) return;
+        x = room.take<A>((long long)rows * k);
+        w = room.take<A>((long long)k * piece);
+        bias = room.take<A>(piece);
+        if (!backward) return;
+        dx = room.take<A>((long long)rows * k);
+        dw = room.take<A>((long long)k * piece);
+        db = room.take<A>(piece);
+    }
+};
+
+struct VocabProduct {
+    void* room;
+    int dtype;
+    int operator()(void* C, const void* A, const void* B, const void* bias, int m, int k, int n, long long a_rs, long long a_cs, long long b_rs, long long b_cs, long long c_rs, int accumulate) const {
+        const GemmWorkspaceLoan loan(room, VOCAB_GEMM_BYTES);
+        return rp_hip_gemm_strided_batched(C, A, B, bias, 1, m, k, n, 0, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, 1, accumulate, dtype);
+    }
+};
+
+// piece by piece: f(first class, classes, logits with unit column stride and rows as long as the piece)
+template <typename T, typename F>
+static int vocab_pieces(const VocabArgs& g, const VocabAnyRoom<T>& r, const VocabProduct& product, F f) {
+    using A = typename traits<T>::acc;
+    const void* x = g.x;
+    long long x_rs = g.x_rs, x_cs = g.x_cs;
+    if constexpr (VocabAnyRoom<T>::WIDE) {
+        hipLaunchKernelGGL((vocab_widen_kernel<T>), dim3(flat_grid((long long)g.rows * g.k)), dim3(256), 0, current_stream(), r.x, (const T*)g.x, g.rows, g.k, g.x_rs, g.x_cs);
+        if (!check_launch("vocab_widen_kernel")) return -1;
+        x = r.x;
+        x_rs = g.k;
+        x_cs = 1;
+    }
+    for (int v0 = 0; v0 < g.classes; v0 += r.piece) {
+        const int width = g.classes - v0 < r.piece ? g.classes - v0 : r.piece;
+        const void *w = (const T*)g.w + v0 * g.w_cs, *bias = g.bias ? (const T*)g.bias + v0 : nullptr;
+        long long w_rs = g.w_rs, w_cs = g.w_cs;
+        if constexpr (VocabAnyRoom<T>::WIDE) {
+            hipLaunchKernelGGL((vocab_widen_kernel<T>), dim3(flat_grid((long long)g.k * width)), dim3(256), 0, current_stream(), r.w, (const T*)w, g.k, width, g.w_rs, g.w_cs);
+            if (!check_launch("vocab_widen_kernel")) return -1;
+            w = r.w;
+            w_rs = width;
+            w_cs = 1;
+            if (bias) {
+                hipLaunchKernelGGL((vocab_widen_kernel<T>), dim3(flat_grid(width)), dim3(256), 0, current_stream(), r.bias, (const T*)bias, 1, width, 0ll, 1ll);
+                if (!check_launch("vocab_widen_kernel")) return -1;
+                bias = r.bias;
+            }
+        }
+        if (product(r.z, x, w, bias, g.rows, g.k, width, x_rs, x_cs, w_rs, w_cs, width, 0) != 0) return -1;
+        if (f(v0, width, (A*)r.z, (const A*)x, x_rs, x_cs, (const A*)w, w_rs, w_cs) != 0) return -1;
+    }
+    return 0;
+}
+
+template <typename T>
+static int vocab_any_forward(void* loss_out, void* stats, const VocabArgs& g, void* workspace) {
+    using A = typename traits<T>::acc;
+    VocabRoom room(workspace);
+    const VocabAnyRoom<T> r(room, g.rows, g.k, g.classes, false);
+    const int rc = vocab_pieces<T>(g, r, VocabProduct{r.gemm, traits<A>::code}, [&](int v0, int width, A* z, const A*, long long, long long, const A*, long long, long long) {
+        hipLaunchKernelGGL((vocab_state_kernel<A>), dim3(g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID), dim3(256), 0, current_stream(), r.state, (const A*)z, g.targets, g.rows, width, v0, v0 == 0);
+        return check_launch("vocab_state_kernel") ? 0 : -1;
+    });
+    if (rc != 0) return -1;
+    hipLaunchKernelGGL((vocab_rows_kernel<A>), dim3(flat_grid(g.rows)), dim3(256), 0, current_stream(), (A*)stats, (const A*)r.state, g.targets, g.rows, g.classes);
+    if (!check_launch("vocab_rows_kernel")) return -1;
+    hipLaunchKernelGGL((vocab_loss_kernel<A>), dim3(1), dim3(1024), 0, current_stream(), (A*)loss_out, (A*)stats, g.targets, g.rows, g.classes, g.reduction);
+    return check_launch("vocab_loss_kernel") ? 0 : -1;
+}
+
+template <typename T>
+static int vocab_any_backward(const VocabGrads& o, const VocabArgs& g, const void* stats, const void* upstream, void* workspace) {
+    using A = typename traits<T>::acc;
+    constexpr bool WIDE = VocabAnyRoom<T>::WIDE;
+    VocabRoom room(workspace);
+    const VocabAnyRoom<T> r(room, g.rows, g.k, g.classes, true);
+    const VocabProduct product{r.gemm, traits<A>::code};
+    auto rounded = [&](void* out, const A* in, int rows, int cols, long long rs, long long cs, int accumulate) {
+        hipLaunchKernelGGL((vocab_round_kernel<T>), dim3(flat_grid((long long)rows * cols)), dim3(256), 0, current_stream(), (T*)out, in, rows, cols, rs, cs, accumulate);
+        return check_launch("vocab_round_kernel") ? 0 : -1;
+    };
+    const int rc = vocab_pieces<T>(g, r, product, [&](int v0, int width, A* z, const A* x, long long x_rs, long long x_cs, const A* w, long long w_rs, long long w_cs) {
+        hipLaunchKernelGGL((vocab_d_kernel<A>), dim3(g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID), dim3(256), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
+        if (!check_launch("vocab_d_kernel")) return -1;
+        if (o.dx && product(WIDE ? (void*)r.dx : o.dx, z, w, nullptr, g.rows, width, g.k, width, 1, w_cs, w_rs, WIDE ? g.k : o.dx_rs, v0 ? 1 : WIDE ? 0 : o.accumulate_dx) != 0) return -1;
+        if (o.dw) {
+            char* dw = (char*)o.dw + v0 * o.dw_cs * (long long)sizeof(T);
+            if (WIDE) {
+                if (product(r.dw, x, z, nullptr, g.k, g.rows, width, x_cs, x_rs, width, 1, width, 0) != 0 || rounded(dw, r.dw, g.k, width, o.dw_rs, o.dw_cs, o.accumulate_dw) != 0) return -1;
+            } else if (o.dw_cs == 1) {
+                if (product(dw, x, z, nullptr, g.k, g.rows, width, x_cs, x_rs, width, 1, o.dw_rs, o.accumulate_dw) != 0) return -1;
+            } else if (product(dw, z, x, nullptr, width, g.rows, g.k, 1, width, x_rs, x_cs, o.dw_cs, o.accumulate_dw) != 0) return -1;      // the transposed product
+        }
+        if (o.db) {
+            if (WIDE) return rp_hip_reduce_rows(r.db, z, g.rows, width, 0, traits<A>::code) != 0 ? -1 : rounded((T*)o.db + v0, r.db, 1, width, 0, 1, o.accumulate_db);
+            return rp_hip_reduce_rows((T*)o.db + v0, z, g.rows, width, o.accumulate_db, traits<A>::code);
+        }
+        return 0;
+    });
+    if (rc != 0) return -1;
+    return WIDE && o.dx ? rounded(o.dx, r.dx, g.rows, g.k, o.dx_rs, 1, o.accumulate_dx) : 0;
+}
+
+static bool vocab_args_ok(const char* who, bool pointers, int rows, int k, int classes, int reduction, std::initializer_list<long long> strides, int dtype) {
+    if (!pointers || rows <= 0 || k <= 0 || classes <= 0 || rows > (1 << 30) || classes > (1 << 30)) {
+        set_error("%s: null operand, non-positive extent, more than 2^30 rows or classes (rows=%d k=%d classes=%d)", who, rows, k, classes);
+        return false;
+    }
+    if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
+    if (reduction < 0 || reduction > 2) { set_error("%s: reduction must be none (0), mean (1) or sum (2)", who); return false; }
+    for (long long s : strides)
+        if (s < 0) { set_error("%s: negative stride", who); return false; }
+    return true;
+}
+
+}  // namespace rp
+
+using namespace rp;
+
+extern "C" {
+
+long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, int backward, int dtype) {
+    if (!vocab_args_ok("rp_hip_linear_cross_entropy_workspace", true, rows, k, classes, 0, {}, dtype)) return -1;
+    VocabRoom room(nullptr);
+    RP_DISPATCH_DTYPE(dtype, const VocabAnyRoom<T> r(room, rows, k, classes, backward != 0); (void)r);
+    return room.used();
+}
+
+int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,
+                                        long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype) {
+    if (!vocab_args_ok("rp_hip_linear_cross_entropy_forward", loss_out && stats && x && w && targets && workspace, rows, k, classes, reduction, {x_rs, x_cs, w_rs, w_cs}, dtype)) return -1;
+    const VocabArgs g{x, w, bias, targets, rows, k, classes, reduction, x_rs, x_cs, w_rs, w_cs};
+    RP_DISPATCH_DTYPE(dtype, return vocab_any_forward<T>(loss_out, stats, g, workspace));
+    return -1;
+}
+
+int rp_hip_linear_cross_entropy_backward(void* dx, void* dw, void* db, const void* x, const void* w, const void* bias, const int* targets, const void* stats, const void* upstream_dev, void* workspace,
+                                         int rows, int k, int classes, int reduction, long long x_rs, long long x_cs, long long w_rs, long long w_cs,
+                                         long long dx_rs, long long dw_rs, long long dw_cs, int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype) {
+    const char* who = "rp_hip_linear_cross_entropy_backward";
+    if (!vocab_args_ok(who, x && w && targets && stats && workspace, rows, k, classes, reduction, {x_rs, x_cs, w_rs, w_cs, dx_rs, dw_rs, dw_cs}, dtype)) return -1;
+    if (dx && rows > 1 && dx_rs < k) { set_error("%s: rows of dx are %lld elements apart and hold %d", who, dx_rs, k); return -1; }
+    if (dw && !(dw_cs == 1 && (k == 1 || dw_rs >= classes)) && !(dw_rs == 1 && (classes == 1 || dw_cs >= k))) {
+        set_error("%s: dw has unit stride along one axis and rows that do not overlap along the other", who);
+        return -1;
+    }
+    if (!dx && !dw && !db) return 0;
+    const VocabArgs g{x, w, bias, targets, rows, k, classes, reduction, x_rs, x_cs, w_rs, w_cs};
+    const VocabGrads o{dx, dw, db, dx_rs, dw_rs, dw_cs, accumulate_dx, accumulate_dw, accumulate_db};
+    RP_DISPATCH_DTYPE(dtype, return vocab_any_backward<T>(o, g, stats, upstream_dev, workspace));
+    return -1;
+}
+
+}  // extern "C"
