@@ -20,7 +20,7 @@ struct AdapterTileArgs {
     AdapterTerm term;
 };
 
-struct AdapterTiles {
+struct AdapterTiles : M16Source {
     static constexpr bool MOVES = false, ONCE = true, TERM = true;
     bool odd = false;              // the wave met an infinity or NaN in b
 

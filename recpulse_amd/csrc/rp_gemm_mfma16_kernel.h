@@ -176,8 +176,12 @@ typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)))
 // Where a workgroup's tiles come from and what else they may do.  M16Plain: the schedule of one matrix of the batch, the reference's roundings.
 // Another source may have MOVES: its `tile` points `g` at the matrix that slot `tile_id` belongs to and answers with the tile's
 // coordinates in it; ONCE: the sum and the bias of its column are rounded together, to nearest even; TERM: `add_term` gives a wave's sums
-// what they start from, and `finish` comes after its rows are stored.
-struct M16Plain { static constexpr bool MOVES = false, ONCE = false, TERM = false; };
+// what they start from, and `finish` comes after its rows are stored.  SCALED: a number that `scale` has is multiplied into the sums before that.
+// PAIRED: B is two matrices of `pair` columns side by side, and a tile is BM rows and BN / 2 columns of each: the first half of a wave's patch (WN / 2 columns) belongs to the
+// first matrix, the other half to the same columns of the second, so that both values of a column are in one lane's registers.
+// TAKES: `take` may have the sums instead of the epilogue here: it answers whether it did.  Its first barrier comes before it touches LDS, and the next tile's first store to LDS comes after a barrier.
+struct M16Source { static constexpr bool MOVES = false, ONCE = false, TERM = false, SCALED = false, PAIRED = false, TAKES = false; };
+struct M16Plain : M16Source {};
 
 // What one workgroup does: slots first_slot, first_slot + stride, ... of the schedule of matrix z
 template <typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE, bool SPLITK, int PF, typename SRC = M16Plain>
@@ -210,7 +214,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
     if constexpr (SRC::MOVES) tc = source->tile(tile_id, g);
     else tc = schedule_tile(tile_id, tiles_m, tiles_n);
     if (!tc.valid) continue;
-    const int m0 = tc.tm * BM, n0 = tc.tn * BN;
+    const int m0 = tc.tm * BM, n0 = tc.tn * (SRC::PAIRED ? BN / 2 : BN);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
     // k range of this block: all of k, or the z-th split of it
@@ -246,6 +250,9 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
         }
     };
 
+    // PAIRED: tile column r is column pair_column(r) behind n0 of matrix pair_half(r)
+    auto pair_column = [](int r) { return r / WN * (WN / 2) + r % (WN / 2); };
+    auto pair_half = [](int r) { return r % WN / (WN / 2); };
     // Per-thread piece offsets (bytes from the slab pointer).  The buffer descriptor ends at the operand's last
     // element, which zero-fills rows past the free extent (KC) or k past the end (MC); the other axis of each
     // layout is masked explicitly by swapping in an offset no descriptor covers.
@@ -264,7 +271,12 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
     for (int i = 0; i < NB; i++) {
         int r = b_r0 + (B_MC ? 0 : i * MapB::PIECE_ROWS), kk = b_kk0 + (B_MC ? i * MapB::PIECE_ROWS : 0);
         b_goff[i] = (uint32_t)(((long long)r * b_fs + (long long)kk * b_ks) * 2) + BACK;
-        if (EDGE && B_MC && n0 + r >= g.n) b_goff[i] = BUFFER_OOB;
+        if (EDGE && B_MC && !SRC::PAIRED && n0 + r >= g.n) b_goff[i] = BUFFER_OOB;
+        if constexpr (SRC::PAIRED) {
+            const int at = pair_column(r), half = pair_half(r);
+            b_goff[i] = (uint32_t)((((long long)half * source->pair + at) * b_fs + (long long)kk * b_ks) * 2) + BACK;
+            if (EDGE && n0 + at >= source->pair) b_goff[i] = BUFFER_OOB;
+        }
         if (n_segmented) {
             const int j = n0 + r, seg = j / g.seg_n, c = j - seg * g.seg_n;
             const long long at = (long long)(seg / g.seg_w) * g.seg_sh + (long long)(seg % g.seg_w) * g.seg_sw + (long long)c * b_fs + (long long)kk * b_ks;
@@ -288,7 +300,8 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
     int a_pull = 0, b_pull = 0;
     if constexpr (EDGE == M16_RAGGED) {
         const int klast = kend - kbeg - (nslabs - 1) * M16_BK;
-        const int a_in = A_MC ? g.m - m0 - a_r0 : klast - a_kk0, b_in = B_MC ? g.n - n0 - b_r0 : klast - b_kk0;
+        int a_in = A_MC ? g.m - m0 - a_r0 : klast - a_kk0, b_in = B_MC ? g.n - n0 - b_r0 : klast - b_kk0;
+        if constexpr (SRC::PAIRED && B_MC) b_in = source->pair - n0 - pair_column(b_r0);
         a_pull = a_in > 0 && a_in < 8 ? 8 - a_in : 0;
         b_pull = b_in > 0 && b_in < 8 ? 8 - b_in : 0;
     }
@@ -320,7 +333,13 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
     auto load_piece_b = [&](auto setc, auto ic) {
         constexpr int i = decltype(ic)::value, S = decltype(setc)::value;
         if constexpr (!EDGE) {
-            rb[S][i] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, n_segmented ? (int)b_goff[i] : (int)b_goff[0], n_segmented ? 0 : i * b_piece_step, 0);
+            if constexpr (SRC::PAIRED && !B_MC) {
+                constexpr int r = i * MapB::PIECE_ROWS;       // (of 32 rows that start a half's or in it: the same half for all threads)
+                const int step = (int)(((long long)(r % WN / (WN / 2)) * source->pair + r / WN * (WN / 2) + r % (WN / 2)) * b_fs * 2);
+                rb[S][i] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, (int)b_goff[0], step, 0);
+            } else {
+                rb[S][i] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, n_segmented ? (int)b_goff[i] : (int)b_goff[0], n_segmented ? 0 : i * b_piece_step, 0);
+            }
         } else {
             uint32_t off = b_goff[i];
             if (!B_MC && b_kk0 >= kleft) off = BUFFER_OOB;
@@ -515,6 +534,9 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
 
     if constexpr (MT == 16) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the in-place MFMAs above are opaque to the compiler: let the last ones drain before their results are read
     // ---- epilogue ----
+    if constexpr (SRC::TAKES) {
+        if (source->template take<T, MT, WGN, TMI, TNI, EDGE>(acc, smem, m0, n0)) continue;
+    }
     T* C = (T*)g.C + (long long)z * g.c_bs;
     const T* bias = (const T*)g.bias;
     const bool has_bias = bias != nullptr, accum = g.accumulate != 0;
@@ -530,6 +552,9 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
             if constexpr (SRC::ONCE) return round_to<T>(widen(was) + widen(y));
             else return narrow<T>(widen(was) + widen(y));
         };
+        float scale = 1.f;
+        if constexpr (SRC::SCALED) scale = source->scale();
+        auto sum_of = [&](float v) { return SRC::SCALED ? v * scale : v; };
         __syncthreads();                                 // every wave is done with the main loop's LDS
         // (compile-time tile indices: a loop that the compiler declines to unroll would index the accumulators at run
         // time and move all of them to scratch memory for the whole kernel)
@@ -563,7 +588,7 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
                         // accumulator register v: 32 x 32 tiles hold rows 8 * (v / 4) + 4 * (lane / 32) + v % 4, 16 x 16 tiles rows 4 * (lane / 16) + v
                         const int row = MT == 32 ? i * 32 + 8 * (v / 4) + 4 * (lane >> 5) + (v % 4) : i * 16 + 4 * (lane >> 4) + v;
                         T y;
-                        if constexpr (SRC::ONCE) y = round_to<T>(decltype(with_bias)::value ? acc[i][j][v] + bcol : acc[i][j][v]);
+                        if constexpr (SRC::ONCE) y = round_to<T>(decltype(with_bias)::value ? sum_of(acc[i][j][v]) + bcol : sum_of(acc[i][j][v]));
                         else y = narrow<T>(acc[i][j][v]);
                         if constexpr (SRC::ONCE) {
                         } else if constexpr (decltype(row_bias)::value) {

@@ -9,7 +9,7 @@ namespace rp {
 
 // By rows: row tiles never span two groups, and how many there are is known on the device only.  All groups' tiles are one list, group by group.
 template <int BM>
-struct GroupedRowTiles {
+struct GroupedRowTiles : M16Source {
     static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     RowTiles rows;
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) group
 
 // By weights: tile for tile the same in every group, each group's tiles a run for each XCD, so that resident workgroups, each with one tile
 // of every group in turn, all do the same work however uneven the groups are.  The reduction runs over the group's rows; an empty group leaves zeros.
-struct GroupedWeightTiles {
+struct GroupedWeightTiles : M16Source {
     static constexpr bool MOVES = true, ONCE = true, TERM = false;
     GroupedArgs ga;
     int tiles_k, tiles_n, slots;

@@ -183,8 +183,14 @@ static int vocab_pieces(const VocabArgs& g, const VocabAnyRoom<T>& r, const Voca
     return 0;
 }
 
+template <typename A>
+static int vocab_result(void* loss_out, void* stats, const VocabArgs& g) {
+    hipLaunchKernelGGL((vocab_loss_kernel<A>), dim3(1), dim3(1024), 0, current_stream(), (A*)loss_out, (A*)stats, g.targets, g.rows, g.classes, g.reduction);
+    return check_launch("vocab_loss_kernel") ? 0 : -1;
+}
+
 template <typename T>
-static int vocab_any_forward(void* loss_out, void* stats, const VocabArgs& g, void* workspace) {
+static int vocab_any_forward(void* stats, const VocabArgs& g, void* workspace) {
     using A = typename traits<T>::acc;
     VocabRoom room(workspace);
     const VocabAnyRoom<T> r(room, g.rows, g.k, g.classes, false);
@@ -194,9 +200,7 @@ static int vocab_any_forward(void* loss_out, void* stats, const VocabArgs& g, vo
     });
     if (rc != 0) return -1;
     hipLaunchKernelGGL((vocab_rows_kernel<A>), dim3(flat_grid(g.rows)), dim3(256), 0, current_stream(), (A*)stats, (const A*)r.state, g.targets, g.rows, g.classes);
-    if (!check_launch("vocab_rows_kernel")) return -1;
-    hipLaunchKernelGGL((vocab_loss_kernel<A>), dim3(1), dim3(1024), 0, current_stream(), (A*)loss_out, (A*)stats, g.targets, g.rows, g.classes, g.reduction);
-    return check_launch("vocab_loss_kernel") ? 0 : -1;
+    return check_launch("vocab_rows_kernel") ? 0 : -1;
 }
 
 template <typename T>
@@ -254,15 +258,20 @@ long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, in
     if (!vocab_args_ok("rp_hip_linear_cross_entropy_workspace", true, rows, k, classes, 0, {}, dtype)) return -1;
     VocabRoom room(nullptr);
     RP_DISPATCH_DTYPE(dtype, const VocabAnyRoom<T> r(room, rows, k, classes, backward != 0); (void)r);
-    return room.used();
+    const long long tiles = dtype_size(dtype) == 2 ? vocab16_room(rows, k, classes, backward != 0) : 0;
+    return tiles > room.used() ? tiles : room.used();         // (how the operands lie is not known here: room for either way)
 }
 
 int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,
                                         long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype) {
     if (!vocab_args_ok("rp_hip_linear_cross_entropy_forward", loss_out && stats && x && w && targets && workspace, rows, k, classes, reduction, {x_rs, x_cs, w_rs, w_cs}, dtype)) return -1;
     const VocabArgs g{x, w, bias, targets, rows, k, classes, reduction, x_rs, x_cs, w_rs, w_cs};
-    RP_DISPATCH_DTYPE(dtype, return vocab_any_forward<T>(loss_out, stats, g, workspace));
-    return -1;
+    if (vocab16_takes(g, dtype)) {
+        if (vocab16_forward((float*)stats, g, workspace, dtype) != 0) return -1;
+    } else {
+        RP_DISPATCH_DTYPE(dtype, if (vocab_any_forward<T>(stats, g, workspace) != 0) return -1);
+    }
+    return dtype == RP_DTYPE_FLOAT64 ? vocab_result<double>(loss_out, stats, g) : vocab_result<float>(loss_out, stats, g);
 }
 
 int rp_hip_linear_cross_entropy_backward(void* dx, void* dw, void* db, const void* x, const void* w, const void* bias, const int* targets, const void* stats, const void* upstream_dev, void* workspace,
@@ -278,6 +287,7 @@ int rp_hip_linear_cross_entropy_backward(void* dx, void* dw, void* db, const voi
     if (!dx && !dw && !db) return 0;
     const VocabArgs g{x, w, bias, targets, rows, k, classes, reduction, x_rs, x_cs, w_rs, w_cs};
     const VocabGrads o{dx, dw, db, dx_rs, dw_rs, dw_cs, accumulate_dx, accumulate_dw, accumulate_db};
+    if (vocab16_takes(g, dtype)) return vocab16_backward(o, g, (const float*)stats, (const float*)upstream_dev, workspace, dtype);
     RP_DISPATCH_DTYPE(dtype, return vocab_any_backward<T>(o, g, stats, upstream_dev, workspace));
     return -1;
 }

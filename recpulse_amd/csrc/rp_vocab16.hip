@@ -1,0 +1,239 @@
+// bf16 / fp16 cross entropy of a large vocabulary on MFMA tiles: which tiles, in which pieces, and the small launches between the products.
+#include "rp_vocab16.h"
+
+namespace rp {
+
+// A piece's d (2 bytes an element) is written once and read by two products.  The wider the pieces the fewer times dx's sums, 4 bytes an element, are read and written between them, and the
+// fewer the products' last rounds of tiles that leave CUs idle.
+constexpr long long VOCAB16_PIECE_BYTES = 256ll << 20;
+
+// ---- which tiles ----
+
+// How an operand lies: rows of whole 16-byte vectors that start on them, rows of at least a vector that do not overlap, or neither
+enum { LIES_WHOLE, LIES_RAGGED, LIES_NEITHER };
+static int lies16(const void* p, long long row_stride, long long length) {
+    if (length < 8 || row_stride < length || row_stride >= (1ll << 22)) return LIES_NEITHER;
+    return ((uintptr_t)p & 15) || row_stride % 8 || length % 8 ? LIES_RAGGED : LIES_WHOLE;
+}
+static int worse16(int a, int b) { return a > b ? a : b; }
+
+// edge 256, 128 or 64 and what of it may hang over
+struct VocabTile { int edge, over; };
+static VocabTile vocab_tile(int m, int n, int k, bool a_mc, bool b_mc, int lie) {
+    Plan p{FAM_MFMA16, 64, 64, a_mc, b_mc, true, ""};
+    p.ragged = lie == LIES_RAGGED;
+    choose_tile16(p, 1, m, k, n);
+    if (p.ragged) return {p.bm >= 128 && p.bn >= 128 ? 128 : 64, M16_RAGGED};
+    if (p.bm == 256 && p.bn == 256) return {256, m % 256 || n % 256 || k % M16_BK ? M16_EDGE : M16_WHOLE};
+    return {p.bm >= 128 && p.bn >= 128 ? 128 : 64, M16_EDGE};
+}
+
+static int launch_logits(const VocabTileArgs& a, VocabStep step, bool b_mc, int lie, int dtype) {
+    const VocabTile t = vocab_tile(a.g.m, a.g.n, a.g.k, false, b_mc, lie);
+    if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_vocab16_logits_256_bf16(a, step, b_mc, t.over) : launch_vocab16_logits_256_f16(a, step, b_mc, t.over);
+    return t.edge == 128 ? launch_vocab16_logits_128(a, step, b_mc, t.over, dtype) : launch_vocab16_logits_64x128(a, step, b_mc, t.over, dtype);
+}
+static int launch_grads(const VocabTileArgs& a, VocabStep step, bool b_mc, const VocabTile& t, int dtype) {
+    if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_vocab16_grads_256_bf16(a, step, b_mc, t.over) : launch_vocab16_grads_256_f16(a, step, b_mc, t.over);
+    return t.edge == 128 ? launch_vocab16_grads_128(a, step, b_mc, t.over, dtype) : launch_vocab16_grads_64(a, step, b_mc, t.over, dtype);
+}
+// Columns that a wave's patch of logits has on the tile of that edge, rows that a group of db's partial sums has
+static int patch_columns(int edge) { return edge == 256 ? 128 : 64; }
+static int patch_rows(int edge) { return edge == 256 ? 128 : edge == 128 ? 64 : 32; }
+
+static int logits_lie(const VocabArgs& g) {
+    return worse16(lies16(g.x, g.x_rs, g.k), g.w_cs == 1 ? lies16(g.w, g.w_rs, g.classes) : lies16(g.w, g.w_cs, g.k));
+}
+bool vocab16_takes(const VocabArgs& g, int dtype) {
+    if ((dtype != RP_DTYPE_BFLOAT16 && dtype != RP_DTYPE_FLOAT16) || g.x_cs != 1 || (g.w_cs != 1 && g.w_rs != 1) || path_disabled("mfma")) return false;
+    return logits_lie(g) != LIES_NEITHER;
+}
+
+// ---- small launches ----
+
+// A row's log sum and loss from its groups' parts: 64 rows to a workgroup, sixteen waves that take every sixteenth group
+__global__ void __launch_bounds__(1024) vocab16_rows_kernel(float* stats, const VocabPart* parts, const float* hits, const int* targets, int rows, int classes, int groups) {
+    __shared__ VocabPart room[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    for (int row0 = blockIdx.x * 64; row0 < rows; row0 += gridDim.x * 64) {
+        const int row = row0 + lane;
+        float top = -INFINITY, sum = 0.f;
+        if (row < rows)
+            for (int i0 = wave; i0 < groups; i0 += 16 * 8) {
+                VocabPart p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) p[e] = i0 + 16 * e < groups ? parts[(long long)(i0 + 16 * e) * rows + row] : VocabPart{-INFINITY, 0.f};
+                float most = top;
+#pragma unroll
+                for (int e = 0; e < 8; e++) most = fmaxf(most, p[e].top);
+                const float base = most == -INFINITY ? 0.f : most;
+                sum *= exp_less(top, base);
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum += p[e].sum * exp_less(p[e].top, base);
+                top = most;
+            }
+        __syncthreads();
+        room[wave][lane] = VocabPart{top, sum};
+        __syncthreads();
+        if (wave || row >= rows) continue;
+        for (int w = 1; w < 16; w++) top = fmaxf(top, room[w][lane].top);
+        const float base = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+        for (int w = 0; w < 16; w++) sum += room[w][lane].sum * exp_less(room[w][lane].top, base);
+        const float lse = base + logf(sum);
+        stats[row] = lse;
+        stats[rows + row] = targets[row] >= 0 && targets[row] < classes ? lse - hits[row] : 0.f;
+    }
+}
+
+// f of each row times a power of two, and that power's inverse: one workgroup
+__global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* scale, const float* stats, const float* upstream, const int* targets, int rows, int classes, int reduction, int most) {
+    __shared__ float room[16];
+    float top = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        float v = 0.f;
+        if (targets[i] >= 0 && targets[i] < classes) {
+            v = upstream ? upstream[reduction == 0 ? i : 0] : 1.f;
+            if (reduction == 1) v /= stats[2ll * rows];
+        }
+        f[i] = v;
+        top = fmaxf(top, __builtin_isfinite(v) ? fabsf(v) : 0.f);
+    }
+    top = team_max<1024>(top, room);
+    int e = 0;
+    if (top > 0.f) (void)frexpf(top, &e);                     // top is below 2^e
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    const float up = ldexpf(1.f, most - e);
+    for (int i = threadIdx.x; i < rows; i += 1024) f[i] *= up;      // (each thread its own)
+    if (threadIdx.x == 0) *scale = ldexpf(1.f, e - most);
+}
+
+// db of a piece from its groups' sums
+template <typename T>
+__global__ void __launch_bounds__(1024) vocab16_db_kernel(T* db, const float* parts, const float* scale, int groups, long long pitch, int width, int accumulate) {
+    __shared__ float room[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane;
+    float sum = 0.f;
+    if (c < width)
+#pragma unroll 8
+        for (int i = wave; i < groups; i += 16) sum += parts[i * pitch + c];
+    room[wave][lane] = sum;
+    __syncthreads();
+    if (wave || c >= width) return;
+#pragma unroll
+    for (int w = 1; w < 16; w++) sum += room[w][lane];
+    sum *= *scale;
+    db[c] = round_to<T>(accumulate ? widen(db[c]) + sum : sum);
+}
+
+// ---- the workspace ----
+
+struct Vocab16Room {
+    VocabPart* parts;
+    float *hits, *f, *scale, *db_parts, *sums;
+    uint16_t* d;
+    int piece, pitch;
+    Vocab16Room(VocabRoom& room, int rows, int k, int classes, bool backward) {
+        // pieces of whole tiles; a last one of a few classes takes some of those before it (no operand is shorter than a vector)
+        const long long fits = VOCAB16_PIECE_BYTES / (2ll * rows) / 256 * 256, all = (classes + 255ll) / 256 * 256;
+        const long long reach = 1 << 21;                      // (the tiles' 32-bit offsets)
+        piece = pitch = (int)(fits < 256 ? 256 : fits < all ? (fits < reach ? fits : reach) : all < reach ? all : reach);
+        if (!backward) {
+            hits = room.take<float>(rows);
+            parts = room.take<VocabPart>((long long)rows * ((classes + 255ll) / 256 * 4));
+            return;
+        }
+        f = room.take<float>(rows);
+        scale = room.take<float>(1);
+        d = room.take<uint16_t>((long long)rows * pitch);
+        db_parts = room.take<float>(((long long)rows + 255) / 256 * 8 * pitch);
+        sums = room.take<float>(classes > piece ? (rows + 255ll) / 256 * 256 * ((k + 255ll) / 256 * 256) : 0);
+        hits = nullptr;
+        parts = nullptr;
+    }
+    int width(int v0, int classes) const {
+        const int left = classes - v0;
+        return left <= piece ? left : left < piece + 64 ? piece - 128 : piece;
+    }
+};
+
+long long vocab16_room(int rows, int k, int classes, bool backward) {
+    VocabRoom forward(nullptr), both(nullptr);
+    const Vocab16Room f(forward, rows, k, classes, false), b(both, rows, k, classes, true);
+    (void)f;
+    (void)b;
+    return backward && both.used() > forward.used() ? both.used() : forward.used();      // (one workspace does for both passes)
+}
+
+// ---- the passes ----
+
+int vocab16_forward(float* stats, const VocabArgs& g, void* workspace, int dtype) {
+    VocabRoom room(workspace);
+    const Vocab16Room r(room, g.rows, g.k, g.classes, false);
+    const bool b_mc = g.w_cs == 1;
+    const int lie = logits_lie(g);
+    VocabTileArgs a{};
+    a.g = GemmArgs{nullptr, g.x, g.w, g.bias, 1, g.rows, g.k, g.classes, 0, g.x_rs, 1, 0, g.w_rs, g.w_cs};
+    a.targets = g.targets;
+    a.classes = g.classes;
+    a.parts = r.parts;
+    a.hits = r.hits;
+    if (launch_logits(a, VOCAB_FORWARD, b_mc, lie, dtype) != 0) return -1;
+    const int edge = vocab_tile(g.rows, g.classes, g.k, false, b_mc, lie).edge, bn = edge == 256 ? 256 : 128, groups = (g.classes + bn - 1) / bn * (bn / patch_columns(edge));
+    const int blocks = (g.rows + 63) / 64;
+    hipLaunchKernelGGL(vocab16_rows_kernel, dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(1024), 0, current_stream(), stats, r.parts, r.hits, g.targets, g.rows, g.classes, groups);
+    return check_launch("vocab16_rows_kernel") ? 0 : -1;
+}
+
+int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats, const float* upstream, void* workspace, int dtype) {
+    VocabRoom room(workspace);
+    const Vocab16Room r(room, g.rows, g.k, g.classes, true);
+    const bool tied = g.w_cs != 1;                            // W is the transpose of [classes, k] rows
+    const int lie = logits_lie(g);
+    // dx on the same tiles for every piece (their sums lie by tile); all but the last piece are whole slabs
+    const int longest = g.classes < r.piece ? g.classes : r.piece;
+    VocabTile dx_tile = vocab_tile(g.rows, g.k, longest, false, tied, worse16(lie, g.classes % 8 ? LIES_RAGGED : LIES_WHOLE));
+    if (dx_tile.over == M16_WHOLE && g.classes % M16_BK) dx_tile.over = M16_EDGE;
+    hipLaunchKernelGGL(vocab16_factors_kernel, dim3(1), dim3(1024), 0, current_stream(), r.f, r.scale, stats, upstream, g.targets, g.rows, g.classes, g.reduction, dtype == RP_DTYPE_FLOAT16 ? 14 : 0);
+    if (!check_launch("vocab16_factors_kernel")) return -1;
+    for (int v0 = 0, width; v0 < g.classes; v0 += width) {
+        width = r.width(v0, g.classes);
+        const char *w = (const char*)g.w + 2 * v0 * g.w_cs, *bias = g.bias ? (const char*)g.bias + 2ll * v0 : nullptr;
+        VocabTileArgs a{};
+        a.g = GemmArgs{nullptr, g.x, w, bias, 1, g.rows, g.k, width, 0, g.x_rs, 1, 0, g.w_rs, g.w_cs};
+        a.targets = g.targets;
+        a.v0 = v0;
+        a.classes = g.classes;
+        a.d = r.d;
+        a.pitch = r.pitch;
+        a.lse = stats;
+        a.f = r.f;
+        a.db_parts = o.db ? r.db_parts : nullptr;
+        const int piece_lie = worse16(lie, g.w_cs == 1 && width % 8 ? LIES_RAGGED : LIES_WHOLE);
+        if (launch_logits(a, VOCAB_GRADIENT, !tied, piece_lie, dtype) != 0) return -1;
+        if (o.db) {
+            const int edge = vocab_tile(g.rows, width, g.k, false, !tied, piece_lie).edge, groups = (g.rows + patch_rows(edge) - 1) / patch_rows(edge);
+            RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vocab16_db_kernel<T>), dim3((width + 63) / 64), dim3(1024), 0, current_stream(), (T*)o.db + v0, r.db_parts, r.scale, groups, (long long)r.pitch, width, o.accumulate_db));
+            if (!check_launch("vocab16_db_kernel")) return -1;
+        }
+        VocabTileArgs p{};
+        p.scale = r.scale;
+        if (o.dx) {
+            p.g = GemmArgs{o.dx, r.d, w, nullptr, 1, g.rows, width, g.k, 0, r.pitch, 1, 0, g.w_cs, g.w_rs, 0, o.dx_rs, 1, o.accumulate_dx};
+            p.sums = r.sums;
+            p.first = v0 == 0;
+            p.last = v0 + width == g.classes;
+            if (launch_grads(p, VOCAB_DX, tied, dx_tile, dtype) != 0) return -1;
+        }
+        if (o.dw) {
+            char* dw = (char*)o.dw + 2 * v0 * o.dw_cs;
+            // x^T . d, or where dW lies as the transpose d^T . x
+            p.g = o.dw_cs == 1 ? GemmArgs{dw, g.x, r.d, nullptr, 1, g.k, g.rows, width, 0, 1, g.x_rs, 0, r.pitch, 1, 0, o.dw_rs, 1, o.accumulate_dw}
+                               : GemmArgs{dw, r.d, g.x, nullptr, 1, width, g.rows, g.k, 0, 1, r.pitch, 0, g.x_rs, 1, 0, o.dw_cs, 1, o.accumulate_dw};
+            if (launch_grads(p, VOCAB_DW, true, vocab_tile(p.g.m, p.g.n, p.g.k, true, true, worse16(lies16(g.x, g.x_rs, g.k), width % 8 ? LIES_RAGGED : LIES_WHOLE)), dtype) != 0) return -1;
+        }
+    }
+    return 0;
+}
+
+}  // namespace rp

@@ -1,0 +1,10 @@
+// f16 cross entropy of a large vocabulary: logits on 256 x 256 tiles.
+#include "rp_vocab16.h"
+
+namespace rp {
+
+int launch_vocab16_logits_256_f16(const VocabTileArgs& a, VocabStep step, bool b_mc, int edge) {
+    return edge == M16_WHOLE ? launch_vocab16_logits<f16_t, 256, 256, 2, M16_WHOLE>(a, step, b_mc) : launch_vocab16_logits<f16_t, 256, 256, 2, M16_EDGE>(a, step, b_mc);
+}
+
+}  // namespace rp
