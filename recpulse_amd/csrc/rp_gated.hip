@@ -5,7 +5,7 @@
 //
 // z is kept in the accumulate type (float32 for the 16-bit types), as the sums that they are: rounded to 16 bits, z's own error would reach dz beside dz's, and the gradients'
 // error would be 1.3 times as large.  dz is rounded to the tensors' type, which is what the matrix cores multiply.
-#include "rp_gated.h"
+#include "rp_gated16.h"
 #include "rp_grouped.h"
 
 namespace rp {
@@ -175,6 +175,28 @@ static int launch_gated_by_product(const GatedArgs& g, int dtype, bool* taken) {
     return 0;
 }
 
+// bf16 and fp16 on MFMA tiles: operands with a unit stride and rows of at least a 16-byte vector
+static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
+    *taken = false;
+    if (g.x_cs != 1 || (g.w_cs != 1 && g.w_rs != 1) || path_disabled("mfma")) return 0;
+    const bool b_mc = g.w_cs == 1;
+    const long long w_stride = b_mc ? g.w_rs : g.w_cs;
+    // rows as long as they have to be, no further apart than the tiles' 32-bit offsets reach
+    if (g.k < 8 || g.x_rs < g.k || g.x_rs >= (1 << 22) || w_stride >= (1 << 22)) return 0;
+    if (b_mc ? g.n < 8 || w_stride < 2ll * g.n : w_stride < g.k || (2ll * g.n + 256) * w_stride * 2 > 0x7fffffffll) return 0;
+    *taken = true;
+    const bool ragged = ((uintptr_t)g.x & 15) || ((uintptr_t)g.w & 15) || g.x_rs % 8 || w_stride % 8 || g.k % 8 || (b_mc && g.n % 8);
+    Plan p{FAM_MFMA16, 64, 64, false, b_mc, true, ""};
+    p.ragged = ragged;
+    choose_tile16(p, 1, g.rows, g.k, 2 * g.n);
+    if (!ragged && p.bm == 256 && p.bn == 256) {
+        const int edge = g.rows % 256 || g.n % 128 || g.k % M16_BK ? M16_EDGE : M16_WHOLE;
+        return dtype == RP_DTYPE_BFLOAT16 ? launch_gated16_256_bf16(g, edge) : launch_gated16_256_f16(g, edge);
+    }
+    const int edge = ragged ? M16_RAGGED : M16_EDGE;
+    return p.bm >= 128 && p.bn >= 128 ? launch_gated16_128(g, edge, dtype) : launch_gated16_64x128(g, edge, dtype);
+}
+
 static bool gated_args_ok(const char* who, bool pointers, int rows, int k, int n, int gate, std::initializer_list<long long> strides, int dtype) {
     if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 30) || n > (1 << 29)) {
         set_error("%s: null operand, non-positive extent, more than 2^30 rows or 2^29 columns (rows=%d k=%d n=%d)", who, rows, k, n);
@@ -206,6 +228,10 @@ int rp_hip_gated_linear_forward(void* h, void* z, const void* x, const void* w, 
     if (dtype == RP_DTYPE_FLOAT32 || dtype == RP_DTYPE_FLOAT64) {
         bool taken;
         const int rc = dtype == RP_DTYPE_FLOAT32 ? launch_gated_by_product<float>(g, dtype, &taken) : launch_gated_by_product<double>(g, dtype, &taken);
+        if (rc != 0 || taken) return rc;
+    } else {
+        bool taken;
+        const int rc = gated16_forward(g, dtype, &taken);
         if (rc != 0 || taken) return rc;
     }
     RP_DISPATCH_DTYPE(dtype, return launch_gated_any<T>(g));

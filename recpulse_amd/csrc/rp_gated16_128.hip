@@ -1,0 +1,11 @@
+// bf16 / fp16 gated linear layer on 128 x 128 tiles: 128 rows, 64 columns of each half of W.
+#include "rp_gated16.h"
+
+namespace rp {
+
+int launch_gated16_128(const GatedArgs& l, int edge, int dtype) {
+    if (dtype == RP_DTYPE_BFLOAT16) return edge == M16_RAGGED ? launch_gated16<bf16_t, 128, 128, 2, M16_RAGGED>(l) : launch_gated16<bf16_t, 128, 128, 2, M16_EDGE>(l);
+    return edge == M16_RAGGED ? launch_gated16<f16_t, 128, 128, 2, M16_RAGGED>(l) : launch_gated16<f16_t, 128, 128, 2, M16_EDGE>(l);
+}
+
+}  // namespace rp

@@ -63,6 +63,9 @@ template <> struct mfma16_ops<f16_t> {
     }
 };
 
+// A sum of in-place MFMAs as it is at this point of the program
+__device__ __forceinline__ void held_in_place(f32x4_t& c) { asm volatile("" : "+a"(c)); }
+
 // MFMA shape of a block tile: the 256 x 256 tile multiplies with 16 x 16 x 32 (k-steps of 32), the others with 32 x 32 x 16.
 // Both run 512 multiply-adds per cycle, but the deeper instruction moves fewer register bytes per multiply-add
 // (2 KB of operands and 2 KB of accumulators per 8 192 against 2 KB and 8 KB per 16 384), and under the power limit
@@ -533,6 +536,12 @@ __device__ __forceinline__ void gemm_mfma16_block(std::conditional_t<SRC::MOVES,
     }
 
     if constexpr (MT == 16) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");      // the in-place MFMAs above are opaque to the compiler: let the last ones drain before their results are read
+    if constexpr (MT == 16 && (SRC::TAKES || SRC::SCALED)) {      // (... and let no read of them move up over that wait)
+        static_for<0, TMI * TNI>([&](auto qc) {
+            constexpr int q = decltype(qc)::value;
+            held_in_place(acc[q / TNI][q % TNI]);
+        });
+    }
     // ---- epilogue ----
     if constexpr (SRC::TAKES) {
         if (source->template take<T, MT, WGN, TMI, TNI, EDGE>(acc, smem, m0, n0)) continue;

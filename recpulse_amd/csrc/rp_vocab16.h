@@ -199,7 +199,7 @@ struct VocabGradProduct : M16Source {
                 constexpr int q = decltype(qc)::value, i = q / (TNI * NV / 4), j = q / (NV / 4) % TNI, v = q % (NV / 4) * 4;
                 const f32x4_t was = own[q * 256];
                 static_for<0, 4>([&](auto ec) { acc[i][j][v + decltype(ec)::value] += was[decltype(ec)::value]; });
-                if constexpr (MT == 16) asm volatile("" : "+a"(acc[i][j]));      // (back where it was: the sums of both ways into the epilogue lie alike)
+                if constexpr (MT == 16) held_in_place(acc[i][j]);      // (back where it was: the sums of both ways into the epilogue lie alike)
                 if constexpr (q % 16 == 15) __builtin_amdgcn_sched_barrier(0);
             });
         }

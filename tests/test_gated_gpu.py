@@ -76,6 +76,17 @@ def test_operands_of_any_stride(dtype):
     assert_within(h.read(), want, rounded(off, want, dtype), "h")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=NAMES.get)
+@pytest.mark.parametrize("tied", [False, True], ids=["rows", "transposed"])
+@pytest.mark.parametrize("rows,k,n", [(2048, 320, 2048), (2000, 328, 2056), (1999, 321, 2051)])
+def test_the_largest_tiles(rows, k, n, tied, dtype):
+    _, x, w, bias = layer(rows, k, n, dtype, n % 2 == 0, rows, tied)
+    z, z_off, _, _, _, _, want, off = reference(x, w, bias, n, "silu", dtype)
+    h, kept = forward(x, w, bias, n, "silu", dtype, True, n + 8 * (rows % 2))
+    assert_within(h.read(), want, rounded(off, want, dtype), "h")
+    assert_within(kept.read(), z, rounded(z_off, z, ACC[dtype]), "z")
+
+
 def test_rows_that_start_at_any_element():
     for rows, k, n in ((40, 128, 96), (150, 200, 264), (9, 520, 72)):
         _, x, w, bias = layer(rows, k, n, BF16, True, 1, lead=3)

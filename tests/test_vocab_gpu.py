@@ -110,6 +110,45 @@ def test_several_pieces_of_the_vocabulary(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=NAMES.get)
+@pytest.mark.parametrize("rows,k,classes,tied", [(4096, 2048, 4096, False), (4000, 2056, 4104, True), (4001, 2056, 4104, False)])
+def test_the_largest_tiles(rows, k, classes, tied, dtype):
+    check_backward(rows, k, classes, tied, dtype, reduction=1, bias=tied)
+
+
+@pytest.mark.parametrize("dtype,tied", [(BF16, False), (F16, True)], ids=["bf16", "f16"])
+def test_several_pieces_on_the_largest_tiles(dtype, tied):
+    """... checked at some rows of dx and some classes of dW, whose logits are few."""
+    rows, k, classes = 8192, 1024, 20008
+    rng, x, w, _, targets = problem(rows, k, classes, dtype, 12, tied, bias=False, without=8)
+    space = room(capi.lib().rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, dtype))
+    _, stats = forward(x, w, None, targets, dtype, 1, space)
+    dx, dw = Output(rows, k, dtype), Output(k, classes, dtype, 1, k) if tied else Output(k, classes, dtype)
+    capi.check(capi.lib().rp_hip_linear_cross_entropy_backward(dx.ptr, dw.ptr, None, x.ptr, w.ptr, None, ints(targets).ptr, stats.ptr, None, space.ptr, rows, k, classes, 1,
+                                                               x.rs, x.cs, w.rs, w.cs, dx.rs, dw.rs, dw.cs, 0, 0, 0, dtype), "rp_hip_linear_cross_entropy_backward")
+    held = targets >= 0
+    f = np.where(held, 1.0 / held.sum(), 0.0)
+    # z is off by at most (k + 8) 2^-24 of the sum of |x w|, below 1e-3 here; lse, from the device, by as much and a little; d by that and its rounding
+    rel = (k + 8) * 2.0 ** -24 * 2.2 * np.sqrt(2 / np.pi) ** 2 * 1.5 * np.sqrt(k) + 1e-4 + HALF[dtype]
+    lse = stats.read()[0, :rows]
+    some = rng.choice(rows, 48, replace=False)
+    z = x.values[some] @ w.values
+    assert np.abs(np.log(np.exp(z).sum(1)) - lse[some]).max() < 1e-3
+    d = np.exp(z - lse[some, None])
+    d[np.arange(48)[held[some]], targets[some][held[some]]] -= 1
+    d *= f[some, None]
+    d_off = rel * np.abs(d) + 2 * rel * np.abs(f[some, None]) * np.exp(z - lse[some, None]) + f.max() * 2.0 ** -38
+    want = d @ w.values.T
+    assert_within(dx.read()[some], want, rounded(d_off @ np.abs(w.values).T + classes * 2.0 ** -24 * (np.abs(d) @ np.abs(w.values).T), want, dtype), "dx")
+    some = rng.choice(classes, 48, replace=False)
+    z = x.values @ w.values[:, some]
+    p = np.exp(z - lse[:, None])
+    d = (p - (targets[:, None] == some)) * f[:, None]
+    d_off = rel * np.abs(d) + 2 * rel * np.abs(f[:, None]) * p + f.max() * 2.0 ** -38
+    want = x.values.T @ d
+    assert_within(dw.read()[:, some], want, rounded(np.abs(x.values).T @ d_off + rows * 2.0 ** -24 * (np.abs(x.values).T @ np.abs(d)), want, dtype), "dw")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=NAMES.get)
 def test_rows_that_start_at_any_element(dtype):
     for tied in (False, True):
         check_backward(70, 136, 520, tied, dtype, reduction=1, lead=3)
