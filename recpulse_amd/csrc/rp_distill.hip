@@ -7,6 +7,7 @@
 // What bounds it is memory: the student's logits once and, backward, their gradient once.  A workgroup holds a row in registers where it fits (131072 classes of 16 bits,
 // 65536 of float32), so that the largest logit, the sum and the gradient cost one read together; longer rows are read once for each of the three.
 // The K entries are handled beside: their classes' gradients are written a second time, after the row's, by the first entry of each class (a class may be named twice).
+#include "rp_gemm.h"
 #include "rp_teams.h"
 
 namespace rp {
@@ -51,20 +52,22 @@ __device__ __forceinline__ bool teacher_entries(const DistillArgs<A>& g, int row
 
 // The gradients of the entries' classes, over what the row's own pass left there
 template <typename T, int THREADS, typename A>
-__device__ __forceinline__ void correct_entries(const DistillArgs<A>& g, const T* logits, T* grad, const int* ids, const A* log_p, A scale, A lse, A log_mass, A factor) {
+__device__ __forceinline__ void correct_entries(const DistillArgs<A>& g, const T* logits, T* grad, const int* ids, A* p, const ScaledExp<A>& q, A log_mass, A factor) {
+    for (int j = threadIdx.x; j < g.k; j += THREADS) p[j] = ids[j] < 0 ? (A)0 : natural_exp(p[j] - log_mass);      // (log p until here)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();                               // the row's stores are done: these come after
     for (int j = threadIdx.x; j < g.k; j += THREADS) {
         const int v = ids[j];
         if (v < 0) continue;
-        A p = 0;
-        bool first = true;
+        A mass = 0;
+        int before = 0;
+#pragma unroll 8
         for (int i = 0; i < g.k; i++) {            // (in the order of the entries, whichever thread adds)
-            if (ids[i] != v) continue;
-            if (i < j) { first = false; break; }
-            p += natural_exp(log_p[i] - log_mass);
+            const bool same = ids[i] == v;
+            mass += same ? p[i] : (A)0;
+            before += same && i < j;
         }
-        if (first) grad[v] = round_to<T>((natural_exp(scaled_less(widen(logits[v]), scale, lse)) - p) * factor);
+        if (!before) grad[v] = round_to<T>((q(widen(logits[v])) - mass) * factor);
     }
 }
 
@@ -74,51 +77,75 @@ template <typename A> __device__ __forceinline__ A row_factor(const DistillArgs<
     return f * g.temperature;
 }
 
+// Vectors a thread holds up to which two workgroups of 1024 share a CU, 64 registers a thread: one's loads and stores fly while the other adds up
+constexpr int DISTILL_SHARED_STEPS = 8;
+constexpr int distill_waves(int threads, int steps, int elem) { return threads == 1024 ? (steps <= DISTILL_SHARED_STEPS && elem < 8 ? 8 : 4) : 1; }
+
 // FORWARD: the row's sums and loss; with a gradient asked for, that too.  Otherwise the gradient from the sums that a forward call left.  STEPS 0: the row is read again for each.
 template <typename T, int THREADS, int STEPS, bool FORWARD>
-__global__ void __launch_bounds__(THREADS) distill_kernel(DistillArgs<typename traits<T>::acc> g) {
+__global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(T))) distill_kernel(DistillArgs<typename traits<T>::acc> g) {
     using A = typename traits<T>::acc;
     constexpr int N = vec16<T>::N, HELD = STEPS ? STEPS : 1;
     __shared__ A room[2 * (THREADS / 64)];
     __shared__ A log_p[DISTILL_MOST_K];
     __shared__ int ids[DISTILL_MOST_K];
-    const int tid = threadIdx.x;
     const A scale = (A)1 / g.temperature;
+    // Vector i of a thread begins at byte tid * 16 + i * THREADS * 16 of the row, which buffer descriptors end with its last whole 4 bytes: what lies behind reads as zeros and is not
+    // written, and one offset does for all loads and stores.  step i is whole where every thread's vector lies in the row; an odd last element of 16 bits goes by itself.
+    auto whole = [&](int i) { return (i + 1) * THREADS * N <= g.classes; };
+    const int row_bytes = STEPS ? g.classes * (int)sizeof(T) / 4 * 4 : 0;
+    const bool odd = STEPS && sizeof(T) == 2 && g.classes % 2;
+    const int odd_tid = (g.classes - 1) / N % THREADS;
     for (int row = blockIdx.x; row < g.rows; row += gridDim.x) {
         const T* s = (const T*)g.logits + row * g.logits_rs;
-        RowVector<T> at[HELD];
-        T raw[HELD][N];
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));              // (the masks of a row's end are made again for each row: kept, they would take more registers than there are)
+        u32x4_t raw[HELD];
+        T last = round_to<T>((A)0);
         if constexpr (STEPS > 0) {
+            const __amdgpu_buffer_rsrc_t from = buffer_rsrc(s, row_bytes);
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) {
-                at[i] = RowVector<T>((i * THREADS + tid) * N, g.classes);
-                at[i].load(raw[i], s);
-#pragma unroll
-                for (int u = 0; u < N; u++) raw[i][u] = at[i].has(u) ? raw[i][u] : round_to<T>(-(A)INFINITY);      // (no mask from here on: exp gives 0)
-            }
+            for (int i = 0; i < STEPS; i++) raw[i] = __builtin_amdgcn_raw_buffer_load_b128(from, tid * 16, i * THREADS * 16, 0);
+            if (odd) last = s[g.classes - 1];
         }
         A lse, log_mass = FORWARD ? (A)0 : g.stats[g.rows + row];
         const bool some = teacher_entries<T, THREADS>(g, row, ids, log_p, room, scale, !FORWARD, log_mass);
+        if constexpr (STEPS > 0) {
+#pragma unroll
+            for (int i = 0; i < STEPS; i++)
+                if (!whole(i)) {
+                    const int left = g.classes - (i * THREADS + tid) * N;
+                    T x[N];
+                    __builtin_memcpy(x, &raw[i], 16);
+#pragma unroll
+                    for (int u = 0; u < N; u++) {
+                        if (odd && u + 1 == left) x[u] = last;
+                        x[u] = u < left ? x[u] : round_to<T>(-(A)INFINITY);      // (no mask from here on: exp gives 0)
+                    }
+                    __builtin_memcpy(&raw[i], x, 16);
+                }
+        }
+        auto each = [&](auto f) {
+            if constexpr (STEPS > 0) {
+#pragma unroll
+                for (int i = 0; i < STEPS; i++) {
+                    T x[N];
+                    asm volatile("" : "+v"(raw[i]));      // (widened anew for each pass)
+                    __builtin_memcpy(x, &raw[i], 16);
+#pragma unroll
+                    for (int u = 0; u < N; u++) f(widen(x[u]));
+                }
+            } else {
+                for (int v = tid; v < g.classes; v += THREADS) f(widen(s[v]));
+            }
+        };
         if constexpr (FORWARD) {
             A top = -(A)INFINITY, sum[1] = {};
-            if constexpr (STEPS > 0) {
-#pragma unroll
-                for (int i = 0; i < STEPS; i++)
-#pragma unroll
-                    for (int u = 0; u < N; u++) top = larger(top, widen(raw[i][u]));
-            } else {
-                for (int v = tid; v < g.classes; v += THREADS) top = larger(top, widen(s[v]));
-            }
+            each([&](A x) { top = plain_max(top, x); });      // (NaN shows in the sum)
             top = team_max<THREADS>(top, room);
             const A base = top == -(A)INFINITY ? (A)0 : top * scale;
-            if constexpr (STEPS > 0) {
-#pragma unroll
-                for (int i = 0; i < STEPS; i++)
-#pragma unroll
-                    for (int u = 0; u < N; u++) sum[0] += natural_exp(scaled_less(widen(raw[i][u]), scale, base));
-            } else {
-                for (int v = tid; v < g.classes; v += THREADS) sum[0] += natural_exp(scaled_less(widen(s[v]), scale, base));
-            }
+            const ScaledExp<A> weight(scale, base);
+            each([&](A x) { sum[0] += weight(x); });
             team_sums<THREADS>(sum, room + THREADS / 64);
             lse = base + natural_log(sum[0]);
             A loss[1] = {};
@@ -140,18 +167,27 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(DistillArgs<typename t
         if (!g.grad) continue;
         T* grad = (T*)g.grad + (long long)row * g.classes;
         const A factor = row_factor(g, row);
+        const ScaledExp<A> q(scale, lse);
+        auto share = [&](A x) { return round_to<T>(some ? q(x) * factor : (A)0); };
         if constexpr (STEPS > 0) {
+            const __amdgpu_buffer_rsrc_t to = buffer_rsrc(grad, row_bytes);
 #pragma unroll
             for (int i = 0; i < STEPS; i++) {
                 T out[N];
+                asm volatile("" : "+v"(raw[i]));
+                __builtin_memcpy(out, &raw[i], 16);
 #pragma unroll
-                for (int u = 0; u < N; u++) out[u] = round_to<T>(some ? natural_exp(scaled_less(widen(raw[i][u]), scale, lse)) * factor : (A)0);
-                at[i].store(grad, out);
+                for (int u = 0; u < N; u++) out[u] = share(widen(out[u]));
+                u32x4_t v;
+                __builtin_memcpy(&v, out, 16);
+                __builtin_amdgcn_raw_buffer_store_b128(v, to, tid * 16, i * THREADS * 16, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (odd && tid == odd_tid) grad[g.classes - 1] = share(widen(last));
         } else {
-            for (int v = tid; v < g.classes; v += THREADS) grad[v] = round_to<T>(some ? natural_exp(scaled_less(widen(s[v]), scale, lse)) * factor : (A)0);
+            for (int v = tid; v < g.classes; v += THREADS) grad[v] = share(widen(s[v]));
         }
-        if (some) correct_entries<T, THREADS>(g, s, grad, ids, log_p, scale, lse, log_mass, factor);
+        if (some) correct_entries<T, THREADS>(g, s, grad, ids, log_p, q, log_mass, factor);
     }
 }
 
