@@ -241,3 +241,56 @@ class AdapterLinear(Module):
     def forward(self, x, ids, lengths):
         """ids[s]: adapter of segment s (-1: none), lengths[s]: how many rows it has."""
         return self.keep(x.op_adapter_linear(self.weight, self.a, self.b, ids, lengths, self.bias, self.scales))
+
+
+class LayerNorm(Module):
+    """y = (x - mean) / sqrt(variance + eps) * w + b for each row of x [rows, features]; w starts as ones, b as zeros."""
+
+    def __init__(self, features, eps=1e-5, bias=True):
+        super().__init__()
+        self.features, self.eps = features, eps
+        self.weight = self.track("weight", rp.ones([features]).requires_grad_(True))
+        self.bias = self.track("bias", rp.zeros([features]).requires_grad_(True)) if bias else None
+
+    def forward(self, x):
+        return self.keep(x.op_layer_norm(self.weight, self.bias, self.eps))
+
+
+class GatedLinear(Module):
+    """y = act(x . Wg + bg) * (x . Wu + bu) with W = [Wg | Wu] of shape [in_features, 2 * out_features]; gate: 'silu', 'gelu', 'gelu_tanh', 'relu' or 'sigmoid'."""
+
+    def __init__(self, in_features, out_features, gate="silu", bias=True):
+        super().__init__()
+        self.in_features, self.out_features, self.gate = in_features, out_features, gate
+        self.weight = self.track("weight", rp.randn([in_features, 2 * out_features]).mul_scalar(1.0 / math.sqrt(in_features)).requires_grad_(True))
+        self.bias = self.track("bias", rp.zeros([2 * out_features]).requires_grad_(True)) if bias else None
+
+    def forward(self, x):
+        return self.keep(x.op_gated_linear(self.weight, self.bias, self.gate))
+
+
+class GatedFeedForward(Module):
+    """The gated linear layer and the projection back: x [rows, features] to [rows, features] over `hidden` columns."""
+
+    def __init__(self, features, hidden, gate="silu", bias=True):
+        super().__init__()
+        self.features, self.hidden = features, hidden
+        self.up = GatedLinear(features, hidden, gate, bias)
+        self.down = Linear(hidden, features, bias)
+
+    def forward(self, x):
+        return self.down(self.up(x))
+
+
+class LinearCrossEntropy(Module):
+    """The last projection of a model together with its loss: the cross entropy of x . W + b against targets (a class for each row, -1: none), without the logits.
+    W [in_features, classes] as in `Linear`."""
+
+    def __init__(self, in_features, classes, bias=True, reduction="mean"):
+        super().__init__()
+        self.in_features, self.classes, self.reduction = in_features, classes, reduction
+        self.weight = self.track("weight", rp.randn([in_features, classes]).mul_scalar(1.0 / math.sqrt(in_features)).requires_grad_(True))
+        self.bias = self.track("bias", rp.zeros([classes]).requires_grad_(True)) if bias else None
+
+    def forward(self, x, targets):
+        return self.keep(x.op_linear_cross_entropy(self.weight, targets, self.bias, self.reduction))

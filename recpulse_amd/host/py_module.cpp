@@ -148,6 +148,11 @@ static py::array routing_array(PyRouting& p, int which) {
     return out;
 }
 
+static int reduction_from(const std::string& name) {
+    const int red = name == "mean" ? 1 : (name == "sum" ? 2 : (name == "none" ? 0 : -1));
+    if (red < 0) throw py::value_error("reduction must be 'none', 'mean' or 'sum'");
+    return red;
+}
 static Tensor* optional_tensor(const py::object& o) { return o.is_none() ? nullptr : o.cast<PyTensor&>().t; }
 
 PYBIND11_MODULE(recpulse_cuda, m) {
@@ -247,6 +252,26 @@ PYBIND11_MODULE(recpulse_cuda, m) {
             if (!scales.is_none() && (a.t->ndim != 3 || (int)sc.size() != a.t->shape[0])) throw std::runtime_error("op_adapter_linear operation failed: one scale for each adapter");
             return wrap(op_adapter_linear(x.t, w.t, optional_tensor(bias), a.t, b.t, scales.is_none() ? nullptr : sc.data(), ids.data(), lengths.data(), (int)ids.size()), "op_adapter_linear");
         }, py::arg("weight"), py::arg("a"), py::arg("b"), py::arg("ids"), py::arg("lengths"), py::arg("bias") = py::none(), py::arg("scales") = py::none())
+        // ---- what stands around a language model's products ----
+        .def("op_layer_norm", [](PyTensor& x, py::object weight, py::object bias, double eps) { return wrap(op_layer_norm(x.t, optional_tensor(weight), optional_tensor(bias), eps), "op_layer_norm"); },
+             py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5)
+        .def("op_gated_linear", [](PyTensor& x, PyTensor& w, py::object bias, const std::string& gate) {
+            const char* names[] = {"silu", "gelu", "gelu_tanh", "relu", "sigmoid"};      // in the order of RP_GATE_*
+            int at = -1;
+            for (int i = 0; i < 5; i++) if (gate == names[i]) at = i;
+            if (at < 0) throw py::value_error("gate must be 'silu', 'gelu', 'gelu_tanh', 'relu' or 'sigmoid'");
+            return wrap(op_gated_linear(x.t, w.t, optional_tensor(bias), at), "op_gated_linear");
+        }, py::arg("weight"), py::arg("bias") = py::none(), py::arg("gate") = "silu")
+        .def("op_linear_cross_entropy", [](PyTensor& x, PyTensor& w, py::object targets, py::object bias, const std::string& reduction) {
+            std::vector<int> t = targets_from(targets);
+            return wrap(op_linear_cross_entropy(x.t, w.t, optional_tensor(bias), t.data(), (int)t.size(), reduction_from(reduction)), "op_linear_cross_entropy");
+        }, py::arg("weight"), py::arg("targets"), py::arg("bias") = py::none(), py::arg("reduction") = "mean")
+        .def("op_distillation_loss", [](PyTensor& x, py::object ids, PyTensor& teacher, double temperature, const std::string& reduction) {
+            std::vector<int> flat;
+            for (auto row : ids) for (auto item : row) flat.push_back(item.cast<int>());
+            if (flat.size() != teacher.t->size) throw std::runtime_error("op_distillation_loss operation failed: one class for each of the teacher's entries");
+            return wrap(op_distillation_loss(x.t, flat.data(), teacher.t, temperature, reduction_from(reduction)), "op_distillation_loss");
+        }, py::arg("ids"), py::arg("teacher"), py::arg("temperature") = 1.0, py::arg("reduction") = "mean")
         .def("op_add", [](PyTensor& a, PyTensor& b) { return wrap(op_add(a.t, b.t), "op_add"); })
         .def("op_relu", [](PyTensor& a) { return wrap(op_relu(a.t), "op_relu"); })
         // `x.op_mul_scalar(s).op_softmax()`: the scaled tensor is a temporary that nothing can read once this call has
@@ -263,8 +288,7 @@ PYBIND11_MODULE(recpulse_cuda, m) {
         .def("op_mean_all", [](PyTensor& a) { return wrap(op_mean_all(a.t), "op_mean_all"); })
         .def("op_cross_entropy_loss", [](PyTensor& a, py::object targets, const std::string& reduction, int from_logits) {
             std::vector<int> t = targets_from(targets);
-            int red = reduction == "mean" ? 1 : (reduction == "sum" ? 2 : (reduction == "none" ? 0 : -1));
-            if (red < 0) throw py::value_error("reduction must be 'none', 'mean' or 'sum'");
+            const int red = reduction_from(reduction);
             if (a.t->ndim != 2 || (int)t.size() != a.t->shape[0]) throw std::runtime_error("op_cross_entropy_loss operation failed: one target per row of a 2-D input");
             return wrap(op_cross_entropy_loss(a.t, t.data(), a.t->shape[0], a.t->shape[1], red, from_logits), "op_cross_entropy_loss");
         }, py::arg("targets"), py::arg("reduction") = "mean", py::arg("from_logits") = -1)

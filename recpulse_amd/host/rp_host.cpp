@@ -1174,6 +1174,117 @@ void backward_adapter_linear_fn(GradFn* self, Tensor* grad_output) {
     free_tensor(gd); free_tensor(ad); free_tensor(bd);
 }
 
+// ---- layer norm, gated layers, the loss of a large vocabulary, distillation ----
+
+// What a node keeps: device memory of its own (stats; z; targets), and its settings
+struct LanguageSaved { int device_id, reduction, choice; double number; void *kept, *plan; Tensor* held; };      // held: the teacher's logits
+
+void free_language_saved(void* p) {
+    LanguageSaved* s = (LanguageSaved*)p;
+    if (on_device(s->device_id)) {
+        if (s->kept) rp_hip_free(s->kept);
+        if (s->plan) rp_hip_free(s->plan);
+    }
+    free_tensor(s->held);
+    free(s);
+}
+LanguageSaved* new_language_saved(int device_id, int reduction = 0, int choice = 0, double number = 0.0) {
+    LanguageSaved* s = (LanguageSaved*)calloc(1, sizeof(LanguageSaved));
+    s->device_id = device_id; s->reduction = reduction; s->choice = choice; s->number = number;
+    return s;
+}
+
+// Gradients that a call has made go where they belong, or are dropped with its error
+void settle(Tensor* const* targets, GradSlot* slots, int count, bool ok, const char* what) {
+    if (!ok) dev_fail(what);
+    for (int i = 0; i < count; i++) {
+        if (!slots[i].fresh) continue;
+        if (ok) accumulate_grad(targets[i], slots[i].fresh);
+        else free_tensor(slots[i].fresh);
+    }
+}
+void* slot_data(const GradSlot& s) { return s.into ? s.into->data : nullptr; }
+
+// The upstream gradient of a loss in the accumulate type, where the loss is: one element, or one for each row
+Tensor* loss_upstream(Tensor* grad_output, DType acc, int device_id, size_t want) {
+    if (grad_output->size != want) return nullptr;
+    return grad_output->device_id == device_id && grad_output->dtype == acc ? dense(grad_output) : tensor_to(grad_output, device_id, acc, false);
+}
+
+// inputs: x and, if there are, w and b (choice: 1 for w, 2 for b)
+void backward_layer_norm_fn(GradFn* self, Tensor* grad_output) {
+    LanguageSaved* s = (LanguageSaved*)self->saved_data;
+    Tensor* x = self->inputs[0];
+    Tensor* w = s->choice & 1 ? self->inputs[1] : nullptr;
+    Tensor* b = s->choice & 2 ? self->inputs[s->choice & 1 ? 2 : 1] : nullptr;
+    const int rows = x->shape[0], d = x->shape[1];
+    Tensor* gd = dense(grad_output); Tensor* xd = dense(x);
+    Tensor* targets[3] = {x, w, b};
+    GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(b)};
+    void* room = nullptr;
+    bool ok = gd && xd && on_device(x->device_id);
+    if (ok && (slots[1].into || slots[2].into)) ok = rp_hip_malloc(&room, (size_t)rp_hip_layer_norm_workspace(rows, d, x->dtype)) == 0;
+    ok = ok && rp_hip_layer_norm_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), gd->data, xd->data, w ? w->data : nullptr, s->kept, room, rows, d, d, d, d,
+                                          slots[0].accumulate, slots[1].accumulate, slots[2].accumulate, x->dtype) == 0;
+    if (room) rp_hip_free(room);
+    settle(targets, slots, 3, ok, "op_layer_norm backward");
+    free_tensor(gd); free_tensor(xd);
+}
+
+// A gradient that lies as a weight of unit stride along its rows does is made in place where one is there already; a new one is dense
+void backward_gated_linear_fn(GradFn* self, Tensor* grad_output) {
+    LanguageSaved* s = (LanguageSaved*)self->saved_data;
+    Tensor* x = self->inputs[0]; Tensor* w = self->inputs[1];
+    Tensor* bias = self->num_inputs > 2 ? self->inputs[2] : nullptr;
+    const int rows = x->shape[0], k = x->shape[1], n = w->shape[1] / 2;
+    Tensor* gd = dense(grad_output);
+    Tensor* targets[3] = {x, w, bias};
+    GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(bias)};
+    void* dz = nullptr;
+    const bool ok = gd && on_device(x->device_id) && rp_hip_malloc(&dz, dtype_size(x->dtype) * 2 * (size_t)rows * n) == 0 &&
+                    rp_hip_gated_linear_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), dz, gd->data, s->kept, x->data, w->data, rows, k, n, s->choice,
+                                                 n, x->strides[0], x->strides[1], w->strides[0], w->strides[1], k, 2ll * n, 1, slots[0].accumulate, slots[1].accumulate, slots[2].accumulate, x->dtype) == 0;
+    if (dz) rp_hip_free(dz);
+    settle(targets, slots, 3, ok, "op_gated_linear backward");
+    free_tensor(gd);
+}
+
+void backward_linear_cross_entropy_fn(GradFn* self, Tensor* grad_output) {
+    LanguageSaved* s = (LanguageSaved*)self->saved_data;
+    Tensor* x = self->inputs[0]; Tensor* w = self->inputs[1];
+    Tensor* bias = self->num_inputs > 2 ? self->inputs[2] : nullptr;
+    const int rows = x->shape[0], k = x->shape[1], classes = w->shape[1];
+    Tensor* up = loss_upstream(grad_output, weights_dtype(x->dtype), x->device_id, s->reduction == 0 ? (size_t)rows : 1);
+    if (!up) { fail("op_linear_cross_entropy backward: upstream gradient has the wrong size"); return; }
+    Tensor* targets[3] = {x, w, bias};
+    GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(bias)};
+    void* room = nullptr;
+    const bool ok = on_device(x->device_id) && rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, x->dtype)) == 0 &&
+                    rp_hip_linear_cross_entropy_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), x->data, w->data, bias ? bias->data : nullptr, (const int*)s->plan, s->kept, up->data, room,
+                                                         rows, k, classes, s->reduction, x->strides[0], x->strides[1], w->strides[0], w->strides[1], k, classes, 1,
+                                                         slots[0].accumulate, slots[1].accumulate, slots[2].accumulate, x->dtype) == 0;
+    if (room) rp_hip_free(room);
+    settle(targets, slots, 3, ok, "op_linear_cross_entropy backward");
+    free_tensor(up);
+}
+
+// (the teacher has no gradient: it is no input of the node, so that a graph of its own stays as it is)
+void backward_distillation_fn(GradFn* self, Tensor* grad_output) {
+    LanguageSaved* s = (LanguageSaved*)self->saved_data;
+    Tensor* x = self->inputs[0]; Tensor* teacher = s->held;
+    if (!needs_grad(x)) return;
+    const int rows = x->shape[0], classes = x->shape[1];
+    Tensor* up = loss_upstream(grad_output, weights_dtype(x->dtype), x->device_id, s->reduction == 0 ? (size_t)rows : 1);
+    if (!up) { fail("op_distillation_loss backward: upstream gradient has the wrong size"); return; }
+    Tensor* xd = dense(x);
+    Tensor* g = empty_tensor(x->dtype, x->device_id, 2, x->shape);
+    const bool ok = xd && g && on_device(x->device_id) &&
+                    rp_hip_distillation_backward(g->data, s->kept, xd->data, (const int*)s->plan, teacher->data, up->data, rows, classes, teacher->shape[1], classes, s->number, s->reduction, x->dtype) == 0;
+    if (ok) accumulate_grad(x, g);
+    else { dev_fail("op_distillation_loss backward"); free_tensor(g); }
+    free_tensor(xd); free_tensor(up);
+}
+
 // ---- conv2d ----------------------------------------------------------------------------
 // The reference lowers one sample at a time: im2col, rp_matmul, and for the gradients col2im or a densified transpose
 // per sample (ops/ops.c:4759-4770, 4533-4551, 4575-4617), with the bias and its gradient done on the host.  Here a
@@ -1982,6 +2093,111 @@ Tensor* op_adapter_linear(Tensor* x, Tensor* w, Tensor* bias, Tensor* a, Tensor*
     } else {
         free_adapter_saved(s);
     }
+    return out;
+}
+
+static bool rows_on_device(const Tensor* x, const char* op) {
+    if (x->device_id == -1) { fail("%s on host tensors is not provided by this build; move the operands to a GPU", op); return false; }
+    if (x->ndim != 2) { fail("%s: [rows, features]", op); return false; }
+    return true;
+}
+static bool vector_beside(const Tensor* x, const Tensor* v, int size, const char* op, const char* what) {
+    if (!v || (v->ndim == 1 && v->shape[0] == size && same_place(x, v) && rp_is_contiguous((Tensor*)v))) return true;
+    fail("%s: %s must be a dense vector of %d values of x's dtype and device", op, what, size);
+    return false;
+}
+static bool reduction_ok(int reduction, const char* op) {
+    if (reduction >= 0 && reduction <= 2) return true;
+    fail("%s: reduction must be none (0), mean (1) or sum (2)", op);
+    return false;
+}
+
+Tensor* op_layer_norm(Tensor* x, Tensor* w, Tensor* b, double eps) {
+    if (!x || !rows_on_device(x, "op_layer_norm")) return nullptr;
+    const int rows = x->shape[0], d = x->shape[1];
+    if (!vector_beside(x, w, d, "op_layer_norm", "weight") || !vector_beside(x, b, d, "op_layer_norm", "bias")) return nullptr;
+    const bool grads = needs_grad(x) || (w && needs_grad(w)) || (b && needs_grad(b));
+    Tensor* xd = dense(x);
+    Tensor* out = xd ? empty_tensor(x->dtype, x->device_id, 2, x->shape) : nullptr;
+    LanguageSaved* s = new_language_saved(x->device_id, 0, (w ? 1 : 0) | (b ? 2 : 0));
+    const bool ok = out && on_device(x->device_id) && (!grads || rp_hip_malloc(&s->kept, dtype_size(weights_dtype(x->dtype)) * 2 * (size_t)rows) == 0) &&
+                    rp_hip_layer_norm_forward(out->data, s->kept, xd->data, w ? w->data : nullptr, b ? b->data : nullptr, rows, d, d, d, eps, x->dtype) == 0;
+    free_tensor(xd);
+    if (!ok) { dev_fail("op_layer_norm"); free_tensor(out); free_language_saved(s); return nullptr; }
+    if (!grads) { free_language_saved(s); return out; }
+    GradFn* gf = w && b ? attach(out, backward_layer_norm_fn, {x, w, b}) : w ? attach(out, backward_layer_norm_fn, {x, w}) : b ? attach(out, backward_layer_norm_fn, {x, b}) : attach(out, backward_layer_norm_fn, {x});
+    gf->saved_data = s;
+    gf->free_saved = free_language_saved;
+    return out;
+}
+
+Tensor* op_gated_linear(Tensor* x, Tensor* w, Tensor* bias, int gate) {
+    if (!x || !w || !rows_on_device(x, "op_gated_linear")) return nullptr;
+    if (w->ndim != 2 || !same_place(x, w) || w->shape[0] != x->shape[1] || w->shape[1] % 2) { fail("op_gated_linear: weight [in_features, 2 * out_features] of x's dtype and device"); return nullptr; }
+    if (!vector_beside(x, bias, w->shape[1], "op_gated_linear", "bias")) return nullptr;
+    const int rows = x->shape[0], k = x->shape[1], n = w->shape[1] / 2, shape[2] = {rows, n};
+    const bool grads = needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias));
+    Tensor* out = empty_tensor(x->dtype, x->device_id, 2, shape);
+    LanguageSaved* s = new_language_saved(x->device_id, 0, gate);
+    const bool ok = out && on_device(x->device_id) && (!grads || rp_hip_malloc(&s->kept, dtype_size(weights_dtype(x->dtype)) * 2 * (size_t)rows * n) == 0) &&
+                    rp_hip_gated_linear_forward(out->data, s->kept, x->data, w->data, bias ? bias->data : nullptr, rows, k, n, gate, x->strides[0], x->strides[1], w->strides[0], w->strides[1], n, x->dtype) == 0;
+    if (!ok) { dev_fail("op_gated_linear"); free_tensor(out); free_language_saved(s); return nullptr; }
+    if (!grads) { free_language_saved(s); return out; }
+    GradFn* gf = bias ? attach(out, backward_gated_linear_fn, {x, w, bias}) : attach(out, backward_gated_linear_fn, {x, w});
+    gf->saved_data = s;
+    gf->free_saved = free_language_saved;
+    return out;
+}
+
+static bool upload_ints(void** to, const int* from, size_t count) { return rp_hip_malloc(to, sizeof(int) * count) == 0 && rp_hip_memcpy_h2d(*to, from, sizeof(int) * count) == 0; }
+
+Tensor* op_linear_cross_entropy(Tensor* x, Tensor* w, Tensor* bias, const int* targets, int count, int reduction) {
+    const char* op = "op_linear_cross_entropy";
+    if (!x || !w || !targets || !rows_on_device(x, op) || !reduction_ok(reduction, op)) return nullptr;
+    if (w->ndim != 2 || !same_place(x, w) || w->shape[0] != x->shape[1]) { fail("%s: weight [in_features, classes] of x's dtype and device", op); return nullptr; }
+    const int rows = x->shape[0], k = x->shape[1], classes = w->shape[1], out_len = reduction == 0 ? rows : 1;
+    if (count != rows) { fail("%s: one target for each of the %d rows", op, rows); return nullptr; }
+    if (!vector_beside(x, bias, classes, op, "bias")) return nullptr;
+    for (int i = 0; i < rows; i++)
+        if (targets[i] < -1 || targets[i] >= classes) { fail("%s: target out of range", op); return nullptr; }
+    const bool grads = needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias));
+    const DType acc = weights_dtype(x->dtype);
+    Tensor* out = empty_tensor(acc, x->device_id, 1, &out_len);
+    LanguageSaved* s = new_language_saved(x->device_id, reduction);
+    void* room = nullptr;
+    const bool ok = out && on_device(x->device_id) && rp_hip_malloc(&s->kept, dtype_size(acc) * (2 * (size_t)rows + 1)) == 0 && upload_ints(&s->plan, targets, rows) &&
+                    rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace(rows, k, classes, 0, x->dtype)) == 0 &&
+                    rp_hip_linear_cross_entropy_forward(out->data, s->kept, x->data, w->data, bias ? bias->data : nullptr, (const int*)s->plan, room, rows, k, classes, reduction,
+                                                        x->strides[0], x->strides[1], w->strides[0], w->strides[1], x->dtype) == 0;
+    if (room) rp_hip_free(room);
+    if (!ok) { dev_fail(op); free_tensor(out); free_language_saved(s); return nullptr; }
+    if (!grads) { free_language_saved(s); return out; }
+    GradFn* gf = bias ? attach(out, backward_linear_cross_entropy_fn, {x, w, bias}) : attach(out, backward_linear_cross_entropy_fn, {x, w});
+    gf->saved_data = s;
+    gf->free_saved = free_language_saved;
+    return out;
+}
+
+Tensor* op_distillation_loss(Tensor* logits, const int* ids, Tensor* teacher, double temperature, int reduction) {
+    const char* op = "op_distillation_loss";
+    if (!logits || !ids || !teacher || !rows_on_device(logits, op) || !reduction_ok(reduction, op)) return nullptr;
+    if (teacher->ndim != 2 || !same_place(logits, teacher) || teacher->shape[0] != logits->shape[0]) { fail("%s: teacher [rows, entries] of the logits' dtype and device", op); return nullptr; }
+    const int rows = logits->shape[0], classes = logits->shape[1], k = teacher->shape[1], out_len = reduction == 0 ? rows : 1;
+    for (long long i = 0; i < (long long)rows * k; i++)
+        if (ids[i] < -1 || ids[i] >= classes) { fail("%s: class out of range", op); return nullptr; }
+    const DType acc = weights_dtype(logits->dtype);
+    Tensor* xd = dense(logits); Tensor* td = dense(teacher);
+    Tensor* out = xd && td ? empty_tensor(acc, logits->device_id, 1, &out_len) : nullptr;
+    LanguageSaved* s = new_language_saved(logits->device_id, reduction, 0, temperature);
+    s->held = td;
+    const bool ok = out && on_device(logits->device_id) && rp_hip_malloc(&s->kept, dtype_size(acc) * 3 * (size_t)rows) == 0 && upload_ints(&s->plan, ids, (size_t)rows * k) &&
+                    rp_hip_distillation_forward(out->data, nullptr, s->kept, xd->data, (const int*)s->plan, td->data, nullptr, rows, classes, k, classes, temperature, reduction, logits->dtype) == 0;
+    free_tensor(xd);
+    if (!ok) { dev_fail(op); free_tensor(out); free_language_saved(s); return nullptr; }
+    if (!needs_grad(logits)) { free_language_saved(s); return out; }
+    GradFn* gf = attach(out, backward_distillation_fn, {logits});
+    gf->saved_data = s;
+    gf->free_saved = free_language_saved;
     return out;
 }
 

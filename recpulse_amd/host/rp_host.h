@@ -129,6 +129,15 @@ Tensor* op_grouped_linear(Tensor* x, Tensor* w, Tensor* bias, Routing* routing);
  * adapter ids[s], -1: none; scales: host array [adapters] or NULL.  Rows behind the last segment have no adapter. */
 Tensor* op_adapter_linear(Tensor* x, Tensor* w, Tensor* bias, Tensor* a, Tensor* b, const float* scales, const int* ids, const int* lengths, int segments);
 
+/* ---- what stands around a language model's products (extensions; device tensors) ---- */
+Tensor* op_layer_norm(Tensor* x, Tensor* w, Tensor* b, double eps);                              /* rows [rows, d]; w, b [d] or NULL */
+Tensor* op_gated_linear(Tensor* x, Tensor* w, Tensor* bias, int gate);                            /* act(x·w[:, :n] + bias[:n]) * (x·w[:, n:] + bias[n:]), w [in, 2 n]; gate as RP_GATE_* in rp_hip.h */
+/* Cross entropy of x·w + bias against the targets (host array, one for each row, -1: none) without the logits: [1], for reduction 0 [rows], in float32 (float64).  reduction as in op_cross_entropy_loss, the mean
+ * over the rows with a target. */
+Tensor* op_linear_cross_entropy(Tensor* x, Tensor* w, Tensor* bias, const int* targets, int rows, int reduction);
+/* Distillation of logits [rows, classes] from the teacher's top logits: ids host array [rows * k] of their classes (-1: none), teacher [rows, k]; [1], for reduction 0 [rows], in float32 (float64). */
+Tensor* op_distillation_loss(Tensor* logits, const int* ids, Tensor* teacher, double temperature, int reduction);
+
 Tensor* op_add(Tensor* x1, Tensor* x2);
 Tensor* op_relu(Tensor* x);
 Tensor* op_softmax(Tensor* x, int dim);
