@@ -6,13 +6,13 @@
 //
 // What bounds it is memory: the student's logits once and, backward, their gradient once.  A workgroup holds a row in registers where it fits (131072 classes of 16 bits,
 // 65536 of float32), so that the largest logit, the sum and the gradient cost one read together; longer rows are read once for each of the three.
-// The K entries are handled beside: their classes' gradients are written a second time, after the row's, by the first entry of each class (a class may be named twice).
+// The K entries are handled beside, one a thread: their classes' gradients are written a second time, after the row's, by the first entry of each class (a class may be named twice).
 #include "rp_gemm.h"
 #include "rp_teams.h"
 
 namespace rp {
 
-constexpr int DISTILL_MOST_K = 1024, DISTILL_GRID = 1 << 20;
+constexpr int DISTILL_MOST_K = 1024;
 
 template <typename A> struct DistillArgs {
     void* grad;
@@ -24,57 +24,26 @@ template <typename A> struct DistillArgs {
     A temperature;
 };
 
-// The K entries in LDS: classes (-1: none) and log p.  Returns whether there is an entry.
-template <typename T, int THREADS, typename A>
-__device__ __forceinline__ bool teacher_entries(const DistillArgs<A>& g, int row, int* ids, A* log_p, A* room, A scale, bool known, A& log_mass) {
-    const int* id = g.ids + (long long)row * g.k;
-    const T* t = (const T*)g.teacher + (long long)row * g.k;
-    A top = -INFINITY;
-    __syncthreads();                               // (the last row's entries are done with)
-    for (int j = threadIdx.x; j < g.k; j += THREADS) {
-        const int v = id[j];
-        const bool in = v >= 0 && v < g.classes;
-        const A u = in ? widen(t[j]) * scale : -(A)INFINITY;
-        ids[j] = in && !(u == -(A)INFINITY) ? v : -1;
-        log_p[j] = u;
-        top = larger(top, u);
-    }
-    if (!known) {
-        top = team_max<THREADS>(top, room);
-        A mass[1] = {};
-        for (int j = threadIdx.x; j < g.k; j += THREADS) mass[0] += ids[j] < 0 ? (A)0 : natural_exp(log_p[j] - top);
-        team_sums<THREADS>(mass, room + THREADS / 64);
-        log_mass = top == -(A)INFINITY ? -(A)INFINITY : top + natural_log(mass[0]);
-    }
-    __syncthreads();
-    return !(log_mass == -(A)INFINITY);
-}
-
-// The gradients of the entries' classes, over what the row's own pass left there
-template <typename T, int THREADS, typename A>
-__device__ __forceinline__ void correct_entries(const DistillArgs<A>& g, const T* logits, T* grad, const int* ids, A* p, const ScaledExp<A>& q, A log_mass, A factor) {
-    for (int j = threadIdx.x; j < g.k; j += THREADS) p[j] = ids[j] < 0 ? (A)0 : natural_exp(p[j] - log_mass);      // (log p until here)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                               // the row's stores are done: these come after
-    for (int j = threadIdx.x; j < g.k; j += THREADS) {
-        const int v = ids[j];
-        if (v < 0) continue;
-        A mass = 0;
-        int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < g.k; i++) {            // (in the order of the entries, whichever thread adds)
-            const bool same = ids[i] == v;
-            mass += same ? p[i] : (A)0;
-            before += same && i < j;
-        }
-        if (!before) grad[v] = round_to<T>((q(widen(logits[v])) - mass) * factor);
-    }
-}
-
 template <typename A> __device__ __forceinline__ A row_factor(const DistillArgs<A>& g, int row) {
     A f = g.upstream ? ((const A*)g.upstream)[g.reduction == 0 ? row : 0] : (A)1;
     if (g.reduction == 1) f /= (A)g.rows;
     return f * g.temperature;
+}
+
+// The gradients of the entries' classes, over what the row's own pass left there: `v`, `value`: this thread's entry (-1: none) and its logit
+template <typename T, typename A>
+__device__ __forceinline__ void correct_entries(int k, T* grad, const int* ids, const A* p, int v, A value, const ScaledExp<A>& q, A factor) {
+    if (v < 0) return;
+    const int j = threadIdx.x;
+    A mass = 0;
+    int before = 0;
+#pragma unroll 8
+    for (int i = 0; i < k; i++) {                  // (in the order of the entries, whichever thread adds)
+        const bool same = ids[i] == v;
+        mass += same ? p[i] : (A)0;
+        before += same && i < j;
+    }
+    if (!before) grad[v] = round_to<T>((q(value) - mass) * factor);
 }
 
 // Vectors a thread holds up to which two workgroups of 1024 share a CU, 64 registers a thread: one's loads and stores fly while the other adds up
@@ -82,34 +51,53 @@ constexpr int DISTILL_SHARED_STEPS = 8;
 constexpr int distill_waves(int threads, int steps, int elem) { return threads == 1024 ? (steps <= DISTILL_SHARED_STEPS && elem < 8 ? 8 : 4) : 1; }
 
 // FORWARD: the row's sums and loss; with a gradient asked for, that too.  Otherwise the gradient from the sums that a forward call left.  STEPS 0: the row is read again for each.
+// A workgroup walks rows; the next row's loads are issued as soon as a row's registers are stored, and fly while its last steps wait for one another.  k <= THREADS: a thread has an entry or none.
 template <typename T, int THREADS, int STEPS, bool FORWARD>
 __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(T))) distill_kernel(DistillArgs<typename traits<T>::acc> g) {
     using A = typename traits<T>::acc;
-    constexpr int N = vec16<T>::N, HELD = STEPS ? STEPS : 1;
-    __shared__ A room[2 * (THREADS / 64)];
-    __shared__ A log_p[DISTILL_MOST_K];
-    __shared__ int ids[DISTILL_MOST_K];
+    constexpr int N = vec16<T>::N, HELD = STEPS ? STEPS : 1, WAVES = THREADS / 64;
+    __shared__ A rooms[3][2][WAVES];
+    __shared__ A entry_p[2][THREADS];              // (of this row and of the one before, which may still be read)
+    __shared__ int entry_ids[2][THREADS];
     const A scale = (A)1 / g.temperature;
     // Vector i of a thread begins at byte tid * 16 + i * THREADS * 16 of the row, which buffer descriptors end with its last whole 4 bytes: what lies behind reads as zeros and is not
-    // written, and one offset does for all loads and stores.  step i is whole where every thread's vector lies in the row; an odd last element of 16 bits goes by itself.
+    // written, and one offset does for all loads.  Step i is whole where every thread's vector lies in the row; an odd last element of 16 bits goes by itself.
     auto whole = [&](int i) { return (i + 1) * THREADS * N <= g.classes; };
     const int row_bytes = STEPS ? g.classes * (int)sizeof(T) / 4 * 4 : 0;
     const bool odd = STEPS && sizeof(T) == 2 && g.classes % 2;
-    const int odd_tid = (g.classes - 1) / N % THREADS;
-    for (int row = blockIdx.x; row < g.rows; row += gridDim.x) {
-        const T* s = (const T*)g.logits + row * g.logits_rs;
+    u32x4_t raw[HELD];
+    T last = round_to<T>((A)0), entry = round_to<T>((A)0);
+    int id = -1;
+    auto row_of = [&](int row) { return (const T*)g.logits + (row < g.rows ? row : g.rows - 1) * g.logits_rs; };      // (a row again rather than none)
+    auto load_step = [&](const __amdgpu_buffer_rsrc_t& from, auto ic) {
+        constexpr int i = decltype(ic)::value;
+        raw[i] = __builtin_amdgcn_raw_buffer_load_b128(from, (int)threadIdx.x * 16, i * THREADS * 16, 0);
+    };
+    auto load_entry = [&](int row) {
+        if (row >= g.rows) row = g.rows - 1;
+        if (odd) last = row_of(row)[g.classes - 1];
+        if ((int)threadIdx.x < g.k) {
+            id = g.ids[(long long)row * g.k + threadIdx.x];
+            entry = ((const T*)g.teacher)[(long long)row * g.k + threadIdx.x];
+        }
+    };
+    {
+        const __amdgpu_buffer_rsrc_t from = buffer_rsrc(row_of(blockIdx.x), row_bytes);
+        static_for<0, STEPS>([&](auto ic) { load_step(from, ic); });
+        load_entry(blockIdx.x);
+    }
+    for (int row = blockIdx.x, turn = 0; row < g.rows; row += gridDim.x, turn ^= 1) {
+        const T* s = row_of(row);
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));              // (the masks of a row's end are made again for each row: kept, they would take more registers than there are)
-        u32x4_t raw[HELD];
-        T last = round_to<T>((A)0);
-        if constexpr (STEPS > 0) {
-            const __amdgpu_buffer_rsrc_t from = buffer_rsrc(s, row_bytes);
-#pragma unroll
-            for (int i = 0; i < STEPS; i++) raw[i] = __builtin_amdgcn_raw_buffer_load_b128(from, tid * 16, i * THREADS * 16, 0);
-            if (odd) last = s[g.classes - 1];
-        }
-        A lse, log_mass = FORWARD ? (A)0 : g.stats[g.rows + row];
-        const bool some = teacher_entries<T, THREADS>(g, row, ids, log_p, room, scale, !FORWARD, log_mass);
+        // the entry: its class (-1: none), log p but for the sum, and the student's logit
+        A* p = entry_p[turn];
+        int* ids = entry_ids[turn];
+        A log_p = id >= 0 && id < g.classes ? widen(entry) * scale : -(A)INFINITY;
+        const int v = log_p == -(A)INFINITY ? -1 : id;
+        const A value = v < 0 ? (A)0 : widen(s[v]);
+        const T row_last = last;
+        if (tid < g.k) ids[tid] = v;
         if constexpr (STEPS > 0) {
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
@@ -119,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                     __builtin_memcpy(x, &raw[i], 16);
 #pragma unroll
                     for (int u = 0; u < N; u++) {
-                        if (odd && u + 1 == left) x[u] = last;
+                        if (odd && u + 1 == left) x[u] = row_last;
                         x[u] = u < left ? x[u] : round_to<T>(-(A)INFINITY);      // (no mask from here on: exp gives 0)
                     }
                     __builtin_memcpy(&raw[i], x, 16);
@@ -136,58 +124,112 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                     for (int u = 0; u < N; u++) f(widen(x[u]));
                 }
             } else {
-                for (int v = tid; v < g.classes; v += THREADS) f(widen(s[v]));
+                for (int c = tid; c < g.classes; c += THREADS) f(widen(s[c]));
             }
         };
+        A lse, log_mass;
         if constexpr (FORWARD) {
-            A top = -(A)INFINITY, sum[1] = {};
-            each([&](A x) { top = plain_max(top, x); });      // (NaN shows in the sum)
-            top = team_max<THREADS>(top, room);
+            A top = -(A)INFINITY;
+            bool again = false;
+            if constexpr (STEPS > 0 && sizeof(T) == 2) {
+                // Two values at a time as whole numbers: of those that are not negative the largest number is the largest value (and +NaN above all).  Rows without one are looked through again.
+                typedef short __attribute__((ext_vector_type(2))) short2_t;
+                u32x4_t most = raw[0];
+#pragma unroll
+                for (int i = 1; i < STEPS; i++)
+#pragma unroll
+                    for (int w = 0; w < 4; w++) most[w] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(short2_t, (uint32_t)most[w]), __builtin_bit_cast(short2_t, (uint32_t)raw[i][w])));
+                int first = -32768;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const short2_t pair = __builtin_bit_cast(short2_t, (uint32_t)most[w]);
+                    first = first > pair[0] ? first : pair[0];
+                    first = first > pair[1] ? first : pair[1];
+                }
+                top = (A)first;
+            } else {
+                each([&](A x) { top = plain_max(top, x); });      // (NaN shows in the sum)
+            }
+            A tops[2] = {top, log_p};
+            team_tops_in_turn<THREADS>(tops, rooms[0][0]);
+            top = tops[0];
+            if constexpr (STEPS > 0 && sizeof(T) == 2) {
+                again = !(top >= (A)0);
+                T x;
+                x.bits = (uint16_t)(int)top;
+                top = widen(x);
+                if (again) {
+                    top = -(A)INFINITY;
+                    each([&](A x) { top = plain_max(top, x); });
+                    __syncthreads();
+                    A one[1] = {top};
+                    team_tops_in_turn<THREADS>(one, rooms[0][0]);
+                    top = one[0];
+                }
+            }
             const A base = top == -(A)INFINITY ? (A)0 : top * scale;
             const ScaledExp<A> weight(scale, base);
-            each([&](A x) { sum[0] += weight(x); });
-            team_sums<THREADS>(sum, room + THREADS / 64);
-            lse = base + natural_log(sum[0]);
-            A loss[1] = {};
-            if (some)
-                for (int j = tid; j < g.k; j += THREADS) {
-                    if (ids[j] < 0) continue;
-                    const A lp = log_p[j] - log_mass, p = natural_exp(lp);
-                    if (p != 0) loss[0] += p * (lp - scaled_less(widen(s[ids[j]]), scale, lse));
-                }
-            team_sums<THREADS>(loss, room);
+            A sums[2] = {(A)0, v < 0 ? (A)0 : natural_exp(log_p - tops[1])};
+            each([&](A x) { sums[0] += weight(x); });
+            team_sums_in_turn<THREADS>(sums, rooms[1][0]);
+            lse = base + natural_log(sums[0]);
+            log_mass = tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]);
+        } else {
+            lse = g.stats[row];
+            log_mass = g.stats[g.rows + row];
+        }
+        const bool some = !(log_mass == -(A)INFINITY);
+        log_p -= log_mass;
+        const A own_p = v < 0 ? (A)0 : natural_exp(log_p);
+        if constexpr (FORWARD) {
+            A loss[1] = {own_p != 0 ? own_p * (log_p - scaled_less(value, scale, lse)) : (A)0};
+            if (g.k > 64) team_sums_in_turn<THREADS>(loss, rooms[2][0]);
+            else loss[0] = wave_sum(loss[0]);          // (the first wave has all entries)
             if (tid == 0) {
                 g.stats[row] = lse;
                 g.stats[g.rows + row] = log_mass;
-                g.stats[2 * (long long)g.rows + row] = loss[0] * g.temperature * g.temperature;
+                g.stats[2 * (long long)g.rows + row] = some ? loss[0] * g.temperature * g.temperature : (A)0;
             }
-        } else {
-            lse = g.stats[row];
         }
-        if (!g.grad) continue;
+        const __amdgpu_buffer_rsrc_t from = buffer_rsrc(row_of(row + gridDim.x), row_bytes);
+        if (!g.grad) {
+            static_for<0, STEPS>([&](auto ic) { load_step(from, ic); });
+            load_entry(row + gridDim.x);
+            continue;                              // (two barriers lie between a room's readers and its next writers)
+        }
         T* grad = (T*)g.grad + (long long)row * g.classes;
         const A factor = row_factor(g, row);
         const ScaledExp<A> q(scale, lse);
-        auto share = [&](A x) { return round_to<T>(some ? q(x) * factor : (A)0); };
+        auto share = [&](A x) { return some ? q(x) * factor : (A)0; };
+        if (tid < g.k) p[tid] = own_p;
         if constexpr (STEPS > 0) {
             const __amdgpu_buffer_rsrc_t to = buffer_rsrc(grad, row_bytes);
-#pragma unroll
-            for (int i = 0; i < STEPS; i++) {
+            static_for<0, STEPS>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
                 T out[N];
+                A values[N];
                 asm volatile("" : "+v"(raw[i]));
                 __builtin_memcpy(out, &raw[i], 16);
 #pragma unroll
-                for (int u = 0; u < N; u++) out[u] = share(widen(out[u]));
-                u32x4_t v;
-                __builtin_memcpy(&v, out, 16);
-                __builtin_amdgcn_raw_buffer_store_b128(v, to, tid * 16, i * THREADS * 16, 0);
+                for (int u = 0; u < N; u++) values[u] = q(widen(out[u])) * factor;
+                if (some) round_vector<T>(out, values);
+                else __builtin_memset(out, 0, 16);           // (whatever the row's logits are)
+                u32x4_t o;
+                __builtin_memcpy(&o, out, 16);
+                // (the whole offset in a vector register: behind a 16-byte store with part of it in a scalar one the compiler lets the next instruction write the data's registers, and zeros of such a
+                // write have been stored here)
+                __builtin_amdgcn_raw_buffer_store_b128(o, to, tid * 16 + i * THREADS * 16, 0, 0);
+                load_step(from, ic);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if (odd && tid == odd_tid) grad[g.classes - 1] = share(widen(last));
+            });
+            if (odd && tid == (g.classes - 1) / N % THREADS) grad[g.classes - 1] = round_to<T>(share(widen(row_last)));
         } else {
-            for (int v = tid; v < g.classes; v += THREADS) grad[v] = share(widen(s[v]));
+            for (int c = tid; c < g.classes; c += THREADS) grad[c] = round_to<T>(share(widen(s[c])));
         }
-        if (some) correct_entries<T, THREADS>(g, s, grad, ids, log_p, q, log_mass, factor);
+        load_entry(row + gridDim.x);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                           // the row's stores are done: the entries' classes come after
+        if (some) correct_entries<T>(g.k, grad, ids, p, v, value, q, factor);
     }
 }
 
@@ -207,7 +249,8 @@ __global__ void __launch_bounds__(1024) distill_loss_kernel(A* out, const A* los
 
 template <typename T, int THREADS, int STEPS>
 static int launch_distill_row(const DistillArgs<typename traits<T>::acc>& g, bool forward) {
-    const int blocks = g.rows < DISTILL_GRID ? g.rows : DISTILL_GRID;
+    // as many workgroups as the CUs hold at a time, each of which walks rows
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256, held = THREADS == 1024 ? distill_waves(THREADS, STEPS, sizeof(T)) / 4 : 8, blocks = g.rows < cus * held ? g.rows : cus * held;
     if (forward) hipLaunchKernelGGL((distill_kernel<T, THREADS, STEPS, true>), dim3(blocks), dim3(THREADS), 0, current_stream(), g);
     else hipLaunchKernelGGL((distill_kernel<T, THREADS, STEPS, false>), dim3(blocks), dim3(THREADS), 0, current_stream(), g);
     return check_launch("distill_kernel") ? 0 : -1;
@@ -217,8 +260,10 @@ template <typename T>
 static int launch_distill(const DistillArgs<typename traits<T>::acc>& g, bool forward) {
     constexpr int N = vec16<T>::N;
     if (g.classes < N || (long long)g.classes > 1024ll * 16 * N) return launch_distill_row<T, 1024, 0>(g, forward);
-    if (g.classes <= 256 * N) return launch_distill_row<T, 256, 1>(g, forward);
-    if (g.classes <= 256 * 4 * N) return launch_distill_row<T, 256, 4>(g, forward);
+    if (g.k > 256) {                               // (an entry a thread)
+        if (g.classes <= 1024 * 2 * N) return launch_distill_row<T, 1024, 2>(g, forward);
+    } else if (g.classes <= 256 * N) return launch_distill_row<T, 256, 1>(g, forward);
+    if (g.k <= 256 && g.classes <= 256 * 4 * N) return launch_distill_row<T, 256, 4>(g, forward);
     if (g.classes <= 1024 * 2 * N) return launch_distill_row<T, 1024, 2>(g, forward);
     if (g.classes <= 1024 * 4 * N) return launch_distill_row<T, 1024, 4>(g, forward);
     if (g.classes <= 1024 * 8 * N) return launch_distill_row<T, 1024, 8>(g, forward);

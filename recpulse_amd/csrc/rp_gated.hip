@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(256) gated_dz_kernel(T* dz, const T* dh, const
         if (n >= N) {
             const RowVector<T> at(c, n);
             T dv[N], og[N], ou[N];
+            A vg[N], vu[N];
             at.load(dv, d);
             A gate[N], up[N];
             __builtin_memcpy(gate, zr + at.at, sizeof(gate));
@@ -108,9 +109,11 @@ __global__ void __launch_bounds__(256) gated_dz_kernel(T* dz, const T* dh, const
 #pragma unroll
             for (int u = 0; u < N; u++) {
                 const A v = widen(dv[u]);
-                og[u] = round_to<T>(v * up[u] * gate_slope<GATE>(gate[u]));
-                ou[u] = round_to<T>(v * gate_value<GATE>(gate[u]));
+                vg[u] = v * up[u] * gate_slope<GATE>(gate[u]);
+                vu[u] = v * gate_value<GATE>(gate[u]);
             }
+            round_vector<T>(og, vg);
+            round_vector<T>(ou, vu);
             at.store(out, og);
             at.store(out + n, ou);
         } else {
@@ -194,7 +197,19 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
         return dtype == RP_DTYPE_BFLOAT16 ? launch_gated16_256_bf16(g, edge) : launch_gated16_256_f16(g, edge);
     }
     const int edge = ragged ? M16_RAGGED : M16_EDGE;
-    return p.bm >= 128 && p.bn >= 128 ? launch_gated16_128(g, edge, dtype) : launch_gated16_64x128(g, edge, dtype);
+    if (g.rows > 64 && p.bm >= 128 && p.bn >= 128) return launch_gated16_128(g, edge, dtype);
+    // Few tiles: k in shares of at least eight slabs, up to three workgroups a CU
+    const long long tiles = (long long)((g.rows + 63) / 64) * ((g.n + 63) / 64), share_bytes = 8ll * g.rows * g.n;
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256, slabs = (g.k + M16_BK - 1) / M16_BK;
+    long long count = 3ll * cus / tiles;
+    if (count > slabs / 8) count = slabs / 8;
+    if (count > (long long)CallScratch::MOST / share_bytes) count = (long long)CallScratch::MOST / share_bytes;
+    if (count >= 2 && !path_disabled("gated_shares")) {
+        const int per = (int)((slabs + count - 1) / count), shares = (slabs + per - 1) / per;
+        const CallScratch memory((size_t)(shares * share_bytes));
+        if (memory.ptr) return launch_gated16_64x128(g, GatedShares{shares, per * M16_BK, (float*)memory.ptr}, edge, dtype);
+    }
+    return launch_gated16_64x128(g, GatedShares{1, 0, nullptr}, edge, dtype);
 }
 
 static bool gated_args_ok(const char* who, bool pointers, int rows, int k, int n, int gate, std::initializer_list<long long> strides, int dtype) {

@@ -3,9 +3,9 @@
 
 namespace rp {
 
-int launch_gated16_64x128(const GatedArgs& l, int edge, int dtype) {
-    if (dtype == RP_DTYPE_BFLOAT16) return edge == M16_RAGGED ? launch_gated16<bf16_t, 64, 128, 2, M16_RAGGED>(l) : launch_gated16<bf16_t, 64, 128, 2, M16_EDGE>(l);
-    return edge == M16_RAGGED ? launch_gated16<f16_t, 64, 128, 2, M16_RAGGED>(l) : launch_gated16<f16_t, 64, 128, 2, M16_EDGE>(l);
+int launch_gated16_64x128(const GatedArgs& l, const GatedShares& shares, int edge, int dtype) {
+    if (dtype == RP_DTYPE_BFLOAT16) return edge == M16_RAGGED ? launch_gated16<bf16_t, 64, 128, 2, M16_RAGGED>(l, shares) : launch_gated16<bf16_t, 64, 128, 2, M16_EDGE>(l, shares);
+    return edge == M16_RAGGED ? launch_gated16<f16_t, 64, 128, 2, M16_RAGGED>(l, shares) : launch_gated16<f16_t, 64, 128, 2, M16_EDGE>(l, shares);
 }
 
 }  // namespace rp

@@ -11,7 +11,7 @@
 namespace rp {
 
 constexpr int NORM_BLOCKS = 512;        // most workgroups of a backward launch, each of which leaves a row of partial sums
-constexpr int NORM_GRID = 1 << 20;      // and of any other, which walk on from there (a launch has fewer than 2^32 threads)
+constexpr int NORM_GRID = 1 << 20;      // and of those for rows that are not held in registers, which walk on from there (a launch has fewer than 2^32 threads)
 static int norm_grid(int blocks) { return blocks < NORM_GRID ? blocks : NORM_GRID; }
 
 template <typename A> struct NormArgs {
@@ -27,57 +27,78 @@ template <typename A> struct NormArgs {
 __device__ __forceinline__ float one_over_root(float v) { return 1.f / sqrtf(v); }
 __device__ __forceinline__ double one_over_root(double v) { return 1.0 / sqrt(v); }
 
+// Where the registers reach, the next row's loads fly while a row is added up, and weight and bias are loaded once
+constexpr bool norm_ahead(int lanes, int steps, int elem) { return elem < 8 && steps * (lanes == 1024 ? 4 : 2) <= 8; }
+
 template <typename T, int LANES, int STEPS>
 __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) layer_norm_kernel(NormArgs<typename traits<T>::acc> g) {
     using A = typename traits<T>::acc;
     constexpr int TEAMS = LANES < 256 ? 256 / LANES : 1, N = vec16<T>::N;
-    __shared__ A room[2 * (LANES / 64)];
-    const int lane = threadIdx.x % LANES;
+    constexpr bool AHEAD = norm_ahead(LANES, STEPS, sizeof(T));
+    __shared__ A room[2][LANES / 64];
+    const int lane = threadIdx.x % LANES, stride = (int)gridDim.x * TEAMS;
+    int row = (int)blockIdx.x * TEAMS + (TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / LANES) : 0);
     RowVector<T> at[STEPS];
+    T next[STEPS][N], w[STEPS][N], b[STEPS][N];
 #pragma unroll
     for (int s = 0; s < STEPS; s++) at[s] = RowVector<T>((s * LANES + lane) * N, g.d);
+    auto load_row = [&](int r) {
+        const T* x = (const T*)g.x + (r < g.rows ? r : g.rows - 1) * g.x_rs;      // (a row again rather than none)
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) at[s].load(next[s], x);
+    };
+    auto load_weights = [&]() {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            if (g.w) at[s].load(w[s], (const T*)g.w);
+            if (g.b) at[s].load(b[s], (const T*)g.b);
+        }
+    };
+    if (AHEAD) load_row(row);
+    if (AHEAD) load_weights();
     // (whole teams; a workgroup of several has no barriers)
-    for (int row = (int)blockIdx.x * TEAMS + (int)threadIdx.x / LANES; row < g.rows; row += (int)gridDim.x * TEAMS) {
-    const T* x = (const T*)g.x + row * g.x_rs;
-    T raw[STEPS][N];
+    for (; row < g.rows; row += stride) {
+        T raw[STEPS][N];
+        if (!AHEAD) load_row(row);
+        __builtin_memcpy(raw, next, sizeof(raw));
+        if (AHEAD) load_row(row + stride);
+        A sum[1] = {};
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) at[s].load(raw[s], x);
-    A sum[1] = {};
+        for (int s = 0; s < STEPS; s++)
 #pragma unroll
-    for (int s = 0; s < STEPS; s++)
+            for (int u = 0; u < N; u++) sum[0] += at[s].has(u) ? widen(raw[s][u]) : (A)0;
+        team_sums_in_turn<LANES>(sum, room[0]);
+        const A mean = sum[0] / (A)g.d;
+        A squares[1] = {};
 #pragma unroll
-        for (int u = 0; u < N; u++) sum[0] += at[s].has(u) ? widen(raw[s][u]) : (A)0;
-    team_sums<LANES>(sum, room);
-    const A mean = sum[0] / (A)g.d;
-    A squares[1] = {};
+        for (int s = 0; s < STEPS; s++)
 #pragma unroll
-    for (int s = 0; s < STEPS; s++)
-#pragma unroll
-        for (int u = 0; u < N; u++) {
-            const A c = at[s].has(u) ? widen(raw[s][u]) - mean : (A)0;
-            squares[0] += c * c;
+            for (int u = 0; u < N; u++) {
+                const A c = at[s].has(u) ? widen(raw[s][u]) - mean : (A)0;
+                squares[0] += c * c;
+            }
+        if (!AHEAD) load_weights();
+        team_sums_in_turn<LANES>(squares, room[1]);
+        const A r = one_over_root(squares[0] / (A)g.d + g.eps);
+        if (g.stats && lane == 0) {
+            g.stats[2 * (long long)row] = mean;
+            g.stats[2 * (long long)row + 1] = r;
         }
-    team_sums<LANES>(squares, room + LANES / 64);
-    const A r = one_over_root(squares[0] / (A)g.d + g.eps);
-    if (g.stats && lane == 0) {
-        g.stats[2 * (long long)row] = mean;
-        g.stats[2 * (long long)row + 1] = r;
-    }
-    T* y = (T*)g.y + row * g.y_rs;
+        T* y = (T*)g.y + row * g.y_rs;
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        T out[N], w[N], b[N];
-        if (g.w) at[s].load(w, (const T*)g.w);
-        if (g.b) at[s].load(b, (const T*)g.b);
+        for (int s = 0; s < STEPS; s++) {
+            T out[N];
+            A value[N];
 #pragma unroll
-        for (int u = 0; u < N; u++) {
-            A h = (widen(raw[s][u]) - mean) * r;
-            if (g.w) h *= widen(w[u]);
-            if (g.b) h += widen(b[u]);
-            out[u] = round_to<T>(h);
+            for (int u = 0; u < N; u++) {
+                A h = (widen(raw[s][u]) - mean) * r;
+                if (g.w) h *= widen(w[s][u]);
+                if (g.b) h += widen(b[s][u]);
+                value[u] = h;
+            }
+            round_vector<T>(out, value);
+            at[s].store(y, out);
         }
-        at[s].store(y, out);
-    }
     }
 }
 
@@ -85,67 +106,81 @@ template <typename T, int LANES, int STEPS, bool WEIGHTS>
 __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) layer_norm_backward_kernel(NormArgs<typename traits<T>::acc> g) {
     using A = typename traits<T>::acc;
     constexpr int TEAMS = LANES < 256 ? 256 / LANES : 1, N = vec16<T>::N;
-    extern __shared__ __attribute__((aligned(16))) char lds[];       // 2 LANES / 64 values; with WEIGHTS and several teams 2 d more
+    constexpr bool AHEAD = norm_ahead(LANES, STEPS, sizeof(T));
+    extern __shared__ __attribute__((aligned(16))) char lds[];       // 4 LANES / 64 values; with WEIGHTS and several teams 2 d more
     A* room = (A*)lds;
-    const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / LANES) : 0, stride = (int)gridDim.x * TEAMS;
     RowVector<T> at[STEPS];
-    A w[STEPS][N], sw[STEPS][N], sb[STEPS][N];
+    T w[STEPS][N], next_x[STEPS][N], next_dy[STEPS][N];
+    A sw[STEPS][N], sb[STEPS][N], next_mean = 0, next_r = 0;
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
         at[s] = RowVector<T>((s * LANES + lane) * N, g.d);
-        T raw[N];
-        if (g.w) at[s].load(raw, (const T*)g.w);
+        if (g.w) at[s].load(w[s], (const T*)g.w);
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            w[s][u] = g.w ? widen(raw[u]) : (A)1;
+            if (!g.w) w[s][u] = round_to<T>((A)1);
             sw[s][u] = sb[s][u] = (A)0;
         }
     }
-    for (int row = (int)blockIdx.x * TEAMS + team; row < g.rows; row += (int)gridDim.x * TEAMS) {
-        T rx[STEPS][N], rg[STEPS][N];
-        const T* x = (const T*)g.x + row * g.x_rs;
-        const T* dy = (const T*)g.dy + row * g.dy_rs;
+    auto load_row = [&](int r) {
+        r = r < g.rows ? r : g.rows - 1;             // (a row again rather than none)
+        const T* x = (const T*)g.x + r * g.x_rs;
+        const T* dy = (const T*)g.dy + r * g.dy_rs;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            at[s].load(rx[s], x);
-            at[s].load(rg[s], dy);
+            at[s].load(next_x[s], x);
+            at[s].load(next_dy[s], dy);
         }
-        const A mean = g.stats[2 * (long long)row], r = g.stats[2 * (long long)row + 1];
+        next_mean = g.stats[2 * (long long)r];
+        next_r = g.stats[2 * (long long)r + 1];
+    };
+    int row = (int)blockIdx.x * TEAMS + team;
+    if (AHEAD) load_row(row);
+    for (int turn = 0; row < g.rows; row += stride, turn ^= 1) {
+        T rx[STEPS][N], rg[STEPS][N];
+        if (!AHEAD) load_row(row);
+        __builtin_memcpy(rx, next_x, sizeof(rx));
+        __builtin_memcpy(rg, next_dy, sizeof(rg));
+        const A mean = next_mean, r = next_r;
+        if (AHEAD) load_row(row + stride);
         A sums[2] = {};
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
             for (int u = 0; u < N; u++) {
-                const A h = at[s].has(u) ? (widen(rx[s][u]) - mean) * r : (A)0, d = at[s].has(u) ? widen(rg[s][u]) : (A)0;
-                sums[0] += d * w[s][u];
-                sums[1] += d * w[s][u] * h;
+                const A h = at[s].has(u) ? (widen(rx[s][u]) - mean) * r : (A)0, d = at[s].has(u) ? widen(rg[s][u]) : (A)0, dw = d * widen(w[s][u]);
+                sums[0] += dw;
+                sums[1] += dw * h;
                 if constexpr (WEIGHTS) {
                     sw[s][u] += d * h;
                     sb[s][u] += d;
                 }
             }
         if (!g.dx) continue;
-        team_sums<LANES>(sums, room);
+        team_sums_in_turn<LANES>(sums, room + turn * 2 * (LANES / 64));
         const A c0 = sums[0] / (A)g.d, c1 = sums[1] / (A)g.d;
         T* dx = (T*)g.dx + row * g.dx_rs;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             T out[N], was[N];
+            A value[N];
             if (g.accumulate_dx) at[s].load(was, dx);
 #pragma unroll
             for (int u = 0; u < N; u++) {
                 const A h = (widen(rx[s][u]) - mean) * r;
-                A v = r * (widen(rg[s][u]) * w[s][u] - c0 - h * c1);
+                A v = r * (widen(rg[s][u]) * widen(w[s][u]) - c0 - h * c1);
                 if (g.accumulate_dx) v += widen(was[u]);
-                out[u] = round_to<T>(v);
+                value[u] = v;
             }
+            round_vector<T>(out, value);
             at[s].store(dx, out);
         }
     }
     if constexpr (WEIGHTS) {
         A* part = g.partials + (long long)blockIdx.x * 2 * g.d;
         if constexpr (TEAMS > 1) {                 // the teams add to the workgroup's row one after the other
-            A* sum = room + 2 * (LANES / 64);
+            A* sum = room + 4 * (LANES / 64);
             for (int i = 0; i < TEAMS; i++) {
                 if (team == i)
 #pragma unroll
@@ -295,12 +330,13 @@ static int launch_norm_team(const NormArgs<typename traits<T>::acc>& g, bool bac
     using A = typename traits<T>::acc;
     constexpr int TEAMS = LANES < 256 ? 256 / LANES : 1, THREADS = LANES < 256 ? 256 : LANES;
     if (!backward) {
-        hipLaunchKernelGGL((layer_norm_kernel<T, LANES, STEPS>), dim3(norm_grid((g.rows + TEAMS - 1) / TEAMS)), dim3(THREADS), 0, current_stream(), g);
+        const int cus = device_cu_count() > 0 ? device_cu_count() : 256, all = (g.rows + TEAMS - 1) / TEAMS, resident = cus * (2048 / THREADS);
+        hipLaunchKernelGGL((layer_norm_kernel<T, LANES, STEPS>), dim3(all < resident ? all : resident), dim3(THREADS), 0, current_stream(), g);
         return check_launch("layer_norm_kernel") ? 0 : -1;
     }
     const bool weights = g.dw || g.db;
     const int blocks = norm_blocks(g.rows, NormPlan{LANES, STEPS});
-    const size_t lds = sizeof(A) * (2 * (LANES / 64) + (weights && TEAMS > 1 ? 2 * (size_t)g.d : 0));
+    const size_t lds = sizeof(A) * (4 * (LANES / 64) + (weights && TEAMS > 1 ? 2 * (size_t)g.d : 0));
     if (weights) hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, STEPS, true>), dim3(blocks), dim3(THREADS), lds, current_stream(), g);
     else hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, STEPS, false>), dim3(blocks), dim3(THREADS), lds, current_stream(), g);
     if (!check_launch("layer_norm_backward_kernel")) return -1;

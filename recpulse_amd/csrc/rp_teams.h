@@ -40,6 +40,23 @@ template <typename T> struct RowVector {
     }
 };
 
+// Eight, four or two sums rounded to a 16-byte vector, 16-bit ones two to an instruction
+template <typename T> __device__ __forceinline__ void round_vector(T (&out)[vec16<T>::N], const typename traits<T>::acc (&v)[vec16<T>::N]) {
+    if constexpr (sizeof(T) == 2) {
+        using half_t = std::conditional_t<std::is_same<T, bf16_t>::value, __bf16, _Float16>;
+        typedef half_t __attribute__((ext_vector_type(2))) half2_t;
+        typedef float __attribute__((ext_vector_type(2))) float2_t;
+#pragma unroll
+        for (int u = 0; u < vec16<T>::N; u += 2) {
+            const half2_t pair = __builtin_convertvector((float2_t{v[u], v[u + 1]}), half2_t);
+            __builtin_memcpy(&out[u], &pair, 4);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < vec16<T>::N; u++) out[u] = round_to<T>(v[u]);
+    }
+}
+
 // The sum (largest) of a value over the wave, in every lane
 template <typename A> __device__ __forceinline__ A wave_sum(A v) {
 #pragma unroll
@@ -68,6 +85,41 @@ template <int LANES, int N, typename A> __device__ __forceinline__ void team_sum
             v[i] = room[i * WAVES];
 #pragma unroll
             for (int w = 1; w < WAVES; w++) v[i] += room[i * WAVES + w];
+        }
+    }
+}
+// The same in a loop that uses two rooms in turn: the other one's barrier lies between a room's last readers and its next writers
+template <int LANES, int N, typename A> __device__ __forceinline__ void team_sums_in_turn(A (&v)[N], A* room) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) room[i * WAVES + threadIdx.x / 64] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = room[i * WAVES];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v[i] += room[i * WAVES + w];
+        }
+    }
+}
+template <int LANES, int N, typename A> __device__ __forceinline__ void team_tops_in_turn(A (&v)[N], A* room) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_max(v[i]);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) room[i * WAVES + threadIdx.x / 64] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = room[i * WAVES];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v[i] = larger(v[i], room[i * WAVES + w]);
         }
     }
 }

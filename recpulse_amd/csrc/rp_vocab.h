@@ -32,10 +32,12 @@ private:
     long long used_ = 0;
 };
 
+// The result from the rows' losses in stats, and how many rows have a target (rp_vocab.hip)
+int vocab_result_f32(float* loss_out, float* stats, const VocabArgs& g);
 // bf16 / fp16 on MFMA tiles (rp_vocab16.hip): operands with a unit stride and rows of at least a 16-byte vector
 bool vocab16_takes(const VocabArgs& g, int dtype);
 long long vocab16_room(int rows, int k, int classes, bool backward);      // bytes of its workspace
-int vocab16_forward(float* stats, const VocabArgs& g, void* workspace, int dtype);      // the rows' log sums and losses
+int vocab16_forward(float* loss_out, float* stats, const VocabArgs& g, void* workspace, int dtype);
 int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats, const float* upstream, void* workspace, int dtype);
 
 }  // namespace rp

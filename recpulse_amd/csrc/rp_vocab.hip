@@ -189,6 +189,8 @@ static int vocab_result(void* loss_out, void* stats, const VocabArgs& g) {
     return check_launch("vocab_loss_kernel") ? 0 : -1;
 }
 
+int vocab_result_f32(float* loss_out, float* stats, const VocabArgs& g) { return vocab_result<float>(loss_out, stats, g); }
+
 template <typename T>
 static int vocab_any_forward(void* stats, const VocabArgs& g, void* workspace) {
     using A = typename traits<T>::acc;
@@ -266,11 +268,8 @@ int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void*
                                         long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype) {
     if (!vocab_args_ok("rp_hip_linear_cross_entropy_forward", loss_out && stats && x && w && targets && workspace, rows, k, classes, reduction, {x_rs, x_cs, w_rs, w_cs}, dtype)) return -1;
     const VocabArgs g{x, w, bias, targets, rows, k, classes, reduction, x_rs, x_cs, w_rs, w_cs};
-    if (vocab16_takes(g, dtype)) {
-        if (vocab16_forward((float*)stats, g, workspace, dtype) != 0) return -1;
-    } else {
-        RP_DISPATCH_DTYPE(dtype, if (vocab_any_forward<T>(stats, g, workspace) != 0) return -1);
-    }
+    if (vocab16_takes(g, dtype)) return vocab16_forward((float*)loss_out, (float*)stats, g, workspace, dtype);
+    RP_DISPATCH_DTYPE(dtype, if (vocab_any_forward<T>(stats, g, workspace) != 0) return -1);
     return dtype == RP_DTYPE_FLOAT64 ? vocab_result<double>(loss_out, stats, g) : vocab_result<float>(loss_out, stats, g);
 }
 

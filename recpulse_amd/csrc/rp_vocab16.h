@@ -29,8 +29,11 @@ struct VocabTileArgs {
     float* db_parts;               // [groups of rows][pitch], or null
     // dx, dw
     const float* scale;            // what d has been multiplied by, inverted
-    float* sums;                   // dx between pieces, tile by tile
+    float* sums;                   // dx between pieces and sums of shares of k, tile by tile in the order of a tile's registers
     int first, last;
+    // k in shares of k_share that workgroups of their own add up (their sums `share_stride` floats apart), where there are few tiles; 1: none
+    int shares, k_share;
+    long long share_stride;
 };
 
 // The value of v in the lane's other lanes of one row of accumulators (MT of them), joined by f
@@ -40,7 +43,10 @@ template <int MT, typename F> __device__ __forceinline__ float over_row(float v,
     v = f(v, dpp(v, std::integral_constant<int, 0x124>{}));
     v = f(v, dpp(v, std::integral_constant<int, 0x122>{}));
     v = f(v, dpp(v, std::integral_constant<int, 0x121>{}));
-    if constexpr (MT == 32) v = f(v, __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401f)));      // the lane 16 away
+    if constexpr (MT == 32) {                                     // the lane 16 away: both halves of 32 lanes, each in both
+        const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(both[0]), __uint_as_float(both[1]));
+    }
     return v;
 }
 
@@ -88,30 +94,51 @@ struct VocabForward : M16Source {
         float* hits = a.hits + m0 + row0;
         const int* row_target = target + row0;
         const int left = a.g.m - m0 - row0;                  // rows behind the lane's first one
-        static_for<0, TMI * NV>([&](auto ivc) {
-            constexpr int i = decltype(ivc)::value / NV, v = decltype(ivc)::value % NV;
-            constexpr int r = patch_step<MT>(i, v);
-            float z[TNI];
-            static_for<0, TNI>([&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                z[j] = in[j] ? acc[i][j][v] + bias[j] : -INFINITY;
-            });
-            float top = z[0];
-            static_for<1, TNI>([&](auto jc) { top = fmaxf(top, z[decltype(jc)::value]); });
-            top = over_row<MT>(top, [](float x, float y) { return fmaxf(x, y); });
-            const float base = top == -INFINITY ? 0.f : top;
-            float sum = exp_less(z[0], base);
-            static_for<1, TNI>([&](auto jc) { sum += exp_less(z[decltype(jc)::value], base); });
-            sum = over_row<MT>(sum, [](float x, float y) { return x + y; });
-            if (lane % MT == 0 && r < left) part[r] = VocabPart{top, sum};
-            const int c = row_target[r] - column0;
-            if (__builtin_amdgcn_ballot_w64(c >= 0 && c < WN && c % MT == 0)) {
+        constexpr int RB = MT == 16 ? 2 : 8;                  // rows at a time: what one waits for the others cover
+        static_for<0, TMI * NV / RB>([&](auto qc) {
+            constexpr int i = decltype(qc)::value / (NV / RB), v = decltype(qc)::value % (NV / RB) * RB;
+            int at[RB];
+            static_for<0, RB>([&](auto ec) { at[decltype(ec)::value] = row_target[patch_step<MT>(i, v + decltype(ec)::value)] - column0; });
+            float z[RB][TNI], top[RB], base[RB], sum[RB];
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
                 static_for<0, TNI>([&](auto jc) {
                     constexpr int j = decltype(jc)::value;
-                    if (c == j * MT && r < left && in[j]) hits[r] = z[j];
+                    z[e][j] = in[j] ? acc[i][j][v + e] + bias[j] : -INFINITY;
+                    top[e] = j == 0 ? z[e][0] : fmaxf(top[e], z[e][j]);
+                });
+            });
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                top[e] = over_row<MT>(top[e], [](float x, float y) { return fmaxf(x, y); });
+                base[e] = top[e] == -INFINITY ? 0.f : top[e];
+            });
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                sum[e] = exp_less(z[e][0], base[e]);
+                static_for<1, TNI>([&](auto jc) { sum[e] += exp_less(z[e][decltype(jc)::value], base[e]); });
+            });
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                sum[e] = over_row<MT>(sum[e], [](float x, float y) { return x + y; });
+            });
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value, r = patch_step<MT>(i, v + e);
+                if (lane % MT == 0 && r < left) part[r] = VocabPart{top[e], sum[e]};
+            });
+            bool any = false;
+            static_for<0, RB>([&](auto ec) { const int c = at[decltype(ec)::value]; any = any || (c >= 0 && c < WN && c % MT == 0); });
+            if (__builtin_amdgcn_ballot_w64(any)) {
+                static_for<0, RB>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value, r = patch_step<MT>(i, v + e);
+                    const int c = at[e];
+                    static_for<0, TNI>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        if (c == j * MT && r < left && in[j]) hits[r] = z[e][j];
+                    });
                 });
             }
-            __builtin_amdgcn_sched_barrier(0);               // (rows mixed with each other take more registers than there are)
+            __builtin_amdgcn_sched_barrier(0);               // (all rows mixed with each other take more registers than there are)
         });
         return true;
     }
@@ -147,16 +174,20 @@ struct VocabGradient : M16Source {
         const float *row_lse = lse + wm0 + row0, *row_f = f + wm0 + row0;
         const int* row_target = target + wm0 + row0;
         uint16_t* staged = region + row0 * EP + lane % MT;
-        static_for<0, TMI * NV>([&](auto ivc) {
-            constexpr int i = decltype(ivc)::value / NV, v = decltype(ivc)::value % NV, r = patch_step<MT>(i, v);
-            const float l = row_lse[r], fr = row_f[r];
-            const int c = row_target[r] - column0;
-            static_for<0, TNI>([&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v] + bias[j], LOG2_E, -l)) - (c == j * MT ? 1.f : 0.f);
-                const float d = in[j] && fr != 0.f ? p * fr : 0.f;      // (a row without a target has no gradient, whatever its logits are)
-                column[j] += d;
-                staged[r * EP + j * MT] = round_to<T>(d).bits;
+        constexpr int RB = 2;
+        static_for<0, TMI * NV / RB>([&](auto qc) {
+            constexpr int i = decltype(qc)::value / (NV / RB), v = decltype(qc)::value % (NV / RB) * RB;
+            static_for<0, RB>([&](auto ec) {
+                constexpr int e = decltype(ec)::value, r = patch_step<MT>(i, v + e);
+                const float l = row_lse[r], fr = row_f[r];
+                const int c = row_target[r] - column0;
+                static_for<0, TNI>([&](auto jc) {
+                    constexpr int j = decltype(jc)::value;
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v + e] + bias[j], LOG2_E, -l)) - (c == j * MT ? 1.f : 0.f);
+                    const float d = in[j] && fr != 0.f ? p * fr : 0.f;      // (a row without a target has no gradient, whatever its logits are)
+                    column[j] += d;
+                    staged[r * EP + j * MT] = round_to<T>(d).bits;
+                });
             });
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -193,7 +224,8 @@ struct VocabGradProduct : M16Source {
     template <typename T, int MT, int WGN, int TMI, int TNI, int EDGE, typename ACC>
     __device__ __forceinline__ bool take(ACC (&acc)[TMI][TNI], uint16_t*, int m0, int n0) {
         constexpr int NV = MT == 32 ? 16 : 4, BM = 4 / WGN * TMI * MT, BN = WGN * TNI * MT;
-        f32x4_t* own = (f32x4_t*)(a.sums + ((long long)(m0 / BM) * a.tiles_n + n0 / BN) * (BM * BN)) + thread_again();
+        const int share = a.shares > 1 ? (int)blockIdx.x / a.total : 0;
+        f32x4_t* own = (f32x4_t*)(a.sums + share * a.share_stride + ((long long)(m0 / BM) * a.tiles_n + n0 / BN) * (BM * BN)) + thread_again();
         if (!a.first) {
             static_for<0, TMI * TNI * NV / 4>([&](auto qc) {
                 constexpr int q = decltype(qc)::value, i = q / (TNI * NV / 4), j = q / (NV / 4) % TNI, v = q % (NV / 4) * 4;
@@ -203,7 +235,7 @@ struct VocabGradProduct : M16Source {
                 if constexpr (q % 16 == 15) __builtin_amdgcn_sched_barrier(0);
             });
         }
-        if (a.last) return false;
+        if (a.last && a.shares == 1) return false;
         static_for<0, TMI * TNI * NV / 4>([&](auto qc) {
             constexpr int q = decltype(qc)::value, i = q / (TNI * NV / 4), j = q / (NV / 4) % TNI, v = q % (NV / 4) * 4;
             own[q * 256] = f32x4_t{acc[i][j][v], acc[i][j][v + 1], acc[i][j][v + 2], acc[i][j][v + 3]};
@@ -215,9 +247,46 @@ struct VocabGradProduct : M16Source {
 template <typename SRC, typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE>
 __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) vocab16_kernel(VocabTileArgs args) {
     SRC source(args);
+    int slot = blockIdx.x, stride = gridDim.x;
     // (one plain matrix: the options that GemmArgs has beside are known to be unused here)
-    const GemmArgs g{args.g.C, args.g.A, args.g.B, args.g.bias, 1, args.g.m, args.g.k, args.g.n, 0, A_MC ? 1 : args.g.a_rs, A_MC ? args.g.a_cs : 1, 0, B_MC ? args.g.b_rs : 1, B_MC ? 1 : args.g.b_cs, 0, args.g.c_rs, 1, args.g.accumulate};
-    gemm_mfma16_block<T, BM, BN, WGM, A_MC, B_MC, EDGE, false, 1, SRC>(g, args.tiles_m, args.tiles_n, nullptr, 0, args.total, (int)blockIdx.x, 0, (int)gridDim.x, &source);
+    GemmArgs g{args.g.C, args.g.A, args.g.B, args.g.bias, 1, args.g.m, args.g.k, args.g.n, 0, A_MC ? 1 : args.g.a_rs, A_MC ? args.g.a_cs : 1, 0, B_MC ? args.g.b_rs : 1, B_MC ? 1 : args.g.b_cs, 0, args.g.c_rs, 1, args.g.accumulate};
+    if constexpr (std::is_same<SRC, VocabGradProduct<true>>::value && BM != 256) {
+        if (args.shares > 1) {
+            const int share = slot / args.total, k0 = share * args.k_share;
+            slot -= share * args.total;
+            stride = args.total;
+            g.A = (const T*)g.A + k0 * g.a_cs;
+            g.B = (const T*)g.B + k0 * g.b_rs;
+            g.k = g.k - k0 < args.k_share ? g.k - k0 : args.k_share;
+        }
+    }
+    gemm_mfma16_block<T, BM, BN, WGM, A_MC, B_MC, EDGE, false, 1, SRC>(g, args.tiles_m, args.tiles_n, nullptr, 0, args.total, slot, 0, stride, &source);
+}
+
+// What the shares of k add up to, in their order, scaled and rounded: a workgroup four quads of a tile's registers (tiles of 32 x 32 MFMAs, two by two waves)
+template <typename T, int BM>
+__global__ void __launch_bounds__(256) vocab16_join_kernel(VocabTileArgs a) {
+    constexpr int TM = BM / 64, QUADS = TM * TM * 4;
+    const int tile = blockIdx.x / (QUADS / 4), q0 = blockIdx.x % (QUADS / 4) * 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int m0 = tile / a.tiles_n * BM + wave / 2 * (BM / 2), n0 = tile % a.tiles_n * BM + wave % 2 * (BM / 2);
+    const f32x4_t* own = (const f32x4_t*)(a.sums + (long long)tile * (BM * BM)) + threadIdx.x;
+    f32x4_t sum[4] = {};
+    for (int s = 0; s < a.shares; s++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] += *(const f32x4_t*)((const float*)(own + (q0 + e) * 256) + s * a.share_stride);
+    const float scale = *a.scale;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int i = (q0 + e) / (TM * 4), j = (q0 + e) / 4 % TM, col = n0 + j * 32 + (lane & 31), row = m0 + i * 32 + 8 * e + 4 * (lane >> 5);
+        if (col >= a.g.n) continue;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (row + u >= a.g.m) continue;
+            T* to = (T*)a.g.C + (row + u) * a.g.c_rs + col;
+            const T y = round_to<T>(sum[e][u] * scale);
+            *to = a.g.accumulate ? round_to<T>(widen(*to) + widen(y)) : y;
+        }
+    }
 }
 
 template <typename SRC, typename T, int BM, int BN, int WGM, bool A_MC, bool B_MC, int EDGE>
@@ -229,11 +298,20 @@ static int launch_vocab16_tile(VocabTileArgs a) {
     const size_t staged = VocabGradient::rows_at(BM, BN, WGM) + 12 * BM;
     if (std::is_same<SRC, VocabGradient>::value && staged > smem) smem = staged;
     const int cus = device_cu_count() / 8 * 8;
-    const int blocks = BM == 256 && BN == 256 && cus >= 8 && a.total > cus ? cus : a.total;      // one resident workgroup a CU, as for a product of its own
+    int blocks = BM == 256 && BN == 256 && cus >= 8 && a.total > cus ? cus : a.total;      // one resident workgroup a CU, as for a product of its own
+    if (a.shares > 1) blocks = a.total * a.shares;
     auto kern = vocab16_kernel<SRC, T, BM, BN, WGM, A_MC, B_MC, EDGE>;
     if (smem > 64 * 1024 && !check_hip(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "hipFuncSetAttribute")) return -1;
     hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), smem, current_stream(), a);
-    return check_launch("vocab16_kernel") ? 0 : -1;
+    if (!check_launch("vocab16_kernel")) return -1;
+    if constexpr (std::is_same<SRC, VocabGradProduct<true>>::value && BM != 256) {
+        if (a.shares > 1 && a.last) {
+            constexpr int TM = BM / 64;
+            hipLaunchKernelGGL((vocab16_join_kernel<T, BM>), dim3(a.tiles_m * a.tiles_n * TM * TM), dim3(256), 0, current_stream(), a);
+            return check_launch("vocab16_join_kernel") ? 0 : -1;
+        }
+    }
+    return 0;
 }
 
 // The launchers of a tile's translation unit.  logits: W row-major (b_mc) or its transpose; dx: likewise (b_mc where W is the transpose); dw: x^T . d or d^T . x.
@@ -245,7 +323,7 @@ static int launch_vocab16_logits(const VocabTileArgs& a, VocabStep step, bool b_
 }
 template <typename T, int BM, int BN, int WGM, int EDGE>
 static int launch_vocab16_grads(const VocabTileArgs& a, VocabStep step, bool b_mc) {
-    if (step == VOCAB_DW) return launch_vocab16_tile<VocabGradProduct<false>, T, BM, BN, WGM, true, true, EDGE>(a);
+    if (step == VOCAB_DW) return launch_vocab16_tile<VocabGradProduct<(BM < 256)>, T, BM, BN, WGM, true, true, EDGE>(a);
     return b_mc ? launch_vocab16_tile<VocabGradProduct<true>, T, BM, BN, WGM, false, true, EDGE>(a) : launch_vocab16_tile<VocabGradProduct<true>, T, BM, BN, WGM, false, false, EDGE>(a);
 }
 

@@ -19,17 +19,21 @@ static int worse16(int a, int b) { return a > b ? a : b; }
 
 // edge 256, 128 or 64 and what of it may hang over
 struct VocabTile { int edge, over; };
-static VocabTile vocab_tile(int m, int n, int k, bool a_mc, bool b_mc, int lie) {
+static VocabTile vocab_tile(int m, int n, int k, bool gradient, bool a_mc, bool b_mc, int lie) {
     Plan p{FAM_MFMA16, 64, 64, a_mc, b_mc, true, ""};
     p.ragged = lie == LIES_RAGGED;
     choose_tile16(p, 1, m, k, n);
+    // (a gradient's few tiles of 128 share k among workgroups, below; fp16, both passes, us with dx on 64 and 128: 1000 rows, 520 -> 10007 155 / 149, 512, 2048 -> 32000 361 / 335, 2000, 256 -> 50000 572 / 534)
+    if (gradient && p.bm != 256 && m > 64 && n > 64 && k >= 16 * M16_BK) p.bm = p.bn = 128;
+    // (logits of four slabs: the epilogue is most of the work, and tiles of 128 have two workgroups a CU for it; 2000 rows, 256 -> 50000, forward 176 / 167)
+    if (!gradient && p.bm == 256 && k <= 4 * M16_BK) p.bm = p.bn = 128;
     if (p.ragged) return {p.bm >= 128 && p.bn >= 128 ? 128 : 64, M16_RAGGED};
     if (p.bm == 256 && p.bn == 256) return {256, m % 256 || n % 256 || k % M16_BK ? M16_EDGE : M16_WHOLE};
     return {p.bm >= 128 && p.bn >= 128 ? 128 : 64, M16_EDGE};
 }
 
 static int launch_logits(const VocabTileArgs& a, VocabStep step, bool b_mc, int lie, int dtype) {
-    const VocabTile t = vocab_tile(a.g.m, a.g.n, a.g.k, false, b_mc, lie);
+    const VocabTile t = vocab_tile(a.g.m, a.g.n, a.g.k, false, false, b_mc, lie);
     if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_vocab16_logits_256_bf16(a, step, b_mc, t.over) : launch_vocab16_logits_256_f16(a, step, b_mc, t.over);
     return t.edge == 128 ? launch_vocab16_logits_128(a, step, b_mc, t.over, dtype) : launch_vocab16_logits_64x128(a, step, b_mc, t.over, dtype);
 }
@@ -37,9 +41,9 @@ static int launch_grads(const VocabTileArgs& a, VocabStep step, bool b_mc, const
     if (t.edge == 256) return dtype == RP_DTYPE_BFLOAT16 ? launch_vocab16_grads_256_bf16(a, step, b_mc, t.over) : launch_vocab16_grads_256_f16(a, step, b_mc, t.over);
     return t.edge == 128 ? launch_vocab16_grads_128(a, step, b_mc, t.over, dtype) : launch_vocab16_grads_64(a, step, b_mc, t.over, dtype);
 }
-// Columns that a wave's patch of logits has on the tile of that edge, rows that a group of db's partial sums has
+// Columns of a wave's patch of logits (what a part of a row's sum comes from) and its rows (of a column's), by the tile's edge in rows; the smallest tile has 64 rows and 128 columns
 static int patch_columns(int edge) { return edge == 256 ? 128 : 64; }
-static int patch_rows(int edge) { return edge == 256 ? 128 : edge == 128 ? 64 : 32; }
+static int patch_rows(int edge) { return edge / 2; }
 
 static int logits_lie(const VocabArgs& g) {
     return worse16(lies16(g.x, g.x_rs, g.k), g.w_cs == 1 ? lies16(g.w, g.w_rs, g.classes) : lies16(g.w, g.w_cs, g.k));
@@ -49,40 +53,87 @@ bool vocab16_takes(const VocabArgs& g, int dtype) {
     return logits_lie(g) != LIES_NEITHER;
 }
 
+// Few tiles and a long k: k goes in shares to workgroups of their own, three a CU, at least eight slabs each.  (fp16, 1000 rows, 520 -> 10007: dx on 144 tiles of 64 walks 157 slabs; us in
+// one share and in four with the launch that joins them: see the measured table)
+constexpr long long VOCAB16_SHARE_BYTES = 32ll << 20;      // of the shares' sums
+struct Shares { int count, k; long long stride; };
+static Shares vocab_shares(int m, int n, int k, const VocabTile& t) {
+    const Shares one{1, k, 0};
+    if (t.edge == 256 || path_disabled("vocab_shares")) return one;
+    const long long tiles = (long long)((m + t.edge - 1) / t.edge) * ((n + t.edge - 1) / t.edge), area = tiles * t.edge * t.edge;
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256, slabs = (k + M16_BK - 1) / M16_BK;
+    long long count = 3ll * cus / tiles;
+    if (count > slabs / 8) count = slabs / 8;
+    if (count > 16) count = 16;
+    if (count > VOCAB16_SHARE_BYTES / (area * 4)) count = VOCAB16_SHARE_BYTES / (area * 4);
+    if (count < 2) return one;
+    const int per = (int)((slabs + count - 1) / count);
+    return {(slabs + per - 1) / per, per * M16_BK, area};
+}
+// Bytes that the sums of an output of m x n may take: the shares' where there are any, whichever tiles are taken
+static long long share_bytes(long long m, long long n) {
+    const long long area = (m + 127) / 128 * 128 * ((n + 127) / 128 * 128) * 4;
+    return area * 16 < VOCAB16_SHARE_BYTES ? area * 16 : VOCAB16_SHARE_BYTES;
+}
+
 // ---- small launches ----
 
-// A row's log sum and loss from its groups' parts: 64 rows to a workgroup, sixteen waves that take every sixteenth group
-__global__ void __launch_bounds__(1024) vocab16_rows_kernel(float* stats, const VocabPart* parts, const float* hits, const int* targets, int rows, int classes, int groups) {
-    __shared__ VocabPart room[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    for (int row0 = blockIdx.x * 64; row0 < rows; row0 += gridDim.x * 64) {
-        const int row = row0 + lane;
-        float top = -INFINITY, sum = 0.f;
+// A row's log sum and loss from its groups' parts, ROWS rows to a workgroup: 16, four lanes of every wave to a row, so that 64 groups are read at a time in whole cache lines; or 64 where there are no
+// more, whose workgroup leaves the result too
+__device__ __forceinline__ VocabPart joined_parts(const VocabPart& p, const VocabPart& q) {
+    const float top = fmaxf(p.top, q.top), base = top == -INFINITY ? 0.f : top;
+    return VocabPart{top, p.sum * exp_less(p.top, base) + q.sum * exp_less(q.top, base)};
+}
+template <int ROWS>
+__global__ void __launch_bounds__(1024) vocab16_rows_kernel(float* stats, const VocabPart* parts, const float* hits, const int* targets, int rows, int classes, int groups, float* out, int reduction) {
+    constexpr int SLICES = 1024 / ROWS, BATCH = 8;
+    __shared__ VocabPart room[16][ROWS];
+    const int r = threadIdx.x % ROWS, slice = threadIdx.x / ROWS, wave = threadIdx.x / 64;
+    for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+        const int row = row0 + r;
+        VocabPart own{-INFINITY, 0.f};
         if (row < rows)
-            for (int i0 = wave; i0 < groups; i0 += 16 * 8) {
-                VocabPart p[8];
+            for (int i0 = slice; i0 < groups; i0 += SLICES * BATCH) {
+                VocabPart p[BATCH];
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = i0 + 16 * e < groups ? parts[(long long)(i0 + 16 * e) * rows + row] : VocabPart{-INFINITY, 0.f};
-                float most = top;
+                for (int e = 0; e < BATCH; e++) p[e] = i0 + SLICES * e < groups ? parts[(long long)(i0 + SLICES * e) * rows + row] : VocabPart{-INFINITY, 0.f};
+                float most = own.top;
 #pragma unroll
-                for (int e = 0; e < 8; e++) most = fmaxf(most, p[e].top);
+                for (int e = 0; e < BATCH; e++) most = fmaxf(most, p[e].top);
                 const float base = most == -INFINITY ? 0.f : most;
-                sum *= exp_less(top, base);
+                own.sum *= exp_less(own.top, base);
 #pragma unroll
-                for (int e = 0; e < 8; e++) sum += p[e].sum * exp_less(p[e].top, base);
-                top = most;
+                for (int e = 0; e < BATCH; e++) own.sum += p[e].sum * exp_less(p[e].top, base);
+                own.top = most;
             }
+#pragma unroll
+        for (int d = ROWS; d < 64; d *= 2) own = joined_parts(own, VocabPart{__shfl_xor(own.top, d), __shfl_xor(own.sum, d)});
         __syncthreads();
-        room[wave][lane] = VocabPart{top, sum};
+        if ((threadIdx.x & 63) < ROWS) room[wave][r] = own;
         __syncthreads();
-        if (wave || row >= rows) continue;
-        for (int w = 1; w < 16; w++) top = fmaxf(top, room[w][lane].top);
+        if (threadIdx.x >= ROWS) continue;
+        const bool there = row < rows;
+        float top = room[0][r].top, sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < 16; w++) top = fmaxf(top, room[w][r].top);
         const float base = top == -INFINITY ? 0.f : top;
-        sum = 0.f;
-        for (int w = 0; w < 16; w++) sum += room[w][lane].sum * exp_less(room[w][lane].top, base);
+#pragma unroll
+        for (int w = 0; w < 16; w++) sum += room[w][r].sum * exp_less(room[w][r].top, base);
         const float lse = base + logf(sum);
-        stats[row] = lse;
-        stats[rows + row] = targets[row] >= 0 && targets[row] < classes ? lse - hits[row] : 0.f;
+        const bool held = there && targets[row] >= 0 && targets[row] < classes;
+        const float loss = held ? lse - hits[row] : 0.f;
+        if (there) {
+            stats[row] = lse;
+            stats[rows + row] = loss;
+        }
+        if constexpr (ROWS == 64) {
+            if (reduction == 0 && there) out[row] = loss;
+            const double total = wave_sum((double)loss), count = wave_sum(held ? 1.0 : 0.0);
+            if (r == 0) {
+                stats[2ll * rows] = (float)count;
+                if (reduction) out[0] = (float)(reduction == 1 ? total / (count > 0 ? count : 1.0) : total);
+            }
+        }
     }
 }
 
@@ -130,7 +181,7 @@ __global__ void __launch_bounds__(1024) vocab16_db_kernel(T* db, const float* pa
 
 struct Vocab16Room {
     VocabPart* parts;
-    float *hits, *f, *scale, *db_parts, *sums;
+    float *hits, *f, *scale, *db_parts, *sums, *dw_sums;
     uint16_t* d;
     int piece, pitch;
     Vocab16Room(VocabRoom& room, int rows, int k, int classes, bool backward) {
@@ -140,14 +191,16 @@ struct Vocab16Room {
         piece = pitch = (int)(fits < 256 ? 256 : fits < all ? (fits < reach ? fits : reach) : all < reach ? all : reach);
         if (!backward) {
             hits = room.take<float>(rows);
-            parts = room.take<VocabPart>((long long)rows * ((classes + 255ll) / 256 * 4));
+            parts = room.take<VocabPart>((long long)rows * ((classes + 255ll) / 256 * 4));      // (a wave's patch has 64 columns or more)
             return;
         }
         f = room.take<float>(rows);
         scale = room.take<float>(1);
         d = room.take<uint16_t>((long long)rows * pitch);
         db_parts = room.take<float>(((long long)rows + 255) / 256 * 8 * pitch);
-        sums = room.take<float>(classes > piece ? (rows + 255ll) / 256 * 256 * ((k + 255ll) / 256 * 256) : 0);
+        const long long between = classes > piece ? (rows + 255ll) / 256 * 256 * ((k + 255ll) / 256 * 256) : 0, shares = share_bytes(rows, k) / 4;
+        sums = room.take<float>(between > shares ? between : shares);
+        dw_sums = room.take<float>(share_bytes(k, classes < piece ? classes : piece) / 4);
         hits = nullptr;
         parts = nullptr;
     }
@@ -167,22 +220,27 @@ long long vocab16_room(int rows, int k, int classes, bool backward) {
 
 // ---- the passes ----
 
-int vocab16_forward(float* stats, const VocabArgs& g, void* workspace, int dtype) {
+int vocab16_forward(float* loss_out, float* stats, const VocabArgs& g, void* workspace, int dtype) {
     VocabRoom room(workspace);
     const Vocab16Room r(room, g.rows, g.k, g.classes, false);
     const bool b_mc = g.w_cs == 1;
     const int lie = logits_lie(g);
     VocabTileArgs a{};
+    a.shares = 1;
     a.g = GemmArgs{nullptr, g.x, g.w, g.bias, 1, g.rows, g.k, g.classes, 0, g.x_rs, 1, 0, g.w_rs, g.w_cs};
     a.targets = g.targets;
     a.classes = g.classes;
     a.parts = r.parts;
     a.hits = r.hits;
     if (launch_logits(a, VOCAB_FORWARD, b_mc, lie, dtype) != 0) return -1;
-    const int edge = vocab_tile(g.rows, g.classes, g.k, false, b_mc, lie).edge, bn = edge == 256 ? 256 : 128, groups = (g.classes + bn - 1) / bn * (bn / patch_columns(edge));
-    const int blocks = (g.rows + 63) / 64;
-    hipLaunchKernelGGL(vocab16_rows_kernel, dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(1024), 0, current_stream(), stats, r.parts, r.hits, g.targets, g.rows, g.classes, groups);
-    return check_launch("vocab16_rows_kernel") ? 0 : -1;
+    const int edge = vocab_tile(g.rows, g.classes, g.k, false, false, b_mc, lie).edge, bn = edge == 256 ? 256 : 128, groups = (g.classes + bn - 1) / bn * (bn / patch_columns(edge));
+    if (g.rows <= 64) {
+        hipLaunchKernelGGL((vocab16_rows_kernel<64>), dim3(1), dim3(1024), 0, current_stream(), stats, r.parts, r.hits, g.targets, g.rows, g.classes, groups, loss_out, g.reduction);
+        return check_launch("vocab16_rows_kernel") ? 0 : -1;
+    }
+    const int blocks = (g.rows + 15) / 16;
+    hipLaunchKernelGGL((vocab16_rows_kernel<16>), dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(1024), 0, current_stream(), stats, r.parts, r.hits, g.targets, g.rows, g.classes, groups, loss_out, g.reduction);
+    return check_launch("vocab16_rows_kernel") ? vocab_result_f32(loss_out, stats, g) : -1;
 }
 
 int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats, const float* upstream, void* workspace, int dtype) {
@@ -192,14 +250,16 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
     const int lie = logits_lie(g);
     // dx on the same tiles for every piece (their sums lie by tile); all but the last piece are whole slabs
     const int longest = g.classes < r.piece ? g.classes : r.piece;
-    VocabTile dx_tile = vocab_tile(g.rows, g.k, longest, false, tied, worse16(lie, g.classes % 8 ? LIES_RAGGED : LIES_WHOLE));
+    VocabTile dx_tile = vocab_tile(g.rows, g.k, longest, true, false, tied, worse16(lie, g.classes % 8 ? LIES_RAGGED : LIES_WHOLE));
     if (dx_tile.over == M16_WHOLE && g.classes % M16_BK) dx_tile.over = M16_EDGE;
+    const Shares dx_shares = g.classes > r.piece ? Shares{1, 0, 0} : vocab_shares(g.rows, g.k, longest, dx_tile);
     hipLaunchKernelGGL(vocab16_factors_kernel, dim3(1), dim3(1024), 0, current_stream(), r.f, r.scale, stats, upstream, g.targets, g.rows, g.classes, g.reduction, dtype == RP_DTYPE_FLOAT16 ? 14 : 0);
     if (!check_launch("vocab16_factors_kernel")) return -1;
     for (int v0 = 0, width; v0 < g.classes; v0 += width) {
         width = r.width(v0, g.classes);
         const char *w = (const char*)g.w + 2 * v0 * g.w_cs, *bias = g.bias ? (const char*)g.bias + 2ll * v0 : nullptr;
         VocabTileArgs a{};
+        a.shares = 1;
         a.g = GemmArgs{nullptr, g.x, w, bias, 1, g.rows, g.k, width, 0, g.x_rs, 1, 0, g.w_rs, g.w_cs};
         a.targets = g.targets;
         a.v0 = v0;
@@ -212,7 +272,7 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
         const int piece_lie = worse16(lie, g.w_cs == 1 && width % 8 ? LIES_RAGGED : LIES_WHOLE);
         if (launch_logits(a, VOCAB_GRADIENT, !tied, piece_lie, dtype) != 0) return -1;
         if (o.db) {
-            const int edge = vocab_tile(g.rows, width, g.k, false, !tied, piece_lie).edge, groups = (g.rows + patch_rows(edge) - 1) / patch_rows(edge);
+            const int patch = patch_rows(vocab_tile(g.rows, width, g.k, false, false, !tied, piece_lie).edge), groups = (g.rows + patch - 1) / patch;
             RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vocab16_db_kernel<T>), dim3((width + 63) / 64), dim3(1024), 0, current_stream(), (T*)o.db + v0, r.db_parts, r.scale, groups, (long long)r.pitch, width, o.accumulate_db));
             if (!check_launch("vocab16_db_kernel")) return -1;
         }
@@ -223,6 +283,9 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
             p.sums = r.sums;
             p.first = v0 == 0;
             p.last = v0 + width == g.classes;
+            p.shares = dx_shares.count;
+            p.k_share = dx_shares.k;
+            p.share_stride = dx_shares.stride;
             if (launch_grads(p, VOCAB_DX, tied, dx_tile, dtype) != 0) return -1;
         }
         if (o.dw) {
@@ -230,7 +293,14 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
             // x^T . d, or where dW lies as the transpose d^T . x
             p.g = o.dw_cs == 1 ? GemmArgs{dw, g.x, r.d, nullptr, 1, g.k, g.rows, width, 0, 1, g.x_rs, 0, r.pitch, 1, 0, o.dw_rs, 1, o.accumulate_dw}
                                : GemmArgs{dw, r.d, g.x, nullptr, 1, width, g.rows, g.k, 0, 1, r.pitch, 0, g.x_rs, 1, 0, o.dw_cs, 1, o.accumulate_dw};
-            if (launch_grads(p, VOCAB_DW, true, vocab_tile(p.g.m, p.g.n, p.g.k, true, true, worse16(lies16(g.x, g.x_rs, g.k), width % 8 ? LIES_RAGGED : LIES_WHOLE)), dtype) != 0) return -1;
+            const VocabTile t = vocab_tile(p.g.m, p.g.n, p.g.k, true, true, true, worse16(lies16(g.x, g.x_rs, g.k), width % 8 ? LIES_RAGGED : LIES_WHOLE));
+            const Shares shares = vocab_shares(p.g.m, p.g.n, p.g.k, t);
+            p.sums = r.dw_sums;
+            p.first = p.last = 1;
+            p.shares = shares.count;
+            p.k_share = shares.k;
+            p.share_stride = shares.stride;
+            if (launch_grads(p, VOCAB_DW, true, t, dtype) != 0) return -1;
         }
     }
     return 0;
