@@ -218,11 +218,22 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 __builtin_memcpy(&o, out, 16);
                 // (the whole offset in a vector register: behind a 16-byte store with part of it in a scalar one the compiler lets the next instruction write the data's registers, and zeros of such a
                 // write have been stored here)
-                __builtin_amdgcn_raw_buffer_store_b128(o, to, tid * 16 + i * THREADS * 16, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(o, to, tid * 16 + i * THREADS * 16, 0, 2);      // (streaming: 4096 x 65536 bf16 297 us, 288 so)
                 load_step(from, ic);
                 __builtin_amdgcn_sched_barrier(0);
             });
             if (odd && tid == (g.classes - 1) / N % THREADS) grad[g.classes - 1] = round_to<T>(share(widen(row_last)));
+        } else if (g.classes >= N) {
+            for (int c = tid * N; c < g.classes; c += THREADS * N) {
+                const RowVector<T> at(c, g.classes);
+                T x[N];
+                A values[N];
+                at.load(x, s);
+#pragma unroll
+                for (int u = 0; u < N; u++) values[u] = share(widen(x[u]));
+                round_vector<T>(x, values);
+                at.store(grad, x);
+            }
         } else {
             for (int c = tid; c < g.classes; c += THREADS) grad[c] = round_to<T>(share(widen(s[c])));
         }
@@ -230,6 +241,77 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                           // the row's stores are done: the entries' classes come after
         if (some) correct_entries<T>(g.k, grad, ids, p, v, value, q, factor);
+    }
+}
+
+// The loss alone: nothing of a row is needed twice, so that a workgroup of 256 walks it with a running largest value and sum, and eight of them share a CU
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 8 : 4) distill_loss_rows_kernel(DistillArgs<typename traits<T>::acc> g) {
+    using A = typename traits<T>::acc;
+    constexpr int N = vec16<T>::N, U = 4, WAVES = THREADS / 64, PIECE = U * THREADS * N;
+    __shared__ A rooms[3][2][WAVES];
+    const A scale = (A)1 / g.temperature;
+    const int row_bytes = g.classes * (int)sizeof(T) / 4 * 4, tid = threadIdx.x;
+    const bool odd = sizeof(T) == 2 && g.classes % 2;
+    for (int row = blockIdx.x; row < g.rows; row += gridDim.x) {
+        const T* s = (const T*)g.logits + row * g.logits_rs;
+        const __amdgpu_buffer_rsrc_t from = buffer_rsrc(s, row_bytes);
+        u32x4_t next[U];
+        auto load = [&](int c0) {
+#pragma unroll
+            for (int i = 0; i < U; i++) next[i] = __builtin_amdgcn_raw_buffer_load_b128(from, (c0 + (i * THREADS + tid) * N) * (int)sizeof(T), 0, 0);
+        };
+        load(0);
+        int v = -1;
+        A log_p = -(A)INFINITY, value = 0;
+        if (tid < g.k) {
+            const int id = g.ids[(long long)row * g.k + tid];
+            if (id >= 0 && id < g.classes) log_p = widen(((const T*)g.teacher)[(long long)row * g.k + tid]) * scale;
+            if (!(log_p == -(A)INFINITY)) { v = id; value = widen(s[id]); }
+        }
+        A top = -(A)INFINITY, sum = 0;
+        if (odd && tid == 0) { top = widen(s[g.classes - 1]); sum = top == -(A)INFINITY ? (A)0 : top == top ? (A)1 : top; }      // (an odd last element of 16 bits goes by itself)
+        for (int c0 = 0; c0 < g.classes; c0 += PIECE) {
+            T x[U][N];
+            __builtin_memcpy(x, next, sizeof(x));
+            if (c0 + PIECE < g.classes) load(c0 + PIECE);
+            if (c0 + PIECE > g.classes) {
+#pragma unroll
+                for (int i = 0; i < U; i++)
+#pragma unroll
+                    for (int u = 0; u < N; u++) x[i][u] = c0 + (i * THREADS + tid) * N + u < g.classes - odd ? x[i][u] : round_to<T>(-(A)INFINITY);
+            }
+            A most = top;
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+                for (int u = 0; u < N; u++) most = plain_max(most, widen(x[i][u]));
+            const A base = most == -(A)INFINITY ? (A)0 : most * scale;
+            const ScaledExp<A> weight(scale, base);
+            sum *= weight(top);
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+                for (int u = 0; u < N; u++) sum += weight(widen(x[i][u]));
+            top = most;
+        }
+        A tops[2] = {top, log_p};
+        team_tops_in_turn<THREADS>(tops, rooms[0][0]);
+        const A base = tops[0] == -(A)INFINITY ? (A)0 : tops[0] * scale;
+        A sums[2] = {sum * ScaledExp<A>(scale, base)(top), v < 0 ? (A)0 : natural_exp(log_p - tops[1])};
+        team_sums_in_turn<THREADS>(sums, rooms[1][0]);
+        const A lse = base + natural_log(sums[0]), log_mass = tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]);
+        const bool some = !(log_mass == -(A)INFINITY);
+        log_p -= log_mass;
+        const A own_p = v < 0 ? (A)0 : natural_exp(log_p);
+        A loss[1] = {own_p != 0 ? own_p * (log_p - scaled_less(value, scale, lse)) : (A)0};
+        if (g.k > 64) team_sums_in_turn<THREADS>(loss, rooms[2][0]);
+        else loss[0] = wave_sum(loss[0]);
+        if (tid == 0) {
+            g.stats[row] = lse;
+            g.stats[g.rows + row] = log_mass;
+            g.stats[2 * (long long)g.rows + row] = some ? loss[0] * g.temperature * g.temperature : (A)0;
+        }
     }
 }
 
@@ -256,10 +338,29 @@ static int launch_distill_row(const DistillArgs<typename traits<T>::acc>& g, boo
     return check_launch("distill_kernel") ? 0 : -1;
 }
 
+template <typename T, int THREADS>
+static int launch_distill_loss_rows(const DistillArgs<typename traits<T>::acc>& g) {
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256, held = cus * (2048 / THREADS);
+    hipLaunchKernelGGL((distill_loss_rows_kernel<T, THREADS>), dim3(g.rows < held ? g.rows : held), dim3(THREADS), 0, current_stream(), g);
+    return check_launch("distill_loss_rows_kernel") ? 0 : -1;
+}
+
 template <typename T>
 static int launch_distill(const DistillArgs<typename traits<T>::acc>& g, bool forward) {
     constexpr int N = vec16<T>::N;
-    if (g.classes < N || (long long)g.classes > 1024ll * 16 * N) return launch_distill_row<T, 1024, 0>(g, forward);
+    // (777 x 50021 fp16, the loss: rows held in registers 42 us, walked: see the measured table; byte offsets in 32 bits)
+    if (forward && !g.grad && g.classes >= N && g.classes < (1 << 27)) return g.k <= 256 ? launch_distill_loss_rows<T, 256>(g) : launch_distill_loss_rows<T, 1024>(g);
+    if (g.classes < N) return launch_distill_row<T, 1024, 0>(g, forward);
+    if ((long long)g.classes > 1024ll * 16 * N) {
+        // (rows longer than registers: walked once for the sums and once for the gradient)
+        if (forward && g.classes < (1 << 27)) {
+            DistillArgs<typename traits<T>::acc> loss = g;
+            loss.grad = nullptr;
+            if (launch_distill<T>(loss, true) != 0) return -1;
+            forward = false;
+        }
+        return launch_distill_row<T, 1024, 0>(g, forward);
+    }
     if (g.k > 256) {                               // (an entry a thread)
         if (g.classes <= 1024 * 2 * N) return launch_distill_row<T, 1024, 2>(g, forward);
     } else if (g.classes <= 256 * N) return launch_distill_row<T, 256, 1>(g, forward);

@@ -6,7 +6,7 @@
 // z is kept in the accumulate type (float32 for the 16-bit types), as the sums that they are: rounded to 16 bits, z's own error would reach dz beside dz's, and the gradients'
 // error would be 1.3 times as large.  dz is rounded to the tensors' type, which is what the matrix cores multiply.
 #include "rp_gated16.h"
-#include "rp_grouped.h"
+#include "rp_grouped_sums.h"
 
 namespace rp {
 
@@ -140,6 +140,38 @@ static int product(void* C, const void* A, const void* B, const void* bias, int 
     return rc;
 }
 
+struct GatedGradients {
+    void *dx, *dw, *db;
+    long long dx_rs, dw_rs, dw_cs;
+    int accumulate_dx, accumulate_dw, accumulate_db;
+};
+// dx = dz . W^T, dW = x^T . dz, db = sum of dz.  16-bit layers of 512 rows and more as one group of a grouped layer, whose launches make the gradients side by side (fp16, us for all three as products of
+// their own and so: 1999 x 519 x 2062 51.9 / 33.1, 4096 x 1031 x 4098 199 / 135, 1000 x 4096 x 1024 39.1 / 27.5, 8192 x 4096 x 16384 1795 / 1746; 300 x 200 x 2062 8.9 / 14.9, 1024 x 512 x 2048 14.4 / 16.8,
+// 8192 x 256 x 512 50.7 / 56.7), the others as a linear layer's.
+static int gated_gradients(const GatedGradients& o, const void* dz, const GatedArgs& g, int dtype) {
+    const int n2 = 2 * g.n;
+    if (dtype_size(dtype) == 2 && g.rows >= 512 && g.k > 512 && (!o.dw || (o.dw_cs == 1 && o.dw_rs == n2))) {
+        const RowGroups all{nullptr, nullptr, 1, g.rows, 1};
+        const GroupedArgs x{o.dx, dz, g.w, nullptr, nullptr, all, n2, g.k, n2, 1, 0, g.w_cs, g.w_rs, 0, o.dx_rs, o.accumulate_dx ? ACCUMULATE : 0};
+        const GroupedArgs w{o.dw, g.x, dz, nullptr, nullptr, all, g.k, n2, g.x_rs, g.x_cs, 0, n2, 1, 0, n2, o.accumulate_dw ? ACCUMULATE : 0};
+        return launch_grouped_backward(x, w, GroupedSums{o.db, dz, all, n2, o.accumulate_db, n2}, dtype);
+    }
+    if (o.dw_cs == 1 && !o.accumulate_dx && !o.accumulate_dw && !o.accumulate_db) {      // (what it has made before it is refused memory is made again)
+        const CallScratch memory(CallScratch::MOST);
+        const GemmWorkspaceLoan loan(memory.ptr, CallScratch::MOST);
+        const int rc = rp_hip_linear_backward(o.dx, o.dw, o.db, dz, g.x, g.w, g.rows, g.k, n2, g.x_rs, g.x_cs, g.w_rs, g.w_cs, o.dx_rs, 1, o.dw_rs, 1, 0, 0, 0, dtype);
+        if (!loan.refused) return rc;
+    }
+    if (o.dx && product(o.dx, dz, g.w, nullptr, g.rows, n2, g.k, n2, 1, g.w_cs, g.w_rs, o.dx_rs, o.accumulate_dx, dtype) != 0) return -1;
+    if (o.dw) {
+        // (a transposed dW is the transposed product)
+        const int rc = o.dw_cs == 1 ? product(o.dw, g.x, dz, nullptr, g.k, g.rows, n2, g.x_cs, g.x_rs, n2, 1, o.dw_rs, o.accumulate_dw, dtype)
+                                    : product(o.dw, dz, g.x, nullptr, n2, g.rows, g.k, 1, n2, g.x_rs, g.x_cs, o.dw_cs, o.accumulate_dw, dtype);
+        if (rc != 0) return -1;
+    }
+    return o.db ? rp_hip_reduce_rows(o.db, dz, g.rows, n2, o.accumulate_db, dtype) : 0;
+}
+
 // float32 and float64: z by a plain product, then h.  Without room for z, as many rows at a time as the stream's own memory holds.
 template <typename T>
 static int launch_gated_by_product(const GatedArgs& g, int dtype, bool* taken) {
@@ -265,14 +297,7 @@ int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const v
         const long long blocks = (long long)rows * across;
         RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_dz_kernel<T, GATE>), dim3((unsigned)(blocks < GATED_GRID ? blocks : GATED_GRID)), dim3(256), 0, current_stream(), (T*)dz, (const T*)dh, (const A*)z, rows, n, dh_rs, across));
         if (!check_launch("gated_dz_kernel")) return -1);
-    if (dx && product(dx, dz, w, nullptr, rows, 2 * n, k, 2ll * n, 1, w_cs, w_rs, dx_rs, accumulate_dx, dtype) != 0) return -1;
-    if (dw) {
-        // (a transposed dW is the transposed product)
-        const int rc = dw_cs == 1 ? product(dw, x, dz, nullptr, k, rows, 2 * n, x_cs, x_rs, 2ll * n, 1, dw_rs, accumulate_dw, dtype)
-                                  : product(dw, dz, x, nullptr, 2 * n, rows, k, 1, 2ll * n, x_rs, x_cs, dw_cs, accumulate_dw, dtype);
-        if (rc != 0) return -1;
-    }
-    return db ? rp_hip_reduce_rows(db, dz, rows, 2 * n, accumulate_db, dtype) : 0;
+    return gated_gradients(GatedGradients{dx, dw, db, dx_rs, dw_rs, dw_cs, accumulate_dx, accumulate_dw, accumulate_db}, dz, GatedArgs{nullptr, nullptr, x, w, nullptr, rows, k, n, gate, x_rs, x_cs, w_rs, w_cs, 0}, dtype);
 }
 
 }  // extern "C"

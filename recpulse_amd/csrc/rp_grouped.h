@@ -41,6 +41,9 @@ enum GroupedLow { LOW_A, LOW_B };
 
 // By rows, on the kernel that suits the sizes (rp_grouped.hip)
 int launch_grouped_rows(const GroupedArgs& g, int dtype);
+// Both gradients of a grouped layer and column sums, those whose output is not null, in as few launches as suit them
+struct GroupedSums;
+int launch_grouped_backward(const GroupedArgs& x, const GroupedArgs& wg, const GroupedSums& sums, int dtype);
 // Any strides and sizes, all types (rp_grouped_generic.hip); low: A is.  No scales; by weights: no ids.
 int launch_grouped_rows_generic(const GroupedArgs& g, bool low, int dtype);
 int launch_grouped_weights_generic(const GroupedArgs& g, int dtype);

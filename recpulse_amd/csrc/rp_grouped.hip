@@ -155,6 +155,19 @@ static int shared_with_term(const GroupedArgs& s, const AdapterTerm& term, int d
     return launch_grouped_rows_generic(GroupedArgs{s.C, term.h, term.b, nullptr, nullptr, term.gr, term.rank, s.n, term.rank, 1, term.b_ws, term.b_rs, term.b_cs, 0, s.c_rs, ACCUMULATE_JOINED}, true, dtype);
 }
 
+int launch_grouped_backward(const GroupedArgs& x, const GroupedArgs& wg, const GroupedSums& sums, int dtype) {
+    GroupedArgs xg = x;
+    int result;
+    if (backward_together(xg, wg, sums, dtype, &result)) return result;
+    if (xg.C) {
+        if (grouped_rows(xg, dtype) != 0) return -1;
+        xg.C = nullptr;
+        if (backward_together(xg, wg, sums, dtype, &result)) return result;
+    }
+    if (wg.C && grouped_weights(wg, dtype) != 0) return -1;
+    return sums.out ? launch_grouped_sums(sums, dtype) : 0;
+}
+
 static bool grouped_args_ok(const char* who, bool pointers, int groups, int rows, int k, int n, std::initializer_list<long long> strides, int dtype) {
     if (!pointers || groups <= 0 || rows <= 0 || k <= 0 || n <= 0) { set_error("%s: null operand or non-positive extent (groups=%d rows=%d k=%d n=%d)", who, groups, rows, k, n); return false; }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
@@ -190,18 +203,10 @@ int rp_hip_grouped_linear_backward(void* dx, void* dw, void* db, const void* dy,
     if (!grouped_args_ok(who, dy && offsets && (!dx || w) && (!dw || x), groups, rows, k, n, {dy_rs, x_rs, x_cs, w_gs, w_rs, w_cs, dx_rs}, dtype)) return -1;
     if (dx && !output_rows_ok(who, "dx", rows, k, dx_rs)) return -1;
     const RowGroups gr{offsets, nullptr, groups, rows, groups};
-    GroupedArgs xg{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
+    const GroupedArgs xg{dx, dy, w, nullptr, nullptr, gr, n, k, dy_rs, 1, w_gs, w_cs, w_rs, 0, dx_rs, accumulate_dx ? ACCUMULATE : 0};
     const GroupedArgs wg{dw, x, dy, nullptr, nullptr, gr, k, n, x_rs, x_cs, 0, dy_rs, 1, (long long)k * n, n, accumulate_dw ? ACCUMULATE : 0};
     const GroupedSums sums{db, dy, gr, n, accumulate_db, dy_rs};
-    int result;
-    if (backward_together(xg, wg, sums, dtype, &result)) return result;
-    if (dx) {
-        if (grouped_rows(xg, dtype) != 0) return -1;
-        xg.C = nullptr;
-        if (backward_together(xg, wg, sums, dtype, &result)) return result;
-    }
-    if (dw && grouped_weights(wg, dtype) != 0) return -1;
-    return db ? launch_grouped_sums(sums, dtype) : 0;
+    return launch_grouped_backward(xg, wg, sums, dtype);
 }
 
 int rp_hip_adapter_linear_forward(void* y, void* h, const void* x, const void* w, const void* bias, const void* a, const void* b, const float* scales, const int* ids, const int* offsets,
