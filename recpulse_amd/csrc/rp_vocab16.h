@@ -4,8 +4,9 @@
 // (8 bytes for 64 or 128 logits), and the target's logit by the lane that holds it.  Backward, the tile is made again and leaves as d = (exp(z - lse) - [v = t]) f, rounded to 16
 // bits, a piece of the vocabulary at a time, which two more products take to dx and dW; db is summed from the same registers.
 //
-// d is stored times a power of two that puts the largest |f| at 2^14 (float16) or 1, and dx, dW and db are scaled back in their epilogues, before their one rounding: as it is, the share of a rare class in
-// a mean over thousands of rows would be zero in float16.  dx is a sum over all pieces: between two of them it stays in float32, a tile's sums in the order of its registers.
+// d is stored over the largest |f| (times 2^14 in float16), and dx, dW and db are scaled back in their epilogues, before their one rounding.  As it is, the share of a rare class in a mean over thousands of
+// rows would be zero in float16; and of rows with one f all targets' d, which is -f but for a small p, would be rounded alike: their common error, up to half a step, would be that of dx and dW (bf16 0.0030
+// against 0.0024 where -1 is exact).  dx is a sum over all pieces: between two of them it stays in float32, a tile's sums in the order of its registers.
 #pragma once
 #include "rp_gemm_mfma16_kernel.h"
 #include "rp_vocab.h"

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(1024) vocab16_rows_kernel(float* stats, const 
     }
 }
 
-// f of each row times a power of two, and that power's inverse: one workgroup
+// f of each row over the largest of them, times 2^most, and what takes that back: one workgroup
 __global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* scale, const float* stats, const float* upstream, const int* targets, int rows, int classes, int reduction, int most) {
     __shared__ float room[16];
     float top = 0.f;
@@ -151,12 +151,10 @@ __global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* 
         top = fmaxf(top, __builtin_isfinite(v) ? fabsf(v) : 0.f);
     }
     top = team_max<1024>(top, room);
-    int e = 0;
-    if (top > 0.f) (void)frexpf(top, &e);                     // top is below 2^e
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
-    const float up = ldexpf(1.f, most - e);
-    for (int i = threadIdx.x; i < rows; i += 1024) f[i] *= up;      // (each thread its own)
-    if (threadIdx.x == 0) *scale = ldexpf(1.f, e - most);
+    if (!(top > 0.f)) top = 1.f;
+    const float up = ldexpf(1.f, most);
+    for (int i = threadIdx.x; i < rows; i += 1024) f[i] = f[i] / top * up;      // (each thread its own)
+    if (threadIdx.x == 0) *scale = top / up;
 }
 
 // db of a piece from its groups' sums

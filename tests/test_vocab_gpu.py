@@ -174,6 +174,25 @@ def test_small_and_uneven_upstream_gradients_keep_their_digits(dtype):
     check_backward(rows, 64, 2000, False, dtype, reduction=2, bias=True, without=3, upstream=np.array([2.0 ** -6]))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=NAMES.get)
+@pytest.mark.parametrize("rows", [37, 300])
+def test_a_mean_does_not_round_all_rows_alike(rows, dtype):
+    """With logits of zero over 128 classes p = 2^-7 and p - 1 are exact in 16 bits; 1.3 / rows is not, and must not be part of what is rounded."""
+    rng = np.random.default_rng(13)
+    k, classes = 64, 128
+    x, w = Operand(rng.normal(size=(rows, k)), dtype), Operand(np.zeros((k, classes)), dtype)
+    targets, up = rng.integers(0, classes, rows), vector([1.3], F32)
+    space = room(capi.lib().rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, dtype))
+    _, stats = forward(x, w, None, targets, dtype, 1, space)
+    dw = Output(k, classes, dtype)
+    capi.check(capi.lib().rp_hip_linear_cross_entropy_backward(None, dw.ptr, None, x.ptr, w.ptr, None, ints(targets).ptr, stats.ptr, up.ptr, space.ptr, rows, k, classes, 1,
+                                                               k, 1, classes, 1, k, classes, 1, 0, 0, 0, dtype), "backward")
+    d = (np.full((rows, classes), 2.0 ** -7) - (targets[:, None] == np.arange(classes))) * up.values[0, 0] / rows
+    # log 128 in float32 and exp of it: 2^-7 to 2^-20 of itself, which 16 bits round back
+    off = (rows + 16) * 2.0 ** -24 * (np.abs(x.values).T @ np.abs(d))
+    assert_within(dw.read(), x.values.T @ d, rounded(off, x.values.T @ d, dtype), "dw")
+
+
 @pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
 @pytest.mark.parametrize("rows,k,classes", [(9, 40, 300), (150, 128, 1100)])
 def test_without_any_target_everything_is_zero(rows, k, classes, dtype):
