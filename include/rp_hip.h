@@ -462,7 +462,8 @@ int rp_hip_adapter_linear_backward(void* dx, void* da, void* db, void* u, const 
  * Layer norm, the gated linear layer, the cross entropy of a large vocabulary from the hidden rows, and distillation from a teacher's top logits.  All types; sums and the values between are
  * in the accumulate type (float32, float64 for float64).  Strides in elements, non-negative; outputs overlap neither an operand nor each other.  `workspace` is device memory of the caller's, as
  * many bytes as the entry's own _workspace function says (-1: arguments that the entry would refuse), aligned to 16; a call leaves nothing there that another call reads, so that calls in turn on one
- * stream may share it and calls on several streams may not.  Results do not depend on the stream, and the same call leaves the same bits. */
+ * stream may share it and calls on several streams may not.  Calls on several streams share nothing else: partial sums of the gated layer lie where those of the layers whose weight depends on the row
+ * lie, and without that memory it goes a way that needs none.  Such a call, and the column sums db on another than the null stream, may add in another order; otherwise the same call leaves the same bits. */
 
 /* Layer norm of rows [rows, d]: y = (x - mean) / sqrt(variance + eps) * w + b, with the mean of the squared differences as variance.  w, b: dense [d] or NULL.  stats: [rows, 2]
  * in the accumulate type, mean and 1 / sqrt(variance + eps), for the backward pass; may be NULL. */
@@ -485,7 +486,8 @@ int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const v
 
 /* Cross entropy of a large vocabulary from the rows before it: with z = x . w + bias (x [rows, k], w [k, classes], bias dense [classes] or NULL),
  *   loss_i = log sum over v of exp(z[i, v]) - z[i, targets[i]].
- * The logits are made in pieces of the vocabulary and not kept.  targets: device int32 [rows]; a row whose target lies outside [0, classes) is left out: its loss and gradient are zeros.
+ * The logits are made in pieces of the vocabulary and not kept.  targets: device int32 [rows]; a row whose target lies outside [0, classes) is left out: its loss and gradient are zeros
+ * (dw still adds zeros times its x, which has to be finite there).
  * reduction 0: loss_out [rows]; 1: the mean over the rows with a target (0 where there are none); 2: their sum; loss_out in the accumulate type.  stats: 2 rows + 1 values of the accumulate type, for the
  * backward pass: log sum exp of each row, its loss, and how many rows have a target. */
 long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, int backward, int dtype);

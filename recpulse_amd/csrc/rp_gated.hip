@@ -230,7 +230,7 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
     }
     const int edge = ragged ? M16_RAGGED : M16_EDGE;
     if (g.rows > 64 && p.bm >= 128 && p.bn >= 128) return launch_gated16_128(g, edge, dtype);
-    // Few tiles: k in shares of at least eight slabs, up to three workgroups a CU
+    // Few tiles: k in shares of at least eight slabs, up to three workgroups a CU (bf16, 16 rows, 4096 -> 8192: 128 tiles 40 us, in six shares 26 and 4.5 for the launch that joins them)
     const long long tiles = (long long)((g.rows + 63) / 64) * ((g.n + 63) / 64), share_bytes = 8ll * g.rows * g.n;
     const int cus = device_cu_count() > 0 ? device_cu_count() : 256, slabs = (g.k + M16_BK - 1) / M16_BK;
     long long count = 3ll * cus / tiles;
@@ -245,8 +245,8 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
 }
 
 static bool gated_args_ok(const char* who, bool pointers, int rows, int k, int n, int gate, std::initializer_list<long long> strides, int dtype) {
-    if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 30) || n > (1 << 29)) {
-        set_error("%s: null operand, non-positive extent, more than 2^30 rows or 2^29 columns (rows=%d k=%d n=%d)", who, rows, k, n);
+    if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 29) || n > (1 << 29)) {
+        set_error("%s: null operand, non-positive extent, more than 2^29 rows or columns (rows=%d k=%d n=%d)", who, rows, k, n);
         return false;
     }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }

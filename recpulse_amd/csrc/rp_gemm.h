@@ -164,7 +164,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t splitk_rsrc(const float* parti
 
 // The device's block of SPLITK_MAX_TILES zeroed arrival counters (created on first use, kept for the life of the
 // process), or nullptr when the single-launch finish cannot be used: more tiles than counters, partials of 2 GiB
-// or more, "one_launch_splitk" in RP_HIP_DISABLE, or an allocation failure (then last_error is set and *failed is true).
+// or more, a workspace on loan, "one_launch_splitk" in RP_HIP_DISABLE, or an allocation failure (then last_error is set and *failed is true).
 // Like the workspace pool the block is not stream-aware: launches that may run at the same time on different
 // streams of one device must be serialised by the caller.
 int* splitk_arrival_counters(long long tiles, size_t partial_bytes, bool* failed);
@@ -174,7 +174,7 @@ int* splitk_arrival_counters(long long tiles, size_t partial_bytes, bool* failed
 int gemm_workspace(void** ws, size_t bytes);
 void gemm_workspace_release(void* ws);
 // While one lives, the calling thread's GEMMs take their workspace from `ptr` (null: there is none) and not from the pool; a product that would need more
-// launches nothing, returns -1 and leaves `refused`.
+// launches nothing, returns -1 and leaves `refused`.  Such a product may run beside another stream's, so it does without the arrival counters too.
 class GemmWorkspaceLoan {
 public:
     GemmWorkspaceLoan(void* ptr, size_t bytes);
@@ -185,6 +185,7 @@ public:
     const size_t bytes;
     bool refused = false;
 };
+bool gemm_workspace_lent();
 // Inside the entry point that allocates nothing: its arrival counters, cleared by a kernel on the current stream the
 // first time a call asks for them (nullptr with an error when that launch fails).
 bool noalloc_active();

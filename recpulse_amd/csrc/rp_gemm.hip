@@ -498,6 +498,7 @@ static unsigned char* noalloc_scratch_of_current_device() {
 static thread_local GemmWorkspaceLoan* g_loan = nullptr;
 GemmWorkspaceLoan::GemmWorkspaceLoan(void* p, size_t b) : ptr(p), bytes(b) { g_loan = this; }
 GemmWorkspaceLoan::~GemmWorkspaceLoan() { g_loan = nullptr; }
+bool gemm_workspace_lent() { return g_loan != nullptr; }
 
 int gemm_workspace(void** ws, size_t bytes) {
     if (g_loan) {

@@ -279,7 +279,7 @@ int* splitk_arrival_counters(long long tiles, size_t partial_bytes, bool* failed
     static std::mutex mu;
     static int* blocks[MAX_DEVICES] = {};
     *failed = false;
-    if (path_disabled("one_launch_splitk") || tiles > SPLITK_MAX_TILES || partial_bytes >= (1ull << 31)) return nullptr;
+    if (gemm_workspace_lent() || path_disabled("one_launch_splitk") || tiles > SPLITK_MAX_TILES || partial_bytes >= (1ull << 31)) return nullptr;
     if (noalloc_active()) {                              // inside the entry point that allocates nothing: its fixed counters
         int* fixed = noalloc_arrival_counters();
         if (!fixed) *failed = true;

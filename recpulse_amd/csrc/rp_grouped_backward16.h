@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(256, 2) grouped_backward16_kernel(GroupedArgs 
         return;
     }
     id -= bg.x_blocks;
-    GroupedWeightTiles source{w, bg.w_tiles_k, bg.w_tiles_n, bg.w_slots};
+    GroupedWeightTiles source{{}, w, bg.w_tiles_k, bg.w_tiles_n, bg.w_slots};
     GemmArgs g{nullptr, nullptr, nullptr, nullptr, 1, w.k, 0, w.n, 0, w.a_cs, w.a_rs, 0, w.b_rs, w.b_cs, 0, w.c_rs, 1, w.accumulate};
     gemm_mfma16_block<T, BW, BW, 2, true, true, EDGE, false, 1, GroupedWeightTiles>(g, 0, 0, nullptr, 0, bg.w_total, id, 0, bg.w_blocks, &source);
 }

@@ -61,7 +61,7 @@ struct GroupedWeightTiles : M16Source {
 
 template <typename T, int BM, int BN, int WGM, int EDGE>
 __global__ void __launch_bounds__(256, m16_blocks_per_cu(BM, BN, EDGE, 1)) grouped_weights16_kernel(GroupedArgs ga, int tiles_k, int tiles_n, int slots, int total) {
-    GroupedWeightTiles source{ga, tiles_k, tiles_n, slots};
+    GroupedWeightTiles source{{}, ga, tiles_k, tiles_n, slots};
     GemmArgs g{nullptr, nullptr, nullptr, nullptr, 1, ga.k, 0, ga.n, 0, ga.a_cs, ga.a_rs, 0, ga.b_rs, ga.b_cs, 0, ga.c_rs, 1, ga.accumulate};
     gemm_mfma16_block<T, BM, BN, WGM, true, true, EDGE, false, 1, GroupedWeightTiles>(g, 0, 0, nullptr, 0, total, (int)blockIdx.x, 0, (int)gridDim.x, &source);
 }

@@ -377,7 +377,7 @@ static int launch_norm(const NormArgs<typename traits<T>::acc>& g, bool backward
 }
 
 static bool norm_args_ok(const char* who, bool pointers, int rows, int d, std::initializer_list<long long> strides, int dtype) {
-    if (!pointers || rows <= 0 || d <= 0 || rows > (1 << 30) || d > (1 << 29)) { set_error("%s: null operand, non-positive extent, more than 2^30 rows or a width above 2^29 (rows=%d d=%d)", who, rows, d); return false; }
+    if (!pointers || rows <= 0 || d <= 0 || rows > (1 << 30) || d > (1 << 26)) { set_error("%s: null operand, non-positive extent, more than 2^30 rows or a width above 2^26 (rows=%d d=%d)", who, rows, d); return false; }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
     for (long long s : strides)
         if (s < 0) { set_error("%s: negative stride", who); return false; }

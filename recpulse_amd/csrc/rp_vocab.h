@@ -1,6 +1,6 @@
 // Cross entropy of a large vocabulary straight from the rows before it: z = x . W + b, loss_i = log sum_v exp(z_iv) - z_it.
 #pragma once
-#include "rp_gemm.h"
+#include "rp_grouped.h"
 #include "rp_teams.h"
 
 namespace rp {

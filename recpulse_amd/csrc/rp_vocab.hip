@@ -11,6 +11,8 @@ namespace rp {
 
 constexpr long long VOCAB_PIECE_BYTES = 64ll << 20;      // of a piece's logits
 constexpr size_t VOCAB_GEMM_BYTES = 16 << 20;            // for the partial sums of its products
+// Few rows: dx of a piece is split along its classes, 2048 a share, and 32 shares of 8 rows and 16384 float32 fill that memory
+constexpr int VOCAB_FEW_ROWS = 8, VOCAB_FEW_PIECE = 65536;
 constexpr int VOCAB_GRID = 1 << 20;
 
 static int vocab_piece(int rows, int classes, int elem, long long bytes) {
@@ -123,7 +125,7 @@ template <typename T> struct VocabAnyRoom {
     A *state, *z, *x, *w, *bias, *dx, *dw, *db;
     char* gemm;
     VocabAnyRoom(VocabRoom& room, int rows, int k, int classes, bool backward) {
-        piece = vocab_piece(rows, classes, sizeof(A), VOCAB_PIECE_BYTES);
+        piece = vocab_piece(rows, rows <= VOCAB_FEW_ROWS && classes > VOCAB_FEW_PIECE ? VOCAB_FEW_PIECE : classes, sizeof(A), VOCAB_PIECE_BYTES);
         state = room.take<A>(3ll * rows);
         z = room.take<A>((long long)rows * piece);
         gemm = room.take<char>(VOCAB_GEMM_BYTES);
@@ -143,8 +145,16 @@ struct VocabProduct {
     void* room;
     int dtype;
     int operator()(void* C, const void* A, const void* B, const void* bias, int m, int k, int n, long long a_rs, long long a_cs, long long b_rs, long long b_cs, long long c_rs, int accumulate) const {
-        const GemmWorkspaceLoan loan(room, VOCAB_GEMM_BYTES);
-        return rp_hip_gemm_strided_batched(C, A, B, bias, 1, m, k, n, 0, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, 1, accumulate, dtype);
+        int rc;
+        bool refused;
+        {
+            const GemmWorkspaceLoan loan(room, VOCAB_GEMM_BYTES);
+            rc = rp_hip_gemm_strided_batched(C, A, B, bias, 1, m, k, n, 0, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, 1, accumulate, dtype);
+            refused = loan.refused;
+        }
+        // (few rows and more than 16384 of x's columns: as one group of all rows, whose k is not split)
+        if (refused) rc = launch_grouped_rows(GroupedArgs{C, A, B, bias, nullptr, RowGroups{nullptr, nullptr, 1, m, 1}, k, n, a_rs, a_cs, 0, b_rs, b_cs, 0, c_rs, accumulate ? ACCUMULATE : 0}, dtype);
+        return rc;
     }
 };
 
@@ -239,8 +249,8 @@ static int vocab_any_backward(const VocabGrads& o, const VocabArgs& g, const voi
 }
 
 static bool vocab_args_ok(const char* who, bool pointers, int rows, int k, int classes, int reduction, std::initializer_list<long long> strides, int dtype) {
-    if (!pointers || rows <= 0 || k <= 0 || classes <= 0 || rows > (1 << 30) || classes > (1 << 30)) {
-        set_error("%s: null operand, non-positive extent, more than 2^30 rows or classes (rows=%d k=%d classes=%d)", who, rows, k, classes);
+    if (!pointers || rows <= 0 || k <= 0 || classes <= 0 || rows > (1 << 29) || classes > (1 << 29)) {
+        set_error("%s: null operand, non-positive extent, more than 2^29 rows or classes (rows=%d k=%d classes=%d)", who, rows, k, classes);
         return false;
     }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }

@@ -50,11 +50,12 @@ static int logits_lie(const VocabArgs& g) {
 }
 bool vocab16_takes(const VocabArgs& g, int dtype) {
     if ((dtype != RP_DTYPE_BFLOAT16 && dtype != RP_DTYPE_FLOAT16) || g.x_cs != 1 || (g.w_cs != 1 && g.w_rs != 1) || path_disabled("mfma")) return false;
-    return logits_lie(g) != LIES_NEITHER;
+    // (the forward pass is one launch, of fewer than 2^32 threads; on 64 x 128 tiles from 2^37 logits on it would not be)
+    return logits_lie(g) != LIES_NEITHER && (long long)((g.rows + 63) / 64) * ((g.classes + 127) / 128) < (1 << 24) - 64;
 }
 
-// Few tiles and a long k: k goes in shares to workgroups of their own, three a CU, at least eight slabs each.  (fp16, 1000 rows, 520 -> 10007: dx on 144 tiles of 64 walks 157 slabs; us in
-// one share and in four with the launch that joins them: see the measured table)
+// Few tiles and a long k: k goes in shares to workgroups of their own, three a CU, at least eight slabs each.  (fp16, 1000 rows, 520 -> 10007: dx
+// on 40 tiles of 128 walks 157 slabs, 72 us; in 12 shares 31 and 8 for the launch that joins them)
 constexpr long long VOCAB16_SHARE_BYTES = 32ll << 20;      // of the shares' sums
 struct Shares { int count, k; long long stride; };
 static Shares vocab_shares(int m, int n, int k, const VocabTile& t) {
