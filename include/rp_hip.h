@@ -479,7 +479,8 @@ enum { RP_GATE_SILU = 0, RP_GATE_GELU = 1, RP_GATE_GELU_TANH = 2, RP_GATE_RELU =
 int rp_hip_gated_linear_forward(void* h, void* z, const void* x, const void* w, const void* bias, int rows, int k, int n, int gate,
                                 long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long h_rs, int dtype);
 /* Its gradients.  dz: [rows, 2 n] dense, room for the gradient of g | u in the tensors' type.  dx [rows, k] with unit column stride, dw [k, 2 n] with unit stride along either axis (the
- * gradient of a transposed weight lies as the weight does), db dense [2 n]; any of the three may be NULL; accumulate_* = 1 adds the rounded product to what is there. */
+ * gradient of a transposed weight lies as the weight does), db dense [2 n]; any of the three may be NULL; accumulate_* = 1 adds the rounded product to what is there.  db is summed before
+ * dz is rounded. */
 int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const void* dh, const void* z, const void* x, const void* w, int rows, int k, int n, int gate,
                                  long long dh_rs, long long x_rs, long long x_cs, long long w_rs, long long w_cs, long long dx_rs, long long dw_rs, long long dw_cs,
                                  int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);

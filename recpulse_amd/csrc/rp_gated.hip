@@ -126,6 +126,128 @@ __global__ void __launch_bounds__(256) gated_dz_kernel(T* dz, const T* dh, const
     }
 }
 
+// dz and, in 16 bits, db from what has not been rounded yet (of the rounded dz, the error of sums of few rows was 1.5 times as large).  A workgroup makes 256 columns of each half of `per` rows and leaves
+// their sums as a row of `parts` [chunks][2 n], which a second launch adds up in order: z and dh are read once.
+template <typename T, int GATE>
+__global__ void __launch_bounds__(256) gated_dz_sums_kernel(T* dz, float* parts, const T* dh, const float* z, int rows, int n, long long dh_rs, int strips, int per) {
+    constexpr int N = vec16<T>::N, LANES = 32, WALK = 256 / LANES;
+    __shared__ float room[WALK][LANES][2 * N + 1];
+    const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips, lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (strip * LANES + lane) * N;
+    const RowVector<T> at(c < n ? c : n - N, n);
+    float sums[2 * N] = {};
+    const int end = rows - chunk * per < per ? rows : chunk * per + per;
+    if (c < n)
+#pragma unroll 2
+        for (int row = chunk * per + slice; row < end; row += WALK) {
+            const float* zr = z + (long long)row * 2 * n;
+            T* out = dz + (long long)row * 2 * n;
+            T dv[N], og[N], ou[N];
+            float gate[N], up[N], vg[N], vu[N];
+            at.load(dv, dh + row * dh_rs);
+            __builtin_memcpy(gate, zr + at.at, sizeof(gate));
+            __builtin_memcpy(up, zr + n + at.at, sizeof(up));
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const float v = widen(dv[u]);
+                vg[u] = v * up[u] * gate_slope<GATE>(gate[u]);
+                vu[u] = v * gate_value<GATE>(gate[u]);
+                sums[u] += vg[u];
+                sums[N + u] += vu[u];
+            }
+            round_vector<T>(og, vg);
+            round_vector<T>(ou, vu);
+            at.store(out, og);
+            at.store(out + n, ou);
+        }
+#pragma unroll
+    for (int u = 0; u < 2 * N; u++) room[slice][lane][u] = sums[u];
+    __syncthreads();
+    float* to = parts + (long long)chunk * 2 * n;
+    for (int e = threadIdx.x; e < LANES * 2 * N; e += 256) {
+        const int half = e / (LANES * N), l = e % (LANES * N) / N, u = e % N, col = (strip * LANES + l) * N;
+        if (col >= n) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < WALK; s++) sum += room[s][l][half * N + u];
+        to[half * n + RowVector<T>(col, n).at + u] = sum;      // (a last vector begins before its own columns and finds the same sums there)
+    }
+}
+template <typename T> __device__ __forceinline__ void put_db(T* db, float sum, int accumulate) {
+    const T y = round_to<T>(sum);
+    *db = accumulate ? round_to<T>(widen(*db) + widen(y)) : y;
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) gated_db_kernel(T* db, const float* parts, int chunks, int width, int accumulate) {
+    __shared__ float room[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane;
+    float sum = 0.f;
+    if (c < width)
+#pragma unroll 8
+        for (int i = wave; i < chunks; i += 16) sum += parts[(long long)i * width + c];
+    room[wave][lane] = sum;
+    __syncthreads();
+    if (wave || c >= width) return;
+#pragma unroll
+    for (int w = 1; w < 16; w++) sum += room[w][lane];
+    put_db(db + c, sum, accumulate);
+}
+// The same without memory for the parts, and for less than a vector of columns: z and dh are read again
+template <typename T, int GATE>
+__global__ void __launch_bounds__(1024) gated_db_any_kernel(T* db, const T* dh, const float* z, int rows, int n, long long dh_rs, int accumulate) {
+    __shared__ float room[2][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane;
+    float sg = 0.f, su = 0.f;
+    if (c < n)
+        for (int row = wave; row < rows; row += 16) {
+            const float v = widen(dh[row * dh_rs + c]), gate = z[(long long)row * 2 * n + c];
+            sg += v * z[(long long)row * 2 * n + n + c] * gate_slope<GATE>(gate);
+            su += v * gate_value<GATE>(gate);
+        }
+    room[0][wave][lane] = sg;
+    room[1][wave][lane] = su;
+    __syncthreads();
+    if (wave || c >= n) return;
+#pragma unroll
+    for (int w = 1; w < 16; w++) { sg += room[0][w][lane]; su += room[1][w][lane]; }
+    put_db(db + c, sg, accumulate);
+    put_db(db + n + c, su, accumulate);
+}
+
+template <typename T>
+static int launch_gated_dz(void* dz, const void* dh, const void* z, int rows, int n, int gate, long long dh_rs) {
+    using A = typename traits<T>::acc;
+    const int across = (n + 256 * vec16<T>::N - 1) / (256 * vec16<T>::N);
+    const long long blocks = (long long)rows * across;
+    RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_dz_kernel<T, GATE>), dim3((unsigned)(blocks < GATED_GRID ? blocks : GATED_GRID)), dim3(256), 0, current_stream(), (T*)dz, (const T*)dh, (const A*)z, rows, n, dh_rs, across));
+    return check_launch("gated_dz_kernel") ? 0 : -1;
+}
+// dz and db in 16 bits
+template <typename T>
+static int launch_gated_dz_sums(void* dz, void* db, const void* dh, const void* z, int rows, int n, int gate, long long dh_rs, int accumulate) {
+    // Two workgroups a CU, of at least eight rows, whose sums find room (fp16, us for both launches with 1, 2, 4 and 8 a CU, silu: 1999 x 1031 11.1 / 10.8 / 11.7 / 11.2, 8192 x 8192 165 / 165 / 176 / 176,
+    // 8192 x 512 13.0 / 13.5 / 14.2 / 16.1; the exact gelu 16.7 / 14.5 / 16.0 / 14.9, 289 / 177 / 185 / 186, 21.4 / 17.4 / 16.4 / 19.5; dz alone, silu: 6.4, 163, 10.0)
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256, strips = (n + 255) / 256;
+    long long chunks = 2ll * cus / strips, room = (long long)(CallScratch::MOST / (8 * (size_t)n));
+    if (chunks < 1) chunks = 1;
+    if (chunks > (rows + 7) / 8) chunks = (rows + 7) / 8;
+    if (chunks > room) chunks = room;
+    if (n >= vec16<T>::N && chunks >= 1) {
+        const int per = (int)((rows + chunks - 1) / chunks + 7) / 8 * 8;
+        chunks = (rows + per - 1) / per;
+        const CallScratch memory((size_t)chunks * 8 * n);
+        if (memory.ptr) {
+            RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_dz_sums_kernel<T, GATE>), dim3((unsigned)(strips * chunks)), dim3(256), 0, current_stream(), (T*)dz, (float*)memory.ptr, (const T*)dh, (const float*)z, rows, n, dh_rs, strips, per));
+            if (!check_launch("gated_dz_sums_kernel")) return -1;
+            hipLaunchKernelGGL((gated_db_kernel<T>), dim3((2 * n + 63) / 64), dim3(1024), 0, current_stream(), (T*)db, (const float*)memory.ptr, (int)chunks, 2 * n, accumulate);
+            return check_launch("gated_db_kernel") ? 0 : -1;
+        }
+    }
+    if (launch_gated_dz<T>(dz, dh, z, rows, n, gate, dh_rs) != 0) return -1;
+    const int blocks = (n + 63) / 64;
+    RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_db_any_kernel<T, GATE>), dim3(blocks), dim3(1024), 0, current_stream(), (T*)db, (const T*)dh, (const float*)z, rows, n, dh_rs, accumulate));
+    return check_launch("gated_db_any_kernel") ? 0 : -1;
+}
+
 // C (+)= A . B by the kernels of the plain products, their partial sums in memory of this stream's own; where k would be split and there is no memory for that, as one group of all rows
 static int product(void* C, const void* A, const void* B, const void* bias, int m, int k, int n, long long a_rs, long long a_cs, long long b_rs, long long b_cs, long long c_rs, int accumulate, int dtype) {
     int rc;
@@ -145,11 +267,12 @@ struct GatedGradients {
     long long dx_rs, dw_rs, dw_cs;
     int accumulate_dx, accumulate_dw, accumulate_db;
 };
-// dx = dz . W^T, dW = x^T . dz, db = sum of dz.  16-bit layers of 512 rows and more as one group of a grouped layer, whose launches make the gradients side by side (fp16, us for all three as products of
+// dx = dz . W^T, dW = x^T . dz, db = sum of dz (asked for here by float32 and float64 layers).  16-bit layers of 512 rows and more as one group of a grouped layer, whose launches make the gradients side by side (fp16, us for all three as products of
 // their own and so: 1999 x 519 x 2062 51.9 / 33.1, 4096 x 1031 x 4098 199 / 135, 1000 x 4096 x 1024 39.1 / 27.5, 8192 x 4096 x 16384 1795 / 1746; 300 x 200 x 2062 8.9 / 14.9, 1024 x 512 x 2048 14.4 / 16.8,
 // 8192 x 256 x 512 50.7 / 56.7), the others as a linear layer's.
 static int gated_gradients(const GatedGradients& o, const void* dz, const GatedArgs& g, int dtype) {
     const int n2 = 2 * g.n;
+    if (!o.dx && !o.dw && !o.db) return 0;
     if (dtype_size(dtype) == 2 && g.rows >= 512 && g.k > 512 && (!o.dw || (o.dw_cs == 1 && o.dw_rs == n2))) {
         const RowGroups all{nullptr, nullptr, 1, g.rows, 1};
         const GroupedArgs x{o.dx, dz, g.w, nullptr, nullptr, all, n2, g.k, n2, 1, 0, g.w_cs, g.w_rs, 0, o.dx_rs, o.accumulate_dx ? ACCUMULATE : 0};
@@ -245,8 +368,8 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
 }
 
 static bool gated_args_ok(const char* who, bool pointers, int rows, int k, int n, int gate, std::initializer_list<long long> strides, int dtype) {
-    if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 29) || n > (1 << 29)) {
-        set_error("%s: null operand, non-positive extent, more than 2^29 rows or columns (rows=%d k=%d n=%d)", who, rows, k, n);
+    if (!pointers || rows <= 0 || k <= 0 || n <= 0 || rows > (1 << 29) || n > (1 << 26)) {
+        set_error("%s: null operand, non-positive extent, more than 2^29 rows or 2^26 columns (rows=%d k=%d n=%d)", who, rows, k, n);
         return false;
     }
     if (!dtype_size(dtype)) { set_error("%s: unsupported dtype %d", who, dtype); return false; }
@@ -292,11 +415,13 @@ int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const v
     if (!gated_args_ok(who, dz && dh && z && (!dx || w) && (!dw || x), rows, k, n, gate, {dh_rs, x_rs, x_cs, w_rs, w_cs, dx_rs, dw_rs, dw_cs}, dtype)) return -1;
     if (dx && !gated_rows_apart(who, "dx", rows, k, dx_rs)) return -1;
     if (dw && !(dw_cs == 1 && (k == 1 || dw_rs >= 2ll * n)) && !(dw_rs == 1 && dw_cs >= k)) { set_error("%s: dw has unit stride along one axis and rows that do not overlap along the other", who); return -1; }
-    RP_DISPATCH_DTYPE(dtype, using A = typename traits<T>::acc;
-        const int across = (n + 256 * vec16<T>::N - 1) / (256 * vec16<T>::N);
-        const long long blocks = (long long)rows * across;
-        RP_DISPATCH_GATE(gate, hipLaunchKernelGGL((gated_dz_kernel<T, GATE>), dim3((unsigned)(blocks < GATED_GRID ? blocks : GATED_GRID)), dim3(256), 0, current_stream(), (T*)dz, (const T*)dh, (const A*)z, rows, n, dh_rs, across));
-        if (!check_launch("gated_dz_kernel")) return -1);
+    if (db && dtype_size(dtype) == 2) {
+        const int rc = dtype == RP_DTYPE_BFLOAT16 ? launch_gated_dz_sums<bf16_t>(dz, db, dh, z, rows, n, gate, dh_rs, accumulate_db) : launch_gated_dz_sums<f16_t>(dz, db, dh, z, rows, n, gate, dh_rs, accumulate_db);
+        if (rc != 0) return -1;
+        db = nullptr;
+    } else {
+        RP_DISPATCH_DTYPE(dtype, if (launch_gated_dz<T>(dz, dh, z, rows, n, gate, dh_rs) != 0) return -1);
+    }
     return gated_gradients(GatedGradients{dx, dw, db, dx_rs, dw_rs, dw_cs, accumulate_dx, accumulate_dw, accumulate_db}, dz, GatedArgs{nullptr, nullptr, x, w, nullptr, rows, k, n, gate, x_rs, x_cs, w_rs, w_cs, 0}, dtype);
 }
 

@@ -159,6 +159,21 @@ def test_gated_layer_of_more_than_2_to_31_sums():
         assert_within(got_dx[row], d @ w.values.T, rounded((2 * n + 8) * 2.0 ** -24 * (np.abs(d) @ np.abs(w.values).T), d @ w.values.T, dtype), "dx")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=NAMES.get)
+@pytest.mark.parametrize("rows,n", [(40, 5), (40, 64), (600, 300), (4, (1 << 21) + 8)])
+def test_sums_of_a_gated_layer_are_made_before_dz_is_rounded(rows, n, dtype):
+    """Rows whose dz are 1 + 2^-12 and -1 by turns: rounded, each pair would cancel."""
+    z, dh = np.full((rows, 2 * n), 1.0), np.ones((rows, n))
+    z[::2, :n], z[::2, n:] = 1 + 2.0 ** -12, 1 + 2.0 ** -11
+    dh[1::2] = -1
+    zd, dhd, dz, db = Operand(z, F32), Operand(dh, dtype), Output(rows, 2 * n, dtype), Output(1, 2 * n, dtype)
+    capi.check(capi.lib().rp_hip_gated_linear_backward(None, None, db.ptr, dz.ptr, dhd.ptr, zd.ptr, None, None, rows, 8, n, GATES["relu"], n, 8, 1, 2 * n, 1, 8, 2 * n, 1, 0, 0, 0, dtype), "backward")
+    got = db.read()[0]
+    assert np.all(got[:n] == rows / 2 * 2.0 ** -11) and np.all(got[n:] == rows / 2 * 2.0 ** -12)      # (exact in every type)
+    # dz: bf16 steps by 2^-7 above 1, float16 by 2^-10
+    assert np.array_equal(np.abs(dz.read()), np.ones((rows, 2 * n)))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=NAMES.get)
 def test_vocabulary_loss_of_rows_far_apart(dtype):
     rows, k, classes = 1200, 136, 1000
