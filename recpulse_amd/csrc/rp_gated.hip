@@ -347,6 +347,9 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
     Plan p{FAM_MFMA16, 64, 64, false, b_mc, true, ""};
     p.ragged = ragged;
     choose_tile16(p, 1, g.rows, g.k, 2 * g.n);
+    // (of four slabs the epilogue is most of the work, and tiles of 128 have two workgroups a CU for it: fp16, z kept, us on 256 and on 128: 256 -> 2048 of 1999 rows 36.9 / 18.9, of 4000 36.1 / 29.8,
+    // of 8192 55.0 / 53.9; 256 -> 8192 of 4000 133 / 106, of 8192 221 / 231; 512 -> 4096 of 2500 44.4 / 46.7)
+    if (p.bm == 256 && g.k <= 4 * M16_BK) p.bm = p.bn = 128;
     if (!ragged && p.bm == 256 && p.bn == 256) {
         const int edge = g.rows % 256 || g.n % 128 || g.k % M16_BK ? M16_EDGE : M16_WHOLE;
         return dtype == RP_DTYPE_BFLOAT16 ? launch_gated16_256_bf16(g, edge) : launch_gated16_256_f16(g, edge);
