@@ -1203,6 +1203,15 @@ void settle(Tensor* const* targets, GradSlot* slots, int count, bool ok, const c
         else free_tensor(slots[i].fresh);
     }
 }
+// Gradients of one tensor that is several of a node's inputs: the calls write their outputs side by side, so that only the first may go where a gradient is already
+void slots_apart(Tensor* const* targets, GradSlot* slots, int count) {
+    for (int i = 1; i < count; i++)
+        for (int j = 0; j < i; j++)
+            if (targets[i] && targets[i] == targets[j] && slots[i].into && !slots[i].fresh) {
+                slots[i].fresh = slots[i].into = empty_tensor(targets[i]->dtype, targets[i]->device_id, targets[i]->ndim, targets[i]->shape);
+                slots[i].accumulate = 0;
+            }
+}
 void* slot_data(const GradSlot& s) { return s.into ? s.into->data : nullptr; }
 
 // The upstream gradient of a loss in the accumulate type, where the loss is: one element, or one for each row
@@ -1221,6 +1230,7 @@ void backward_layer_norm_fn(GradFn* self, Tensor* grad_output) {
     Tensor* gd = dense(grad_output); Tensor* xd = dense(x);
     Tensor* targets[3] = {x, w, b};
     GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(b)};
+    slots_apart(targets, slots, 3);
     void* room = nullptr;
     bool ok = gd && xd && on_device(x->device_id);
     if (ok && (slots[1].into || slots[2].into)) ok = rp_hip_malloc(&room, (size_t)rp_hip_layer_norm_workspace(rows, d, x->dtype)) == 0;
@@ -1240,6 +1250,7 @@ void backward_gated_linear_fn(GradFn* self, Tensor* grad_output) {
     Tensor* gd = dense(grad_output);
     Tensor* targets[3] = {x, w, bias};
     GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(bias)};
+    slots_apart(targets, slots, 3);
     void* dz = nullptr;
     const bool ok = gd && on_device(x->device_id) && rp_hip_malloc(&dz, dtype_size(x->dtype) * 2 * (size_t)rows * n) == 0 &&
                     rp_hip_gated_linear_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), dz, gd->data, s->kept, x->data, w->data, rows, k, n, s->choice,
@@ -1258,6 +1269,7 @@ void backward_linear_cross_entropy_fn(GradFn* self, Tensor* grad_output) {
     if (!up) { fail("op_linear_cross_entropy backward: upstream gradient has the wrong size"); return; }
     Tensor* targets[3] = {x, w, bias};
     GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(bias)};
+    slots_apart(targets, slots, 3);
     void* room = nullptr;
     const bool ok = on_device(x->device_id) && rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, x->dtype)) == 0 &&
                     rp_hip_linear_cross_entropy_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), x->data, w->data, bias ? bias->data : nullptr, (const int*)s->plan, s->kept, up->data, room,

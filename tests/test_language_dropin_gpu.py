@@ -253,3 +253,22 @@ def test_training_step_in_few_bits(dtype):
     for name, want in results["float64"].items():
         off = np.linalg.norm(results[dtype][name] - want) / np.linalg.norm(want)
         assert off <= 12 * HALF_STEP[dtype] + 2000 * UNIT[dtype], (name, off)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_one_tensor_as_several_inputs(dtype):
+    """... whose gradients add up, those of a second pass to those of the first."""
+    rng = np.random.default_rng(11)
+    x, w = spread(rng, 300, 24), spread(rng, 24)
+    xd, wd = dev(x, dtype), dev(w, dtype, True)
+    for _ in range(2):
+        xd.op_layer_norm(wd, wd, 1e-3).op_sum_all().backward()
+    _, dw, db = norm_gradients(x, w, np.ones((300, 24)), 1e-3)
+    close(host(wd.grad), 2 * (dw + db), dtype, 400)
+    k = 544
+    x = spread(rng, k, k) / 16
+    xd = dev(x, dtype, True)
+    for _ in range(2):
+        xd.op_gated_linear(xd, None, "sigmoid").op_sum_all().backward()
+    _, dx, dw, _ = gate_and_gradients(x, x, np.zeros(k), "sigmoid", np.ones((k, k // 2)))
+    close(host(xd.grad), 2 * (dx + dw), dtype, 2 * k)
