@@ -356,10 +356,12 @@ static int gated16_forward(const GatedArgs& g, int dtype, bool* taken) {
     }
     const int edge = ragged ? M16_RAGGED : M16_EDGE;
     if (g.rows > 64 && p.bm >= 128 && p.bn >= 128) return launch_gated16_128(g, edge, dtype);
-    // Few tiles: k in shares of at least eight slabs, up to three workgroups a CU (bf16, 16 rows, 4096 -> 8192: 128 tiles 40 us, in six shares 26 and 4.5 for the launch that joins them)
+    // Few tiles: k in shares of at least eight slabs, a workgroup a CU where that keeps seven eighths of them busy, else two (bf16, us with one, two and three a CU: 16 rows, 4096 -> 8192 32.4 / 32.1 / 36.7
+    // (one share: 40), -> 5120 18.9 / 19.8 / 23.0, -> 6144 31.2 / 25.4 / 29.7, -> 10240 53.2 / 41.3 / 50.1; 64 rows, -> 8192 34.2 / 38.8 / 38.8, -> 6144 33.4 / 31.7 / 31.5)
     const long long tiles = (long long)((g.rows + 63) / 64) * ((g.n + 63) / 64), share_bytes = 8ll * g.rows * g.n;
     const int cus = device_cu_count() > 0 ? device_cu_count() : 256, slabs = (g.k + M16_BK - 1) / M16_BK;
-    long long count = 3ll * cus / tiles;
+    long long count = cus / tiles;
+    if (8 * count * tiles < 7ll * cus) count = 2ll * cus / tiles;
     if (count > slabs / 8) count = slabs / 8;
     if (count > (long long)CallScratch::MOST / share_bytes) count = (long long)CallScratch::MOST / share_bytes;
     if (count >= 2 && !path_disabled("gated_shares")) {

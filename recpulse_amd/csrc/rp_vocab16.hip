@@ -54,8 +54,9 @@ bool vocab16_takes(const VocabArgs& g, int dtype) {
     return logits_lie(g) != LIES_NEITHER && (long long)((g.rows + 63) / 64) * ((g.classes + 127) / 128) < (1 << 24) - 64;
 }
 
-// Few tiles and a long k: k goes in shares to workgroups of their own, three a CU, at least eight slabs each.  (fp16, 1000 rows, 520 -> 10007: dx
-// on 40 tiles of 128 walks 157 slabs, 72 us; in 12 shares 31 and 8 for the launch that joins them)
+// Few tiles and a long k: k goes in shares of at least eight slabs to workgroups of their own, three a CU, or one where tiles of 128 keep seven eighths of the CUs busy so.  (fp16, 1000 rows, 520 -> 10007:
+// dx on 40 tiles of 128 walks 157 slabs, 72 us; in 12 shares 31 and 8 for the launch that joins them.  Both passes, us with three a CU and one: 1000, 520 -> 10007 147 / 141, 512, 1024 -> 32000 231 / 217,
+// 1024, 768 -> 50000 589 / 584; on tiles of 64: 16, 4096 -> 32000 247 / 268)
 constexpr long long VOCAB16_SHARE_BYTES = 32ll << 20;      // of the shares' sums
 struct Shares { int count, k; long long stride; };
 static Shares vocab_shares(int m, int n, int k, const VocabTile& t) {
@@ -63,7 +64,8 @@ static Shares vocab_shares(int m, int n, int k, const VocabTile& t) {
     if (t.edge == 256 || path_disabled("vocab_shares")) return one;
     const long long tiles = (long long)((m + t.edge - 1) / t.edge) * ((n + t.edge - 1) / t.edge), area = tiles * t.edge * t.edge;
     const int cus = device_cu_count() > 0 ? device_cu_count() : 256, slabs = (k + M16_BK - 1) / M16_BK;
-    long long count = 3ll * cus / tiles;
+    long long count = cus / tiles;
+    if (t.edge == 64 || 8 * count * tiles < 7ll * cus) count = 3ll * cus / tiles;
     if (count > slabs / 8) count = slabs / 8;
     if (count > 16) count = 16;
     if (count > VOCAB16_SHARE_BYTES / (area * 4)) count = VOCAB16_SHARE_BYTES / (area * 4);
