@@ -50,6 +50,19 @@ __device__ __forceinline__ void correct_entries(int k, T* grad, const int* ids, 
 constexpr int DISTILL_SHARED_STEPS = 8;
 constexpr int distill_waves(int threads, int steps, int elem) { return threads == 1024 ? (steps <= DISTILL_SHARED_STEPS && elem < 8 ? 8 : 4) : 1; }
 
+// Whether a forward pass corrects a row's entries during the next row, whose loads it does not wait for then: not in the kernels whose row leaves no registers for it (bf16, us at once and later:
+// 4096 x 32000 131 / 123, 2000 x 130000 286 / 271; 4096 x 65536 272 / 288)
+constexpr bool distill_later(int threads, int steps, int elem) { return !(threads == 1024 && steps == DISTILL_SHARED_STEPS && elem < 8); }
+
+// A value that all lanes have, in scalar registers
+__device__ __forceinline__ float in_scalar(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ double in_scalar(double v) { return __hiloint2double(__builtin_amdgcn_readfirstlane(__double2hiint(v)), __builtin_amdgcn_readfirstlane(__double2loint(v))); }
+template <typename T> __device__ __forceinline__ void load_one(T& x, const __amdgpu_buffer_rsrc_t& from, int offset) {
+    if constexpr (sizeof(T) == 2) { const uint16_t v = __builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0); __builtin_memcpy(&x, &v, 2); }
+    else if constexpr (sizeof(T) == 4) { const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0); __builtin_memcpy(&x, &v, 4); }
+    else { const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0); __builtin_memcpy(&x, &v, 8); }
+}
+
 // FORWARD: the row's sums and loss; with a gradient asked for, that too.  Otherwise the gradient from the sums that a forward call left.  STEPS 0: the row is read again for each.
 // A workgroup walks rows; the next row's loads are issued as soon as a row's registers are stored, and fly while its last steps wait for one another.  k <= THREADS: a thread has an entry or none.
 template <typename T, int THREADS, int STEPS, bool FORWARD>
@@ -59,7 +72,8 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
     __shared__ A rooms[3][2][WAVES];
     __shared__ A entry_p[2][THREADS];              // (of this row and of the one before, which may still be read)
     __shared__ int entry_ids[2][THREADS];
-    const A scale = (A)1 / g.temperature;
+    __shared__ A entry_value[2][THREADS];          // (the thread's own: registers are for the row.  With these and what all lanes share in scalar ones 4096 x 65536 bf16 288 us -> 272)
+    const A scale = in_scalar((A)1 / g.temperature);
     // Vector i of a thread begins at byte tid * 16 + i * THREADS * 16 of the row, which buffer descriptors end with its last whole 4 bytes: what lies behind reads as zeros and is not
     // written, and one offset does for all loads.  Step i is whole where every thread's vector lies in the row; an odd last element of 16 bits goes by itself.
     auto whole = [&](int i) { return (i + 1) * THREADS * N <= g.classes; };
@@ -76,9 +90,10 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
     auto load_entry = [&](int row) {
         if (row >= g.rows) row = g.rows - 1;
         if (odd) last = row_of(row)[g.classes - 1];
+        // (one offset a thread for either, no addresses)
         if ((int)threadIdx.x < g.k) {
-            id = g.ids[(long long)row * g.k + threadIdx.x];
-            entry = ((const T*)g.teacher)[(long long)row * g.k + threadIdx.x];
+            id = (int)__builtin_amdgcn_raw_buffer_load_b32(buffer_rsrc(g.ids + (long long)row * g.k, g.k * 4ll), (int)threadIdx.x * 4, 0, 0);
+            load_one(entry, buffer_rsrc((const T*)g.teacher + (long long)row * g.k, g.k * (long long)sizeof(T)), (int)threadIdx.x * (int)sizeof(T));
         }
     };
     {
@@ -86,7 +101,18 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
         static_for<0, STEPS>([&](auto ic) { load_step(from, ic); });
         load_entry(blockIdx.x);
     }
-    for (int row = blockIdx.x, turn = 0; row < g.rows; row += gridDim.x, turn ^= 1) {
+    // The entries of the row before are corrected once this row's loads have been waited for, before which its stores were issued, and all threads have met
+    A lse_before = 0, factor_before = 0;
+    bool some_before = false;
+    auto correct_before = [&](int row, int turn) {
+        if (!some_before) return;
+        const bool own = (int)threadIdx.x < g.k;
+        correct_entries<T>(g.k, (T*)g.grad + (long long)row * g.classes, entry_ids[turn], entry_p[turn], own ? entry_ids[turn][threadIdx.x] : -1, own ? entry_value[turn][threadIdx.x] : (A)0,
+                           ScaledExp<A>(scale, lse_before), factor_before);
+    };
+    constexpr bool LATER = FORWARD && distill_later(THREADS, STEPS, sizeof(T));
+    int row = blockIdx.x, turn = 0;
+    for (; row < g.rows; row += gridDim.x, turn ^= 1) {
         const T* s = row_of(row);
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));              // (the masks of a row's end are made again for each row: kept, they would take more registers than there are)
@@ -94,10 +120,14 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
         A* p = entry_p[turn];
         int* ids = entry_ids[turn];
         A log_p = id >= 0 && id < g.classes ? widen(entry) * scale : -(A)INFINITY;
-        const int v = log_p == -(A)INFINITY ? -1 : id;
-        const A value = v < 0 ? (A)0 : widen(s[v]);
+        int v = log_p == -(A)INFINITY ? -1 : id;
+        A value = v < 0 ? (A)0 : widen(s[v]);
         const T row_last = last;
-        if (tid < g.k) ids[tid] = v;
+        if (tid < g.k) {
+            ids[tid] = v;
+            p[tid] = log_p;
+            entry_value[turn][tid] = value;
+        }
         if constexpr (STEPS > 0) {
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
@@ -151,7 +181,9 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 each([&](A x) { top = plain_max(top, x); });      // (NaN shows in the sum)
             }
             A tops[2] = {top, log_p};
+            if (LATER) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             team_tops_in_turn<THREADS>(tops, rooms[0][0]);
+            if (LATER) correct_before(row - (int)gridDim.x, turn ^ 1);
             top = tops[0];
             if constexpr (STEPS > 0 && sizeof(T) == 2) {
                 again = !(top >= (A)0);
@@ -167,16 +199,21 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                     top = one[0];
                 }
             }
-            const A base = top == -(A)INFINITY ? (A)0 : top * scale;
+            const A base = in_scalar(top == -(A)INFINITY ? (A)0 : top * scale);
             const ScaledExp<A> weight(scale, base);
             A sums[2] = {(A)0, v < 0 ? (A)0 : natural_exp(log_p - tops[1])};
             each([&](A x) { sums[0] += weight(x); });
             team_sums_in_turn<THREADS>(sums, rooms[1][0]);
-            lse = base + natural_log(sums[0]);
-            log_mass = tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]);
+            lse = in_scalar(base + natural_log(sums[0]));
+            log_mass = in_scalar(tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]));
         } else {
             lse = g.stats[row];
             log_mass = g.stats[g.rows + row];
+        }
+        if (FORWARD) {                             // (two barriers ago)
+            v = tid < g.k ? ids[tid] : -1;
+            log_p = tid < g.k ? p[tid] : -(A)INFINITY;
+            value = tid < g.k ? entry_value[turn][tid] : (A)0;
         }
         const bool some = !(log_mass == -(A)INFINITY);
         log_p -= log_mass;
@@ -198,7 +235,7 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
             continue;                              // (two barriers lie between a room's readers and its next writers)
         }
         T* grad = (T*)g.grad + (long long)row * g.classes;
-        const A factor = row_factor(g, row);
+        const A factor = in_scalar(row_factor(g, row));
         const ScaledExp<A> q(scale, lse);
         auto share = [&](A x) { return some ? q(x) * factor : (A)0; };
         if (tid < g.k) p[tid] = own_p;
@@ -238,9 +275,20 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
             for (int c = tid; c < g.classes; c += THREADS) grad[c] = round_to<T>(share(widen(s[c])));
         }
         load_entry(row + gridDim.x);
+        if (LATER) {
+            lse_before = lse;
+            factor_before = factor;
+            some_before = some;
+            continue;
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                           // the row's stores are done: the entries' classes come after
         if (some) correct_entries<T>(g.k, grad, ids, p, v, value, q, factor);
+    }
+    if (LATER && g.grad) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        correct_before(row - (int)gridDim.x, turn ^ 1);
     }
 }
 
@@ -250,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 8 : 4) distill_loss_r
     using A = typename traits<T>::acc;
     constexpr int N = vec16<T>::N, U = 4, WAVES = THREADS / 64, PIECE = U * THREADS * N;
     __shared__ A rooms[3][2][WAVES];
-    const A scale = (A)1 / g.temperature;
+    const A scale = in_scalar((A)1 / g.temperature);
     const int row_bytes = g.classes * (int)sizeof(T) / 4 * 4, tid = threadIdx.x;
     const bool odd = sizeof(T) == 2 && g.classes % 2;
     for (int row = blockIdx.x; row < g.rows; row += gridDim.x) {
