@@ -55,7 +55,7 @@ bool vocab16_takes(const VocabArgs& g, int dtype) {
 }
 
 // Few tiles and a long k: k goes in shares of at least eight slabs to workgroups of their own, three a CU, or one where tiles of 128 keep seven eighths of the CUs busy so.  (fp16, 1000 rows, 520 -> 10007:
-// dx on 40 tiles of 128 walks 157 slabs, 72 us; in 12 shares 31 and 8 for the launch that joins them.  Both passes, us with three a CU and one: 1000, 520 -> 10007 147 / 141, 512, 1024 -> 32000 231 / 217,
+// dx on 40 tiles of 128 walks 157 slabs, 72 us; in six shares 29 and 5 for the launch that joins them.  Both passes, us with three a CU and one: 1000, 520 -> 10007 147 / 141, 512, 1024 -> 32000 231 / 217,
 // 1024, 768 -> 50000 589 / 584; on tiles of 64: 16, 4096 -> 32000 247 / 268)
 constexpr long long VOCAB16_SHARE_BYTES = 32ll << 20;      // of the shares' sums
 struct Shares { int count, k; long long stride; };

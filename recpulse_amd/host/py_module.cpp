@@ -268,8 +268,13 @@ PYBIND11_MODULE(recpulse_cuda, m) {
         }, py::arg("weight"), py::arg("targets"), py::arg("bias") = py::none(), py::arg("reduction") = "mean")
         .def("op_distillation_loss", [](PyTensor& x, py::object ids, PyTensor& teacher, double temperature, const std::string& reduction) {
             std::vector<int> flat;
-            for (auto row : ids) for (auto item : row) flat.push_back(item.cast<int>());
-            if (flat.size() != teacher.t->size) throw std::runtime_error("op_distillation_loss operation failed: one class for each of the teacher's entries");
+            size_t rows = 0;
+            bool even = teacher.t->ndim == 2;
+            for (auto row : ids) {
+                for (auto item : row) flat.push_back(item.cast<int>());
+                even = even && flat.size() == ++rows * (size_t)teacher.t->shape[1];      // (not one row's classes among the next one's)
+            }
+            if (!even || flat.size() != teacher.t->size) throw std::runtime_error("op_distillation_loss operation failed: one class for each of the teacher's entries");
             return wrap(op_distillation_loss(x.t, flat.data(), teacher.t, temperature, reduction_from(reduction)), "op_distillation_loss");
         }, py::arg("ids"), py::arg("teacher"), py::arg("temperature") = 1.0, py::arg("reduction") = "mean")
         .def("op_add", [](PyTensor& a, PyTensor& b) { return wrap(op_add(a.t, b.t), "op_add"); })

@@ -22,6 +22,8 @@ def test_names_that_do_not_exist_are_refused():
         LinearCrossEntropy(6, 9, reduction="max")(x, [0, 1, 2, 3])
     with pytest.raises(RuntimeError, match="one class for each"):
         x.op_distillation_loss([[0, 1]], rp.from_numpy(np.ones((4, 1), np.float32)))
+    with pytest.raises(RuntimeError, match="one class for each"):      # as many as the teacher has, but not a row's
+        x.op_distillation_loss([[0, 1, 2], [3], [0, 1], [2, 3]], rp.from_numpy(np.ones((4, 2), np.float32)))
 
 
 def test_modules_keep_their_parameters():
