@@ -26,10 +26,14 @@ struct VocabTileArgs {
     // gradient of the logits
     uint16_t* d;                   // [rows][pitch]
     long long pitch;
-    const float *lse, *f;          // [rows]
+    const float *lse, *f;          // [rows]; f null: every row with a target has the same (its rows are 2^most, and row_weight says what it is)
     float* db_parts;               // [groups of rows][pitch], or null
-    // dx, dw
-    const float* scale;            // what d has been multiplied by, inverted
+    void* db;                      // where one wave has all rows: db of the piece instead, or null
+    int accumulate_db;
+    // ... and of dx, dw
+    const float* scale;            // what d has been multiplied by, inverted; null where f is
+    const float *upstream, *count; // one element each, or null: 1
+    int most;
     float* sums;                   // dx between pieces and sums of shares of k, tile by tile in the order of a tile's registers
     int first, last;
     // k in shares of k_share that workgroups of their own add up (their sums `share_stride` floats apart), where there are few tiles; 1: none
@@ -145,6 +149,21 @@ struct VocabForward : M16Source {
     }
 };
 
+// f of every row that has a target, where it is the same, and what d is multiplied by for it and dx, dw and db afterwards
+__device__ __forceinline__ float row_weight(const VocabTileArgs& a) {
+    const float u = a.upstream ? *a.upstream : 1.f;
+    return a.count ? u / *a.count : u;
+}
+__device__ __forceinline__ float stored_weight(const VocabTileArgs& a) {
+    const float u = row_weight(a);
+    return __builtin_isfinite(u) ? ldexpf(1.f, a.most) : u;      // (an infinity belongs to the rows that have a target)
+}
+__device__ __forceinline__ float scale_back(const VocabTileArgs& a) {
+    if (a.scale) return *a.scale;
+    const float u = row_weight(a);
+    return __builtin_isfinite(u) ? ldexpf(u, -a.most) : 1.f;
+}
+
 // Logits to their gradient
 struct VocabGradient : M16Source {
     static constexpr bool ONCE = true, TAKES = true;
@@ -159,12 +178,14 @@ struct VocabGradient : M16Source {
         float* lse = (float*)(smem + 4 * WM * EP);
         float* f = lse + BM;
         int* target = (int*)(f + BM);
+        const float same_f = a.f ? 0.f : stored_weight(a);
         __syncthreads();
         for (int r = t; r < BM; r += 256) {
             const bool there = m0 + r < a.g.m;
             lse[r] = there ? a.lse[m0 + r] * LOG2_E : 0.f;
-            f[r] = there ? a.f[m0 + r] : 0.f;
-            target[r] = there ? a.targets[m0 + r] - a.v0 : -1;
+            const int goal = there ? a.targets[m0 + r] : -1;
+            f[r] = a.f ? there ? a.f[m0 + r] : 0.f : goal >= 0 && goal < a.classes ? same_f : 0.f;
+            target[r] = there ? goal - a.v0 : -1;
         }
         __syncthreads();
         float bias[TNI], column[TNI];
@@ -192,6 +213,19 @@ struct VocabGradient : M16Source {
             });
             __builtin_amdgcn_sched_barrier(0);
         });
+        if (a.db && wave / WGN == 0) {
+            const float scale = scale_back(a);
+            static_for<0, TNI>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                if constexpr (MT == 16) column[j] += __shfl_xor(column[j], 16);
+                column[j] += __shfl_xor(column[j], 32);
+                const int col = n0 + wn0 + j * MT + lane;
+                if (lane < MT && col < a.g.n) {
+                    T* to = (T*)a.db + col;
+                    *to = round_to<T>(a.accumulate_db ? widen(*to) + column[j] * scale : column[j] * scale);
+                }
+            });
+        }
         if (a.db_parts) {
             float* to = a.db_parts + (long long)(m0 / WM + wave / WGN) * a.pitch + n0 + wn0;
             static_for<0, TNI>([&](auto jc) {
@@ -221,7 +255,7 @@ struct VocabGradProduct : M16Source {
     static constexpr bool ONCE = true, SCALED = true, TAKES = SUMS;
     const VocabTileArgs& a;
     __device__ __forceinline__ VocabGradProduct(const VocabTileArgs& args) : a(args) {}
-    __device__ __forceinline__ float scale() const { return *a.scale; }
+    __device__ __forceinline__ float scale() const { return scale_back(a); }
     template <typename T, int MT, int WGN, int TMI, int TNI, int EDGE, typename ACC>
     __device__ __forceinline__ bool take(ACC (&acc)[TMI][TNI], uint16_t*, int m0, int n0) {
         constexpr int NV = MT == 32 ? 16 : 4, BM = 4 / WGN * TMI * MT, BN = WGN * TNI * MT;
@@ -275,7 +309,7 @@ __global__ void __launch_bounds__(256) vocab16_join_kernel(VocabTileArgs a) {
     for (int s = 0; s < a.shares; s++)
 #pragma unroll
         for (int e = 0; e < 4; e++) sum[e] += *(const f32x4_t*)((const float*)(own + (q0 + e) * 256) + s * a.share_stride);
-    const float scale = *a.scale;
+    const float scale = scale_back(a);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const int i = (q0 + e) / (TM * 4), j = (q0 + e) / 4 % TM, col = n0 + j * 32 + (lane & 31), row = m0 + i * 32 + 8 * e + 4 * (lane >> 5);

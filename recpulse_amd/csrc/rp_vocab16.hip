@@ -140,16 +140,13 @@ __global__ void __launch_bounds__(1024) vocab16_rows_kernel(float* stats, const 
     }
 }
 
-// f of each row over the largest of them, times 2^most, and what takes that back: one workgroup
-__global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* scale, const float* stats, const float* upstream, const int* targets, int rows, int classes, int reduction, int most) {
+// Rows with an upstream gradient of their own: f of each over the largest of them, times 2^most, and what takes that back: one workgroup
+__global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* scale, const float* upstream, const int* targets, int rows, int classes, int most) {
     __shared__ float room[16];
     float top = 0.f;
     for (int i = threadIdx.x; i < rows; i += 1024) {
         float v = 0.f;
-        if (targets[i] >= 0 && targets[i] < classes) {
-            v = upstream ? upstream[reduction == 0 ? i : 0] : 1.f;
-            if (reduction == 1) v /= stats[2ll * rows];
-        }
+        if (targets[i] >= 0 && targets[i] < classes) v = upstream ? upstream[i] : 1.f;
         f[i] = v;
         top = fmaxf(top, __builtin_isfinite(v) ? fabsf(v) : 0.f);
     }
@@ -162,7 +159,7 @@ __global__ void __launch_bounds__(1024) vocab16_factors_kernel(float* f, float* 
 
 // db of a piece from its groups' sums
 template <typename T>
-__global__ void __launch_bounds__(1024) vocab16_db_kernel(T* db, const float* parts, const float* scale, int groups, long long pitch, int width, int accumulate) {
+__global__ void __launch_bounds__(1024) vocab16_db_kernel(VocabTileArgs a, T* db, const float* parts, int groups, long long pitch, int width, int accumulate) {
     __shared__ float room[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane;
     float sum = 0.f;
@@ -174,7 +171,7 @@ __global__ void __launch_bounds__(1024) vocab16_db_kernel(T* db, const float* pa
     if (wave || c >= width) return;
 #pragma unroll
     for (int w = 1; w < 16; w++) sum += room[w][lane];
-    sum *= *scale;
+    sum *= scale_back(a);
     db[c] = round_to<T>(accumulate ? widen(db[c]) + sum : sum);
 }
 
@@ -254,8 +251,20 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
     VocabTile dx_tile = vocab_tile(g.rows, g.k, longest, true, false, tied, worse16(lie, g.classes % 8 ? LIES_RAGGED : LIES_WHOLE));
     if (dx_tile.over == M16_WHOLE && g.classes % M16_BK) dx_tile.over = M16_EDGE;
     const Shares dx_shares = g.classes > r.piece ? Shares{1, 0, 0} : vocab_shares(g.rows, g.k, longest, dx_tile);
-    hipLaunchKernelGGL(vocab16_factors_kernel, dim3(1), dim3(1024), 0, current_stream(), r.f, r.scale, stats, upstream, g.targets, g.rows, g.classes, g.reduction, dtype == RP_DTYPE_FLOAT16 ? 14 : 0);
-    if (!check_launch("vocab16_factors_kernel")) return -1;
+    // one f for all rows, or one for each
+    const bool same = g.reduction != 0;
+    const int most = dtype == RP_DTYPE_FLOAT16 ? 14 : 0;
+    if (!same) {
+        hipLaunchKernelGGL(vocab16_factors_kernel, dim3(1), dim3(1024), 0, current_stream(), r.f, r.scale, upstream, g.targets, g.rows, g.classes, most);
+        if (!check_launch("vocab16_factors_kernel")) return -1;
+    }
+    auto weighted = [&](VocabTileArgs& a) {
+        a.f = same ? nullptr : r.f;
+        a.scale = same ? nullptr : r.scale;
+        a.upstream = upstream;
+        a.count = g.reduction == 1 ? stats + 2ll * g.rows : nullptr;
+        a.most = most;
+    };
     for (int v0 = 0, width; v0 < g.classes; v0 += width) {
         width = r.width(v0, g.classes);
         const char *w = (const char*)g.w + 2 * v0 * g.w_cs, *bias = g.bias ? (const char*)g.bias + 2ll * v0 : nullptr;
@@ -268,17 +277,20 @@ int vocab16_backward(const VocabGrads& o, const VocabArgs& g, const float* stats
         a.d = r.d;
         a.pitch = r.pitch;
         a.lse = stats;
-        a.f = r.f;
-        a.db_parts = o.db ? r.db_parts : nullptr;
+        weighted(a);
         const int piece_lie = worse16(lie, g.w_cs == 1 && width % 8 ? LIES_RAGGED : LIES_WHOLE);
+        const int patch = patch_rows(vocab_tile(g.rows, width, g.k, false, false, !tied, piece_lie).edge), groups = (g.rows + patch - 1) / patch;
+        if (o.db && groups == 1) {
+            a.db = (char*)o.db + 2ll * v0;
+            a.accumulate_db = o.accumulate_db;
+        } else if (o.db) a.db_parts = r.db_parts;
         if (launch_logits(a, VOCAB_GRADIENT, !tied, piece_lie, dtype) != 0) return -1;
-        if (o.db) {
-            const int patch = patch_rows(vocab_tile(g.rows, width, g.k, false, false, !tied, piece_lie).edge), groups = (g.rows + patch - 1) / patch;
-            RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vocab16_db_kernel<T>), dim3((width + 63) / 64), dim3(1024), 0, current_stream(), (T*)o.db + v0, r.db_parts, r.scale, groups, (long long)r.pitch, width, o.accumulate_db));
+        if (a.db_parts) {
+            RP_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vocab16_db_kernel<T>), dim3((width + 63) / 64), dim3(1024), 0, current_stream(), a, (T*)o.db + v0, r.db_parts, groups, (long long)r.pitch, width, o.accumulate_db));
             if (!check_launch("vocab16_db_kernel")) return -1;
         }
         VocabTileArgs p{};
-        p.scale = r.scale;
+        weighted(p);
         if (o.dx) {
             p.g = GemmArgs{o.dx, r.d, w, nullptr, 1, g.rows, width, g.k, 0, r.pitch, 1, 0, g.w_cs, g.w_rs, 0, o.dx_rs, 1, o.accumulate_dx};
             p.sums = r.sums;
