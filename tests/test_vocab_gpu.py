@@ -314,3 +314,25 @@ def test_recorded_calls_replay_to_the_eager_result(rows, k, classes, dtype):
             graph.launch()
             capi.check(capi.lib().rp_hip_stream_synchronize(), "sync")
             assert all(np.array_equal(a, o.bits()) for a, o in zip(eager, outs))
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("rows,k,classes", [(24, 128, 1000), (300, 136, 1104)])
+@pytest.mark.parametrize("upstream", [0.0, np.inf, np.nan, -2.0 ** -100])
+def test_upstream_gradients_that_are_not_ordinary_numbers(upstream, rows, k, classes, dtype):
+    """Rows without a target stay zeros; with a gradient of zero, or one too small for any product of it, all are."""
+    _, x, w, _, targets = problem(rows, k, classes, dtype, 15, bias=False)
+    for reduction in (0, 1, 2):
+        space = room(capi.lib().rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, dtype))
+        _, stats = forward(x, w, None, targets, dtype, reduction, space)
+        up = vector(np.full(rows if reduction == 0 else 1, upstream), ACC[dtype])
+        dx, db = Output(rows, k, dtype), Output(1, classes, dtype)
+        capi.check(capi.lib().rp_hip_linear_cross_entropy_backward(dx.ptr, None, db.ptr, x.ptr, w.ptr, None, ints(targets).ptr, stats.ptr, up.ptr, space.ptr, rows, k, classes, reduction,
+                                                                   x.rs, 1, classes, 1, k, 0, 1, 0, 0, 0, dtype), "backward")
+        got = dx.read()
+        assert np.all(got[targets < 0] == 0)
+        if np.isfinite(upstream):
+            assert np.all(np.abs(got) <= abs(upstream) * 64)             # (|d| adds up to less than two, |w| is below 32)
+            assert np.all(np.abs(db.read()) <= abs(upstream) * rows)
+        else:
+            assert not np.any(np.isfinite(got[targets >= 0])) and not np.any(np.isfinite(db.read()))
