@@ -13,7 +13,7 @@ constexpr long long VOCAB_PIECE_BYTES = 64ll << 20;      // of a piece's logits
 constexpr size_t VOCAB_GEMM_BYTES = 16 << 20;            // for the partial sums of its products
 // Few rows: dx of a piece is split along its classes, 2048 a share, and 32 shares of 8 rows and 16384 float32 fill that memory
 constexpr int VOCAB_FEW_ROWS = 8, VOCAB_FEW_PIECE = 65536;
-constexpr int VOCAB_GRID = 1 << 20;
+constexpr int VOCAB_GRID = 1 << 20;                      // (of 1024 threads: fewer than 2^32)
 
 static int vocab_piece(int rows, int classes, int elem, long long bytes) {
     const long long fits = bytes / ((long long)rows * elem) / 256 * 256, all = (classes + 255ll) / 256 * 256;
@@ -48,21 +48,34 @@ static unsigned flat_grid(long long total) {
     return (unsigned)(blocks < VOCAB_GRID ? blocks : VOCAB_GRID);
 }
 
+// A row of logits takes a workgroup of 1024 threads where there are few (f32, 567 x 29440, us with 256 and 1024: the state 78 / 19, d 54 / 24), each with eight values in flight
+constexpr int VOCAB_AT_ONCE = 8;
+static int vocab_threads(int rows) { return rows <= 4 * (device_cu_count() > 0 ? device_cu_count() : 256) ? 1024 : 256; }
+
 // The piece's share of each row's running largest logit, sum and target's logit: state [rows][3]
-template <typename A>
-__global__ void __launch_bounds__(256) vocab_state_kernel(A* state, const A* z, const int* targets, int rows, int width, int v0, int first) {
-    __shared__ A room[8];
+template <typename A, int THREADS>
+__global__ void __launch_bounds__(THREADS) vocab_state_kernel(A* state, const A* z, const int* targets, int rows, int width, int v0, int first) {
+    __shared__ A room[2 * (THREADS / 64)];
     for (int row = blockIdx.x; row < rows; row += gridDim.x) {
         const A* zr = z + (long long)row * width;
         A* st = state + 3ll * row;
-        A top = first ? -(A)INFINITY : st[0];
-        const A was = top;
-        for (int c = threadIdx.x; c < width; c += 256) top = larger(top, zr[c]);
-        top = team_max<256>(top, room);
-        const A base = top == -(A)INFINITY ? (A)0 : top;
-        A sum[1] = {};
-        for (int c = threadIdx.x; c < width; c += 256) sum[0] += natural_exp(zr[c] - base);
-        team_sums<256>(sum, room + 4);
+        const A was = first ? -(A)INFINITY : st[0];
+        A own = -(A)INFINITY, own_sum = 0;
+        for (int c0 = threadIdx.x; c0 < width; c0 += THREADS * VOCAB_AT_ONCE) {
+            A v[VOCAB_AT_ONCE], most = own;
+#pragma unroll
+            for (int u = 0; u < VOCAB_AT_ONCE; u++) v[u] = c0 + u * THREADS < width ? zr[c0 + u * THREADS] : -(A)INFINITY;
+#pragma unroll
+            for (int u = 0; u < VOCAB_AT_ONCE; u++) most = larger(most, v[u]);
+            const A base = most == -(A)INFINITY ? (A)0 : most;
+            own_sum *= natural_exp(own - base);
+#pragma unroll
+            for (int u = 0; u < VOCAB_AT_ONCE; u++) own_sum += natural_exp(v[u] - base);
+            own = most;
+        }
+        const A top = team_max<THREADS>(larger(own, was), room), base = top == -(A)INFINITY ? (A)0 : top;
+        A sum[1] = {own_sum * natural_exp(own - base)};
+        team_sums<THREADS>(sum, room + THREADS / 64);
         if (threadIdx.x == 0) {
             st[1] = (first || was == -(A)INFINITY ? (A)0 : st[1] * natural_exp(was - base)) + sum[0];
             st[0] = top;
@@ -105,14 +118,23 @@ template <typename A> __device__ __forceinline__ A vocab_factor(const A* stats, 
     return f;
 }
 // z of a piece becomes d
-template <typename A>
-__global__ void __launch_bounds__(256) vocab_d_kernel(A* z, const A* stats, const A* upstream, const int* targets, int rows, int width, int v0, int classes, int reduction) {
+template <typename A, int THREADS>
+__global__ void __launch_bounds__(THREADS) vocab_d_kernel(A* z, const A* stats, const A* upstream, const int* targets, int rows, int width, int v0, int classes, int reduction) {
     for (int row = blockIdx.x; row < rows; row += gridDim.x) {
         const A f = vocab_factor(stats, upstream, targets, row, rows, classes, reduction), lse = stats[row];
         const bool held = targets[row] >= 0 && targets[row] < classes;
         const int t = held ? targets[row] - v0 : -1;
         A* zr = z + (long long)row * width;
-        for (int c = threadIdx.x; c < width; c += 256) zr[c] = held ? (natural_exp(zr[c] - lse) - (c == t ? (A)1 : (A)0)) * f : (A)0;
+        for (int c0 = threadIdx.x; c0 < width; c0 += THREADS * VOCAB_AT_ONCE) {
+            A v[VOCAB_AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < VOCAB_AT_ONCE; u++) v[u] = c0 + u * THREADS < width ? zr[c0 + u * THREADS] : (A)0;
+#pragma unroll
+            for (int u = 0; u < VOCAB_AT_ONCE; u++) {
+                const int c = c0 + u * THREADS;
+                if (c < width) zr[c] = held ? (natural_exp(v[u] - lse) - (c == t ? (A)1 : (A)0)) * f : (A)0;
+            }
+        }
     }
 }
 
@@ -207,7 +229,9 @@ static int vocab_any_forward(void* stats, const VocabArgs& g, void* workspace) {
     VocabRoom room(workspace);
     const VocabAnyRoom<T> r(room, g.rows, g.k, g.classes, false);
     const int rc = vocab_pieces<T>(g, r, VocabProduct{r.gemm, traits<A>::code}, [&](int v0, int width, A* z, const A*, long long, long long, const A*, long long, long long) {
-        hipLaunchKernelGGL((vocab_state_kernel<A>), dim3(g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID), dim3(256), 0, current_stream(), r.state, (const A*)z, g.targets, g.rows, width, v0, v0 == 0);
+        const int blocks = g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID;
+        if (vocab_threads(g.rows) == 1024) hipLaunchKernelGGL((vocab_state_kernel<A, 1024>), dim3(blocks), dim3(1024), 0, current_stream(), r.state, (const A*)z, g.targets, g.rows, width, v0, v0 == 0);
+        else hipLaunchKernelGGL((vocab_state_kernel<A, 256>), dim3(blocks), dim3(256), 0, current_stream(), r.state, (const A*)z, g.targets, g.rows, width, v0, v0 == 0);
         return check_launch("vocab_state_kernel") ? 0 : -1;
     });
     if (rc != 0) return -1;
@@ -227,7 +251,9 @@ static int vocab_any_backward(const VocabGrads& o, const VocabArgs& g, const voi
         return check_launch("vocab_round_kernel") ? 0 : -1;
     };
     const int rc = vocab_pieces<T>(g, r, product, [&](int v0, int width, A* z, const A* x, long long x_rs, long long x_cs, const A* w, long long w_rs, long long w_cs) {
-        hipLaunchKernelGGL((vocab_d_kernel<A>), dim3(g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID), dim3(256), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
+        const int blocks = g.rows < VOCAB_GRID ? g.rows : VOCAB_GRID;
+        if (vocab_threads(g.rows) == 1024) hipLaunchKernelGGL((vocab_d_kernel<A, 1024>), dim3(blocks), dim3(1024), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
+        else hipLaunchKernelGGL((vocab_d_kernel<A, 256>), dim3(blocks), dim3(256), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
         if (!check_launch("vocab_d_kernel")) return -1;
         if (o.dx && product(WIDE ? (void*)r.dx : o.dx, z, w, nullptr, g.rows, width, g.k, width, 1, w_cs, w_rs, WIDE ? g.k : o.dx_rs, v0 ? 1 : WIDE ? 0 : o.accumulate_dx) != 0) return -1;
         if (o.dw) {
