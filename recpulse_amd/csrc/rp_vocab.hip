@@ -144,14 +144,15 @@ template <typename T> struct VocabAnyRoom {
     using A = typename traits<T>::acc;
     static constexpr bool WIDE = sizeof(T) != sizeof(A);          // operands that are widened first
     int piece;
-    A *state, *z, *x, *w, *bias, *dx, *dw, *db;
+    A *state, *z, *x, *w, *bias, *dx, *dw, *db, *parts;
     char* gemm;
     VocabAnyRoom(VocabRoom& room, int rows, int k, int classes, bool backward) {
         piece = vocab_piece(rows, rows <= VOCAB_FEW_ROWS && classes > VOCAB_FEW_PIECE ? VOCAB_FEW_PIECE : classes, sizeof(A), VOCAB_PIECE_BYTES);
         state = room.take<A>(3ll * rows);
         z = room.take<A>((long long)rows * piece);
         gemm = room.take<char>(VOCAB_GEMM_BYTES);
-        x = w = bias = dx = dw = db = nullptr;
+        x = w = bias = dx = dw = db = parts = nullptr;
+        if (backward) parts = room.take<A>((long long)VOCAB_GEMM_BYTES / sizeof(A));
         if (!WIDE) return;
         x = room.take<A>((long long)rows * k);
         w = room.take<A>((long long)k * piece);
@@ -179,6 +180,19 @@ struct VocabProduct {
         return rc;
     }
 };
+
+// dx of float32 on few tiles: the classes of a piece in shares, as a batch of products that fills the CUs with tiles of 128, added up by a second launch (567 rows, 29440 classes, 1064 columns: 515 us in one
+// product, 392 so.  Both passes: 567, 1064 -> 74105 3493 / 3130, 300, 1024 -> 32000 939 / 753, 1000, 512 -> 10000 420 / 413; fewer columns: 600, 256 -> 100000 1510 / 1626, 200, 256 -> 4000 53.5 / 58.9)
+static int vocab_dx_shares(int rows, int k, int width, int elem) {
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+    const long long tiles = (long long)((rows + 127) / 128) * ((k + 127) / 128);
+    if (elem != 4 || rows < 128 || k < 512 || 2 * tiles > cus || path_disabled("vocab_shares")) return 1;
+    long long count = cus / tiles;
+    if (count > width / 1024) count = width / 1024;
+    const long long fits = (long long)(VOCAB_GEMM_BYTES / 4) / ((long long)rows * k);
+    if (count > fits) count = fits;
+    return count > 8 ? 8 : count < 1 ? 1 : (int)count;
+}
 
 // piece by piece: f(first class, classes, logits with unit column stride and rows as long as the piece)
 template <typename T, typename F>
@@ -255,7 +269,21 @@ static int vocab_any_backward(const VocabGrads& o, const VocabArgs& g, const voi
         if (vocab_threads(g.rows) == 1024) hipLaunchKernelGGL((vocab_d_kernel<A, 1024>), dim3(blocks), dim3(1024), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
         else hipLaunchKernelGGL((vocab_d_kernel<A, 256>), dim3(blocks), dim3(256), 0, current_stream(), z, (const A*)stats, (const A*)upstream, g.targets, g.rows, width, v0, g.classes, g.reduction);
         if (!check_launch("vocab_d_kernel")) return -1;
-        if (o.dx && product(WIDE ? (void*)r.dx : o.dx, z, w, nullptr, g.rows, width, g.k, width, 1, w_cs, w_rs, WIDE ? g.k : o.dx_rs, v0 ? 1 : WIDE ? 0 : o.accumulate_dx) != 0) return -1;
+        if (o.dx) {
+            void* dx = WIDE ? (void*)r.dx : o.dx;
+            const long long dx_rs = WIDE ? g.k : o.dx_rs;
+            const int accumulate = v0 ? 1 : WIDE ? 0 : o.accumulate_dx, shares = dx_rs == g.k ? vocab_dx_shares(g.rows, g.k, width, sizeof(A)) : 1, share = width / shares / 64 * 64, rest = width - shares * share;
+            bool done = false;
+            if (shares > 1) {
+                const GemmWorkspaceLoan loan(r.gemm, VOCAB_GEMM_BYTES);
+                const int rc = rp_hip_gemm_strided_batched(r.parts, z, w, nullptr, shares, g.rows, share, g.k, share, width, 1, share * w_cs, w_cs, w_rs, (long long)g.rows * g.k, g.k, 1, 0, traits<A>::code);
+                if (rc != 0 && !loan.refused) return -1;
+                done = rc == 0;
+            }
+            if (done && rest && product(r.parts, z + (long long)shares * share, w + shares * share * w_cs, nullptr, g.rows, rest, g.k, width, 1, w_cs, w_rs, g.k, 1) != 0) return -1;
+            if (done ? rp_hip_reduce_rows(dx, r.parts, shares, g.rows * g.k, accumulate, traits<A>::code) != 0
+                     : product(dx, z, w, nullptr, g.rows, width, g.k, width, 1, w_cs, w_rs, dx_rs, accumulate) != 0) return -1;
+        }
         if (o.dw) {
             char* dw = (char*)o.dw + v0 * o.dw_cs * (long long)sizeof(T);
             if (WIDE) {

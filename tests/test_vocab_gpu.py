@@ -336,3 +336,28 @@ def test_upstream_gradients_that_are_not_ordinary_numbers(upstream, rows, k, cla
             assert np.all(np.abs(db.read()) <= abs(upstream) * rows)
         else:
             assert not np.any(np.isfinite(got[targets >= 0])) and not np.any(np.isfinite(db.read()))
+
+
+@pytest.mark.parametrize("tied", [False, True], ids=["rows", "transposed"])
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("rows,k,classes", [(300, 200, 9001), (130, 520, 4160), (128, 128, 2048)])
+def test_dense_gradients_of_few_tiles_in_float32(rows, k, classes, accumulate, tied):
+    """The classes in shares, with some left over; the shares' sums are added up in float32."""
+    rng, x, w, _, targets = problem(rows, k, classes, F32, 21, tied, bias=False)
+    space = room(capi.lib().rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, F32))
+    _, stats = forward(x, w, None, targets, F32, 1, space)
+    _, _, d, f, p = vocab_reference(x.values, w.values, None, targets, 1, 1.0)
+    z_off, lse_off = offs(x, w, None, F32)
+    start = rng.normal(size=(rows, k)) * np.abs(f).max() if accumulate else None
+    dx = Output(rows, k, F32, start=start)
+    capi.check(capi.lib().rp_hip_linear_cross_entropy_backward(dx.ptr, None, None, x.ptr, w.ptr, None, ints(targets).ptr, stats.ptr, None, space.ptr, rows, k, classes, 1,
+                                                               x.rs, 1, w.rs, w.cs, k, 0, 1, accumulate, 0, 0, F32), "backward")
+    u = UNIT[F32]
+    d_off = np.abs(f)[:, None] * (p * 1.1 * (z_off + lse_off[:, None] + 16 * u * (1 + np.abs(np.log(p)))) + 4 * u * p) + 4 * u * np.abs(d)
+    wide, want = np.abs(d) + d_off, d @ w.values.T
+    off = d_off @ np.abs(w.values).T + ((classes + 8) * u + 2.0 ** -22) * (wide @ np.abs(w.values).T)      # (in any order; 2^-22 where the products are split into halves)
+    bound = rounded(off, want, F32)
+    if accumulate:
+        want = want + dx.values
+        bound = bound + HALF[F32] * (np.abs(want) + np.abs(dx.values) + bound)
+    assert_within(dx.read(), want, bound, "dx")
