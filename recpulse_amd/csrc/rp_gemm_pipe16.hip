@@ -29,6 +29,7 @@ namespace rp {
 constexpr int P16_BM = 128, P16_BN = 128, P16_MAXK = 64;
 constexpr int P16_ROW_BYTES = 128;                                   // one LDS row: 64 16-bit values
 constexpr int P16_TILE_BYTES = (P16_BM + P16_BN) * P16_ROW_BYTES;    // 32 KB: A rows, then B rows
+constexpr long long P16_REACH = 1ll << 30;                            // bytes that an offset from a descriptor's base stays below
 constexpr int P16_NBUF = 3;                                          // LDS tiles in rotation
 
 typedef __attribute__((address_space(3))) void* p16_lds_t;
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(512) gemm_pipe16_kernel(GemmArgs g, int tiles_
     const uint32_t st_write = (uint32_t)(r * P16_ROW_BYTES + 8 * h), st_swz = (uint32_t)((r >> 1) & 7);
     const int rr = lane >> 3, rp = lane & 7;
     const uint32_t c_lane = (uint32_t)(((long long)rr * g.c_rs + 8 * rp) * 2);
-    const long long c_span = ((long long)(g.m - 1) * g.c_rs + g.n) * 2;
+    const uint32_t c_step = (uint32_t)(16 * g.c_rs);      // bytes from a row to the eighth behind it
 
     f32x16_t acc[2][2];                 // [jm: rows of C][in: columns of C]
     u32x2_t packed[16];                 // the previous tile, narrowed: [jm][in][q]
@@ -218,14 +219,16 @@ __global__ void __launch_bounds__(512) gemm_pipe16_kernel(GemmArgs g, int tiles_
                 rows[e][d] = p16_ops<T>::pack(widen_lo(rows[e][d]) + widen_lo(bias_prev[d]), widen_hi(rows[e][d]) + widen_hi(bias_prev[d]));
         }
     };
-    // ... and to memory
-    auto row_store = [&](auto e_c, const TileOrigin& t, const __amdgpu_buffer_rsrc_t& rc) {
+    // ... and to memory, from the patch's first element on
+    auto patch_of = [&](const TileOrigin& t) { return (unsigned char*)g.C + ((long long)t.z * g.c_bs + (long long)(t.m0 + wm0) * g.c_rs + t.n0 + wn0) * 2; };
+    auto row_store = [&](auto e_c, const TileOrigin& t, unsigned char* c) {
         constexpr int e = decltype(e_c)::value;
         const int gm = t.m0 + wm0 + 8 * e, gn = t.n0 + wn0;
-        const int soff = (int)(((long long)gm * g.c_rs + gn) * 2);
+        // (the row's place is in the descriptor's base and not in a scalar offset: behind a 16-byte store with such an offset the compiler lets the next instruction write the data's registers;
+        // 64 products 576 x 64 x 3136 in bf16 49 us either way, 51.4 with the place added to the lane's offset)
         uint32_t voff = c_lane;
         if constexpr (EDGE) voff = (gm + rr < g.m && gn + 8 * rp < g.n) ? c_lane : BUFFER_OOB;      // (n is a multiple of 8: a piece is inside or outside as a whole)
-        __builtin_amdgcn_raw_buffer_store_b128(rows[e], rc, (int)voff, soff, 2);          // (streaming store: the output is not read again by this kernel)
+        __builtin_amdgcn_raw_buffer_store_b128(rows[e], buffer_rsrc(c + (uint32_t)e * c_step, P16_REACH), (int)voff, 0, 2);      // (streaming store: the output is not read again by this kernel)
     };
 
     auto read_frags = [&](const unsigned char* base, auto s_c) {
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(512) gemm_pipe16_kernel(GemmArgs g, int tiles_
         constexpr int NM = 4 * KST, Q = NM / 4;                    // MFMAs per tile and per quarter
         constexpr int WR = 8 / Q, RD = 4 / Q;                       // staging writes and row reads / stores per MFMA in their quarters
         const unsigned char* next_base = p16_smem + next * P16_TILE_BYTES;
-        const __amdgpu_buffer_rsrc_t rc = buffer_rsrc((uint16_t*)g.C + (long long)prev.z * g.c_bs, c_span);
+        unsigned char* const c = patch_of(prev);
         __syncthreads();                                   // the next tile is in LDS; this tile's pieces have all arrived in registers
         static_for<0, KST>([&](auto sc) {
             constexpr int s = decltype(sc)::value;
@@ -271,10 +274,10 @@ __global__ void __launch_bounds__(512) gemm_pipe16_kernel(GemmArgs g, int tiles_
                         static_for<0, RD>([&](auto ec) { row_read(std::integral_constant<int, idx * RD + decltype(ec)::value>{}); });
                     }
                     if constexpr (phase == 2) {
-                        static_for<0, RD>([&](auto ec) { row_store(std::integral_constant<int, idx * RD + decltype(ec)::value>{}, prev, rc); });
+                        static_for<0, RD>([&](auto ec) { row_store(std::integral_constant<int, idx * RD + decltype(ec)::value>{}, prev, c); });
                         static_for<0, RD>([&](auto ec) { row_read(std::integral_constant<int, 4 + idx * RD + decltype(ec)::value>{}); });
                     }
-                    if constexpr (phase == 3) static_for<0, RD>([&](auto ec) { row_store(std::integral_constant<int, 4 + idx * RD + decltype(ec)::value>{}, prev, rc); });
+                    if constexpr (phase == 3) static_for<0, RD>([&](auto ec) { row_store(std::integral_constant<int, 4 + idx * RD + decltype(ec)::value>{}, prev, c); });
                     __builtin_amdgcn_sched_barrier(0);
                 }
             });
@@ -303,10 +306,10 @@ __global__ void __launch_bounds__(512) gemm_pipe16_kernel(GemmArgs g, int tiles_
         next = next + 1 == P16_NBUF ? 0 : next + 1;
     }
     // the last tile
-    const __amdgpu_buffer_rsrc_t rc = buffer_rsrc((uint16_t*)g.C + (long long)prev.z * g.c_bs, c_span);
+    unsigned char* const c = patch_of(prev);
     static_for<0, 16>([&](auto nc) { stage_write(nc); });
     static_for<0, 8>([&](auto ec) { row_read(ec); });
-    static_for<0, 8>([&](auto ec) { row_store(ec, prev, rc); });
+    static_for<0, 8>([&](auto ec) { row_store(ec, prev, c); });
 }
 
 // ---- host side ----
@@ -325,7 +328,7 @@ bool pipe16_takes(const GemmArgs& g) {
     if (!(a_kc || a_mc) || !(b_kc || b_mc) || g.a_bs % 8 || g.b_bs % 8 || g.a_rs < 0 || g.a_cs < 0 || g.b_rs < 0 || g.b_cs < 0) return false;
     if (g.c_cs != 1 || g.c_rs % 8 || g.c_bs % 8 || g.c_rs < 0) return false;
     if (((uintptr_t)g.A & 15) || ((uintptr_t)g.B & 15) || ((uintptr_t)g.C & 15)) return false;
-    const long long lim = 1ll << 30;
+    const long long lim = P16_REACH;
     // free indices up to a whole tile past the last one are addressed (and read as zero, or as values that only reach
     // outputs which are not stored)
     const long long a_reach = (a_kc ? (long long)(g.m + P16_BM) * g.a_rs + P16_MAXK : (long long)P16_MAXK * g.a_cs + g.m + P16_BM) * 2;

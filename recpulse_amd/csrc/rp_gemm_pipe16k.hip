@@ -268,10 +268,10 @@ __global__ void __launch_bounds__(512) gemm_pipe16k_kernel(GemmArgs g, int tiles
     auto row_store = [&](auto e_c, int pm0, const __amdgpu_buffer_rsrc_t& rc) {
         constexpr int e = decltype(e_c)::value;
         const int gm = pm0 + 32 * wave + 8 * e;
-        const int soff = (int)((long long)gm * g.c_rs * 2);
-        uint32_t voff = c_lane;
-        if constexpr (EDGE) voff = (gm + rr < g.m && 8 * rp < g.n) ? c_lane : BUFFER_OOB;      // (n is a multiple of 8: a piece is inside or outside as a whole)
-        __builtin_amdgcn_raw_buffer_store_b128(rows[e], rc, (int)voff, soff, 2);          // (streaming store: the output is not read again by this kernel)
+        // (the whole offset in a vector register: behind a 16-byte store with part of it in a scalar one the compiler lets the next instruction write the data's registers)
+        uint32_t voff = c_lane + (uint32_t)((long long)gm * g.c_rs * 2);
+        if constexpr (EDGE) voff = (gm + rr < g.m && 8 * rp < g.n) ? voff : BUFFER_OOB;        // (n is a multiple of 8: a piece is inside or outside as a whole)
+        __builtin_amdgcn_raw_buffer_store_b128(rows[e], rc, (int)voff, 0, 2);             // (streaming store: the output is not read again by this kernel)
     };
 
     // EPI: request the rows of C that tile (pm0, rc) will be added to; add them to the finished rows
