@@ -490,8 +490,11 @@ int rp_hip_gated_linear_backward(void* dx, void* dw, void* db, void* dz, const v
  * The logits are made in pieces of the vocabulary and not kept.  targets: device int32 [rows]; a row whose target lies outside [0, classes) is left out: its loss and gradient are zeros
  * (dw still adds zeros times its x, which has to be finite there).
  * reduction 0: loss_out [rows]; 1: the mean over the rows with a target (0 where there are none); 2: their sum; loss_out in the accumulate type.  stats: 2 rows + 1 values of the accumulate type, for the
- * backward pass: log sum exp of each row, its loss, and how many rows have a target. */
+ * backward pass: log sum exp of each row, its loss, and how many rows have a target.
+ * The workspace does for operands however they lie: 16-bit ones without a unit stride are widened a piece at a time, of up to 128 MiB of w and as much again of dw.  The _strided one is for operands
+ * that lie as it is told, for both passes on them: of 64 rows before 32768 classes, k = 4096 in 16 bits, less than 1 MiB forward where they have unit strides. */
 long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, int backward, int dtype);
+long long rp_hip_linear_cross_entropy_workspace_strided(int rows, int k, int classes, int backward, long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype);
 int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,
                                         long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype);
 /* Its gradients times upstream_dev, accumulate type on the device ([rows] for reduction 0, one element otherwise; NULL: 1): dx [rows, k] with unit column stride, dw [k, classes] with unit stride along

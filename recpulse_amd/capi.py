@@ -115,6 +115,7 @@ SIGNATURES = {
     "rp_hip_gated_linear_forward": (_i, [_vp] * 5 + [_i] * 4 + [_ll] * 5 + [_i]),
     "rp_hip_gated_linear_backward": (_i, [_vp] * 8 + [_i] * 4 + [_ll] * 8 + [_i] * 4),
     "rp_hip_linear_cross_entropy_workspace": (_ll, [_i] * 5),
+    "rp_hip_linear_cross_entropy_workspace_strided": (_ll, [_i] * 4 + [_ll] * 4 + [_i]),
     "rp_hip_linear_cross_entropy_forward": (_i, [_vp] * 7 + [_i] * 4 + [_ll] * 4 + [_i]),
     "rp_hip_linear_cross_entropy_backward": (_i, [_vp] * 10 + [_i] * 4 + [_ll] * 7 + [_i] * 4),
     "rp_hip_distillation_forward": (_i, [_vp] * 7 + [_i] * 3 + [_ll, _d, _i, _i]),

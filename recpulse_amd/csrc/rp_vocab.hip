@@ -10,6 +10,10 @@
 namespace rp {
 
 constexpr long long VOCAB_PIECE_BYTES = 64ll << 20;      // of a piece's logits
+// ... and of a piece of W that is widened first, and of its dW (bf16, w with a column stride of 2, us forward / backward with 64, 128 and 256 MiB and with one piece of all classes: 64 rows, 4096 -> 32768
+// 613 / 1390, 602 / 1342, 574 / 1310, 625 / 1348; 512, 2048 -> 32000 760 / 1890, 544 / 1627, 565 / 1650, 564 / 1645; 8, 4096 -> 131072 2608 / 4918, 2200 / 4507, 2067 / 4325, 2016 / 4755, which take 160,
+// 289, 545 and 2083 MiB)
+constexpr long long VOCAB_WIDE_BYTES = 128ll << 20;
 constexpr size_t VOCAB_GEMM_BYTES = 16 << 20;            // for the partial sums of its products
 // Few rows: dx of a piece is split along its classes, 2048 a share, and 32 shares of 8 rows and 16384 float32 fill that memory
 constexpr int VOCAB_FEW_ROWS = 8, VOCAB_FEW_PIECE = 65536;
@@ -148,6 +152,7 @@ template <typename T> struct VocabAnyRoom {
     char* gemm;
     VocabAnyRoom(VocabRoom& room, int rows, int k, int classes, bool backward) {
         piece = vocab_piece(rows, rows <= VOCAB_FEW_ROWS && classes > VOCAB_FEW_PIECE ? VOCAB_FEW_PIECE : classes, sizeof(A), VOCAB_PIECE_BYTES);
+        if (WIDE) piece = vocab_piece(k, piece, sizeof(A), VOCAB_WIDE_BYTES);      // (of few rows the widened W is by far the larger)
         state = room.take<A>(3ll * rows);
         z = room.take<A>((long long)rows * piece);
         gemm = room.take<char>(VOCAB_GEMM_BYTES);
@@ -302,6 +307,12 @@ static int vocab_any_backward(const VocabGrads& o, const VocabArgs& g, const voi
     return WIDE && o.dx ? rounded(o.dx, r.dx, g.rows, g.k, o.dx_rs, 1, o.accumulate_dx) : 0;
 }
 
+static long long vocab_any_room(int rows, int k, int classes, bool backward, int dtype) {
+    VocabRoom room(nullptr);
+    RP_DISPATCH_DTYPE(dtype, const VocabAnyRoom<T> r(room, rows, k, classes, backward); (void)r);
+    return room.used();
+}
+
 static bool vocab_args_ok(const char* who, bool pointers, int rows, int k, int classes, int reduction, std::initializer_list<long long> strides, int dtype) {
     if (!pointers || rows <= 0 || k <= 0 || classes <= 0 || rows > (1 << 29) || classes > (1 << 29)) {
         set_error("%s: null operand, non-positive extent, more than 2^29 rows or classes (rows=%d k=%d classes=%d)", who, rows, k, classes);
@@ -322,10 +333,15 @@ extern "C" {
 
 long long rp_hip_linear_cross_entropy_workspace(int rows, int k, int classes, int backward, int dtype) {
     if (!vocab_args_ok("rp_hip_linear_cross_entropy_workspace", true, rows, k, classes, 0, {}, dtype)) return -1;
-    VocabRoom room(nullptr);
-    RP_DISPATCH_DTYPE(dtype, const VocabAnyRoom<T> r(room, rows, k, classes, backward != 0); (void)r);
-    const long long tiles = dtype_size(dtype) == 2 ? vocab16_room(rows, k, classes, backward != 0) : 0;
-    return tiles > room.used() ? tiles : room.used();         // (how the operands lie is not known here: room for either way)
+    const long long tiles = dtype_size(dtype) == 2 ? vocab16_room(rows, k, classes, backward != 0) : 0, any = vocab_any_room(rows, k, classes, backward != 0, dtype);
+    return tiles > any ? tiles : any;                         // (how the operands lie is not known here: room for either way)
+}
+
+long long rp_hip_linear_cross_entropy_workspace_strided(int rows, int k, int classes, int backward, long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype) {
+    if (!vocab_args_ok("rp_hip_linear_cross_entropy_workspace_strided", true, rows, k, classes, 0, {x_rs, x_cs, w_rs, w_cs}, dtype)) return -1;
+    // (where they start decides nothing but the tiles' kind)
+    const bool tiles = vocab16_takes(VocabArgs{nullptr, nullptr, nullptr, nullptr, rows, k, classes, 0, x_rs, x_cs, w_rs, w_cs}, dtype);
+    return tiles ? vocab16_room(rows, k, classes, backward != 0) : vocab_any_room(rows, k, classes, backward != 0, dtype);
 }
 
 int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,

@@ -1271,7 +1271,7 @@ void backward_linear_cross_entropy_fn(GradFn* self, Tensor* grad_output) {
     GradSlot slots[3] = {grad_slot(x), grad_slot(w), grad_slot(bias)};
     slots_apart(targets, slots, 3);
     void* room = nullptr;
-    const bool ok = on_device(x->device_id) && rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace(rows, k, classes, 1, x->dtype)) == 0 &&
+    const bool ok = on_device(x->device_id) && rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace_strided(rows, k, classes, 1, x->strides[0], x->strides[1], w->strides[0], w->strides[1], x->dtype)) == 0 &&
                     rp_hip_linear_cross_entropy_backward(slot_data(slots[0]), slot_data(slots[1]), slot_data(slots[2]), x->data, w->data, bias ? bias->data : nullptr, (const int*)s->plan, s->kept, up->data, room,
                                                          rows, k, classes, s->reduction, x->strides[0], x->strides[1], w->strides[0], w->strides[1], k, classes, 1,
                                                          slots[0].accumulate, slots[1].accumulate, slots[2].accumulate, x->dtype) == 0;
@@ -2178,7 +2178,7 @@ Tensor* op_linear_cross_entropy(Tensor* x, Tensor* w, Tensor* bias, const int* t
     LanguageSaved* s = new_language_saved(x->device_id, reduction);
     void* room = nullptr;
     const bool ok = out && on_device(x->device_id) && rp_hip_malloc(&s->kept, dtype_size(acc) * (2 * (size_t)rows + 1)) == 0 && upload_ints(&s->plan, targets, rows) &&
-                    rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace(rows, k, classes, 0, x->dtype)) == 0 &&
+                    rp_hip_malloc(&room, (size_t)rp_hip_linear_cross_entropy_workspace_strided(rows, k, classes, 0, x->strides[0], x->strides[1], w->strides[0], w->strides[1], x->dtype)) == 0 &&
                     rp_hip_linear_cross_entropy_forward(out->data, s->kept, x->data, w->data, bias ? bias->data : nullptr, (const int*)s->plan, room, rows, k, classes, reduction,
                                                         x->strides[0], x->strides[1], w->strides[0], w->strides[1], x->dtype) == 0;
     if (room) rp_hip_free(room);
