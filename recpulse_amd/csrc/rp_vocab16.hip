@@ -45,7 +45,9 @@ static int launch_grads(const VocabTileArgs& a, VocabStep step, bool b_mc, const
 static int patch_columns(int edge) { return edge == 256 ? 128 : 64; }
 static int patch_rows(int edge) { return edge / 2; }
 
+// (d has as many columns as W, and is an operand of unaligned tiles too: fewer classes than a vector go the other way however W lies)
 static int logits_lie(const VocabArgs& g) {
+    if (g.classes < 8) return LIES_NEITHER;
     return worse16(lies16(g.x, g.x_rs, g.k), g.w_cs == 1 ? lies16(g.w, g.w_rs, g.classes) : lies16(g.w, g.w_cs, g.k));
 }
 bool vocab16_takes(const VocabArgs& g, int dtype) {

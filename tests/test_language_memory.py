@@ -44,6 +44,15 @@ def test_no_way_to_lie_takes_more_than_the_question_without_strides_says(dtype):
                 assert 0 < strided(rows, k, classes, backward, strides, dtype) <= workspace(rows, k, classes, backward, dtype)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+def test_fewer_classes_than_a_vector_go_one_way_however_the_weight_lies(dtype):
+    """The tiles' unaligned loads of the logits' gradient would begin before it: the kernels for any strides take these, and ask for the same memory either way."""
+    for rows, k in ((20, 64), (300, 72), (1, 4096)):
+        for classes in range(1, 8):
+            for backward in (0, 1):
+                assert strided(rows, k, classes, backward, (k, 1, 1, k), dtype) == strided(rows, k, classes, backward, (k, 1, classes, 1), dtype)
+
+
 def test_refusals():
     lib = capi.lib()
     for args, why in (((0, 64, 100, 1, 64, 1, 100, 1, capi.BF16), "extent"), ((4, 64, 100, 1, 64, -1, 100, 1, capi.BF16), "negative stride"), ((4, 64, 100, 1, 64, 1, 100, 1, 9), "unsupported dtype")):
