@@ -18,7 +18,7 @@ template <typename A> struct DistillArgs {
     void* grad;
     const void *logits, *teacher, *upstream;
     const int* ids;
-    A* stats;                                      // [rows] log sum exp(s / T), [rows] log sum exp(t / T), [rows] losses
+    A* stats;                                      // [rows] largest logit, [rows] sum of exp((s - that) / T) or, without entries, -1, [rows] losses
     int rows, classes, k, reduction;
     long long logits_rs;
     A temperature;
@@ -30,9 +30,9 @@ template <typename A> __device__ __forceinline__ A row_factor(const DistillArgs<
     return f * g.temperature;
 }
 
-// The gradients of the entries' classes, over what the row's own pass left there: `v`, `value`: this thread's entry (-1: none) and its logit
+// The gradients of the entries' classes, over what the row's own pass left there.  `v`, `value`: this thread's entry (-1: none) and its logit; `p`: exp((t - largest t) / T) of all entries
 template <typename T, typename A>
-__device__ __forceinline__ void correct_entries(int k, T* grad, const int* ids, const A* p, int v, A value, const ScaledExp<A>& q, A factor) {
+__device__ __forceinline__ void correct_entries(int k, T* grad, const int* ids, const A* p, int v, A value, const ScaledExp<A>& weight, A share, A part, A factor) {
     if (v < 0) return;
     const int j = threadIdx.x;
     A mass = 0;
@@ -43,7 +43,7 @@ __device__ __forceinline__ void correct_entries(int k, T* grad, const int* ids, 
         mass += same ? p[i] : (A)0;
         before += same && i < j;
     }
-    if (!before) grad[v] = round_to<T>((q(value) - mass) * factor);
+    if (!before) grad[v] = round_to<T>((weight(value) * share - mass * part) * factor);
 }
 
 // Vectors a thread holds up to which two workgroups of 1024 share a CU, 64 registers a thread: one's loads and stores fly while the other adds up
@@ -57,13 +57,15 @@ constexpr bool distill_later(int threads, int steps, int elem) { return !(thread
 // A value that all lanes have, in scalar registers
 __device__ __forceinline__ float in_scalar(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ double in_scalar(double v) { return __hiloint2double(__builtin_amdgcn_readfirstlane(__double2hiint(v)), __builtin_amdgcn_readfirstlane(__double2loint(v))); }
+__device__ __forceinline__ float one_over(float v) { return __builtin_amdgcn_rcpf(v); }      // (off by one place)
+__device__ __forceinline__ double one_over(double v) { return 1.0 / v; }
 template <typename T> __device__ __forceinline__ void load_one(T& x, const __amdgpu_buffer_rsrc_t& from, int offset) {
     if constexpr (sizeof(T) == 2) { const uint16_t v = __builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0); __builtin_memcpy(&x, &v, 2); }
     else if constexpr (sizeof(T) == 4) { const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0); __builtin_memcpy(&x, &v, 4); }
     else { const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0); __builtin_memcpy(&x, &v, 8); }
 }
 
-// FORWARD: the row's sums and loss; with a gradient asked for, that too.  Otherwise the gradient from the sums that a forward call left.  STEPS 0: the row is read again for each.
+// FORWARD: the row's sums and loss; with a gradient asked for, that too.  Otherwise the gradient from the largest logit and sum that a forward call left.  STEPS 0: the row is read again for each.
 // A workgroup walks rows; the next row's loads are issued as soon as a row's registers are stored, and fly while its last steps wait for one another.  k <= THREADS: a thread has an entry or none.
 template <typename T, int THREADS, int STEPS, bool FORWARD>
 __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(T))) distill_kernel(DistillArgs<typename traits<T>::acc> g) {
@@ -102,13 +104,14 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
         load_entry(blockIdx.x);
     }
     // The entries of the row before are corrected once this row's loads have been waited for, before which its stores were issued, and all threads have met
-    A lse_before = 0, factor_before = 0;
+    A top_before = 0, share_before = 0, part_before = 0, factor_before = 0;
     bool some_before = false;
-    auto correct_before = [&](int row, int turn) {
-        if (!some_before) return;
+    auto correct_row = [&](T* grad, int turn, const ScaledExp<A>& weight, A share, A part, A factor) {
         const bool own = (int)threadIdx.x < g.k;
-        correct_entries<T>(g.k, (T*)g.grad + (long long)row * g.classes, entry_ids[turn], entry_p[turn], own ? entry_ids[turn][threadIdx.x] : -1, own ? entry_value[turn][threadIdx.x] : (A)0,
-                           ScaledExp<A>(scale, lse_before), factor_before);
+        correct_entries<T>(g.k, grad, entry_ids[turn], entry_p[turn], own ? entry_ids[turn][threadIdx.x] : -1, own ? entry_value[turn][threadIdx.x] : (A)0, weight, share, part, factor);
+    };
+    auto correct_before = [&](int row, int turn) {
+        if (some_before) correct_row((T*)g.grad + (long long)row * g.classes, turn, ScaledExp<A>(scale, top_before), share_before, part_before, factor_before);
     };
     constexpr bool LATER = FORWARD && distill_later(THREADS, STEPS, sizeof(T));
     int row = blockIdx.x, turn = 0;
@@ -116,16 +119,16 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
         const T* s = row_of(row);
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));              // (the masks of a row's end are made again for each row: kept, they would take more registers than there are)
-        // the entry: its class (-1: none), log p but for the sum, and the student's logit
+        // the entry: its class (-1: none), the teacher's logit and the student's
         A* p = entry_p[turn];
         int* ids = entry_ids[turn];
-        A log_p = id >= 0 && id < g.classes ? widen(entry) * scale : -(A)INFINITY;
-        int v = log_p == -(A)INFINITY ? -1 : id;
+        A goal = id >= 0 && id < g.classes ? widen(entry) : -(A)INFINITY;
+        int v = goal == -(A)INFINITY ? -1 : id;
         A value = v < 0 ? (A)0 : widen(s[v]);
         const T row_last = last;
         if (tid < g.k) {
             ids[tid] = v;
-            p[tid] = log_p;
+            p[tid] = goal;
             entry_value[turn][tid] = value;
         }
         if constexpr (STEPS > 0) {
@@ -157,9 +160,9 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 for (int c = tid; c < g.classes; c += THREADS) f(widen(s[c]));
             }
         };
-        A lse, log_mass;
+        A top = -(A)INFINITY, sum, part = 0;       // part: 1 over the entries' sum
+        bool some;                                 // an entry counts
         if constexpr (FORWARD) {
-            A top = -(A)INFINITY;
             bool again = false;
             if constexpr (STEPS > 0 && sizeof(T) == 2) {
                 // Two values at a time as whole numbers: of those that are not negative the largest number is the largest value (and +NaN above all).  Rows without one are looked through again.
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
             } else {
                 each([&](A x) { top = plain_max(top, x); });      // (NaN shows in the sum)
             }
-            A tops[2] = {top, log_p};
+            A tops[2] = {top, goal};
             if (LATER) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             team_tops_in_turn<THREADS>(tops, rooms[0][0]);
             if (LATER) correct_before(row - (int)gridDim.x, turn ^ 1);
@@ -199,34 +202,35 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                     top = one[0];
                 }
             }
-            const A base = in_scalar(top == -(A)INFINITY ? (A)0 : top * scale);
-            const ScaledExp<A> weight(scale, base);
-            A sums[2] = {(A)0, v < 0 ? (A)0 : natural_exp(log_p - tops[1])};
+            top = in_scalar(top);
+            const A goal_top = in_scalar(tops[1]);
+            const ScaledExp<A> weight(scale, top);
+            A sums[2] = {(A)0, v < 0 ? (A)0 : ScaledExp<A>(scale, goal_top)(goal)};
             each([&](A x) { sums[0] += weight(x); });
             team_sums_in_turn<THREADS>(sums, rooms[1][0]);
-            lse = in_scalar(base + natural_log(sums[0]));
-            log_mass = in_scalar(tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]));
-        } else {
-            lse = g.stats[row];
-            log_mass = g.stats[g.rows + row];
-        }
-        if (FORWARD) {                             // (two barriers ago)
+            sum = in_scalar(sums[0]);
+            const A goal_sum = in_scalar(sums[1]);
+            some = !(goal_top == -(A)INFINITY);
+            // (from LDS again, two barriers later)
             v = tid < g.k ? ids[tid] : -1;
-            log_p = tid < g.k ? p[tid] : -(A)INFINITY;
+            goal = tid < g.k ? p[tid] : -(A)INFINITY;
             value = tid < g.k ? entry_value[turn][tid] : (A)0;
-        }
-        const bool some = !(log_mass == -(A)INFINITY);
-        log_p -= log_mass;
-        const A own_p = v < 0 ? (A)0 : natural_exp(log_p);
-        if constexpr (FORWARD) {
-            A loss[1] = {own_p != 0 ? own_p * (log_p - scaled_less(value, scale, lse)) : (A)0};
+            const ScaledExp<A> goal_weight(scale, goal_top);
+            part = in_scalar(one_over(goal_sum));
+            const A own_weight = v < 0 ? (A)0 : goal_weight(goal), own_p = own_weight * part;
+            if (tid < g.k) p[tid] = own_weight;
+            A loss[1] = {own_p != 0 ? own_p * ((goal_weight.log(goal) - natural_log(goal_sum)) - (weight.log(value) - natural_log(sum))) : (A)0};
             if (g.k > 64) team_sums_in_turn<THREADS>(loss, rooms[2][0]);
             else loss[0] = wave_sum(loss[0]);          // (the first wave has all entries)
             if (tid == 0) {
-                g.stats[row] = lse;
-                g.stats[g.rows + row] = log_mass;
+                g.stats[row] = top;
+                g.stats[g.rows + row] = some ? sum : (A)-1;
                 g.stats[2 * (long long)g.rows + row] = some ? loss[0] * g.temperature * g.temperature : (A)0;
             }
+        } else {
+            top = g.stats[row];
+            sum = g.stats[g.rows + row];
+            some = !(sum < 0);
         }
         const __amdgpu_buffer_rsrc_t from = buffer_rsrc(row_of(row + gridDim.x), row_bytes);
         if (!g.grad) {
@@ -235,10 +239,9 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
             continue;                              // (two barriers lie between a room's readers and its next writers)
         }
         T* grad = (T*)g.grad + (long long)row * g.classes;
-        const A factor = in_scalar(row_factor(g, row));
-        const ScaledExp<A> q(scale, lse);
-        auto share = [&](A x) { return some ? q(x) * factor : (A)0; };
-        if (tid < g.k) p[tid] = own_p;
+        const ScaledExp<A> weight(scale, top);
+        const A factor = in_scalar(row_factor(g, row)), share = in_scalar(one_over(sum)), scaled = in_scalar(share * factor);
+        auto rest = [&](A x) { return some ? weight(x) * scaled : (A)0; };
         if constexpr (STEPS > 0) {
             const __amdgpu_buffer_rsrc_t to = buffer_rsrc(grad, row_bytes);
             static_for<0, STEPS>([&](auto ic) {
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 asm volatile("" : "+v"(raw[i]));
                 __builtin_memcpy(out, &raw[i], 16);
 #pragma unroll
-                for (int u = 0; u < N; u++) values[u] = q(widen(out[u])) * factor;
+                for (int u = 0; u < N; u++) values[u] = weight(widen(out[u])) * scaled;
                 if (some) round_vector<T>(out, values);
                 else __builtin_memset(out, 0, 16);           // (whatever the row's logits are)
                 u32x4_t o;
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 load_step(from, ic);
                 __builtin_amdgcn_sched_barrier(0);
             });
-            if (odd && tid == (g.classes - 1) / N % THREADS) grad[g.classes - 1] = round_to<T>(share(widen(row_last)));
+            if (odd && tid == (g.classes - 1) / N % THREADS) grad[g.classes - 1] = round_to<T>(rest(widen(row_last)));
         } else if (g.classes >= N) {
             for (int c = tid * N; c < g.classes; c += THREADS * N) {
                 const RowVector<T> at(c, g.classes);
@@ -267,23 +270,42 @@ __global__ void __launch_bounds__(THREADS, distill_waves(THREADS, STEPS, sizeof(
                 A values[N];
                 at.load(x, s);
 #pragma unroll
-                for (int u = 0; u < N; u++) values[u] = share(widen(x[u]));
+                for (int u = 0; u < N; u++) values[u] = rest(widen(x[u]));
                 round_vector<T>(x, values);
                 at.store(grad, x);
             }
         } else {
-            for (int c = tid; c < g.classes; c += THREADS) grad[c] = round_to<T>(share(widen(s[c])));
+            for (int c = tid; c < g.classes; c += THREADS) grad[c] = round_to<T>(rest(widen(s[c])));
         }
         load_entry(row + gridDim.x);
         if (LATER) {
-            lse_before = lse;
+            top_before = top;
+            share_before = share;
+            part_before = part;
             factor_before = factor;
             some_before = some;
             continue;
         }
+        if (!FORWARD && some) {                    // the entries' weights, while the stores fly, added up in the order of a forward call
+            goal = tid < g.k ? p[tid] : -(A)INFINITY;
+            A most = wave_max(goal);
+            if (g.k > 64) {
+                if ((tid & 63) == 0) rooms[0][0][tid / 64] = most;
+                __syncthreads();
+                for (int w = 0; w < (g.k + 63) / 64; w++) most = larger(most, rooms[0][0][w]);
+            }
+            const A own_weight = goal == -(A)INFINITY ? (A)0 : ScaledExp<A>(scale, in_scalar(most))(goal), all = wave_sum(own_weight);
+            if (tid < g.k) p[tid] = own_weight;
+            if ((tid & 63) == 0) rooms[1][0][tid / 64] = all;
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                           // the row's stores are done: the entries' classes come after
-        if (some) correct_entries<T>(g.k, grad, ids, p, v, value, q, factor);
+        if (!FORWARD && some) {
+            A all = rooms[1][0][0];                // (of few entries the first wave, which has them all, is the only one that this is for)
+            for (int w = 1; w < (g.k + 63) / 64; w++) all += rooms[1][0][w];
+            part = one_over(all);
+        }
+        if (some) correct_row(grad, turn, weight, share, part, factor);
     }
     if (LATER && g.grad) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -311,14 +333,16 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 8 : 4) distill_loss_r
         };
         load(0);
         int v = -1;
-        A log_p = -(A)INFINITY, value = 0;
+        A goal = -(A)INFINITY, value = 0;
         if (tid < g.k) {
             const int id = g.ids[(long long)row * g.k + tid];
-            if (id >= 0 && id < g.classes) log_p = widen(((const T*)g.teacher)[(long long)row * g.k + tid]) * scale;
-            if (!(log_p == -(A)INFINITY)) { v = id; value = widen(s[id]); }
+            if (id >= 0 && id < g.classes) goal = widen(((const T*)g.teacher)[(long long)row * g.k + tid]);
+            if (!(goal == -(A)INFINITY)) { v = id; value = widen(s[id]); }
         }
         A top = -(A)INFINITY, sum = 0;
-        if (odd && tid == 0) { top = widen(s[g.classes - 1]); sum = top == -(A)INFINITY ? (A)0 : top == top ? (A)1 : top; }      // (an odd last element of 16 bits goes by itself)
+        if (odd && tid == 0) top = widen(s[g.classes - 1]);      // (an odd last element of 16 bits goes by itself)
+        ScaledExp<A> weight(scale, top);
+        if (odd && tid == 0) sum = weight(top);
         for (int c0 = 0; c0 < g.classes; c0 += PIECE) {
             T x[U][N];
             __builtin_memcpy(x, next, sizeof(x));
@@ -334,30 +358,28 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 8 : 4) distill_loss_r
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int u = 0; u < N; u++) most = plain_max(most, widen(x[i][u]));
-            const A base = most == -(A)INFINITY ? (A)0 : most * scale;
-            const ScaledExp<A> weight(scale, base);
-            sum *= weight(top);
+            const ScaledExp<A> next_weight(scale, most);
+            sum *= top == -(A)INFINITY ? (A)0 : weight.as(next_weight);
+            weight = next_weight;
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
                 for (int u = 0; u < N; u++) sum += weight(widen(x[i][u]));
             top = most;
         }
-        A tops[2] = {top, log_p};
+        A tops[2] = {top, goal};
         team_tops_in_turn<THREADS>(tops, rooms[0][0]);
-        const A base = tops[0] == -(A)INFINITY ? (A)0 : tops[0] * scale;
-        A sums[2] = {sum * ScaledExp<A>(scale, base)(top), v < 0 ? (A)0 : natural_exp(log_p - tops[1])};
+        const ScaledExp<A> row_weight(scale, tops[0]), goal_weight(scale, tops[1]);
+        A sums[2] = {top == -(A)INFINITY ? sum * 0 : sum * weight.as(row_weight), v < 0 ? (A)0 : goal_weight(goal)};
         team_sums_in_turn<THREADS>(sums, rooms[1][0]);
-        const A lse = base + natural_log(sums[0]), log_mass = tops[1] == -(A)INFINITY ? tops[1] : tops[1] + natural_log(sums[1]);
-        const bool some = !(log_mass == -(A)INFINITY);
-        log_p -= log_mass;
-        const A own_p = v < 0 ? (A)0 : natural_exp(log_p);
-        A loss[1] = {own_p != 0 ? own_p * (log_p - scaled_less(value, scale, lse)) : (A)0};
+        const bool some = !(tops[1] == -(A)INFINITY);
+        const A own_p = v < 0 ? (A)0 : goal_weight(goal) * one_over(sums[1]);
+        A loss[1] = {own_p != 0 ? own_p * ((goal_weight.log(goal) - natural_log(sums[1])) - (row_weight.log(value) - natural_log(sums[0]))) : (A)0};
         if (g.k > 64) team_sums_in_turn<THREADS>(loss, rooms[2][0]);
         else loss[0] = wave_sum(loss[0]);
         if (tid == 0) {
-            g.stats[row] = lse;
-            g.stats[g.rows + row] = log_mass;
+            g.stats[row] = tops[0];
+            g.stats[g.rows + row] = some ? sums[0] : (A)-1;
             g.stats[2 * (long long)g.rows + row] = some ? loss[0] * g.temperature * g.temperature : (A)0;
         }
     }

@@ -142,23 +142,25 @@ __device__ __forceinline__ double natural_exp(double x) { return exp(x); }
 __device__ __forceinline__ float natural_log(float x) { return logf(x); }
 __device__ __forceinline__ double natural_log(double x) { return log(x); }
 
-// exp(x scale - base) for many x: in float32 as 2 to the (x scale') - base', one multiply-add and the hardware's exponential
+// exp((x - top) scale) for many x of a row, as 2 to x s - b with s = scale log2 e and b = top s: in float32 one multiply-add and the hardware's exponential.  s and b are rounded, but the same for
+// every x, and x s - b is rounded once: what two of them have in common, however far from zero the row lies, leaves their quotient, and `log`, which is of the same x s - b, a difference from another's.
 template <typename A> struct ScaledExp;
 template <> struct ScaledExp<float> {
     float scale, base;
-    __device__ __forceinline__ ScaledExp(float s, float b) : scale(s * 1.44269504088896341f), base(b * 1.44269504088896341f) {}
+    __device__ __forceinline__ ScaledExp(float s, float top) : scale(s * 1.44269504088896341f), base(top == -INFINITY ? 0.f : top * scale) {}
     __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -base)); }
+    __device__ __forceinline__ float log(float x) const { return __builtin_fmaf(x, scale, -base) * 0.693147180559945309f; }
+    // what a sum of these is multiplied by to be one of `other`'s
+    __device__ __forceinline__ float as(const ScaledExp& other) const { return __builtin_amdgcn_exp2f(base - other.base); }
 };
 template <> struct ScaledExp<double> {
     double scale, base;
-    __device__ __forceinline__ ScaledExp(double s, double b) : scale(s), base(b) {}
+    __device__ __forceinline__ ScaledExp(double s, double top) : scale(s), base(top == -(double)INFINITY ? 0.0 : top * s) {}
     __device__ __forceinline__ double operator()(double x) const { return exp(__builtin_fma(x, scale, -base)); }
+    __device__ __forceinline__ double log(double x) const { return __builtin_fma(x, scale, -base); }
+    __device__ __forceinline__ double as(const ScaledExp& other) const { return exp(base - other.base); }
 };
 __device__ __forceinline__ float plain_max(float a, float b) { return fmaxf(a, b); }       // (of a number and NaN the number)
 __device__ __forceinline__ double plain_max(double a, double b) { return fmax(a, b); }
-
-// x * scale - base with one rounding, so that what a value comes to does not depend on what a compiler joins in one kernel or another
-__device__ __forceinline__ float scaled_less(float x, float scale, float base) { return __builtin_fmaf(x, scale, -base); }
-__device__ __forceinline__ double scaled_less(double x, double scale, double base) { return __builtin_fma(x, scale, -base); }
 
 }  // namespace rp
