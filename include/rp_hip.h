@@ -498,7 +498,9 @@ long long rp_hip_linear_cross_entropy_workspace_strided(int rows, int k, int cla
 int rp_hip_linear_cross_entropy_forward(void* loss_out, void* stats, const void* x, const void* w, const void* bias, const int* targets, void* workspace, int rows, int k, int classes, int reduction,
                                         long long x_rs, long long x_cs, long long w_rs, long long w_cs, int dtype);
 /* Its gradients times upstream_dev, accumulate type on the device ([rows] for reduction 0, one element otherwise; NULL: 1): dx [rows, k] with unit column stride, dw [k, classes] with unit stride along
- * either axis, db dense [classes]; any may be NULL.  The logits are made again, piece by piece, and each piece's gradient (rounded to the tensors' type, whatever its magnitude) multiplied at once. */
+ * either axis, db dense [classes]; any may be NULL.  The logits are made again, piece by piece, and each piece's gradient (16-bit operands with unit strides: rounded to their type, whatever its
+ * magnitude) multiplied at once.  accumulate_* = 1 adds to what is there, before the one rounding; to dx and dw of 16-bit operands with unit strides the rounded product is added.
+ * Logits and their log sums are values of the accumulate type: where they are large, a probability is off by half a step of the largest |logit| in it and the log sum's (around 1000 in float32 3e-5 each). */
 int rp_hip_linear_cross_entropy_backward(void* dx, void* dw, void* db, const void* x, const void* w, const void* bias, const int* targets, const void* stats, const void* upstream_dev, void* workspace,
                                          int rows, int k, int classes, int reduction, long long x_rs, long long x_cs, long long w_rs, long long w_cs,
                                          long long dx_rs, long long dw_rs, long long dw_cs, int accumulate_dx, int accumulate_dw, int accumulate_db, int dtype);

@@ -5,8 +5,10 @@
 // with f the row's share of the result (1, or 1 / rows for the mean) times the upstream gradient.  A row without an entry is left out: its loss and gradient are zeros.
 //
 // What bounds it is memory: the student's logits once and, backward, their gradient once.  A workgroup holds a row in registers where it fits (131072 classes of 16 bits,
-// 65536 of float32), so that the largest logit, the sum and the gradient cost one read together; longer rows are read once for each of the three.
-// The K entries are handled beside, one a thread: their classes' gradients are written a second time, after the row's, by the first entry of each class (a class may be named twice).
+// 65536 of float32), so that the largest logit, the sum and the gradient cost one read together; longer rows are read once for the two sums and again for the gradient (from 2^27 classes on, whose byte offsets pass
+// 32 bits, once for each of the three).
+// The largest logit and the sum are kept apart, and every difference is one of two logits: a row far from zero would lose its digits to the rounding of a log sum (float32 around 4096: 1e-4 of every
+// probability).  The K entries are handled beside, one a thread: their classes' gradients are written a second time, after the row's, by the first entry of each class (a class may be named twice).
 #include "rp_gemm.h"
 #include "rp_teams.h"
 

@@ -27,7 +27,9 @@ template <typename A> struct NormArgs {
 __device__ __forceinline__ float one_over_root(float v) { return 1.f / sqrtf(v); }
 __device__ __forceinline__ double one_over_root(double v) { return 1.0 / sqrt(v); }
 
-// Where the registers reach, the next row's loads fly while a row is added up, and weight and bias are loaded once
+// Rows of up to four vectors a thread, two of 1024 threads: the next row's loads fly while a row is added up, and weight and bias are loaded once.  Up to a width of 8192 (16 bits) that fits the registers.
+// Wider, the sums of dw and db beside it do not: 122 registers of a thread lie in scratch memory from 8193 on in bf16, 326 from 16385 and 846 from 32769 (8192 rows, us and TB/s backward with dw and db, and for
+// dx alone: width 8192 117, 3.4 and 78, 5.2; 12288 779, 0.8 and 113, 5.4; 16384 816, 1.0 and 145, 5.6; float32, 4096 rows, 12288 309, 2.0 and 114, 5.3)
 constexpr bool norm_ahead(int lanes, int steps, int elem) { return elem < 8 && steps * (lanes == 1024 ? 4 : 2) <= 8; }
 
 template <typename T, int LANES, int STEPS>

@@ -1241,7 +1241,7 @@ void backward_layer_norm_fn(GradFn* self, Tensor* grad_output) {
     free_tensor(gd); free_tensor(xd);
 }
 
-// A gradient that lies as a weight of unit stride along its rows does is made in place where one is there already; a new one is dense
+// Gradients are made row-major, in place where a contiguous one is there already; that of a transposed weight goes back through its view afterwards
 void backward_gated_linear_fn(GradFn* self, Tensor* grad_output) {
     LanguageSaved* s = (LanguageSaved*)self->saved_data;
     Tensor* x = self->inputs[0]; Tensor* w = self->inputs[1];
